@@ -262,8 +262,7 @@ def _plain_step(c, s):
         h = h * torch.exp(dt[:, j] * s["a"])[..., None, None] + (dt[:, j, :, None] * x)[..., None] * B[:, :, None, :]
         out.append((h * C[:, :, None, :]).sum(3) + x * s["d"][:, None])
     s["h1"][slots] = h
-    fresh = pos[:, None] + torch.arange(max(0, each - TAPS + 1), each, device=pos.device)
-    s["ring"][slots[:, None], fresh % s["cap"]] = raw[:, max(0, each - TAPS + 1):]
+    s["ring"][slots[:, None], (pos[:, None] + torch.arange(each, device=pos.device)) % s["cap"]] = raw
     return {"y": torch.stack(out, 1).reshape(S * each, inner).to(DTYPE[c["io"]]), "state": s["h1"], "ring": s["ring"]}
 
 
@@ -471,7 +470,6 @@ def _exact_scan(c, s):
         g.mul_(keep[:, t].view(S, G, per, 1, 1)).add_(x * step[:, t].view(S, G, per, 1, 1) * b)
         y[:, t] = (torch.matmul(g, cc)[..., 0] + s["d"].double().view(G, per, 1) * x[..., 0]).reshape(S, inner)
     out[slots] = h
-    fresh = range(max(0, each - TAPS + 1), each)
-    for t in fresh:
+    for t in range(max(0, each - TAPS + 1) if prompt else 0, each):
         ring[slots, (pos + t) % cap] = raw[:, t]
     return {"y": y.view(S * each, inner), "state": out[0] if prompt else out, "ring": ring[0] if prompt else ring}
