@@ -1,4 +1,4 @@
-"""The attention ABI (include/ns_attn.h) bound by name, and the size-checked wrappers an engine calls.
+"""The library's ABI (include/ns_attn.h, ns_mla.h, ns_pre.h, ns_layer.h) bound by name, and the size-checked wrappers an engine calls.
 
 `Kernels` is the table of function pointers - the counterpart of an engine's `ffi.rs` (llm/qwen35/src/ffi.rs:42-52,
 70-136; llm/museglimmer/src/ffi.rs; llm/deepseek2/src/ffi.rs:36-39): every entry point looked up by name when the table
@@ -137,12 +137,25 @@ PRE_H = {
 }
 
 
+# include/ns_layer.h
+LAYER_H = {
+    "ns_ssm_prompt_scratch": (i64, [i64, i64, i64, i64, i64, i64]),
+    "ns_ssm_prompt": (i32, [P, i32, P, i64, P, i64, P, P, P, P, P, f32, f32, P, i64, i64, i64, i64, i64, i64, i64, i64, P, P, P, i64, P]),
+    "ns_ssm_step": (i32, [P, i32, P, i64, P, i64, P, P, P, P, P, f32, f32, P, i64, i64, P, P, i64, i64, i64, i64, i64, i64, i64, P, P, P, i64]),
+    "ns_norm_gated": (i32, [P, i32, P, i64, P, i64, P, P, i64, i64, i64, i64, f32, i32]),
+    "ns_norm_residual": (i32, [P, i32, i32, P, i64, P, i64, P, i64, P, i64, i64, i64, f32, f32, P, P, P]),
+    "ns_q4_bytes": (i64, [i64, i64, i64]),
+    "ns_q4_pack": (i32, [P, i32, P, i64, i64, i64, i64, P]),
+    "ns_q4_product": (i32, [P, i32, P, i64, P, i64, P, i64, i64, i64, i64]),
+}
+
+
 class Kernels:
     """Every attention entry point bound by name; a missing symbol fails the load."""
 
     def __init__(self, a=None):
         self.api = a or api()
-        for name, (res, args) in list(ATTN_H.items()) + list(MLA_H.items()) + list(PRE_H.items()):
+        for name, (res, args) in list(ATTN_H.items()) + list(MLA_H.items()) + list(PRE_H.items()) + list(LAYER_H.items()):
             setattr(self, name[3:], self.api.symbol(name, res, args))
 
 
@@ -161,6 +174,12 @@ def _need(buf, nbytes, what):
         raise Error("%s: no buffer" % what)
     if buf.len < nbytes:
         raise Error("%s: %d bytes, needs %d" % (what, buf.len, nbytes))
+
+
+def _elt(qt, what):
+    if qt not in ELT:
+        raise Error("%s: rows of type 0 (float32), 1 (half) or 2 (bfloat16)" % what)
+    return ELT[qt]
 
 
 try:
@@ -599,6 +618,99 @@ class Ops:
         _need(bs, T * G * nblk * 4, "idx_topk scores")
         _need(sel, T * G * K * 4, "idx_topk lists")
         self.ok(self.k.llm_minimaxm3_idx_topk(self.raw(), bs.ptr, sel.ptr, T, G, nblk, K), "idx_topk")
+
+    # ---- a hybrid model's layers beside attention (include/ns_layer.h)
+    def ssm_prompt_scratch(self, T, H, P, N, G, K):
+        """Floats of scratch ssm_prompt needs."""
+        return self.k.ssm_prompt_scratch(T, H, P, N, G, K)
+
+    def _ssm_need(self, what, qt, xbc, xs, dt, dts, cw, cb, a, dtb, d, rows, H, P, N, G, K, y, ys):
+        e, chan = _elt(qt, what), H * P + 2 * G * N
+        if rows > 0:
+            _need(xbc, ((rows - 1) * xs + chan) * e, what + " x B C")
+            _need(dt, ((rows - 1) * dts + H) * e, what + " step sizes")
+            _need(y, ((rows - 1) * ys + H * P) * e, what + " y")
+        _need(cw, chan * K * 4, what + " taps")
+        _need(a, H * 4, what + " rates")
+        for b, n, name in ((cb, chan, " tap bias"), (dtb, H, " step bias"), (d, H, " skip")):
+            if b is not None:
+                _need(b, n * 4, what + name)
+        return chan
+
+    def ssm_prompt(self, qt, xbc, xs, dt, dts, cw, cb, a, dtb, d, conv, cap, p0, T, H, P, N, G, K, h0, h1, y, ys, scratch, dt_lo=0.0, dt_hi=float("inf")):
+        """ns_ssm_prompt: T projected rows of one sequence at positions p0.. through the convolution and the scan; h0 None: a
+        state of zeros; the state behind the last row in h1, the last K - 1 raw rows in the ring conv [cap][chan]."""
+        chan = self._ssm_need("ssm_prompt", qt, xbc, xs, dt, dts, cw, cb, a, dtb, d, T, H, P, N, G, K, y, ys)
+        if K > 1:
+            _need(conv, cap * chan * 4, "ssm_prompt ring")
+        if h0 is not None:
+            _need(h0, H * P * N * 4, "ssm_prompt state")
+        _need(h1, H * P * N * 4, "ssm_prompt state")
+        _need(scratch, self.ssm_prompt_scratch(T, H, P, N, G, K) * 4, "ssm_prompt scratch")
+        opt = lambda b: b.ptr if b is not None else None
+        self.ok(self.k.ssm_prompt(self.raw(), qt, xbc.ptr, xs, dt.ptr, dts, cw.ptr, opt(cb), a.ptr, opt(dtb), opt(d), dt_lo, dt_hi, opt(conv), cap, p0, T, H, P, N,
+                                  G, K, opt(h0), h1.ptr, y.ptr, ys, scratch.ptr), "ssm_prompt")
+
+    def ssm_step(self, qt, xbc, xs, dt, dts, cw, cb, a, dtb, d, conv, cap, p0, R, H, P, N, G, K, h0, h1, y, ys, nslots=1, slots=None, pos=None, dt_lo=0.0,
+                 dt_hi=float("inf")):
+        """ns_ssm_step: a token, or a few successive ones, of each of several sequences: R rows, row r of slot slots[r] (None: r)
+        at position pos[r] (None: p0); rings [nslots][cap][chan], states [nslots][H][P][N]."""
+        chan = self._ssm_need("ssm_step", qt, xbc, xs, dt, dts, cw, cb, a, dtb, d, R, H, P, N, G, K, y, ys)
+        if K > 1:
+            _need(conv, nslots * cap * chan * 4, "ssm_step rings")
+        if h0 is not None:
+            _need(h0, nslots * H * P * N * 4, "ssm_step states")
+        _need(h1, nslots * H * P * N * 4, "ssm_step states")
+        for b, name in ((slots, "slots"), (pos, "positions")):
+            if b is not None:
+                _need(b, R * 4, "ssm_step " + name)
+        opt = lambda b: b.ptr if b is not None else None
+        self.ok(self.k.ssm_step(self.raw(), qt, xbc.ptr, xs, dt.ptr, dts, cw.ptr, opt(cb), a.ptr, opt(dtb), opt(d), dt_lo, dt_hi, opt(conv), cap, p0, opt(pos),
+                                opt(slots), nslots, R, H, P, N, G, K, opt(h0), h1.ptr, y.ptr, ys), "ssm_step")
+
+    def norm_gated(self, qt, y, ys, z, zs, w, out, os, T, D, groups, eps, order=0):
+        """ns_norm_gated: out = rms(y silu(z)) w over each of `groups` parts of a row (order 1: rms(y) w silu(z))."""
+        if T > 0:
+            e = _elt(qt, "norm_gated")
+            _need(y, ((T - 1) * ys + D) * e, "norm_gated y")
+            _need(z, ((T - 1) * zs + D) * e, "norm_gated z")
+            _need(out, ((T - 1) * os + D) * e, "norm_gated out")
+        if w is not None:
+            _need(w, D * 4, "norm_gated weight")
+        self.ok(self.k.norm_gated(self.raw(), qt, y.ptr, ys, z.ptr, zs, w.ptr if w is not None else None, out.ptr, os, T, D, groups, eps, order), "norm_gated")
+
+    def norm_residual(self, qt, rt, x, xs, h, hs, h1, h1s, out, os, T, D, eps, scale=1.0, post=None, gate=None, pre=None):
+        """ns_norm_residual: h1 = s = h + scale gate (x, or rms(x) post), out = rms(s) pre; x None: s = h; h1 or out None: not wanted."""
+        if T > 0:
+            for b, stride, t, name in ((x, xs, qt, "x"), (h, hs, rt, "stream"), (h1, h1s, rt, "stream out"), (out, os, qt, "out")):
+                if b is not None:
+                    _need(b, ((T - 1) * stride + D) * _elt(t, "norm_residual"), "norm_residual " + name)
+        for b, name in ((post, "norm behind"), (gate, "gate"), (pre, "norm in front")):
+            if b is not None:
+                _need(b, D * 4, "norm_residual " + name)
+        opt = lambda b: b.ptr if b is not None else None
+        self.ok(self.k.norm_residual(self.raw(), qt, rt, opt(x), xs, opt(h), hs, opt(h1), h1s, opt(out), os, T, D, eps, scale, opt(post), opt(gate), opt(pre)),
+                "norm_residual")
+
+    def q4_bytes(self, M, K, group):
+        """Bytes of an M x K matrix of 4-bit weights in the library's tiles."""
+        return self.k.q4_bytes(M, K, group)
+
+    def q4_pack(self, form, src, ss, M, K, group, w):
+        """ns_q4_pack: M rows of K weights - form 0 float32 rows ss values apart, 1 q4_0 blocks of 18 bytes, rows ss bytes apart - into tiles."""
+        if M > 0 and K > 0:
+            _need(src, (M - 1) * ss + K // 32 * 18 if form else ((M - 1) * ss + K) * 4, "q4_pack source")
+            _need(w, self.q4_bytes(M, K, group), "q4_pack weights")
+        self.ok(self.k.q4_pack(self.raw(), form, src.ptr, ss, M, K, group, w.ptr), "q4_pack")
+
+    def q4_product(self, qt, x, xs, w, group, y, ys, T, M, K):
+        """ns_q4_product: y [T][M] = x [T][K] . w^T, 1 to 16 rows, w M x K 4-bit weights in the library's tiles."""
+        if T > 0 and M > 0:
+            e = _elt(qt, "q4_product")
+            _need(x, ((T - 1) * xs + K) * e, "q4_product x")
+            _need(w, self.q4_bytes(M, K, group), "q4_product weights")
+            _need(y, ((T - 1) * ys + M) * e, "q4_product y")
+        self.ok(self.k.q4_product(self.raw(), qt, x.ptr, xs, w.ptr, group, y.ptr, ys, T, M, K), "q4_product")
 
     # ---- the step in front of attention: norm, rotary positions, store
     def q35_qk_norm_rope(self, src, ss, hs, dst, ds, T, H, D, w, eps, n_rot, theta, p0, pos3=None, sections=(0, 0, 0)):

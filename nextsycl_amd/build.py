@@ -34,6 +34,10 @@ SOURCES = {
     "attn_api.cpp": [],
     "mla.hip": [],
     "gemm_h.hip": [],
+    "ssm_step.hip": [],
+    "ssm_prompt.hip": [],
+    "norm_rows.hip": [],
+    "q4.hip": [],
 }
 
 

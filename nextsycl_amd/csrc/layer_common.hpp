@@ -1,0 +1,111 @@
+// layer_common.hpp: rows of the library's three types read and written in wide pieces, and what the state-space kernels
+// share.
+#pragma once
+#include <cstdint>
+#include <hip/hip_runtime.h>
+
+#include "attn_common.hpp"
+#include "kv_formats.hpp"
+#include "ns_internal.hpp"
+
+// VEC elements of type QT from element i on, as float32 (VEC 1, 2, 4 or 8; more than one: aligned to the piece, up to 16 bytes)
+template <int QT, int VEC>
+__device__ __forceinline__ void load_row(const void* p, int64_t i, float (&v)[VEC]) {
+    if constexpr (VEC == 1) v[0] = load_q<QT>(p, i);
+    else if constexpr (QT == 0) {
+        if constexpr (VEC == 2) {
+            const float2 a = *reinterpret_cast<const float2*>(static_cast<const float*>(p) + i);
+            v[0] = a.x, v[1] = a.y;
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; j += 4) {
+                const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + j);
+                v[j] = a.x, v[j + 1] = a.y, v[j + 2] = a.z, v[j + 3] = a.w;
+            }
+        }
+    } else {
+        uint32_t w[VEC / 2];
+        const uint16_t* s = static_cast<const uint16_t*>(p) + i;
+        if constexpr (VEC == 8) {
+            const uint4 a = *reinterpret_cast<const uint4*>(s);
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        } else if constexpr (VEC == 4) {
+            const uint2 a = *reinterpret_cast<const uint2*>(s);
+            w[0] = a.x, w[1] = a.y;
+        } else w[0] = *reinterpret_cast<const uint32_t*>(s);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const uint16_t b = (uint16_t) (j % 2 ? w[j / 2] >> 16 : w[j / 2]);
+            v[j] = QT == 1 ? f16_to_f32(b) : bf16_to_f32(b);
+        }
+    }
+}
+template <int QT, int VEC>
+__device__ __forceinline__ void store_row(void* p, int64_t i, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) store_o<QT>(p, i, v[0]);
+    else if constexpr (QT == 0) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4*>(static_cast<float*>(p) + i + j) = float4{v[j], v[j + 1], v[j + 2], v[j + 3]};
+    } else {
+        uint32_t w[VEC / 2];
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+            const uint32_t a = QT == 1 ? f32_to_f16(v[2 * j]) : f32_to_bf16(v[2 * j]), b = QT == 1 ? f32_to_f16(v[2 * j + 1]) : f32_to_bf16(v[2 * j + 1]);
+            w[j] = a | b << 16;
+        }
+        uint16_t* d = static_cast<uint16_t*>(p) + i;
+        if constexpr (VEC == 8) *reinterpret_cast<uint4*>(d) = uint4{w[0], w[1], w[2], w[3]};
+        else *reinterpret_cast<uint2*>(d) = uint2{w[0], w[1]};
+    }
+}
+
+// v / (1 + e^-v); where e^-v is infinite the quotient is 0
+__device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
+__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))) + (v != v ? v : 0.0f); }
+
+// the sum over each run of L lanes (L a power of two up to 64), in every lane of the run
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+    auto add = [&](auto c) { v += __builtin_bit_cast(float, dpp_u32<decltype(c)::value>(__builtin_bit_cast(uint32_t, v))); };
+    if constexpr (L >= 2) add(std::integral_constant<int, 0xB1>());
+    if constexpr (L >= 4) add(std::integral_constant<int, 0x4E>());
+    if constexpr (L >= 8) add(std::integral_constant<int, 0x141>());
+    if constexpr (L >= 16) add(std::integral_constant<int, 0x140>());
+    float a, b;
+    if constexpr (L >= 32) {
+        pair16(v, a, b);
+        v = a + b;
+    }
+    if constexpr (L >= 64) {
+        pair32(v, a, b);
+        v = a + b;
+    }
+    return v;
+}
+
+// a state-space layer's sizes, weights and places, as ns_ssm_prompt and ns_ssm_step take them
+struct SsmLayer {
+    const void *xbc, *dt;
+    int64_t xs, dts;
+    const float *cw, *cb, *a, *dtb, *d;
+    float lo, hi;
+    float* conv;
+    int64_t cap, p0;
+    int H, P, N, G, K, chan;
+    const float* h0;
+    float* h1;
+    void* y;
+    int64_t ys;
+};
+
+// the step size of a row's head
+template <int QT>
+__device__ __forceinline__ float ssm_dt(const SsmLayer& p, int64_t row, int head) {
+    const float s = softplus(load_q<QT>(p.dt, row * p.dts + head) + (p.dtb ? p.dtb[head] : 0.0f));
+    return s < p.lo ? p.lo : s > p.hi ? p.hi : s;
+}
+// tap k of 4 of a channel: the layer's K taps are the last K of them
+__device__ __forceinline__ float ssm_tap(const SsmLayer& p, int ch, int k) { return k >= 4 - p.K ? p.cw[(int64_t) ch * p.K + k - 4 + p.K] : 0.0f; }
+
+// ssm_step.hip: what the two state-space calls refuse alike (a ring of fewer than `least` rows among it); 0 or -1
+int ns_ssm_check(const char* who, ns_gpu* g, int qt, const SsmLayer& p, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K, int64_t least);

@@ -1,0 +1,215 @@
+// ssm_step.hip: a token, or a few successive ones, of each of several sequences through a state-space layer's convolution
+// and recurrence (ns_ssm_step).
+//
+// A row's head: h = exp(dt a) h + dt x (outer) B, y = h C + d x over a state of P x N floats that nothing else of the call
+// touches. Bound: HBM - the state is read and written once (8 H P N bytes a sequence, 8.4 MB at 128 heads of 64 x 128) for
+// 5 operations a float. So a lane holds 4 consecutive features of a few of the head's P rows, asks for them before anything
+// else, and the convolution (a few hundred channels, each group's B and C by every head of the group: 4 multiply-adds and
+// a few KB that the cache holds) runs while they are on their way; y is a sum over a row's lanes, by DPP. Rows of one slot
+// are walked with the state in registers.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "ns_internal.hpp"
+#include "ns_layer.h"
+#include "layer_common.hpp"
+
+namespace {
+
+constexpr int64_t MOST_ROWS = 4096;
+
+struct StepParams {
+    SsmLayer l;
+    const int32_t *pos, *slots;
+    int64_t nslots;
+    int R, pblocks;
+};
+
+// LR lanes a state row, U rows a lane; VEC: a lane's 4 floats as one piece
+template <int QT, int LR, int U, bool VEC>
+__global__ __launch_bounds__(256) void ssm_step_kernel(StepParams s) {
+    constexpr int RW = 256 / LR, PB = RW * U, NMAX = 4 * LR, CH = (2 * NMAX + PB + 255) / 256;
+    __shared__ float ub[NMAX], uc[NMAX], ux[PB];
+    __shared__ uint64_t mine[MOST_ROWS / 64];
+    const SsmLayer& p = s.l;
+    const int tid = threadIdx.x, lane = tid % 64, head = blockIdx.x / s.pblocks, pb = blockIdx.x % s.pblocks, r0 = blockIdx.y;
+    const int group = head / (p.H / p.G), n0 = tid % LR * 4, prow = pb * PB + tid / LR;
+    const int64_t slot = s.slots ? s.slots[r0] : r0;
+    const int64_t first = s.pos ? (int64_t) s.pos[r0] : p.p0;
+    if (slot < 0 || slot >= s.nslots || first < 0) return;
+    // the state, asked for first
+    float h[U][4];
+    const int64_t hrow = (slot * p.H + head) * p.P;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int pr = prow + u * RW;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[u][i] = 0.0f;
+        if (!p.h0 || pr >= p.P) continue;
+        const float* src = p.h0 + (hrow + pr) * p.N + n0;
+        if constexpr (VEC) {
+            if (n0 < p.N) {
+                const float4 v = *reinterpret_cast<const float4*>(src);
+                h[u][0] = v.x, h[u][1] = v.y, h[u][2] = v.z, h[u][3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n0 + i < p.N) h[u][i] = src[i];
+        }
+    }
+    // the slot's rows: this work-group is the first's, or has nothing to do
+    if (s.slots) {
+        for (int w = tid / 64; w * 64 < s.R; w += 4) {
+            const int at = w * 64 + lane;
+            const uint64_t m = __ballot(at < s.R && s.slots[at < s.R ? at : 0] == (int32_t) slot);
+            if (lane == 0) mine[w] = m;
+        }
+        __syncthreads();
+        for (int w = 0; w <= r0 / 64; ++w) {
+            const uint64_t m = w == r0 / 64 ? mine[w] & (((uint64_t) 1 << r0 % 64) - 1) : mine[w];
+            if (m) return;
+        }
+    }
+    // this thread's channels: B, C, then the block's part of x; their taps and the raw values in front of the first row
+    int ch[CH];
+    float w4[CH][4], bias[CH], past[CH][3];
+    float* to[CH];
+    bool keep[CH];
+    const int64_t ringb = slot * p.cap;
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+        const int c = tid + 256 * j;
+        ch[j] = -1, to[j] = nullptr, keep[j] = false;
+        if (c < NMAX) {
+            if (c < p.N) ch[j] = p.H * p.P + group * p.N + c;
+            to[j] = ub + c, keep[j] = true;
+        } else if (c < 2 * NMAX) {
+            if (c - NMAX < p.N) ch[j] = p.H * p.P + (p.G + group) * p.N + c - NMAX;
+            to[j] = uc + (c - NMAX), keep[j] = true;
+        } else if (c < 2 * NMAX + PB) {
+            const int pr = pb * PB + c - 2 * NMAX;
+            if (pr < p.P) ch[j] = head * p.P + pr;
+            to[j] = ux + (c - 2 * NMAX);
+        }
+        // a group's B and C are kept by its first head's first block, x by its own
+        keep[j] = ch[j] >= 0 && p.K > 1 && (!keep[j] || (head % (p.H / p.G) == 0 && pb == 0));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w4[j][k] = ch[j] >= 0 ? ssm_tap(p, ch[j], k) : 0.0f;
+        bias[j] = ch[j] >= 0 && p.cb ? p.cb[ch[j]] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const int64_t at = first - 3 + k;
+            past[j][k] = ch[j] >= 0 && k >= 4 - p.K && at >= 0 ? p.conv[(ringb + at % p.cap) * p.chan + ch[j]] : 0.0f;
+        }
+    }
+    const float rate = p.a[head], skip = p.d ? p.d[head] : 0.0f;
+    int64_t most = p.K > 1 ? p.cap - p.K + 1 : s.R;
+    int row = r0;
+    for (int64_t i = 0;;) {
+        if (i) __syncthreads();          // the row before has been read
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            if (!to[j]) continue;
+            float c = 0.0f;
+            if (ch[j] >= 0) {
+                const float v = load_q<QT>(p.xbc, row * p.xs + ch[j]);
+                c = silu(fmaf(w4[j][3], v, fmaf(w4[j][2], past[j][2], fmaf(w4[j][1], past[j][1], fmaf(w4[j][0], past[j][0], bias[j])))));
+                past[j][0] = past[j][1], past[j][1] = past[j][2], past[j][2] = v;
+                if (keep[j]) p.conv[(ringb + (first + i) % p.cap) * p.chan + ch[j]] = v;
+            }
+            *to[j] = c;
+        }
+        const float dt = ssm_dt<QT>(p, row, head), decay = expf(dt * rate);
+        __syncthreads();
+        const float4 b = *reinterpret_cast<const float4*>(ub + n0), c = *reinterpret_cast<const float4*>(uc + n0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float x = ux[tid / LR + u * RW], dx = dt * x;
+            h[u][0] = fmaf(h[u][0], decay, dx * b.x), h[u][1] = fmaf(h[u][1], decay, dx * b.y);
+            h[u][2] = fmaf(h[u][2], decay, dx * b.z), h[u][3] = fmaf(h[u][3], decay, dx * b.w);
+            const float sum = lanes_sum<LR>(fmaf(h[u][0], c.x, h[u][1] * c.y) + fmaf(h[u][2], c.z, h[u][3] * c.w));
+            const int pr = prow + u * RW;
+            if (tid % LR == 0 && pr < p.P) store_o<QT>(p.y, row * p.ys + head * p.P + pr, fmaf(skip, x, sum));
+        }
+        // the slot's next row
+        if (!s.slots || ++i >= most) break;
+        int w = (row + 1) / 64, words = (s.R + 63) / 64;
+        uint64_t m = w < words ? mine[w] & ~(((uint64_t) 1 << (row + 1) % 64) - 1) : 0;
+        while (!m && ++w < words) m = mine[w];
+        if (!m) break;
+        row = w * 64 + __builtin_ctzll(m);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int pr = prow + u * RW;
+        if (pr >= p.P) continue;
+        float* dst = p.h1 + (hrow + pr) * p.N + n0;
+        if constexpr (VEC) {
+            if (n0 < p.N) *reinterpret_cast<float4*>(dst) = float4{h[u][0], h[u][1], h[u][2], h[u][3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n0 + i < p.N) dst[i] = h[u][i];
+        }
+    }
+}
+
+template <int QT, int LR, int U>
+void launch_step(ns_gpu* g, StepParams& s, bool vec) {
+    s.pblocks = (s.l.P + 256 / LR * U - 1) / (256 / LR * U);
+    const dim3 grid((unsigned) (s.l.H * s.pblocks), (unsigned) s.R);
+    if (vec) ssm_step_kernel<QT, LR, U, true><<<grid, 256, 0, g->q>>>(s);
+    else ssm_step_kernel<QT, LR, U, false><<<grid, 256, 0, g->q>>>(s);
+}
+template <int QT>
+void launch_step(ns_gpu* g, StepParams& s, bool vec) {
+    const int N = s.l.N;
+    if (N <= 16) launch_step<QT, 4, 1>(g, s, vec);
+    else if (N <= 32) launch_step<QT, 8, 2>(g, s, vec);
+    else if (N <= 64) launch_step<QT, 16, 4>(g, s, vec);
+    else if (N <= 128) launch_step<QT, 32, 4>(g, s, vec);
+    else launch_step<QT, 64, 4>(g, s, vec);
+}
+
+}  // namespace
+
+// what the two state-space calls refuse alike
+int ns_ssm_check(const char* who, ns_gpu* g, int qt, const SsmLayer& p, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K,
+                 int64_t least) {
+    const std::string s(who);
+    if (qt < 0 || qt > 2) return ns_fail(s + ": rows of type 0 (float32), 1 (half) or 2 (bfloat16)");
+    if (H <= 0 || P <= 0 || N <= 0 || G <= 0 || H % G || N > 256 || H > 65536 || P > 65536 || H * P + 2 * G * N > (int64_t) 1 << 24)
+        return ns_fail(s + ": heads a multiple of the groups, a state of 1 to 256 features, up to 2^24 channels");
+    if (K < 1 || K > 4) return ns_fail(s + ": 1 to 4 taps");
+    if (p.xs < H * P + 2 * G * N || p.dts < H || p.ys < H * P) return ns_fail(s + ": rows at least as far apart as they are long");
+    if (!(p.lo <= p.hi)) return ns_fail(s + ": step sizes between dt_lo and dt_hi");
+    if (p.p0 < 0) return ns_fail(s + ": a position in front of the first");
+    if (K > 1 && p.cap < least) return ns_fail(s + ": a ring of at least " + std::to_string(least) + " rows");
+    if (!g || !p.xbc || !p.dt || !p.cw || !p.a || !p.h1 || !p.y || (K > 1 && !p.conv)) return ns_fail(s + ": a null buffer");
+    return 0;
+}
+
+extern "C" int ns_ssm_step(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt, int64_t dts, const float* cw, const float* cb,
+                           const float* a, const float* dtb, const float* d, float dt_lo, float dt_hi, float* conv, int64_t cap, int64_t p0,
+                           const int32_t* pos, const int32_t* slots, int64_t nslots, int64_t R, int64_t H, int64_t P, int64_t N, int64_t G,
+                           int64_t K, const float* h0, float* h1, void* y, int64_t ys) {
+    NS_TRY
+    if (R <= 0) return 0;
+    StepParams s{};
+    s.l = SsmLayer{xbc, dt, xs, dts, cw, cb, a, dtb, d, dt_lo, dt_hi, conv, cap, p0, (int) H, (int) P, (int) N, (int) G, (int) K, 0, h0, h1, y, ys};
+    if (R > MOST_ROWS) return ns_fail("ns_ssm_step: up to 4096 rows");
+    if (nslots <= 0 || (!slots && R > nslots) || nslots > INT32_MAX) return ns_fail("ns_ssm_step: more rows than slots");
+    if (ns_ssm_check("ns_ssm_step", g, qt, s.l, H, P, N, G, K, K)) return -1;
+    s.l.chan = (int) (H * P + 2 * G * N);
+    s.pos = pos, s.slots = slots, s.nslots = nslots, s.R = (int) R;
+    NS_HIP(hipSetDevice(g->dev));
+    const bool vec = N % 4 == 0 && (uintptr_t) h0 % 16 == 0 && (uintptr_t) h1 % 16 == 0;
+    if (qt == 0) launch_step<0>(g, s, vec);
+    else if (qt == 1) launch_step<1>(g, s, vec);
+    else launch_step<2>(g, s, vec);
+    NS_LAUNCHED("ssm_step");
+    return 0;
+    NS_CATCH
+}
