@@ -59,8 +59,8 @@ __device__ __forceinline__ void store_row(void* p, int64_t i, const float (&v)[V
     }
 }
 
-// v / (1 + e^-v); where e^-v is infinite the quotient is 0
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
+// v / (1 + e^-v) by the hardware's exponential and reciprocal (one unit in the last place each); where e^-v is infinite, 0
+__device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + fast_exp2(v * -1.44269504f)); }
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))) + (v != v ? v : 0.0f); }
 
 // the sum over each run of L lanes (L a power of two up to 64), in every lane of the run

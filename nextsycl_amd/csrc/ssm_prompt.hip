@@ -1,4 +1,24 @@
 // ssm_prompt.hip: a prompt's rows through a state-space layer's convolution and scan (ns_ssm_prompt).
+//
+// The recurrence h_t = exp(dt_t a) h_{t-1} + dt_t x_t (outer) B_t, y_t = h_t C_t + d x_t, in chunks of 64 rows: with cum_l the sum of
+// dt a over a chunk's rows up to l, and h the state in front of the chunk,
+//   y_l = exp(cum_l) C_l h + sum over s <= l of [(C_l . B_s) exp(cum_l - cum_s) dt_s + (s = l) d] x_s
+//   h'  = exp(cum_63) h + sum over s of exp(cum_63 - cum_s) dt_s x_s (outer) B_s
+// three matrix products a chunk and head, and one (C . B) a chunk and group. They run on the matrix unit: an operand is two
+// halfs (22 bits), scaled by a power of two that puts the largest value of its column, row or block at 2^13, and three
+// instructions a product drop nothing above 2^-22; sums, states and scales are float32. (bfloat16 rows: the products that
+// reach y alone take their operands' first halfs, 2^-11 beside the rows' own rounding of 2^-8.)
+//
+// ssm_prep_kernel, a work-group a (chunk, group): convolves B and C, lays them out as operands, multiplies them, and sums
+// the exponents (in 64 bits; what the exponentials see is a difference within 16 rows, plus one between such runs).
+// ssm_scan_kernel, a work-group a (head, 64 of its features, segment of the prompt): walks its chunks with the state in
+// the accumulators of 4 waves, wave w rows 32 w .. 32 w + 31 of it. In a chunk wave w convolves 16 columns of x into the
+// operands that all read (LDS), splits its part of the state into another, then takes 16 rows of y and its part of h'. Matrix
+// results come as (column, 4 consecutive rows) a lane, operands go in as (row or column, 8 values of the summed index) a
+// lane; the summed index may come in any order that both sides share, so in runs of 4 of two neighbouring tiles a result
+// is an operand as it stands: neither the state nor C . B is ever moved between lanes.
+// Where heads alone do not fill the chip the prompt is cut in segments: the same kernel first leaves each segment's state from a
+// start of zero (STATE: a third of the work), and each segment's scan starts from those before it, decayed.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -9,68 +29,571 @@
 
 namespace {
 
-constexpr int64_t PASS_ROWS = 8192;   // rows a pass works on: what bounds the scratch
+constexpr int L = 64;                     // rows a chunk
+constexpr int64_t PASS_ROWS = 8192;       // rows a pass works on: what bounds the scratch
+constexpr int MOST_SEGS = 8;
+// a chunk and head's header: exponents (base 2) from the start of each run of 16 rows, step sizes, weights in the chunk's
+// state, decays from the chunk's start; differences between runs' starts [4][4], the whole chunk's exponent and decay
+constexpr int HDR_C = 0, HDR_DT = 64, HDR_W = 128, HDR_E = 192, HDR_BD = 256, HDR_END = 272, HDR = 288;
 
-// the convolved rows and step sizes of rows t0 .. t0 + T - 1, as float32: u [T][chan], dt [T][H]
-template <int QT>
-__global__ __launch_bounds__(256) void ssm_conv_kernel(SsmLayer p, int64_t t0, int T, float* __restrict__ u, float* __restrict__ dt) {
-    const int c = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
-    if (c < p.chan) {
-        float acc = p.cb ? p.cb[c] : 0.0f;
-        for (int k = 4 - p.K; k < 4; ++k) {
-            const int64_t at = t0 + t - 3 + k;
-            const float v = at >= 0 ? load_q<QT>(p.xbc, at * p.xs + c) : p.p0 + at >= 0 ? p.conv[(p.p0 + at) % p.cap * p.chan + c] : 0.0f;
-            acc = fmaf(ssm_tap(p, c, k), v, acc);
-        }
-        u[(int64_t) t * p.chan + c] = silu(acc);
-    }
-    if (c < p.H) dt[(int64_t) t * p.H + c] = ssm_dt<QT>(p, t0 + t, c);
+// bytes of a chunk and group's operands: C (hi, lo), B (hi, lo) of KK = padded N / 32 steps, C . B as float32
+constexpr int64_t op_c(int kk) { return (int64_t) 4 * kk * 1024; }
+constexpr int64_t op_bytes(int kk) { return 4 * op_c(kk) + 16 * 1024; }
+
+struct ScanParams {
+    SsmLayer l;
+    int64_t t0, all;            // the pass's first row, the call's rows
+    int T, chunks, segs, per;   // rows and chunks of the pass; segments, chunks a segment
+    int blocks, vec_y, vec_h;   // blocks of 64 features a head; y in pieces of 4 values, the state too
+    uint8_t* ops;               // [chunk][group] operands
+    float* scales;              // [chunk][group]: what B's and C's operands are to be multiplied with
+    float* hdr;                 // [chunk][head]
+    float* hist;                // [3][chan]: the raw rows in front of the call's first
+    float* segst;               // [1 + segment][head, block]: the pass's first state, then what each segment leaves - the first
+                                // from that state, the others from zero
+    float* segtot;              // [segment][head]: their exponents
+};
+
+// a power of two that takes `big` to 2^13 .. 2^14, and its inverse
+__device__ __forceinline__ void to_half_range(float big, float& up, float& down) {
+    const int e = min(267 - (int) (__builtin_bit_cast(uint32_t, big) >> 23 & 255), 253);
+    up = __builtin_bit_cast(float, (uint32_t) e << 23);
+    down = __builtin_bit_cast(float, (uint32_t) (254 - e) << 23);
+}
+// 8 floats as two operands: halfs and the halfs of what they leave
+__device__ __forceinline__ void split8(const float (&v)[8], float up, s8v& hi, s8v& lo) {
+    h8v a, b;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = (_Float16) (v[j] * up);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = (_Float16) (fmaf(v[j], up, -(float) a[j]));
+    hi = __builtin_bit_cast(s8v, a);
+    lo = __builtin_bit_cast(s8v, b);
 }
 
-// a wave a state row at a time: one lane a few of its features
+// the raw value of channel ch, `at` rows behind the call's first (negative: in front of it)
 template <int QT>
-__global__ __launch_bounds__(64) void ssm_scan_kernel(SsmLayer p, int64_t t0, int T, const float* __restrict__ u, const float* __restrict__ dt) {
-    const int head = blockIdx.x / p.P, pr = blockIdx.x % p.P, lane = threadIdx.x, group = head / (p.H / p.G);
-    const float* src = t0 ? p.h1 : p.h0;
-    const int64_t hrow = ((int64_t) head * p.P + pr) * p.N;
-    float h[4];
-    for (int i = 0; i < 4; ++i) h[i] = src && lane + 64 * i < p.N ? src[hrow + lane + 64 * i] : 0.0f;
-    const float rate = p.a[head], skip = p.d ? p.d[head] : 0.0f;
-    for (int t = 0; t < T; ++t) {
-        const float* row = u + (int64_t) t * p.chan;
-        const float x = row[head * p.P + pr], s = dt[(int64_t) t * p.H + head], decay = expf(s * rate);
-        const float *b = row + p.H * p.P + group * p.N, *c = b + p.G * p.N;
-        float sum = 0.0f;
-        for (int i = 0; i < 4; ++i) {
-            const int n = lane + 64 * i;
-            if (n >= p.N) continue;
-            h[i] = fmaf(h[i], decay, s * x * b[n]);
-            sum = fmaf(h[i], c[n], sum);
-        }
-        sum = lanes_sum<64>(sum);
-        if (lane == 0) store_o<QT>(p.y, (t0 + t) * p.ys + head * p.P + pr, fmaf(skip, x, sum));
-    }
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < p.N) p.h1[hrow + lane + 64 * i] = h[i];
+__device__ __forceinline__ float raw_row(const SsmLayer& p, const float* hist, int64_t at, int ch) {
+    return at >= 0 ? load_q<QT>(p.xbc, at * p.xs + ch) : hist[(at + 3) * p.chan + ch];
+}
+// the ring's value at that row: zeros in front of the sequence, and of taps that there are not
+__device__ __forceinline__ float ring_row(const SsmLayer& p, int64_t at, int ch) {
+    return at >= 1 - p.K && p.p0 + at >= 0 ? p.conv[(p.p0 + at) % p.cap * p.chan + ch] : 0.0f;
 }
 
-// the last raw rows into the ring
-template <int QT>
-__global__ __launch_bounds__(256) void ssm_ring_kernel(SsmLayer p, int64_t T) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    const int64_t t = T - 1 - blockIdx.y;
-    if (c < p.chan && t >= 0) p.conv[(p.p0 + t) % p.cap * p.chan + c] = load_q<QT>(p.xbc, t * p.xs + c);
+template <int QT, int KW>
+__global__ __launch_bounds__(256, 3 - KW) void ssm_prep_kernel(ScanParams s) {
+    constexpr int NP = 128 * KW, KK = 4 * KW, ROW = NP + 8;
+    __shared__ __align__(16) short plane[2][2][L * ROW];       // [B, C][hi, lo][row][feature]
+    __shared__ float part[2][4];
+    const SsmLayer& p = s.l;
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n16 = lane % 16, g = lane / 16;
+    const int chunk = blockIdx.x / p.G, group = blockIdx.x % p.G, per = p.H / p.G;
+    const int here = min(L, s.T - chunk * L);
+    const int64_t first = s.t0 + (int64_t) chunk * L;
+    uint8_t* ops = s.ops + (int64_t) blockIdx.x * op_bytes(KK);
+    // the rows in front of the call, for the scan's x: the ring is written while that runs
+    if (first == 0) {
+        const int ch0 = group * per * p.P, chn = per * p.P;
+        for (int i = tid; i < 3 * chn; i += 256) s.hist[(int64_t) (i / chn) * p.chan + ch0 + i % chn] = ring_row(p, i / chn - 3, ch0 + i % chn);
+    }
+    float downs[2] = {1.0f, 1.0f};
+#pragma unroll
+    for (int j = 0; j < KW; ++j) {
+        // a thread a channel: its rows from the first on
+        const int isc = KW == 1 ? tid / 128 : j, n = KW == 1 ? tid % 128 : tid, ch = p.H * p.P + (isc * p.G + group) * p.N + n;
+        float v[L], big = 0.0f;
+        if (n < p.N) {
+            float a0, a1, a2;
+            const float w0 = ssm_tap(p, ch, 0), w1 = ssm_tap(p, ch, 1), w2 = ssm_tap(p, ch, 2), w3 = ssm_tap(p, ch, 3), b = p.cb ? p.cb[ch] : 0.0f;
+            if (first >= 3) {
+                a0 = load_q<QT>(p.xbc, (first - 3) * p.xs + ch), a1 = load_q<QT>(p.xbc, (first - 2) * p.xs + ch), a2 = load_q<QT>(p.xbc, (first - 1) * p.xs + ch);
+            } else {
+                a0 = ring_row(p, first - 3, ch), a1 = ring_row(p, first - 2, ch), a2 = ring_row(p, first - 1, ch);      // (first is 0)
+            }
+#pragma unroll
+            for (int t = 0; t < L; ++t) v[t] = load_q<QT>(p.xbc, (first + min(t, here - 1)) * p.xs + ch);
+#pragma unroll
+            for (int t = 0; t < L; ++t) {
+                const float a3 = v[t];
+                const float c = silu(fmaf(w3, a3, fmaf(w2, a2, fmaf(w1, a1, fmaf(w0, a0, b)))));
+                a0 = a1, a1 = a2, a2 = a3;
+                v[t] = t < here ? c : 0.0f;
+                big = fmaxf(big, fabsf(v[t]));
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < L; ++t) v[t] = 0.0f;
+        }
+        big = wave_max(big);
+        if (lane == 0) part[j][wave] = big;
+        __syncthreads();
+        big = KW == 1 ? fmaxf(part[j][2 * isc], part[j][2 * isc + 1]) : fmaxf(fmaxf(part[j][0], part[j][1]), fmaxf(part[j][2], part[j][3]));
+        float up, down;
+        to_half_range(big, up, down);
+        if constexpr (KW == 1) {
+            float u2;
+            to_half_range(fmaxf(part[j][0], part[j][1]), u2, downs[0]);
+            to_half_range(fmaxf(part[j][2], part[j][3]), u2, downs[1]);
+        } else downs[j] = down;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                // rows 32 ks + 4 q .. + 3 and 16 behind them: an operand's 8
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = v[32 * ks + 16 * (i / 4) + 4 * q + i % 4];
+                s8v hi, lo;
+                split8(e, up, hi, lo);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int at = (32 * ks + 16 * (i / 4) + 4 * q + i % 4) * ROW + n;
+                    plane[isc][0][at] = hi[i];
+                    plane[isc][1][at] = lo[i];
+                }
+                if (!isc) {
+                    s8v* to = reinterpret_cast<s8v*>(ops + 2 * op_c(KK)) + ((n / 16) * 2 + ks) * 64 + n % 16 + 16 * q;
+                    to[0] = hi;
+                    to[op_c(KK) / 16] = lo;
+                }
+            }
+    }
+    if (tid < 2) s.scales[(int64_t) blockIdx.x * 2 + tid] = tid ? downs[1] : downs[0];
+    __syncthreads();
+    // C as operands: (row, features 32 kk + 4 g .. + 3 and 16 behind them)
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const short* src = plane[1][h] + (16 * wave + n16) * ROW + 32 * kk + 4 * g;
+            const s4v a = *reinterpret_cast<const s4v*>(src), b = *reinterpret_cast<const s4v*>(src + 16);
+            reinterpret_cast<s8v*>(ops + h * op_c(KK))[(wave * KK + kk) * 64 + lane] = s8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        }
+    // C . B of 16 rows of C against the rows of B that they see: column a row of C, 4 consecutive rows of B a lane
+    const float down = downs[0] * downs[1];
+    for (int st = 0; st <= wave; ++st) {
+        f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const int ab = (16 * st + n16) * ROW + 32 * kk + 8 * g, ac = (16 * wave + n16) * ROW + 32 * kk + 8 * g;
+            const s8v bh = *reinterpret_cast<const s8v*>(plane[0][0] + ab), bl = *reinterpret_cast<const s8v*>(plane[0][1] + ab);
+            const s8v chh = *reinterpret_cast<const s8v*>(plane[1][0] + ac), cl = *reinterpret_cast<const s8v*>(plane[1][1] + ac);
+            acc = mfma16<false>(bh, chh, acc);
+            acc = mfma16<false>(bl, chh, acc);
+            acc = mfma16<false>(bh, cl, acc);
+        }
+        reinterpret_cast<f4v*>(ops + 4 * op_c(KK))[((wave * 2 + st / 2) * 64 + lane) * 2 + st % 2] = acc * down;
+    }
+    // the heads' step sizes and exponents, a lane a row
+    for (int hh = wave; hh < per; hh += 4) {
+        const int head = group * per + hh;
+        const float dt = lane < here ? ssm_dt<QT>(p, first + lane, head) : 0.0f;
+        const double add = (double) dt * (double) p.a[head] * 1.4426950408889634074;
+        double cum = add;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double b = __shfl_up(cum, o);
+            if (lane >= o) cum += b;
+        }
+        const double end = __shfl(cum, 63), base = __shfl(cum - add, lane / 16 * 16);
+        float* to = s.hdr + ((int64_t) chunk * p.H + head) * HDR;
+        to[HDR_C + lane] = (float) (cum - base);
+        to[HDR_DT + lane] = dt;
+        to[HDR_W + lane] = exp2f((float) (end - cum)) * dt;
+        to[HDR_E + lane] = exp2f((float) cum);
+        // starts of run lane / 4 and lane % 4 of 16
+        const double from = __shfl(cum - add, lane % 16 / 4 * 16), of = __shfl(cum - add, lane % 4 * 16);
+        if (lane < 16) to[HDR_BD + lane] = (float) (from - of);
+        if (lane < 2) to[HDR_END + lane] = lane ? exp2f((float) end) : (float) end;
+    }
+}
+
+template <int QT, int KW, bool STATE>
+__global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
+    constexpr int KK = 4 * KW;
+    constexpr bool Y3 = QT != 2;                                  // y's products from both halfs of their operands
+    __shared__ __align__(16) s8v xop[2][2][2][4][64];             // [x, weighted x][hi, lo][32 rows][16 columns][lane]
+    __shared__ __align__(16) s8v hop[STATE ? 1 : 2][STATE ? 1 : KK][4][64];   // the state: [hi, lo][32 features][16 columns][lane]
+    __shared__ float xs[2][64], hs[STATE ? 1 : KK][64];           // what their results are to be multiplied with, a column
+    __shared__ __align__(16) float hdr[HDR];
+    __shared__ int bad[64], anybad[2];                            // a column's first row that is not finite; whether there is one
+    const SsmLayer& p = s.l;
+    const int tid = threadIdx.x, lane = tid % 64, w = tid / 64, n = lane % 16, g = lane / 16;
+    // heads of a group read the same operands: consecutive work-groups of one XCD (every eighth of the launch)
+    int id = blockIdx.x;
+    const int total = gridDim.x;
+    if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
+    const int per = p.H / p.G, hb = per * s.blocks;
+    const int in_group = id % hb, seg = id / hb % s.segs, group = id / (hb * s.segs);
+    const int head = group * per + in_group / s.blocks, block = in_group % s.blocks, c0 = block * 64;
+    const int col = c0 + 16 * w + n;                              // the column of x this lane convolves
+    const bool has = col < p.P;
+    const int xch = head * p.P + (has ? col : 0);
+    const float w0 = ssm_tap(p, xch, 0), w1 = ssm_tap(p, xch, 1), w2 = ssm_tap(p, xch, 2), w3 = ssm_tap(p, xch, 3), bias = p.cb ? p.cb[xch] : 0.0f;
+    const float skip = p.d ? p.d[head] : 0.0f;
+    const int from = seg * s.per, to = min(s.chunks, from + s.per);
+    const int64_t owner = (int64_t) head * s.blocks + block, owners = (int64_t) p.H * s.blocks;
+
+    // features 32 (w KW + i / 2) + 16 (i % 2) + 4 g .. + 3 of column 16 ct + n
+    f4v st[2 * KW][4];
+    auto feature = [&](int i) { return 32 * (w * KW + i / 2) + 16 * (i % 2) + 4 * g; };
+    auto kept = [&](int slot) { return reinterpret_cast<f4v*>(s.segst) + ((slot * owners + owner) * 4 + w) * (2 * KW * 4 * 64) + lane; };
+    // (a cut pass's first state is read from where the state kernel has put it: the last segment may write h1 = h0 meanwhile)
+    if (STATE ? seg == 0 : s.segs == 1) {
+        const float* h0 = s.t0 ? p.h1 : p.h0;
+#pragma unroll
+        for (int i = 0; i < 2 * KW; ++i)
+#pragma unroll
+            for (int ct = 0; ct < 4; ++ct) {
+                f4v v = {0.0f, 0.0f, 0.0f, 0.0f};
+                const int f = feature(i), c = c0 + 16 * ct + n;
+                if (h0 && c < p.P && f < p.N) {
+                    const float* src = h0 + ((int64_t) head * p.P + c) * p.N + f;
+                    if (s.vec_h) v = *reinterpret_cast<const f4v*>(src);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (f + e < p.N) v[e] = src[e];
+                    }
+                }
+                st[i][ct] = v;
+                if (STATE) kept(0)[(i * 4 + ct) * 64] = v;
+            }
+    } else {
+        const f4v* src = kept(seg > 0 && !STATE);
+#pragma unroll
+        for (int i = 0; i < 2 * KW; ++i)
+#pragma unroll
+            for (int ct = 0; ct < 4; ++ct) st[i][ct] = STATE ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : src[(i * 4 + ct) * 64];
+        for (int r = 1; !STATE && r < seg; ++r) {
+            const float keep = exp2f(s.segtot[(int64_t) r * p.H + head]);
+            const f4v* add = kept(1 + r);
+#pragma unroll
+            for (int i = 0; i < 2 * KW; ++i)
+#pragma unroll
+                for (int ct = 0; ct < 4; ++ct) st[i][ct] = st[i][ct] * keep + add[(i * 4 + ct) * 64];
+        }
+    }
+    float exponent = 0.0f;
+    if (tid < 2) anybad[tid] = 0;
+    __syncthreads();
+
+    for (int c = from; c < to; ++c) {
+        const float* hd = s.hdr + ((int64_t) c * p.H + head) * HDR;
+        const uint8_t* ops = s.ops + ((int64_t) c * p.G + group) * op_bytes(KK);
+        const float sb = s.scales[((int64_t) c * p.G + group) * 2], sc = s.scales[((int64_t) c * p.G + group) * 2 + 1];
+        hdr[tid] = hd[tid];
+        if (tid < HDR - 256) hdr[256 + tid] = hd[256 + tid];
+        if (tid == 0) anybad[(c + 1) % 2] = 0;
+        // x: 16 rows of this lane's column - 32 ks + 16 h + 4 g .. + 3 - and their operands
+        {
+            const int here = min(L, s.T - c * L);
+            const int64_t first = s.t0 + (int64_t) c * L;
+            float x[2][8], xw[2][8], v[4][7], big = 0.0f, bigw = 0.0f;
+            int where = L;
+            if (first) {
+                const char* rows = static_cast<const char*>(p.xbc) + (first - 3) * p.xs * (QT ? 2 : 4);
+#pragma unroll
+                for (int j = 0; j < 28; ++j) {
+                    const uint32_t r = min(16 * (j / 7) + 4 * g + j % 7, here + 2);
+                    v[j / 7][j % 7] = load_q<QT>(rows + (r * (uint32_t) p.xs + (uint32_t) xch) * (QT ? 2 : 4), 0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 28; ++j) v[j / 7][j % 7] = raw_row<QT>(p, s.hist, min(16 * (j / 7) + 4 * g + j % 7 - 3, here - 1), xch);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = 32 * ks + 16 * h + 4 * g;
+                    const f4v wt = *reinterpret_cast<const f4v*>(hd + HDR_W + r);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float* u = v[2 * ks + h] + i;
+                        float y = silu(fmaf(w3, u[3], fmaf(w2, u[2], fmaf(w1, u[1], fmaf(w0, u[0], bias)))));
+                        if (!has || r + i >= here) y = 0.0f;
+                        x[ks][4 * h + i] = y;
+                        xw[ks][4 * h + i] = y * wt[i];
+                        if (!STATE) big = fmaxf(big, fabsf(y));
+                        bigw = fmaxf(bigw, fabsf(y * wt[i]));
+                        if (!STATE && !(fabsf(y) < __builtin_inff()) && where == L) where = r + i;
+                    }
+                }
+            float up, down;
+            s8v hi, lo;
+            bigw = rows_max(bigw);
+            to_half_range(bigw, up, down);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                split8(xw[ks], up, hi, lo);
+                xop[1][0][ks][w][lane] = hi;
+                xop[1][1][ks][w][lane] = lo;
+            }
+            if (g == 0) xs[1][16 * w + n] = down;
+            if constexpr (!STATE) {
+                // a row that is not finite must not reach the rows in front of it (0 times it is not 0): it goes in as 0, and
+                // from it on the column is NaN
+                if (__ballot(where < L)) {
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (!(fabsf(x[ks][i]) < __builtin_inff())) x[ks][i] = 0.0f;
+                    where = min(where, __shfl_xor(where, 16));
+                    where = min(where, __shfl_xor(where, 32));
+                    big = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(x[i / 8][i % 8]));
+                    if (lane == 0) anybad[c % 2] = 1;
+                }
+                if (g == 0) bad[16 * w + n] = where;
+                big = rows_max(big);
+                to_half_range(big, up, down);
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    split8(x[ks], up, hi, lo);
+                    xop[0][0][ks][w][lane] = hi;
+                    if constexpr (Y3) xop[0][1][ks][w][lane] = lo;
+                }
+                if (g == 0) xs[0][16 * w + n] = down;
+            }
+        }
+        // this wave's part of the state
+        if constexpr (!STATE) {
+#pragma unroll
+            for (int j = 0; j < KW; ++j)
+#pragma unroll
+                for (int ct = 0; ct < 4; ++ct) {
+                    float v[8], big = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = st[2 * j + i / 4][ct][i % 4], big = fmaxf(big, fabsf(v[i]));
+                    float up, down;
+                    to_half_range(rows_max(big), up, down);
+                    s8v hi, lo;
+                    split8(v, up, hi, lo);
+                    hop[0][w * KW + j][ct][lane] = hi;
+                    if constexpr (Y3) hop[1][w * KW + j][ct][lane] = lo;
+                    if (g == 0) hs[w * KW + j][16 * ct + n] = down;
+                }
+        }
+        __syncthreads();
+        if constexpr (!STATE) {
+            // 16 rows of y: this lane row 16 w + n, columns 16 ct + 4 g .. + 3
+            f4v y[4], yi[4];
+#pragma unroll
+            for (int ct = 0; ct < 4; ++ct) y[ct] = yi[ct] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            const s8v* cop = reinterpret_cast<const s8v*>(ops) + w * KK * 64 + lane;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                const s8v chi = cop[kk * 64];
+                s8v clo = chi;
+                if constexpr (Y3) clo = cop[op_c(KK) / 16 + kk * 64];
+#pragma unroll
+                for (int ct = 0; ct < 4; ++ct) {
+                    f4v a = mfma16<false>(hop[0][kk][ct][lane], chi, f4v{0.0f, 0.0f, 0.0f, 0.0f});
+                    if constexpr (Y3) {
+                        a = mfma16<false>(hop[1][kk][ct][lane], chi, a);
+                        a = mfma16<false>(hop[0][kk][ct][lane], clo, a);
+                    }
+                    const f4v f = *reinterpret_cast<const f4v*>(&hs[kk][16 * ct + 4 * g]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) yi[ct][e] = fmaf(a[e], f[e], yi[ct][e]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // the chunk's own rows: C . B decayed, d on the diagonal
+            const int row = 16 * w + n;
+            const float cl = hdr[HDR_C + row];
+            const f4v* cbp = reinterpret_cast<const f4v*>(ops + 4 * op_c(KK)) + w * 2 * 64 * 2;
+            float m[2][8], big = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks > w / 2) break;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int sr = 32 * ks + 16 * h + 4 * g;
+                    const float base = cl + hdr[HDR_BD + 4 * w + 2 * ks + h];
+                    const f4v cb = cbp[(ks * 64 + lane) * 2 + h], cs = *reinterpret_cast<const f4v*>(hdr + HDR_C + sr), dt = *reinterpret_cast<const f4v*>(hdr + HDR_DT + sr);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v = cb[i] * dt[i] * fast_exp2(base - cs[i]);
+                        v = sr + i == row ? v + skip : v;
+                        v = sr + i > row ? 0.0f : v;
+                        m[ks][4 * h + i] = v;
+                        big = fmaxf(big, fabsf(v));
+                    }
+                }
+            }
+            float up, down;
+            to_half_range(rows_max(big), up, down);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks > w / 2) break;
+                s8v hi, lo;
+                split8(m[ks], up, hi, lo);
+#pragma unroll
+                for (int ct = 0; ct < 4; ++ct) {
+                    y[ct] = mfma16<false>(xop[0][0][ks][ct][lane], hi, y[ct]);
+                    if constexpr (Y3) {
+                        y[ct] = mfma16<false>(xop[0][1][ks][ct][lane], hi, y[ct]);
+                        y[ct] = mfma16<false>(xop[0][0][ks][ct][lane], lo, y[ct]);
+                    }
+                }
+            }
+            const int t = c * L + row;
+            const float el = hdr[HDR_E + row] * sc;
+            const bool spoilt = anybad[c % 2];
+#pragma unroll
+            for (int ct = 0; ct < 4; ++ct) {
+                const f4v f = *reinterpret_cast<const f4v*>(&xs[0][16 * ct + 4 * g]);
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = fmaf(y[ct][e], f[e] * down, yi[ct][e] * el);
+                if (spoilt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (row >= bad[16 * ct + 4 * g + e]) v[e] = __builtin_nanf("");
+                }
+                if (t >= s.T) continue;
+                const int pc = c0 + 16 * ct + 4 * g;
+                const int64_t at = (s.t0 + t) * p.ys + (int64_t) head * p.P + pc;
+                if (s.vec_y && pc + 4 <= p.P) store_row<QT, 4>(p.y, at, v);
+                else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (pc + e < p.P) store_o<QT>(p.y, at + e, v[e]);
+                }
+            }
+        }
+        // the state behind the chunk
+        {
+            const float keep = hdr[HDR_END + 1];
+            exponent += hdr[HDR_END];
+            const s8v* bop = reinterpret_cast<const s8v*>(ops + 2 * op_c(KK)) + lane;
+#pragma unroll
+            for (int i = 0; i < 2 * KW; ++i) {
+                const s8v* b = bop + (w * 2 * KW + i) * 2 * 64;
+                f4v a[4];
+#pragma unroll
+                for (int ct = 0; ct < 4; ++ct) a[ct] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    const s8v hi = b[ks * 64], lo = b[op_c(KK) / 16 + ks * 64];
+#pragma unroll
+                    for (int ct = 0; ct < 4; ++ct) {
+                        a[ct] = mfma16<false>(hi, xop[1][0][ks][ct][lane], a[ct]);
+                        a[ct] = mfma16<false>(lo, xop[1][0][ks][ct][lane], a[ct]);
+                        a[ct] = mfma16<false>(hi, xop[1][1][ks][ct][lane], a[ct]);
+                    }
+                }
+#pragma unroll
+                for (int ct = 0; ct < 4; ++ct) {
+                    const float f = sb * xs[1][16 * ct + n];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st[i][ct][e] = fmaf(st[i][ct][e], keep, a[ct][e] * f);
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+    if constexpr (STATE) {
+        f4v* dst = kept(1 + seg);
+#pragma unroll
+        for (int i = 0; i < 2 * KW; ++i)
+#pragma unroll
+            for (int ct = 0; ct < 4; ++ct) dst[(i * 4 + ct) * 64] = st[i][ct];
+        if (tid == 0 && block == 0) s.segtot[(int64_t) seg * p.H + head] = exponent;
+    } else {
+        if (seg == s.segs - 1) {
+#pragma unroll
+            for (int i = 0; i < 2 * KW; ++i)
+#pragma unroll
+                for (int ct = 0; ct < 4; ++ct) {
+                    const int f = feature(i), cc = c0 + 16 * ct + n;
+                    if (cc >= p.P || f >= p.N) continue;
+                    float* dst = p.h1 + ((int64_t) head * p.P + cc) * p.N + f;
+                    if (s.vec_h) *reinterpret_cast<f4v*>(dst) = st[i][ct];
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (f + e < p.N) dst[e] = st[i][ct][e];
+                    }
+                }
+        }
+        // the call's last raw rows into the ring: this block's x, and the group's B and C
+        if (seg == 0 && s.t0 + s.T == s.all) {
+            for (int64_t t = max((int64_t) 0, s.all - (p.K - 1)); t < s.all; ++t) {
+                float* dst = p.conv + (p.p0 + t) % p.cap * p.chan;
+                if (tid < 64 && c0 + tid < p.P) dst[head * p.P + c0 + tid] = load_q<QT>(p.xbc, t * p.xs + head * p.P + c0 + tid);
+                if (in_group == 0)
+                    for (int i = tid; i < 2 * p.N; i += 256) {
+                        const int ch = p.H * p.P + (i / p.N * p.G + group) * p.N + i % p.N;
+                        dst[ch] = load_q<QT>(p.xbc, t * p.xs + ch);
+                    }
+            }
+        }
+    }
+}
+
+// how a pass of T rows is cut, and where its scratch lies
+struct Plan {
+    int kk, chunks, segs, per, blocks;
+    int64_t ops, scales, hdr, hist, segst, segtot, floats;
+};
+Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G) {
+    Plan q{};
+    q.kk = N <= 128 ? 4 : 8;
+    q.chunks = (int) ((T + L - 1) / L);
+    q.blocks = (int) ((P + 63) / 64);
+    const int64_t owners = H * q.blocks;
+    // enough segments for two work-groups a CU, of 4 chunks at least
+    int64_t segs = std::max<int64_t>(1, std::min<int64_t>({MOST_SEGS, 512 / owners, q.chunks / 4}));
+    q.per = (int) ((q.chunks + segs - 1) / segs);
+    q.segs = (q.chunks + q.per - 1) / q.per;
+    int64_t at = 0;
+    auto take = [&](int64_t floats) {
+        const int64_t here = at;
+        at += (floats + 3) / 4 * 4;
+        return here;
+    };
+    q.ops = take(q.chunks * G * op_bytes(q.kk) / 4);
+    q.scales = take(q.chunks * G * 2);
+    q.hdr = take(q.chunks * H * HDR);
+    q.hist = take(3 * (H * P + 2 * G * N));
+    q.segst = take(q.segs > 1 ? q.segs * owners * 64 * q.kk * 32 : 0);
+    q.segtot = take(q.segs > 1 ? q.segs * H : 0);
+    q.floats = at;
+    return q;
+}
+
+template <int QT, int KW>
+void launch_pass(ns_gpu* g, ScanParams& s, const Plan& q) {
+    ssm_prep_kernel<QT, KW><<<(unsigned) (q.chunks * s.l.G), 256, 0, g->q>>>(s);
+    const unsigned owners = (unsigned) (s.l.H * q.blocks);
+    if (q.segs > 1) {
+        ScanParams f = s;
+        f.segs = q.segs - 1;            // (the last segment's state is the scan's own)
+        ssm_scan_kernel<QT, KW, true><<<owners * f.segs, 256, 0, g->q>>>(f);
+    }
+    ssm_scan_kernel<QT, KW, false><<<owners * q.segs, 256, 0, g->q>>>(s);
 }
 
 template <int QT>
 void run_prompt(ns_gpu* g, const SsmLayer& p, int64_t T, float* scratch) {
-    float *u = scratch, *dt = scratch + std::min(T, PASS_ROWS) * p.chan;
     for (int64_t t0 = 0; t0 < T; t0 += PASS_ROWS) {
-        const int n = (int) std::min(PASS_ROWS, T - t0);
-        ssm_conv_kernel<QT><<<dim3((unsigned) ((std::max(p.chan, p.H) + 255) / 256), (unsigned) n), 256, 0, g->q>>>(p, t0, n, u, dt);
-        ssm_scan_kernel<QT><<<(unsigned) (p.H * p.P), 64, 0, g->q>>>(p, t0, n, u, dt);
+        const int64_t n = std::min(PASS_ROWS, T - t0);
+        const Plan q = plan_of(n, p.H, p.P, p.N, p.G);
+        ScanParams s{p, t0, T, (int) n, q.chunks, q.segs, q.per, q.blocks};
+        s.vec_y = (uintptr_t) p.y % (QT ? 8 : 16) == 0 && p.ys % 4 == 0 && p.P % 4 == 0;
+        s.vec_h = p.N % 4 == 0 && (uintptr_t) p.h0 % 16 == 0 && (uintptr_t) p.h1 % 16 == 0;
+        s.ops = reinterpret_cast<uint8_t*>(scratch + q.ops);
+        s.scales = scratch + q.scales, s.hdr = scratch + q.hdr, s.hist = scratch + q.hist, s.segst = scratch + q.segst, s.segtot = scratch + q.segtot;
+        if (q.kk == 4) launch_pass<QT, 1>(g, s, q);
+        else launch_pass<QT, 2>(g, s, q);
     }
-    if (p.K > 1) ssm_ring_kernel<QT><<<dim3((unsigned) ((p.chan + 255) / 256), (unsigned) (p.K - 1)), 256, 0, g->q>>>(p, T);
 }
 
 }  // namespace
@@ -79,7 +602,10 @@ extern "C" {
 
 int64_t ns_ssm_prompt_scratch(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K) {
     if (T <= 0 || H <= 0 || P <= 0 || N <= 0 || G <= 0 || K <= 0) return 0;
-    return std::min(T, PASS_ROWS) * (H * P + 2 * G * N + H);
+    // (a last pass of fewer rows may be cut in more segments than a full one)
+    int64_t most = plan_of(std::min(T, PASS_ROWS), H, P, N, G).floats;
+    if (T > PASS_ROWS && T % PASS_ROWS) most = std::max(most, plan_of(T % PASS_ROWS, H, P, N, G).floats);
+    return most;
 }
 
 int ns_ssm_prompt(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt, int64_t dts, const float* cw, const float* cb, const float* a,
@@ -90,7 +616,10 @@ int ns_ssm_prompt(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt
     SsmLayer p{xbc, dt, xs, dts, cw, cb, a, dtb, d, dt_lo, dt_hi, conv, cap, p0, (int) H, (int) P, (int) N, (int) G, (int) K, 0, h0, h1, y, ys};
     if (ns_ssm_check("ns_ssm_prompt", g, qt, p, H, P, N, G, K, K - 1)) return -1;
     if (!scratch) return ns_fail("ns_ssm_prompt: a null buffer");
+    if (xs > (int64_t) 1 << 23) return ns_fail("ns_ssm_prompt: rows up to 2^23 values apart");
+    if ((uintptr_t) scratch % 16) return ns_fail("ns_ssm_prompt: scratch 16-byte aligned");
     p.chan = (int) (H * P + 2 * G * N);
+    if (K == 1) p.conv = nullptr, p.cap = 1;
     NS_HIP(hipSetDevice(g->dev));
     if (qt == 0) run_prompt<0>(g, p, T, scratch);
     else if (qt == 1) run_prompt<1>(g, p, T, scratch);

@@ -232,9 +232,11 @@ def test_wrappers_check_their_buffers(ops):
     L = Layer(2, 8, 16, 1, 4, seed=0)
     W, b = Weights(g, L), DevBuf(g, 1 << 16)
     T, row = 3, L.chan + 2
+    own = lambda: DevBuf(g, max(1 << 16, 4 * ops.ssm_prompt_scratch(T, 2, 8, 16, 1, 4)))  # noqa: E731
+    buffers = dict(ring=own(), h1=own(), y=own(), sc=own())
 
     def prompt(**k):
-        a = dict(rows=b, ring=b, h1=b, y=b, sc=b, qt=F32)
+        a = dict(rows=b, qt=F32, **buffers)
         a.update(k)
         ops.ssm_prompt(a["qt"], a["rows"], row, b, row, *W.args(), a["ring"], 4, 0, T, 2, 8, 16, 1, 4, None, a["h1"], a["y"], 16, a["sc"])
 
@@ -242,7 +244,7 @@ def test_wrappers_check_their_buffers(ops):
     for name, size in (("rows", (T - 1) * row * 4 + L.chan * 4 - 4), ("ring", 4 * L.chan * 4 - 4), ("h1", 2 * 8 * 16 * 4 - 4), ("y", T * 16 * 4 - 4),
                        ("sc", ops.ssm_prompt_scratch(T, 2, 8, 16, 1, 4) * 4 - 4)):
         with pytest.raises(Error, match="needs"):
-            prompt(**{name: b.view(0, size)})
+            prompt(**{name: buffers.get(name, b).view(0, size)})
     with pytest.raises(Error, match="rows of type"):
         prompt(qt=3)
     g.sync()
