@@ -71,14 +71,24 @@ __device__ __forceinline__ void split8(const float (&v)[8], float up, s8v& hi, s
     lo = __builtin_bit_cast(s8v, b);
 }
 
-// the raw value of channel ch, `at` rows behind the call's first (negative: in front of it)
-template <int QT>
-__device__ __forceinline__ float raw_row(const SsmLayer& p, const float* hist, int64_t at, int ch) {
-    return at >= 0 ? load_q<QT>(p.xbc, at * p.xs + ch) : hist[(at + 3) * p.chan + ch];
-}
-// the ring's value at that row: zeros in front of the sequence, and of taps that there are not
+// the ring's value `at` rows (negative) from the call's first: zeros in front of the sequence, and of taps that there are not
 __device__ __forceinline__ float ring_row(const SsmLayer& p, int64_t at, int ch) {
     return at >= 1 - p.K && p.p0 + at >= 0 ? p.conv[(p.p0 + at) % p.cap * p.chan + ch] : 0.0f;
+}
+
+// A work-group's barrier for what its waves exchange through LDS: memory loads for the next chunk and rows on their way out
+// stay in flight across it (a __syncthreads waits for both)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// a row's value as it lies in memory, and as a number
+template <int QT>
+__device__ __forceinline__ uint32_t raw_bits(const char* p, uint32_t off) {
+    if constexpr (QT == 0) return *reinterpret_cast<const uint32_t*>(p + off);
+    else return *reinterpret_cast<const uint16_t*>(p + off);
+}
+template <int QT>
+__device__ __forceinline__ float raw_value(uint32_t b) {
+    return QT == 0 ? __builtin_bit_cast(float, b) : QT == 1 ? f16_to_f32((uint16_t) b) : bf16_to_f32((uint16_t) b);
 }
 
 template <int QT, int KW>
@@ -87,7 +97,7 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_prep_kernel(ScanParams s) {
     __shared__ __align__(16) short plane[2][2][L * ROW];       // [B, C][hi, lo][row][feature]
     __shared__ float part[2][4];
     const SsmLayer& p = s.l;
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n16 = lane % 16, g = lane / 16;
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n16 = lane % 16, g = lane / 16;
     const int chunk = blockIdx.x / p.G, group = blockIdx.x % p.G, per = p.H / p.G;
     const int here = min(L, s.T - chunk * L);
     const int64_t first = s.t0 + (int64_t) chunk * L;
@@ -216,10 +226,10 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
     __shared__ __align__(16) s8v xop[2][2][2][4][64];             // [x, weighted x][hi, lo][32 rows][16 columns][lane]
     __shared__ __align__(16) s8v hop[STATE ? 1 : 2][STATE ? 1 : KK][4][64];   // the state: [hi, lo][32 features][16 columns][lane]
     __shared__ float xs[2][64], hs[STATE ? 1 : KK][64];           // what their results are to be multiplied with, a column
-    __shared__ __align__(16) float hdr[HDR];
+    __shared__ __align__(16) float hdrs[2][HDR];
     __shared__ int bad[64], anybad[2];                            // a column's first row that is not finite; whether there is one
     const SsmLayer& p = s.l;
-    const int tid = threadIdx.x, lane = tid % 64, w = tid / 64, n = lane % 16, g = lane / 16;
+    const int tid = threadIdx.x, lane = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, g = lane / 16;
     // heads of a group read the same operands: consecutive work-groups of one XCD (every eighth of the launch)
     int id = blockIdx.x;
     const int total = gridDim.x;
@@ -277,48 +287,113 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
     }
     float exponent = 0.0f;
     if (tid < 2) anybad[tid] = 0;
+    // a chunk's header, through registers into LDS; x: 16 rows of this lane's column - 16 j + 4 g .. + 3 - and 3 in front of each 4
+    float head0, head1;
+    auto fetch_header = [&](int c) {
+        const float* hd = s.hdr + ((int64_t) min(c, s.chunks - 1) * p.H + head) * HDR;
+        head0 = hd[tid];
+        head1 = hd[256 + tid % (HDR - 256)];
+    };
+    auto put_header = [&](int c) {
+        hdrs[c % 2][tid] = head0;
+        if (tid < HDR - 256) hdrs[c % 2][256 + tid] = head1;
+    };
+    uint32_t raw[28];
+    const int64_t row_bytes = p.xs * (QT ? 2 : 4);
+    const uint32_t lane_off = (uint32_t) (4 * g * row_bytes + (int64_t) xch * (QT ? 2 : 4));
+    auto fetch_x = [&](int c, int g) {
+        const int here = min(L, s.T - c * L);
+        const int64_t first = s.t0 + (int64_t) c * L;
+        if (first > 0 && here == L) {
+            // (opaque too: the compiler would carry 28 addresses from chunk to chunk)
+            const char* rows = static_cast<const char*>(p.xbc) + (first - 3) * row_bytes;
+            int64_t step = row_bytes;
+            asm volatile("" : "+s"(rows), "+s"(step));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const char* run = rows + 16 * j * step;
+#pragma unroll
+                for (int i = 0; i < 7; ++i, run += step) raw[7 * j + i] = raw_bits<QT>(run, lane_off);
+            }
+        } else {
+            // the call's first chunk, or one that is not whole: rows held to those that there are (those in front of the call come from the ring)
+            const int skipped = first > 0 ? 3 : 0;
+            const char* rows = static_cast<const char*>(p.xbc) + (first - skipped) * row_bytes;
+#pragma unroll
+            for (int j = 0; j < 28; ++j) {
+                const int r = min(max(16 * (j / 7) + 4 * g + j % 7 - 3 + skipped, 0), here - 1 + skipped);
+                raw[j] = raw_bits<QT>(rows, (uint32_t) r * (uint32_t) row_bytes + (uint32_t) xch * (QT ? 2 : 4));
+            }
+        }
+    };
+    fetch_header(from);
+    put_header(from);
+    fetch_x(from, g);
     __syncthreads();
 
     for (int c = from; c < to; ++c) {
-        const float* hd = s.hdr + ((int64_t) c * p.H + head) * HDR;
+        const float* hdr = hdrs[c % 2];
         const uint8_t* ops = s.ops + ((int64_t) c * p.G + group) * op_bytes(KK);
         const float sb = s.scales[((int64_t) c * p.G + group) * 2], sc = s.scales[((int64_t) c * p.G + group) * 2 + 1];
-        hdr[tid] = hd[tid];
-        if (tid < HDR - 256) hdr[256 + tid] = hd[256 + tid];
+        // (opaque copies: addresses and comparisons made of them are a few instructions where they are needed, and not a
+        // hundred registers kept over the loop)
+        int ln = n, lg = g;
+        asm volatile("" : "+v"(ln), "+v"(lg));
+        fetch_header(c + 1);
+        // this chunk's operands, on their way while x and the state become theirs
+        s8v bop[2 * KW][2][2], cop[STATE ? 1 : KK][2];
+        f4v cbv[2][2];
+        {
+            const s8v* b = reinterpret_cast<const s8v*>(ops + 2 * op_c(KK)) + lane;
+#pragma unroll
+            for (int i = 0; i < 2 * KW; ++i)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) bop[i][ks][h] = b[((w * 2 * KW + i) * 2 + ks) * 64 + h * (op_c(KK) / 16)];
+        }
+        if constexpr (!STATE) {
+            const s8v* cp = reinterpret_cast<const s8v*>(ops) + w * KK * 64 + lane;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int h = 0; h < (Y3 ? 2 : 1); ++h) cop[kk][h] = cp[kk * 64 + h * (op_c(KK) / 16)];
+            const f4v* cbp = reinterpret_cast<const f4v*>(ops + 4 * op_c(KK)) + w * 2 * 64 * 2;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (ks <= w / 2) cbv[ks][h] = cbp[(ks * 64 + lane) * 2 + h];
+        }
         if (tid == 0) anybad[(c + 1) % 2] = 0;
-        // x: 16 rows of this lane's column - 32 ks + 16 h + 4 g .. + 3 - and their operands
+        // x's operands
         {
             const int here = min(L, s.T - c * L);
-            const int64_t first = s.t0 + (int64_t) c * L;
-            float x[2][8], xw[2][8], v[4][7], big = 0.0f, bigw = 0.0f;
+            const bool whole = here == L;
+            float x[2][8], xw[2][8], big = 0.0f, bigw = 0.0f;
             int where = L;
-            if (first) {
-                const char* rows = static_cast<const char*>(p.xbc) + (first - 3) * p.xs * (QT ? 2 : 4);
-#pragma unroll
-                for (int j = 0; j < 28; ++j) {
-                    const uint32_t r = min(16 * (j / 7) + 4 * g + j % 7, here + 2);
-                    v[j / 7][j % 7] = load_q<QT>(rows + (r * (uint32_t) p.xs + (uint32_t) xch) * (QT ? 2 : 4), 0);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 28; ++j) v[j / 7][j % 7] = raw_row<QT>(p, s.hist, min(16 * (j / 7) + 4 * g + j % 7 - 3, here - 1), xch);
-            }
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int r = 32 * ks + 16 * h + 4 * g;
-                    const f4v wt = *reinterpret_cast<const f4v*>(hd + HDR_W + r);
+                    const int r = 32 * ks + 16 * h + 4 * lg;
+                    const f4v wt = *reinterpret_cast<const f4v*>(hdr + HDR_W + r);
+                    float u[7];
+#pragma unroll
+                    for (int i = 0; i < 7; ++i) u[i] = raw_value<QT>(raw[(2 * ks + h) * 7 + i]);
+                    if (ks == 0 && h == 0 && c == 0 && s.t0 == 0) {
+                        // (in front of the call: float32 from the ring, whatever the rows' type)
+#pragma unroll
+                        for (int i = 0; i < 3; ++i) u[i] = lg == 0 ? s.hist[(int64_t) i * p.chan + xch] : u[i];
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float* u = v[2 * ks + h] + i;
-                        float y = silu(fmaf(w3, u[3], fmaf(w2, u[2], fmaf(w1, u[1], fmaf(w0, u[0], bias)))));
-                        if (!has || r + i >= here) y = 0.0f;
+                        float y = silu(fmaf(w3, u[i + 3], fmaf(w2, u[i + 2], fmaf(w1, u[i + 1], fmaf(w0, u[i], bias)))));
+                        if (!whole) y = r + i < here ? y : 0.0f;
                         x[ks][4 * h + i] = y;
                         xw[ks][4 * h + i] = y * wt[i];
                         if (!STATE) big = fmaxf(big, fabsf(y));
                         bigw = fmaxf(bigw, fabsf(y * wt[i]));
-                        if (!STATE && !(fabsf(y) < __builtin_inff()) && where == L) where = r + i;
                     }
                 }
             float up, down;
@@ -334,18 +409,23 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
             if (g == 0) xs[1][16 * w + n] = down;
             if constexpr (!STATE) {
                 // a row that is not finite must not reach the rows in front of it (0 times it is not 0): it goes in as 0, and
-                // from it on the column is NaN
-                if (__ballot(where < L)) {
+                // from it on the column is NaN. (Sixteen numbers times 0 sum to 0, or to NaN where one is not finite)
+                float zero = 0.0f;
 #pragma unroll
-                    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (!(fabsf(x[ks][i]) < __builtin_inff())) x[ks][i] = 0.0f;
-                    where = min(where, __shfl_xor(where, 16));
-                    where = min(where, __shfl_xor(where, 32));
+                for (int i = 0; i < 16; ++i) zero = fmaf(x[i / 8][i % 8], 0.0f, zero);
+                if (__ballot(zero != zero)) {
                     big = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(x[i / 8][i % 8]));
+                    for (int i = 15; i >= 0; --i) {
+                        float& y = x[i / 8][i % 8];
+                        if (!(fabsf(y) < __builtin_inff())) {
+                            y = 0.0f;
+                            where = 16 * (i / 4) + 4 * lg + i % 4;
+                        }
+                        big = fmaxf(big, fabsf(y));
+                    }
+                    where = min(where, __shfl_xor(where, 16));
+                    where = min(where, __shfl_xor(where, 32));
                     if (lane == 0) anybad[c % 2] = 1;
                 }
                 if (g == 0) bad[16 * w + n] = where;
@@ -378,53 +458,56 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
                     if (g == 0) hs[w * KW + j][16 * ct + n] = down;
                 }
         }
-        __syncthreads();
+        lds_barrier();
+        if (c + 1 < to) fetch_x(c + 1, lg);
         if constexpr (!STATE) {
             // 16 rows of y: this lane row 16 w + n, columns 16 ct + 4 g .. + 3
             f4v y[4], yi[4];
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) y[ct] = yi[ct] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-            const s8v* cop = reinterpret_cast<const s8v*>(ops) + w * KK * 64 + lane;
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                const s8v chi = cop[kk * 64];
-                s8v clo = chi;
-                if constexpr (Y3) clo = cop[op_c(KK) / 16 + kk * 64];
 #pragma unroll
                 for (int ct = 0; ct < 4; ++ct) {
-                    f4v a = mfma16<false>(hop[0][kk][ct][lane], chi, f4v{0.0f, 0.0f, 0.0f, 0.0f});
+                    f4v a = mfma16<false>(hop[0][kk][ct][lane], cop[kk][0], f4v{0.0f, 0.0f, 0.0f, 0.0f});
                     if constexpr (Y3) {
-                        a = mfma16<false>(hop[1][kk][ct][lane], chi, a);
-                        a = mfma16<false>(hop[0][kk][ct][lane], clo, a);
+                        a = mfma16<false>(hop[1][kk][ct][lane], cop[kk][0], a);
+                        a = mfma16<false>(hop[0][kk][ct][lane], cop[kk][1], a);
                     }
                     const f4v f = *reinterpret_cast<const f4v*>(&hs[kk][16 * ct + 4 * g]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) yi[ct][e] = fmaf(a[e], f[e], yi[ct][e]);
                 }
-                __builtin_amdgcn_sched_barrier(0);
+                // (here, and not where y is written: the compiler would keep every step's results and scales until then)
+#pragma unroll
+                for (int ct = 0; ct < 4; ++ct) asm volatile("" : "+v"(yi[ct]));
             }
             // the chunk's own rows: C . B decayed, d on the diagonal
-            const int row = 16 * w + n;
+            const int row = 16 * w + ln;
             const float cl = hdr[HDR_C + row];
-            const f4v* cbp = reinterpret_cast<const f4v*>(ops + 4 * op_c(KK)) + w * 2 * 64 * 2;
             float m[2][8], big = 0.0f;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (ks > w / 2) break;
+            for (int st = 0; st < 4; ++st) {
+                const int sr = 16 * st + 4 * lg;
+                float* to_m = m[st / 2] + 4 * (st % 2);
+                if (st > w) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int sr = 32 * ks + 16 * h + 4 * g;
-                    const float base = cl + hdr[HDR_BD + 4 * w + 2 * ks + h];
-                    const f4v cb = cbp[(ks * 64 + lane) * 2 + h], cs = *reinterpret_cast<const f4v*>(hdr + HDR_C + sr), dt = *reinterpret_cast<const f4v*>(hdr + HDR_DT + sr);
+                    for (int i = 0; i < 4; ++i) to_m[i] = 0.0f;
+                    continue;
+                }
+                const float base = cl + hdr[HDR_BD + 4 * w + st];
+                const f4v cb = cbv[st / 2][st % 2], cs = *reinterpret_cast<const f4v*>(hdr + HDR_C + sr), dt = *reinterpret_cast<const f4v*>(hdr + HDR_DT + sr);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) to_m[i] = cb[i] * dt[i] * fast_exp2(base - cs[i]);
+                if (st == w) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float v = cb[i] * dt[i] * fast_exp2(base - cs[i]);
-                        v = sr + i == row ? v + skip : v;
-                        v = sr + i > row ? 0.0f : v;
-                        m[ks][4 * h + i] = v;
-                        big = fmaxf(big, fabsf(v));
+                        to_m[i] = 4 * lg + i == ln ? to_m[i] + skip : to_m[i];
+                        to_m[i] = 4 * lg + i > ln ? 0.0f : to_m[i];
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(to_m[i]));
             }
             float up, down;
             to_half_range(rows_max(big), up, down);
@@ -447,17 +530,17 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
             const bool spoilt = anybad[c % 2];
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) {
-                const f4v f = *reinterpret_cast<const f4v*>(&xs[0][16 * ct + 4 * g]);
+                const f4v f = *reinterpret_cast<const f4v*>(&xs[0][16 * ct + 4 * lg]);
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = fmaf(y[ct][e], f[e] * down, yi[ct][e] * el);
                 if (spoilt) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (row >= bad[16 * ct + 4 * g + e]) v[e] = __builtin_nanf("");
+                        if (row >= bad[16 * ct + 4 * lg + e]) v[e] = __builtin_nanf("");
                 }
                 if (t >= s.T) continue;
-                const int pc = c0 + 16 * ct + 4 * g;
+                const int pc = c0 + 16 * ct + 4 * lg;
                 const int64_t at = (s.t0 + t) * p.ys + (int64_t) head * p.P + pc;
                 if (s.vec_y && pc + 4 <= p.P) store_row<QT, 4>(p.y, at, v);
                 else {
@@ -471,23 +554,19 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
         {
             const float keep = hdr[HDR_END + 1];
             exponent += hdr[HDR_END];
-            const s8v* bop = reinterpret_cast<const s8v*>(ops + 2 * op_c(KK)) + lane;
 #pragma unroll
             for (int i = 0; i < 2 * KW; ++i) {
-                const s8v* b = bop + (w * 2 * KW + i) * 2 * 64;
                 f4v a[4];
 #pragma unroll
                 for (int ct = 0; ct < 4; ++ct) a[ct] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    const s8v hi = b[ks * 64], lo = b[op_c(KK) / 16 + ks * 64];
+                for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                     for (int ct = 0; ct < 4; ++ct) {
-                        a[ct] = mfma16<false>(hi, xop[1][0][ks][ct][lane], a[ct]);
-                        a[ct] = mfma16<false>(lo, xop[1][0][ks][ct][lane], a[ct]);
-                        a[ct] = mfma16<false>(hi, xop[1][1][ks][ct][lane], a[ct]);
+                        a[ct] = mfma16<false>(bop[i][ks][0], xop[1][0][ks][ct][lane], a[ct]);
+                        a[ct] = mfma16<false>(bop[i][ks][1], xop[1][0][ks][ct][lane], a[ct]);
+                        a[ct] = mfma16<false>(bop[i][ks][0], xop[1][1][ks][ct][lane], a[ct]);
                     }
-                }
 #pragma unroll
                 for (int ct = 0; ct < 4; ++ct) {
                     const float f = sb * xs[1][16 * ct + n];
@@ -496,7 +575,8 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
                 }
             }
         }
-        __syncthreads();
+        put_header(c + 1);
+        lds_barrier();
     }
 
     if constexpr (STATE) {
