@@ -63,6 +63,10 @@ __device__ __forceinline__ void store_row(void* p, int64_t i, const float (&v)[V
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + fast_exp2(v * -1.44269504f)); }
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))) + (v != v ? v : 0.0f); }
 
+// A work-group's barrier for what its waves exchange through LDS: memory loads asked for ahead and stores on their
+// way out stay in flight across it (a __syncthreads waits for both)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // the sum over each run of L lanes (L a power of two up to 64), in every lane of the run
 template <int L>
 __device__ __forceinline__ float lanes_sum(float v) {
@@ -98,10 +102,9 @@ struct SsmLayer {
     int64_t ys;
 };
 
-// the step size of a row's head
-template <int QT>
-__device__ __forceinline__ float ssm_dt(const SsmLayer& p, int64_t row, int head) {
-    const float s = softplus(load_q<QT>(p.dt, row * p.dts + head) + (p.dtb ? p.dtb[head] : 0.0f));
+// a head's step size: its row's value with the bias added, through softplus, held to the layer's limits
+__device__ __forceinline__ float ssm_dt(const SsmLayer& p, float v) {
+    const float s = softplus(v);
     return s < p.lo ? p.lo : s > p.hi ? p.hi : s;
 }
 // tap k of 4 of a channel: the layer's K taps are the last K of them

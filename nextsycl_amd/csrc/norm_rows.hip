@@ -4,7 +4,8 @@
 // Bound: HBM for prompts (each row read once and written once: 6 bytes a value of bfloat16 rows for the gated norm), a
 // launch and one memory latency for a token. A unit - a group of a row, or a row - is held in registers by 64, 256 or 1024
 // threads, so nothing is read twice; sums of squares and everything between load and store are float32, rounded once at
-// the end. A unit too long for 1024 threads' registers is read twice (ranges past 16384 to 32768 values).
+// the end. A unit of more than 4096 pieces (16384 to 32768
+// values, 4096 where rows are not aligned) is read twice.
 #include <algorithm>
 #include <type_traits>
 
@@ -14,20 +15,28 @@
 
 namespace {
 
-// the sum over a unit's TPU threads, in all of them (units of more than a wave: one a block)
-template <int TPU>
+// the sum over a unit's threads, in all of them (WIDE: a unit is its whole block; else a wave)
+template <bool WIDE>
 __device__ __forceinline__ float unit_sum(float v, float* part) {
     v = wave_sum(v);
-    if constexpr (TPU > 64) {
+    if constexpr (WIDE) {
         __syncthreads();                 // (what an earlier sum of the unit left has been read)
         if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
         __syncthreads();
         v = 0.0f;
-#pragma unroll
-        for (int i = 0; i < TPU / 64; ++i) v += part[i];
+        for (int i = 0; i < (int) blockDim.x / 64; ++i) v += part[i];
     }
     return v;
 }
+// VEC weights from element i on, or ones
+template <int VEC>
+__device__ __forceinline__ void load_weights(const float* w, int64_t i, float (&v)[VEC]) {
+    if (w) load_row<0, VEC>(w, i, v);
+    else
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = 1.0f;
+}
+__device__ __forceinline__ float inverse_root(float sum, int n, float eps) { return 1.0f / sqrtf(sum / (float) n + eps); }
 
 struct GatedParams {
     const void *y, *z;
@@ -39,25 +48,22 @@ struct GatedParams {
 };
 
 // IT pieces of VEC values a thread; IT 0: any number, read twice
-template <int QT, int VEC, int TPU, int IT>
-__global__ __launch_bounds__(TPU > 256 ? TPU : 256) void norm_gated_kernel(GatedParams p) {
-    constexpr int UNITS = TPU > 256 ? 1 : 256 / TPU;
+template <int QT, int VEC, bool WIDE, int IT>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_gated_kernel(GatedParams p) {
     __shared__ float part[16];
-    const int64_t unit = (int64_t) blockIdx.x * UNITS + threadIdx.x / TPU;
+    const int tpu = WIDE ? blockDim.x : 64, tid = WIDE ? threadIdx.x : threadIdx.x % 64;
+    const int64_t unit = WIDE ? blockIdx.x : (int64_t) blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64;
     if (unit >= p.units) return;         // (whole waves; a unit of more than one is its whole block)
-    const int tid = threadIdx.x % TPU;
     const int64_t t = unit / p.groups, c0 = unit % p.groups * p.W;
     auto values = [&](int at, float (&v)[VEC], float (&s)[VEC]) {
         load_row<QT, VEC>(p.y, t * p.ys + c0 + at, v);
         load_row<QT, VEC>(p.z, t * p.zs + c0 + at, s);
     };
     auto result = [&](int at, float (&v)[VEC], const float (&s)[VEC], float inv) {
+        float w[VEC];
+        load_weights<VEC>(p.w, c0 + at, w);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            v[j] *= inv;
-            if (p.w) v[j] *= p.w[c0 + at + j];
-            if (p.order) v[j] *= s[j];
-        }
+        for (int j = 0; j < VEC; ++j) v[j] *= p.order ? inv * w[j] * s[j] : inv * w[j];
         store_row<QT, VEC>(p.out, t * p.os + c0 + at, v);
     };
     float sum = 0.0f;
@@ -73,26 +79,26 @@ __global__ __launch_bounds__(TPU > 256 ? TPU : 256) void norm_gated_kernel(Gated
         float v[IT][VEC], s[IT][VEC];
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int at = (i * TPU + tid) * VEC;
+            const int at = (i * tpu + tid) * VEC;
             if (at < p.W) values(at, v[i], s[i]);
         }
 #pragma unroll
         for (int i = 0; i < IT; ++i)
-            if ((i * TPU + tid) * VEC < p.W) square(v[i], s[i]);
-        const float inv = 1.0f / sqrtf(unit_sum<TPU>(sum, part) / (float) p.W + p.eps);
+            if ((i * tpu + tid) * VEC < p.W) square(v[i], s[i]);
+        const float inv = inverse_root(unit_sum<WIDE>(sum, part), p.W, p.eps);
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int at = (i * TPU + tid) * VEC;
+            const int at = (i * tpu + tid) * VEC;
             if (at < p.W) result(at, v[i], s[i], inv);
         }
     } else {
         float v[VEC], s[VEC];
-        for (int at = tid * VEC; at < p.W; at += TPU * VEC) {
+        for (int at = tid * VEC; at < p.W; at += tpu * VEC) {
             values(at, v, s);
             square(v, s);
         }
-        const float inv = 1.0f / sqrtf(unit_sum<TPU>(sum, part) / (float) p.W + p.eps);
-        for (int at = tid * VEC; at < p.W; at += TPU * VEC) {
+        const float inv = inverse_root(unit_sum<WIDE>(sum, part), p.W, p.eps);
+        for (int at = tid * VEC; at < p.W; at += tpu * VEC) {
             values(at, v, s);
             square(v, s);
             result(at, v, s, inv);
@@ -109,14 +115,12 @@ struct ResidualParams {
     float eps, scale;
 };
 
-template <int QT, int RT, int VEC, int TPU, int IT>
-__global__ __launch_bounds__(TPU > 256 ? TPU : 256) void norm_residual_kernel(ResidualParams p) {
-    constexpr int UNITS = TPU > 256 ? 1 : 256 / TPU;
+template <int QT, int RT, int VEC, bool WIDE, int IT>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_residual_kernel(ResidualParams p) {
     __shared__ float part[16];
-    const int64_t t = (int64_t) blockIdx.x * UNITS + threadIdx.x / TPU;
+    const int tpu = WIDE ? blockDim.x : 64, tid = WIDE ? threadIdx.x : threadIdx.x % 64;
+    const int64_t t = WIDE ? blockIdx.x : (int64_t) blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64;
     if (t >= p.T) return;
-    const int tid = threadIdx.x % TPU;
-    const float mean = 1.0f / (float) p.D;
     auto load_x = [&](int at, float (&v)[VEC]) {
         if (p.x) load_row<QT, VEC>(p.x, t * p.xs + at, v);
         else
@@ -125,17 +129,30 @@ __global__ __launch_bounds__(TPU > 256 ? TPU : 256) void norm_residual_kernel(Re
     };
     // s = h + scale gate post (x inv)
     auto stream = [&](int at, float (&v)[VEC], const float (&h)[VEC], float inv) {
+        if (!p.x) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            float a = v[j];
-            if (p.post) a = a * inv * p.post[at + j];
-            if (p.gate) a *= p.gate[at + j];
-            v[j] = p.x ? fmaf(p.scale, a, h[j]) : h[j];
+            for (int j = 0; j < VEC; ++j) v[j] = h[j];
+            return;
         }
+        float w[VEC];
+        if (p.post) {
+            load_weights<VEC>(p.post, at, w);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = v[j] * inv * w[j];
+        }
+        if (p.gate) {
+            load_weights<VEC>(p.gate, at, w);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] *= w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = fmaf(p.scale, v[j], h[j]);
     };
     auto result = [&](int at, float (&v)[VEC], float inv) {
+        float w[VEC];
+        load_weights<VEC>(p.pre, at, w);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = v[j] * inv * (p.pre ? p.pre[at + j] : 1.0f);
+        for (int j = 0; j < VEC; ++j) v[j] = v[j] * inv * w[j];
         store_row<QT, VEC>(p.out, t * p.os + at, v);
     };
     auto squares = [&](const float (&v)[VEC]) {
@@ -148,7 +165,7 @@ __global__ __launch_bounds__(TPU > 256 ? TPU : 256) void norm_residual_kernel(Re
         float v[IT][VEC], h[IT][VEC];
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int at = (i * TPU + tid) * VEC;
+            const int at = (i * tpu + tid) * VEC;
             if (at < p.D) {
                 load_x(at, v[i]);
                 load_row<RT, VEC>(p.h, t * p.hs + at, h[i]);
@@ -159,44 +176,44 @@ __global__ __launch_bounds__(TPU > 256 ? TPU : 256) void norm_residual_kernel(Re
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < IT; ++i)
-                if ((i * TPU + tid) * VEC < p.D) sum += squares(v[i]);
-            inv = 1.0f / sqrtf(unit_sum<TPU>(sum, part) * mean + p.eps);
+                if ((i * tpu + tid) * VEC < p.D) sum += squares(v[i]);
+            inv = inverse_root(unit_sum<WIDE>(sum, part), p.D, p.eps);
         }
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int at = (i * TPU + tid) * VEC;
+            const int at = (i * tpu + tid) * VEC;
             if (at >= p.D) continue;
             stream(at, v[i], h[i], inv);
             sum += squares(v[i]);
             if (p.h1) store_row<RT, VEC>(p.h1, t * p.h1s + at, v[i]);
         }
         if (!p.out) return;
-        inv = 1.0f / sqrtf(unit_sum<TPU>(sum, part) * mean + p.eps);
+        inv = inverse_root(unit_sum<WIDE>(sum, part), p.D, p.eps);
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int at = (i * TPU + tid) * VEC;
+            const int at = (i * tpu + tid) * VEC;
             if (at < p.D) result(at, v[i], inv);
         }
     } else {
         // too long for registers: x and h are read again for each step, the stream written last (h1 may be h)
         float v[VEC], h[VEC], inv = 1.0f, sum = 0.0f;
         if (p.post) {
-            for (int at = tid * VEC; at < p.D; at += TPU * VEC) {
+            for (int at = tid * VEC; at < p.D; at += tpu * VEC) {
                 load_x(at, v);
                 sum += squares(v);
             }
-            inv = 1.0f / sqrtf(unit_sum<TPU>(sum, part) * mean + p.eps);
+            inv = inverse_root(unit_sum<WIDE>(sum, part), p.D, p.eps);
             sum = 0.0f;
         }
-        for (int at = tid * VEC; at < p.D; at += TPU * VEC) {
+        for (int at = tid * VEC; at < p.D; at += tpu * VEC) {
             load_x(at, v);
             load_row<RT, VEC>(p.h, t * p.hs + at, h);
             stream(at, v, h, inv);
             sum += squares(v);
         }
-        const float inv2 = 1.0f / sqrtf(unit_sum<TPU>(sum, part) * mean + p.eps);
-        for (int at = tid * VEC; at < p.D; at += TPU * VEC) {
+        const float inv2 = inverse_root(unit_sum<WIDE>(sum, part), p.D, p.eps);
+        for (int at = tid * VEC; at < p.D; at += tpu * VEC) {
             load_x(at, v);
             load_row<RT, VEC>(p.h, t * p.hs + at, h);
             stream(at, v, h, inv);
@@ -206,39 +223,35 @@ __global__ __launch_bounds__(TPU > 256 ? TPU : 256) void norm_residual_kernel(Re
     }
 }
 
-// threads a unit and pieces a thread for a unit of n pieces: a wave while its lanes hold the unit in 4 pieces, then 4, then 16 waves
+// How `units` units of n pieces run: f(WIDE, IT, threads a block, blocks). A wave a unit of up to 2 pieces a lane, in
+// blocks of 4; longer ones a block of as many waves as leave a thread 1 or 2 pieces - 1 while there are too few units to
+// fill the chip, 2 (half the sums' barriers) where there are many
 template <typename F>
-void by_size(int64_t n, F f) {
-    using std::integral_constant;
-    auto it = [&](auto tpu) {
-        constexpr int TPU = decltype(tpu)::value;
-        if (n <= TPU) f(tpu, integral_constant<int, 1>());
-        else if (n <= 2 * TPU) f(tpu, integral_constant<int, 2>());
-        else f(tpu, integral_constant<int, 4>());
-    };
-    if (n <= 256) it(integral_constant<int, 64>());
-    else if (n <= 1024) it(integral_constant<int, 256>());
-    else if (n <= 4096) it(integral_constant<int, 1024>());
-    else f(integral_constant<int, 1024>(), integral_constant<int, 0>());
+void by_size(int64_t n, int64_t units, F f) {
+    using std::false_type, std::true_type, std::integral_constant;
+    if (n <= 64) return f(false_type(), integral_constant<int, 1>(), 256, (units + 3) / 4);
+    if (n <= 128) return f(false_type(), integral_constant<int, 2>(), 256, (units + 3) / 4);
+    if (n <= 1024 && units < 512) return f(true_type(), integral_constant<int, 1>(), (int) ((n + 63) / 64 * 64), units);
+    if (n <= 2048) return f(true_type(), integral_constant<int, 2>(), (int) ((n + 127) / 128 * 64), units);
+    if (n <= 4096) return f(true_type(), integral_constant<int, 4>(), 1024, units);
+    return f(true_type(), integral_constant<int, 0>(), 1024, units);
 }
 
 template <int QT, int VEC>
 int launch_gated(ns_gpu* g, const GatedParams& p) {
     int rc = 0;
-    by_size((p.W + VEC - 1) / VEC, [&](auto tpu, auto it) {
-        constexpr int TPU = decltype(tpu)::value, UNITS = TPU > 256 ? 1 : 256 / TPU;
-        if ((p.units + UNITS - 1) / UNITS > INT32_MAX) rc = ns_fail("ns_norm_gated: too many rows");
-        else norm_gated_kernel<QT, VEC, TPU, decltype(it)::value><<<(unsigned) ((p.units + UNITS - 1) / UNITS), TPU > 256 ? TPU : 256, 0, g->q>>>(p);
+    by_size((p.W + VEC - 1) / VEC, p.units, [&](auto wide, auto it, int threads, int64_t blocks) {
+        if (blocks > INT32_MAX) rc = ns_fail("ns_norm_gated: too many rows");
+        else norm_gated_kernel<QT, VEC, decltype(wide)::value, decltype(it)::value><<<(unsigned) blocks, threads, 0, g->q>>>(p);
     });
     return rc;
 }
 template <int QT, int RT, int VEC>
 int launch_residual(ns_gpu* g, const ResidualParams& p) {
     int rc = 0;
-    by_size((p.D + VEC - 1) / VEC, [&](auto tpu, auto it) {
-        constexpr int TPU = decltype(tpu)::value, UNITS = TPU > 256 ? 1 : 256 / TPU;
-        if ((p.T + UNITS - 1) / UNITS > INT32_MAX) rc = ns_fail("ns_norm_residual: too many rows");
-        else norm_residual_kernel<QT, RT, VEC, TPU, decltype(it)::value><<<(unsigned) ((p.T + UNITS - 1) / UNITS), TPU > 256 ? TPU : 256, 0, g->q>>>(p);
+    by_size((p.D + VEC - 1) / VEC, p.T, [&](auto wide, auto it, int threads, int64_t blocks) {
+        if (blocks > INT32_MAX) rc = ns_fail("ns_norm_residual: too many rows");
+        else norm_residual_kernel<QT, RT, VEC, decltype(wide)::value, decltype(it)::value><<<(unsigned) blocks, threads, 0, g->q>>>(p);
     });
     return rc;
 }
@@ -266,7 +279,7 @@ int ns_norm_gated(ns_gpu* g, int qt, const void* y, int64_t ys, const void* z, i
     NS_HIP(hipSetDevice(g->dev));
     const GatedParams p{y, z, w, out, ys, zs, os, T * groups, (int) (D / groups), (int) groups, order, eps};
     const int vec = qt ? 8 : 4;
-    const bool v = D / groups % vec == 0 && wide(y, ys, qt, vec) && wide(z, zs, qt, vec) && wide(out, os, qt, vec);
+    const bool v = D / groups % vec == 0 && (uintptr_t) w % 16 == 0 && wide(y, ys, qt, vec) && wide(z, zs, qt, vec) && wide(out, os, qt, vec);
     const int rc = qt == 0 ? (v ? launch_gated<0, 4>(g, p) : launch_gated<0, 1>(g, p))
                  : qt == 1 ? (v ? launch_gated<1, 8>(g, p) : launch_gated<1, 1>(g, p))
                            : (v ? launch_gated<2, 8>(g, p) : launch_gated<2, 1>(g, p));
@@ -289,7 +302,7 @@ int ns_norm_residual(ns_gpu* g, int qt, int rt, const void* x, int64_t xs, const
     NS_HIP(hipSetDevice(g->dev));
     const ResidualParams p{x, h, post, gate, pre, h1, out, xs, hs, h1s, os, T, (int) D, eps, scale};
     const int vec = qt ? 8 : 4;
-    const bool v = D % vec == 0 && (!x || wide(x, xs, qt, vec)) && wide(h, hs, rt, vec) && (!h1 || wide(h1, h1s, rt, vec)) && (!out || wide(out, os, qt, vec));
+    const bool v = D % vec == 0 && (uintptr_t) post % 16 == 0 && (uintptr_t) gate % 16 == 0 && (uintptr_t) pre % 16 == 0 && (!x || wide(x, xs, qt, vec)) && wide(h, hs, rt, vec) && (!h1 || wide(h1, h1s, rt, vec)) && (!out || wide(out, os, qt, vec));
     const int rc = qt == 0   ? (v ? launch_residual<0, 0, 4>(g, p) : launch_residual<0, 0, 1>(g, p))
                    : rt == 0 ? (qt == 1 ? (v ? launch_residual<1, 0, 8>(g, p) : launch_residual<1, 0, 1>(g, p))
                                         : (v ? launch_residual<2, 0, 8>(g, p) : launch_residual<2, 0, 1>(g, p)))

@@ -10,18 +10,20 @@
 // then fit as they are, float32 rows as two halfs (22 bits, two matrix instructions), half rows need neither.
 //
 // A work-group of 8 waves takes 16 outputs and shares K among its waves, tile by tile; the waves' sums meet in LDS in a
-// fixed order. Its rows lie in LDS as operands, a stretch of K at a time.
+// fixed order. Rows that fit its LDS as operands are laid out there by each work-group, while its first weights are on
+// their way; longer ones once, by a kernel in front, in the library's own scratch.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
 
 #include "ns_internal.hpp"
 #include "ns_layer.h"
+#include "attn_host.hpp"
 #include "layer_common.hpp"
 
 namespace {
 
-constexpr int WAVES = 8, PF = 4, LDS_ROWS = 64 * 1024;
+constexpr int WAVES = 8, PF = 2, LDS_ROWS = 64 * 1024;
 
 constexpr int64_t q4_tile_bytes(int64_t group) { return 1024 + 16 * (128 / group) * 2; }
 
@@ -30,8 +32,9 @@ struct Q4Params {
     const uint8_t* w;
     void* y;
     int64_t xs, ys;
-    int T, M, K, kt, chunk;      // kt: tiles along K; chunk: tiles of K that LDS holds at a time
+    int T, M, K, kt;             // kt: tiles along K
     int vec;                     // rows readable in pieces of 8 values
+    uint8_t* ops;                // the rows as operands, where LDS does not hold them
 };
 
 // 8 weights of a word as halfs, -8 .. 7 exactly: nibble i under the exponent byte is 1024 + q, one 4 bits up 1024 + 16 q
@@ -46,109 +49,134 @@ __device__ __forceinline__ s8v q4_operand(uint32_t w) {
     return __builtin_bit_cast(s8v, r);
 }
 
-// GR: groups a tile (4, 2, 1)
-template <int QT, int GR>
-__global__ __launch_bounds__(64 * WAVES) void q4_product_kernel(Q4Params p) {
-    constexpr int PLANES = QT == 0 ? 2 : 1, TILE = 1024 + 32 * GR, SW = 2 * GR;     // SW: a lane's scales, in words
+// The rows as operands: [plane][tile][16 pieces of 8][row], then a power of two a (tile, row)
+template <int QT>
+constexpr int PLANES = QT == 0 ? 2 : 1;
+template <int QT>
+__device__ __forceinline__ int64_t q4_plane(const Q4Params& p) { return (int64_t) p.kt * 16 * p.T; }
+// 16 threads (u) a (tile kl, row t): 8 values each
+template <int QT>
+__device__ __forceinline__ void q4_rows(const Q4Params& p, int kl, int t, int u, s8v* xo, float* xscale) {
+    const int k = kl * 128 + u * 8;
+    float v[8];
+    if (p.vec && k + 8 <= p.K) load_row<QT, 8>(p.x, t * p.xs + k, v);
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? load_q<QT>(p.x, t * p.xs + k + j) : 0.0f;
+    }
+    s8v hi, lo;
+    float up = 1.0f;
+    if constexpr (QT != 1) {
+        float big = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(v[j]));
+        big = row16_max(big);
+        // 2^(13 - exponent of the largest), its exponent field between 12 and 253: it has an inverse
+        const int e = min(267 - (int) (__builtin_bit_cast(uint32_t, big) >> 23), 253);
+        up = __builtin_bit_cast(float, (uint32_t) e << 23);
+        if (u == 0) xscale[kl * p.T + t] = __builtin_bit_cast(float, (uint32_t) (254 - e) << 23);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float f = v[j] * up;
+        const _Float16 half = (_Float16) f;
+        hi[j] = __builtin_bit_cast(short, half);
+        if constexpr (PLANES<QT> == 2) lo[j] = to16<false>(fabsf(f) < 65504.0f ? f - (float) half : 0.0f);
+    }
+    const int64_t at = (int64_t) (kl * 16 + u) * p.T + t;
+    xo[at] = hi;
+    if constexpr (PLANES<QT> == 2) xo[q4_plane<QT>(p) + at] = lo;
+}
+template <int QT>
+__global__ __launch_bounds__(256) void q4_rows_kernel(Q4Params p) {
+    const int task = blockIdx.x * 16 + threadIdx.x / 16;
+    if (task >= p.kt * p.T) return;
+    s8v* xo = reinterpret_cast<s8v*>(p.ops);
+    q4_rows<QT>(p, task / p.T, task % p.T, threadIdx.x % 16, xo, reinterpret_cast<float*>(xo + q4_plane<QT>(p) * PLANES<QT>));
+}
+
+// GR: groups a tile (4, 2, 1); MEM: the rows' operands lie in memory, else in LDS
+template <int QT, int GR, bool MEM>
+__global__ __launch_bounds__(64 * WAVES, MEM ? 2 : 4) void q4_product_kernel(Q4Params p) {
+    constexpr int TILE = 1024 + 32 * GR, SW = 2 * GR;             // SW: a lane's scales, in words
     extern __shared__ __align__(16) uint8_t lds[];
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = lane % 16, g = lane / 16;
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, g = lane / 16;
     const int col = n < p.T ? n : p.T - 1;             // (columns behind the rows: some row's, never written)
-    s8v* xo = reinterpret_cast<s8v*>(lds);             // [plane][tile][16 pieces of 8][row]
-    const int plane = p.chunk * 16 * p.T;
-    float* xscale = reinterpret_cast<float*>(lds + (size_t) plane * PLANES * 16);   // [tile][row]
+    const int64_t plane = q4_plane<QT>(p);
+    s8v* const xo = reinterpret_cast<s8v*>(MEM ? p.ops : lds);
+    float* const xscale = reinterpret_cast<float*>(xo + plane * PLANES<QT>);
     const uint8_t* wt = p.w + (int64_t) blockIdx.x * p.kt * TILE;
     f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c0 = 0; c0 < p.kt; c0 += p.chunk) {
-        const int here = min(p.chunk, p.kt - c0);
+    // a wave's next tiles: their nibbles, scales, and the rows' operands where those come from memory
+    constexpr int XS = MEM ? 4 : 1, XP = MEM ? PLANES<QT> : 1;
+    struct Ahead {
         uint4 nib[PF];
         uint32_t sc[PF][SW];
-        auto fetch = [&](int i, uint4& q, uint32_t (&s)[SW]) {
-            const int at = min(wave + WAVES * i, here - 1);
-            const uint8_t* tile = wt + (int64_t) (c0 + at) * TILE;
-            q = *reinterpret_cast<const uint4*>(tile + lane * 16);
+        s8v x[PF][XS][XP];
+        float down[PF];
+    } ahead[2];
+    auto fetch = [&](int i0, Ahead& f) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            const int kl = min(wave + WAVES * (i0 + i), p.kt - 1);
+            const uint8_t* tile = wt + (int64_t) kl * TILE;
+            f.nib[i] = *reinterpret_cast<const uint4*>(tile + lane * 16);
             const uint32_t* ss = reinterpret_cast<const uint32_t*>(tile + 1024 + g * 8 * GR);
 #pragma unroll
-            for (int j = 0; j < SW; ++j) s[j] = ss[j];
-        };
+            for (int j = 0; j < SW; ++j) f.sc[i][j] = ss[j];
+            if constexpr (MEM) {
+                const s8v* x = xo + ((int64_t) kl * 16 + g) * p.T + col;
 #pragma unroll
-        for (int i = 0; i < PF; ++i) fetch(i, nib[i], sc[i]);
-        // the rows' stretch as operands: 16 threads a (row, tile), 8 values each
-        if (c0) __syncthreads();
-        for (int task = tid / 16; task < here * p.T; task += 64 * WAVES / 16) {
-            const int kl = task / p.T, t = task - kl * p.T, u = tid % 16, k = (c0 + kl) * 128 + u * 8;
-            float v[8];
-            if (p.vec && k + 8 <= p.K) load_row<QT, 8>(p.x, t * p.xs + k, v);
-            else {
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? load_q<QT>(p.x, t * p.xs + k + j) : 0.0f;
-            }
-            s8v hi, lo;
-            float up = 1.0f;
-            if constexpr (QT != 1) {
-                float big = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(v[j]));
-                big = row16_max(big);
-                // 2^(13 - exponent of the largest), its exponent field between 12 and 253: it has an inverse
-                const int e = min(267 - (int) (__builtin_bit_cast(uint32_t, big) >> 23), 253);
-                up = __builtin_bit_cast(float, (uint32_t) e << 23);
-                if (u == 0) xscale[kl * p.T + t] = __builtin_bit_cast(float, (uint32_t) (254 - e) << 23);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float f = v[j] * up;
-                const _Float16 half = (_Float16) f;
-                hi[j] = __builtin_bit_cast(short, half);
-                if constexpr (PLANES == 2) lo[j] = to16<false>(fabsf(f) < 65504.0f ? f - (float) half : 0.0f);
-            }
-            xo[(kl * 16 + u) * p.T + t] = hi;
-            if constexpr (PLANES == 2) xo[plane + (kl * 16 + u) * p.T + t] = lo;
-        }
-        __syncthreads();
-        for (int i0 = 0; wave + WAVES * i0 < here; i0 += PF) {
-            uint4 nib2[PF];
-            uint32_t sc2[PF][SW];
-            const bool more = wave + WAVES * (i0 + PF) < here;
-            if (more) {
-#pragma unroll
-                for (int i = 0; i < PF; ++i) fetch(i0 + PF + i, nib2[i], sc2[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < PF; ++i) {
-                const int kl = wave + WAVES * (i0 + i);
-                if (kl >= here) break;
-                f4v tile = {0.0f, 0.0f, 0.0f, 0.0f}, s = tile;
-                const uint32_t words[4] = {nib[i].x, nib[i].y, nib[i].z, nib[i].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const s8v a = q4_operand(words[j]);
-                    const int at = (kl * 16 + 4 * j + g) * p.T + col;
-                    s = mfma16<false>(a, xo[at], s);
-                    if constexpr (PLANES == 2) s = mfma16<false>(a, xo[plane + at], s);
-                    if ((j + 1) % (4 / GR) == 0) {
-                        constexpr int PER = 4 / GR;
-                        const int grp = j / PER;
-                        const uint32_t s0 = sc[i][grp * 2], s1 = sc[i][grp * 2 + 1];
-                        tile[0] = fmaf(f16_to_f32((uint16_t) s0), s[0], tile[0]);
-                        tile[1] = fmaf(f16_to_f32((uint16_t) (s0 >> 16)), s[1], tile[1]);
-                        tile[2] = fmaf(f16_to_f32((uint16_t) s1), s[2], tile[2]);
-                        tile[3] = fmaf(f16_to_f32((uint16_t) (s1 >> 16)), s[3], tile[3]);
-                        s = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-                    }
-                }
-                const float down = QT == 1 ? 1.0f : xscale[kl * p.T + col];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e] = QT == 1 ? acc[e] + tile[e] : fmaf(down, tile[e], acc[e]);
-            }
-            if (more) {
-#pragma unroll
-                for (int i = 0; i < PF; ++i) {
-                    nib[i] = nib2[i];
-#pragma unroll
-                    for (int j = 0; j < SW; ++j) sc[i][j] = sc2[i][j];
-                }
+                    for (int h = 0; h < XP; ++h) f.x[i][j][h] = x[h * plane + 4 * j * p.T];
+                if (QT != 1) f.down[i] = xscale[kl * p.T + col];
             }
         }
+    };
+    auto compute = [&](int i0, const Ahead& f) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            const int kl = wave + WAVES * (i0 + i);
+            if (kl >= p.kt) break;
+            f4v tile = {0.0f, 0.0f, 0.0f, 0.0f}, s = tile;
+            const uint32_t words[4] = {f.nib[i].x, f.nib[i].y, f.nib[i].z, f.nib[i].w};
+            const s8v* x = xo + ((int64_t) kl * 16 + g) * p.T + col;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const s8v a = q4_operand(words[j]);
+                if constexpr (MEM) {
+#pragma unroll
+                    for (int h = 0; h < XP; ++h) s = mfma16<false>(a, f.x[i][j][h], s);
+                } else {
+                    s = mfma16<false>(a, x[4 * j * p.T], s);
+                    if constexpr (PLANES<QT> == 2) s = mfma16<false>(a, x[plane + 4 * j * p.T], s);
+                }
+                if ((j + 1) % (4 / GR) == 0) {
+                    const int grp = j / (4 / GR);
+                    const uint32_t s0 = f.sc[i][grp * 2], s1 = f.sc[i][grp * 2 + 1];
+                    tile[0] = fmaf(f16_to_f32((uint16_t) s0), s[0], tile[0]);
+                    tile[1] = fmaf(f16_to_f32((uint16_t) (s0 >> 16)), s[1], tile[1]);
+                    tile[2] = fmaf(f16_to_f32((uint16_t) s1), s[2], tile[2]);
+                    tile[3] = fmaf(f16_to_f32((uint16_t) (s1 >> 16)), s[3], tile[3]);
+                    s = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+            }
+            const float down = QT == 1 ? 1.0f : MEM ? f.down[i] : xscale[kl * p.T + col];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = QT == 1 ? acc[e] + tile[e] : fmaf(down, tile[e], acc[e]);
+        }
+    };
+    fetch(0, ahead[0]);
+    if constexpr (!MEM) {
+        for (int task = tid / 16; task < p.kt * p.T; task += 64 * WAVES / 16) q4_rows<QT>(p, task / p.T, task % p.T, tid % 16, xo, xscale);
+        lds_barrier();                   // (the weights stay in flight)
+    }
+    for (int i0 = 0; wave + WAVES * i0 < p.kt; i0 += 2 * PF) {
+        if (wave + WAVES * (i0 + PF) < p.kt) fetch(i0 + PF, ahead[1]);
+        compute(i0, ahead[0]);
+        if (wave + WAVES * (i0 + 2 * PF) < p.kt) fetch(i0 + 2 * PF, ahead[0]);
+        compute(i0 + PF, ahead[1]);
     }
     // the waves' sums, in the waves' order
     __syncthreads();
@@ -207,19 +235,22 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(int form, const void* src,
 bool q4_group(int64_t group) { return group == 32 || group == 64 || group == 128; }
 
 template <int QT, int GR>
-void launch_product(ns_gpu* g, Q4Params& p) {
-    constexpr int PLANES = QT == 0 ? 2 : 1;
-    const int row = p.T * (256 * PLANES + 4);          // bytes of LDS a tile of K
-    const int fit = LDS_ROWS / row;
-    p.chunk = std::min(p.kt, fit < WAVES ? fit : fit / WAVES * WAVES);
-    const size_t lds = std::max<size_t>((size_t) p.chunk * row, WAVES * 64 * sizeof(f4v));
-    q4_product_kernel<QT, GR><<<(unsigned) ((p.M + 15) / 16), 64 * WAVES, lds, g->q>>>(p);
+int launch_product(ns_gpu* g, Q4Params& p) {
+    const int64_t rows = (int64_t) p.kt * p.T * (256 * PLANES<QT> + 4), sums = WAVES * 64 * sizeof(f4v);
+    const unsigned grid = (unsigned) ((p.M + 15) / 16);
+    if (rows <= LDS_ROWS) {
+        q4_product_kernel<QT, GR, false><<<grid, 64 * WAVES, std::max(rows, sums), g->q>>>(p);
+        return 0;
+    }
+    if ((size_t) (rows + 3) / 4 > ns_own_floats(g)) return ns_fail("ns_q4_product: more scratch than the library has");
+    p.ops = reinterpret_cast<uint8_t*>(g->own_scratch);
+    q4_rows_kernel<QT><<<(unsigned) ((p.kt * p.T + 15) / 16), 256, 0, g->q>>>(p);
+    q4_product_kernel<QT, GR, true><<<grid, 64 * WAVES, sums, g->q>>>(p);
+    return 0;
 }
 template <int QT>
-void launch_product(ns_gpu* g, Q4Params& p, int64_t group) {
-    if (group == 32) launch_product<QT, 4>(g, p);
-    else if (group == 64) launch_product<QT, 2>(g, p);
-    else launch_product<QT, 1>(g, p);
+int launch_product(ns_gpu* g, Q4Params& p, int64_t group) {
+    return group == 32 ? launch_product<QT, 4>(g, p) : group == 64 ? launch_product<QT, 2>(g, p) : launch_product<QT, 1>(g, p);
 }
 
 }  // namespace
@@ -256,16 +287,15 @@ int ns_q4_product(ns_gpu* g, int qt, const void* x, int64_t xs, const void* w, i
     if (qt < 0 || qt > 2) return ns_fail("ns_q4_product: rows of type 0 (float32), 1 (half) or 2 (bfloat16)");
     if (T > 16) return ns_fail("ns_q4_product: 1 to 16 rows");
     if (!q4_group(group)) return ns_fail("ns_q4_product: groups of 32, 64 or 128");
-    if (K <= 0 || M > (int64_t) 1 << 30 || K > (int64_t) 1 << 30) return ns_fail("ns_q4_product: 1 to 2^30 outputs and inputs");
+    if (K <= 0 || M > (int64_t) 1 << 30 || K > (int64_t) 1 << 22) return ns_fail("ns_q4_product: up to 2^30 outputs, 1 to 2^22 inputs");
     if (xs < K || ys < M) return ns_fail("ns_q4_product: rows at least as far apart as they are long");
     if ((uintptr_t) w % 16) return ns_fail("ns_q4_product: weights 16-byte aligned");
     if (!g || !x || !w || !y) return ns_fail("ns_q4_product: a null buffer");
     NS_HIP(hipSetDevice(g->dev));
     const int64_t e = qt ? 2 : 4;
-    Q4Params p{x, static_cast<const uint8_t*>(w), y, xs, ys, (int) T, (int) M, (int) K, (int) ((K + 127) / 128), 0, (uintptr_t) x % 16 == 0 && xs * e % 16 == 0};
-    if (qt == 0) launch_product<0>(g, p, group);
-    else if (qt == 1) launch_product<1>(g, p, group);
-    else launch_product<2>(g, p, group);
+    Q4Params p{x, static_cast<const uint8_t*>(w), y, xs, ys, (int) T, (int) M, (int) K, (int) ((K + 127) / 128), (uintptr_t) x % 16 == 0 && xs * e % 16 == 0};
+    const int rc = qt == 0 ? launch_product<0>(g, p, group) : qt == 1 ? launch_product<1>(g, p, group) : launch_product<2>(g, p, group);
+    if (rc) return rc;
     NS_LAUNCHED("q4_product");
     return 0;
     NS_CATCH

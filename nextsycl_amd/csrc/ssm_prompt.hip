@@ -76,10 +76,6 @@ __device__ __forceinline__ float ring_row(const SsmLayer& p, int64_t at, int ch)
     return at >= 1 - p.K && p.p0 + at >= 0 ? p.conv[(p.p0 + at) % p.cap * p.chan + ch] : 0.0f;
 }
 
-// A work-group's barrier for what its waves exchange through LDS: memory loads for the next chunk and rows on their way out
-// stay in flight across it (a __syncthreads waits for both)
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
 // a row's value as it lies in memory, and as a number
 template <int QT>
 __device__ __forceinline__ uint32_t raw_bits(const char* p, uint32_t off) {
@@ -91,6 +87,31 @@ __device__ __forceinline__ float raw_value(uint32_t b) {
     return QT == 0 ? __builtin_bit_cast(float, b) : QT == 1 ? f16_to_f32((uint16_t) b) : bf16_to_f32((uint16_t) b);
 }
 
+// a head's step sizes and exponents in a chunk, a lane a row
+template <int QT>
+__device__ __forceinline__ void ssm_header(const ScanParams& s, int chunk, int head, int lane) {
+    const SsmLayer& p = s.l;
+    const int t = chunk * L + lane;
+    const float dt = t < s.T ? ssm_dt(p, load_q<QT>(p.dt, (s.t0 + t) * p.dts + head) + (p.dtb ? p.dtb[head] : 0.0f)) : 0.0f;
+    const double add = (double) dt * (double) p.a[head] * 1.4426950408889634074;
+    double cum = add;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double b = __shfl_up(cum, o);
+        if (lane >= o) cum += b;
+    }
+    const double end = __shfl(cum, 63), base = __shfl(cum - add, lane / 16 * 16);
+    float* to = s.hdr + ((int64_t) chunk * p.H + head) * HDR;
+    to[HDR_C + lane] = (float) (cum - base);
+    to[HDR_DT + lane] = dt;
+    to[HDR_W + lane] = exp2f((float) (end - cum)) * dt;
+    to[HDR_E + lane] = exp2f((float) cum);
+    // starts of run lane / 4 and lane % 4 of 16
+    const double from = __shfl(cum - add, lane % 16 / 4 * 16), of = __shfl(cum - add, lane % 4 * 16);
+    if (lane < 16) to[HDR_BD + lane] = (float) (from - of);
+    if (lane < 2) to[HDR_END + lane] = lane ? exp2f((float) end) : (float) end;
+}
+
 template <int QT, int KW>
 __global__ __launch_bounds__(256, 3 - KW) void ssm_prep_kernel(ScanParams s) {
     constexpr int NP = 128 * KW, KK = 4 * KW, ROW = NP + 8;
@@ -98,6 +119,12 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_prep_kernel(ScanParams s) {
     __shared__ float part[2][4];
     const SsmLayer& p = s.l;
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n16 = lane % 16, g = lane / 16;
+    if ((int) blockIdx.x >= s.chunks * p.G) {
+        // work-groups behind those: headers, a wave a (chunk, head)
+        const int64_t i = (int64_t) (blockIdx.x - s.chunks * p.G) * 4 + wave;
+        if (i < (int64_t) s.chunks * p.H) ssm_header<QT>(s, (int) (i / p.H), (int) (i % p.H), lane);
+        return;
+    }
     const int chunk = blockIdx.x / p.G, group = blockIdx.x % p.G, per = p.H / p.G;
     const int here = min(L, s.T - chunk * L);
     const int64_t first = s.t0 + (int64_t) chunk * L;
@@ -194,28 +221,6 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_prep_kernel(ScanParams s) {
             acc = mfma16<false>(bh, cl, acc);
         }
         reinterpret_cast<f4v*>(ops + 4 * op_c(KK))[((wave * 2 + st / 2) * 64 + lane) * 2 + st % 2] = acc * down;
-    }
-    // the heads' step sizes and exponents, a lane a row
-    for (int hh = wave; hh < per; hh += 4) {
-        const int head = group * per + hh;
-        const float dt = lane < here ? ssm_dt<QT>(p, first + lane, head) : 0.0f;
-        const double add = (double) dt * (double) p.a[head] * 1.4426950408889634074;
-        double cum = add;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double b = __shfl_up(cum, o);
-            if (lane >= o) cum += b;
-        }
-        const double end = __shfl(cum, 63), base = __shfl(cum - add, lane / 16 * 16);
-        float* to = s.hdr + ((int64_t) chunk * p.H + head) * HDR;
-        to[HDR_C + lane] = (float) (cum - base);
-        to[HDR_DT + lane] = dt;
-        to[HDR_W + lane] = exp2f((float) (end - cum)) * dt;
-        to[HDR_E + lane] = exp2f((float) cum);
-        // starts of run lane / 4 and lane % 4 of 16
-        const double from = __shfl(cum - add, lane % 16 / 4 * 16), of = __shfl(cum - add, lane % 4 * 16);
-        if (lane < 16) to[HDR_BD + lane] = (float) (from - of);
-        if (lane < 2) to[HDR_END + lane] = lane ? exp2f((float) end) : (float) end;
     }
 }
 
@@ -651,7 +656,7 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G) {
 
 template <int QT, int KW>
 void launch_pass(ns_gpu* g, ScanParams& s, const Plan& q) {
-    ssm_prep_kernel<QT, KW><<<(unsigned) (q.chunks * s.l.G), 256, 0, g->q>>>(s);
+    ssm_prep_kernel<QT, KW><<<(unsigned) (q.chunks * s.l.G + ((int64_t) q.chunks * s.l.H + 3) / 4), 256, 0, g->q>>>(s);
     const unsigned owners = (unsigned) (s.l.H * q.blocks);
     if (q.segs > 1) {
         ScanParams f = s;

@@ -29,16 +29,44 @@ struct StepParams {
 // LR lanes a state row, U rows a lane; VEC: a lane's 4 floats as one piece
 template <int QT, int LR, int U, bool VEC>
 __global__ __launch_bounds__(256) void ssm_step_kernel(StepParams s) {
-    constexpr int RW = 256 / LR, PB = RW * U, NMAX = 4 * LR, CH = (2 * NMAX + PB + 255) / 256;
-    __shared__ float ub[NMAX], uc[NMAX], ux[PB];
+    constexpr int RW = 256 / LR, PB = RW * U, AHEAD = 4, NMAX = 4 * LR, CH = (2 * NMAX + PB + 255) / 256;
+    __shared__ __align__(16) float row_in[AHEAD][2 * NMAX + PB];      // B, C, the block's x of a row
+    __shared__ float step[AHEAD][2];                                  // its step size and decay
     __shared__ uint64_t mine[MOST_ROWS / 64];
+    __shared__ uint16_t list[MOST_ROWS];
     const SsmLayer& p = s.l;
     const int tid = threadIdx.x, lane = tid % 64, head = blockIdx.x / s.pblocks, pb = blockIdx.x % s.pblocks, r0 = blockIdx.y;
     const int group = head / (p.H / p.G), n0 = tid % LR * 4, prow = pb * PB + tid / LR;
     const int64_t slot = s.slots ? s.slots[r0] : r0;
     const int64_t first = s.pos ? (int64_t) s.pos[r0] : p.p0;
     if (slot < 0 || slot >= s.nslots || first < 0) return;
-    // the state, asked for first
+    // the slot's rows in their order, as many as its ring has room for: this work-group is the first's, or has nothing to do
+    const int cap = (int) p.cap;
+    int count = 1;
+    if (s.slots) {
+        for (int w = tid / 64; w * 64 < s.R; w += 4) {
+            const int at = w * 64 + lane;
+            const uint64_t m = __ballot(at < s.R && s.slots[at < s.R ? at : 0] == (int32_t) slot);
+            if (lane == 0) mine[w] = m;
+        }
+        __syncthreads();
+        for (int w = 0; w <= r0 / 64; ++w) {
+            const uint64_t m = w == r0 / 64 ? mine[w] & (((uint64_t) 1 << r0 % 64) - 1) : mine[w];
+            if (m) return;
+        }
+        const int most = p.K > 1 ? cap - p.K + 1 : s.R;
+        count = 0;
+        for (int w = r0 / 64; w * 64 < s.R; ++w) {
+            const uint64_t m = mine[w];
+            const int rank = count + __builtin_popcountll(m & (((uint64_t) 1 << lane) - 1));
+            if (tid < 64 && (m >> lane & 1) && rank < most) list[rank] = (uint16_t) (w * 64 + lane);
+            count += __builtin_popcountll(m);
+        }
+        count = min(count, most);
+        if (count > 1) __syncthreads();
+    }
+    auto row_of = [&](int i) { return count > 1 ? (int64_t) list[i] : (int64_t) r0; };
+    // the state, on its way while the convolution runs
     float h[U][4];
     const int64_t hrow = (slot * p.H + head) * p.P;
 #pragma unroll
@@ -59,39 +87,27 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(StepParams s) {
                 if (n0 + i < p.N) h[u][i] = src[i];
         }
     }
-    // the slot's rows: this work-group is the first's, or has nothing to do
-    if (s.slots) {
-        for (int w = tid / 64; w * 64 < s.R; w += 4) {
-            const int at = w * 64 + lane;
-            const uint64_t m = __ballot(at < s.R && s.slots[at < s.R ? at : 0] == (int32_t) slot);
-            if (lane == 0) mine[w] = m;
-        }
-        __syncthreads();
-        for (int w = 0; w <= r0 / 64; ++w) {
-            const uint64_t m = w == r0 / 64 ? mine[w] & (((uint64_t) 1 << r0 % 64) - 1) : mine[w];
-            if (m) return;
-        }
-    }
     // this thread's channels: B, C, then the block's part of x; their taps and the raw values in front of the first row
     int ch[CH];
     float w4[CH][4], bias[CH], past[CH][3];
-    float* to[CH];
+    int to[CH];
     bool keep[CH];
-    const int64_t ringb = slot * p.cap;
+    // the ring's slot of the first row (one division, of 32 bits where they do), those behind it one further each
+    const int slot0 = (uint64_t) first >> 32 ? (int) (first % p.cap) : (int) ((uint32_t) first % (uint32_t) cap);
+    float* ring = p.conv + slot * p.cap * p.chan;
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
         const int c = tid + 256 * j;
-        ch[j] = -1, to[j] = nullptr, keep[j] = false;
+        ch[j] = -1, to[j] = c < 2 * NMAX + PB ? c : -1, keep[j] = false;
         if (c < NMAX) {
             if (c < p.N) ch[j] = p.H * p.P + group * p.N + c;
-            to[j] = ub + c, keep[j] = true;
+            keep[j] = true;
         } else if (c < 2 * NMAX) {
             if (c - NMAX < p.N) ch[j] = p.H * p.P + (p.G + group) * p.N + c - NMAX;
-            to[j] = uc + (c - NMAX), keep[j] = true;
+            keep[j] = true;
         } else if (c < 2 * NMAX + PB) {
             const int pr = pb * PB + c - 2 * NMAX;
             if (pr < p.P) ch[j] = head * p.P + pr;
-            to[j] = ux + (c - 2 * NMAX);
         }
         // a group's B and C are kept by its first head's first block, x by its own
         keep[j] = ch[j] >= 0 && p.K > 1 && (!keep[j] || (head % (p.H / p.G) == 0 && pb == 0));
@@ -100,46 +116,66 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(StepParams s) {
         bias[j] = ch[j] >= 0 && p.cb ? p.cb[ch[j]] : 0.0f;
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-            const int64_t at = first - 3 + k;
-            past[j][k] = ch[j] >= 0 && k >= 4 - p.K && at >= 0 ? p.conv[(ringb + at % p.cap) * p.chan + ch[j]] : 0.0f;
+            const int at = slot0 - 3 + k;
+            past[j][k] = ch[j] >= 0 && k >= 4 - p.K && first - 3 + k >= 0 ? ring[(int64_t) (at < 0 ? at + cap : at) * p.chan + ch[j]] : 0.0f;
         }
     }
-    const float rate = p.a[head], skip = p.d ? p.d[head] : 0.0f;
-    int64_t most = p.K > 1 ? p.cap - p.K + 1 : s.R;
-    int row = r0;
-    for (int64_t i = 0;;) {
-        if (i) __syncthreads();          // the row before has been read
+    const float rate = p.a[head], skip = p.d ? p.d[head] : 0.0f, dtb = p.dtb ? p.dtb[head] : 0.0f;
+    int here = slot0;
+    for (int i0 = 0; i0 < count; i0 += AHEAD) {
+        // four rows at a time: their convolutions and step sizes, in LDS, then the state through them
+        const int rows = min(AHEAD, count - i0);
+        float raw[AHEAD][CH], size = 0.0f;
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            if (!to[j]) continue;
-            float c = 0.0f;
-            if (ch[j] >= 0) {
-                const float v = load_q<QT>(p.xbc, row * p.xs + ch[j]);
-                c = silu(fmaf(w4[j][3], v, fmaf(w4[j][2], past[j][2], fmaf(w4[j][1], past[j][1], fmaf(w4[j][0], past[j][0], bias[j])))));
+        for (int a = 0; a < AHEAD; ++a) {
+            if (a >= rows) break;
+            const int64_t r = row_of(i0 + a);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) raw[a][j] = ch[j] >= 0 ? load_q<QT>(p.xbc, r * p.xs + ch[j]) : 0.0f;
+        }
+        // (a lane a row, of the wave that has no channels of x)
+        const bool sizes = tid >= 192 && lane < rows;
+        if (sizes) size = load_q<QT>(p.dt, row_of(i0 + lane) * p.dts + head);
+        if (i0) lds_barrier();           // the rows before have been read
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (a >= rows) break;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                if (to[j] < 0) continue;
+                const float v = raw[a][j];
+                row_in[a][to[j]] = ch[j] >= 0 ? silu(fmaf(w4[j][3], v, fmaf(w4[j][2], past[j][2], fmaf(w4[j][1], past[j][1], fmaf(w4[j][0], past[j][0], bias[j]))))) : 0.0f;
                 past[j][0] = past[j][1], past[j][1] = past[j][2], past[j][2] = v;
-                if (keep[j]) p.conv[(ringb + (first + i) % p.cap) * p.chan + ch[j]] = v;
+                if (keep[j]) ring[(int64_t) here * p.chan + ch[j]] = v;
             }
-            *to[j] = c;
+            here = here + 1 == cap ? 0 : here + 1;
         }
-        const float dt = ssm_dt<QT>(p, row, head), decay = expf(dt * rate);
-        __syncthreads();
-        const float4 b = *reinterpret_cast<const float4*>(ub + n0), c = *reinterpret_cast<const float4*>(uc + n0);
+        if (sizes) {
+            const float dt = ssm_dt(p, size + dtb);
+            step[lane][0] = dt, step[lane][1] = expf(dt * rate);
+        }
+        lds_barrier();
+        for (int a = 0; a < rows; ++a) {
+            const float dt = step[a][0], decay = step[a][1];
+            const float4 b = *reinterpret_cast<const float4*>(row_in[a] + n0), c = *reinterpret_cast<const float4*>(row_in[a] + NMAX + n0);
+            // (the sums of a lane's U state rows side by side; lane u of a row's lanes then writes the one of row u)
+            float sum[U], x[U], out = 0.0f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float x = ux[tid / LR + u * RW], dx = dt * x;
-            h[u][0] = fmaf(h[u][0], decay, dx * b.x), h[u][1] = fmaf(h[u][1], decay, dx * b.y);
-            h[u][2] = fmaf(h[u][2], decay, dx * b.z), h[u][3] = fmaf(h[u][3], decay, dx * b.w);
-            const float sum = lanes_sum<LR>(fmaf(h[u][0], c.x, h[u][1] * c.y) + fmaf(h[u][2], c.z, h[u][3] * c.w));
-            const int pr = prow + u * RW;
-            if (tid % LR == 0 && pr < p.P) store_o<QT>(p.y, row * p.ys + head * p.P + pr, fmaf(skip, x, sum));
+            for (int u = 0; u < U; ++u) {
+                x[u] = row_in[a][2 * NMAX + tid / LR + u * RW];
+                const float dx = dt * x[u];
+                h[u][0] = fmaf(h[u][0], decay, dx * b.x), h[u][1] = fmaf(h[u][1], decay, dx * b.y);
+                h[u][2] = fmaf(h[u][2], decay, dx * b.z), h[u][3] = fmaf(h[u][3], decay, dx * b.w);
+                sum[u] = fmaf(h[u][0], c.x, h[u][1] * c.y) + fmaf(h[u][2], c.z, h[u][3] * c.w);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                sum[u] = fmaf(skip, x[u], lanes_sum<LR>(sum[u]));
+                out = tid % LR == u ? sum[u] : out;
+            }
+            const int mine_p = prow + tid % LR * RW;
+            if (tid % LR < U && mine_p < p.P) store_o<QT>(p.y, row_of(i0 + a) * p.ys + head * p.P + mine_p, out);
         }
-        // the slot's next row
-        if (!s.slots || ++i >= most) break;
-        int w = (row + 1) / 64, words = (s.R + 63) / 64;
-        uint64_t m = w < words ? mine[w] & ~(((uint64_t) 1 << (row + 1) % 64) - 1) : 0;
-        while (!m && ++w < words) m = mine[w];
-        if (!m) break;
-        row = w * 64 + __builtin_ctzll(m);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -169,7 +205,7 @@ void launch_step(ns_gpu* g, StepParams& s, bool vec) {
     if (N <= 16) launch_step<QT, 4, 1>(g, s, vec);
     else if (N <= 32) launch_step<QT, 8, 2>(g, s, vec);
     else if (N <= 64) launch_step<QT, 16, 4>(g, s, vec);
-    else if (N <= 128) launch_step<QT, 32, 4>(g, s, vec);
+    else if (N <= 128) launch_step<QT, 32, 8>(g, s, vec);
     else launch_step<QT, 64, 4>(g, s, vec);
 }
 
@@ -202,6 +238,8 @@ extern "C" int ns_ssm_step(ns_gpu* g, int qt, const void* xbc, int64_t xs, const
     if (R > MOST_ROWS) return ns_fail("ns_ssm_step: up to 4096 rows");
     if (nslots <= 0 || (!slots && R > nslots) || nslots > INT32_MAX) return ns_fail("ns_ssm_step: more rows than slots");
     if (ns_ssm_check("ns_ssm_step", g, qt, s.l, H, P, N, G, K, K)) return -1;
+    if (cap > INT32_MAX) return ns_fail("ns_ssm_step: a ring of up to 2^31 - 1 rows");
+    if (K == 1) s.l.conv = nullptr, s.l.cap = 1;      // (nothing is kept)
     s.l.chan = (int) (H * P + 2 * G * N);
     s.pos = pos, s.slots = slots, s.nslots = nslots, s.R = (int) R;
     NS_HIP(hipSetDevice(g->dev));
