@@ -206,6 +206,8 @@ class Ops:
         # what the native step calls, and the entries those addresses are of: one replaced on k is called the general way
         self._of = [getattr(self.k, name, None) for name in ("attn_decode_scratch", "attn_decode_t", "attn_prompt_t", "attn_pre_store")]
         self._at = _addresses(self._of) if _ops_fast else None
+        self._layer_of = [getattr(self.k, name, None) for name in ("norm_gated", "norm_residual", "q4_bytes", "q4_product", "ssm_step")]
+        self._layer_at = _addresses(self._layer_of) if hasattr(_ops_fast, "ssm_step") else None
 
     def raw(self):
         return self.gpu.raw
@@ -655,6 +657,11 @@ class Ops:
                  dt_hi=float("inf")):
         """ns_ssm_step: a token, or a few successive ones, of each of several sequences: R rows, row r of slot slots[r] (None: r)
         at position pos[r] (None: p0); rings [nslots][cap][chan], states [nslots][H][P][N]."""
+        if self._layer_at and self.k.ssm_step is self._layer_of[4]:
+            r = _ops_fast.ssm_step(self._layer_at[4], getattr(self.gpu, "handle", None), qt, xbc, xs, dt, dts, cw, cb, a, dtb, d, conv, cap, p0, R, H, P, N, G, K, h0,
+                                   h1, y, ys, nslots, slots, pos, dt_lo, dt_hi)
+            if r is not False:                              # (False: nothing was called)
+                return None if r is True else self.ok(r, "ssm_step")
         chan = self._ssm_need("ssm_step", qt, xbc, xs, dt, dts, cw, cb, a, dtb, d, R, H, P, N, G, K, y, ys)
         if K > 1:
             _need(conv, nslots * cap * chan * 4, "ssm_step rings")
@@ -670,6 +677,10 @@ class Ops:
 
     def norm_gated(self, qt, y, ys, z, zs, w, out, os, T, D, groups, eps, order=0):
         """ns_norm_gated: out = rms(y silu(z)) w over each of `groups` parts of a row (order 1: rms(y) w silu(z))."""
+        if self._layer_at and self.k.norm_gated is self._layer_of[0]:
+            r = _ops_fast.norm_gated(self._layer_at[0], getattr(self.gpu, "handle", None), qt, y, ys, z, zs, w, out, os, T, D, groups, eps, order)
+            if r is not False:
+                return None if r is True else self.ok(r, "norm_gated")
         if T > 0:
             e = _elt(qt, "norm_gated")
             _need(y, ((T - 1) * ys + D) * e, "norm_gated y")
@@ -681,6 +692,10 @@ class Ops:
 
     def norm_residual(self, qt, rt, x, xs, h, hs, h1, h1s, out, os, T, D, eps, scale=1.0, post=None, gate=None, pre=None):
         """ns_norm_residual: h1 = s = h + scale gate (x, or rms(x) post), out = rms(s) pre; x None: s = h; h1 or out None: not wanted."""
+        if self._layer_at and self.k.norm_residual is self._layer_of[1]:
+            r = _ops_fast.norm_residual(self._layer_at[1], getattr(self.gpu, "handle", None), qt, rt, x, xs, h, hs, h1, h1s, out, os, T, D, eps, scale, post, gate, pre)
+            if r is not False:
+                return None if r is True else self.ok(r, "norm_residual")
         if T > 0:
             for b, stride, t, name in ((x, xs, qt, "x"), (h, hs, rt, "stream"), (h1, h1s, rt, "stream out"), (out, os, qt, "out")):
                 if b is not None:
@@ -705,6 +720,10 @@ class Ops:
 
     def q4_product(self, qt, x, xs, w, group, y, ys, T, M, K):
         """ns_q4_product: y [T][M] = x [T][K] . w^T, 1 to 16 rows, w M x K 4-bit weights in the library's tiles."""
+        if self._layer_at and self.k.q4_product is self._layer_of[3] and self.k.q4_bytes is self._layer_of[2]:
+            r = _ops_fast.q4_product(self._layer_at[2], self._layer_at[3], getattr(self.gpu, "handle", None), qt, x, xs, w, group, y, ys, T, M, K)
+            if r is not False:
+                return None if r is True else self.ok(r, "q4_product")
         if T > 0 and M > 0:
             e = _elt(qt, "q4_product")
             _need(x, ((T - 1) * xs + K) * e, "q4_product x")

@@ -23,7 +23,7 @@
 
 namespace {
 
-constexpr int WAVES = 8, PF = 2, LDS_ROWS = 64 * 1024;
+constexpr int WAVES = 8, PF = 1, LDS_ROWS = 64 * 1024;
 
 constexpr int64_t q4_tile_bytes(int64_t group) { return 1024 + 16 * (128 / group) * 2; }
 

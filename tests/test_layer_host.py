@@ -94,3 +94,94 @@ def test_the_layout_of_4_bit_weights_is_a_permutation():
     w[0, 0, 16 * (3 + 16 * 1) + 4 * 2 + 2 + 0] = 0xF0             # row 3, value 64 + 8 + 3: byte 2, the high nibble
     _, q, _ = q4_weights(w, 16, 128, 128)
     assert q[3, 64 + 8 + 3] == 15 and q.sum() == 15
+
+
+# ---- the wrappers' native step (csrc/ops_fast.c): the call the general way makes, or none
+
+class Buf:
+    def __init__(self, ptr, n):
+        self.ptr, self.len = ptr, n
+
+
+def recorded(rc=0):
+    """An Ops over entry points that note their arguments, and the notes."""
+    import types
+
+    from nextsycl_amd.attn import Ops
+    notes, keep = [], []
+
+    def entry(name):
+        res, args = LAYER_H[name]
+
+        def f(*a):
+            if name == "ns_q4_bytes":
+                return 5000
+            notes.append((name, a))
+            return rc
+        keep.append(C.CFUNCTYPE(res, *args)(f))
+        return keep[-1]
+
+    k = types.SimpleNamespace(keep=keep, api=types.SimpleNamespace(error=lambda: "refused"), **{n[3:]: entry(n) for n in LAYER_H})
+    return Ops(types.SimpleNamespace(raw=C.c_void_p(4096), handle=4096), k), notes
+
+
+def layer_calls(qt):
+    """name -> (arguments by name, the buffers' least sizes, the buffers that may be None)."""
+    e, T, D, H, P, N, G, K, cap, slots = {0: 4, 1: 2, 2: 2}[qt], 3, 48, 4, 8, 6, 2, 4, 7, 5
+    chan = H * P + 2 * G * N
+    rows = lambda stride, last, e=e: ((T - 1) * stride + last) * e  # noqa: E731
+    return {
+        "norm_gated": (dict(qt=qt, ys=50, zs=52, os=49, T=T, D=D, groups=2, eps=1e-5, order=1), dict(y=rows(50, D), z=rows(52, D), out=rows(49, D), w=4 * D), ["w"]),
+        "norm_residual": (dict(qt=qt, rt=0, xs=50, hs=52, h1s=49, os=51, T=T, D=D, eps=1e-5, scale=0.5),
+                          dict(x=rows(50, D), h=rows(52, D, 4), h1=rows(49, D, 4), out=rows(51, D), post=4 * D, gate=4 * D, pre=4 * D), ["x", "h1", "out", "post", "gate", "pre"]),
+        "q4_product": (dict(qt=qt, xs=70, group=64, ys=40, T=T, M=33, K=65), dict(x=rows(70, 65), w=5000, y=rows(40, 33)), []),
+        "ssm_step": (dict(qt=qt, xs=chan + 9, dts=chan + 9, cap=cap, p0=11, R=T, H=H, P=P, N=N, G=G, K=K, ys=H * P + 2, nslots=slots, dt_lo=0.01, dt_hi=float("inf")),
+                     dict(xbc=rows(chan + 9, chan), dt=rows(chan + 9, H), cw=chan * K * 4, cb=chan * 4, a=H * 4, dtb=H * 4, d=H * 4, conv=slots * cap * chan * 4,
+                          h0=slots * H * P * N * 4, h1=slots * H * P * N * 4, y=rows(H * P + 2, H * P), slots=T * 4, pos=T * 4), ["cb", "dtb", "d", "h0", "slots", "pos"]),
+    }
+
+
+@pytest.mark.parametrize("name", ["norm_gated", "norm_residual", "q4_product", "ssm_step"])
+@pytest.mark.parametrize("qt", [0, 1, 2])
+def test_the_native_step_makes_the_general_ways_call(name, qt):
+    from nextsycl_amd import Error
+    fast = pytest.importorskip("nextsycl_amd._ops_fast")
+    args, need, optional = layer_calls(qt)[name]
+    bufs = {b: Buf(1 << 20 | i << 12, n) for i, (b, n) in enumerate(need.items())}
+    for without in [None] + optional:
+        given = dict(bufs, **({without: None} if without else {}))
+        got, took = [], []
+        for general in (False, True):
+            ops, notes = recorded()
+            native = getattr(fast, name)
+            if general:
+                ops._layer_at = None
+            else:
+                assert ops._layer_at
+            getattr(ops, name)(**args, **given)
+            took.append(native)
+            assert len(notes) == 1
+            got.append(notes[0])
+        assert got[0] == got[1], without
+    for b in need:
+        short, words = dict(bufs), []
+        short[b] = Buf(bufs[b].ptr, need[b] - 1)
+        for general in (False, True):
+            ops, notes = recorded()
+            if general:
+                ops._layer_at = None
+            with pytest.raises(Error) as err:
+                getattr(ops, name)(**args, **short)
+            words.append(str(err.value))
+            assert not notes
+        assert words[0] == words[1]
+    # a failure is raised once, behind one call; an entry replaced on the kernels is the one that is called
+    ops, notes = recorded(rc=-1)
+    with pytest.raises(Error, match="refused"):
+        getattr(ops, name)(**args, **bufs)
+    assert len(notes) == 1
+    ops, notes = recorded()
+    other = []
+    setattr(ops.k, name, lambda *a: other.append(a) or 0)
+    getattr(ops, name)(**args, **bufs)
+    assert len(other) == 1 and not notes
