@@ -33,7 +33,8 @@ constexpr int L = 64;                     // rows a chunk
 constexpr int64_t PASS_ROWS = 8192;       // rows a pass works on: what bounds the scratch
 constexpr int MOST_SEGS = 8;
 // a chunk and head's header: exponents (base 2) from the start of each run of 16 rows, step sizes, weights in the chunk's
-// state, decays from the chunk's start; differences between runs' starts [4][4], the whole chunk's exponent and decay
+// state, decays from the chunk's start; differences between runs' starts [4][4], the whole chunk's exponent and decay, what the weights are
+// to be multiplied with
 constexpr int HDR_C = 0, HDR_DT = 64, HDR_W = 128, HDR_E = 192, HDR_BD = 256, HDR_END = 272, HDR = 288;
 
 // bytes of a chunk and group's operands: C (hi, lo), B (hi, lo) of KK = padded N / 32 steps, C . B as float32
@@ -61,12 +62,12 @@ __device__ __forceinline__ void to_half_range(float big, float& up, float& down)
     down = __builtin_bit_cast(float, (uint32_t) (254 - e) << 23);
 }
 // 8 floats as two operands: halfs and the halfs of what they leave
-__device__ __forceinline__ void split8(const float (&v)[8], float up, s8v& hi, s8v& lo) {
+__device__ __forceinline__ void split8(const float (&v)[8], s8v& hi, s8v& lo) {
     h8v a, b;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = (_Float16) (v[j] * up);
+    for (int j = 0; j < 8; ++j) a[j] = (_Float16) v[j];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = (_Float16) (fmaf(v[j], up, -(float) a[j]));
+    for (int j = 0; j < 8; ++j) b[j] = (_Float16) (v[j] - (float) a[j]);
     hi = __builtin_bit_cast(s8v, a);
     lo = __builtin_bit_cast(s8v, b);
 }
@@ -104,12 +105,15 @@ __device__ __forceinline__ void ssm_header(const ScanParams& s, int chunk, int h
     float* to = s.hdr + ((int64_t) chunk * p.H + head) * HDR;
     to[HDR_C + lane] = (float) (cum - base);
     to[HDR_DT + lane] = dt;
-    to[HDR_W + lane] = exp2f((float) (end - cum)) * dt;
+    // (the weights times a power of two that puts the largest between 1/2 and 1: they enter operands)
+    const float weight = exp2f((float) (end - cum)) * dt, most = wave_max(weight);
+    const int e = min(max((int) (__builtin_bit_cast(uint32_t, most) >> 23 & 255), 1), 252);
+    to[HDR_W + lane] = weight * __builtin_bit_cast(float, (uint32_t) (253 - e) << 23);
     to[HDR_E + lane] = exp2f((float) cum);
     // starts of run lane / 4 and lane % 4 of 16
     const double from = __shfl(cum - add, lane % 16 / 4 * 16), of = __shfl(cum - add, lane % 4 * 16);
     if (lane < 16) to[HDR_BD + lane] = (float) (from - of);
-    if (lane < 2) to[HDR_END + lane] = lane ? exp2f((float) end) : (float) end;
+    if (lane < 3) to[HDR_END + lane] = lane == 0 ? (float) end : lane == 1 ? exp2f((float) end) : __builtin_bit_cast(float, (uint32_t) (e + 1) << 23);
 }
 
 template <int QT, int KW>
@@ -180,9 +184,9 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_prep_kernel(ScanParams s) {
                 // rows 32 ks + 4 q .. + 3 and 16 behind them: an operand's 8
                 float e[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = v[32 * ks + 16 * (i / 4) + 4 * q + i % 4];
+                for (int i = 0; i < 8; ++i) e[i] = v[32 * ks + 16 * (i / 4) + 4 * q + i % 4] * up;
                 s8v hi, lo;
-                split8(e, up, hi, lo);
+                split8(e, hi, lo);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int at = (32 * ks + 16 * (i / 4) + 4 * q + i % 4) * ROW + n;
@@ -228,11 +232,14 @@ template <int QT, int KW, bool STATE>
 __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
     constexpr int KK = 4 * KW;
     constexpr bool Y3 = QT != 2;                                  // y's products from both halfs of their operands
-    __shared__ __align__(16) s8v xop[2][2][2][4][64];             // [x, weighted x][hi, lo][32 rows][16 columns][lane]
-    __shared__ __align__(16) s8v hop[STATE ? 1 : 2][STATE ? 1 : KK][4][64];   // the state: [hi, lo][32 features][16 columns][lane]
-    __shared__ float xs[2][64], hs[STATE ? 1 : KK][64];           // what their results are to be multiplied with, a column
+    // x weighted for the state (hi, lo) and as it is (hi, for Y3 lo): [32 rows][16 columns][lane]; the state: [32 features][..]
+    constexpr int WH = 0, WL = 1, XH = 2, XL = 3, PLANES = STATE ? 2 : Y3 ? 4 : 3, HP = STATE ? 0 : Y3 ? 2 : 1;
+    __shared__ __align__(16) s8v xop[PLANES][2][4][64];
+    __shared__ __align__(16) s8v hop[HP + !HP][STATE ? 1 : KK][4][64];
+    __shared__ __align__(16) float xs[64], hs[64];                // what their results are to be multiplied with, a column
+    __shared__ float hmax[4][64];                                 // the largest of each wave's part of the state, a column
     __shared__ __align__(16) float hdrs[2][HDR];
-    __shared__ int bad[64], anybad[2];                            // a column's first row that is not finite; whether there is one
+    __shared__ int bad[64], spoilt[4];                            // a column's first row that is not finite; whether 16 columns have one
     const SsmLayer& p = s.l;
     const int tid = threadIdx.x, lane = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, g = lane / 16;
     // heads of a group read the same operands: consecutive work-groups of one XCD (every eighth of the launch)
@@ -245,7 +252,10 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
     const int col = c0 + 16 * w + n;                              // the column of x this lane convolves
     const bool has = col < p.P;
     const int xch = head * p.P + (has ? col : 0);
-    const float w0 = ssm_tap(p, xch, 0), w1 = ssm_tap(p, xch, 1), w2 = ssm_tap(p, xch, 2), w3 = ssm_tap(p, xch, 3), bias = p.cb ? p.cb[xch] : 0.0f;
+    // (the taps times log2 e: x comes out times it too, which its operand's scale takes back, and the exponential takes it as it is)
+    constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+    const float w0 = ssm_tap(p, xch, 0) * LOG2E, w1 = ssm_tap(p, xch, 1) * LOG2E, w2 = ssm_tap(p, xch, 2) * LOG2E, w3 = ssm_tap(p, xch, 3) * LOG2E;
+    const float bias = p.cb ? p.cb[xch] * LOG2E : 0.0f;
     const float skip = p.d ? p.d[head] : 0.0f;
     const int from = seg * s.per, to = min(s.chunks, from + s.per);
     const int64_t owner = (int64_t) head * s.blocks + block, owners = (int64_t) p.H * s.blocks;
@@ -291,7 +301,6 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
         }
     }
     float exponent = 0.0f;
-    if (tid < 2) anybad[tid] = 0;
     // a chunk's header, through registers into LDS; x: 16 rows of this lane's column - 16 j + 4 g .. + 3 - and 3 in front of each 4
     float head0, head1;
     auto fetch_header = [&](int c) {
@@ -331,6 +340,20 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
             }
         }
     };
+    // each column's largest in this wave's part of the state: what the next chunk's operands of it are scaled by
+    auto column_max = [&] {
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) {
+            float big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2 * KW; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(st[i][ct][e]));
+            big = rows_max(big);
+            if (g == 0) hmax[w][16 * ct + n] = big;
+        }
+    };
+    if constexpr (!STATE) column_max();
     fetch_header(from);
     put_header(from);
     fetch_x(from, g);
@@ -339,7 +362,7 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
     for (int c = from; c < to; ++c) {
         const float* hdr = hdrs[c % 2];
         const uint8_t* ops = s.ops + ((int64_t) c * p.G + group) * op_bytes(KK);
-        const float sb = s.scales[((int64_t) c * p.G + group) * 2], sc = s.scales[((int64_t) c * p.G + group) * 2 + 1];
+        const float scale_b = s.scales[((int64_t) c * p.G + group) * 2], sc = s.scales[((int64_t) c * p.G + group) * 2 + 1];
         // (opaque copies: addresses and comparisons made of them are a few instructions where they are needed, and not a
         // hundred registers kept over the loop)
         int ln = n, lg = g;
@@ -370,98 +393,107 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
                 for (int h = 0; h < 2; ++h)
                     if (ks <= w / 2) cbv[ks][h] = cbp[(ks * 64 + lane) * 2 + h];
         }
-        if (tid == 0) anybad[(c + 1) % 2] = 0;
         // x's operands
         {
             const int here = min(L, s.T - c * L);
             const bool whole = here == L;
-            float x[2][8], xw[2][8], big = 0.0f, bigw = 0.0f;
-            int where = L;
+            float x[2][8], big = 0.0f;
+            f4v wt[4];
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+            for (int j = 0; j < 4; ++j) {
+                // rows 16 j + 4 g .. + 3
+                wt[j] = *reinterpret_cast<const f4v*>(hdr + HDR_W + 16 * j + 4 * lg);
+                float u[7];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int r = 32 * ks + 16 * h + 4 * lg;
-                    const f4v wt = *reinterpret_cast<const f4v*>(hdr + HDR_W + r);
-                    float u[7];
+                for (int i = 0; i < 7; ++i) u[i] = raw_value<QT>(raw[7 * j + i]);
+                if (j == 0 && c == 0 && s.t0 == 0) {
+                    // (in front of the call: float32 from the ring, whatever the rows' type)
 #pragma unroll
-                    for (int i = 0; i < 7; ++i) u[i] = raw_value<QT>(raw[(2 * ks + h) * 7 + i]);
-                    if (ks == 0 && h == 0 && c == 0 && s.t0 == 0) {
-                        // (in front of the call: float32 from the ring, whatever the rows' type)
-#pragma unroll
-                        for (int i = 0; i < 3; ++i) u[i] = lg == 0 ? s.hist[(int64_t) i * p.chan + xch] : u[i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float y = silu(fmaf(w3, u[i + 3], fmaf(w2, u[i + 2], fmaf(w1, u[i + 1], fmaf(w0, u[i], bias)))));
-                        if (!whole) y = r + i < here ? y : 0.0f;
-                        x[ks][4 * h + i] = y;
-                        xw[ks][4 * h + i] = y * wt[i];
-                        if (!STATE) big = fmaxf(big, fabsf(y));
-                        bigw = fmaxf(bigw, fabsf(y * wt[i]));
-                    }
+                    for (int i = 0; i < 3; ++i) u[i] = lg == 0 ? s.hist[(int64_t) i * p.chan + xch] : u[i];
                 }
-            float up, down;
-            s8v hi, lo;
-            bigw = rows_max(bigw);
-            to_half_range(bigw, up, down);
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                split8(xw[ks], up, hi, lo);
-                xop[1][0][ks][w][lane] = hi;
-                xop[1][1][ks][w][lane] = lo;
+                for (int i = 0; i < 4; ++i) {
+                    const float v = fmaf(w3, u[i + 3], fmaf(w2, u[i + 2], fmaf(w1, u[i + 1], fmaf(w0, u[i], bias))));
+                    x[j / 2][4 * (j % 2) + i] = v * __builtin_amdgcn_rcpf(1.0f + fast_exp2(-v));
+                }
             }
-            if (g == 0) xs[1][16 * w + n] = down;
-            if constexpr (!STATE) {
-                // a row that is not finite must not reach the rows in front of it (0 times it is not 0): it goes in as 0, and
-                // from it on the column is NaN. (Sixteen numbers times 0 sum to 0, or to NaN where one is not finite)
-                float zero = 0.0f;
+            if (!whole) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) zero = fmaf(x[i / 8][i % 8], 0.0f, zero);
-                if (__ballot(zero != zero)) {
-                    big = 0.0f;
+                for (int i = 0; i < 16; ++i) x[i / 8][i % 8] = 16 * (i / 4) + 4 * lg + i % 4 < here ? x[i / 8][i % 8] : 0.0f;
+            }
+            // (a NaN among them stays one)
 #pragma unroll
-                    for (int i = 15; i >= 0; --i) {
-                        float& y = x[i / 8][i % 8];
-                        if (!(fabsf(y) < __builtin_inff())) {
-                            y = 0.0f;
-                            where = 16 * (i / 4) + 4 * lg + i % 4;
-                        }
-                        big = fmaxf(big, fabsf(y));
-                    }
-                    where = min(where, __shfl_xor(where, 16));
-                    where = min(where, __shfl_xor(where, 32));
-                    if (lane == 0) anybad[c % 2] = 1;
-                }
-                if (g == 0) bad[16 * w + n] = where;
-                big = rows_max(big);
-                to_half_range(big, up, down);
+            for (int i = 0; i < 16; ++i) big = __builtin_elementwise_maximum(big, fabsf(x[i / 8][i % 8]));
+            auto operands = [&](float big, auto held) {
+                float up, down;
+                to_half_range(rows_max(big), up, down);
+                if (g == 0) xs[16 * w + n] = down * LN2;
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
-                    split8(x[ks], up, hi, lo);
-                    xop[0][0][ks][w][lane] = hi;
-                    if constexpr (Y3) xop[0][1][ks][w][lane] = lo;
+                    float v[8], r[8];
+                    s8v hi, lo;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        v[i] = x[ks][i] * up;
+                        r[i] = v[i] * wt[2 * ks + i / 4][i % 4];
+                        // (a float32 from here on: rounded to a half in two ways - as it is, and fused with this product - it
+                        // may be two halfs, and the second operand is what the first leaves)
+                        asm volatile("" : "+v"(r[i]));
+                    }
+                    split8(r, hi, lo);
+                    xop[WH][ks][w][lane] = hi;
+                    xop[WL][ks][w][lane] = lo;
+                    if constexpr (!STATE) {
+                        if constexpr (decltype(held)::value) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) v[i] = fabsf(v[i]) < __builtin_inff() ? v[i] : 0.0f;
+                        }
+                        split8(v, hi, lo);
+                        xop[XH][ks][w][lane] = hi;
+                        if constexpr (Y3) xop[XL][ks][w][lane] = lo;
+                    }
                 }
-                if (g == 0) xs[0][16 * w + n] = down;
+            };
+            const bool fine = STATE || !__ballot(!(big < __builtin_inff()));
+            if (!STATE && lane == 0) spoilt[w] = !fine;
+            if (fine) operands(big, std::false_type());
+            else {
+                // a row that is not finite must not reach the rows in front of it (0 times it is not 0): among x's operands it is
+                // 0, and from it on the column is NaN
+                int where = L;
+                big = 0.0f;
+#pragma unroll
+                for (int i = 15; i >= 0; --i) {
+                    const float y = fabsf(x[i / 8][i % 8]);
+                    if (y < __builtin_inff()) big = fmaxf(big, y);
+                    else where = 16 * (i / 4) + 4 * lg + i % 4;
+                }
+                where = min(where, __shfl_xor(where, 16));
+                where = min(where, __shfl_xor(where, 32));
+                operands(big, std::true_type());
+                if (g == 0) bad[16 * w + n] = where;
             }
         }
         // this wave's part of the state
         if constexpr (!STATE) {
 #pragma unroll
-            for (int j = 0; j < KW; ++j)
+            for (int ct = 0; ct < 4; ++ct) {
+                const int at = 16 * ct + n;
+                const float most = fmaxf(fmaxf(hmax[0][at], hmax[1][at]), fmaxf(hmax[2][at], hmax[3][at]));
+                float up, down;
+                to_half_range(most, up, down);
+                if (w == 0 && g == 0) hs[at] = down;
 #pragma unroll
-                for (int ct = 0; ct < 4; ++ct) {
-                    float v[8], big = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = st[2 * j + i / 4][ct][i % 4], big = fmaxf(big, fabsf(v[i]));
-                    float up, down;
-                    to_half_range(rows_max(big), up, down);
+                for (int j = 0; j < KW; ++j) {
+                    float v[8];
                     s8v hi, lo;
-                    split8(v, up, hi, lo);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = st[2 * j + i / 4][ct][i % 4] * up;
+                    split8(v, hi, lo);
                     hop[0][w * KW + j][ct][lane] = hi;
                     if constexpr (Y3) hop[1][w * KW + j][ct][lane] = lo;
-                    if (g == 0) hs[w * KW + j][16 * ct + n] = down;
                 }
+            }
         }
         lds_barrier();
         if (c + 1 < to) fetch_x(c + 1, lg);
@@ -474,18 +506,12 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
             for (int kk = 0; kk < KK; ++kk) {
 #pragma unroll
                 for (int ct = 0; ct < 4; ++ct) {
-                    f4v a = mfma16<false>(hop[0][kk][ct][lane], cop[kk][0], f4v{0.0f, 0.0f, 0.0f, 0.0f});
+                    yi[ct] = mfma16<false>(hop[0][kk][ct][lane], cop[kk][0], yi[ct]);
                     if constexpr (Y3) {
-                        a = mfma16<false>(hop[1][kk][ct][lane], cop[kk][0], a);
-                        a = mfma16<false>(hop[0][kk][ct][lane], cop[kk][1], a);
+                        yi[ct] = mfma16<false>(hop[HP - 1][kk][ct][lane], cop[kk][0], yi[ct]);
+                        yi[ct] = mfma16<false>(hop[0][kk][ct][lane], cop[kk][1], yi[ct]);
                     }
-                    const f4v f = *reinterpret_cast<const f4v*>(&hs[kk][16 * ct + 4 * g]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) yi[ct][e] = fmaf(a[e], f[e], yi[ct][e]);
                 }
-                // (here, and not where y is written: the compiler would keep every step's results and scales until then)
-#pragma unroll
-                for (int ct = 0; ct < 4; ++ct) asm volatile("" : "+v"(yi[ct]));
             }
             // the chunk's own rows: C . B decayed, d on the diagonal
             const int row = 16 * w + ln;
@@ -520,26 +546,27 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
             for (int ks = 0; ks < 2; ++ks) {
                 if (ks > w / 2) break;
                 s8v hi, lo;
-                split8(m[ks], up, hi, lo);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m[ks][i] *= up;
+                split8(m[ks], hi, lo);
 #pragma unroll
                 for (int ct = 0; ct < 4; ++ct) {
-                    y[ct] = mfma16<false>(xop[0][0][ks][ct][lane], hi, y[ct]);
+                    y[ct] = mfma16<false>(xop[XH][ks][ct][lane], hi, y[ct]);
                     if constexpr (Y3) {
-                        y[ct] = mfma16<false>(xop[0][1][ks][ct][lane], hi, y[ct]);
-                        y[ct] = mfma16<false>(xop[0][0][ks][ct][lane], lo, y[ct]);
+                        y[ct] = mfma16<false>(xop[PLANES - 1][ks][ct][lane], hi, y[ct]);
+                        y[ct] = mfma16<false>(xop[XH][ks][ct][lane], lo, y[ct]);
                     }
                 }
             }
             const int t = c * L + row;
             const float el = hdr[HDR_E + row] * sc;
-            const bool spoilt = anybad[c % 2];
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) {
-                const f4v f = *reinterpret_cast<const f4v*>(&xs[0][16 * ct + 4 * lg]);
+                const f4v f = *reinterpret_cast<const f4v*>(&xs[16 * ct + 4 * lg]), fi = *reinterpret_cast<const f4v*>(&hs[16 * ct + 4 * lg]);
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = fmaf(y[ct][e], f[e] * down, yi[ct][e] * el);
-                if (spoilt) {
+                for (int e = 0; e < 4; ++e) v[e] = fmaf(y[ct][e], f[e] * down, yi[ct][e] * (fi[e] * el));
+                if (spoilt[ct]) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (row >= bad[16 * ct + 4 * lg + e]) v[e] = __builtin_nanf("");
@@ -557,7 +584,7 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
         }
         // the state behind the chunk
         {
-            const float keep = hdr[HDR_END + 1];
+            const float keep = hdr[HDR_END + 1], sb = scale_b * hdr[HDR_END + 2];
             exponent += hdr[HDR_END];
 #pragma unroll
             for (int i = 0; i < 2 * KW; ++i) {
@@ -568,19 +595,20 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
                 for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                     for (int ct = 0; ct < 4; ++ct) {
-                        a[ct] = mfma16<false>(bop[i][ks][0], xop[1][0][ks][ct][lane], a[ct]);
-                        a[ct] = mfma16<false>(bop[i][ks][1], xop[1][0][ks][ct][lane], a[ct]);
-                        a[ct] = mfma16<false>(bop[i][ks][0], xop[1][1][ks][ct][lane], a[ct]);
+                        a[ct] = mfma16<false>(bop[i][ks][0], xop[WH][ks][ct][lane], a[ct]);
+                        a[ct] = mfma16<false>(bop[i][ks][1], xop[WH][ks][ct][lane], a[ct]);
+                        a[ct] = mfma16<false>(bop[i][ks][0], xop[WL][ks][ct][lane], a[ct]);
                     }
 #pragma unroll
                 for (int ct = 0; ct < 4; ++ct) {
-                    const float f = sb * xs[1][16 * ct + n];
+                    const float f = sb * xs[16 * ct + n];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) st[i][ct][e] = fmaf(st[i][ct][e], keep, a[ct][e] * f);
                 }
             }
         }
         put_header(c + 1);
+        if constexpr (!STATE) column_max();
         lds_barrier();
     }
 
