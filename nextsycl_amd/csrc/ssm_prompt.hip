@@ -228,18 +228,23 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_prep_kernel(ScanParams s) {
     }
 }
 
+// work-groups a CU: what LDS has room for, and the registers that leaves a wave
 template <int QT, int KW, bool STATE>
-__global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
+constexpr int SCAN_WGS = KW == 2 ? 1 : STATE ? 4 : QT == 2 ? 3 : 2;
+template <int QT, int KW, bool STATE>
+__global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kernel(ScanParams s) {
     constexpr int KK = 4 * KW;
+    constexpr bool AHEAD = SCAN_WGS<QT, KW, STATE> <= 2;          // x and the operands asked for early: no third work-group hides their latency
     constexpr bool Y3 = QT != 2;                                  // y's products from both halfs of their operands
     // x weighted for the state (hi, lo) and as it is (hi, for Y3 lo): [32 rows][16 columns][lane]; the state: [32 features][..]
     constexpr int WH = 0, WL = 1, XH = 2, XL = 3, PLANES = STATE ? 2 : Y3 ? 4 : 3, HP = STATE ? 0 : Y3 ? 2 : 1;
     __shared__ __align__(16) s8v xop[PLANES][2][4][64];
     __shared__ __align__(16) s8v hop[HP + !HP][STATE ? 1 : KK][4][64];
     __shared__ __align__(16) float xs[64], hs[64];                // what their results are to be multiplied with, a column
-    __shared__ float hmax[4][64];                                 // the largest of each wave's part of the state, a column
+    __shared__ __align__(16) float hmax[64][4];                   // the largest of each wave's part of the state, a column
     __shared__ __align__(16) float hdrs[2][HDR];
-    __shared__ int bad[64], spoilt[4];                            // a column's first row that is not finite; whether 16 columns have one
+    __shared__ int bad[64];
+    __shared__ __align__(16) int spoilt[4];                       // a column's first row that is not finite; whether 16 columns have one
     const SsmLayer& p = s.l;
     const int tid = threadIdx.x, lane = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, g = lane / 16;
     // heads of a group read the same operands: consecutive work-groups of one XCD (every eighth of the launch)
@@ -350,13 +355,13 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(st[i][ct][e]));
             big = rows_max(big);
-            if (g == 0) hmax[w][16 * ct + n] = big;
+            if (g == 0) hmax[16 * ct + n][w] = big;
         }
     };
     if constexpr (!STATE) column_max();
     fetch_header(from);
     put_header(from);
-    fetch_x(from, g);
+    if constexpr (AHEAD) fetch_x(from, g);
     __syncthreads();
 
     for (int c = from; c < to; ++c) {
@@ -371,7 +376,7 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
         // this chunk's operands, on their way while x and the state become theirs
         s8v bop[2 * KW][2][2], cop[STATE ? 1 : KK][2];
         f4v cbv[2][2];
-        {
+        auto fetch_b = [&] {
             const s8v* b = reinterpret_cast<const s8v*>(ops + 2 * op_c(KK)) + lane;
 #pragma unroll
             for (int i = 0; i < 2 * KW; ++i)
@@ -379,8 +384,8 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
                 for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) bop[i][ks][h] = b[((w * 2 * KW + i) * 2 + ks) * 64 + h * (op_c(KK) / 16)];
-        }
-        if constexpr (!STATE) {
+        };
+        auto fetch_c = [&] {
             const s8v* cp = reinterpret_cast<const s8v*>(ops) + w * KK * 64 + lane;
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
@@ -392,7 +397,11 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                     if (ks <= w / 2) cbv[ks][h] = cbp[(ks * 64 + lane) * 2 + h];
-        }
+        };
+        if constexpr (AHEAD) {
+            fetch_b();
+            if constexpr (!STATE) fetch_c();
+        } else fetch_x(c, lg);
         // x's operands
         {
             const int here = min(L, s.T - c * L);
@@ -476,10 +485,13 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
         }
         // this wave's part of the state
         if constexpr (!STATE) {
+            f4v parts[4];
+#pragma unroll
+            for (int ct = 0; ct < 4; ++ct) parts[ct] = *reinterpret_cast<const f4v*>(hmax[16 * ct + n]);
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) {
                 const int at = 16 * ct + n;
-                const float most = fmaxf(fmaxf(hmax[0][at], hmax[1][at]), fmaxf(hmax[2][at], hmax[3][at]));
+                const float most = fmaxf(fmaxf(parts[ct][0], parts[ct][1]), fmaxf(parts[ct][2], parts[ct][3]));
                 float up, down;
                 to_half_range(most, up, down);
                 if (w == 0 && g == 0) hs[at] = down;
@@ -495,8 +507,11 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
                 }
             }
         }
+        if constexpr (!AHEAD && !STATE) fetch_c();
         lds_barrier();
-        if (c + 1 < to) fetch_x(c + 1, lg);
+        if constexpr (AHEAD) {
+            if (c + 1 < to) fetch_x(c + 1, lg);
+        } else if constexpr (STATE) fetch_b();
         if constexpr (!STATE) {
             // 16 rows of y: this lane row 16 w + n, columns 16 ct + 4 g .. + 3
             f4v y[4], yi[4];
@@ -517,19 +532,27 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
             const int row = 16 * w + ln;
             const float cl = hdr[HDR_C + row];
             float m[2][8], big = 0.0f;
+            const f4v bd = *reinterpret_cast<const f4v*>(hdr + HDR_BD + 4 * w);
+            f4v cs[4], dts[4];
+            auto fetch_run = [&](int st) {
+                cs[st] = *reinterpret_cast<const f4v*>(hdr + HDR_C + 16 * st + 4 * lg);
+                dts[st] = *reinterpret_cast<const f4v*>(hdr + HDR_DT + 16 * st + 4 * lg);
+            };
+#pragma unroll
+            for (int st = 0; st < 4 && AHEAD; ++st) fetch_run(st);
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
-                const int sr = 16 * st + 4 * lg;
                 float* to_m = m[st / 2] + 4 * (st % 2);
                 if (st > w) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) to_m[i] = 0.0f;
                     continue;
                 }
-                const float base = cl + hdr[HDR_BD + 4 * w + st];
-                const f4v cb = cbv[st / 2][st % 2], cs = *reinterpret_cast<const f4v*>(hdr + HDR_C + sr), dt = *reinterpret_cast<const f4v*>(hdr + HDR_DT + sr);
+                if (!AHEAD) fetch_run(st);
+                const float base = cl + bd[st];
+                const f4v cb = cbv[st / 2][st % 2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) to_m[i] = cb[i] * dt[i] * fast_exp2(base - cs[i]);
+                for (int i = 0; i < 4; ++i) to_m[i] = cb[i] * dts[st][i] * fast_exp2(base - cs[st][i]);
                 if (st == w) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -558,27 +581,37 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
                     }
                 }
             }
+            if constexpr (!AHEAD) fetch_b();
             const int t = c * L + row;
             const float el = hdr[HDR_E + row] * sc;
+            const int4 sp = *reinterpret_cast<const int4*>(spoilt);
+            const bool finite = !__builtin_amdgcn_readfirstlane(sp.x | sp.y | sp.z | sp.w);
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) {
                 const f4v f = *reinterpret_cast<const f4v*>(&xs[16 * ct + 4 * lg]), fi = *reinterpret_cast<const f4v*>(&hs[16 * ct + 4 * lg]);
-                float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = fmaf(y[ct][e], f[e] * down, yi[ct][e] * (fi[e] * el));
-                if (spoilt[ct]) {
+                for (int e = 0; e < 4; ++e) y[ct][e] = fmaf(y[ct][e], f[e] * down, yi[ct][e] * (fi[e] * el));
+                if (!AHEAD) asm volatile("" : "+v"(y[ct]));          // (few registers: one column tile after another)
+            }
+            if (!finite) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (row >= bad[16 * ct + 4 * lg + e]) v[e] = __builtin_nanf("");
-                }
-                if (t >= s.T) continue;
-                const int pc = c0 + 16 * ct + 4 * lg;
-                const int64_t at = (s.t0 + t) * p.ys + (int64_t) head * p.P + pc;
-                if (s.vec_y && pc + 4 <= p.P) store_row<QT, 4>(p.y, at, v);
-                else {
+                for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (pc + e < p.P) store_o<QT>(p.y, at + e, v[e]);
+                        if (spoilt[ct] && row >= bad[16 * ct + 4 * lg + e]) y[ct][e] = __builtin_nanf("");
+            }
+            if (t < s.T) {
+                const int64_t at = (s.t0 + t) * p.ys + (int64_t) head * p.P + c0 + 4 * lg;
+                if (s.vec_y) {
+#pragma unroll
+                    for (int ct = 0; ct < 4; ++ct) {
+                        const float v[4] = {y[ct][0], y[ct][1], y[ct][2], y[ct][3]};
+                        if (c0 + 16 * ct + 4 * lg < p.P) store_row<QT, 4>(p.y, at + 16 * ct, v);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (c0 + 16 * (i / 4) + 4 * lg + i % 4 < p.P) store_o<QT>(p.y, at + 16 * (i / 4) + i % 4, y[i / 4][i % 4]);
                 }
             }
         }
@@ -586,24 +619,40 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_scan_kernel(ScanParams s) {
         {
             const float keep = hdr[HDR_END + 1], sb = scale_b * hdr[HDR_END + 2];
             exponent += hdr[HDR_END];
+            s8v ahead[2][2][2];
+            float fs[4];
 #pragma unroll
-            for (int i = 0; i < 2 * KW; ++i) {
-                f4v a[4];
+            for (int ct = 0; ct < 4; ++ct) fs[ct] = xs[16 * ct + n];
+            auto operands = [&](int ct) {
 #pragma unroll
-                for (int ct = 0; ct < 4; ++ct) a[ct] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int ks = 0; ks < 2; ++ks) ahead[ct % 2][ks][0] = xop[WH][ks][ct][lane], ahead[ct % 2][ks][1] = xop[WL][ks][ct][lane];
+            };
+            // (a column tile ahead, but where four work-groups a CU hide the reads)
+            if constexpr (!STATE) operands(0);
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks)
+            for (int ct = 0; ct < 4; ++ct) {
+                if constexpr (STATE) operands(ct);
+                else if (ct < 3) operands(ct + 1);
+                f4v a[2 * KW];
 #pragma unroll
-                    for (int ct = 0; ct < 4; ++ct) {
-                        a[ct] = mfma16<false>(bop[i][ks][0], xop[WH][ks][ct][lane], a[ct]);
-                        a[ct] = mfma16<false>(bop[i][ks][1], xop[WH][ks][ct][lane], a[ct]);
-                        a[ct] = mfma16<false>(bop[i][ks][0], xop[WL][ks][ct][lane], a[ct]);
-                    }
+                for (int i = 0; i < 2 * KW; ++i) a[i] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int ct = 0; ct < 4; ++ct) {
-                    const float f = sb * xs[16 * ct + n];
+                for (int ks = 0; ks < 2; ++ks) {
+                    const s8v hi = ahead[ct % 2][ks][0], lo = ahead[ct % 2][ks][1];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) st[i][ct][e] = fmaf(st[i][ct][e], keep, a[ct][e] * f);
+                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][0], hi, a[i]);
+#pragma unroll
+                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][1], hi, a[i]);
+#pragma unroll
+                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][0], lo, a[i]);
+                }
+                const float f = sb * fs[ct];
+#pragma unroll
+                for (int i = 0; i < 2 * KW; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st[i][ct][e] = fmaf(st[i][ct][e], keep, a[i][e] * f);
+                    // (here: the compiler would ask for all columns' operands at once)
+                    asm volatile("" : "+v"(st[i][ct]));
                 }
             }
         }
