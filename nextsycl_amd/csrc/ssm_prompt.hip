@@ -45,14 +45,15 @@ struct ScanParams {
     SsmLayer l;
     int64_t t0, all;            // the pass's first row, the call's rows
     int T, chunks, segs, per;   // rows and chunks of the pass; segments, chunks a segment
+    int sub, piece;             // pieces a segment whose states are found apart, chunks a piece
     int blocks, vec_y, vec_h;   // blocks of 64 features a head; y in pieces of 4 values, the state too
     uint8_t* ops;               // [chunk][group] operands
     float* scales;              // [chunk][group]: what B's and C's operands are to be multiplied with
     float* hdr;                 // [chunk][head]
     float* hist;                // [3][chan]: the raw rows in front of the call's first
-    float* segst;               // [1 + segment][head, block]: the pass's first state, then what each segment leaves - the first
-                                // from that state, the others from zero
-    float* segtot;              // [segment][head]: their exponents
+    float* segst;               // [1 + piece][head, block]: the pass's first state, then what each piece of the segments but the
+                                // last leaves - the first from that state, the others from zero
+    float* segtot;              // [piece][head]: their exponents
 };
 
 // a power of two that takes `big` to 2^13 .. 2^14, and its inverse
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     const int total = gridDim.x;
     if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
     const int per = p.H / p.G, hb = per * s.blocks;
-    const int in_group = id % hb, seg = id / hb % s.segs, group = id / (hb * s.segs);
+    const int in_group = id % hb, seg = id / hb % s.segs, group = id / (hb * s.segs);       // (STATE: seg counts pieces)
     const int head = group * per + in_group / s.blocks, block = in_group % s.blocks, c0 = block * 64;
     const int col = c0 + 16 * w + n;                              // the column of x this lane convolves
     const bool has = col < p.P;
@@ -262,7 +263,8 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     const float w0 = ssm_tap(p, xch, 0) * LOG2E, w1 = ssm_tap(p, xch, 1) * LOG2E, w2 = ssm_tap(p, xch, 2) * LOG2E, w3 = ssm_tap(p, xch, 3) * LOG2E;
     const float bias = p.cb ? p.cb[xch] * LOG2E : 0.0f;
     const float skip = p.d ? p.d[head] : 0.0f;
-    const int from = seg * s.per, to = min(s.chunks, from + s.per);
+    const int from = STATE ? seg / s.sub * s.per + seg % s.sub * s.piece : seg * s.per;
+    const int to = min(s.chunks, STATE ? min(from + s.piece, (seg / s.sub + 1) * s.per) : from + s.per);
     const int64_t owner = (int64_t) head * s.blocks + block, owners = (int64_t) p.H * s.blocks;
 
     // features 32 (w KW + i / 2) + 16 (i % 2) + 4 g .. + 3 of column 16 ct + n
@@ -296,7 +298,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
         for (int i = 0; i < 2 * KW; ++i)
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) st[i][ct] = STATE ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : src[(i * 4 + ct) * 64];
-        for (int r = 1; !STATE && r < seg; ++r) {
+        for (int r = 1; !STATE && r < seg * s.sub; ++r) {
             const float keep = exp2f(s.segtot[(int64_t) r * p.H + head]);
             const f4v* add = kept(1 + r);
 #pragma unroll
@@ -702,19 +704,22 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
 
 // how a pass of T rows is cut, and where its scratch lies
 struct Plan {
-    int kk, chunks, segs, per, blocks;
+    int kk, chunks, segs, per, sub, piece, blocks;
     int64_t ops, scales, hdr, hist, segst, segtot, floats;
 };
-Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G) {
+Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
     Plan q{};
     q.kk = N <= 128 ? 4 : 8;
     q.chunks = (int) ((T + L - 1) / L);
     q.blocks = (int) ((P + 63) / 64);
     const int64_t owners = H * q.blocks;
-    // enough segments for two work-groups a CU, of 4 chunks at least
-    int64_t segs = std::max<int64_t>(1, std::min<int64_t>({MOST_SEGS, 512 / owners, q.chunks / 4}));
+    // as many segments as fill the chip's places for the scan's work-groups, of 4 chunks at least
+    const int64_t segs = std::max<int64_t>(1, std::min<int64_t>({MOST_SEGS, 256 * wgs / owners, q.chunks / 4}));
     q.per = (int) ((q.chunks + segs - 1) / segs);
     q.segs = (q.chunks + q.per - 1) / q.per;
+    // their states in as many pieces as fill those of the state kernel's, of 4 chunks at least
+    q.sub = q.segs == 1 ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>(q.per / 4, (1024 + owners * (q.segs - 1) - 1) / (owners * (q.segs - 1))));
+    q.piece = (q.per + q.sub - 1) / q.sub;
     int64_t at = 0;
     auto take = [&](int64_t floats) {
         const int64_t here = at;
@@ -725,8 +730,9 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G) {
     q.scales = take(q.chunks * G * 2);
     q.hdr = take(q.chunks * H * HDR);
     q.hist = take(3 * (H * P + 2 * G * N));
-    q.segst = take(q.segs > 1 ? q.segs * owners * 64 * q.kk * 32 : 0);
-    q.segtot = take(q.segs > 1 ? q.segs * H : 0);
+    const int64_t pieces = (q.segs - 1) * (int64_t) q.sub;
+    q.segst = take(pieces ? (1 + pieces) * owners * 64 * q.kk * 32 : 0);
+    q.segtot = take(pieces * H);
     q.floats = at;
     return q;
 }
@@ -737,7 +743,7 @@ void launch_pass(ns_gpu* g, ScanParams& s, const Plan& q) {
     const unsigned owners = (unsigned) (s.l.H * q.blocks);
     if (q.segs > 1) {
         ScanParams f = s;
-        f.segs = q.segs - 1;            // (the last segment's state is the scan's own)
+        f.segs = (q.segs - 1) * q.sub;      // (the last segment's state is the scan's own)
         ssm_scan_kernel<QT, KW, true><<<owners * f.segs, 256, 0, g->q>>>(f);
     }
     ssm_scan_kernel<QT, KW, false><<<owners * q.segs, 256, 0, g->q>>>(s);
@@ -747,8 +753,8 @@ template <int QT>
 void run_prompt(ns_gpu* g, const SsmLayer& p, int64_t T, float* scratch) {
     for (int64_t t0 = 0; t0 < T; t0 += PASS_ROWS) {
         const int64_t n = std::min(PASS_ROWS, T - t0);
-        const Plan q = plan_of(n, p.H, p.P, p.N, p.G);
-        ScanParams s{p, t0, T, (int) n, q.chunks, q.segs, q.per, q.blocks};
+        const Plan q = plan_of(n, p.H, p.P, p.N, p.G, p.N <= 128 ? SCAN_WGS<QT, 1, false> : SCAN_WGS<QT, 2, false>);
+        ScanParams s{p, t0, T, (int) n, q.chunks, q.segs, q.per, q.sub, q.piece, q.blocks};
         s.vec_y = (uintptr_t) p.y % (QT ? 8 : 16) == 0 && p.ys % 4 == 0 && p.P % 4 == 0;
         s.vec_h = p.N % 4 == 0 && (uintptr_t) p.h0 % 16 == 0 && (uintptr_t) p.h1 % 16 == 0;
         s.ops = reinterpret_cast<uint8_t*>(scratch + q.ops);
@@ -764,9 +770,12 @@ extern "C" {
 
 int64_t ns_ssm_prompt_scratch(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K) {
     if (T <= 0 || H <= 0 || P <= 0 || N <= 0 || G <= 0 || K <= 0) return 0;
-    // (a last pass of fewer rows may be cut in more segments than a full one)
-    int64_t most = plan_of(std::min(T, PASS_ROWS), H, P, N, G).floats;
-    if (T > PASS_ROWS && T % PASS_ROWS) most = std::max(most, plan_of(T % PASS_ROWS, H, P, N, G).floats);
+    // (whatever the rows' type; and a last pass of fewer rows may be cut in more segments than a full one)
+    int64_t most = 0;
+    for (int wgs = 1; wgs <= 3; ++wgs) {
+        most = std::max(most, plan_of(std::min(T, PASS_ROWS), H, P, N, G, wgs).floats);
+        if (T > PASS_ROWS && T % PASS_ROWS) most = std::max(most, plan_of(T % PASS_ROWS, H, P, N, G, wgs).floats);
+    }
     return most;
 }
 
