@@ -62,15 +62,23 @@ __device__ __forceinline__ void to_half_range(float big, float& up, float& down)
     up = __builtin_bit_cast(float, (uint32_t) e << 23);
     down = __builtin_bit_cast(float, (uint32_t) (254 - e) << 23);
 }
-// 8 floats as two operands: halfs and the halfs of what they leave
-__device__ __forceinline__ void split8(const float (&v)[8], s8v& hi, s8v& lo) {
-    h8v a, b;
+// 8 floats as two operands: halfs and the halfs of what they leave. (The first halfs are opaque from where they are made: the
+// compiler would round a float a second time for the difference, and may round it otherwise there - fused with the product it
+// comes from -, which leaves two operands that do not belong together.)
+__device__ __forceinline__ s8v half8(const float (&v)[8]) {
+    h8v a;
 #pragma unroll
     for (int j = 0; j < 8; ++j) a[j] = (_Float16) v[j];
+    return __builtin_bit_cast(s8v, a);
+}
+__device__ __forceinline__ void split8(const float (&v)[8], s8v& hi, s8v& lo) {
+    hi = half8(v);
+    asm volatile("" : "+v"(hi));
+    const h8v a = __builtin_bit_cast(h8v, hi);
+    float r[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = (_Float16) (v[j] - (float) a[j]);
-    hi = __builtin_bit_cast(s8v, a);
-    lo = __builtin_bit_cast(s8v, b);
+    for (int j = 0; j < 8; ++j) r[j] = fmaf((float) a[j], -1.0f, v[j]);
+    lo = half8(r);
 }
 
 // the ring's value `at` rows (negative) from the call's first: zeros in front of the sequence, and of taps that there are not
@@ -78,12 +86,7 @@ __device__ __forceinline__ float ring_row(const SsmLayer& p, int64_t at, int ch)
     return at >= 1 - p.K && p.p0 + at >= 0 ? p.conv[(p.p0 + at) % p.cap * p.chan + ch] : 0.0f;
 }
 
-// a row's value as it lies in memory, and as a number
-template <int QT>
-__device__ __forceinline__ uint32_t raw_bits(const char* p, uint32_t off) {
-    if constexpr (QT == 0) return *reinterpret_cast<const uint32_t*>(p + off);
-    else return *reinterpret_cast<const uint16_t*>(p + off);
-}
+// a row's value out of its bits
 template <int QT>
 __device__ __forceinline__ float raw_value(uint32_t b) {
     return QT == 0 ? __builtin_bit_cast(float, b) : QT == 1 ? f16_to_f32((uint16_t) b) : bf16_to_f32((uint16_t) b);
@@ -325,25 +328,25 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     auto fetch_x = [&](int c, int g) {
         const int here = min(L, s.T - c * L);
         const int64_t first = s.t0 + (int64_t) c * L;
-        if (first > 0 && here == L) {
-            // (opaque too: the compiler would carry 28 addresses from chunk to chunk)
-            const char* rows = static_cast<const char*>(p.xbc) + (first - 3) * row_bytes;
-            int64_t step = row_bytes;
-            asm volatile("" : "+s"(rows), "+s"(step));
+        // as a buffer of its own, from the first row of the chunk that there is in front of its first: a lane's offset in a vector
+        // register, a row's in a scalar one
+        const int front = first > 0 ? 3 : 0;
+        const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.xbc) + (first - front) * row_bytes), (short) 0, -1, 0x00020000);
+        auto at = [&](uint32_t lane_off, uint32_t off) {
+            if constexpr (QT == 0) return (uint32_t) __builtin_amdgcn_raw_buffer_load_b32(rows, lane_off, off, 0);
+            else return (uint32_t) (uint16_t) __builtin_amdgcn_raw_buffer_load_b16(rows, lane_off, off, 0);
+        };
+        if (front && here == L) {
+            uint32_t step = (uint32_t) row_bytes;
+            asm volatile("" : "+s"(step));           // (or the compiler carries 28 offsets from chunk to chunk)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const char* run = rows + 16 * j * step;
-#pragma unroll
-                for (int i = 0; i < 7; ++i, run += step) raw[7 * j + i] = raw_bits<QT>(run, lane_off);
-            }
+            for (int j = 0; j < 28; ++j) raw[j] = at(lane_off, (16 * (j / 7) + j % 7) * step);
         } else {
             // the call's first chunk, or one that is not whole: rows held to those that there are (those in front of the call come from the ring)
-            const int skipped = first > 0 ? 3 : 0;
-            const char* rows = static_cast<const char*>(p.xbc) + (first - skipped) * row_bytes;
 #pragma unroll
             for (int j = 0; j < 28; ++j) {
-                const int r = min(max(16 * (j / 7) + 4 * g + j % 7 - 3 + skipped, 0), here - 1 + skipped);
-                raw[j] = raw_bits<QT>(rows, (uint32_t) r * (uint32_t) row_bytes + (uint32_t) xch * (QT ? 2 : 4));
+                const int r = min(max(16 * (j / 7) + 4 * g + j % 7 - 3 + front, 0), here - 1 + front);
+                raw[j] = at((uint32_t) r * (uint32_t) row_bytes + (uint32_t) xch * (QT ? 2 : 4), 0);
             }
         }
     };
@@ -355,7 +358,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
 #pragma unroll
             for (int i = 0; i < 2 * KW; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(st[i][ct][e]));
+                for (int e = 0; e < 4; ++e) big = __builtin_elementwise_maximum(big, fabsf(st[i][ct][e]));
             big = rows_max(big);
             if (g == 0) hmax[16 * ct + n][w] = big;
         }
@@ -429,6 +432,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                 }
             }
             if (!whole) {
+                asm volatile("");        // (a branch, not 32 instructions of every chunk)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[i / 8][i % 8] = 16 * (i / 4) + 4 * lg + i % 4 < here ? x[i / 8][i % 8] : 0.0f;
             }
@@ -447,9 +451,6 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                     for (int i = 0; i < 8; ++i) {
                         v[i] = x[ks][i] * up;
                         r[i] = v[i] * wt[2 * ks + i / 4][i % 4];
-                        // (a float32 from here on: rounded to a half in two ways - as it is, and fused with this product - it
-                        // may be two halfs, and the second operand is what the first leaves)
-                        asm volatile("" : "+v"(r[i]));
                     }
                     split8(r, hi, lo);
                     xop[WH][ks][w][lane] = hi;
@@ -459,9 +460,11 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
 #pragma unroll
                             for (int i = 0; i < 8; ++i) v[i] = fabsf(v[i]) < __builtin_inff() ? v[i] : 0.0f;
                         }
-                        split8(v, hi, lo);
+                        if constexpr (Y3) {
+                            split8(v, hi, lo);
+                            xop[XL][ks][w][lane] = lo;
+                        } else hi = half8(v);
                         xop[XH][ks][w][lane] = hi;
-                        if constexpr (Y3) xop[XL][ks][w][lane] = lo;
                     }
                 }
             };
@@ -503,9 +506,11 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                     s8v hi, lo;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = st[2 * j + i / 4][ct][i % 4] * up;
-                    split8(v, hi, lo);
+                    if constexpr (Y3) {
+                        split8(v, hi, lo);
+                        hop[1][w * KW + j][ct][lane] = lo;
+                    } else hi = half8(v);
                     hop[0][w * KW + j][ct][lane] = hi;
-                    if constexpr (Y3) hop[1][w * KW + j][ct][lane] = lo;
                 }
             }
         }
@@ -573,7 +578,8 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                 s8v hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) m[ks][i] *= up;
-                split8(m[ks], hi, lo);
+                if constexpr (Y3) split8(m[ks], hi, lo);
+                else hi = half8(m[ks]);
 #pragma unroll
                 for (int ct = 0; ct < 4; ++ct) {
                     y[ct] = mfma16<false>(xop[XH][ks][ct][lane], hi, y[ct]);
@@ -637,12 +643,10 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                 else if (ct < 3) operands(ct + 1);
                 f4v a[2 * KW];
 #pragma unroll
-                for (int i = 0; i < 2 * KW; ++i) a[i] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     const s8v hi = ahead[ct % 2][ks][0], lo = ahead[ct % 2][ks][1];
 #pragma unroll
-                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][0], hi, a[i]);
+                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][0], hi, ks ? a[i] : f4v{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
                     for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][1], hi, a[i]);
 #pragma unroll
