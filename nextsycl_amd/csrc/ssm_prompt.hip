@@ -121,15 +121,15 @@ __device__ __forceinline__ void ssm_header(const ScanParams& s, int chunk, int h
 }
 
 template <int QT, int KW>
-__global__ __launch_bounds__(256, 3 - KW) void ssm_prep_kernel(ScanParams s) {
+__global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
     constexpr int NP = 128 * KW, KK = 4 * KW, ROW = NP + 8;
     __shared__ __align__(16) short plane[2][2][L * ROW];       // [B, C][hi, lo][row][feature]
-    __shared__ float part[2][4];
+    __shared__ float part[2][8];
     const SsmLayer& p = s.l;
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n16 = lane % 16, g = lane / 16;
     if ((int) blockIdx.x >= s.chunks * p.G) {
         // work-groups behind those: headers, a wave a (chunk, head)
-        const int64_t i = (int64_t) (blockIdx.x - s.chunks * p.G) * 4 + wave;
+        const int64_t i = (int64_t) (blockIdx.x - s.chunks * p.G) * 8 + wave;
         if (i < (int64_t) s.chunks * p.H) ssm_header<QT>(s, (int) (i / p.H), (int) (i % p.H), lane);
         return;
     }
@@ -140,95 +140,95 @@ __global__ __launch_bounds__(256, 3 - KW) void ssm_prep_kernel(ScanParams s) {
     // the rows in front of the call, for the scan's x: the ring is written while that runs
     if (first == 0) {
         const int ch0 = group * per * p.P, chn = per * p.P;
-        for (int i = tid; i < 3 * chn; i += 256) s.hist[(int64_t) (i / chn) * p.chan + ch0 + i % chn] = ring_row(p, i / chn - 3, ch0 + i % chn);
+        for (int i = tid; i < 3 * chn; i += 512) s.hist[(int64_t) (i / chn) * p.chan + ch0 + i % chn] = ring_row(p, i / chn - 3, ch0 + i % chn);
     }
     float downs[2] = {1.0f, 1.0f};
 #pragma unroll
     for (int j = 0; j < KW; ++j) {
-        // a thread a channel: its rows from the first on
-        const int isc = KW == 1 ? tid / 128 : j, n = KW == 1 ? tid % 128 : tid, ch = p.H * p.P + (isc * p.G + group) * p.N + n;
-        float v[L], big = 0.0f;
+        // a thread half a channel: its 32 rows
+        const int half = tid / 256, r0 = 32 * half;
+        const int isc = KW == 1 ? tid / 128 % 2 : j, n = KW == 1 ? tid % 128 : tid % 256, ch = p.H * p.P + (isc * p.G + group) * p.N + n;
+        float v[L / 2], big = 0.0f;
         if (n < p.N) {
             float a0, a1, a2;
             const float w0 = ssm_tap(p, ch, 0), w1 = ssm_tap(p, ch, 1), w2 = ssm_tap(p, ch, 2), w3 = ssm_tap(p, ch, 3), b = p.cb ? p.cb[ch] : 0.0f;
-            if (first >= 3) {
-                a0 = load_q<QT>(p.xbc, (first - 3) * p.xs + ch), a1 = load_q<QT>(p.xbc, (first - 2) * p.xs + ch), a2 = load_q<QT>(p.xbc, (first - 1) * p.xs + ch);
-            } else {
-                a0 = ring_row(p, first - 3, ch), a1 = ring_row(p, first - 2, ch), a2 = ring_row(p, first - 1, ch);      // (first is 0)
-            }
+            auto row = [&](int t) { return load_q<QT>(p.xbc, (first + min(t, here - 1)) * p.xs + ch); };
+            if (half || first >= 3) a0 = row(r0 - 3), a1 = row(r0 - 2), a2 = row(r0 - 1);
+            else a0 = ring_row(p, first - 3, ch), a1 = ring_row(p, first - 2, ch), a2 = ring_row(p, first - 1, ch);      // (first is 0)
 #pragma unroll
-            for (int t = 0; t < L; ++t) v[t] = load_q<QT>(p.xbc, (first + min(t, here - 1)) * p.xs + ch);
+            for (int t = 0; t < L / 2; ++t) v[t] = row(r0 + t);
 #pragma unroll
-            for (int t = 0; t < L; ++t) {
+            for (int t = 0; t < L / 2; ++t) {
                 const float a3 = v[t];
                 const float c = silu(fmaf(w3, a3, fmaf(w2, a2, fmaf(w1, a1, fmaf(w0, a0, b)))));
                 a0 = a1, a1 = a2, a2 = a3;
-                v[t] = t < here ? c : 0.0f;
+                v[t] = r0 + t < here ? c : 0.0f;
                 big = fmaxf(big, fabsf(v[t]));
             }
         } else {
 #pragma unroll
-            for (int t = 0; t < L; ++t) v[t] = 0.0f;
+            for (int t = 0; t < L / 2; ++t) v[t] = 0.0f;
         }
         big = wave_max(big);
         if (lane == 0) part[j][wave] = big;
         __syncthreads();
-        big = KW == 1 ? fmaxf(part[j][2 * isc], part[j][2 * isc + 1]) : fmaxf(fmaxf(part[j][0], part[j][1]), fmaxf(part[j][2], part[j][3]));
-        float up, down;
-        to_half_range(big, up, down);
+        auto most = [&](int from, int n) {
+            float m = 0.0f;
+            for (int i = 0; i < n; ++i) m = fmaxf(m, fmaxf(part[j][from + i], part[j][from + 4 + i]));
+            return m;
+        };
+        float up;
         if constexpr (KW == 1) {
-            float u2;
-            to_half_range(fmaxf(part[j][0], part[j][1]), u2, downs[0]);
-            to_half_range(fmaxf(part[j][2], part[j][3]), u2, downs[1]);
-        } else downs[j] = down;
+            float ups[2];
+            to_half_range(most(0, 2), ups[0], downs[0]);
+            to_half_range(most(2, 2), ups[1], downs[1]);
+            up = isc ? ups[1] : ups[0];
+        } else to_half_range(most(0, 4), up, downs[j]);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int q = 0; q < 4; ++q) {
+            // rows 32 half + 4 q .. + 3 and 16 behind them: an operand's 8
+            float e[8];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                // rows 32 ks + 4 q .. + 3 and 16 behind them: an operand's 8
-                float e[8];
+            for (int i = 0; i < 8; ++i) e[i] = v[16 * (i / 4) + 4 * q + i % 4] * up;
+            s8v hi, lo;
+            split8(e, hi, lo);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = v[32 * ks + 16 * (i / 4) + 4 * q + i % 4] * up;
-                s8v hi, lo;
-                split8(e, hi, lo);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int at = (32 * ks + 16 * (i / 4) + 4 * q + i % 4) * ROW + n;
-                    plane[isc][0][at] = hi[i];
-                    plane[isc][1][at] = lo[i];
-                }
-                if (!isc) {
-                    s8v* to = reinterpret_cast<s8v*>(ops + 2 * op_c(KK)) + ((n / 16) * 2 + ks) * 64 + n % 16 + 16 * q;
-                    to[0] = hi;
-                    to[op_c(KK) / 16] = lo;
-                }
+            for (int i = 0; i < 8; ++i) {
+                const int at = (r0 + 16 * (i / 4) + 4 * q + i % 4) * ROW + n;
+                plane[isc][0][at] = hi[i];
+                plane[isc][1][at] = lo[i];
             }
+            if (!isc) {
+                s8v* to = reinterpret_cast<s8v*>(ops + 2 * op_c(KK)) + ((n / 16) * 2 + half) * 64 + n % 16 + 16 * q;
+                to[0] = hi;
+                to[op_c(KK) / 16] = lo;
+            }
+        }
     }
     if (tid < 2) s.scales[(int64_t) blockIdx.x * 2 + tid] = tid ? downs[1] : downs[0];
     __syncthreads();
     // C as operands: (row, features 32 kk + 4 g .. + 3 and 16 behind them)
+    const int w = wave % 4, h = wave / 4;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const short* src = plane[1][h] + (16 * wave + n16) * ROW + 32 * kk + 4 * g;
-            const s4v a = *reinterpret_cast<const s4v*>(src), b = *reinterpret_cast<const s4v*>(src + 16);
-            reinterpret_cast<s8v*>(ops + h * op_c(KK))[(wave * KK + kk) * 64 + lane] = s8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        }
+    for (int kk = 0; kk < KK; ++kk) {
+        const short* src = plane[1][h] + (16 * w + n16) * ROW + 32 * kk + 4 * g;
+        const s4v a = *reinterpret_cast<const s4v*>(src), b = *reinterpret_cast<const s4v*>(src + 16);
+        reinterpret_cast<s8v*>(ops + h * op_c(KK))[(w * KK + kk) * 64 + lane] = s8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
     // C . B of 16 rows of C against the rows of B that they see: column a row of C, 4 consecutive rows of B a lane
     const float down = downs[0] * downs[1];
-    for (int st = 0; st <= wave; ++st) {
+    for (int st = h; st <= w; st += 2) {
         f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-            const int ab = (16 * st + n16) * ROW + 32 * kk + 8 * g, ac = (16 * wave + n16) * ROW + 32 * kk + 8 * g;
+            const int ab = (16 * st + n16) * ROW + 32 * kk + 8 * g, ac = (16 * w + n16) * ROW + 32 * kk + 8 * g;
             const s8v bh = *reinterpret_cast<const s8v*>(plane[0][0] + ab), bl = *reinterpret_cast<const s8v*>(plane[0][1] + ab);
             const s8v chh = *reinterpret_cast<const s8v*>(plane[1][0] + ac), cl = *reinterpret_cast<const s8v*>(plane[1][1] + ac);
             acc = mfma16<false>(bh, chh, acc);
             acc = mfma16<false>(bl, chh, acc);
             acc = mfma16<false>(bh, cl, acc);
         }
-        reinterpret_cast<f4v*>(ops + 4 * op_c(KK))[((wave * 2 + st / 2) * 64 + lane) * 2 + st % 2] = acc * down;
+        reinterpret_cast<f4v*>(ops + 4 * op_c(KK))[((w * 2 + st / 2) * 64 + lane) * 2 + st % 2] = acc * down;
     }
 }
 
@@ -743,7 +743,7 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
 
 template <int QT, int KW>
 void launch_pass(ns_gpu* g, ScanParams& s, const Plan& q) {
-    ssm_prep_kernel<QT, KW><<<(unsigned) (q.chunks * s.l.G + ((int64_t) q.chunks * s.l.H + 3) / 4), 256, 0, g->q>>>(s);
+    ssm_prep_kernel<QT, KW><<<(unsigned) (q.chunks * s.l.G + ((int64_t) q.chunks * s.l.H + 7) / 8), 512, 0, g->q>>>(s);
     const unsigned owners = (unsigned) (s.l.H * q.blocks);
     if (q.segs > 1) {
         ScanParams f = s;
