@@ -81,6 +81,14 @@ __device__ __forceinline__ void split8(const float (&v)[8], s8v& hi, s8v& lo) {
     lo = half8(r);
 }
 
+// the largest of 4 lanes 16 apart, without the canonicalising copies of fmaxf
+__device__ __forceinline__ float rows_most(float v) {
+    float a, b;
+    pair16(v, a, b);
+    pair32(__builtin_elementwise_maximum(a, b), a, b);
+    return __builtin_elementwise_maximum(a, b);
+}
+
 // the ring's value `at` rows (negative) from the call's first: zeros in front of the sequence, and of taps that there are not
 __device__ __forceinline__ float ring_row(const SsmLayer& p, int64_t at, int ch) {
     return at >= 1 - p.K && p.p0 + at >= 0 ? p.conv[(p.p0 + at) % p.cap * p.chan + ch] : 0.0f;
@@ -234,11 +242,11 @@ __global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
 
 // work-groups a CU: what LDS has room for, and the registers that leaves a wave
 template <int QT, int KW, bool STATE>
-constexpr int SCAN_WGS = KW == 2 ? 1 : STATE ? 4 : QT == 2 ? 3 : 2;
+constexpr int SCAN_WGS = KW == 2 ? 1 : STATE || QT == 2 ? 3 : 2;
 template <int QT, int KW, bool STATE>
 __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kernel(ScanParams s) {
     constexpr int KK = 4 * KW;
-    constexpr bool AHEAD = SCAN_WGS<QT, KW, STATE> <= 2;          // x and the operands asked for early: no third work-group hides their latency
+    constexpr bool AHEAD = STATE || SCAN_WGS<QT, KW, STATE> <= 2;     // x and the operands asked for early, where there are registers for them
     constexpr bool Y3 = QT != 2;                                  // y's products from both halfs of their operands
     // x weighted for the state (hi, lo) and as it is (hi, for Y3 lo): [32 rows][16 columns][lane]; the state: [32 features][..]
     constexpr int WH = 0, WL = 1, XH = 2, XL = 3, PLANES = STATE ? 2 : Y3 ? 4 : 3, HP = STATE ? 0 : Y3 ? 2 : 1;
@@ -359,7 +367,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             for (int i = 0; i < 2 * KW; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) big = __builtin_elementwise_maximum(big, fabsf(st[i][ct][e]));
-            big = rows_max(big);
+            big = rows_most(big);
             if (g == 0) hmax[16 * ct + n][w] = big;
         }
     };
@@ -441,7 +449,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             for (int i = 0; i < 16; ++i) big = __builtin_elementwise_maximum(big, fabsf(x[i / 8][i % 8]));
             auto operands = [&](float big, auto held) {
                 float up, down;
-                to_half_range(rows_max(big), up, down);
+                to_half_range(rows_most(big), up, down);
                 if (g == 0) xs[16 * w + n] = down * LN2;
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
@@ -496,7 +504,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) {
                 const int at = 16 * ct + n;
-                const float most = fmaxf(fmaxf(parts[ct][0], parts[ct][1]), fmaxf(parts[ct][2], parts[ct][3]));
+                const float most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(parts[ct][0], parts[ct][1]), __builtin_elementwise_maximum(parts[ct][2], parts[ct][3]));
                 float up, down;
                 to_half_range(most, up, down);
                 if (w == 0 && g == 0) hs[at] = down;
@@ -516,9 +524,8 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
         }
         if constexpr (!AHEAD && !STATE) fetch_c();
         lds_barrier();
-        if constexpr (AHEAD) {
+        if constexpr (AHEAD)
             if (c + 1 < to) fetch_x(c + 1, lg);
-        } else if constexpr (STATE) fetch_b();
         if constexpr (!STATE) {
             // 16 rows of y: this lane row 16 w + n, columns 16 ct + 4 g .. + 3
             f4v y[4], yi[4];
@@ -539,14 +546,8 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             const int row = 16 * w + ln;
             const float cl = hdr[HDR_C + row];
             float m[2][8], big = 0.0f;
-            const f4v bd = *reinterpret_cast<const f4v*>(hdr + HDR_BD + 4 * w);
             f4v cs[4], dts[4];
-            auto fetch_run = [&](int st) {
-                cs[st] = *reinterpret_cast<const f4v*>(hdr + HDR_C + 16 * st + 4 * lg);
-                dts[st] = *reinterpret_cast<const f4v*>(hdr + HDR_DT + 16 * st + 4 * lg);
-            };
-#pragma unroll
-            for (int st = 0; st < 4 && AHEAD; ++st) fetch_run(st);
+            const f4v bd = *reinterpret_cast<const f4v*>(hdr + HDR_BD + 4 * w);
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
                 float* to_m = m[st / 2] + 4 * (st % 2);
@@ -555,7 +556,8 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                     for (int i = 0; i < 4; ++i) to_m[i] = 0.0f;
                     continue;
                 }
-                if (!AHEAD) fetch_run(st);
+                cs[st] = *reinterpret_cast<const f4v*>(hdr + HDR_C + 16 * st + 4 * lg);
+                dts[st] = *reinterpret_cast<const f4v*>(hdr + HDR_DT + 16 * st + 4 * lg);
                 const float base = cl + bd[st];
                 const f4v cb = cbv[st / 2][st % 2];
 #pragma unroll
@@ -568,10 +570,10 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(to_m[i]));
+                for (int i = 0; i < 4; ++i) big = __builtin_elementwise_maximum(big, fabsf(to_m[i]));
             }
             float up, down;
-            to_half_range(rows_max(big), up, down);
+            to_half_range(rows_most(big), up, down);
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 if (ks > w / 2) break;
@@ -628,6 +630,9 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             const float keep = hdr[HDR_END + 1], sb = scale_b * hdr[HDR_END + 2];
             exponent += hdr[HDR_END];
             s8v ahead[2][2][2];
+            // (in registers of its own, that a product's first step starts from: the compiler would clear each sum apart)
+            f4v zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (!STATE) asm volatile("" : "+v"(zero));
             float fs[4];
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) fs[ct] = xs[16 * ct + n];
@@ -646,7 +651,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                 for (int ks = 0; ks < 2; ++ks) {
                     const s8v hi = ahead[ct % 2][ks][0], lo = ahead[ct % 2][ks][1];
 #pragma unroll
-                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][0], hi, ks ? a[i] : f4v{0.0f, 0.0f, 0.0f, 0.0f});
+                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][0], hi, ks ? a[i] : zero);
 #pragma unroll
                     for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][1], hi, a[i]);
 #pragma unroll
@@ -722,7 +727,7 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
     q.per = (int) ((q.chunks + segs - 1) / segs);
     q.segs = (q.chunks + q.per - 1) / q.per;
     // their states in as many pieces as fill those of the state kernel's, of 4 chunks at least
-    q.sub = q.segs == 1 ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>(q.per / 4, (1024 + owners * (q.segs - 1) - 1) / (owners * (q.segs - 1))));
+    q.sub = q.segs == 1 ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>(q.per / 4, (768 + owners * (q.segs - 1) - 1) / (owners * (q.segs - 1))));
     q.piece = (q.per + q.sub - 1) / q.sub;
     int64_t at = 0;
     auto take = [&](int64_t floats) {
