@@ -496,6 +496,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                 if (g == 0) bad[16 * w + n] = where;
             }
         }
+        if constexpr (!AHEAD && !STATE) fetch_c();
         // this wave's part of the state
         if constexpr (!STATE) {
             f4v parts[4];
@@ -522,7 +523,6 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                 }
             }
         }
-        if constexpr (!AHEAD && !STATE) fetch_c();
         lds_barrier();
         if constexpr (AHEAD)
             if (c + 1 < to) fetch_x(c + 1, lg);
