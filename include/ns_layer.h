@@ -21,13 +21,17 @@ extern "C" {
  *   c = silu(sum over k < K of cw[:][k] u(p - K + 1 + k) + cb)                      -> x, B, C
  *   dt = softplus(step + dtb), held to dt_lo .. dt_hi
  *   h = exp(dt a) h + dt x (outer) B[group],  y = h C[group] + d x                  a head
- * cw [chan][K], cb [chan] or null, a, dtb, d [H] (dtb, d or null), all float32. K 1 to 4, N up to 256, H a multiple of G.
+ * cw [chan][K], cb [chan] or null, a, dtb, d [H] (dtb, d or null), all float32. K 1 to 4, N up to 256, H a multiple of G,
+ * H and P up to 65536, chan up to 2^24. dt_lo and dt_hi: 0 and infinity where the model has no limits.
  * conv: a ring of `cap` raw rows [cap][chan] float32, the row of position p in slot p % cap; the K - 1 rows in front of a
  * call's first have to be there (none in front of position 0 is read: a new sequence needs no clearing). K 1: may be null.
  * State: [H][P][N] float32; h0 is read and h1 written, and they may be the same (h0 null: zeros). */
 
 /* T rows of one sequence at positions p0 .. p0 + T - 1: y [T] rows of H P, h1, and the last min(T, K - 1) raw rows into
- * the ring (cap >= K - 1). scratch: ns_ssm_prompt_scratch(..) floats, 16-byte aligned. N a value up to 256. */
+ * the ring (cap >= K - 1). Rows up to 2^23 values apart (xs). scratch: ns_ssm_prompt_scratch(..) floats, 16-byte aligned:
+ * it grows with T up to 8192 rows. The scan's matrix products keep 22 bits of each operand (half rows too; of bfloat16 rows
+ * those that reach y alone 11) and nothing below 2^-38 of the largest value of a column or block of 64 rows. A value that is
+ * not finite reaches what the recurrence takes it to, rows in front of it never. */
 int64_t ns_ssm_prompt_scratch(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K);
 int ns_ssm_prompt(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt, int64_t dts, const float* cw, const float* cb, const float* a,
                   const float* dtb, const float* d, float dt_lo, float dt_hi, float* conv, int64_t cap, int64_t p0, int64_t T, int64_t H,

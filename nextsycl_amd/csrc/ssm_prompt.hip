@@ -171,7 +171,8 @@ __global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
                 const float c = silu(fmaf(w3, a3, fmaf(w2, a2, fmaf(w1, a1, fmaf(w0, a0, b)))));
                 a0 = a1, a1 = a2, a2 = a3;
                 v[t] = r0 + t < here ? c : 0.0f;
-                big = fmaxf(big, fabsf(v[t]));
+                // (what is not finite has no part in the scale: it would leave the other rows' values none)
+                big = fabsf(v[t]) < __builtin_inff() ? fmaxf(big, fabsf(v[t])) : big;
             }
         } else {
 #pragma unroll

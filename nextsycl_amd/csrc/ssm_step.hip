@@ -221,7 +221,7 @@ int ns_ssm_check(const char* who, ns_gpu* g, int qt, const SsmLayer& p, int64_t 
     if (K < 1 || K > 4) return ns_fail(s + ": 1 to 4 taps");
     if (p.xs < H * P + 2 * G * N || p.dts < H || p.ys < H * P) return ns_fail(s + ": rows at least as far apart as they are long");
     if (!(p.lo <= p.hi)) return ns_fail(s + ": step sizes between dt_lo and dt_hi");
-    if (p.p0 < 0) return ns_fail(s + ": a position in front of the first");
+    if (p.p0 < 0 || p.p0 > INT64_MAX / 2) return ns_fail(s + ": positions from 0 to 2^62");
     if (K > 1 && p.cap < least) return ns_fail(s + ": a ring of at least " + std::to_string(least) + " rows");
     if (!g || !p.xbc || !p.dt || !p.cw || !p.a || !p.h1 || !p.y || (K > 1 && !p.conv)) return ns_fail(s + ": a null buffer");
     return 0;

@@ -185,3 +185,17 @@ def test_the_native_step_makes_the_general_ways_call(name, qt):
     setattr(ops.k, name, lambda *a: other.append(a) or 0)
     getattr(ops, name)(**args, **bufs)
     assert len(other) == 1 and not notes
+
+
+@pytest.mark.parametrize("name,good", [("ns_ssm_prompt", PROMPT), ("ns_ssm_step", STEP)])
+def test_positions_past_any_sequence(lib, name, good):
+    f = getattr(lib, name)
+    assert f(*{**good, "p0": (1 << 62) + 1}.values()) == -1 and "positions" in lib.ns_last_error().decode()
+    assert f(*{**good, "p0": (1 << 62) - 1}.values()) == -1 and lib.ns_last_error().decode() == name + ": a null buffer"
+
+
+def test_rows_too_far_apart_and_scratch_off_its_alignment(lib):
+    g = C.create_string_buffer(1 << 16)        # (a handle that is not looked at: the call ends in front of any use of it)
+    for change, word in ((dict(xs=(1 << 23) + 1), "apart"), (dict(scratch=AT + 4), "aligned")):
+        assert lib.ns_ssm_prompt(*{**PROMPT, "g": C.addressof(g), **change}.values()) == -1
+        assert word in lib.ns_last_error().decode()
