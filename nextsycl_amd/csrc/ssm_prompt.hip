@@ -331,7 +331,9 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
         hdrs[c % 2][tid] = head0;
         if (tid < HDR - 256) hdrs[c % 2][256 + tid] = head1;
     };
-    uint32_t raw[28];
+    // (as they are loaded: widened to 32 bits they would be awaited at once)
+    typedef std::conditional_t<QT == 0, uint32_t, uint16_t> raw_t;
+    raw_t raw[28];
     const int64_t row_bytes = p.xs * (QT ? 2 : 4);
     const uint32_t lane_off = (uint32_t) (4 * g * row_bytes + (int64_t) xch * (QT ? 2 : 4));
     auto fetch_x = [&](int c, int g) {
@@ -342,8 +344,8 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
         const int front = first > 0 ? 3 : 0;
         const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.xbc) + (first - front) * row_bytes), (short) 0, -1, 0x00020000);
         auto at = [&](uint32_t lane_off, uint32_t off) {
-            if constexpr (QT == 0) return (uint32_t) __builtin_amdgcn_raw_buffer_load_b32(rows, lane_off, off, 0);
-            else return (uint32_t) (uint16_t) __builtin_amdgcn_raw_buffer_load_b16(rows, lane_off, off, 0);
+            if constexpr (QT == 0) return (raw_t) __builtin_amdgcn_raw_buffer_load_b32(rows, lane_off, off, 0);
+            else return (raw_t) __builtin_amdgcn_raw_buffer_load_b16(rows, lane_off, off, 0);
         };
         if (front && here == L) {
             uint32_t step = (uint32_t) row_bytes;
@@ -430,9 +432,14 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
 #pragma unroll
                 for (int i = 0; i < 7; ++i) u[i] = raw_value<QT>(raw[7 * j + i]);
                 if (j == 0 && c == 0 && s.t0 == 0) {
-                    // (in front of the call: float32 from the ring, whatever the rows' type)
+                    // (in front of the call: float32 from the ring, whatever the rows' type; awaited here, or every chunk would
+                    // wait for all that it has asked for where the two ways meet)
+                    float old[3];
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) u[i] = lg == 0 ? s.hist[(int64_t) i * p.chan + xch] : u[i];
+                    for (int i = 0; i < 3; ++i) old[i] = s.hist[(int64_t) i * p.chan + xch];
+                    asm volatile("" : "+v"(old[0]), "+v"(old[1]), "+v"(old[2]));
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) u[i] = lg == 0 ? old[i] : u[i];
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
