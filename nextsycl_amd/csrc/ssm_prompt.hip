@@ -44,6 +44,7 @@ constexpr int64_t op_bytes(int kk) { return 4 * op_c(kk) + 16 * 1024; }
 struct ScanParams {
     SsmLayer l;
     int64_t t0, all;            // the pass's first row, the call's rows
+    int64_t slot0;              // the ring's slot of the call's first row
     int T, chunks, segs, per;   // rows and chunks of the pass; segments, chunks a segment
     int sub, piece;             // pieces a segment whose states are found apart, chunks a piece
     int blocks, vec_y, vec_h;   // blocks of 64 features a head; y in pieces of 4 values, the state too
@@ -90,8 +91,11 @@ __device__ __forceinline__ float rows_most(float v) {
 }
 
 // the ring's value `at` rows (negative) from the call's first: zeros in front of the sequence, and of taps that there are not
-__device__ __forceinline__ float ring_row(const SsmLayer& p, int64_t at, int ch) {
-    return at >= 1 - p.K && p.p0 + at >= 0 ? p.conv[(p.p0 + at) % p.cap * p.chan + ch] : 0.0f;
+__device__ __forceinline__ float ring_row(const ScanParams& s, int at, int ch) {
+    const SsmLayer& p = s.l;
+    if (at < 1 - p.K || p.p0 + at < 0) return 0.0f;
+    const int64_t slot = s.slot0 + at;                         // (the ring has K - 1 slots at least)
+    return p.conv[(slot < 0 ? slot + p.cap : slot) * p.chan + ch];
 }
 
 // a row's value out of its bits
@@ -130,26 +134,26 @@ __device__ __forceinline__ void ssm_header(const ScanParams& s, int chunk, int h
 
 template <int QT, int KW>
 __global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
-    constexpr int NP = 128 * KW, KK = 4 * KW, ROW = NP + 8;
-    __shared__ __align__(16) short plane[2][2][L * ROW];       // [B, C][hi, lo][row][feature]
+    constexpr int NP = 128 * KW, KK = 4 * KW, ROW = L + 4;     // (34 words: a column of LDS banks on for each feature)
+    __shared__ __align__(16) short plane[2][2][NP * ROW];      // [B, C][hi, lo][feature][row]
     __shared__ float part[2][8];
     const SsmLayer& p = s.l;
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n16 = lane % 16, g = lane / 16;
     if ((int) blockIdx.x >= s.chunks * p.G) {
         // work-groups behind those: headers, a wave a (chunk, head)
-        const int64_t i = (int64_t) (blockIdx.x - s.chunks * p.G) * 8 + wave;
-        if (i < (int64_t) s.chunks * p.H) ssm_header<QT>(s, (int) (i / p.H), (int) (i % p.H), lane);
+        const int64_t i = (int64_t) (blockIdx.x - s.chunks * p.G) * 8 + wave, heads = (int64_t) s.chunks * p.H;
+        if (i < heads) ssm_header<QT>(s, (int) (i / p.H), (int) (i % p.H), lane);
+        else if (s.t0 == 0) {
+            // and x's rows in front of the call, for the scan: the ring is written while that runs
+            const int64_t at = (i - heads) * 64 + lane, inner = (int64_t) p.H * p.P;
+            if (at < 3 * inner) s.hist[at / inner * p.chan + at % inner] = ring_row(s, (int) (at / inner) - 3, (int) (at % inner));
+        }
         return;
     }
-    const int chunk = blockIdx.x / p.G, group = blockIdx.x % p.G, per = p.H / p.G;
+    const int chunk = blockIdx.x / p.G, group = blockIdx.x % p.G;
     const int here = min(L, s.T - chunk * L);
     const int64_t first = s.t0 + (int64_t) chunk * L;
     uint8_t* ops = s.ops + (int64_t) blockIdx.x * op_bytes(KK);
-    // the rows in front of the call, for the scan's x: the ring is written while that runs
-    if (first == 0) {
-        const int ch0 = group * per * p.P, chn = per * p.P;
-        for (int i = tid; i < 3 * chn; i += 512) s.hist[(int64_t) (i / chn) * p.chan + ch0 + i % chn] = ring_row(p, i / chn - 3, ch0 + i % chn);
-    }
     float downs[2] = {1.0f, 1.0f};
 #pragma unroll
     for (int j = 0; j < KW; ++j) {
@@ -162,7 +166,7 @@ __global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
             const float w0 = ssm_tap(p, ch, 0), w1 = ssm_tap(p, ch, 1), w2 = ssm_tap(p, ch, 2), w3 = ssm_tap(p, ch, 3), b = p.cb ? p.cb[ch] : 0.0f;
             auto row = [&](int t) { return load_q<QT>(p.xbc, (first + min(t, here - 1)) * p.xs + ch); };
             if (half || first >= 3) a0 = row(r0 - 3), a1 = row(r0 - 2), a2 = row(r0 - 1);
-            else a0 = ring_row(p, first - 3, ch), a1 = ring_row(p, first - 2, ch), a2 = ring_row(p, first - 1, ch);      // (first is 0)
+            else a0 = ring_row(s, -3, ch), a1 = ring_row(s, -2, ch), a2 = ring_row(s, -1, ch);      // (first is 0)
 #pragma unroll
             for (int t = 0; t < L / 2; ++t) v[t] = row(r0 + t);
 #pragma unroll
@@ -202,10 +206,10 @@ __global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
             s8v hi, lo;
             split8(e, hi, lo);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = (r0 + 16 * (i / 4) + 4 * q + i % 4) * ROW + n;
-                plane[isc][0][at] = hi[i];
-                plane[isc][1][at] = lo[i];
+            for (int i = 0; i < 8; i += 4) {
+                const int at = n * ROW + r0 + 4 * i + 4 * q;
+                *reinterpret_cast<s4v*>(plane[isc][0] + at) = s4v{hi[i], hi[i + 1], hi[i + 2], hi[i + 3]};
+                *reinterpret_cast<s4v*>(plane[isc][1] + at) = s4v{lo[i], lo[i + 1], lo[i + 2], lo[i + 3]};
             }
             if (!isc) {
                 s8v* to = reinterpret_cast<s8v*>(ops + 2 * op_c(KK)) + ((n / 16) * 2 + half) * 64 + n % 16 + 16 * q;
@@ -216,23 +220,22 @@ __global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
     }
     if (tid < 2) s.scales[(int64_t) blockIdx.x * 2 + tid] = tid ? downs[1] : downs[0];
     __syncthreads();
-    // C as operands: (row, features 32 kk + 4 g .. + 3 and 16 behind them)
+    // 16 rows of a plane as operands: (row, features 32 kk + 4 g .. + 3 and 16 behind them)
+    auto operand = [&](short* from, int tile, int kk) {
+        short* at = from + (32 * kk + 4 * g + n16 / 4) * ROW + 16 * tile + 4 * (n16 % 4);
+        const s4v a = lds_read_tr16(at), b = lds_read_tr16(at + 16 * ROW);
+        return s8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    };
     const int w = wave % 4, h = wave / 4;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-        const short* src = plane[1][h] + (16 * w + n16) * ROW + 32 * kk + 4 * g;
-        const s4v a = *reinterpret_cast<const s4v*>(src), b = *reinterpret_cast<const s4v*>(src + 16);
-        reinterpret_cast<s8v*>(ops + h * op_c(KK))[(w * KK + kk) * 64 + lane] = s8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    }
+    for (int kk = 0; kk < KK; ++kk) reinterpret_cast<s8v*>(ops + h * op_c(KK))[(w * KK + kk) * 64 + lane] = operand(plane[1][h], w, kk);
     // C . B of 16 rows of C against the rows of B that they see: column a row of C, 4 consecutive rows of B a lane
     const float down = downs[0] * downs[1];
     for (int st = h; st <= w; st += 2) {
         f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-            const int ab = (16 * st + n16) * ROW + 32 * kk + 8 * g, ac = (16 * w + n16) * ROW + 32 * kk + 8 * g;
-            const s8v bh = *reinterpret_cast<const s8v*>(plane[0][0] + ab), bl = *reinterpret_cast<const s8v*>(plane[0][1] + ab);
-            const s8v chh = *reinterpret_cast<const s8v*>(plane[1][0] + ac), cl = *reinterpret_cast<const s8v*>(plane[1][1] + ac);
+            const s8v bh = operand(plane[0][0], st, kk), bl = operand(plane[0][1], st, kk), chh = operand(plane[1][0], w, kk), cl = operand(plane[1][1], w, kk);
             acc = mfma16<false>(bh, chh, acc);
             acc = mfma16<false>(bl, chh, acc);
             acc = mfma16<false>(bh, cl, acc);
@@ -756,7 +759,8 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
 
 template <int QT, int KW>
 void launch_pass(ns_gpu* g, ScanParams& s, const Plan& q) {
-    ssm_prep_kernel<QT, KW><<<(unsigned) (q.chunks * s.l.G + ((int64_t) q.chunks * s.l.H + 7) / 8), 512, 0, g->q>>>(s);
+    const int64_t waves = (int64_t) q.chunks * s.l.H + (s.t0 ? 0 : (3 * (int64_t) s.l.H * s.l.P + 63) / 64);
+    ssm_prep_kernel<QT, KW><<<(unsigned) (q.chunks * s.l.G + (waves + 7) / 8), 512, 0, g->q>>>(s);
     const unsigned owners = (unsigned) (s.l.H * q.blocks);
     if (q.segs > 1) {
         ScanParams f = s;
@@ -771,7 +775,7 @@ void run_prompt(ns_gpu* g, const SsmLayer& p, int64_t T, float* scratch) {
     for (int64_t t0 = 0; t0 < T; t0 += PASS_ROWS) {
         const int64_t n = std::min(PASS_ROWS, T - t0);
         const Plan q = plan_of(n, p.H, p.P, p.N, p.G, p.N <= 128 ? SCAN_WGS<QT, 1, false> : SCAN_WGS<QT, 2, false>);
-        ScanParams s{p, t0, T, (int) n, q.chunks, q.segs, q.per, q.sub, q.piece, q.blocks};
+        ScanParams s{p, t0, T, p.p0 % p.cap, (int) n, q.chunks, q.segs, q.per, q.sub, q.piece, q.blocks};
         s.vec_y = (uintptr_t) p.y % (QT ? 8 : 16) == 0 && p.ys % 4 == 0 && p.P % 4 == 0;
         s.vec_h = p.N % 4 == 0 && (uintptr_t) p.h0 % 16 == 0 && (uintptr_t) p.h1 % 16 == 0;
         s.ops = reinterpret_cast<uint8_t*>(scratch + q.ops);
