@@ -31,7 +31,7 @@ namespace {
 
 constexpr int L = 64;                     // rows a chunk
 constexpr int64_t PASS_ROWS = 8192;       // rows a pass works on: what bounds the scratch
-constexpr int MOST_SEGS = 8;
+constexpr int MOST_SEGS = 32;
 // a chunk and head's header: exponents (base 2) from the start of each run of 16 rows, step sizes, weights in the chunk's
 // state, decays from the chunk's start; differences between runs' starts [4][4], the whole chunk's exponent and decay, what the weights are
 // to be multiplied with
@@ -733,11 +733,15 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
     q.chunks = (int) ((T + L - 1) / L);
     q.blocks = (int) ((P + 63) / 64);
     const int64_t owners = H * q.blocks;
-    // as many segments as fill the chip's places for the scan's work-groups, of 4 chunks at least
-    const int64_t segs = std::max<int64_t>(1, std::min<int64_t>({MOST_SEGS, 256 * wgs / owners, q.chunks / 4}));
+    // as many segments as fill the chip's places for the scan's work-groups, of 2 chunks at least. (Rows of 32 heads of 64 x 128: 512
+    // 46.7 us in segments of 4 chunks, 33.1 in those of 2, and 256 rows, left whole, 30.0 - in two segments 32.4; 8192 rows of
+    // 8 heads of 64 x 64 99.9 us with up to 8 segments, 56.4 with up to 32, 69.8 with 64: a segment's start walks the states in
+    // front of it)
+    const int64_t segs = std::max<int64_t>(1, std::min<int64_t>({MOST_SEGS, 256 * wgs / owners, q.chunks < 6 ? 1 : q.chunks / 2}));
     q.per = (int) ((q.chunks + segs - 1) / segs);
     q.segs = (q.chunks + q.per - 1) / q.per;
-    // their states in as many pieces as fill those of the state kernel's, of 4 chunks at least
+    // their states in as many pieces as fill those of the state kernel's, of 4 chunks at least (2: 2051 rows of 64 heads 75.8 us for
+    // 73.3)
     q.sub = q.segs == 1 ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>(q.per / 4, (768 + owners * (q.segs - 1) - 1) / (owners * (q.segs - 1))));
     q.piece = (q.per + q.sub - 1) / q.sub;
     int64_t at = 0;
