@@ -19,6 +19,30 @@ namespace {
 
 constexpr int64_t MOST_ROWS = 4096;
 
+// The sums over each run of LR lanes of U values, value lane / (LR / U) in a lane: at each step two values' halves of the run
+// change places, so that U values take U - 1 additions (and as many exchanges) until one a lane is left, not U each
+template <int LR, int U>
+__device__ __forceinline__ float lanes_sums(const float (&v)[U], int lane) {
+    if constexpr (U == 1) return lanes_sum<LR>(v[0]);
+    else {
+        float w[U / 2];
+#pragma unroll
+        for (int u = 0; u < U / 2; ++u) {
+            const float a = v[u], b = v[u + U / 2];
+            if constexpr (LR >= 32) {
+                const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+                const auto r = LR == 64 ? __builtin_amdgcn_permlane32_swap(x, y, false, false) : __builtin_amdgcn_permlane16_swap(x, y, false, false);
+                w[u] = __builtin_bit_cast(float, (uint32_t) r[0]) + __builtin_bit_cast(float, (uint32_t) r[1]);
+            } else {
+                const bool upper = lane & LR / 2;
+                const float mine = upper ? b : a, other = upper ? a : b;
+                w[u] = mine + __builtin_bit_cast(float, dpp_u32<LR == 16 ? 0x140 : LR == 8 ? 0x141 : 0x4E>(__builtin_bit_cast(uint32_t, other)));
+            }
+        }
+        return lanes_sums<LR / 2, U / 2>(w, lane);
+    }
+}
+
 struct StepParams {
     SsmLayer l;
     const int32_t *pos, *slots;
@@ -28,7 +52,7 @@ struct StepParams {
 
 // LR lanes a state row, U rows a lane; VEC: a lane's 4 floats as one piece
 template <int QT, int LR, int U, bool VEC>
-__global__ __launch_bounds__(256) void ssm_step_kernel(StepParams s) {
+__global__ __launch_bounds__(256, 4) void ssm_step_kernel(StepParams s) {
     constexpr int RW = 256 / LR, PB = RW * U, AHEAD = 4, NMAX = 4 * LR, CH = (2 * NMAX + PB + 255) / 256;
     __shared__ __align__(16) float row_in[AHEAD][2 * NMAX + PB];      // B, C, the block's x of a row
     __shared__ float step[AHEAD][2];                                  // its step size and decay
@@ -158,23 +182,19 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(StepParams s) {
         for (int a = 0; a < rows; ++a) {
             const float dt = step[a][0], decay = step[a][1];
             const float4 b = *reinterpret_cast<const float4*>(row_in[a] + n0), c = *reinterpret_cast<const float4*>(row_in[a] + NMAX + n0);
-            // (the sums of a lane's U state rows side by side; lane u of a row's lanes then writes the one of row u)
-            float sum[U], x[U], out = 0.0f;
+            const float bx = dt * b.x, by = dt * b.y, bz = dt * b.z, bw = dt * b.w;
+            float sum[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                x[u] = row_in[a][2 * NMAX + tid / LR + u * RW];
-                const float dx = dt * x[u];
-                h[u][0] = fmaf(h[u][0], decay, dx * b.x), h[u][1] = fmaf(h[u][1], decay, dx * b.y);
-                h[u][2] = fmaf(h[u][2], decay, dx * b.z), h[u][3] = fmaf(h[u][3], decay, dx * b.w);
-                sum[u] = fmaf(h[u][0], c.x, h[u][1] * c.y) + fmaf(h[u][2], c.z, h[u][3] * c.w);
+                const float x = row_in[a][2 * NMAX + tid / LR + u * RW];
+                h[u][0] = fmaf(h[u][0], decay, x * bx), h[u][1] = fmaf(h[u][1], decay, x * by);
+                h[u][2] = fmaf(h[u][2], decay, x * bz), h[u][3] = fmaf(h[u][3], decay, x * bw);
+                sum[u] = fmaf(h[u][3], c.w, fmaf(h[u][2], c.z, fmaf(h[u][1], c.y, h[u][0] * c.x)));
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                sum[u] = fmaf(skip, x[u], lanes_sum<LR>(sum[u]));
-                out = tid % LR == u ? sum[u] : out;
-            }
-            const int mine_p = prow + tid % LR * RW;
-            if (tid % LR < U && mine_p < p.P) store_o<QT>(p.y, row_of(i0 + a) * p.ys + head * p.P + mine_p, out);
+            // (a lane then holds the sum of one of its U state rows; the first of those that hold the same one writes it)
+            const int mine_u = tid % LR / (LR / U), mine_p = prow + mine_u * RW;
+            const float out = fmaf(skip, row_in[a][2 * NMAX + tid / LR + mine_u * RW], lanes_sums<LR, U>(sum, lane));
+            if (tid % (LR / U) == 0 && mine_p < p.P) store_o<QT>(p.y, row_of(i0 + a) * p.ys + head * p.P + mine_p, out);
         }
     }
 #pragma unroll
