@@ -43,7 +43,7 @@ int ns_ssm_prompt(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt
  * pos[r] (pos null: p0). Every row goes into its slot's ring, so a sequence can be taken back to any row of the call whose
  * state the caller kept (h0 and h1 apart). A slot takes up to cap - K + 1 rows a call (cap >= K): the ring holds the rows
  * in front of them at the same time; rows of a slot beyond that are passed over too. Slots that have no row: nothing of
- * theirs is written. */
+ * theirs is written. A row's results have the same bits in a call of its own and among others. */
 int ns_ssm_step(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt, int64_t dts, const float* cw, const float* cb, const float* a,
                 const float* dtb, const float* d, float dt_lo, float dt_hi, float* conv, int64_t cap, int64_t p0, const int32_t* pos,
                 const int32_t* slots, int64_t nslots, int64_t R, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K, const float* h0,
@@ -75,7 +75,8 @@ int64_t ns_q4_bytes(int64_t M, int64_t K, int64_t group);
  * bytes apart. */
 int ns_q4_pack(ns_gpu* g, int form, const void* src, int64_t ss, int64_t M, int64_t K, int64_t group, void* w);
 /* y [T][M] = x [T][K] . w^T, 1 to 16 rows (a token, or a verify pass's rows), rows of type qt. The weights are exact in
- * the products; float32 rows enter as two halfs (22 bits), bfloat16 and half rows as they are. K up to 2^22. */
+ * the products; float32 rows enter as two halfs (22 bits), bfloat16 and half rows as they are. K up to 2^22. A row has the
+ * same bits alone and among others. */
 int ns_q4_product(ns_gpu* g, int qt, const void* x, int64_t xs, const void* w, int64_t group, void* y, int64_t ys, int64_t T, int64_t M, int64_t K);
 
 #ifdef __cplusplus

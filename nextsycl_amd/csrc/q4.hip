@@ -9,7 +9,7 @@
 // two a (row, tile) that puts the largest at 2^13 (no overflow, and nothing lost above 2^-37 of the largest): bfloat16 rows
 // then fit as they are, float32 rows as two halfs (22 bits, two matrix instructions), half rows need neither.
 //
-// A work-group of 8 waves takes 16 outputs and shares K among its waves, tile by tile; the waves' sums meet in LDS in a
+// A work-group of 8 or 16 waves takes 16 outputs and shares K among its waves, tile by tile; the waves' sums meet in LDS in a
 // fixed order. Rows that fit its LDS as operands are laid out there by each work-group, while its first weights are on
 // their way; longer ones once, by a kernel in front, in the library's own scratch.
 #include <algorithm>
@@ -23,8 +23,9 @@
 
 namespace {
 
-constexpr int WAVES = 8, PF = 1, LDS_ROWS = 64 * 1024;
+constexpr int PF = 1, LDS_ROWS = 64 * 1024;
 
+constexpr int WIDE_M = 4096;
 constexpr int64_t q4_tile_bytes(int64_t group) { return 1024 + 16 * (128 / group) * 2; }
 
 struct Q4Params {
@@ -95,9 +96,9 @@ __global__ __launch_bounds__(256) void q4_rows_kernel(Q4Params p) {
     q4_rows<QT>(p, task / p.T, task % p.T, threadIdx.x % 16, xo, reinterpret_cast<float*>(xo + q4_plane<QT>(p) * PLANES<QT>));
 }
 
-// GR: groups a tile (4, 2, 1); MEM: the rows' operands lie in memory, else in LDS
-template <int QT, int GR, bool MEM>
-__global__ __launch_bounds__(64 * WAVES, MEM ? 2 : 4) void q4_product_kernel(Q4Params p) {
+// GR: groups a tile (4, 2, 1); MEM: the rows' operands lie in memory, else in LDS; WAVES: 8, or 16
+template <int QT, int GR, bool MEM, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, MEM && WAVES == 8 ? 2 : 4) void q4_product_kernel(Q4Params p) {
     constexpr int TILE = 1024 + 32 * GR, SW = 2 * GR;             // SW: a lane's scales, in words
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, g = lane / 16;
@@ -108,7 +109,9 @@ __global__ __launch_bounds__(64 * WAVES, MEM ? 2 : 4) void q4_product_kernel(Q4P
     const uint8_t* wt = p.w + (int64_t) blockIdx.x * p.kt * TILE;
     f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
     // a wave's next tiles: their nibbles, scales, and the rows' operands where those come from memory
-    constexpr int XS = MEM ? 4 : 1, XP = MEM ? PLANES<QT> : 1;
+    // (16 waves: not float32 rows' two planes where a tile has several groups, for which there are no registers)
+    constexpr bool XAHEAD = MEM && !(WAVES == 16 && PLANES<QT> == 2 && GR > 1);
+    constexpr int XS = XAHEAD ? 4 : 1, XP = XAHEAD ? PLANES<QT> : 1;
     struct Ahead {
         uint4 nib[PF];
         uint32_t sc[PF][SW];
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(64 * WAVES, MEM ? 2 : 4) void q4_product_kernel(Q4P
             const uint32_t* ss = reinterpret_cast<const uint32_t*>(tile + 1024 + g * 8 * GR);
 #pragma unroll
             for (int j = 0; j < SW; ++j) f.sc[i][j] = ss[j];
-            if constexpr (MEM) {
+            if constexpr (XAHEAD) {
                 const s8v* x = xo + ((int64_t) kl * 16 + g) * p.T + col;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -145,7 +148,7 @@ __global__ __launch_bounds__(64 * WAVES, MEM ? 2 : 4) void q4_product_kernel(Q4P
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const s8v a = q4_operand(words[j]);
-                if constexpr (MEM) {
+                if constexpr (XAHEAD) {
 #pragma unroll
                     for (int h = 0; h < XP; ++h) s = mfma16<false>(a, f.x[i][j][h], s);
                 } else {
@@ -162,7 +165,7 @@ __global__ __launch_bounds__(64 * WAVES, MEM ? 2 : 4) void q4_product_kernel(Q4P
                     s = f4v{0.0f, 0.0f, 0.0f, 0.0f};
                 }
             }
-            const float down = QT == 1 ? 1.0f : MEM ? f.down[i] : xscale[kl * p.T + col];
+            const float down = QT == 1 ? 1.0f : XAHEAD ? f.down[i] : xscale[kl * p.T + col];
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] = QT == 1 ? acc[e] + tile[e] : fmaf(down, tile[e], acc[e]);
         }
@@ -234,19 +237,26 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(int form, const void* src,
 
 bool q4_group(int64_t group) { return group == 32 || group == 64 || group == 128; }
 
-template <int QT, int GR>
+template <int QT, int GR, int WAVES>
 int launch_product(ns_gpu* g, Q4Params& p) {
     const int64_t rows = (int64_t) p.kt * p.T * (256 * PLANES<QT> + 4), sums = WAVES * 64 * sizeof(f4v);
     const unsigned grid = (unsigned) ((p.M + 15) / 16);
     if (rows <= LDS_ROWS) {
-        q4_product_kernel<QT, GR, false><<<grid, 64 * WAVES, std::max(rows, sums), g->q>>>(p);
+        q4_product_kernel<QT, GR, false, WAVES><<<grid, 64 * WAVES, std::max(rows, sums), g->q>>>(p);
         return 0;
     }
     if ((size_t) (rows + 3) / 4 > ns_own_floats(g)) return ns_fail("ns_q4_product: more scratch than the library has");
     p.ops = reinterpret_cast<uint8_t*>(g->own_scratch);
     q4_rows_kernel<QT><<<(unsigned) ((p.kt * p.T + 15) / 16), 256, 0, g->q>>>(p);
-    q4_product_kernel<QT, GR, true><<<grid, 64 * WAVES, sums, g->q>>>(p);
+    q4_product_kernel<QT, GR, true, WAVES><<<grid, 64 * WAVES, sums, g->q>>>(p);
     return 0;
+}
+// 16 waves where each work-group has a CU of its own (up to 256 of them: 4096 outputs), else 8: a row x 4096 outputs of 8192 half inputs
+// 6.81 us with 8 waves, 5.96 with 16; 8 float32 rows of them 11.0 and 10.2 - 10.7; 2 half rows x 8192 of 5120 7.85 and 9.10, a row
+// x 18560 of 4096 11.1 and 16.5. Whatever the rows' number, so that a row has the same bits alone and among others
+template <int QT, int GR>
+int launch_product(ns_gpu* g, Q4Params& p) {
+    return p.M <= WIDE_M ? launch_product<QT, GR, 16>(g, p) : launch_product<QT, GR, 8>(g, p);
 }
 template <int QT>
 int launch_product(ns_gpu* g, Q4Params& p, int64_t group) {

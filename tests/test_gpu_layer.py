@@ -393,3 +393,22 @@ def test_wrappers_check_their_buffers(ops):
                  lambda: ops.q4_product(-1, b, 16, b, 32, b, 16, 1, 16, 16)):
         with pytest.raises(Error, match="rows of type"):
             call()
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("qt", TYPES)
+@pytest.mark.parametrize("M,K", [(40, 4100), (4112, 4096), (1000, 9000)])
+def test_a_q4_products_row_alone_and_among_others(ops, qt, group, M, K):
+    """A verify pass's rows have the bits of their own tokens' passes, whether the rows' operands fit LDS or not."""
+    g, T = ops.gpu, 16
+    wb = DevBuf.of(g, random_q4(M, K, group, 3))
+    raw, _ = to_type(qt, np.random.default_rng(8).standard_normal((T, K)))
+    rows, y = DevBuf.of(g, raw), DevBuf(g, T * M * E[qt])
+    whole = None
+    for n in (16, 5, 1):
+        for t in range(0, T, n):
+            m = min(n, T - t)
+            ops.q4_product(qt, rows.view(t * K * E[qt], m * K * E[qt]), K, wb, group, y.view(t * M * E[qt], m * M * E[qt]), M, m, M, K)
+        got = y.read(np.uint8)
+        whole = got if whole is None else whole
+        assert np.array_equal(got, whole), n

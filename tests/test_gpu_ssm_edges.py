@@ -187,3 +187,27 @@ def test_two_prompts_at_once(ops):
         del calls, c
     finally:
         other.close()
+
+
+@pytest.mark.parametrize("qt", [F32, F16, BF16])
+@pytest.mark.parametrize("H,P,N", [(4, 80, 128), (2, 50, 100), (2, 16, 16)])
+def test_a_verify_passes_rows_are_their_tokens(ops, qt, H, P, N):
+    """Seven successive rows of a slot in one call, among another slot's, against seven calls of a row: the same bits."""
+    g, R, cap, e = ops.gpu, 7, 16, E[qt]
+    L = Layer(H, P, N, 1, 4, seed=11)
+    raw, _ = rows_of(L, qt, 2 * R, 12)
+    row, of = L.chan + L.H, lambda a: DevBuf.of(g, a)  # noqa: E731
+    w, rows = tuple(of(a) for a in (L.cw, L.cb, L.a, L.dtb, L.d)), of(raw)
+    r = np.random.default_rng(13)
+    h0, ring0 = r.standard_normal((2, H, P, N)).astype(np.float32), r.standard_normal((2, cap, L.chan)).astype(np.float32)
+    slots, pos = np.array([0, 1] * R, np.int32), np.repeat(np.arange(R, dtype=np.int32), 2) + np.array([40, 7] * R, np.int32)
+    out = []
+    for n in (2 * R, 2):
+        h, ring, y = of(h0), of(ring0), DevBuf(g, 2 * R * L.inner * e)
+        for t in range(0, 2 * R, n):
+            at = lambda o: rows.view((t * row + o) * e, rows.len - (t * row + o) * e)  # noqa: E731,B023
+            ops.ssm_step(qt, at(0), row, at(L.chan), row, *w, ring, cap, 0, n, H, P, N, 1, 4, h, h, y.view(t * L.inner * e, n * L.inner * e), L.inner, nslots=2,
+                         slots=of(slots[t:t + n]), pos=of(pos[t:t + n]))
+            g.sync()
+        out.append((y.read(np.uint8), h.read(np.uint8), ring.read(np.uint8)))
+    assert all(np.array_equal(a, b) for a, b in zip(*out))
