@@ -9,16 +9,27 @@
 // instructions a product drop nothing above 2^-22; sums, states and scales are float32. (bfloat16 rows: the products that
 // reach y alone take their operands' first halfs, 2^-11 beside the rows' own rounding of 2^-8.)
 //
-// ssm_prep_kernel, a work-group a (chunk, group): convolves B and C, lays them out as operands, multiplies them, and sums
-// the exponents (in 64 bits; what the exponentials see is a difference within 16 rows, plus one between such runs).
+// ssm_prep_kernel, 8 waves a (chunk, group): convolves B and C (a thread half a channel's rows), leaves them in LDS as [feature]
+// [row] - an operand's rows are a thread's own, C's come back through transposing reads - and multiplies them; the work-groups
+// behind sum the exponents (in 64 bits; what the exponentials see is a difference within 16 rows, plus one between such runs).
 // ssm_scan_kernel, a work-group a (head, 64 of its features, segment of the prompt): walks its chunks with the state in
 // the accumulators of 4 waves, wave w rows 32 w .. 32 w + 31 of it. In a chunk wave w convolves 16 columns of x into the
 // operands that all read (LDS), splits its part of the state into another, then takes 16 rows of y and its part of h'. Matrix
 // results come as (column, 4 consecutive rows) a lane, operands go in as (row or column, 8 values of the summed index) a
 // lane; the summed index may come in any order that both sides share, so in runs of 4 of two neighbouring tiles a result
-// is an operand as it stands: neither the state nor C . B is ever moved between lanes.
-// Where heads alone do not fill the chip the prompt is cut in segments: the same kernel first leaves each segment's state from a
-// start of zero (STATE: a third of the work), and each segment's scan starts from those before it, decayed.
+// is an operand as it stands: neither the state nor C . B is ever moved between lanes. A wave's barriers wait for LDS alone:
+// what it has asked memory for stays on its way.
+// Where heads alone do not fill the chip the prompt is cut in segments: the same kernel first leaves the states of their
+// pieces from a start of zero (STATE: half of the work), and each segment's scan starts from those before it, decayed.
+//
+// Bound: vector instructions. 8192 bfloat16 rows of 128 heads of 64 x 128 (308 MB in and out: 60 us at a copy's rate; 85 GFLOP as
+// executed: 75 us at a large product's) take 297 - 305 us: 42 in the first kernel (134 MB: 26 us), 89 for the segments' states, 175 for the
+// scan - of x's convolution, the splits, the decays and the state's scaling and sums 8 to 11 vector instructions a matrix
+// instruction, in three waves a SIMD that spend 24 % of their life issuing one, 31 % ready for it and the rest at barriers and
+// loads (matrix unit 20 % busy). 2051 float32 rows of 64 heads 73 us (10 + 22 + 43), 85 half rows of 128 heads of 80 24 us:
+// two launches and two chunks of 5 us each. Work-groups a CU, 8192 bfloat16 rows: three of the scan 297 us, two - with x and
+// the operands asked for a chunk ahead, for which they have the registers - 309; of the segments' states three, with that, 297, four without it 304, two
+// 298. Float32 and half rows have both halfs of each operand in LDS, and so two.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -5,8 +5,11 @@
 // touches. Bound: HBM - the state is read and written once (8 H P N bytes a sequence, 8.4 MB at 128 heads of 64 x 128) for
 // 5 operations a float. So a lane holds 4 consecutive features of a few of the head's P rows, asks for them before anything
 // else, and the convolution (a few hundred channels, each group's B and C by every head of the group: 4 multiply-adds and
-// a few KB that the cache holds) runs while they are on their way; y is a sum over a row's lanes, by DPP. Rows of one slot
-// are walked with the state in registers.
+// a few KB that the cache holds) runs while they are on their way; y is a sum over a row's lanes. Rows of one slot
+// are walked with the state in registers, their convolutions four rows at a time.
+// 128 heads of 64 x 128: 64 tokens (548 MB) 107 - 109 us, 5.1 TB/s - a copy's rate; one token 5.6 us, a launch and the two latencies of
+// its loads and sums (1.6 us of bytes); 12 half rows of 3 slots, 128 heads of 80 x 128, 15.8 us (33 MB: 6.3), four work-groups a CU;
+// with three 17.0, with two rows at a time 16.5.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -225,6 +228,8 @@ void launch_step(ns_gpu* g, StepParams& s, bool vec) {
     if (N <= 16) launch_step<QT, 4, 1>(g, s, vec);
     else if (N <= 32) launch_step<QT, 8, 2>(g, s, vec);
     else if (N <= 64) launch_step<QT, 16, 4>(g, s, vec);
+    // (8 state rows a lane, but 4 while there is no work-group of 8 for each CU: a token 5.98 us with 8, 5.54 with 4; 64 tokens 107 and 115, 12 rows of 3 slots of 80 wide heads 15.8 and 16.4)
+    else if (N <= 128 && (int64_t) s.l.H * ((s.l.P + 63) / 64) * s.R <= 128) launch_step<QT, 32, 4>(g, s, vec);
     else if (N <= 128) launch_step<QT, 32, 8>(g, s, vec);
     else launch_step<QT, 64, 4>(g, s, vec);
 }
