@@ -67,23 +67,23 @@ __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log
 // way out stay in flight across it (a __syncthreads waits for both)
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// the sum over each run of L lanes (L a power of two up to 64), in every lane of the run
+// the sum over each run of L lanes (L a power of two up to 64), in every lane of the run: the run's halves first, then theirs
 template <int L>
 __device__ __forceinline__ float lanes_sum(float v) {
     auto add = [&](auto c) { v += __builtin_bit_cast(float, dpp_u32<decltype(c)::value>(__builtin_bit_cast(uint32_t, v))); };
-    if constexpr (L >= 2) add(std::integral_constant<int, 0xB1>());
-    if constexpr (L >= 4) add(std::integral_constant<int, 0x4E>());
-    if constexpr (L >= 8) add(std::integral_constant<int, 0x141>());
-    if constexpr (L >= 16) add(std::integral_constant<int, 0x140>());
     float a, b;
-    if constexpr (L >= 32) {
-        pair16(v, a, b);
-        v = a + b;
-    }
     if constexpr (L >= 64) {
         pair32(v, a, b);
         v = a + b;
     }
+    if constexpr (L >= 32) {
+        pair16(v, a, b);
+        v = a + b;
+    }
+    if constexpr (L >= 16) add(std::integral_constant<int, 0x140>());
+    if constexpr (L >= 8) add(std::integral_constant<int, 0x141>());
+    if constexpr (L >= 4) add(std::integral_constant<int, 0x4E>());
+    if constexpr (L >= 2) add(std::integral_constant<int, 0xB1>());
     return v;
 }
 

@@ -23,7 +23,8 @@ namespace {
 constexpr int64_t MOST_ROWS = 4096;
 
 // The sums over each run of LR lanes of U values, value lane / (LR / U) in a lane: at each step two values' halves of the run
-// change places, so that U values take U - 1 additions (and as many exchanges) until one a lane is left, not U each
+// change places, so that U values take U - 1 additions (and as many exchanges) until one a lane is left, not U each. (The lanes of a value are
+// added in lanes_sum's order, whatever U: a state row's sum has the same bits from every instance)
 template <int LR, int U>
 __device__ __forceinline__ float lanes_sums(const float (&v)[U], int lane) {
     if constexpr (U == 1) return lanes_sum<LR>(v[0]);
