@@ -5,8 +5,8 @@
  * nothing, record into a graph (kernel launches only) and give the same bits every time.
  *
  * Row types qt: 0 float32, 1 half, 2 bfloat16. Sums, norms, states and the convolution are float32. Strides are in
- * elements of their rows' type, at least a row long; rows may start at any element (16-byte aligned rows of a multiple of
- * 16 bytes are read in wider pieces). Outputs overlap no input except where a call says that they may. */
+ * elements of their rows' type, at least a row long; rows may start at any element (they are read in wide pieces wherever
+ * they start). Outputs overlap no input except where a call says that they may. */
 #ifndef NS_LAYER_H
 #define NS_LAYER_H
 #include <stdint.h>

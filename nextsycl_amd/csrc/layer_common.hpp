@@ -8,31 +8,30 @@
 #include "kv_formats.hpp"
 #include "ns_internal.hpp"
 
-// VEC elements of type QT from element i on, as float32 (VEC 1, 2, 4 or 8; more than one: aligned to the piece, up to 16 bytes)
+// VEC elements of type QT from element i on, as float32 (VEC 1, or pieces of 8 to 16 bytes at any element: global memory is read and
+// written in wide pieces whatever their alignment)
+typedef uint32_t piece4_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t piece2_t __attribute__((ext_vector_type(2), aligned(2)));
+typedef float floats4_t __attribute__((ext_vector_type(4), aligned(4)));
 template <int QT, int VEC>
 __device__ __forceinline__ void load_row(const void* p, int64_t i, float (&v)[VEC]) {
     if constexpr (VEC == 1) v[0] = load_q<QT>(p, i);
     else if constexpr (QT == 0) {
-        if constexpr (VEC == 2) {
-            const float2 a = *reinterpret_cast<const float2*>(static_cast<const float*>(p) + i);
-            v[0] = a.x, v[1] = a.y;
-        } else {
 #pragma unroll
-            for (int j = 0; j < VEC; j += 4) {
-                const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + j);
-                v[j] = a.x, v[j + 1] = a.y, v[j + 2] = a.z, v[j + 3] = a.w;
-            }
+        for (int j = 0; j < VEC; j += 4) {
+            const floats4_t a = *reinterpret_cast<const floats4_t*>(static_cast<const float*>(p) + i + j);
+            v[j] = a.x, v[j + 1] = a.y, v[j + 2] = a.z, v[j + 3] = a.w;
         }
     } else {
         uint32_t w[VEC / 2];
         const uint16_t* s = static_cast<const uint16_t*>(p) + i;
         if constexpr (VEC == 8) {
-            const uint4 a = *reinterpret_cast<const uint4*>(s);
+            const piece4_t a = *reinterpret_cast<const piece4_t*>(s);
             w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-        } else if constexpr (VEC == 4) {
-            const uint2 a = *reinterpret_cast<const uint2*>(s);
+        } else {
+            const piece2_t a = *reinterpret_cast<const piece2_t*>(s);
             w[0] = a.x, w[1] = a.y;
-        } else w[0] = *reinterpret_cast<const uint32_t*>(s);
+        }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             const uint16_t b = (uint16_t) (j % 2 ? w[j / 2] >> 16 : w[j / 2]);
@@ -45,7 +44,7 @@ __device__ __forceinline__ void store_row(void* p, int64_t i, const float (&v)[V
     if constexpr (VEC == 1) store_o<QT>(p, i, v[0]);
     else if constexpr (QT == 0) {
 #pragma unroll
-        for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4*>(static_cast<float*>(p) + i + j) = float4{v[j], v[j + 1], v[j + 2], v[j + 3]};
+        for (int j = 0; j < VEC; j += 4) *reinterpret_cast<floats4_t*>(static_cast<float*>(p) + i + j) = floats4_t{v[j], v[j + 1], v[j + 2], v[j + 3]};
     } else {
         uint32_t w[VEC / 2];
 #pragma unroll
@@ -54,9 +53,25 @@ __device__ __forceinline__ void store_row(void* p, int64_t i, const float (&v)[V
             w[j] = a | b << 16;
         }
         uint16_t* d = static_cast<uint16_t*>(p) + i;
-        if constexpr (VEC == 8) *reinterpret_cast<uint4*>(d) = uint4{w[0], w[1], w[2], w[3]};
-        else *reinterpret_cast<uint2*>(d) = uint2{w[0], w[1]};
+        if constexpr (VEC == 8) *reinterpret_cast<piece4_t*>(d) = piece4_t{w[0], w[1], w[2], w[3]};
+        else *reinterpret_cast<piece2_t*>(d) = piece2_t{w[0], w[1]};
     }
+}
+// the same of the `left` elements that there are (TAIL: there may be fewer than VEC); those that there are not: zeros
+template <int QT, int VEC, bool TAIL>
+__device__ __forceinline__ void load_piece(const void* p, int64_t i, int left, float (&v)[VEC]) {
+    if (!TAIL || left >= VEC) load_row<QT, VEC>(p, i, v);
+    else
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = j < left ? load_q<QT>(p, i + j) : 0.0f;
+}
+template <int QT, int VEC, bool TAIL>
+__device__ __forceinline__ void store_piece(void* p, int64_t i, int left, const float (&v)[VEC]) {
+    if (!TAIL || left >= VEC) store_row<QT, VEC>(p, i, v);
+    else
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (j < left) store_o<QT>(p, i + j, v[j]);
 }
 
 // v / (1 + e^-v) by the hardware's exponential and reciprocal (one unit in the last place each); where e^-v is infinite, 0

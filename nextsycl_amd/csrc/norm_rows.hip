@@ -4,7 +4,7 @@
 // Bound: HBM for prompts (each row read once and written once: 6 bytes a value of bfloat16 rows for the gated norm), a
 // launch and one memory latency for a token. A unit - a group of a row, or a row - is held in registers by 1 to 16
 // waves, so nothing is read twice; sums of squares and everything between load and store are float32, rounded once at
-// the end. A unit of more than 4096 pieces (16384 to 32768 values, 4096 where rows are not aligned) is read twice.
+// the end. A unit of more than 4096 pieces of 16 bytes is read twice.
 // 8192 bfloat16 rows of 8192 in 8 groups 73 us (403 MB, 5.5 TB/s; a large copy 5.1), 4001 bfloat16 rows of 5120 into a float32 stream
 // with both norms and a gate 52 us (246 MB, 4.7 TB/s: two sums over a row's waves, each in front of the next step); a token's
 // row 3.0 - 3.3 us of kernel, 4.2 a call.
@@ -31,9 +31,9 @@ __device__ __forceinline__ float unit_sum(float v, float* part) {
     return v;
 }
 // VEC weights from element i on, or ones
-template <int VEC>
-__device__ __forceinline__ void load_weights(const float* w, int64_t i, float (&v)[VEC]) {
-    if (w) load_row<0, VEC>(w, i, v);
+template <int VEC, bool TAIL>
+__device__ __forceinline__ void load_weights(const float* w, int64_t i, int left, float (&v)[VEC]) {
+    if (w) load_piece<0, VEC, TAIL>(w, i, left, v);
     else
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] = 1.0f;
@@ -49,8 +49,8 @@ struct GatedParams {
     float eps;
 };
 
-// IT pieces of VEC values a thread; IT 0: any number, read twice
-template <int QT, int VEC, bool WIDE, int IT>
+// IT pieces of VEC values a thread (TAIL: the unit's last is not whole); IT 0: any number, read twice
+template <int QT, int VEC, bool TAIL, bool WIDE, int IT>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_gated_kernel(GatedParams p) {
     __shared__ float part[16];
     const int tpu = WIDE ? blockDim.x : 64, tid = WIDE ? threadIdx.x : threadIdx.x % 64;
@@ -58,15 +58,15 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_gated_kernel(GatedPara
     if (unit >= p.units) return;         // (whole waves; a unit of more than one is its whole block)
     const int64_t t = unit / p.groups, c0 = unit % p.groups * p.W;
     auto values = [&](int at, float (&v)[VEC], float (&s)[VEC]) {
-        load_row<QT, VEC>(p.y, t * p.ys + c0 + at, v);
-        load_row<QT, VEC>(p.z, t * p.zs + c0 + at, s);
+        load_piece<QT, VEC, TAIL>(p.y, t * p.ys + c0 + at, p.W - at, v);
+        load_piece<QT, VEC, TAIL>(p.z, t * p.zs + c0 + at, p.W - at, s);
     };
     auto result = [&](int at, float (&v)[VEC], const float (&s)[VEC], float inv) {
         float w[VEC];
-        load_weights<VEC>(p.w, c0 + at, w);
+        load_weights<VEC, TAIL>(p.w, c0 + at, p.W - at, w);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] *= p.order ? inv * w[j] * s[j] : inv * w[j];
-        store_row<QT, VEC>(p.out, t * p.os + c0 + at, v);
+        store_piece<QT, VEC, TAIL>(p.out, t * p.os + c0 + at, p.W - at, v);
     };
     float sum = 0.0f;
     auto square = [&](float (&v)[VEC], float (&s)[VEC]) {
@@ -117,14 +117,14 @@ struct ResidualParams {
     float eps, scale;
 };
 
-template <int QT, int RT, int VEC, bool WIDE, int IT>
+template <int QT, int RT, int VEC, bool TAIL, bool WIDE, int IT>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_residual_kernel(ResidualParams p) {
     __shared__ float part[16];
     const int tpu = WIDE ? blockDim.x : 64, tid = WIDE ? threadIdx.x : threadIdx.x % 64;
     const int64_t t = WIDE ? blockIdx.x : (int64_t) blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64;
     if (t >= p.T) return;
     auto load_x = [&](int at, float (&v)[VEC]) {
-        if (p.x) load_row<QT, VEC>(p.x, t * p.xs + at, v);
+        if (p.x) load_piece<QT, VEC, TAIL>(p.x, t * p.xs + at, p.D - at, v);
         else
 #pragma unroll
             for (int j = 0; j < VEC; ++j) v[j] = 0.0f;
@@ -138,12 +138,12 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_residual_kernel(Residu
         }
         float w[VEC];
         if (p.post) {
-            load_weights<VEC>(p.post, at, w);
+            load_weights<VEC, TAIL>(p.post, at, p.D - at, w);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) v[j] = v[j] * inv * w[j];
         }
         if (p.gate) {
-            load_weights<VEC>(p.gate, at, w);
+            load_weights<VEC, TAIL>(p.gate, at, p.D - at, w);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) v[j] *= w[j];
         }
@@ -152,10 +152,10 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_residual_kernel(Residu
     };
     auto result = [&](int at, float (&v)[VEC], float inv) {
         float w[VEC];
-        load_weights<VEC>(p.pre, at, w);
+        load_weights<VEC, TAIL>(p.pre, at, p.D - at, w);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] = v[j] * inv * w[j];
-        store_row<QT, VEC>(p.out, t * p.os + at, v);
+        store_piece<QT, VEC, TAIL>(p.out, t * p.os + at, p.D - at, v);
     };
     auto squares = [&](const float (&v)[VEC]) {
         float sum = 0.0f;
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_residual_kernel(Residu
             const int at = (i * tpu + tid) * VEC;
             if (at < p.D) {
                 load_x(at, v[i]);
-                load_row<RT, VEC>(p.h, t * p.hs + at, h[i]);
+                load_piece<RT, VEC, TAIL>(p.h, t * p.hs + at, p.D - at, h[i]);
             }
         }
         float inv = 1.0f;
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_residual_kernel(Residu
             if (at >= p.D) continue;
             stream(at, v[i], h[i], inv);
             sum += squares(v[i]);
-            if (p.h1) store_row<RT, VEC>(p.h1, t * p.h1s + at, v[i]);
+            if (p.h1) store_piece<RT, VEC, TAIL>(p.h1, t * p.h1s + at, p.D - at, v[i]);
         }
         if (!p.out) return;
         inv = inverse_root(unit_sum<WIDE>(sum, part), p.D, p.eps);
@@ -210,16 +210,16 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_residual_kernel(Residu
         }
         for (int at = tid * VEC; at < p.D; at += tpu * VEC) {
             load_x(at, v);
-            load_row<RT, VEC>(p.h, t * p.hs + at, h);
+            load_piece<RT, VEC, TAIL>(p.h, t * p.hs + at, p.D - at, h);
             stream(at, v, h, inv);
             sum += squares(v);
         }
         const float inv2 = inverse_root(unit_sum<WIDE>(sum, part), p.D, p.eps);
         for (int at = tid * VEC; at < p.D; at += tpu * VEC) {
             load_x(at, v);
-            load_row<RT, VEC>(p.h, t * p.hs + at, h);
+            load_piece<RT, VEC, TAIL>(p.h, t * p.hs + at, p.D - at, h);
             stream(at, v, h, inv);
-            if (p.h1) store_row<RT, VEC>(p.h1, t * p.h1s + at, v);
+            if (p.h1) store_piece<RT, VEC, TAIL>(p.h1, t * p.h1s + at, p.D - at, v);
             if (p.out) result(at, v, inv2);
         }
     }
@@ -239,29 +239,39 @@ void by_size(int64_t n, int64_t units, F f) {
     return f(true_type(), integral_constant<int, 0>(), 1024, units);
 }
 
-template <int QT, int VEC>
+// Pieces of 16 bytes of the rows' type, wherever rows start; where the last is not whole and a wave's lanes have room for all of a unit one by
+// one, single values (17048 groups of 35 half values 5.2 us, 9.9 in pieces; 4608 groups of 541 13.1 us in pieces, 28.6 one by one)
+template <int VEC>
+bool one_by_one(int64_t n) { return n % VEC && n <= 64; }
+template <int QT, int VEC, bool TAIL>
 int launch_gated(ns_gpu* g, const GatedParams& p) {
     int rc = 0;
     by_size((p.W + VEC - 1) / VEC, p.units, [&](auto wide, auto it, int threads, int64_t blocks) {
         if (blocks > INT32_MAX) rc = ns_fail("ns_norm_gated: too many rows");
-        else norm_gated_kernel<QT, VEC, decltype(wide)::value, decltype(it)::value><<<(unsigned) blocks, threads, 0, g->q>>>(p);
+        else if constexpr (VEC > 1 || (!decltype(wide)::value && decltype(it)::value == 1))
+            norm_gated_kernel<QT, VEC, TAIL, decltype(wide)::value, decltype(it)::value><<<(unsigned) blocks, threads, 0, g->q>>>(p);
     });
     return rc;
 }
-template <int QT, int RT, int VEC>
+template <int QT>
+int launch_gated(ns_gpu* g, const GatedParams& p) {
+    constexpr int VEC = QT ? 8 : 4;
+    return one_by_one<VEC>(p.W) ? launch_gated<QT, 1, false>(g, p) : p.W % VEC ? launch_gated<QT, VEC, true>(g, p) : launch_gated<QT, VEC, false>(g, p);
+}
+template <int QT, int RT, int VEC, bool TAIL>
 int launch_residual(ns_gpu* g, const ResidualParams& p) {
     int rc = 0;
     by_size((p.D + VEC - 1) / VEC, p.T, [&](auto wide, auto it, int threads, int64_t blocks) {
         if (blocks > INT32_MAX) rc = ns_fail("ns_norm_residual: too many rows");
-        else norm_residual_kernel<QT, RT, VEC, decltype(wide)::value, decltype(it)::value><<<(unsigned) blocks, threads, 0, g->q>>>(p);
+        else if constexpr (VEC > 1 || (!decltype(wide)::value && decltype(it)::value == 1))
+            norm_residual_kernel<QT, RT, VEC, TAIL, decltype(wide)::value, decltype(it)::value><<<(unsigned) blocks, threads, 0, g->q>>>(p);
     });
     return rc;
 }
-
-// whether rows of type t at p, s elements apart, can be read in pieces of vec values
-bool wide(const void* p, int64_t s, int t, int vec) {
-    const int64_t e = t ? 2 : 4, piece = std::min<int64_t>(16, vec * e);
-    return (uintptr_t) p % piece == 0 && s * e % piece == 0;
+template <int QT, int RT>
+int launch_residual(ns_gpu* g, const ResidualParams& p) {
+    constexpr int VEC = QT ? 8 : 4;
+    return one_by_one<VEC>(p.D) ? launch_residual<QT, RT, 1, false>(g, p) : p.D % VEC ? launch_residual<QT, RT, VEC, true>(g, p) : launch_residual<QT, RT, VEC, false>(g, p);
 }
 
 }  // namespace
@@ -280,11 +290,7 @@ int ns_norm_gated(ns_gpu* g, int qt, const void* y, int64_t ys, const void* z, i
     if (T > ((int64_t) 1 << 40) / groups) return ns_fail("ns_norm_gated: too many rows");
     NS_HIP(hipSetDevice(g->dev));
     const GatedParams p{y, z, w, out, ys, zs, os, T * groups, (int) (D / groups), (int) groups, order, eps};
-    const int vec = qt ? 8 : 4;
-    const bool v = D / groups % vec == 0 && (uintptr_t) w % 16 == 0 && wide(y, ys, qt, vec) && wide(z, zs, qt, vec) && wide(out, os, qt, vec);
-    const int rc = qt == 0 ? (v ? launch_gated<0, 4>(g, p) : launch_gated<0, 1>(g, p))
-                 : qt == 1 ? (v ? launch_gated<1, 8>(g, p) : launch_gated<1, 1>(g, p))
-                           : (v ? launch_gated<2, 8>(g, p) : launch_gated<2, 1>(g, p));
+    const int rc = qt == 0 ? launch_gated<0>(g, p) : qt == 1 ? launch_gated<1>(g, p) : launch_gated<2>(g, p);
     if (rc) return rc;
     NS_LAUNCHED("norm_gated");
     return 0;
@@ -303,13 +309,10 @@ int ns_norm_residual(ns_gpu* g, int qt, int rt, const void* x, int64_t xs, const
     if (!x && (post || gate)) return ns_fail("ns_norm_residual: a norm or gate of no block");
     NS_HIP(hipSetDevice(g->dev));
     const ResidualParams p{x, h, post, gate, pre, h1, out, xs, hs, h1s, os, T, (int) D, eps, scale};
-    const int vec = qt ? 8 : 4;
-    const bool v = D % vec == 0 && (uintptr_t) post % 16 == 0 && (uintptr_t) gate % 16 == 0 && (uintptr_t) pre % 16 == 0 && (!x || wide(x, xs, qt, vec)) && wide(h, hs, rt, vec) && (!h1 || wide(h1, h1s, rt, vec)) && (!out || wide(out, os, qt, vec));
-    const int rc = qt == 0   ? (v ? launch_residual<0, 0, 4>(g, p) : launch_residual<0, 0, 1>(g, p))
-                   : rt == 0 ? (qt == 1 ? (v ? launch_residual<1, 0, 8>(g, p) : launch_residual<1, 0, 1>(g, p))
-                                        : (v ? launch_residual<2, 0, 8>(g, p) : launch_residual<2, 0, 1>(g, p)))
-                   : qt == 1 ? (v ? launch_residual<1, 1, 8>(g, p) : launch_residual<1, 1, 1>(g, p))
-                             : (v ? launch_residual<2, 2, 8>(g, p) : launch_residual<2, 2, 1>(g, p));
+    const int rc = qt == 0   ? launch_residual<0, 0>(g, p)
+                   : rt == 0 ? (qt == 1 ? launch_residual<1, 0>(g, p) : launch_residual<2, 0>(g, p))
+                   : qt == 1 ? launch_residual<1, 1>(g, p)
+                             : launch_residual<2, 2>(g, p);
     if (rc) return rc;
     NS_LAUNCHED("norm_residual");
     return 0;

@@ -38,7 +38,6 @@ struct Q4Params {
     void* y;
     int64_t xs, ys;
     int T, M, K, kt;             // kt: tiles along K
-    int vec;                     // rows readable in pieces of 8 values
     uint8_t* ops;                // the rows as operands, where LDS does not hold them
 };
 
@@ -64,7 +63,7 @@ template <int QT>
 __device__ __forceinline__ void q4_rows(const Q4Params& p, int kl, int t, int u, s8v* xo, float* xscale) {
     const int k = kl * 128 + u * 8;
     float v[8];
-    if (p.vec && k + 8 <= p.K) load_row<QT, 8>(p.x, t * p.xs + k, v);
+    if (k + 8 <= p.K) load_row<QT, 8>(p.x, t * p.xs + k, v);
     else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? load_q<QT>(p.x, t * p.xs + k + j) : 0.0f;
@@ -306,8 +305,7 @@ int ns_q4_product(ns_gpu* g, int qt, const void* x, int64_t xs, const void* w, i
     if ((uintptr_t) w % 16) return ns_fail("ns_q4_product: weights 16-byte aligned");
     if (!g || !x || !w || !y) return ns_fail("ns_q4_product: a null buffer");
     NS_HIP(hipSetDevice(g->dev));
-    const int64_t e = qt ? 2 : 4;
-    Q4Params p{x, static_cast<const uint8_t*>(w), y, xs, ys, (int) T, (int) M, (int) K, (int) ((K + 127) / 128), (uintptr_t) x % 16 == 0 && xs * e % 16 == 0};
+    Q4Params p{x, static_cast<const uint8_t*>(w), y, xs, ys, (int) T, (int) M, (int) K, (int) ((K + 127) / 128)};
     const int rc = qt == 0 ? launch_product<0>(g, p, group) : qt == 1 ? launch_product<1>(g, p, group) : launch_product<2>(g, p, group);
     if (rc) return rc;
     NS_LAUNCHED("q4_product");

@@ -791,7 +791,7 @@ void run_prompt(ns_gpu* g, const SsmLayer& p, int64_t T, float* scratch) {
         const int64_t n = std::min(PASS_ROWS, T - t0);
         const Plan q = plan_of(n, p.H, p.P, p.N, p.G, p.N <= 128 ? SCAN_WGS<QT, 1, false> : SCAN_WGS<QT, 2, false>);
         ScanParams s{p, t0, T, p.p0 % p.cap, (int) n, q.chunks, q.segs, q.per, q.sub, q.piece, q.blocks};
-        s.vec_y = (uintptr_t) p.y % (QT ? 8 : 16) == 0 && p.ys % 4 == 0 && p.P % 4 == 0;
+        s.vec_y = p.P % 4 == 0;
         s.vec_h = p.N % 4 == 0 && (uintptr_t) p.h0 % 16 == 0 && (uintptr_t) p.h1 % 16 == 0;
         s.ops = reinterpret_cast<uint8_t*>(scratch + q.ops);
         s.scales = scratch + q.scales, s.hdr = scratch + q.hdr, s.hist = scratch + q.hist, s.segst = scratch + q.segst, s.segtot = scratch + q.segtot;

@@ -56,7 +56,7 @@ struct StepParams {
 
 // LR lanes a state row, U rows a lane; VEC: a lane's 4 floats as one piece
 template <int QT, int LR, int U, bool VEC>
-__global__ __launch_bounds__(256, 4) void ssm_step_kernel(StepParams s) {
+__global__ __launch_bounds__(256, VEC ? 4 : 3) void ssm_step_kernel(StepParams s) {
     constexpr int RW = 256 / LR, PB = RW * U, AHEAD = 4, NMAX = 4 * LR, CH = (2 * NMAX + PB + 255) / 256;
     __shared__ __align__(16) float row_in[AHEAD][2 * NMAX + PB];      // B, C, the block's x of a row
     __shared__ float step[AHEAD][2];                                  // its step size and decay
@@ -94,27 +94,6 @@ __global__ __launch_bounds__(256, 4) void ssm_step_kernel(StepParams s) {
         if (count > 1) __syncthreads();
     }
     auto row_of = [&](int i) { return count > 1 ? (int64_t) list[i] : (int64_t) r0; };
-    // the state, on its way while the convolution runs
-    float h[U][4];
-    const int64_t hrow = (slot * p.H + head) * p.P;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int pr = prow + u * RW;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[u][i] = 0.0f;
-        if (!p.h0 || pr >= p.P) continue;
-        const float* src = p.h0 + (hrow + pr) * p.N + n0;
-        if constexpr (VEC) {
-            if (n0 < p.N) {
-                const float4 v = *reinterpret_cast<const float4*>(src);
-                h[u][0] = v.x, h[u][1] = v.y, h[u][2] = v.z, h[u][3] = v.w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (n0 + i < p.N) h[u][i] = src[i];
-        }
-    }
     // this thread's channels: B, C, then the block's part of x; their taps and the raw values in front of the first row
     int ch[CH];
     float w4[CH][4], bias[CH], past[CH][3];
@@ -149,21 +128,38 @@ __global__ __launch_bounds__(256, 4) void ssm_step_kernel(StepParams s) {
         }
     }
     const float rate = p.a[head], skip = p.d ? p.d[head] : 0.0f, dtb = p.dtb ? p.dtb[head] : 0.0f;
-    int here = slot0;
-    for (int i0 = 0; i0 < count; i0 += AHEAD) {
-        // four rows at a time: their convolutions and step sizes, in LDS, then the state through them
-        const int rows = min(AHEAD, count - i0);
-        float raw[AHEAD][CH], size = 0.0f;
+    // (a lane a row, of the wave that has no channels of x)
+    float raw[AHEAD][CH], size = 0.0f;
+    auto fetch = [&](int i0) {
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-            if (a >= rows) break;
+            if (i0 + a >= count) break;
             const int64_t r = row_of(i0 + a);
 #pragma unroll
             for (int j = 0; j < CH; ++j) raw[a][j] = ch[j] >= 0 ? load_q<QT>(p.xbc, r * p.xs + ch[j]) : 0.0f;
         }
-        // (a lane a row, of the wave that has no channels of x)
-        const bool sizes = tid >= 192 && lane < rows;
-        if (sizes) size = load_q<QT>(p.dt, row_of(i0 + lane) * p.dts + head);
+        if (tid >= 192 && lane < AHEAD && i0 + lane < count) size = load_q<QT>(p.dt, row_of(i0 + lane) * p.dts + head);
+    };
+    fetch(0);
+    // the state, asked for last: the convolution waits for what it reads alone (a load a piece whatever the lane, so that their number is known:
+    // what a lane has no place for is a neighbour's, and set to 0 before its first use)
+    float h[U][4];
+    const int64_t hrow = (slot * p.H + head) * p.P;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int pr = prow + u * RW;
+        if constexpr (VEC) {
+            const floats4_t v = *reinterpret_cast<const floats4_t*>((p.h0 ? p.h0 : p.h1) + (hrow + min(pr, p.P - 1)) * p.N + (n0 < p.N ? n0 : 0));
+            h[u][0] = v.x, h[u][1] = v.y, h[u][2] = v.z, h[u][3] = v.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[u][i] = p.h0 && pr < p.P && n0 + i < p.N ? p.h0[(hrow + pr) * p.N + n0 + i] : 0.0f;
+        }
+    }
+    int here = slot0;
+    for (int i0 = 0; i0 < count; i0 += AHEAD) {
+        // four rows at a time: their convolutions and step sizes, in LDS, then the state through them
+        const int rows = min(AHEAD, count - i0);
         if (i0) lds_barrier();           // the rows before have been read
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
@@ -178,11 +174,16 @@ __global__ __launch_bounds__(256, 4) void ssm_step_kernel(StepParams s) {
             }
             here = here + 1 == cap ? 0 : here + 1;
         }
-        if (sizes) {
+        if (tid >= 192 && lane < rows) {
             const float dt = ssm_dt(p, size + dtb);
             step[lane][0] = dt, step[lane][1] = expf(dt * rate);
         }
         lds_barrier();
+        if (i0 + AHEAD < count) fetch(i0 + AHEAD);
+        if (VEC && i0 == 0 && (!p.h0 || n0 >= p.N)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) h[u][0] = h[u][1] = h[u][2] = h[u][3] = 0.0f;
+        }
         for (int a = 0; a < rows; ++a) {
             const float dt = step[a][0], decay = step[a][1];
             const float4 b = *reinterpret_cast<const float4*>(row_in[a] + n0), c = *reinterpret_cast<const float4*>(row_in[a] + NMAX + n0);
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(256, 4) void ssm_step_kernel(StepParams s) {
         if (pr >= p.P) continue;
         float* dst = p.h1 + (hrow + pr) * p.N + n0;
         if constexpr (VEC) {
-            if (n0 < p.N) *reinterpret_cast<float4*>(dst) = float4{h[u][0], h[u][1], h[u][2], h[u][3]};
+            if (n0 < p.N) *reinterpret_cast<floats4_t*>(dst) = floats4_t{h[u][0], h[u][1], h[u][2], h[u][3]};
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -269,7 +270,7 @@ extern "C" int ns_ssm_step(ns_gpu* g, int qt, const void* xbc, int64_t xs, const
     s.l.chan = (int) (H * P + 2 * G * N);
     s.pos = pos, s.slots = slots, s.nslots = nslots, s.R = (int) R;
     NS_HIP(hipSetDevice(g->dev));
-    const bool vec = N % 4 == 0 && (uintptr_t) h0 % 16 == 0 && (uintptr_t) h1 % 16 == 0;
+    const bool vec = N % 4 == 0;
     if (qt == 0) launch_step<0>(g, s, vec);
     else if (qt == 1) launch_step<1>(g, s, vec);
     else launch_step<2>(g, s, vec);
