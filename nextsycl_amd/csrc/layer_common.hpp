@@ -125,5 +125,8 @@ __device__ __forceinline__ float ssm_dt(const SsmLayer& p, float v) {
 // tap k of 4 of a channel: the layer's K taps are the last K of them
 __device__ __forceinline__ float ssm_tap(const SsmLayer& p, int ch, int k) { return k >= 4 - p.K ? p.cw[(int64_t) ch * p.K + k - 4 + p.K] : 0.0f; }
 
+// ssm_step.hip: a few successive rows of one sequence from p.p0 on, the last K - 1 of them into the ring (which holds those in front of the
+// call and those behind it at once)
+void ns_ssm_few(ns_gpu* g, int qt, const SsmLayer& p, int rows);
 // ssm_step.hip: what the two state-space calls refuse alike (a ring of fewer than `least` rows among it); 0 or -1
 int ns_ssm_check(const char* who, ns_gpu* g, int qt, const SsmLayer& p, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K, int64_t least);

@@ -43,6 +43,9 @@ namespace {
 constexpr int L = 64;                     // rows a chunk
 constexpr int64_t PASS_ROWS = 8192;       // rows a pass works on: what bounds the scratch
 constexpr int MOST_SEGS = 32;
+// up to these row by row, as steps (128 heads of 64 x 128: 1 row 6.4 us and 17.5 as a chunk, 8 9.2 and 18.2, 16 14.5 and 18.2, 24 19.6
+// and 18.4; of 80 x 128 16 17.5 and 18.2)
+constexpr int64_t FEW_ROWS = 16;
 // a chunk and head's header: exponents (base 2) from the start of each run of 16 rows, step sizes, weights in the chunk's
 // state, decays from the chunk's start; differences between runs' starts [4][4], the whole chunk's exponent and decay, what the weights are
 // to be multiplied with
@@ -828,7 +831,8 @@ int ns_ssm_prompt(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt
     p.chan = (int) (H * P + 2 * G * N);
     if (K == 1) p.conv = nullptr, p.cap = 1;
     NS_HIP(hipSetDevice(g->dev));
-    if (qt == 0) run_prompt<0>(g, p, T, scratch);
+    if (T <= FEW_ROWS && p.cap >= K - 1 + (K > 1 ? T : 0) && p.cap <= INT32_MAX) ns_ssm_few(g, qt, p, (int) T);
+    else if (qt == 0) run_prompt<0>(g, p, T, scratch);
     else if (qt == 1) run_prompt<1>(g, p, T, scratch);
     else run_prompt<2>(g, p, T, scratch);
     NS_LAUNCHED("ssm_prompt");

@@ -52,6 +52,7 @@ struct StepParams {
     const int32_t *pos, *slots;
     int64_t nslots;
     int R, pblocks;
+    int one;              // all R rows are one sequence's, as a short prompt's are: of those only the last K - 1 go into the ring
 };
 
 // LR lanes a state row, U rows a lane; VEC: a lane's 4 floats as one piece
@@ -70,7 +71,7 @@ __global__ __launch_bounds__(256, VEC ? 4 : 3) void ssm_step_kernel(StepParams s
     if (slot < 0 || slot >= s.nslots || first < 0) return;
     // the slot's rows in their order, as many as its ring has room for: this work-group is the first's, or has nothing to do
     const int cap = (int) p.cap;
-    int count = 1;
+    int count = s.one ? s.R : 1;
     if (s.slots) {
         for (int w = tid / 64; w * 64 < s.R; w += 4) {
             const int at = w * 64 + lane;
@@ -93,7 +94,8 @@ __global__ __launch_bounds__(256, VEC ? 4 : 3) void ssm_step_kernel(StepParams s
         count = min(count, most);
         if (count > 1) __syncthreads();
     }
-    auto row_of = [&](int i) { return count > 1 ? (int64_t) list[i] : (int64_t) r0; };
+    auto row_of = [&](int i) { return s.slots && count > 1 ? (int64_t) list[i] : (int64_t) (r0 + i); };
+    const int kept_from = s.one ? count - (p.K - 1) : 0;
     // this thread's channels: B, C, then the block's part of x; their taps and the raw values in front of the first row
     int ch[CH];
     float w4[CH][4], bias[CH], past[CH][3];
@@ -170,7 +172,7 @@ __global__ __launch_bounds__(256, VEC ? 4 : 3) void ssm_step_kernel(StepParams s
                 const float v = raw[a][j];
                 row_in[a][to[j]] = ch[j] >= 0 ? silu(fmaf(w4[j][3], v, fmaf(w4[j][2], past[j][2], fmaf(w4[j][1], past[j][1], fmaf(w4[j][0], past[j][0], bias[j]))))) : 0.0f;
                 past[j][0] = past[j][1], past[j][1] = past[j][2], past[j][2] = v;
-                if (keep[j]) ring[(int64_t) here * p.chan + ch[j]] = v;
+                if (keep[j] && i0 + a >= kept_from) ring[(int64_t) here * p.chan + ch[j]] = v;
             }
             here = here + 1 == cap ? 0 : here + 1;
         }
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(256, VEC ? 4 : 3) void ssm_step_kernel(StepParams s
 template <int QT, int LR, int U>
 void launch_step(ns_gpu* g, StepParams& s, bool vec) {
     s.pblocks = (s.l.P + 256 / LR * U - 1) / (256 / LR * U);
-    const dim3 grid((unsigned) (s.l.H * s.pblocks), (unsigned) s.R);
+    const dim3 grid((unsigned) (s.l.H * s.pblocks), (unsigned) (s.one ? 1 : s.R));
     if (vec) ssm_step_kernel<QT, LR, U, true><<<grid, 256, 0, g->q>>>(s);
     else ssm_step_kernel<QT, LR, U, false><<<grid, 256, 0, g->q>>>(s);
 }
@@ -231,12 +233,25 @@ void launch_step(ns_gpu* g, StepParams& s, bool vec) {
     else if (N <= 32) launch_step<QT, 8, 2>(g, s, vec);
     else if (N <= 64) launch_step<QT, 16, 4>(g, s, vec);
     // (8 state rows a lane, but 4 while there is no work-group of 8 for each CU: a token 5.98 us with 8, 5.54 with 4; 64 tokens 107 and 115, 12 rows of 3 slots of 80 wide heads 15.8 and 16.4)
-    else if (N <= 128 && (int64_t) s.l.H * ((s.l.P + 63) / 64) * s.R <= 128) launch_step<QT, 32, 4>(g, s, vec);
+    else if (N <= 128 && (int64_t) s.l.H * ((s.l.P + 63) / 64) * (s.one ? 1 : s.R) <= 128) launch_step<QT, 32, 4>(g, s, vec);
     else if (N <= 128) launch_step<QT, 32, 8>(g, s, vec);
     else launch_step<QT, 64, 4>(g, s, vec);
 }
 
+void launch_step(ns_gpu* g, int qt, StepParams& s) {
+    const bool vec = s.l.N % 4 == 0;
+    if (qt == 0) launch_step<0>(g, s, vec);
+    else if (qt == 1) launch_step<1>(g, s, vec);
+    else launch_step<2>(g, s, vec);
+}
+
 }  // namespace
+
+void ns_ssm_few(ns_gpu* g, int qt, const SsmLayer& p, int rows) {
+    StepParams s{};
+    s.l = p, s.nslots = 1, s.R = rows, s.one = 1;
+    launch_step(g, qt, s);
+}
 
 // what the two state-space calls refuse alike
 int ns_ssm_check(const char* who, ns_gpu* g, int qt, const SsmLayer& p, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K,
@@ -270,10 +285,7 @@ extern "C" int ns_ssm_step(ns_gpu* g, int qt, const void* xbc, int64_t xs, const
     s.l.chan = (int) (H * P + 2 * G * N);
     s.pos = pos, s.slots = slots, s.nslots = nslots, s.R = (int) R;
     NS_HIP(hipSetDevice(g->dev));
-    const bool vec = N % 4 == 0;
-    if (qt == 0) launch_step<0>(g, s, vec);
-    else if (qt == 1) launch_step<1>(g, s, vec);
-    else launch_step<2>(g, s, vec);
+    launch_step(g, qt, s);
     NS_LAUNCHED("ssm_step");
     return 0;
     NS_CATCH

@@ -45,6 +45,36 @@ def plain(L, val):
     return scan(L, val[:, :L.chan], val[:, L.chan:], np.zeros((L.K - 1, L.chan)), np.zeros((L.H, L.P, L.N)))
 
 
+@pytest.mark.parametrize("qt", [F32, F16, BF16])
+@pytest.mark.parametrize("H,P,N,G,K,T,p0,cap", [(4, 64, 128, 2, 4, 1, 0, 4), (4, 64, 128, 2, 4, 16, 3, 19), (2, 50, 100, 1, 4, 9, 2, 40), (3, 8, 33, 3, 3, 5, 50, 7), (2, 16, 256, 1, 1, 12, 9, 1),
+                                                (2, 40, 20, 1, 2, 2, 0, 3), (2, 64, 128, 1, 4, 16, 3, 18), (2, 64, 128, 1, 4, 17, 3, 20)])
+def test_a_prompt_of_a_few_rows(ops, qt, H, P, N, G, K, T, p0, cap):
+    """Those that run row by row and their neighbours: y, the state (h0 kept), and of the rows the last K - 1 in the ring, nothing else."""
+    g, e = ops.gpu, E[qt]
+    L = Layer(H, P, N, G, K, seed=T)
+    raw, val = rows_of(L, qt, T, 14)
+    r = np.random.default_rng(15)
+    past = r.standard_normal((K - 1, L.chan)).astype(np.float32)
+    ring = np.full((cap, L.chan), np.nan, np.float32)
+    for k in range(K - 1):
+        if p0 - (K - 1) + k < 0:
+            past[k] = 0.0
+        else:
+            ring[(p0 - (K - 1) + k) % cap] = past[k]
+    h0 = r.standard_normal((H, P, N)).astype(np.float32)
+    y, h, yb, hb = scan(L, val[:, :L.chan], val[:, L.chan:], past, h0)
+    c = Call(ops, L, qt, raw)
+    ringb, h0b, row = DevBuf.of(g, ring), DevBuf.of(g, h0), L.chan + H
+    ops.ssm_prompt(qt, c.rows, row, c.rows.view(L.chan * e, c.rows.len - L.chan * e), row, *c.w, ringb if K > 1 else None, cap, p0, T, H, P, N, G, K, h0b, c.h, c.y, L.inner, c.sc)
+    got, state = c.out()
+    check_scan(got, y, yb, qt, T, N, "y")
+    check_scan(state, h[T], hb[T], F32, T, N, "state")
+    assert np.array_equal(h0b.read(np.float32), h0.ravel())
+    for t in range(max(0, T - (K - 1)), T):
+        ring[(p0 + t) % cap] = val[t, :L.chan]
+    assert np.array_equal(ringb.read(np.uint32), ring.view(np.uint32).ravel())
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("part", ["x", "B", "C", "step"])
 @pytest.mark.parametrize("qt,T,at", [(F32, 150, 70), (F32, 600, 333), (BF16, 150, 64), (F16, 600, 63)])
