@@ -63,7 +63,10 @@ public:
     X(ns_attn_kv_store) X(ns_attn_decode_scratch) X(ns_attn_decode_t) X(ns_attn_prompt_t) X(ns_attn_decode_static)                       \
     X(ns_ds2_rope) X(ns_ds2_kv_store) X(ns_ds2_mla_decode) X(ns_ds2_mla_decode_q6k) X(ns_mla_decode_latent_scratch) X(ns_mla_decode_latent)             \
     X(ns_mla_attend) X(ns_mla_attend_sel) X(ns_mla_attend_sel_q8) X(ns_to_q8row) X(ns_gather_q8_h)                                     \
-    X(ns_idx_pool) X(ns_idx_score) X(ns_topk) X(ns_mla_cells) X(ns_softmax_masked) X(ns_gemm_f16) X(ns_gemm_batch_h) X(ns_to_f16) X(ns_gather_h) \
+    X(ns_idx_pool) X(ns_idx_score) X(ns_topk) X(ns_mla_cells) X(ns_softmax_masked) X(ns_gemm_f16) X(ns_gemm_batch_h) X(ns_to_f16) X(ns_gather_h)
+
+// a hybrid model's other layers (ns_layer.h)
+#define NS_HOST_LAYER_SYMBOLS(X)                                                                                                         \
     X(ns_ssm_prompt_scratch) X(ns_ssm_prompt) X(ns_ssm_step) X(ns_norm_gated) X(ns_norm_residual) X(ns_q4_bytes) X(ns_q4_pack) X(ns_q4_product)
 
 class Api {
@@ -114,6 +117,20 @@ private:
     void* handle_ = nullptr;
     std::string file_;
     mutable int bound_ = 0;
+};
+
+// The layers' table, bound apart from Api's: a host that runs none of them loads a library without them. It uses the Api's
+// library and ends before it does.
+class LayerApi {
+public:
+#define NS_HOST_FIELD(name) decltype(&::name) name = nullptr;
+    NS_HOST_LAYER_SYMBOLS(NS_HOST_FIELD)
+#undef NS_HOST_FIELD
+    explicit LayerApi(const Api& a) {
+#define NS_HOST_BIND(name) name = a.symbol<decltype(name)>(#name);
+        NS_HOST_LAYER_SYMBOLS(NS_HOST_BIND)
+#undef NS_HOST_BIND
+    }
 };
 
 inline void check(const Api& a, int rc, const std::string& what) {

@@ -3,6 +3,7 @@ their sizes. Arguments that nothing is wrong with end at the null handle."""
 import ctypes as C
 import os
 import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -199,3 +200,24 @@ def test_rows_too_far_apart_and_scratch_off_its_alignment(lib):
     for change, word in ((dict(xs=(1 << 23) + 1), "apart"), (dict(scratch=AT + 4), "aligned")):
         assert lib.ns_ssm_prompt(*{**PROMPT, "g": C.addressof(g), **change}.values()) == -1
         assert word in lib.ns_last_error().decode()
+
+
+def test_a_cpp_host_binds_the_layers(lib, tmp_path):
+    """LayerApi of include/nextsycl_host.hpp: every entry point of the header, called through the table."""
+    src, exe = tmp_path / "layers.cpp", tmp_path / "layers"
+    src.write_text("""#include <cstdio>
+#include "nextsycl_host.hpp"
+int main() {
+    const nextsycl::Api api;
+    const nextsycl::LayerApi layers(api);
+    int bound = 0;
+#define COUNT(name) bound += layers.name != nullptr;
+    NS_HOST_LAYER_SYMBOLS(COUNT)
+    const int rc = layers.ns_norm_gated(nullptr, 3, nullptr, 1, nullptr, 1, nullptr, nullptr, 1, 1, 1, 1, 0.0f, 0);
+    std::printf("%d %lld %lld %d %s\\n", bound, (long long) layers.ns_q4_bytes(17, 129, 128), (long long) layers.ns_ssm_prompt_scratch(0, 1, 1, 1, 1, 1), rc,
+                api.error().c_str());
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe), "-ldl"], check=True)
+    out = subprocess.run([str(exe)], env=dict(os.environ, NEXTSYCL_LIB=library_path()), check=True, capture_output=True, text=True, timeout=120).stdout
+    assert out.startswith("%d %d 0 -1 ns_norm_gated: " % (len(LAYER_H), 4 * 1056)), out
