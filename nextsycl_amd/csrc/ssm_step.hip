@@ -7,9 +7,9 @@
 // else, and the convolution (a few hundred channels, each group's B and C by every head of the group: 4 multiply-adds and
 // a few KB that the cache holds) runs while they are on their way; y is a sum over a row's lanes. Rows of one slot
 // are walked with the state in registers, their convolutions four rows at a time.
-// 128 heads of 64 x 128: 64 tokens (548 MB) 107 - 109 us, 5.1 TB/s - a copy's rate; one token 5.6 us, a launch and the two latencies of
-// its loads and sums (1.6 us of bytes); 12 half rows of 3 slots, 128 heads of 80 x 128, 15.8 us (33 MB: 6.3), four work-groups a CU;
-// with three 17.0, with two rows at a time 16.5.
+// 128 heads of 64 x 128: 64 tokens (548 MB) 107 - 109 us, 5.1 TB/s - a copy's rate; one token 5.4 us, a launch and the two latencies of
+// its loads and sums (1.6 us of bytes); 12 half rows of 3 slots, 128 heads of 80 x 128, 14.7 us (33 MB: 6.3). Four work-groups a CU (those
+// rows with three, 8 state rows a lane: 17.0, for 15.8), four rows at a time (two: 16.5).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -58,7 +58,7 @@ struct StepParams {
 // LR lanes a state row, U rows a lane; VEC: a lane's 4 floats as one piece
 template <int QT, int LR, int U, bool VEC>
 __global__ __launch_bounds__(256, VEC ? 4 : 3) void ssm_step_kernel(StepParams s) {
-    constexpr int RW = 256 / LR, PB = RW * U, AHEAD = 4, NMAX = 4 * LR, CH = (2 * NMAX + PB + 255) / 256;
+    constexpr int RW = 256 / LR, PB = RW * U, UP = U > 4 ? 8 : U, AHEAD = 4, NMAX = 4 * LR, CH = (2 * NMAX + PB + 255) / 256;
     __shared__ __align__(16) float row_in[AHEAD][2 * NMAX + PB];      // B, C, the block's x of a row
     __shared__ float step[AHEAD][2];                                  // its step size and decay
     __shared__ uint64_t mine[MOST_ROWS / 64];
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256, VEC ? 4 : 3) void ssm_step_kernel(StepParams s
             const float dt = step[a][0], decay = step[a][1];
             const float4 b = *reinterpret_cast<const float4*>(row_in[a] + n0), c = *reinterpret_cast<const float4*>(row_in[a] + NMAX + n0);
             const float bx = dt * b.x, by = dt * b.y, bz = dt * b.z, bw = dt * b.w;
-            float sum[U];
+            float sum[UP] = {};
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const float x = row_in[a][2 * NMAX + tid / LR + u * RW];
@@ -199,9 +199,9 @@ __global__ __launch_bounds__(256, VEC ? 4 : 3) void ssm_step_kernel(StepParams s
                 sum[u] = fmaf(h[u][3], c.w, fmaf(h[u][2], c.z, fmaf(h[u][1], c.y, h[u][0] * c.x)));
             }
             // (a lane then holds the sum of one of its U state rows; the first of those that hold the same one writes it)
-            const int mine_u = tid % LR / (LR / U), mine_p = prow + mine_u * RW;
-            const float out = fmaf(skip, row_in[a][2 * NMAX + tid / LR + mine_u * RW], lanes_sums<LR, U>(sum, lane));
-            if (tid % (LR / U) == 0 && mine_p < p.P) store_o<QT>(p.y, row_of(i0 + a) * p.ys + head * p.P + mine_p, out);
+            const int mine_u = tid % LR / (LR / UP), mine_p = prow + mine_u * RW;
+            const float out = fmaf(skip, row_in[a][2 * NMAX + tid / LR + min(mine_u, U - 1) * RW], lanes_sums<LR, UP>(sum, lane));
+            if (tid % (LR / UP) == 0 && mine_u < U && mine_p < p.P) store_o<QT>(p.y, row_of(i0 + a) * p.ys + head * p.P + mine_p, out);
         }
     }
 #pragma unroll
@@ -232,9 +232,16 @@ void launch_step(ns_gpu* g, StepParams& s, bool vec) {
     if (N <= 16) launch_step<QT, 4, 1>(g, s, vec);
     else if (N <= 32) launch_step<QT, 8, 2>(g, s, vec);
     else if (N <= 64) launch_step<QT, 16, 4>(g, s, vec);
-    // (8 state rows a lane, but 4 while there is no work-group of 8 for each CU: a token 5.98 us with 8, 5.54 with 4; 64 tokens 107 and 115, 12 rows of 3 slots of 80 wide heads 15.8 and 16.4)
-    else if (N <= 128 && (int64_t) s.l.H * ((s.l.P + 63) / 64) * (s.one ? 1 : s.R) <= 128) launch_step<QT, 32, 4>(g, s, vec);
-    else if (N <= 128) launch_step<QT, 32, 8>(g, s, vec);
+    else if (N <= 128) {
+        // as many state rows a lane as share a head's out evenly, 8 at most, and 4 while there is no work-group of more for each CU (12 half rows
+        // of 3 slots, heads of 80, 14.7 us with 5 of them, 16.2 with 8 and 4; 20 tokens, heads of 32, 18.4 with 4, 20.1 with 8; a token, heads of
+        // 64, 5.5 with 4, 6.0 with 8; 64 of them 107 with 8, 115 with 4)
+        const int per = 64 * ((s.l.P + 63) / 64), need = (s.l.P + per / 8 - 1) / (per / 8);
+        if (need <= 4 || (int64_t) s.l.H * (per / 64) * (s.one ? 1 : s.R) <= 128) launch_step<QT, 32, 4>(g, s, vec);
+        else if (need == 5) launch_step<QT, 32, 5>(g, s, vec);
+        else if (need == 6) launch_step<QT, 32, 6>(g, s, vec);
+        else launch_step<QT, 32, 8>(g, s, vec);
+    }
     else launch_step<QT, 64, 4>(g, s, vec);
 }
 

@@ -220,7 +220,7 @@ def test_two_prompts_at_once(ops):
 
 
 @pytest.mark.parametrize("qt", [F32, F16, BF16])
-@pytest.mark.parametrize("H,P,N", [(4, 80, 128), (2, 50, 100), (2, 16, 16), (16, 64, 128)])
+@pytest.mark.parametrize("H,P,N", [(4, 80, 128), (2, 50, 100), (2, 16, 16), (16, 64, 128), (16, 80, 128), (20, 90, 124)])
 def test_a_verify_passes_rows_are_their_tokens(ops, qt, H, P, N):
     """Seven successive rows of a slot in one call, among another slot's, against seven calls of a row: the same bits."""
     g, R, cap, e = ops.gpu, 7, 16, E[qt]
