@@ -12,7 +12,7 @@
 // ssm_prep_kernel, 8 waves a (chunk, group): convolves B and C (a thread half a channel's rows), leaves them in LDS as [feature]
 // [row] - an operand's rows are a thread's own, C's come back through transposing reads - and multiplies them; the work-groups
 // behind sum the exponents (in 64 bits; what the exponentials see is a difference within 16 rows, plus one between such runs).
-// ssm_scan_kernel, a work-group a (head, 64 of its features, segment of the prompt): walks its chunks with the state in
+// ssm_scan_kernel, a work-group a (head, up to 64 of its features, segment of the prompt): walks its chunks with the state in
 // the accumulators of 4 waves, wave w rows 32 w .. 32 w + 31 of it. In a chunk wave w convolves 16 columns of x into the
 // operands that all read (LDS), splits its part of the state into another, then takes 16 rows of y and its part of h'. Matrix
 // results come as (column, 4 consecutive rows) a lane, operands go in as (row or column, 8 values of the summed index) a
@@ -26,7 +26,7 @@
 // executed: 75 us at a large product's) take 297 - 305 us: 42 in the first kernel (134 MB: 26 us), 89 for the segments' states, 175 for the
 // scan - of x's convolution, the splits, the decays and the state's scaling and sums 8 to 11 vector instructions a matrix
 // instruction, in three waves a SIMD that spend 24 % of their life issuing one, 31 % ready for it and the rest at barriers and
-// loads (matrix unit 20 % busy). 2051 float32 rows of 64 heads 73 us (10 + 22 + 43), 85 half rows of 128 heads of 80 24 us:
+// loads (matrix unit 20 % busy). 2051 float32 rows of 64 heads 73 us (10 + 22 + 43), 85 half rows of 128 heads of 80 23 us:
 // two launches and two chunks of 5 us each. Work-groups a CU, 8192 bfloat16 rows: three of the scan 297 us, two - with x and
 // the operands asked for a chunk ahead, for which they have the registers - 309; of the segments' states three, with that, 297, four without it 304, two
 // 298. Float32 and half rows have both halfs of each operand in LDS, and so two.
@@ -261,19 +261,19 @@ __global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
 // work-groups a CU: what LDS has room for, and the registers that leaves a wave
 template <int QT, int KW, bool STATE>
 constexpr int SCAN_WGS = KW == 2 ? 1 : STATE || QT == 2 ? 3 : 2;
-template <int QT, int KW, bool STATE>
+template <int QT, int KW, int CT, bool STATE>
 __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kernel(ScanParams s) {
     constexpr int KK = 4 * KW;
     constexpr bool AHEAD = STATE || SCAN_WGS<QT, KW, STATE> <= 2;     // x and the operands asked for early, where there are registers for them
     constexpr bool Y3 = QT != 2;                                  // y's products from both halfs of their operands
     // x weighted for the state (hi, lo) and as it is (hi, for Y3 lo): [32 rows][16 columns][lane]; the state: [32 features][..]
     constexpr int WH = 0, WL = 1, XH = 2, XL = 3, PLANES = STATE ? 2 : Y3 ? 4 : 3, HP = STATE ? 0 : Y3 ? 2 : 1;
-    __shared__ __align__(16) s8v xop[PLANES][2][4][64];
-    __shared__ __align__(16) s8v hop[HP + !HP][STATE ? 1 : KK][4][64];
-    __shared__ __align__(16) float xs[64], hs[64];                // what their results are to be multiplied with, a column
-    __shared__ __align__(16) float hmax[64][4];                   // the largest of each wave's part of the state, a column
+    __shared__ __align__(16) s8v xop[PLANES][2][CT][64];
+    __shared__ __align__(16) s8v hop[HP + !HP][STATE ? 1 : KK][CT][64];
+    __shared__ __align__(16) float xs[16 * CT], hs[16 * CT];                // what their results are to be multiplied with, a column
+    __shared__ __align__(16) float hmax[16 * CT][4];                   // the largest of each wave's part of the state, a column
     __shared__ __align__(16) float hdrs[2][HDR];
-    __shared__ int bad[64];
+    __shared__ int bad[16 * CT];
     __shared__ __align__(16) int spoilt[4];                       // a column's first row that is not finite; whether 16 columns have one
     const SsmLayer& p = s.l;
     const int tid = threadIdx.x, lane = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, g = lane / 16;
@@ -283,9 +283,9 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
     const int per = p.H / p.G, hb = per * s.blocks;
     const int in_group = id % hb, seg = id / hb % s.segs, group = id / (hb * s.segs);       // (STATE: seg counts pieces)
-    const int head = group * per + in_group / s.blocks, block = in_group % s.blocks, c0 = block * 64;
+    const int head = group * per + in_group / s.blocks, block = in_group % s.blocks, c0 = block * 16 * CT;
     const int col = c0 + 16 * w + n;                              // the column of x this lane convolves
-    const bool has = col < p.P;
+    const bool has = (CT == 4 || w < CT) && col < p.P;            // (fewer column tiles than waves: the last have none)
     const int xch = head * p.P + (has ? col : 0);
     // (the taps times log2 e: x comes out times it too, which its operand's scale takes back, and the exponential takes it as it is)
     constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
@@ -297,16 +297,16 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     const int64_t owner = (int64_t) head * s.blocks + block, owners = (int64_t) p.H * s.blocks;
 
     // features 32 (w KW + i / 2) + 16 (i % 2) + 4 g .. + 3 of column 16 ct + n
-    f4v st[2 * KW][4];
+    f4v st[2 * KW][CT];
     auto feature = [&](int i) { return 32 * (w * KW + i / 2) + 16 * (i % 2) + 4 * g; };
-    auto kept = [&](int slot) { return reinterpret_cast<f4v*>(s.segst) + ((slot * owners + owner) * 4 + w) * (2 * KW * 4 * 64) + lane; };
+    auto kept = [&](int slot) { return reinterpret_cast<f4v*>(s.segst) + ((slot * owners + owner) * 4 + w) * (2 * KW * CT * 64) + lane; };
     // (a cut pass's first state is read from where the state kernel has put it: the last segment may write h1 = h0 meanwhile)
     if (STATE ? seg == 0 : s.segs == 1) {
         const float* h0 = s.t0 ? p.h1 : p.h0;
 #pragma unroll
         for (int i = 0; i < 2 * KW; ++i)
 #pragma unroll
-            for (int ct = 0; ct < 4; ++ct) {
+            for (int ct = 0; ct < CT; ++ct) {
                 f4v v = {0.0f, 0.0f, 0.0f, 0.0f};
                 const int f = feature(i), c = c0 + 16 * ct + n;
                 if (h0 && c < p.P && f < p.N) {
@@ -319,23 +319,24 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                     }
                 }
                 st[i][ct] = v;
-                if (STATE) kept(0)[(i * 4 + ct) * 64] = v;
+                if (STATE) kept(0)[(i * CT + ct) * 64] = v;
             }
     } else {
         const f4v* src = kept(seg > 0 && !STATE);
 #pragma unroll
         for (int i = 0; i < 2 * KW; ++i)
 #pragma unroll
-            for (int ct = 0; ct < 4; ++ct) st[i][ct] = STATE ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : src[(i * 4 + ct) * 64];
+            for (int ct = 0; ct < CT; ++ct) st[i][ct] = STATE ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : src[(i * CT + ct) * 64];
         for (int r = 1; !STATE && r < seg * s.sub; ++r) {
             const float keep = exp2f(s.segtot[(int64_t) r * p.H + head]);
             const f4v* add = kept(1 + r);
 #pragma unroll
             for (int i = 0; i < 2 * KW; ++i)
 #pragma unroll
-                for (int ct = 0; ct < 4; ++ct) st[i][ct] = st[i][ct] * keep + add[(i * 4 + ct) * 64];
+                for (int ct = 0; ct < CT; ++ct) st[i][ct] = st[i][ct] * keep + add[(i * CT + ct) * 64];
         }
     }
+    if (CT < 4 && tid < 4) spoilt[tid] = 0;
     float exponent = 0.0f;
     // a chunk's header, through registers into LDS; x: 16 rows of this lane's column - 16 j + 4 g .. + 3 - and 3 in front of each 4
     float head0, head1;
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     // each column's largest in this wave's part of the state: what the next chunk's operands of it are scaled by
     auto column_max = [&] {
 #pragma unroll
-        for (int ct = 0; ct < 4; ++ct) {
+        for (int ct = 0; ct < CT; ++ct) {
             float big = 0.0f;
 #pragma unroll
             for (int i = 0; i < 2 * KW; ++i)
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             if constexpr (!STATE) fetch_c();
         } else fetch_x(c, lg);
         // x's operands
-        {
+        if (CT == 4 || w < CT) {
             const int here = min(L, s.T - c * L);
             const bool whole = here == L;
             float x[2][8], big = 0.0f;
@@ -524,11 +525,11 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
         if constexpr (!AHEAD && !STATE) fetch_c();
         // this wave's part of the state
         if constexpr (!STATE) {
-            f4v parts[4];
+            f4v parts[CT];
 #pragma unroll
-            for (int ct = 0; ct < 4; ++ct) parts[ct] = *reinterpret_cast<const f4v*>(hmax[16 * ct + n]);
+            for (int ct = 0; ct < CT; ++ct) parts[ct] = *reinterpret_cast<const f4v*>(hmax[16 * ct + n]);
 #pragma unroll
-            for (int ct = 0; ct < 4; ++ct) {
+            for (int ct = 0; ct < CT; ++ct) {
                 const int at = 16 * ct + n;
                 const float most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(parts[ct][0], parts[ct][1]), __builtin_elementwise_maximum(parts[ct][2], parts[ct][3]));
                 float up, down;
@@ -553,13 +554,13 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             if (c + 1 < to) fetch_x(c + 1, lg);
         if constexpr (!STATE) {
             // 16 rows of y: this lane row 16 w + n, columns 16 ct + 4 g .. + 3
-            f4v y[4], yi[4];
+            f4v y[CT], yi[CT];
 #pragma unroll
-            for (int ct = 0; ct < 4; ++ct) y[ct] = yi[ct] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int ct = 0; ct < CT; ++ct) y[ct] = yi[ct] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
 #pragma unroll
-                for (int ct = 0; ct < 4; ++ct) {
+                for (int ct = 0; ct < CT; ++ct) {
                     yi[ct] = mfma16<false>(hop[0][kk][ct][lane], cop[kk][0], yi[ct]);
                     if constexpr (Y3) {
                         yi[ct] = mfma16<false>(hop[HP - 1][kk][ct][lane], cop[kk][0], yi[ct]);
@@ -608,7 +609,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                 if constexpr (Y3) split8(m[ks], hi, lo);
                 else hi = half8(m[ks]);
 #pragma unroll
-                for (int ct = 0; ct < 4; ++ct) {
+                for (int ct = 0; ct < CT; ++ct) {
                     y[ct] = mfma16<false>(xop[XH][ks][ct][lane], hi, y[ct]);
                     if constexpr (Y3) {
                         y[ct] = mfma16<false>(xop[PLANES - 1][ks][ct][lane], hi, y[ct]);
@@ -622,7 +623,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             const int4 sp = *reinterpret_cast<const int4*>(spoilt);
             const bool finite = !__builtin_amdgcn_readfirstlane(sp.x | sp.y | sp.z | sp.w);
 #pragma unroll
-            for (int ct = 0; ct < 4; ++ct) {
+            for (int ct = 0; ct < CT; ++ct) {
                 const f4v f = *reinterpret_cast<const f4v*>(&xs[16 * ct + 4 * lg]), fi = *reinterpret_cast<const f4v*>(&hs[16 * ct + 4 * lg]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[ct][e] = fmaf(y[ct][e], f[e] * down, yi[ct][e] * (fi[e] * el));
@@ -630,7 +631,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             }
             if (!finite) {
 #pragma unroll
-                for (int ct = 0; ct < 4; ++ct)
+                for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (spoilt[ct] && row >= bad[16 * ct + 4 * lg + e]) y[ct][e] = __builtin_nanf("");
@@ -639,13 +640,13 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                 const int64_t at = (s.t0 + t) * p.ys + (int64_t) head * p.P + c0 + 4 * lg;
                 if (s.vec_y) {
 #pragma unroll
-                    for (int ct = 0; ct < 4; ++ct) {
+                    for (int ct = 0; ct < CT; ++ct) {
                         const float v[4] = {y[ct][0], y[ct][1], y[ct][2], y[ct][3]};
                         if (c0 + 16 * ct + 4 * lg < p.P) store_row<QT, 4>(p.y, at + 16 * ct, v);
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
+                    for (int i = 0; i < 4 * CT; ++i)
                         if (c0 + 16 * (i / 4) + 4 * lg + i % 4 < p.P) store_o<QT>(p.y, at + 16 * (i / 4) + i % 4, y[i / 4][i % 4]);
                 }
             }
@@ -658,9 +659,9 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             // (in registers of its own, that a product's first step starts from: the compiler would clear each sum apart)
             f4v zero = {0.0f, 0.0f, 0.0f, 0.0f};
             if constexpr (!STATE) asm volatile("" : "+v"(zero));
-            float fs[4];
+            float fs[CT];
 #pragma unroll
-            for (int ct = 0; ct < 4; ++ct) fs[ct] = xs[16 * ct + n];
+            for (int ct = 0; ct < CT; ++ct) fs[ct] = xs[16 * ct + n];
             auto operands = [&](int ct) {
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) ahead[ct % 2][ks][0] = xop[WH][ks][ct][lane], ahead[ct % 2][ks][1] = xop[WL][ks][ct][lane];
@@ -668,9 +669,9 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             // (a column tile ahead, but where four work-groups a CU hide the reads)
             if constexpr (!STATE) operands(0);
 #pragma unroll
-            for (int ct = 0; ct < 4; ++ct) {
+            for (int ct = 0; ct < CT; ++ct) {
                 if constexpr (STATE) operands(ct);
-                else if (ct < 3) operands(ct + 1);
+                else if (ct < CT - 1) operands(ct + 1);
                 f4v a[2 * KW];
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
@@ -702,14 +703,14 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
 #pragma unroll
         for (int i = 0; i < 2 * KW; ++i)
 #pragma unroll
-            for (int ct = 0; ct < 4; ++ct) dst[(i * 4 + ct) * 64] = st[i][ct];
+            for (int ct = 0; ct < CT; ++ct) dst[(i * CT + ct) * 64] = st[i][ct];
         if (tid == 0 && block == 0) s.segtot[(int64_t) seg * p.H + head] = exponent;
     } else {
         if (seg == s.segs - 1) {
 #pragma unroll
             for (int i = 0; i < 2 * KW; ++i)
 #pragma unroll
-                for (int ct = 0; ct < 4; ++ct) {
+                for (int ct = 0; ct < CT; ++ct) {
                     const int f = feature(i), cc = c0 + 16 * ct + n;
                     if (cc >= p.P || f >= p.N) continue;
                     float* dst = p.h1 + ((int64_t) head * p.P + cc) * p.N + f;
@@ -725,7 +726,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
         if (seg == 0 && s.t0 + s.T == s.all) {
             for (int64_t t = max((int64_t) 0, s.all - (p.K - 1)); t < s.all; ++t) {
                 float* dst = p.conv + (p.p0 + t) % p.cap * p.chan;
-                if (tid < 64 && c0 + tid < p.P) dst[head * p.P + c0 + tid] = load_q<QT>(p.xbc, t * p.xs + head * p.P + c0 + tid);
+                if (tid < 16 * CT && c0 + tid < p.P) dst[head * p.P + c0 + tid] = load_q<QT>(p.xbc, t * p.xs + head * p.P + c0 + tid);
                 if (in_group == 0)
                     for (int i = tid; i < 2 * p.N; i += 256) {
                         const int ch = p.H * p.P + (i / p.N * p.G + group) * p.N + i % p.N;
@@ -775,6 +776,16 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
     return q;
 }
 
+// column tiles of 16 a work-group: what a head's fewest work-groups of up to 4 share out evenly (128 heads of 80: 796 bfloat16 rows 57.3 us
+// with 3 tiles a work-group, 63.8 with 4; 64 heads of 32: 4096 rows 72.0 with 2, 96.0 with 4)
+template <int QT, int KW, bool STATE>
+void launch_scan(ns_gpu* g, const ScanParams& s, unsigned blocks) {
+    const int tiles = ((s.l.P + 15) / 16 + s.blocks - 1) / s.blocks;
+    if (tiles <= 2) ssm_scan_kernel<QT, KW, 2, STATE><<<blocks, 256, 0, g->q>>>(s);
+    else if (tiles == 3) ssm_scan_kernel<QT, KW, 3, STATE><<<blocks, 256, 0, g->q>>>(s);
+    else ssm_scan_kernel<QT, KW, 4, STATE><<<blocks, 256, 0, g->q>>>(s);
+}
+
 template <int QT, int KW>
 void launch_pass(ns_gpu* g, ScanParams& s, const Plan& q) {
     const int64_t waves = (int64_t) q.chunks * s.l.H + (s.t0 ? 0 : (3 * (int64_t) s.l.H * s.l.P + 63) / 64);
@@ -783,9 +794,9 @@ void launch_pass(ns_gpu* g, ScanParams& s, const Plan& q) {
     if (q.segs > 1) {
         ScanParams f = s;
         f.segs = (q.segs - 1) * q.sub;      // (the last segment's state is the scan's own)
-        ssm_scan_kernel<QT, KW, true><<<owners * f.segs, 256, 0, g->q>>>(f);
+        launch_scan<QT, KW, true>(g, f, owners * f.segs);
     }
-    ssm_scan_kernel<QT, KW, false><<<owners * q.segs, 256, 0, g->q>>>(s);
+    launch_scan<QT, KW, false>(g, s, owners * q.segs);
 }
 
 template <int QT>
