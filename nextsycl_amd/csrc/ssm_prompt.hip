@@ -355,6 +355,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     const int64_t row_bytes = p.xs * (QT ? 2 : 4);
     const uint32_t lane_off = (uint32_t) (4 * g * row_bytes + (int64_t) xch * (QT ? 2 : 4));
     auto fetch_x = [&](int c, int g) {
+        if (AHEAD && CT < 4 && w >= CT) return;           // (without AHEAD the branch costs more registers than the loads)
         const int here = min(L, s.T - c * L);
         const int64_t first = s.t0 + (int64_t) c * L;
         // as a buffer of its own, from the first row of the chunk that there is in front of its first: a lane's offset in a vector
@@ -777,7 +778,7 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
 }
 
 // column tiles of 16 a work-group: what a head's fewest work-groups of up to 4 share out evenly (128 heads of 80: 796 bfloat16 rows 57.3 us
-// with 3 tiles a work-group, 63.8 with 4; 64 heads of 32: 4096 rows 72.0 with 2, 96.0 with 4)
+// with 3 tiles a work-group, 63.8 with 4; 64 heads of 32: 4096 rows 68.8 with 2, 96.0 with 4)
 template <int QT, int KW, bool STATE>
 void launch_scan(ns_gpu* g, const ScanParams& s, unsigned blocks) {
     const int tiles = ((s.l.P + 15) / 16 + s.blocks - 1) / s.blocks;
