@@ -23,15 +23,8 @@ __device__ __forceinline__ void load_row(const void* p, int64_t i, float (&v)[VE
             v[j] = a.x, v[j + 1] = a.y, v[j + 2] = a.z, v[j + 3] = a.w;
         }
     } else {
-        uint32_t w[VEC / 2];
-        const uint16_t* s = static_cast<const uint16_t*>(p) + i;
-        if constexpr (VEC == 8) {
-            const piece4_t a = *reinterpret_cast<const piece4_t*>(s);
-            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-        } else {
-            const piece2_t a = *reinterpret_cast<const piece2_t*>(s);
-            w[0] = a.x, w[1] = a.y;
-        }
+        static_assert(VEC == 8);
+        const piece4_t w = *reinterpret_cast<const piece4_t*>(static_cast<const uint16_t*>(p) + i);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             const uint16_t b = (uint16_t) (j % 2 ? w[j / 2] >> 16 : w[j / 2]);
@@ -82,23 +75,14 @@ __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log
 // way out stay in flight across it (a __syncthreads waits for both)
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// the sum over each run of L lanes (L a power of two up to 64), in every lane of the run: the run's halves first, then theirs
+// the sum over each run of L lanes (4, 8 or 16), in every lane of the run: the run's halves first, then theirs
 template <int L>
 __device__ __forceinline__ float lanes_sum(float v) {
     auto add = [&](auto c) { v += __builtin_bit_cast(float, dpp_u32<decltype(c)::value>(__builtin_bit_cast(uint32_t, v))); };
-    float a, b;
-    if constexpr (L >= 64) {
-        pair32(v, a, b);
-        v = a + b;
-    }
-    if constexpr (L >= 32) {
-        pair16(v, a, b);
-        v = a + b;
-    }
     if constexpr (L >= 16) add(std::integral_constant<int, 0x140>());
     if constexpr (L >= 8) add(std::integral_constant<int, 0x141>());
-    if constexpr (L >= 4) add(std::integral_constant<int, 0x4E>());
-    if constexpr (L >= 2) add(std::integral_constant<int, 0xB1>());
+    add(std::integral_constant<int, 0x4E>());
+    add(std::integral_constant<int, 0xB1>());
     return v;
 }
 

@@ -40,7 +40,8 @@ __device__ __forceinline__ float lanes_sums(const float (&v)[U], int lane) {
             } else {
                 const bool upper = lane & LR / 2;
                 const float mine = upper ? b : a, other = upper ? a : b;
-                w[u] = mine + __builtin_bit_cast(float, dpp_u32<LR == 16 ? 0x140 : LR == 8 ? 0x141 : 0x4E>(__builtin_bit_cast(uint32_t, other)));
+                static_assert(LR == 16 || LR == 8);
+                w[u] = mine + __builtin_bit_cast(float, dpp_u32<LR == 16 ? 0x140 : 0x141>(__builtin_bit_cast(uint32_t, other)));
             }
         }
         return lanes_sums<LR / 2, U / 2>(w, lane);

@@ -97,7 +97,8 @@ def test_norm_residual(ops, qt, rt, T, D, pad):
         slack = U32 * (n + 6) * (np.abs(v) + np.abs(hv)) + ROUND[rt] * np.abs(ref) + TINY[rt]
         assert (err <= slack).all()
         err = np.abs(from_type(qt, np.ascontiguousarray(go[:, :D])) - out)
-        most = (np.abs(v) + np.abs(hv)) * (np.abs(out) / np.maximum(np.abs(ref), 1e-300))
+        # (the sum's error times what the norm multiplies it with: |out / ref|, and the same number where the sum is 0 and that is 0 / 0)
+        most = (np.abs(v) + np.abs(hv)) * (1.0 if pre is None else np.abs(pre)) / np.sqrt((ref * ref).mean(-1, keepdims=True) + eps)
         assert (err <= U32 * 2 * (n + 8) * most + ROUND[qt] * np.abs(out) + TINY[qt] + U32 * np.abs(out) * n).all()
         for a in (gs, go):
             assert (np.ascontiguousarray(a[:, D:]).view(np.uint8) == 0xFF).all()
@@ -412,3 +413,22 @@ def test_a_q4_products_row_alone_and_among_others(ops, qt, group, M, K):
         got = y.read(np.uint8)
         whole = got if whole is None else whole
         assert np.array_equal(got, whole), n
+
+
+# lengths about a wave's and a work-group's pieces of 4 and 8 values, whole and not, at every alignment of a row
+RAGGED = [63, 65, 67, 253, 257, 509, 513, 4093, 4097, 8191, 8193, 16385, 16387, 32769]
+
+
+@pytest.mark.parametrize("qt", TYPES)
+@pytest.mark.parametrize("W", RAGGED)
+def test_norms_of_ragged_rows(ops, qt, W):
+    for order, (T, groups, py, pz, po) in enumerate([(2, 3, 1, 0, 3), (3, 1, 0, 2, 1)]):
+        test_norm_gated(ops, qt, order, T, W * groups, groups, py, pz, po)
+    test_norm_residual(ops, qt, F32, 2, W, 1)
+    test_norm_residual(ops, qt, qt, 3, W, 0)
+
+
+@pytest.mark.parametrize("qt", TYPES)
+@pytest.mark.parametrize("M,K,T,px,py", [(48, 257, 7, 0, 1), (4112, 1843, 3, 0, 0), (17, 8191, 16, 3, 0), (5, 9, 2, 0, 0)])
+def test_q4_product_of_ragged_rows(ops, qt, M, K, T, px, py):
+    test_q4_product(ops, qt, 64, M, K, T, px, py)
