@@ -13,7 +13,7 @@
 // [row] - an operand's rows are a thread's own, C's come back through transposing reads - and multiplies them; the work-groups
 // behind sum the exponents (in 64 bits; what the exponentials see is a difference within 16 rows, plus one between such runs).
 // ssm_scan_kernel, a work-group a (head, up to 64 of its features, segment of the prompt): walks its chunks with the state in
-// the accumulators of 4 waves, wave w rows 32 w .. 32 w + 31 of it. In a chunk wave w convolves 16 columns of x into the
+// the accumulators of 4 waves, a quarter of its features each (wave w 32 w .. 32 w + 31 of 128). In a chunk wave w convolves 16 columns of x into the
 // operands that all read (LDS), splits its part of the state into another, then takes 16 rows of y and its part of h'. Matrix
 // results come as (column, 4 consecutive rows) a lane, operands go in as (row or column, 8 values of the summed index) a
 // lane; the summed index may come in any order that both sides share, so in runs of 4 of two neighbouring tiles a result
@@ -146,9 +146,11 @@ __device__ __forceinline__ void ssm_header(const ScanParams& s, int chunk, int h
     if (lane < 3) to[HDR_END + lane] = lane == 0 ? (float) end : lane == 1 ? exp2f((float) end) : __builtin_bit_cast(float, (uint32_t) (e + 1) << 23);
 }
 
-template <int QT, int KW>
-__global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
-    constexpr int NP = 128 * KW, KK = 4 * KW, ROW = L + 4;     // (34 words: a column of LDS banks on for each feature)
+// KT: tiles of 16 features that each of 4 waves of the scan holds: 1 up to 64 features, 2 up to 128, 4 up to 256 (4096 bfloat16 rows of 80 heads of
+// 64 x 64 110.8 us with 1, 140.6 with 2)
+template <int QT, int KT>
+__global__ __launch_bounds__(512, KT == 4 ? 1 : 2) void ssm_prep_kernel(ScanParams s) {
+    constexpr int KW = KT == 4 ? 2 : 1, NP = 128 * KW, KK = 2 * KT, ROW = L + 4;     // (34 words: a column of LDS banks on for each feature)
     __shared__ __align__(16) short plane[2][2][NP * ROW];      // [B, C][hi, lo][feature][row]
     __shared__ float part[2][8];
     const SsmLayer& p = s.l;
@@ -225,7 +227,7 @@ __global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
                 *reinterpret_cast<s4v*>(plane[isc][0] + at) = s4v{hi[i], hi[i + 1], hi[i + 2], hi[i + 3]};
                 *reinterpret_cast<s4v*>(plane[isc][1] + at) = s4v{lo[i], lo[i + 1], lo[i + 2], lo[i + 3]};
             }
-            if (!isc) {
+            if (!isc && (KT > 1 || n < 64)) {
                 s8v* to = reinterpret_cast<s8v*>(ops + 2 * op_c(KK)) + ((n / 16) * 2 + half) * 64 + n % 16 + 16 * q;
                 to[0] = hi;
                 to[op_c(KK) / 16] = lo;
@@ -259,12 +261,12 @@ __global__ __launch_bounds__(512, 3 - KW) void ssm_prep_kernel(ScanParams s) {
 }
 
 // work-groups a CU: what LDS has room for, and the registers that leaves a wave
-template <int QT, int KW, bool STATE>
-constexpr int SCAN_WGS = KW == 2 ? 1 : STATE || QT == 2 ? 3 : 2;
-template <int QT, int KW, int CT, bool STATE>
-__global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kernel(ScanParams s) {
-    constexpr int KK = 4 * KW;
-    constexpr bool AHEAD = STATE || SCAN_WGS<QT, KW, STATE> <= 2;     // x and the operands asked for early, where there are registers for them
+template <int QT, int KT, bool STATE>
+constexpr int SCAN_WGS = KT == 4 ? 1 : STATE || QT == 2 ? 3 : 2;
+template <int QT, int KT, int CT, bool STATE>
+__global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kernel(ScanParams s) {
+    constexpr int KK = 2 * KT;
+    constexpr bool AHEAD = STATE || SCAN_WGS<QT, KT, STATE> <= 2;     // x and the operands asked for early, where there are registers for them
     constexpr bool Y3 = QT != 2;                                  // y's products from both halfs of their operands
     // x weighted for the state (hi, lo) and as it is (hi, for Y3 lo): [32 rows][16 columns][lane]; the state: [32 features][..]
     constexpr int WH = 0, WL = 1, XH = 2, XL = 3, PLANES = STATE ? 2 : Y3 ? 4 : 3, HP = STATE ? 0 : Y3 ? 2 : 1;
@@ -296,15 +298,15 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     const int to = min(s.chunks, STATE ? min(from + s.piece, (seg / s.sub + 1) * s.per) : from + s.per);
     const int64_t owner = (int64_t) head * s.blocks + block, owners = (int64_t) p.H * s.blocks;
 
-    // features 32 (w KW + i / 2) + 16 (i % 2) + 4 g .. + 3 of column 16 ct + n
-    f4v st[2 * KW][CT];
-    auto feature = [&](int i) { return 32 * (w * KW + i / 2) + 16 * (i % 2) + 4 * g; };
-    auto kept = [&](int slot) { return reinterpret_cast<f4v*>(s.segst) + ((slot * owners + owner) * 4 + w) * (2 * KW * CT * 64) + lane; };
+    // features 16 (w KT + i) + 4 g .. + 3 of column 16 ct + n
+    f4v st[KT][CT];
+    auto feature = [&](int i) { return 16 * (w * KT + i) + 4 * g; };
+    auto kept = [&](int slot) { return reinterpret_cast<f4v*>(s.segst) + ((slot * owners + owner) * 4 + w) * (KT * CT * 64) + lane; };
     // (a cut pass's first state is read from where the state kernel has put it: the last segment may write h1 = h0 meanwhile)
     if (STATE ? seg == 0 : s.segs == 1) {
         const float* h0 = s.t0 ? p.h1 : p.h0;
 #pragma unroll
-        for (int i = 0; i < 2 * KW; ++i)
+        for (int i = 0; i < KT; ++i)
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
                 f4v v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -324,14 +326,14 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     } else {
         const f4v* src = kept(seg > 0 && !STATE);
 #pragma unroll
-        for (int i = 0; i < 2 * KW; ++i)
+        for (int i = 0; i < KT; ++i)
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) st[i][ct] = STATE ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : src[(i * CT + ct) * 64];
         for (int r = 1; !STATE && r < seg * s.sub; ++r) {
             const float keep = exp2f(s.segtot[(int64_t) r * p.H + head]);
             const f4v* add = kept(1 + r);
 #pragma unroll
-            for (int i = 0; i < 2 * KW; ++i)
+            for (int i = 0; i < KT; ++i)
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) st[i][ct] = st[i][ct] * keep + add[(i * CT + ct) * 64];
         }
@@ -386,7 +388,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
         for (int ct = 0; ct < CT; ++ct) {
             float big = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2 * KW; ++i)
+            for (int i = 0; i < KT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) big = __builtin_elementwise_maximum(big, fabsf(st[i][ct][e]));
             big = rows_most(big);
@@ -409,16 +411,16 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
         asm volatile("" : "+v"(ln), "+v"(lg));
         fetch_header(c + 1);
         // this chunk's operands, on their way while x and the state become theirs
-        s8v bop[2 * KW][2][2], cop[STATE ? 1 : KK][2];
+        s8v bop[KT][2][2], cop[STATE ? 1 : KK][2];
         f4v cbv[2][2];
         auto fetch_b = [&] {
             const s8v* b = reinterpret_cast<const s8v*>(ops + 2 * op_c(KK)) + lane;
 #pragma unroll
-            for (int i = 0; i < 2 * KW; ++i)
+            for (int i = 0; i < KT; ++i)
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) bop[i][ks][h] = b[((w * 2 * KW + i) * 2 + ks) * 64 + h * (op_c(KK) / 16)];
+                    for (int h = 0; h < 2; ++h) bop[i][ks][h] = b[((w * KT + i) * 2 + ks) * 64 + h * (op_c(KK) / 16)];
         };
         auto fetch_c = [&] {
             const s8v* cp = reinterpret_cast<const s8v*>(ops) + w * KK * 64 + lane;
@@ -536,17 +538,27 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
                 float up, down;
                 to_half_range(most, up, down);
                 if (w == 0 && g == 0) hs[at] = down;
+                if constexpr (KT == 1) {
+                    // (half an operand: its neighbour's tile is the other)
+                    const float v[8] = {st[0][ct][0] * up, st[0][ct][1] * up, st[0][ct][2] * up, st[0][ct][3] * up, 0.0f, 0.0f, 0.0f, 0.0f};
+                    s8v hi, lo;
+                    if constexpr (Y3) {
+                        split8(v, hi, lo);
+                        reinterpret_cast<s4v*>(&hop[1][w / 2][ct][lane])[w % 2] = s4v{lo[0], lo[1], lo[2], lo[3]};
+                    } else hi = half8(v);
+                    reinterpret_cast<s4v*>(&hop[0][w / 2][ct][lane])[w % 2] = s4v{hi[0], hi[1], hi[2], hi[3]};
+                }
 #pragma unroll
-                for (int j = 0; j < KW; ++j) {
+                for (int j = 0; j < KT / 2; ++j) {
                     float v[8];
                     s8v hi, lo;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = st[2 * j + i / 4][ct][i % 4] * up;
                     if constexpr (Y3) {
                         split8(v, hi, lo);
-                        hop[1][w * KW + j][ct][lane] = lo;
+                        hop[1][w * (KT / 2) + j][ct][lane] = lo;
                     } else hi = half8(v);
-                    hop[0][w * KW + j][ct][lane] = hi;
+                    hop[0][w * (KT / 2) + j][ct][lane] = hi;
                 }
             }
         }
@@ -673,20 +685,20 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
             for (int ct = 0; ct < CT; ++ct) {
                 if constexpr (STATE) operands(ct);
                 else if (ct < CT - 1) operands(ct + 1);
-                f4v a[2 * KW];
+                f4v a[KT];
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     const s8v hi = ahead[ct % 2][ks][0], lo = ahead[ct % 2][ks][1];
 #pragma unroll
-                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][0], hi, ks ? a[i] : zero);
+                    for (int i = 0; i < KT; ++i) a[i] = mfma16<false>(bop[i][ks][0], hi, ks ? a[i] : zero);
 #pragma unroll
-                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][1], hi, a[i]);
+                    for (int i = 0; i < KT; ++i) a[i] = mfma16<false>(bop[i][ks][1], hi, a[i]);
 #pragma unroll
-                    for (int i = 0; i < 2 * KW; ++i) a[i] = mfma16<false>(bop[i][ks][0], lo, a[i]);
+                    for (int i = 0; i < KT; ++i) a[i] = mfma16<false>(bop[i][ks][0], lo, a[i]);
                 }
                 const float f = sb * fs[ct];
 #pragma unroll
-                for (int i = 0; i < 2 * KW; ++i) {
+                for (int i = 0; i < KT; ++i) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) st[i][ct][e] = fmaf(st[i][ct][e], keep, a[i][e] * f);
                     // (here: the compiler would ask for all columns' operands at once)
@@ -702,14 +714,14 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KW, STATE>)) void ssm_scan_kerne
     if constexpr (STATE) {
         f4v* dst = kept(1 + seg);
 #pragma unroll
-        for (int i = 0; i < 2 * KW; ++i)
+        for (int i = 0; i < KT; ++i)
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) dst[(i * CT + ct) * 64] = st[i][ct];
         if (tid == 0 && block == 0) s.segtot[(int64_t) seg * p.H + head] = exponent;
     } else {
         if (seg == s.segs - 1) {
 #pragma unroll
-            for (int i = 0; i < 2 * KW; ++i)
+            for (int i = 0; i < KT; ++i)
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) {
                     const int f = feature(i), cc = c0 + 16 * ct + n;
@@ -745,7 +757,7 @@ struct Plan {
 };
 Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
     Plan q{};
-    q.kk = N <= 128 ? 4 : 8;
+    q.kk = N <= 64 ? 2 : N <= 128 ? 4 : 8;
     q.chunks = (int) ((T + L - 1) / L);
     q.blocks = (int) ((P + 63) / 64);
     const int64_t owners = H * q.blocks;
@@ -779,39 +791,40 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
 
 // column tiles of 16 a work-group: what a head's fewest work-groups of up to 4 share out evenly (128 heads of 80: 796 bfloat16 rows 57.3 us
 // with 3 tiles a work-group, 63.8 with 4; 64 heads of 32: 4096 rows 68.8 with 2, 96.0 with 4)
-template <int QT, int KW, bool STATE>
+template <int QT, int KT, bool STATE>
 void launch_scan(ns_gpu* g, const ScanParams& s, unsigned blocks) {
     const int tiles = ((s.l.P + 15) / 16 + s.blocks - 1) / s.blocks;
-    if (tiles <= 2) ssm_scan_kernel<QT, KW, 2, STATE><<<blocks, 256, 0, g->q>>>(s);
-    else if (tiles == 3) ssm_scan_kernel<QT, KW, 3, STATE><<<blocks, 256, 0, g->q>>>(s);
-    else ssm_scan_kernel<QT, KW, 4, STATE><<<blocks, 256, 0, g->q>>>(s);
+    if (tiles <= 2) ssm_scan_kernel<QT, KT, 2, STATE><<<blocks, 256, 0, g->q>>>(s);
+    else if (tiles == 3) ssm_scan_kernel<QT, KT, 3, STATE><<<blocks, 256, 0, g->q>>>(s);
+    else ssm_scan_kernel<QT, KT, 4, STATE><<<blocks, 256, 0, g->q>>>(s);
 }
 
-template <int QT, int KW>
+template <int QT, int KT>
 void launch_pass(ns_gpu* g, ScanParams& s, const Plan& q) {
     const int64_t waves = (int64_t) q.chunks * s.l.H + (s.t0 ? 0 : (3 * (int64_t) s.l.H * s.l.P + 63) / 64);
-    ssm_prep_kernel<QT, KW><<<(unsigned) (q.chunks * s.l.G + (waves + 7) / 8), 512, 0, g->q>>>(s);
+    ssm_prep_kernel<QT, KT><<<(unsigned) (q.chunks * s.l.G + (waves + 7) / 8), 512, 0, g->q>>>(s);
     const unsigned owners = (unsigned) (s.l.H * q.blocks);
     if (q.segs > 1) {
         ScanParams f = s;
         f.segs = (q.segs - 1) * q.sub;      // (the last segment's state is the scan's own)
-        launch_scan<QT, KW, true>(g, f, owners * f.segs);
+        launch_scan<QT, KT, true>(g, f, owners * f.segs);
     }
-    launch_scan<QT, KW, false>(g, s, owners * q.segs);
+    launch_scan<QT, KT, false>(g, s, owners * q.segs);
 }
 
 template <int QT>
 void run_prompt(ns_gpu* g, const SsmLayer& p, int64_t T, float* scratch) {
     for (int64_t t0 = 0; t0 < T; t0 += PASS_ROWS) {
         const int64_t n = std::min(PASS_ROWS, T - t0);
-        const Plan q = plan_of(n, p.H, p.P, p.N, p.G, p.N <= 128 ? SCAN_WGS<QT, 1, false> : SCAN_WGS<QT, 2, false>);
+        const Plan q = plan_of(n, p.H, p.P, p.N, p.G, p.N <= 128 ? SCAN_WGS<QT, 2, false> : SCAN_WGS<QT, 4, false>);
         ScanParams s{p, t0, T, p.p0 % p.cap, (int) n, q.chunks, q.segs, q.per, q.sub, q.piece, q.blocks};
         s.vec_y = p.P % 4 == 0;
         s.vec_h = p.N % 4 == 0 && (uintptr_t) p.h0 % 16 == 0 && (uintptr_t) p.h1 % 16 == 0;
         s.ops = reinterpret_cast<uint8_t*>(scratch + q.ops);
         s.scales = scratch + q.scales, s.hdr = scratch + q.hdr, s.hist = scratch + q.hist, s.segst = scratch + q.segst, s.segtot = scratch + q.segtot;
-        if (q.kk == 4) launch_pass<QT, 1>(g, s, q);
-        else launch_pass<QT, 2>(g, s, q);
+        if (q.kk == 2) launch_pass<QT, 1>(g, s, q);
+        else if (q.kk == 4) launch_pass<QT, 2>(g, s, q);
+        else launch_pass<QT, 4>(g, s, q);
     }
 }
 
