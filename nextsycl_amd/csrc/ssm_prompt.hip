@@ -11,7 +11,7 @@
 //
 // ssm_prep_kernel, 8 waves a (chunk, group): convolves B and C (a thread half a channel's rows), leaves them in LDS as [feature]
 // [row] - an operand's rows are a thread's own, C's come back through transposing reads - and multiplies them; the work-groups
-// behind sum the exponents (in 64 bits; what the exponentials see is a difference within 16 rows, plus one between such runs).
+// behind sum the exponents (ssm_header).
 // ssm_scan_kernel, a work-group a (head, up to 64 of its features, segment of the prompt): walks its chunks with the state in
 // the accumulators of 4 waves, a quarter of its features each (wave w 32 w .. 32 w + 31 of 128). In a chunk wave w convolves 16 columns of x into the
 // operands that all read (LDS), splits its part of the state into another, then takes 16 rows of y and its part of h'. Matrix
@@ -46,10 +46,15 @@ constexpr int MOST_SEGS = 32;
 // up to these row by row, as steps (128 heads of 64 x 128: 1 row 6.4 us and 17.5 as a chunk, 8 9.2 and 18.2, 16 14.5 and 18.2, 24 19.6
 // and 18.4; of 80 x 128 16 17.5 and 18.2)
 constexpr int64_t FEW_ROWS = 16;
-// a chunk and head's header: exponents (base 2) from the start of each run of 16 rows, step sizes, weights in the chunk's
-// state, decays from the chunk's start; differences between runs' starts [4][4], the whole chunk's exponent and decay, what the weights are
-// to be multiplied with
-constexpr int HDR_C = 0, HDR_DT = 64, HDR_W = 128, HDR_E = 192, HDR_BD = 256, HDR_END = 272, HDR = 288;
+// a chunk and head's header, exponents base 2. Rows' exponents from their run of 16's start, step sizes, weights in the chunk's state, decays from the
+// chunk's start; exponents between a run's end and a later one's start [later][run], the whole chunk's exponent and decay, what the weights
+// are to be multiplied with (the states' kernel reads up to here); rows' own exponents, to their run's end, from their quarter of the run's
+// start. All are sums of rows' exponents, which have one sign, and an exponent between two rows is the sum of those that lie between the two:
+// none is larger than what it enters. (As differences of 64-bit sums that floats held from a run's start, rows behind a step of 50 lost 9 of
+// their decays' bits. 2051 float32 rows 72.8 us so, 74.6 now, 8192 bfloat16 rows 293 and 298)
+constexpr int HDR_L = 0, HDR_DT = 64, HDR_W = 128, HDR_E = 192, HDR_BD = 256, HDR_END = 272, HDR_STATE = 288, HDR_A = 288, HDR_R = 352, HDR_Q = 416, HDR = 480;
+// a row's exponent is held to these: 2 to it is 0 or infinite in 32 bits, a chunk's sums are finite
+constexpr double MOST_EXPONENT = 4096.0;
 
 // bytes of a chunk and group's operands: C (hi, lo), B (hi, lo) of KK = padded N / 32 steps, C . B as float32
 constexpr int64_t op_c(int kk) { return (int64_t) 4 * kk * 1024; }
@@ -124,26 +129,47 @@ __device__ __forceinline__ void ssm_header(const ScanParams& s, int chunk, int h
     const SsmLayer& p = s.l;
     const int t = chunk * L + lane;
     const float dt = t < s.T ? ssm_dt(p, load_q<QT>(p.dt, (s.t0 + t) * p.dts + head) + (p.dtb ? p.dtb[head] : 0.0f)) : 0.0f;
-    const double add = (double) dt * (double) p.a[head] * 1.4426950408889634074;
-    double cum = add;
+    const double own = (double) dt * (double) p.a[head] * 1.4426950408889634074;
+    const float add = (float) (own < -MOST_EXPONENT ? -MOST_EXPONENT : own > MOST_EXPONENT ? MOST_EXPONENT : own);       // (a NaN stays one)
+    // its sums with the rows in front of it in its quarter of its run of 16, in its run, and of the rows behind it in its run (0x110 + n: the value of
+    // n lanes in front within 16, 0x100 + n: behind; 0 where there is none)
+    auto of = [](auto at, float v) { return __builtin_bit_cast(float, dpp_u32<decltype(at)::value>(__builtin_bit_cast(uint32_t, v))); };
+    using std::integral_constant;
+    const float add1 = of(integral_constant<int, 0x111>(), add);
+    float quarter = add + (lane % 4 > 0 ? add1 : 0.0f), run = add + add1, behind = of(integral_constant<int, 0x101>(), add);
+    const float quarter2 = of(integral_constant<int, 0x112>(), quarter);
+    quarter += lane % 4 > 1 ? quarter2 : 0.0f;
+    run += of(integral_constant<int, 0x112>(), run);
+    run += of(integral_constant<int, 0x114>(), run);
+    run += of(integral_constant<int, 0x118>(), run);
+    behind += of(integral_constant<int, 0x101>(), behind);
+    behind += of(integral_constant<int, 0x102>(), behind);
+    behind += of(integral_constant<int, 0x104>(), behind);
+    behind += of(integral_constant<int, 0x108>(), behind);
+    // the runs' own
+    float whole[4];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double b = __shfl_up(cum, o);
-        if (lane >= o) cum += b;
-    }
-    const double end = __shfl(cum, 63), base = __shfl(cum - add, lane / 16 * 16);
+    for (int k = 0; k < 4; ++k) whole[k] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, run), 16 * k + 15));
+    auto runs = [&](int first, int last) {       // of runs first .. last
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v += k >= first && k <= last ? whole[k] : 0.0f;
+        return v;
+    };
+    const float end = runs(0, 3), between = runs(lane % 4 + 1, lane % 16 / 4 - 1);
     float* to = s.hdr + ((int64_t) chunk * p.H + head) * HDR;
-    to[HDR_C + lane] = (float) (cum - base);
     to[HDR_DT + lane] = dt;
+    to[HDR_E + lane] = exp2f(run + runs(0, lane / 16 - 1));
+    to[HDR_A + lane] = add;
+    to[HDR_L + lane] = run;
+    to[HDR_R + lane] = behind;
+    to[HDR_Q + lane] = quarter;
     // (the weights times a power of two that puts the largest between 1/2 and 1: they enter operands)
-    const float weight = exp2f((float) (end - cum)) * dt, most = wave_max(weight);
+    const float weight = exp2f(behind + runs(lane / 16 + 1, 3)) * dt, most = wave_max(weight);
     const int e = min(max((int) (__builtin_bit_cast(uint32_t, most) >> 23 & 255), 1), 252);
     to[HDR_W + lane] = weight * __builtin_bit_cast(float, (uint32_t) (253 - e) << 23);
-    to[HDR_E + lane] = exp2f((float) cum);
-    // starts of run lane / 4 and lane % 4 of 16
-    const double from = __shfl(cum - add, lane % 16 / 4 * 16), of = __shfl(cum - add, lane % 4 * 16);
-    if (lane < 16) to[HDR_BD + lane] = (float) (from - of);
-    if (lane < 3) to[HDR_END + lane] = lane == 0 ? (float) end : lane == 1 ? exp2f((float) end) : __builtin_bit_cast(float, (uint32_t) (e + 1) << 23);
+    if (lane < 16) to[HDR_BD + lane] = between;         // (run lane % 4, the later lane / 4)
+    if (lane < 3) to[HDR_END + lane] = lane == 0 ? end : lane == 1 ? exp2f(end) : __builtin_bit_cast(float, (uint32_t) (e + 1) << 23);
 }
 
 // KT: tiles of 16 features that each of 4 waves of the scan holds: 1 up to 64 features, 2 up to 128, 4 up to 256 (4096 bfloat16 rows of 80 heads of
@@ -274,7 +300,8 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kerne
     __shared__ __align__(16) s8v hop[HP + !HP][STATE ? 1 : KK][CT][64];
     __shared__ __align__(16) float xs[16 * CT], hs[16 * CT];                // what their results are to be multiplied with, a column
     __shared__ __align__(16) float hmax[16 * CT][4];                   // the largest of each wave's part of the state, a column
-    __shared__ __align__(16) float hdrs[2][HDR];
+    constexpr int HDRS = STATE ? HDR_STATE : HDR;
+    __shared__ __align__(16) float hdrs[2][HDRS];
     __shared__ int bad[16 * CT];
     __shared__ __align__(16) int spoilt[4];                       // a column's first row that is not finite; whether 16 columns have one
     const SsmLayer& p = s.l;
@@ -345,11 +372,11 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kerne
     auto fetch_header = [&](int c) {
         const float* hd = s.hdr + ((int64_t) min(c, s.chunks - 1) * p.H + head) * HDR;
         head0 = hd[tid];
-        head1 = hd[256 + tid % (HDR - 256)];
+        head1 = hd[256 + tid % (HDRS - 256)];
     };
     auto put_header = [&](int c) {
         hdrs[c % 2][tid] = head0;
-        if (tid < HDR - 256) hdrs[c % 2][256 + tid] = head1;
+        if (tid < HDRS - 256) hdrs[c % 2][256 + tid] = head1;
     };
     // (as they are loaded: widened to 32 bits they would be awaited at once)
     typedef std::conditional_t<QT == 0, uint32_t, uint16_t> raw_t;
@@ -566,6 +593,21 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kerne
         if constexpr (AHEAD)
             if (c + 1 < to) fetch_x(c + 1, lg);
         if constexpr (!STATE) {
+            const int row = 16 * w + ln;
+            // of rows of one run: those of s's quarter of it behind s, up to this row; then whole quarters; then this row's up to it
+            f4v in_run;
+            {
+                const f4v own = *reinterpret_cast<const f4v*>(hdr + HDR_A + 16 * w + 4 * lg);
+                const float* quarters = hdr + HDR_Q + 16 * w;
+                const float q1 = quarters[min(4 * lg + 7, 15)], q2 = quarters[min(4 * lg + 11, 15)], q = quarters[ln];
+                const int apart = ln / 4 - lg;
+                float past = (apart > 0 ? q : 0.0f) + ((apart > 1 ? q1 : 0.0f) + (apart > 2 ? q2 : 0.0f));
+#pragma unroll
+                for (int i = 3; i >= 0; --i) {
+                    in_run[i] = past;
+                    past += 4 * lg + i <= ln ? own[i] : 0.0f;
+                }
+            }
             // 16 rows of y: this lane row 16 w + n, columns 16 ct + 4 g .. + 3
             f4v y[CT], yi[CT];
 #pragma unroll
@@ -582,10 +624,8 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kerne
                 }
             }
             // the chunk's own rows: C . B decayed, d on the diagonal
-            const int row = 16 * w + ln;
-            const float cl = hdr[HDR_C + row];
+            const float cl = hdr[HDR_L + row];
             float m[2][8], big = 0.0f;
-            f4v cs[4], dts[4];
             const f4v bd = *reinterpret_cast<const f4v*>(hdr + HDR_BD + 4 * w);
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
@@ -595,12 +635,12 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kerne
                     for (int i = 0; i < 4; ++i) to_m[i] = 0.0f;
                     continue;
                 }
-                cs[st] = *reinterpret_cast<const f4v*>(hdr + HDR_C + 16 * st + 4 * lg);
-                dts[st] = *reinterpret_cast<const f4v*>(hdr + HDR_DT + 16 * st + 4 * lg);
-                const float base = cl + bd[st];
+                const f4v dts = *reinterpret_cast<const f4v*>(hdr + HDR_DT + 16 * st + 4 * lg);
+                // from s to its run's end, to this row's run's start, to this row
+                const f4v apart = *reinterpret_cast<const f4v*>(hdr + HDR_R + 16 * st + 4 * lg) + (cl + bd[st]), between = st < w ? apart : in_run;
                 const f4v cb = cbv[st / 2][st % 2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) to_m[i] = cb[i] * dts[st][i] * fast_exp2(base - cs[st][i]);
+                for (int i = 0; i < 4; ++i) to_m[i] = cb[i] * dts[i] * fast_exp2(between[i]);
                 if (st == w) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
