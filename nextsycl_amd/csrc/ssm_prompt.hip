@@ -211,15 +211,23 @@ __global__ __launch_bounds__(512, KT == 4 ? 1 : 2) void ssm_prep_kernel(ScanPara
             else a0 = ring_row(s, -3, ch), a1 = ring_row(s, -2, ch), a2 = ring_row(s, -1, ch);      // (first is 0)
 #pragma unroll
             for (int t = 0; t < L / 2; ++t) v[t] = row(r0 + t);
+            auto convolve = [&](auto all) {
+                // (FEW taps: of those that there are not 0, as 0 times what is not finite is not)
+                constexpr bool FEW = !decltype(all)::value;
+                if (FEW) a0 = 0.0f, a1 = p.K > 2 ? a1 : 0.0f, a2 = p.K > 1 ? a2 : 0.0f;
 #pragma unroll
-            for (int t = 0; t < L / 2; ++t) {
-                const float a3 = v[t];
-                const float c = silu(fmaf(w3, a3, fmaf(w2, a2, fmaf(w1, a1, fmaf(w0, a0, b)))));
-                a0 = a1, a1 = a2, a2 = a3;
-                v[t] = r0 + t < here ? c : 0.0f;
-                // (what is not finite has no part in the scale: it would leave the other rows' values none)
-                big = fabsf(v[t]) < __builtin_inff() ? fmaxf(big, fabsf(v[t])) : big;
-            }
+                for (int t = 0; t < L / 2; ++t) {
+                    const float a3 = v[t];
+                    const float c = silu(fmaf(w3, a3, fmaf(w2, a2, fmaf(w1, a1, fmaf(w0, a0, b)))));
+                    if (FEW) a1 = p.K > 2 ? a2 : 0.0f, a2 = p.K > 1 ? a3 : 0.0f;
+                    else a0 = a1, a1 = a2, a2 = a3;
+                    v[t] = r0 + t < here ? c : 0.0f;
+                    // (what is not finite has no part in the scale: it would leave the other rows' values none)
+                    big = fabsf(v[t]) < __builtin_inff() ? fmaxf(big, fabsf(v[t])) : big;
+                }
+            };
+            if (p.K == 4) convolve(std::true_type());
+            else convolve(std::false_type());
         } else {
 #pragma unroll
             for (int t = 0; t < L / 2; ++t) v[t] = 0.0f;
@@ -316,7 +324,8 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kerne
     const int col = c0 + 16 * w + n;                              // the column of x this lane convolves
     const bool has = (CT == 4 || w < CT) && col < p.P;            // (fewer column tiles than waves: the last have none)
     const int xch = head * p.P + (has ? col : 0);
-    // (the taps times log2 e: x comes out times it too, which its operand's scale takes back, and the exponential takes it as it is)
+    // (the taps times log2 e: x comes out times it too, which its operand's scale takes back, and the exponential takes it as it is; a tap that
+    // there is not is 0 times what is not finite for rows whose column that has already ended)
     constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
     const float w0 = ssm_tap(p, xch, 0) * LOG2E, w1 = ssm_tap(p, xch, 1) * LOG2E, w2 = ssm_tap(p, xch, 2) * LOG2E, w3 = ssm_tap(p, xch, 3) * LOG2E;
     const float bias = p.cb ? p.cb[xch] * LOG2E : 0.0f;

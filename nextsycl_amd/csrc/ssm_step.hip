@@ -172,7 +172,8 @@ __global__ __launch_bounds__(256, VEC ? 4 : 3) void ssm_step_kernel(StepParams s
                 if (to[j] < 0) continue;
                 const float v = raw[a][j];
                 row_in[a][to[j]] = ch[j] >= 0 ? silu(fmaf(w4[j][3], v, fmaf(w4[j][2], past[j][2], fmaf(w4[j][1], past[j][1], fmaf(w4[j][0], past[j][0], bias[j]))))) : 0.0f;
-                past[j][0] = past[j][1], past[j][1] = past[j][2], past[j][2] = v;
+                // (of taps that there are not: 0 times what is not finite is not 0)
+                past[j][0] = p.K > 3 ? past[j][1] : 0.0f, past[j][1] = p.K > 2 ? past[j][2] : 0.0f, past[j][2] = p.K > 1 ? v : 0.0f;
                 if (keep[j] && i0 + a >= kept_from) ring[(int64_t) here * p.chan + ch[j]] = v;
             }
             here = here + 1 == cap ? 0 : here + 1;
