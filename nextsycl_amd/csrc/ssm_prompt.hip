@@ -165,7 +165,7 @@ __device__ __forceinline__ void ssm_header(const ScanParams& s, int chunk, int h
     to[HDR_R + lane] = behind;
     to[HDR_Q + lane] = quarter;
     // (the weights times a power of two that puts the largest between 1/2 and 1: they enter operands)
-    const float weight = exp2f(behind + runs(lane / 16 + 1, 3)) * dt, most = wave_max(weight);
+    const float weight = exp2f(behind + runs(lane / 16 + 1, 3)) * dt, most = wave_max(fabsf(weight));
     const int e = min(max((int) (__builtin_bit_cast(uint32_t, most) >> 23 & 255), 1), 252);
     to[HDR_W + lane] = weight * __builtin_bit_cast(float, (uint32_t) (253 - e) << 23);
     if (lane < 16) to[HDR_BD + lane] = between;         // (run lane % 4, the later lane / 4)
