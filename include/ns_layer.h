@@ -76,7 +76,8 @@ int64_t ns_q4_bytes(int64_t M, int64_t K, int64_t group);
 int ns_q4_pack(ns_gpu* g, int form, const void* src, int64_t ss, int64_t M, int64_t K, int64_t group, void* w);
 /* y [T][M] = x [T][K] . w^T, 1 to 16 rows (a token, or a verify pass's rows), rows of type qt. The weights are exact in
  * the products; float32 rows enter as two halfs (22 bits), bfloat16 and half rows as they are. K up to 2^22. A row has the
- * same bits alone and among others. */
+ * same bits alone and among others. Rows that take more than 64 KiB as operands (16 half rows or 8 float32 rows of more
+ * than 1920 values) are laid out in the library's own scratch by a launch in front, in order with the handle's other calls. */
 int ns_q4_product(ns_gpu* g, int qt, const void* x, int64_t xs, const void* w, int64_t group, void* y, int64_t ys, int64_t T, int64_t M, int64_t K);
 
 #ifdef __cplusplus

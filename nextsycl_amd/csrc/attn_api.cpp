@@ -161,6 +161,7 @@ static int mm3_attend(ns_gpu* g, const char* who, const float* q, const uint16_t
     if (G <= 0 || H <= 0 || H % G) return ns_fail(w + ": heads");
     if (!(scale > 0.0f)) return ns_fail(w + ": a positive scale");
     if (pos0 < 0) return ns_fail(w + ": a position");
+    NS_OWN_SCRATCH(g);
     float* sc = g->own_scratch;
     int64_t sc_floats = (int64_t) ns_own_floats(g);
     if (sel) {

@@ -127,6 +127,7 @@ int ns_q35_attn_probs(ns_gpu* g, int kt, const float* q, const void* kc, int64_t
     const int64_t nb = std::max<int64_t>(1, std::min<int64_t>(64, n / 8192)), per = (n + nb - 1) / nb;
     if ((size_t) (Hq * n + 2 * Hq * nb) > ns_own_floats(g)) return ns_fail("ns_q35_attn_probs: more scores (heads x keys) than the library's scratch holds");
     NS_HIP(hipSetDevice(g->dev));
+    NS_OWN_SCRATCH(g);
     float* scores = g->own_scratch;
     float* part = scores + Hq * n;
     const float scale = 1.0f / sqrtf((float) D);

@@ -1375,6 +1375,7 @@ static int ds2_decode(ns_gpu* g, const char* who, const float* q, const uint16_t
     if (!q || !cache || !out || (kvb ? false : !kb || !vb)) return ns_fail(w + ": a null buffer");
     if (kvb && (uintptr_t) kvb % 2) return ns_fail(w + ": kv_b 2-byte aligned");
     NS_HIP(hipSetDevice(g->dev));
+    NS_OWN_SCRATCH(g);
     for (int64_t t0 = 0; t0 < T; t0 += 16) {
         const int64_t n = std::min<int64_t>(16, T - t0);
         // the library's own scratch (the reference's signature has none): the absorbed queries, u, then the partials
@@ -1466,6 +1467,7 @@ int ns_mla_attend_sel(ns_gpu* g, const float* qa, const uint16_t* c, float* u, i
     if (T <= 0) return 0;
     // (both of the reference's widths, kernels/llm/glm5next/glm.cpp:1254-1266, each an instance of the latent kernel)
     if (L != 256 && L != 512) return ns_fail("ns_mla_attend_sel: latent width 256 or 512");
+    NS_OWN_SCRATCH(g);
     return mla_sel_rows(g, "ns_mla_attend_sel", false, qa, c, u, T, H, pos0, scale, sel, sel_cnt, K, g->own_scratch, ns_own_floats(g), (int) L);
     NS_CATCH
 }
@@ -1475,6 +1477,7 @@ int ns_mla_attend_sel_q8(ns_gpu* g, const float* qa, const void* c, float* u, in
     NS_TRY
     if (T <= 0) return 0;
     if (L != 512) return ns_fail("ns_mla_attend_sel_q8: latent width 512");
+    NS_OWN_SCRATCH(g);
     return mla_sel_rows(g, "ns_mla_attend_sel_q8", true, qa, c, u, T, H, pos0, scale, sel, sel_cnt, K, g->own_scratch, ns_own_floats(g));
     NS_CATCH
 }
@@ -1491,6 +1494,7 @@ int ns_mla_attend(ns_gpu* g, const float* qa, const float* c, float* u, int64_t 
     if ((size_t) ch_floats + (size_t) (H > 0 ? 16 * H * PSTRIDE : 0) > ns_own_floats(g))
         return ns_fail("ns_mla_attend: more cells than the library's scratch holds as half rows (use a half cache and ns_mla_attend_sel)");
     NS_HIP(hipSetDevice(g->dev));
+    NS_OWN_SCRATCH(g);
     uint16_t* ch = (uint16_t*) g->own_scratch;
     to_half_kernel<<<(unsigned) ((cells * L / 8 + 255) / 256), 256, 0, g->q>>>(c, ch, cells * L / 8);
     NS_LAUNCHED("to_half");

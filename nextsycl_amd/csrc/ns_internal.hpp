@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <cstdint>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -21,6 +22,9 @@ struct ns_gpu {
     // scratch the library keeps for entry points whose reference signature has no scratch argument
     // (ns_llm_minimaxm3_attend); allocated once at ns_gpu_open, never inside a kernel call
     float* own_scratch = nullptr;
+    // held by a call from its first launch that writes the scratch to its last that reads it: another thread's launches on this
+    // handle come before them all or behind (recursive: such calls are made of one another)
+    std::recursive_mutex own_use;
     size_t own_scratch_floats = 0;          // OWN_SCRATCH_FLOATS
     // ns_attn_profile: events around the kernels of the last attention call (measurement only; off by default)
     bool profile = false;
@@ -57,6 +61,9 @@ int ns_hip_check(hipError_t e, const char* what);
     }                                                                 \
     catch (const std::exception& e) { return ns_fail(e.what()); }     \
     catch (...) { return ns_fail("unknown C++ exception"); }
+
+// the rest of the scope queues launches that hand each other data in g's own scratch
+#define NS_OWN_SCRATCH(g) const std::lock_guard<std::recursive_mutex> own_use_lock((g)->own_use)
 
 // after a kernel launch: launch errors (bad configuration) surface here, not at the next sync
 #define NS_LAUNCHED(name) NS_HIP(hipGetLastError())

@@ -249,6 +249,7 @@ int launch_product(ns_gpu* g, Q4Params& p) {
         return 0;
     }
     if ((size_t) (rows + 3) / 4 > ns_own_floats(g)) return ns_fail("ns_q4_product: more scratch than the library has");
+    NS_OWN_SCRATCH(g);
     p.ops = reinterpret_cast<uint8_t*>(g->own_scratch);
     q4_rows_kernel<QT><<<(unsigned) ((p.kt * p.T + 15) / 16), 256, 0, g->q>>>(p);
     q4_product_kernel<QT, GR, true, WAVES><<<grid, 64 * WAVES, sums, g->q>>>(p);
