@@ -2,7 +2,7 @@
 
 `Kernels` is the table of function pointers - the counterpart of an engine's `ffi.rs` (llm/qwen35/src/ffi.rs:42-52,
 70-136; llm/museglimmer/src/ffi.rs; llm/deepseek2/src/ffi.rs:36-39): every entry point looked up by name when the table
-is built, a missing symbol being a load error. `Ops` is the counterpart of `ops.rs` (llm/deepseek2/src/ops.rs:391-445):
+is built, a missing symbol being a load error (ns_layer.h's apart: those raise where they are called). `Ops` is the counterpart of `ops.rs` (llm/deepseek2/src/ops.rs:391-445):
 each wrapper checks that its buffers hold what the kernel will touch, then makes the C call and turns -1 into
 Error("<what>: <ns_last_error>"). The call order of a pass is the engines': kv_store -> *_scratch -> attention
 (llm/museglimmer/src/engine.rs:856-873). Nothing here computes: the HIP library does, or the call fails."""
@@ -150,13 +150,26 @@ LAYER_H = {
 }
 
 
+def _absent(why):
+    def call(*args):
+        raise Error(why)
+    return call
+
+
 class Kernels:
-    """Every attention entry point bound by name; a missing symbol fails the load."""
+    """Every attention entry point bound by name; a missing symbol fails the load. A hybrid model's other layers (LAYER_H) are not every engine's: a
+    library without them loads, and calling one raises Error."""
 
     def __init__(self, a=None):
         self.api = a or api()
-        for name, (res, args) in list(ATTN_H.items()) + list(MLA_H.items()) + list(PRE_H.items()) + list(LAYER_H.items()):
+        for name, (res, args) in list(ATTN_H.items()) + list(MLA_H.items()) + list(PRE_H.items()):
             setattr(self, name[3:], self.api.symbol(name, res, args))
+        for name, (res, args) in LAYER_H.items():
+            try:
+                entry = self.api.symbol(name, res, args)
+            except OSError as e:
+                entry = _absent(str(e))
+            setattr(self, name[3:], entry)
 
 
 _k = None
