@@ -49,7 +49,8 @@ int ns_ssm_step(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt, 
                 const int32_t* slots, int64_t nslots, int64_t R, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K, const float* h0,
                 float* h1, void* y, int64_t ys);
 
-/* ---- norms. rms(v) = v / sqrt(mean(v^2) + eps) */
+/* ---- norms. rms(v) = v / sqrt(mean(v^2) + eps). A call's groups (rows) are a launch's: fewer than 2^32 threads, 64 of them a
+ * group of up to 64 pieces of 16 bytes (rounded up to 4 groups), 64 for each 64 pieces, 1024 at most, a longer one. */
 
 /* The norm behind the scan, over each of `groups` equal parts of a row of D: order 0 out = rms(y silu(z)) w, order 1
  * out = rms(y) w silu(z); w [D] float32 or null (ones). Rows y, z, out of type qt; out may be y or z. */
@@ -72,10 +73,10 @@ int64_t ns_q4_bytes(int64_t M, int64_t K, int64_t group);
 /* Lays out M rows of K values: form 0 float32 rows ss values apart, each group rounded by the q4_0 rule (s = the value of
  * the largest magnitude, the first of a tie, / -8; q = min(15, (int) (v / s + 8.5))); form 1 q4_0 blocks as model files
  * hold them (18 bytes: a half scale, then 16 bytes that pair value j with j + 16; group 32, K a multiple of 32), rows ss
- * bytes apart. */
+ * bytes apart. Fewer than 2^32 groups (rows rounded up to 16, values to 128) a call. */
 int ns_q4_pack(ns_gpu* g, int form, const void* src, int64_t ss, int64_t M, int64_t K, int64_t group, void* w);
 /* y [T][M] = x [T][K] . w^T, 1 to 16 rows (a token, or a verify pass's rows), rows of type qt. The weights are exact in
- * the products; float32 rows enter as two halfs (22 bits), bfloat16 and half rows as they are. K up to 2^22. A row has the
+ * the products; float32 rows enter as two halfs (22 bits), bfloat16 and half rows as they are. M up to 2^27 - 16, K up to 2^22. A row has the
  * same bits alone and among others. Rows that take more than 64 KiB as operands (16 half rows or 8 float32 rows of more
  * than 1920 values) are laid out in the library's own scratch by a launch in front, in order with the handle's other calls. */
 int ns_q4_product(ns_gpu* g, int qt, const void* x, int64_t xs, const void* w, int64_t group, void* y, int64_t ys, int64_t T, int64_t M, int64_t K);

@@ -244,34 +244,36 @@ void by_size(int64_t n, int64_t units, F f) {
 template <int VEC>
 bool one_by_one(int64_t n) { return n % VEC && n <= 64; }
 template <int QT, int VEC, bool TAIL>
-int launch_gated(ns_gpu* g, const GatedParams& p) {
-    int rc = 0;
+void launch_gated(ns_gpu* g, const GatedParams& p) {
     by_size((p.W + VEC - 1) / VEC, p.units, [&](auto wide, auto it, int threads, int64_t blocks) {
-        if (blocks > INT32_MAX) rc = ns_fail("ns_norm_gated: too many rows");
-        else if constexpr (VEC > 1 || (!decltype(wide)::value && decltype(it)::value == 1))
+        if constexpr (VEC > 1 || (!decltype(wide)::value && decltype(it)::value == 1))
             norm_gated_kernel<QT, VEC, TAIL, decltype(wide)::value, decltype(it)::value><<<(unsigned) blocks, threads, 0, g->q>>>(p);
     });
-    return rc;
 }
 template <int QT>
-int launch_gated(ns_gpu* g, const GatedParams& p) {
+void launch_gated(ns_gpu* g, const GatedParams& p) {
     constexpr int VEC = QT ? 8 : 4;
     return one_by_one<VEC>(p.W) ? launch_gated<QT, 1, false>(g, p) : p.W % VEC ? launch_gated<QT, VEC, true>(g, p) : launch_gated<QT, VEC, false>(g, p);
 }
 template <int QT, int RT, int VEC, bool TAIL>
-int launch_residual(ns_gpu* g, const ResidualParams& p) {
-    int rc = 0;
+void launch_residual(ns_gpu* g, const ResidualParams& p) {
     by_size((p.D + VEC - 1) / VEC, p.T, [&](auto wide, auto it, int threads, int64_t blocks) {
-        if (blocks > INT32_MAX) rc = ns_fail("ns_norm_residual: too many rows");
-        else if constexpr (VEC > 1 || (!decltype(wide)::value && decltype(it)::value == 1))
+        if constexpr (VEC > 1 || (!decltype(wide)::value && decltype(it)::value == 1))
             norm_residual_kernel<QT, RT, VEC, TAIL, decltype(wide)::value, decltype(it)::value><<<(unsigned) blocks, threads, 0, g->q>>>(p);
     });
-    return rc;
 }
 template <int QT, int RT>
-int launch_residual(ns_gpu* g, const ResidualParams& p) {
+void launch_residual(ns_gpu* g, const ResidualParams& p) {
     constexpr int VEC = QT ? 8 : 4;
     return one_by_one<VEC>(p.D) ? launch_residual<QT, RT, 1, false>(g, p) : p.D % VEC ? launch_residual<QT, RT, VEC, true>(g, p) : launch_residual<QT, RT, VEC, false>(g, p);
+}
+
+// whether `units` units of n values run in one launch
+bool one_launch(int qt, int64_t n, int64_t units) {
+    const int64_t vec = qt ? 8 : 4;
+    bool fits = units <= (int64_t) 1 << 40;
+    if (fits) by_size((qt ? one_by_one<8>(n) : one_by_one<4>(n)) ? n : (n + vec - 1) / vec, units, [&](auto, auto, int threads, int64_t blocks) { fits = ns_grid_fits(blocks, threads); });
+    return fits;
 }
 
 }  // namespace
@@ -286,12 +288,13 @@ int ns_norm_gated(ns_gpu* g, int qt, const void* y, int64_t ys, const void* z, i
     if (groups <= 0 || D % groups || D > (int64_t) 1 << 24) return ns_fail("ns_norm_gated: up to 2^24 values in equal groups");
     if (order != 0 && order != 1) return ns_fail("ns_norm_gated: order 0 (gate, then norm) or 1 (norm, then gate)");
     if (ys < D || zs < D || os < D) return ns_fail("ns_norm_gated: rows at least as far apart as they are long");
+    if (T > ((int64_t) 1 << 40) / groups || !one_launch(qt, D / groups, T * groups)) return ns_fail("ns_norm_gated: too many rows");
     if (!g || !y || !z || !out) return ns_fail("ns_norm_gated: a null buffer");
-    if (T > ((int64_t) 1 << 40) / groups) return ns_fail("ns_norm_gated: too many rows");
     NS_HIP(hipSetDevice(g->dev));
     const GatedParams p{y, z, w, out, ys, zs, os, T * groups, (int) (D / groups), (int) groups, order, eps};
-    const int rc = qt == 0 ? launch_gated<0>(g, p) : qt == 1 ? launch_gated<1>(g, p) : launch_gated<2>(g, p);
-    if (rc) return rc;
+    if (qt == 0) launch_gated<0>(g, p);
+    else if (qt == 1) launch_gated<1>(g, p);
+    else launch_gated<2>(g, p);
     NS_LAUNCHED("norm_gated");
     return 0;
     NS_CATCH
@@ -305,15 +308,14 @@ int ns_norm_residual(ns_gpu* g, int qt, int rt, const void* x, int64_t xs, const
     if (rt != 0 && rt != qt) return ns_fail("ns_norm_residual: a stream of float32 or of the rows' type");
     if (D > (int64_t) 1 << 24) return ns_fail("ns_norm_residual: up to 2^24 values");
     if ((x && xs < D) || hs < D || (h1 && h1s < D) || (out && os < D)) return ns_fail("ns_norm_residual: rows at least as far apart as they are long");
+    if (!one_launch(qt, D, T)) return ns_fail("ns_norm_residual: too many rows");
     if (!g || !h || (!h1 && !out)) return ns_fail("ns_norm_residual: a null buffer");
     if (!x && (post || gate)) return ns_fail("ns_norm_residual: a norm or gate of no block");
     NS_HIP(hipSetDevice(g->dev));
     const ResidualParams p{x, h, post, gate, pre, h1, out, xs, hs, h1s, os, T, (int) D, eps, scale};
-    const int rc = qt == 0   ? launch_residual<0, 0>(g, p)
-                   : rt == 0 ? (qt == 1 ? launch_residual<1, 0>(g, p) : launch_residual<2, 0>(g, p))
-                   : qt == 1 ? launch_residual<1, 1>(g, p)
-                             : launch_residual<2, 2>(g, p);
-    if (rc) return rc;
+    if (qt == 0) launch_residual<0, 0>(g, p);
+    else if (qt == 1) rt == 0 ? launch_residual<1, 0>(g, p) : launch_residual<1, 1>(g, p);
+    else rt == 0 ? launch_residual<2, 0>(g, p) : launch_residual<2, 2>(g, p);
     NS_LAUNCHED("norm_residual");
     return 0;
     NS_CATCH

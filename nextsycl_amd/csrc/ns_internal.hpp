@@ -62,6 +62,9 @@ int ns_hip_check(hipError_t e, const char* what);
     catch (const std::exception& e) { return ns_fail(e.what()); }     \
     catch (...) { return ns_fail("unknown C++ exception"); }
 
+// whether one launch takes so many work-groups in a row: fewer than 2^32 threads
+inline bool ns_grid_fits(int64_t blocks, int64_t threads) { return blocks <= UINT32_MAX / threads; }
+
 // the rest of the scope queues launches that hand each other data in g's own scratch
 #define NS_OWN_SCRATCH(g) const std::lock_guard<std::recursive_mutex> own_use_lock((g)->own_use)
 

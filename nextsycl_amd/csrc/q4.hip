@@ -30,6 +30,7 @@ namespace {
 constexpr int PF = 1, LDS_ROWS = 64 * 1024;
 
 constexpr int WIDE_M = 4096;
+constexpr int64_t MOST_M = ((int64_t) 1 << 27) - 16;        // (8 waves for 16 of them: what one launch takes)
 constexpr int64_t q4_tile_bytes(int64_t group) { return 1024 + 16 * (128 / group) * 2; }
 
 struct Q4Params {
@@ -285,9 +286,9 @@ int ns_q4_pack(ns_gpu* g, int form, const void* src, int64_t ss, int64_t M, int6
     if (M > (int64_t) 1 << 30 || K > (int64_t) 1 << 30) return ns_fail("ns_q4_pack: up to 2^30 rows and values a row");
     if (ss < (form ? K / 32 * 18 : K)) return ns_fail("ns_q4_pack: rows at least as far apart as they are long");
     if ((uintptr_t) w % 16) return ns_fail("ns_q4_pack: weights 16-byte aligned");
-    if (!g || !src || !w) return ns_fail("ns_q4_pack: a null buffer");
     const int64_t kt = (K + 127) / 128, threads = (M + 15) / 16 * 16 * kt * (128 / group);
-    if ((threads + 255) / 256 > INT32_MAX) return ns_fail("ns_q4_pack: too many weights");
+    if (!ns_grid_fits((threads + 255) / 256, 256)) return ns_fail("ns_q4_pack: too many weights");
+    if (!g || !src || !w) return ns_fail("ns_q4_pack: a null buffer");
     NS_HIP(hipSetDevice(g->dev));
     q4_pack_kernel<<<(unsigned) ((threads + 255) / 256), 256, 0, g->q>>>(form, src, ss, M, K, (int) group, kt, static_cast<uint8_t*>(w));
     NS_LAUNCHED("q4_pack");
@@ -301,7 +302,7 @@ int ns_q4_product(ns_gpu* g, int qt, const void* x, int64_t xs, const void* w, i
     if (qt < 0 || qt > 2) return ns_fail("ns_q4_product: rows of type 0 (float32), 1 (half) or 2 (bfloat16)");
     if (T > 16) return ns_fail("ns_q4_product: 1 to 16 rows");
     if (!q4_group(group)) return ns_fail("ns_q4_product: groups of 32, 64 or 128");
-    if (K <= 0 || M > (int64_t) 1 << 30 || K > (int64_t) 1 << 22) return ns_fail("ns_q4_product: up to 2^30 outputs, 1 to 2^22 inputs");
+    if (K <= 0 || M > MOST_M || K > (int64_t) 1 << 22) return ns_fail("ns_q4_product: up to 2^27 - 16 outputs, 1 to 2^22 inputs");
     if (xs < K || ys < M) return ns_fail("ns_q4_product: rows at least as far apart as they are long");
     if ((uintptr_t) w % 16) return ns_fail("ns_q4_product: weights 16-byte aligned");
     if (!g || !x || !w || !y) return ns_fail("ns_q4_product: a null buffer");
