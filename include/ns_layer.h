@@ -29,7 +29,7 @@ extern "C" {
 
 /* T rows of one sequence at positions p0 .. p0 + T - 1: y [T] rows of H P, h1, and the last min(T, K - 1) raw rows into
  * the ring (cap >= K - 1). Rows up to 2^23 values apart (xs). scratch: ns_ssm_prompt_scratch(..) floats, 16-byte aligned:
- * it grows with T up to 8192 rows. Up to 16 rows, where the ring holds K - 1 + T, run as ns_ssm_step's do; else the scan's matrix products keep 22 bits of each operand (half rows too; of bfloat16 rows
+ * it grows with T up to 8192 rows (0: sizes that the call does not take). Up to 16 rows, where the ring holds K - 1 + T, run as ns_ssm_step's do; else the scan's matrix products keep 22 bits of each operand (half rows too; of bfloat16 rows
  * those that reach y alone 11) and nothing below 2^-38 of the largest value of a column or block of 64 rows. A value that is
  * not finite reaches what the recurrence takes it to, rows in front of it never. */
 int64_t ns_ssm_prompt_scratch(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K);

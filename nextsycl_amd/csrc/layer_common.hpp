@@ -109,6 +109,10 @@ __device__ __forceinline__ float ssm_dt(const SsmLayer& p, float v) {
 // tap k of 4 of a channel: the layer's K taps are the last K of them
 __device__ __forceinline__ float ssm_tap(const SsmLayer& p, int ch, int k) { return k >= 4 - p.K ? p.cw[(int64_t) ch * p.K + k - 4 + p.K] : 0.0f; }
 
+// the sizes that the state-space calls take
+inline bool ns_ssm_sizes(int64_t H, int64_t P, int64_t N, int64_t G) {
+    return H > 0 && P > 0 && N > 0 && G > 0 && H <= 65536 && P <= 65536 && N <= 256 && H % G == 0 && H * P + 2 * G * N <= (int64_t) 1 << 24;
+}
 // ssm_step.hip: a few successive rows of one sequence from p.p0 on, the last K - 1 of them into the ring (which holds those in front of the
 // call and those behind it at once)
 void ns_ssm_few(ns_gpu* g, int qt, const SsmLayer& p, int rows);

@@ -882,7 +882,7 @@ void run_prompt(ns_gpu* g, const SsmLayer& p, int64_t T, float* scratch) {
 extern "C" {
 
 int64_t ns_ssm_prompt_scratch(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K) {
-    if (T <= 0 || H <= 0 || P <= 0 || N <= 0 || G <= 0 || K <= 0) return 0;
+    if (T <= 0 || !ns_ssm_sizes(H, P, N, G) || K < 1 || K > 4) return 0;
     // (whatever the rows' type; and a last pass of fewer rows may be cut in more segments than a full one)
     int64_t most = 0;
     for (int wgs = 1; wgs <= 3; ++wgs) {

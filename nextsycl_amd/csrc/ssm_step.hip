@@ -267,7 +267,7 @@ int ns_ssm_check(const char* who, ns_gpu* g, int qt, const SsmLayer& p, int64_t 
                  int64_t least) {
     const std::string s(who);
     if (qt < 0 || qt > 2) return ns_fail(s + ": rows of type 0 (float32), 1 (half) or 2 (bfloat16)");
-    if (H <= 0 || P <= 0 || N <= 0 || G <= 0 || H % G || N > 256 || H > 65536 || P > 65536 || H * P + 2 * G * N > (int64_t) 1 << 24)
+    if (!ns_ssm_sizes(H, P, N, G))
         return ns_fail(s + ": heads a multiple of the groups, a state of 1 to 256 features, up to 2^24 channels");
     if (K < 1 || K > 4) return ns_fail(s + ": 1 to 4 taps");
     if (p.xs < H * P + 2 * G * N || p.dts < H || p.ys < H * P) return ns_fail(s + ": rows at least as far apart as they are long");
