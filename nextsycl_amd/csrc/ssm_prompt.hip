@@ -7,7 +7,7 @@
 // three matrix products a chunk and head, and one (C . B) a chunk and group. They run on the matrix unit: an operand is two
 // halfs (22 bits), scaled by a power of two that puts the largest value of its column, row or block at 2^13, and three
 // instructions a product drop nothing above 2^-22; sums, states and scales are float32. (bfloat16 rows: the products that
-// reach y alone take their operands' first halfs, 2^-11 beside the rows' own rounding of 2^-8.)
+// reach y alone take their operands' first halfs, 2^-11 beside the rows' own rounding of 2^-8; Y3 below.)
 //
 // ssm_prep_kernel, 8 waves a (chunk, group): convolves B and C (a thread half a channel's rows), leaves them in LDS as [feature]
 // [row] - an operand's rows are a thread's own, C's come back through transposing reads - and multiplies them; the work-groups
@@ -277,8 +277,11 @@ __global__ __launch_bounds__(512, KT == 4 ? 1 : 2) void ssm_prep_kernel(ScanPara
         return s8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     };
     const int w = wave % 4, h = wave / 4;
+    // (of bfloat16 rows the scan takes C's first halfs alone)
+    if (QT != 2 || h == 0) {
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) reinterpret_cast<s8v*>(ops + h * op_c(KK))[(w * KK + kk) * 64 + lane] = operand(plane[1][h], w, kk);
+        for (int kk = 0; kk < KK; ++kk) reinterpret_cast<s8v*>(ops + h * op_c(KK))[(w * KK + kk) * 64 + lane] = operand(plane[1][h], w, kk);
+    }
     // C . B of 16 rows of C against the rows of B that they see: column a row of C, 4 consecutive rows of B a lane
     const float down = downs[0] * downs[1];
     for (int st = h; st <= w; st += 2) {
@@ -301,7 +304,10 @@ template <int QT, int KT, int CT, bool STATE>
 __global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kernel(ScanParams s) {
     constexpr int KK = 2 * KT;
     constexpr bool AHEAD = STATE || SCAN_WGS<QT, KT, STATE> <= 2;     // x and the operands asked for early, where there are registers for them
-    constexpr bool Y3 = QT != 2;                                  // y's products from both halfs of their operands
+    // y's products from both halfs of their operands - the state, C, x, C . B with its decays -, but for bfloat16 rows: what first halfs lose, 2^-11
+    // each, is an eighth of y's own rounding (8192 rows' error against 64 bits is 1.7e-3 of y either way), and one plane of the state and of x
+    // leaves LDS and registers for three work-groups a CU (298 us; 365 with both halfs, two work-groups)
+    constexpr bool Y3 = QT != 2;
     // x weighted for the state (hi, lo) and as it is (hi, for Y3 lo): [32 rows][16 columns][lane]; the state: [32 features][..]
     constexpr int WH = 0, WL = 1, XH = 2, XL = 3, PLANES = STATE ? 2 : Y3 ? 4 : 3, HP = STATE ? 0 : Y3 ? 2 : 1;
     __shared__ __align__(16) s8v xop[PLANES][2][CT][64];
