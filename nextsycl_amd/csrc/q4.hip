@@ -27,7 +27,7 @@
 
 namespace {
 
-constexpr int PF = 1, LDS_ROWS = 64 * 1024;
+constexpr int LDS_ROWS = 64 * 1024;
 
 constexpr int WIDE_M = 4096;
 constexpr int64_t MOST_M = ((int64_t) 1 << 27) - 16;        // (8 waves for 16 of them: what one launch takes)
@@ -57,7 +57,6 @@ __device__ __forceinline__ s8v q4_operand(uint32_t w) {
 // The rows as operands: [plane][tile][16 pieces of 8][row], then a power of two a (tile, row)
 template <int QT>
 constexpr int PLANES = QT == 0 ? 2 : 1;
-template <int QT>
 __device__ __forceinline__ int64_t q4_plane(const Q4Params& p) { return (int64_t) p.kt * 16 * p.T; }
 // 16 threads (u) a (tile kl, row t): 8 values each
 template <int QT>
@@ -90,14 +89,14 @@ __device__ __forceinline__ void q4_rows(const Q4Params& p, int kl, int t, int u,
     }
     const int64_t at = (int64_t) (kl * 16 + u) * p.T + t;
     xo[at] = hi;
-    if constexpr (PLANES<QT> == 2) xo[q4_plane<QT>(p) + at] = lo;
+    if constexpr (PLANES<QT> == 2) xo[q4_plane(p) + at] = lo;
 }
 template <int QT>
 __global__ __launch_bounds__(256) void q4_rows_kernel(Q4Params p) {
     const int task = blockIdx.x * 16 + threadIdx.x / 16;
     if (task >= p.kt * p.T) return;
     s8v* xo = reinterpret_cast<s8v*>(p.ops);
-    q4_rows<QT>(p, task / p.T, task % p.T, threadIdx.x % 16, xo, reinterpret_cast<float*>(xo + q4_plane<QT>(p) * PLANES<QT>));
+    q4_rows<QT>(p, task / p.T, task % p.T, threadIdx.x % 16, xo, reinterpret_cast<float*>(xo + q4_plane(p) * PLANES<QT>));
 }
 
 // GR: groups a tile (4, 2, 1); MEM: the rows' operands lie in memory, else in LDS; WAVES: 8, or 16
@@ -107,7 +106,7 @@ __global__ __launch_bounds__(64 * WAVES, MEM && WAVES == 8 ? 2 : 4) void q4_prod
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, g = lane / 16;
     const int col = n < p.T ? n : p.T - 1;             // (columns behind the rows: some row's, never written)
-    const int64_t plane = q4_plane<QT>(p);
+    const int64_t plane = q4_plane(p);
     s8v* const xo = reinterpret_cast<s8v*>(MEM ? p.ops : lds);
     float* const xscale = reinterpret_cast<float*>(xo + plane * PLANES<QT>);
     const uint8_t* wt = p.w + (int64_t) blockIdx.x * p.kt * TILE;
@@ -117,73 +116,67 @@ __global__ __launch_bounds__(64 * WAVES, MEM && WAVES == 8 ? 2 : 4) void q4_prod
     constexpr bool XAHEAD = MEM && !(WAVES == 16 && PLANES<QT> == 2 && GR > 1);
     constexpr int XS = XAHEAD ? 4 : 1, XP = XAHEAD ? PLANES<QT> : 1;
     struct Ahead {
-        uint4 nib[PF];
-        uint32_t sc[PF][SW];
-        s8v x[PF][XS][XP];
-        float down[PF];
+        uint4 nib;
+        uint32_t sc[SW];
+        s8v x[XS][XP];
+        float down;
     } ahead[2];
-    auto fetch = [&](int i0, Ahead& f) {
+    auto fetch = [&](int i, Ahead& f) {
+        const int kl = wave + WAVES * i;
+        const uint8_t* tile = wt + (int64_t) kl * TILE;
+        f.nib = *reinterpret_cast<const uint4*>(tile + lane * 16);
+        const uint32_t* ss = reinterpret_cast<const uint32_t*>(tile + 1024 + g * 8 * GR);
 #pragma unroll
-        for (int i = 0; i < PF; ++i) {
-            const int kl = min(wave + WAVES * (i0 + i), p.kt - 1);
-            const uint8_t* tile = wt + (int64_t) kl * TILE;
-            f.nib[i] = *reinterpret_cast<const uint4*>(tile + lane * 16);
-            const uint32_t* ss = reinterpret_cast<const uint32_t*>(tile + 1024 + g * 8 * GR);
-#pragma unroll
-            for (int j = 0; j < SW; ++j) f.sc[i][j] = ss[j];
-            if constexpr (XAHEAD) {
-                const s8v* x = xo + ((int64_t) kl * 16 + g) * p.T + col;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int h = 0; h < XP; ++h) f.x[i][j][h] = x[h * plane + 4 * j * p.T];
-                if (QT != 1) f.down[i] = xscale[kl * p.T + col];
-            }
-        }
-    };
-    auto compute = [&](int i0, const Ahead& f) {
-#pragma unroll
-        for (int i = 0; i < PF; ++i) {
-            const int kl = wave + WAVES * (i0 + i);
-            if (kl >= p.kt) break;
-            f4v tile = {0.0f, 0.0f, 0.0f, 0.0f}, s = tile;
-            const uint32_t words[4] = {f.nib[i].x, f.nib[i].y, f.nib[i].z, f.nib[i].w};
+        for (int j = 0; j < SW; ++j) f.sc[j] = ss[j];
+        if constexpr (XAHEAD) {
             const s8v* x = xo + ((int64_t) kl * 16 + g) * p.T + col;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const s8v a = q4_operand(words[j]);
-                if constexpr (XAHEAD) {
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int h = 0; h < XP; ++h) s = mfma16<false>(a, f.x[i][j][h], s);
-                } else {
-                    s = mfma16<false>(a, x[4 * j * p.T], s);
-                    if constexpr (PLANES<QT> == 2) s = mfma16<false>(a, x[plane + 4 * j * p.T], s);
-                }
-                if ((j + 1) % (4 / GR) == 0) {
-                    const int grp = j / (4 / GR);
-                    const uint32_t s0 = f.sc[i][grp * 2], s1 = f.sc[i][grp * 2 + 1];
-                    tile[0] = fmaf(f16_to_f32((uint16_t) s0), s[0], tile[0]);
-                    tile[1] = fmaf(f16_to_f32((uint16_t) (s0 >> 16)), s[1], tile[1]);
-                    tile[2] = fmaf(f16_to_f32((uint16_t) s1), s[2], tile[2]);
-                    tile[3] = fmaf(f16_to_f32((uint16_t) (s1 >> 16)), s[3], tile[3]);
-                    s = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-                }
-            }
-            const float down = QT == 1 ? 1.0f : XAHEAD ? f.down[i] : xscale[kl * p.T + col];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = QT == 1 ? acc[e] + tile[e] : fmaf(down, tile[e], acc[e]);
+                for (int h = 0; h < XP; ++h) f.x[j][h] = x[h * plane + 4 * j * p.T];
+            if (QT != 1) f.down = xscale[kl * p.T + col];
         }
     };
-    fetch(0, ahead[0]);
+    auto compute = [&](int i, const Ahead& f) {
+        const int kl = wave + WAVES * i;
+        f4v tile = {0.0f, 0.0f, 0.0f, 0.0f}, s = tile;
+        const uint32_t words[4] = {f.nib.x, f.nib.y, f.nib.z, f.nib.w};
+        const s8v* x = xo + ((int64_t) kl * 16 + g) * p.T + col;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const s8v a = q4_operand(words[j]);
+            if constexpr (XAHEAD) {
+#pragma unroll
+                for (int h = 0; h < XP; ++h) s = mfma16<false>(a, f.x[j][h], s);
+            } else {
+                s = mfma16<false>(a, x[4 * j * p.T], s);
+                if constexpr (PLANES<QT> == 2) s = mfma16<false>(a, x[plane + 4 * j * p.T], s);
+            }
+            if ((j + 1) % (4 / GR) == 0) {
+                const int grp = j / (4 / GR);
+                const uint32_t s0 = f.sc[grp * 2], s1 = f.sc[grp * 2 + 1];
+                tile[0] = fmaf(f16_to_f32((uint16_t) s0), s[0], tile[0]);
+                tile[1] = fmaf(f16_to_f32((uint16_t) (s0 >> 16)), s[1], tile[1]);
+                tile[2] = fmaf(f16_to_f32((uint16_t) s1), s[2], tile[2]);
+                tile[3] = fmaf(f16_to_f32((uint16_t) (s1 >> 16)), s[3], tile[3]);
+                s = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+        const float down = QT == 1 ? 1.0f : XAHEAD ? f.down : xscale[kl * p.T + col];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = QT == 1 ? acc[e] + tile[e] : fmaf(down, tile[e], acc[e]);
+    };
+    if (wave < p.kt) fetch(0, ahead[0]);
     if constexpr (!MEM) {
         for (int task = tid / 16; task < p.kt * p.T; task += 64 * WAVES / 16) q4_rows<QT>(p, task / p.T, task % p.T, tid % 16, xo, xscale);
         lds_barrier();                   // (the weights stay in flight)
     }
-    for (int i0 = 0; wave + WAVES * i0 < p.kt; i0 += 2 * PF) {
-        if (wave + WAVES * (i0 + PF) < p.kt) fetch(i0 + PF, ahead[1]);
-        compute(i0, ahead[0]);
-        if (wave + WAVES * (i0 + 2 * PF) < p.kt) fetch(i0 + 2 * PF, ahead[0]);
-        compute(i0 + PF, ahead[1]);
+    for (int i = 0; wave + WAVES * i < p.kt; i += 2) {
+        if (wave + WAVES * (i + 1) < p.kt) fetch(i + 1, ahead[1]);
+        compute(i, ahead[0]);
+        if (wave + WAVES * (i + 1) >= p.kt) break;
+        if (wave + WAVES * (i + 2) < p.kt) fetch(i + 2, ahead[0]);
+        compute(i + 1, ahead[1]);
     }
     // the waves' sums, in the waves' order
     __syncthreads();
@@ -258,7 +251,9 @@ int launch_product(ns_gpu* g, Q4Params& p) {
 }
 // 16 waves where each work-group has a CU of its own (up to 256 of them: 4096 outputs), else 8: a row x 4096 outputs of 8192 half inputs
 // 6.81 us with 8 waves, 5.96 with 16; 8 float32 rows of them 11.0 and 10.2 - 10.7; 2 half rows x 8192 of 5120 7.85 and 9.10, a row
-// x 18560 of 4096 11.1 and 16.5. Whatever the rows' number, so that a row has the same bits alone and among others
+// x 18560 of 4096 11.1 and 16.5. On both sides of the line, inputs of 2048 and 8192: a half row x 4096 in groups of 32 3.9 and 7.2 us with 8, 3.5 and
+// 6.4 with 16, x 4112 3.6 and 8.7, 4.6 and 10.1, x 6144 3.9 and 9.5, 5.0 and 10.8; 8 float32 rows x 4112 in groups of 128 6.9 and 14.6, 7.8 and
+// 15.8. Whatever the rows' number, so that a row has the same bits alone and among others
 template <int QT, int GR>
 int launch_product(ns_gpu* g, Q4Params& p) {
     return p.M <= WIDE_M ? launch_product<QT, GR, 16>(g, p) : launch_product<QT, GR, 8>(g, p);

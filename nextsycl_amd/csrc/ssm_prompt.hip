@@ -43,8 +43,9 @@ namespace {
 constexpr int L = 64;                     // rows a chunk
 constexpr int64_t PASS_ROWS = 8192;       // rows a pass works on: what bounds the scratch
 constexpr int MOST_SEGS = 32;
-// up to these row by row, as steps (128 heads of 64 x 128: 1 row 6.4 us and 17.5 as a chunk, 8 9.2 and 18.2, 16 14.5 and 18.2, 24 19.6
-// and 18.4; of 80 x 128 16 17.5 and 18.2)
+// up to these row by row, as steps: bfloat16 rows of 128 heads of 64 x 128 4 7.6 us and 17.3 as a chunk, 16 16.7 and 17.3, 20 19.9 and 17.4; of 24
+// heads of them 16 16.1 and 16.4, 20 19.3 and 16.5; of 80 heads of 64 x 64 16 12.8 and 15.1, 20 15.3 and 15.1; of 64 heads of 32 x 256 16
+// 20.2 and 24.7, 24 28.2 and 25.1; only of few and small heads are more (7 of 64 x 16: 24 14.4 and 16.9)
 constexpr int64_t FEW_ROWS = 16;
 // a chunk and head's header, exponents base 2. Rows' exponents from their run of 16's start, step sizes, weights in the chunk's state, decays from the
 // chunk's start; exponents between a run's end and a later one's start [later][run], the whole chunk's exponent and decay, what the weights
@@ -734,7 +735,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kerne
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) ahead[ct % 2][ks][0] = xop[WH][ks][ct][lane], ahead[ct % 2][ks][1] = xop[WL][ks][ct][lane];
             };
-            // (a column tile ahead, but where four work-groups a CU hide the reads)
+            // (a column tile ahead, but in the states' kernel: its three work-groups a CU hide the reads)
             if constexpr (!STATE) operands(0);
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
