@@ -29,8 +29,12 @@ extern "C" {
 
 /* T rows of one sequence at positions p0 .. p0 + T - 1: y [T] rows of H P, h1, and the last min(T, K - 1) raw rows into
  * the ring (cap >= K - 1). Rows up to 2^23 values apart (xs). scratch: ns_ssm_prompt_scratch(..) floats, 16-byte aligned:
- * it grows with T up to 8192 rows (0: sizes that the call does not take). Up to 16 rows, where the ring holds K - 1 + T, run as ns_ssm_step's do; else the scan's matrix products keep 22 bits of each operand (half rows too; of bfloat16 rows
- * those that reach y alone 11) and nothing below 2^-38 of the largest value of a column or block of 64 rows. A value that is
+ * it grows with T up to 8192 rows (0: sizes that the call does not take). Up to 16 rows, where the ring holds K - 1 + T, run as
+ * ns_ssm_step's do; else in blocks of 64 rows whose matrix products keep 22 bits of each operand (half rows too; of bfloat16
+ * rows those that reach y alone 11) and nothing below 2^-38 of the largest value of a column of x or of the state, of a block's B
+ * or C, or of a row's products of B and C with steps and decays; x enters the state times its row's step, the largest step with the
+ * column's largest x. Exponents of decays are sums of the steps between two rows alone: a large step takes no bits of others'. Finite
+ * values of a block whose largest ones' products pass float32's range may leave rows that do not hold them not finite. A value that is
  * not finite reaches what the recurrence takes it to, rows in front of it never. */
 int64_t ns_ssm_prompt_scratch(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K);
 int ns_ssm_prompt(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt, int64_t dts, const float* cw, const float* cb, const float* a,
@@ -42,8 +46,8 @@ int ns_ssm_prompt(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt
  * as it was. The rows of one slot are successive tokens of its sequence, in the rows' order; its first is at position
  * pos[r] (pos null: p0). Every row goes into its slot's ring, so a sequence can be taken back to any row of the call whose
  * state the caller kept (h0 and h1 apart). A slot takes up to cap - K + 1 rows a call (cap >= K): the ring holds the rows
- * in front of them at the same time; rows of a slot beyond that are passed over too. Slots that have no row: nothing of
- * theirs is written. A row's results have the same bits in a call of its own and among others. */
+ * in front of them at the same time; rows of a slot beyond that are passed over too, and all of a slot whose first is at a
+ * negative position. Slots that have no row: nothing of theirs is written. A row's results have the same bits in a call of its own and among others. */
 int ns_ssm_step(ns_gpu* g, int qt, const void* xbc, int64_t xs, const void* dt, int64_t dts, const float* cw, const float* cb, const float* a,
                 const float* dtb, const float* d, float dt_lo, float dt_hi, float* conv, int64_t cap, int64_t p0, const int32_t* pos,
                 const int32_t* slots, int64_t nslots, int64_t R, int64_t H, int64_t P, int64_t N, int64_t G, int64_t K, const float* h0,
@@ -76,7 +80,8 @@ int64_t ns_q4_bytes(int64_t M, int64_t K, int64_t group);
  * bytes apart. Fewer than 2^32 groups (rows rounded up to 16, values to 128) a call. */
 int ns_q4_pack(ns_gpu* g, int form, const void* src, int64_t ss, int64_t M, int64_t K, int64_t group, void* w);
 /* y [T][M] = x [T][K] . w^T, 1 to 16 rows (a token, or a verify pass's rows), rows of type qt. The weights are exact in
- * the products; float32 rows enter as two halfs (22 bits), bfloat16 and half rows as they are. M up to 2^27 - 16, K up to 2^22. A row has the
+ * the products; float32 rows enter as two halfs (22 bits), half rows as they are, bfloat16 rows too but for
+ * what lies below 2^-29 of the largest of a row's 128 values. M up to 2^27 - 16, K up to 2^22. A row has the
  * same bits alone and among others. Rows that take more than 64 KiB as operands (16 half rows or 8 float32 rows of more
  * than 1920 values) are laid out in the library's own scratch by a launch in front, in order with the handle's other calls. */
 int ns_q4_product(ns_gpu* g, int qt, const void* x, int64_t xs, const void* w, int64_t group, void* y, int64_t ys, int64_t T, int64_t M, int64_t K);

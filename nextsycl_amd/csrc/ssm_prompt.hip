@@ -173,8 +173,8 @@ __device__ __forceinline__ void ssm_header(const ScanParams& s, int chunk, int h
     if (lane < 3) to[HDR_END + lane] = lane == 0 ? end : lane == 1 ? exp2f(end) : __builtin_bit_cast(float, (uint32_t) (e + 1) << 23);
 }
 
-// KT: tiles of 16 features that each of 4 waves of the scan holds: 1 up to 64 features, 2 up to 128, 4 up to 256 (4096 bfloat16 rows of 80 heads of
-// 64 x 64 110.8 us with 1, 140.6 with 2)
+// KT: tiles of 16 features that each of 4 waves of the scan holds: 1 up to 64 features, 2 up to 128, 4 up to 256 (bfloat16 rows of 80 heads of
+// 64 x 64: 4096 112 us with 1, 144 with 2, 588 33.8 and 40.0)
 template <int QT, int KT>
 __global__ __launch_bounds__(512, KT == 4 ? 1 : 2) void ssm_prep_kernel(ScanParams s) {
     constexpr int KW = KT == 4 ? 2 : 1, NP = 128 * KW, KK = 2 * KT, ROW = L + 4;     // (34 words: a column of LDS banks on for each feature)
@@ -817,15 +817,15 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
     q.chunks = (int) ((T + L - 1) / L);
     q.blocks = (int) ((P + 63) / 64);
     const int64_t owners = H * q.blocks;
-    // as many segments as fill the chip's places for the scan's work-groups, of 2 chunks at least. (Rows of 32 heads of 64 x 128: 512
-    // 46.7 us in segments of 4 chunks, 33.1 in those of 2, and 256 rows, left whole, 30.0 - in two segments 32.4; 8192 rows of
-    // 8 heads of 64 x 64 99.9 us with up to 8 segments, 56.4 with up to 32, 69.8 with 64: a segment's start walks the states in
+    // as many segments as fill the chip's places for the scan's work-groups, of 2 chunks at least. (bfloat16 rows of 32 heads of 64 x 128:
+    // 512 44.6 us in segments of 4 chunks, 32.5 in those of 2, and 256 rows, left whole, 29.8 - in two segments 30.4; 8192 rows of
+    // 8 heads of 64 x 64 91.2 us with up to 8 segments, 49.9 with up to 32, 52.3 with 64: a segment's start walks the states in
     // front of it)
     const int64_t segs = std::max<int64_t>(1, std::min<int64_t>({MOST_SEGS, 256 * wgs / owners, q.chunks < 6 ? 1 : q.chunks / 2}));
     q.per = (int) ((q.chunks + segs - 1) / segs);
     q.segs = (q.chunks + q.per - 1) / q.per;
-    // their states in as many pieces as fill those of the state kernel's, of 4 chunks at least (2: 2051 rows of 64 heads 75.8 us for
-    // 73.3)
+    // their states in as many pieces as fill those of the state kernel's, of 4 chunks at least (2: 2051 float32 rows of 64 heads of
+    // 64 x 128 76.1 us for 73.6)
     q.sub = q.segs == 1 ? 1 : (int) std::max<int64_t>(1, std::min<int64_t>(q.per / 4, (768 + owners * (q.segs - 1) - 1) / (owners * (q.segs - 1))));
     q.piece = (q.per + q.sub - 1) / q.sub;
     int64_t at = 0;
@@ -845,8 +845,8 @@ Plan plan_of(int64_t T, int64_t H, int64_t P, int64_t N, int64_t G, int wgs) {
     return q;
 }
 
-// column tiles of 16 a work-group: what a head's fewest work-groups of up to 4 share out evenly (128 heads of 80: 796 bfloat16 rows 57.3 us
-// with 3 tiles a work-group, 63.8 with 4; 64 heads of 32: 4096 rows 68.8 with 2, 96.0 with 4)
+// column tiles of 16 a work-group: what a head's fewest work-groups of up to 4 share out evenly (bfloat16 rows: 796 of 128 heads of
+// 80 x 128 58.7 us with 3 tiles a work-group, 65.3 with 4; 4096 of 64 heads of 32 x 128 66.7 with 2, 89.8 with 4, of 32 x 256 146.8 and 193.8)
 template <int QT, int KT, bool STATE>
 void launch_scan(ns_gpu* g, const ScanParams& s, unsigned blocks) {
     const int tiles = ((s.l.P + 15) / 16 + s.blocks - 1) / s.blocks;

@@ -27,3 +27,21 @@ def test_limits_of_either_sign(ops, qt, T, rate, lo, hi):
     got, state = c.out()
     check_scan(got, y, yb, qt, T, N, "y")
     check_scan(state, h[T], hb[T], F32, T, N, "state")
+
+
+def test_a_slot_whose_first_position_is_negative_is_passed_over(ops):
+    g, H, P, N, K, cap = ops.gpu, 2, 8, 16, 4, 7
+    L = Layer(H, P, N, 1, K, seed=43)
+    raw, val = rows_of(L, F32, 3, 44)
+    ring = np.random.default_rng(45).standard_normal((2, cap, L.chan)).astype(np.float32)
+    h0 = np.random.default_rng(46).standard_normal((2, H, P, N)).astype(np.float32)
+    w = [DevBuf.of(g, a) for a in (L.cw, L.cb, L.a, L.dtb, L.d)]
+    rows, ringb, h0b, h1b, y, row = DevBuf.of(g, raw), DevBuf.of(g, ring), DevBuf.of(g, h0), DevBuf(g, h0.nbytes), DevBuf(g, 3 * L.inner * 4), L.chan + H
+    h1b.fill(0xFF)
+    y.fill(0xFF)
+    ops.ssm_step(F32, rows, row, rows.view(L.chan * 4, rows.len - L.chan * 4), row, *w, ringb, cap, 0, 3, H, P, N, 1, K, h0b, h1b, y, L.inner, nslots=2,
+                 slots=DevBuf.of(g, np.array([1, 0, 1], np.int32)), pos=DevBuf.of(g, np.array([-1, 5, 0], np.int32)))
+    got = y.read(np.uint32).reshape(3, -1)
+    assert (got[[0, 2]] == 0xFFFFFFFF).all() and (h1b.read(np.uint32).reshape(2, -1)[1] == 0xFFFFFFFF).all() and np.array_equal(ringb.read(np.float32).reshape(ring.shape)[1], ring[1])
+    r, h, rb, hb = scan(L, val[1:2, :L.chan], val[1:2, L.chan:], ring[0][np.arange(2, 5) % cap], h0[0])
+    check_scan(got[1:2].view(np.float32), r, rb, F32, 1, N, "the other slot")
