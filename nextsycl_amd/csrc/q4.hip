@@ -12,10 +12,9 @@
 // A work-group of 8 or 16 waves takes 16 outputs and shares K among its waves, tile by tile; the waves' sums meet in LDS in a
 // fixed order. Rows that fit its LDS as operands are laid out there by each work-group, while its first weights are on
 // their way; longer ones once, by a kernel in front, in the library's own scratch. A wave asks for a tile while it takes the
-// one before (two ahead: a half row x 18560 outputs of 4096 inputs in groups of 32 12.8 us, one ahead 11.1: more waves fit).
-// That row: 43 MB, 3.8 TB/s, 8.3 us at a copy's rate - four waves a SIMD ask for 1.1 KB each and unpack between (30 vector
-// instructions a matrix instruction). 8 float32 rows x 4096 of 8192 in groups of 128 10.6 us: the rows' kernel 2.6, then the
-// weights' 17 MB in 9.0, a work-group a CU.
+// one before. A half row x 18560 outputs of 4096 inputs in groups of 32: 10.4 us, 43 MB, 4.1 TB/s (8.3 us at a copy's rate) - four waves a SIMD ask
+// for 1.1 KB each and unpack between (28 vector instructions a matrix instruction). 8 float32 rows x 4096 of 8192 in groups of 128 9.8 us: the rows'
+// kernel 2.6, then the weights' 17 MB in 8.3, a work-group a CU, four tiles a wave one behind the other.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

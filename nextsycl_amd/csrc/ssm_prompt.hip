@@ -22,14 +22,14 @@
 // Where heads alone do not fill the chip the prompt is cut in segments: the same kernel first leaves the states of their
 // pieces from a start of zero (STATE: half of the work), and each segment's scan starts from those before it, decayed.
 //
-// Bound: vector instructions. 8192 bfloat16 rows of 128 heads of 64 x 128 (308 MB in and out: 60 us at a copy's rate; 85 GFLOP as
-// executed: 75 us at a large product's) take 297 - 305 us: 42 in the first kernel (134 MB: 26 us), 89 for the segments' states, 175 for the
-// scan - of x's convolution, the splits, the decays and the state's scaling and sums 8 to 11 vector instructions a matrix
-// instruction, in three waves a SIMD that spend 24 % of their life issuing one, 31 % ready for it and the rest at barriers and
-// loads (matrix unit 20 % busy). 2051 float32 rows of 64 heads 73 us (10 + 22 + 43), 85 half rows of 128 heads of 80 23 us:
-// two launches and two chunks of 5 us each. Work-groups a CU, 8192 bfloat16 rows: three of the scan 297 us, two - with x and
-// the operands asked for a chunk ahead, for which they have the registers - 309; of the segments' states three, with that, 297, four without it 304, two
-// 298. Float32 and half rows have both halfs of each operand in LDS, and so two.
+// Bound: no unit's rate, but steps that wait for one another. 8192 bfloat16 rows of 128 heads of 64 x 128 (308 MB in and out: 60 us at a copy's
+// rate; 121 GFLOP of half products as executed, the segments' states and C . B among them: 113 us at a large product's) take 298 - 306 us: 40 in
+// the first kernel (51 MB read, 94 written), 87 for the segments' states, 178 for the scan - 8 to 12 vector instructions a matrix instruction, of
+// x's convolution, the splits, the decays and the state's scaling and sums, in three waves a SIMD that spend 24 % of their life issuing one, 29 %
+// ready for it and the rest at barriers and loads (matrix unit 19 - 23 % busy). 2051 float32 rows of 64 heads (80 MB: 16 us; 22 GFLOP: 21) 71 - 76
+// us (10 + 22 + 45), 85 half rows of 128 heads of 80 24: two launches and two chunks of 5 us each. Work-groups a CU, 8192 bfloat16 rows: three of
+// the scan 300 us, two - with x and the operands asked for a chunk ahead, for which they have the registers - 320; of the segments' states two or
+// three alike. Float32 and half rows have both halfs of each operand in LDS, and so two.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(256, (SCAN_WGS<QT, KT, STATE>)) void ssm_scan_kerne
     constexpr int KK = 2 * KT;
     constexpr bool AHEAD = STATE || SCAN_WGS<QT, KT, STATE> <= 2;     // x and the operands asked for early, where there are registers for them
     // y's products from both halfs of their operands - the state, C, x, C . B with its decays -, but for bfloat16 rows: what first halfs lose, 2^-11
-    // each, is an eighth of y's own rounding (8192 rows' error against 64 bits is 1.7e-3 of y either way), and one plane of the state and of x
+    // each, is an eighth of y's own rounding (8192 rows' error against 64 bits is 1.680e-3 of y, 1.658e-3 with both), and one plane of the state and of x
     // leaves LDS and registers for three work-groups a CU (298 us; 365 with both halfs, two work-groups)
     constexpr bool Y3 = QT != 2;
     // x weighted for the state (hi, lo) and as it is (hi, for Y3 lo): [32 rows][16 columns][lane]; the state: [32 features][..]

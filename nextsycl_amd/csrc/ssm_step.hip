@@ -3,12 +3,13 @@
 //
 // A row's head: h = exp(dt a) h + dt x (outer) B, y = h C + d x over a state of P x N floats that nothing else of the call
 // touches. Bound: HBM - the state is read and written once (8 H P N bytes a sequence, 8.4 MB at 128 heads of 64 x 128) for
-// 5 operations a float. So a lane holds 4 consecutive features of a few of the head's P rows, asks for them before anything
-// else, and the convolution (a few hundred channels, each group's B and C by every head of the group: 4 multiply-adds and
+// 5 operations a float. So a lane holds 4 consecutive features of a few of the head's P rows and asks for them right behind
+// what the convolution reads, which (a few hundred channels, each group's B and C by every head of the group: 4 multiply-adds and
 // a few KB that the cache holds) runs while they are on their way; y is a sum over a row's lanes. Rows of one slot
 // are walked with the state in registers, their convolutions four rows at a time.
 // 128 heads of 64 x 128: 64 tokens (548 MB) 107 - 109 us, 5.1 TB/s - a copy's rate; one token 5.4 us, a launch and the two latencies of
-// its loads and sums (1.6 us of bytes); 12 half rows of 3 slots, 128 heads of 80 x 128, 14.7 us (33 MB: 6.3). Four work-groups a CU (those
+// its loads and sums (1.6 us of bytes); 12 half rows of 3 slots, 128 heads of 80 x 128, 14.7 us (33 MB: 6.3): a row of each 9.3, each further
+// row 1.9. Four work-groups a CU (those
 // rows with three, 8 state rows a lane: 17.0, for 15.8), four rows at a time (two: 16.5).
 #include <algorithm>
 #include <cmath>
