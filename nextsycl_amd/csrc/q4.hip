@@ -248,11 +248,10 @@ int launch_product(ns_gpu* g, Q4Params& p) {
     q4_product_kernel<QT, GR, true, WAVES><<<grid, 64 * WAVES, sums, g->q>>>(p);
     return 0;
 }
-// 16 waves where each work-group has a CU of its own (up to 256 of them: 4096 outputs), else 8: a row x 4096 outputs of 8192 half inputs
-// 6.81 us with 8 waves, 5.96 with 16; 8 float32 rows of them 11.0 and 10.2 - 10.7; 2 half rows x 8192 of 5120 7.85 and 9.10, a row
-// x 18560 of 4096 11.1 and 16.5. On both sides of the line, inputs of 2048 and 8192: a half row x 4096 in groups of 32 3.9 and 7.2 us with 8, 3.5 and
-// 6.4 with 16, x 4112 3.6 and 8.7, 4.6 and 10.1, x 6144 3.9 and 9.5, 5.0 and 10.8; 8 float32 rows x 4112 in groups of 128 6.9 and 14.6, 7.8 and
-// 15.8. Whatever the rows' number, so that a row has the same bits alone and among others
+// 16 waves where each work-group has a CU of its own (up to 256 of them: 4096 outputs), else 8. Of 8192 inputs, a half row in groups of 32: 4096
+// outputs 7.2 us with 8 waves, 6.3 with 16; 4112 8.7 and 8.0, 6144 9.4 and 8.7, 8192 9.7 and 9.2, but 18560 of 4096 10.9 and 12.2. 8 float32 rows
+// in groups of 128: 4096 10.2 and 9.8, 4112 14.2 and 15.5, 6144 14.8 and 15.6. Whatever the rows' number, so that a row has the same bits alone
+// and among others
 template <int QT, int GR>
 int launch_product(ns_gpu* g, Q4Params& p) {
     return p.M <= WIDE_M ? launch_product<QT, GR, 16>(g, p) : launch_product<QT, GR, 8>(g, p);
