@@ -24,6 +24,7 @@
 
 #include "ns.h"
 #include "ns_attn.h"
+#include "ns_kv8.h"
 #include "ns_layer.h"
 #include "ns_mla.h"
 #include "ns_pre.h"
@@ -68,6 +69,10 @@ public:
 // a hybrid model's other layers (ns_layer.h)
 #define NS_HOST_LAYER_SYMBOLS(X)                                                                                                         \
     X(ns_ssm_prompt_scratch) X(ns_ssm_prompt) X(ns_ssm_step) X(ns_norm_gated) X(ns_norm_residual) X(ns_q4_bytes) X(ns_q4_pack) X(ns_q4_product)
+
+// caches of 8-bit values in blocks of tokens (ns_kv8.h)
+#define NS_HOST_KV8_SYMBOLS(X)                                                                                                           \
+    X(ns_kv8_store) X(ns_kv8_attend_scratch) X(ns_kv8_attend) X(ns_kv8_prompt) X(ns_kv8_weights) X(ns_kv8_evict)
 
 class Api {
 public:
@@ -129,6 +134,19 @@ public:
     explicit LayerApi(const Api& a) {
 #define NS_HOST_BIND(name) name = a.symbol<decltype(name)>(#name);
         NS_HOST_LAYER_SYMBOLS(NS_HOST_BIND)
+#undef NS_HOST_BIND
+    }
+};
+
+// The same for caches of 8-bit values in blocks.
+class Kv8Api {
+public:
+#define NS_HOST_FIELD(name) decltype(&::name) name = nullptr;
+    NS_HOST_KV8_SYMBOLS(NS_HOST_FIELD)
+#undef NS_HOST_FIELD
+    explicit Kv8Api(const Api& a) {
+#define NS_HOST_BIND(name) name = a.symbol<decltype(name)>(#name);
+        NS_HOST_KV8_SYMBOLS(NS_HOST_BIND)
 #undef NS_HOST_BIND
     }
 };

@@ -8,7 +8,7 @@ Error("<what>: <ns_last_error>"). The call order of a pass is the engines': kv_s
 (llm/museglimmer/src/engine.rs:856-873). Nothing here computes: the HIP library does, or the call fails."""
 import ctypes as C
 
-from .core import Error, api
+from .core import DevBuf, Error, api
 from .sys import P, f32, i32, i64
 
 F32, F16, BF16 = 0, 1, 2                       # q / out element types (NS_F32, NS_F16, NS_BF16)
@@ -150,6 +150,17 @@ LAYER_H = {
 }
 
 
+# include/ns_kv8.h
+KV8_H = {
+    "ns_kv8_store": (i32, [P, i32, i32, P, i64, P, i64, i64, P, P, i64, i64, P, i64, i64, i64, i64, i64, P, P, P, P]),
+    "ns_kv8_attend_scratch": (i64, [i64, i64, i64, i64, i64, i64, i32]),
+    "ns_kv8_attend": (i32, [P, i32, i32, P, i64, i64, P, P, i64, i64, i64, P, i64, i64, i64, i64, i64, i64, P, P, P, P, i64, f32, P, P, P, P]),
+    "ns_kv8_prompt": (i32, [P, i32, i32, P, i64, i64, P, i64, i64, i64, i64, i64, i64, i64, P, P, P, P, i64, f32, P]),
+    "ns_kv8_weights": (i32, [P, i32, i32, P, i64, i64, P, i64, i64, i64, i64, i64, i64, i64, P, P, i64, f32, P, P]),
+    "ns_kv8_evict": (i32, [P, i32, P, P, i64, i64, i64, i64, i64, P, P, i64, i64, i64, i64, i64, P, P, P, P, P]),
+}
+
+
 def _absent(why):
     def call(*args):
         raise Error(why)
@@ -157,14 +168,14 @@ def _absent(why):
 
 
 class Kernels:
-    """Every attention entry point bound by name; a missing symbol fails the load. A hybrid model's other layers (LAYER_H) are not every engine's: a
-    library without them loads, and calling one raises Error."""
+    """Every attention entry point bound by name; a missing symbol fails the load. A hybrid model's other layers (LAYER_H) and 8-bit caches in blocks
+    (KV8_H) are not every engine's: a library without them loads, and calling one raises Error."""
 
     def __init__(self, a=None):
         self.api = a or api()
         for name, (res, args) in list(ATTN_H.items()) + list(MLA_H.items()) + list(PRE_H.items()):
             setattr(self, name[3:], self.api.symbol(name, res, args))
-        for name, (res, args) in LAYER_H.items():
+        for name, (res, args) in list(LAYER_H.items()) + list(KV8_H.items()):
             try:
                 entry = self.api.symbol(name, res, args)
             except OSError as e:
@@ -208,6 +219,25 @@ def _addresses(entries):
     except (C.ArgumentError, TypeError):
         return None
     return at if all(at) else None
+
+
+KV8_INT8, KV8_E4M3 = 0, 1                      # forms of a cache of 8-bit values in blocks
+
+
+class Kv8:
+    """A cache of 8-bit values in blocks of tokens (include/ns_kv8.h): pools k, v [blocks][Hkv][block][D] bytes, scales ks, vs [blocks][Hkv] float32."""
+
+    def __init__(self, form, blocks, Hkv, block, D, k, v, ks, vs):
+        self.form, self.blocks, self.Hkv, self.block, self.D = form, blocks, Hkv, block, D
+        self.k, self.v, self.ks, self.vs = k, v, ks, vs
+        for b, n, what in ((k, D * block, "key pool"), (v, D * block, "value pool"), (ks, 4, "key scales"), (vs, 4, "value scales")):
+            _need(b, blocks * Hkv * n, "kv8 " + what)
+
+    @staticmethod
+    def new(gpu, form, blocks, Hkv, block, D):
+        """One with memory of its own."""
+        pool, scales = blocks * Hkv * block * D, blocks * Hkv * 4
+        return Kv8(form, blocks, Hkv, block, D, DevBuf(gpu, pool), DevBuf(gpu, pool), DevBuf(gpu, scales), DevBuf(gpu, scales))
 
 
 class Ops:
@@ -743,6 +773,82 @@ class Ops:
             _need(w, self.q4_bytes(M, K, group), "q4_product weights")
             _need(y, ((T - 1) * ys + M) * e, "q4_product y")
         self.ok(self.k.q4_product(self.raw(), qt, x.ptr, xs, w.ptr, group, y.ptr, ys, T, M, K), "q4_product")
+
+    # ---- caches of 8-bit values in blocks of tokens (include/ns_kv8.h): `cache` a Kv8, `table` [S][tmax] int32, `lens` [S] and `start` [S + 1] int32 on the GPU
+    def _kv8_seqs(self, what, table, tmax, S, lens, start):
+        _need(table, S * tmax * 4, what + " tables")
+        _need(lens, S * 4, what + " lengths")
+        if start is not None:
+            _need(start, (S + 1) * 4, what + " starts")
+
+    def kv8_store(self, cache, qt, k, ks, v, vs, T, table, tmax, S, most, lens, start=None):
+        """ns_kv8_store: rows k, v [T][Hkv D] of S sequences, `most` each at most, behind their lens[s] tokens."""
+        c, e = cache, _elt(qt, "kv8_store")
+        if T > 0:
+            _need(k, ((T - 1) * ks + c.Hkv * c.D) * e, "kv8_store k")
+            _need(v, ((T - 1) * vs + c.Hkv * c.D) * e, "kv8_store v")
+        self._kv8_seqs("kv8_store", table, tmax, S, lens, start)
+        self.ok(self.k.kv8_store(self.raw(), c.form, qt, k.ptr, ks, v.ptr, vs, T, start.ptr if start is not None else None, lens.ptr, S, most, table.ptr, tmax,
+                                 c.Hkv, c.D, c.block, c.blocks, c.k.ptr, c.v.ptr, c.ks.ptr, c.vs.ptr), "kv8_store")
+
+    def kv8_attend_scratch(self, S, most, Hq, Hkv, D, longest, acc=False):
+        """Floats of scratch kv8_attend needs."""
+        return self.k.kv8_attend_scratch(S, most, Hq, Hkv, D, longest, int(acc))
+
+    def kv8_attend(self, cache, qt, q, qs, T, table, tmax, S, most, longest, lens, Hq, out, scratch, start=None, win=0, scale=0.0, acc0=None, acc1=None):
+        """ns_kv8_attend: T rows of S sequences, 1 to 16 each, over their cached tokens and their own; acc1 = acc0 (None: zeros) + the weights they give."""
+        c, e = cache, _elt(qt, "kv8_attend")
+        if T > 0:
+            _need(q, ((T - 1) * qs + Hq * c.D) * e, "kv8_attend q")
+            _need(out, T * Hq * c.D * e, "kv8_attend out")
+        self._kv8_seqs("kv8_attend", table, tmax, S, lens, start)
+        need = self.kv8_attend_scratch(S, most, Hq, c.Hkv, c.D, longest, acc1 is not None) * 4
+        if need:
+            _need(scratch, need, "kv8_attend scratch")
+        self._kv8_acc("kv8_attend", c, acc0, acc1)
+        opt = lambda b: b.ptr if b is not None else None
+        self.ok(self.k.kv8_attend(self.raw(), c.form, qt, q.ptr, qs, T, opt(start), lens.ptr, S, most, longest, table.ptr, tmax, Hq, c.Hkv, c.D, c.block, c.blocks,
+                                  c.k.ptr, c.v.ptr, c.ks.ptr, c.vs.ptr, win, scale, out.ptr, opt(acc0), opt(acc1), opt(scratch)), "kv8_attend")
+
+    def _kv8_acc(self, what, c, *accs):
+        for b in accs:
+            if b is not None:
+                _need(b, c.blocks * c.Hkv * c.block * 4, what + " weights")
+
+    def kv8_prompt(self, cache, qt, q, qs, T, table, tmax, p0, Hq, out, win=0, scale=0.0):
+        """ns_kv8_prompt: T rows of one sequence, tokens p0 .. p0 + T - 1, over the tokens up to their own."""
+        c, e = cache, _elt(qt, "kv8_prompt")
+        if T > 0:
+            _need(q, ((T - 1) * qs + Hq * c.D) * e, "kv8_prompt q")
+            _need(out, T * Hq * c.D * e, "kv8_prompt out")
+        _need(table, tmax * 4, "kv8_prompt table")
+        self.ok(self.k.kv8_prompt(self.raw(), c.form, qt, q.ptr, qs, T, table.ptr, tmax, p0, Hq, c.Hkv, c.D, c.block, c.blocks, c.k.ptr, c.v.ptr, c.ks.ptr, c.vs.ptr,
+                                  win, scale, out.ptr), "kv8_prompt")
+
+    def kv8_weights(self, cache, qt, q, qs, T, table, tmax, p0, Hq, acc0, acc1, win=0, scale=0.0):
+        """ns_kv8_weights: acc1 = acc0 (None: zeros) + what T rows of one sequence give every token up to theirs."""
+        c, e = cache, _elt(qt, "kv8_weights")
+        if T > 0:
+            _need(q, ((T - 1) * qs + Hq * c.D) * e, "kv8_weights q")
+        _need(table, tmax * 4, "kv8_weights table")
+        if acc1 is None:
+            raise Error("kv8_weights weights: no buffer")
+        self._kv8_acc("kv8_weights", c, acc0, acc1)
+        self.ok(self.k.kv8_weights(self.raw(), c.form, qt, q.ptr, qs, T, table.ptr, tmax, p0, Hq, c.Hkv, c.D, c.block, c.blocks, c.k.ptr, c.ks.ptr, win, scale,
+                                   acc0.ptr if acc0 is not None else None, acc1.ptr), "kv8_weights")
+
+    def kv8_evict(self, cache, acc, table, tmax, S, longest, lens, lens1, keep, first=0, last=0, to=None):
+        """ns_kv8_evict: every sequence of more than `keep` tokens down to its first, its last and its heaviest ones, in place or into the blocks of `to`."""
+        c = cache
+        if acc is None:
+            raise Error("kv8_evict weights: no buffer")
+        self._kv8_acc("kv8_evict", c, acc)
+        self._kv8_seqs("kv8_evict", table, tmax, S, lens, None)
+        _need(lens1, S * 4, "kv8_evict lengths")
+        if to is not None:
+            _need(to, S * tmax * 4, "kv8_evict tables")
+        self.ok(self.k.kv8_evict(self.raw(), c.form, lens.ptr, lens1.ptr, S, longest, keep, first, last, table.ptr, to.ptr if to is not None else None, tmax, c.Hkv, c.D,
+                                 c.block, c.blocks, c.k.ptr, c.v.ptr, c.ks.ptr, c.vs.ptr, acc.ptr), "kv8_evict")
 
     # ---- the step in front of attention: norm, rotary positions, store
     def q35_qk_norm_rope(self, src, ss, hs, dst, ds, T, H, D, w, eps, n_rot, theta, p0, pos3=None, sections=(0, 0, 0)):

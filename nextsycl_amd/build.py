@@ -38,6 +38,10 @@ SOURCES = {
     "ssm_prompt.hip": [],
     "norm_rows.hip": [],
     "q4.hip": [],
+    "kv8_store.hip": [],
+    "kv8_attend.hip": [],
+    "kv8_weights.hip": [],
+    "kv8_evict.hip": [],
 }
 
 

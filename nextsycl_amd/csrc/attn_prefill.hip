@@ -593,7 +593,7 @@ PromptPlan prompt_plan(size_t own, int qt, int kt, int64_t T, int64_t Hq, int64_
 
 int ns_attn_prompt_any(ns_gpu* g, const char* who, int qt, int kt, int pm, const void* q, int64_t qs, const void* kc, const void* vc, int64_t T,
                        int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, int64_t p0, int64_t win, int causal, int64_t kfirst, float scale,
-                       void* out) {
+                       void* out, size_t own) {
     NS_TRY
     const std::string w(who);
     if (T <= 0) return 0;
@@ -611,7 +611,7 @@ int ns_attn_prompt_any(ns_gpu* g, const char* who, int qt, int kt, int pm, const
     // rows are fetched in 16-byte chunks: every 16-bit row keeps that alignment, q8_0 / q4_0 rows do at D = 256 (272 / 144
     // bytes; the reference's quantized prompt form is D = 256 only); at D = 128 (136 / 72 bytes) the chunks are 8-byte aligned
     if (((uintptr_t) kc | (uintptr_t) vc) % (rb % 16 ? 8 : 16)) return ns_fail(w + (rb % 16 ? ": caches 8-byte aligned" : ": caches 16-byte aligned"));
-    const PromptPlan pl = prompt_plan(ns_own_floats(g), qt, kt, T, Hq, Hkv, D, p0, win, causal, kfirst);
+    const PromptPlan pl = prompt_plan(own ? own : ns_own_floats(g), qt, kt, T, Hq, Hkv, D, p0, win, causal, kfirst);
     const int PWs = pl.waves;
     const int64_t ROWS = rows_of((int) D, PWs);
     if (T > (int64_t) 1 << 30 || ((T + ROWS - 1) / ROWS + 1) * Hq > (int64_t) 1 << 30) return ns_fail(w + ": too many rows or heads");

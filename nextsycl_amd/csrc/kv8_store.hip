@@ -1,0 +1,162 @@
+// kv8_store.hip: key and value rows into a cache of 8-bit values in blocks of tokens, and blocks widened to half rows (gfx950).
+//
+// A block's scale is a power of two: 2^x m / M against the largest magnitude 2^x m needs only its exponent and a comparison of m, a value
+// over it is exact, its code the one rounding. In a block that holds rows the scale only grows; the codes that were there, whole numbers
+// (or e4m3) of the old unit, are re-rounded to the new one, 2^k of it: half a step of the new unit at most, and over any number of
+// growths 1/2 + 1/4 + .. of the final one.
+//
+// Bound: HBM, rows read once and codes written. A work-group takes one block of one key head and stream, all of its new rows
+// in registers (16 threads a row of 128, 8 values each): their largest magnitude, then their codes.
+#include "attn_host.hpp"
+#include "kv8_common.hpp"
+
+namespace {
+
+struct StoreParams {
+    Kv8Cache c;
+    const void *k, *v;
+    int64_t ks, vs;
+    const int32_t *start, *lens;
+    int T, most;
+};
+
+// TH threads, NP passes over a block's rows: block x D = 8 TH NP values
+template <int QT, int FORM, int D, int TH, int NP>
+__global__ __launch_bounds__(TH) void kv8_store_kernel(const StoreParams p) {
+    constexpr int TPR = D / 8, RPP = TH / TPR, B = RPP * NP;      // threads a row, rows a pass, rows a block
+    __shared__ float red[TH / 64];
+    const int tid = threadIdx.x, s = blockIdx.z;
+    const int h = blockIdx.y >> 1, val = blockIdx.y & 1;
+    const Kv8Seq q = kv8_seq(p.start, p.lens, s, p.T, p.most);
+    const int64_t e = q.len / B + (int) blockIdx.x;
+    const int64_t t0 = e * B, end = (int64_t) q.len + q.n;        // the block's tokens from t0 on; the call's end at `end`
+    if (q.n <= 0 || t0 >= end) return;
+    const int b = kv8_block(p.c, p.c.table, s, e);
+    if (b < 0) return;
+    const bool fresh = t0 >= q.len;
+    uint8_t* pool = (val ? p.c.vc : p.c.kc) + kv8_rows(p.c, b, h) * D;
+    float* scale = (val ? p.c.vsc : p.c.ksc) + (int64_t) b * p.c.Hkv + h;
+    const void* src = val ? p.v : p.k;
+    const int64_t stride = val ? p.vs : p.ks;
+    const int row = tid / TPR, col = tid % TPR * 8;
+    const float s0 = fresh ? 0.0f : *scale;
+
+    float x[NP][8], most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int64_t t = t0 + i * RPP + row;
+        if (t < q.len || t >= end) continue;
+        const int64_t at = (q.first + (t - q.len)) * stride + (int64_t) h * D + col;
+        if constexpr (QT == 0) {
+            float lo[4], hi[4];
+            load_row<0, 4>(src, at, lo), load_row<0, 4>(src, at + 4, hi);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i][j] = lo[j], x[i][4 + j] = hi[j];
+        } else load_row<QT, 8>(src, at, x[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[i][j]));      // (fmaxf: NaN counts as nothing)
+    }
+    most = wave_max(most);
+    if (tid % 64 == 0) red[tid / 64] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TH / 64; ++w) most = fmaxf(most, red[w]);
+    const float s1 = fmaxf(s0, kv8_pow2(kv8_exponent<FORM>(most))), inv = 1.0f / s1, ratio = s0 * inv;
+    if (!fresh && s1 > s0) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int64_t t = t0 + i * RPP + row;
+            if (t >= q.len && t < end) continue;
+            uint2* at = reinterpret_cast<uint2*>(pool + (i * RPP + row) * D + col);
+            const uint2 w = *at;
+            *at = uint2{kv8_reround<FORM>(w.x, ratio), kv8_reround<FORM>(w.y, ratio)};
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int64_t t = t0 + i * RPP + row;
+        if (t < q.len || t >= end) continue;
+        *reinterpret_cast<uint2*>(pool + (i * RPP + row) * D + col) =
+            uint2{kv8_codes<FORM>(x[i][0] * inv, x[i][1] * inv, x[i][2] * inv, x[i][3] * inv), kv8_codes<FORM>(x[i][4] * inv, x[i][5] * inv, x[i][6] * inv, x[i][7] * inv)};
+    }
+    if (tid == 0 && (fresh || s1 > s0)) *scale = s1;
+}
+
+template <int QT, int FORM, int D>
+void launch_store(ns_gpu* g, const StoreParams& p, dim3 grid) {
+    if (p.c.block == 16) kv8_store_kernel<QT, FORM, D, 16 * D / 8, 1><<<grid, 16 * D / 8, 0, g->q>>>(p);
+    else if (p.c.block == 32) kv8_store_kernel<QT, FORM, D, 16 * D / 8, 2><<<grid, 16 * D / 8, 0, g->q>>>(p);
+    else if (p.c.block == 64) kv8_store_kernel<QT, FORM, D, 16 * D / 8, 4><<<grid, 16 * D / 8, 0, g->q>>>(p);
+    else kv8_store_kernel<QT, FORM, D, 16 * D / 8, 8><<<grid, 16 * D / 8, 0, g->q>>>(p);
+}
+template <int QT>
+void launch_store(ns_gpu* g, int form, const StoreParams& p, dim3 grid) {
+    if (p.c.D == 128) form == 0 ? launch_store<QT, 0, 128>(g, p, grid) : launch_store<QT, 1, 128>(g, p, grid);
+    else form == 0 ? launch_store<QT, 0, 256>(g, p, grid) : launch_store<QT, 1, 256>(g, p, grid);
+}
+
+// tokens from .. from + n of one sequence as half rows, k and v [heads][n][D]: a thread 16 values
+template <int FORM>
+__global__ __launch_bounds__(256) void kv8_widen_kernel(const Kv8Cache c, int h0, int64_t from, int64_t n, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
+    const int tpr = c.D / 16, h = h0 + blockIdx.y;
+    const int64_t j = ((int64_t) blockIdx.x * 256 + threadIdx.x) / tpr;
+    if (j >= n) return;
+    const int col = threadIdx.x % tpr * 16;
+    const int64_t t = from + j;
+    const int b = kv8_block(c, c.table, 0, t >> c.shift);
+    s8v lo = {0, 0, 0, 0, 0, 0, 0, 0}, hi = lo;
+    if (b >= 0) {
+        const uint4 w = *reinterpret_cast<const uint4*>((blockIdx.z ? c.vc : c.kc) + (kv8_rows(c, b, h) + (t & (c.block - 1))) * c.D + col);
+        const float s = (blockIdx.z ? c.vsc : c.ksc)[(int64_t) b * c.Hkv + h];
+        lo = kv8_halfs8<FORM>(w.x, w.y, s, s), hi = kv8_halfs8<FORM>(w.z, w.w, s, s);
+    }
+    s8v* d = reinterpret_cast<s8v*>((blockIdx.z ? v : k) + ((int64_t) blockIdx.y * n + j) * c.D + col);
+    d[0] = lo, d[1] = hi;
+}
+
+}  // namespace
+
+int ns_kv8_widen(ns_gpu* g, int form, const Kv8Cache& c, int h0, int nh, int64_t from, int64_t n, uint16_t* k, uint16_t* v) {
+    const dim3 grid((unsigned) ((n * (c.D / 16) + 255) / 256), (unsigned) nh, v ? 2 : 1);
+    if (form == 0) kv8_widen_kernel<0><<<grid, 256, 0, g->q>>>(c, h0, from, n, k, v);
+    else kv8_widen_kernel<1><<<grid, 256, 0, g->q>>>(c, h0, from, n, k, v);
+    NS_LAUNCHED("kv8_widen");
+    return 0;
+}
+
+int ns_kv8_check(const std::string& who, int form, int64_t Hkv, int64_t D, int64_t block, int64_t blocks, int64_t S, int64_t tmax, const Kv8Cache& c) {
+    if (form < 0 || form > 1) return ns_fail(who + ": a cache form 0 (int8) or 1 (e4m3)");
+    if (D != 128 && D != 256) return ns_fail(who + ": heads of 128 or 256");
+    if (block != 16 && block != 32 && block != 64 && block != 128) return ns_fail(who + ": blocks of 16, 32, 64 or 128 tokens");
+    if (Hkv <= 0 || Hkv > 32767) return ns_fail(who + ": 1 to 32767 key heads");
+    if (blocks <= 0 || blocks > INT32_MAX || tmax <= 0 || tmax > INT32_MAX) return ns_fail(who + ": a pool and tables of 1 to 2^31 - 1 blocks");
+    if (S <= 0 || S > 65535) return ns_fail(who + ": 1 to 65535 sequences");
+    if (!c.kc || !c.ksc || !c.table) return ns_fail(who + ": a null buffer");
+    if (((uintptr_t) c.kc | (uintptr_t) c.vc) % 16) return ns_fail(who + ": pools 16-byte aligned");
+    return 0;
+}
+
+extern "C" int ns_kv8_store(ns_gpu* g, int form, int qt, const void* k, int64_t ks, const void* v, int64_t vs, int64_t T, const int32_t* start, const int32_t* lens,
+                            int64_t S, int64_t most, const int32_t* table, int64_t tmax, int64_t Hkv, int64_t D, int64_t block, int64_t blocks, void* kc,
+                            void* vc, float* ksc, float* vsc) {
+    NS_TRY
+    const std::string w("ns_kv8_store");
+    if (T <= 0 || S <= 0 || most <= 0) return 0;
+    StoreParams p{kv8_cache(kc, vc, ksc, vsc, table, tmax, Hkv, D, block, blocks), k, v, ks, vs, start, lens, 0, 0};
+    if (qt < 0 || qt > 2) return ns_fail(w + ": rows of type 0 (float32), 1 (half) or 2 (bfloat16)");
+    if (ns_kv8_check(w, form, Hkv, D, block, blocks, S, tmax, p.c)) return -1;
+    if (T > KV8_TOKENS || most > KV8_TOKENS) return ns_fail(w + ": up to 2^30 rows");
+    if (ks < Hkv * D || vs < Hkv * D) return ns_fail(w + ": rows at least as far apart as they are long");
+    if (!g || !k || !v || !lens || !vc || !vsc) return ns_fail(w + ": a null buffer");
+    most = std::min(most, T);
+    p.T = (int) T, p.most = (int) most;
+    const dim3 grid((unsigned) ((most + block - 2) / block + 1), (unsigned) (2 * Hkv), (unsigned) S);
+    if (!ns_grid_fits(grid.x, 16 * D / 8)) return ns_fail(w + ": more rows than a launch takes");
+    NS_HIP(hipSetDevice(g->dev));
+    if (qt == 0) launch_store<0>(g, form, p, grid);
+    else if (qt == 1) launch_store<1>(g, form, p, grid);
+    else launch_store<2>(g, form, p, grid);
+    NS_LAUNCHED("kv8_store");
+    return 0;
+    NS_CATCH
+}
