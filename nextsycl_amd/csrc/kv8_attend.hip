@@ -4,10 +4,12 @@
 // Bound: HBM - every visible key and value byte read once for all rows and query heads of its key head; 4 D flops a (row, head,
 // token), far under the matrix unit's ridge.
 //
-// Work split: a work-group of 4 waves takes tokens [s kbs, (s + 1) kbs) of one sequence and key head (and 16 or 32 of its row, head
-// pairs, i G + g); wave w the 32-token tiles t % 4 == w, each through two buffers of its own in LDS (the next tile's transfers under
-// way while this one is worked on): no barrier in the loop. The waves' (O, m, l) meet in LDS in wave order; of several splits a second
-// kernel makes one. A wave holds its split's table entries and scales in two registers a lane and picks them by lane reads.
+// Work split: the tokens of all sequences and key heads lie end to end in chunks of 128, and each work-group takes an equal run of them - the
+// lengths are known on the device only, and differ: with a grid over the longest sequence's splits 64 sequences of 125 to 8000 tokens
+// kept a quarter of the waves' places busy. A run that ends inside a (sequence, key head) leaves a partial there, one that begins inside it another: two places a
+// work-group hold them, and a second kernel puts a unit's pieces together. Wave w takes a chunk's tile w of 32 tokens through one buffer of keys
+// and one of values of its own in LDS, asked for again as soon as their values lie in registers: no barrier in the loop. The waves' (O, m, l) meet in LDS
+// in wave order. A wave holds its next 128 table entries and scales in two registers a lane and picks them by lane reads.
 //
 // A tile in the transposed orientation, as in attn_decode.hip: S^T[token][pair] = K Q^T with K's codes as halfs and the block's scale on
 // the score; online softmax in base 2, float32; O^T[d][pair] += V^T P^T with V as halfs code x scale - exactly - read by the
@@ -23,8 +25,7 @@
 
 namespace {
 
-constexpr int WAVES = 4, TILE = 32;
-constexpr int MOST_SPLIT = 2048;                  // tokens a split, at most: 128 table entries of 16 tokens, two a lane
+constexpr int WAVES = 4, TILE = 32, CHUNK = WAVES * TILE;
 
 struct AttendParams {
     Kv8Cache c;
@@ -33,11 +34,12 @@ struct AttendParams {
     const int32_t *start, *lens;
     int64_t p0;                 // lens null: the one sequence's tokens in front of the call, its T rows
     int T, most, S, Hq, G;
-    int64_t longest, win, kbs;
-    int ns, nz;                 // splits of the longest sequence; chunks of pairs
+    int64_t longest, win;
+    int nw, nz;                 // work-groups the chunks are dealt to; chunks of pairs
     float sl2;                  // scale x log2(e)
     void* out;
-    float* part;                // [S][Hkv][most G][ns] x (D + 4): O, m, l, -, -
+    float* part;                // [nw][2][most G] x (D + 4): O, m, l, -, - of a run that begins inside a unit; of one that ends in it
+    int2* units;                // [S][Hkv]: the first and the last work-group with tokens of a unit
     float* scores;              // [S][Hkv][most G][pad]: scores in log2 units, or null
     float* stats;               // [S][Hkv][most G][2]: a pair's largest score and its sum, or null
     int64_t pad;
@@ -55,97 +57,90 @@ __device__ __forceinline__ void span_of(const AttendParams& p, const Kv8Seq& q, 
     lo = p.win > 0 ? std::max<int64_t>(0, (int64_t) q.len + 1 - p.win) : 0;
 }
 
-// QT: the rows' type; RT row tiles of 16 pairs a wave
-template <int D, int RT, int FORM, int QT>
-__global__ __launch_bounds__(WAVES * 64, D == 128 ? 2 : 1) void kv8_attend_kernel(const AttendParams p) {
-    constexpr bool QS = QT == 0;                                  // rows in two parts
+// a sequence's chunks a key head: chunk `first` and on (a sequence with rows has one at least)
+__device__ __forceinline__ int chunks_of(const AttendParams& p, const Kv8Seq& q, int& first) {
+    int64_t lo, hi;
+    span_of(p, q, lo, hi);
+    first = (int) (lo / CHUNK);
+    return q.n <= 0 ? 0 : std::max(1, (int) ((hi + CHUNK - 1) / CHUNK) - first);
+}
+
+// QT: the rows' type; RT row tiles of 16 pairs a wave; ACC: the scores are kept
+template <int D, int RT, int FORM, int QT, bool ACC>
+__global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_attend_kernel(const AttendParams p) {
+    constexpr bool QS = QT == 0;                                  // rows and weights in two parts
     constexpr int CH = D / 16, KJ = D / 64, DT = D / 16;          // 16-byte chunks a row; chunks a lane reads of a key; tiles of 16 features
     constexpr int TB = TILE * D, NI = TB / 1024;                  // bytes a tile and stream; transfers
-    constexpr int STAGE = 4 * TB;                                 // two buffers of keys and values
     constexpr int OROW = D + 4, MERGE = RT * 16 * OROW * 4;
-    constexpr int WREG = ((STAGE > MERGE ? STAGE : MERGE) + 1023) / 1024 * 1024;
+    constexpr int WREG = ((2 * TB > MERGE ? 2 * TB : MERGE) + 1023) / 1024 * 1024;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * WREG];
     __shared__ __attribute__((aligned(16))) float ml[RT * 16][2][WAVES];
+    __shared__ int64_t sums[WAVES + 1], found[2];
 
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g4 = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // consecutive work-groups go round the 8 XCDs; the chunks of one (split, key head, sequence) follow each other on one of them
-    const int xj = blockIdx.x / 8, u = (xj / p.nz) * 8 + (int) (blockIdx.x % 8), z = xj % p.nz;
+    // consecutive work-groups go round the 8 XCDs; a run's chunks of pairs follow each other on one of them (the grid is then a multiple of 8)
+    int wg = blockIdx.x, z = 0;
+    if (p.nz > 1) {
+        const int xj = blockIdx.x / 8;
+        wg = (xj / p.nz) * 8 + (int) (blockIdx.x % 8), z = xj % p.nz;
+        if (wg >= p.nw) return;
+    }
     const int Hkv = p.c.Hkv;
-    if (u >= p.ns * Hkv * p.S) return;
-    const int split = u % p.ns, hk = u / p.ns % Hkv, s = u / (p.ns * Hkv);
-    const Kv8Seq q = seq_of(p, s);
-    const int pairs = q.n * p.G, pair0 = z * RT * 16;
-    if (q.n <= 0 || pair0 >= pairs) return;
-    int64_t lo, hi;
-    span_of(p, q, lo, hi);
-    const int64_t j0 = split * p.kbs, jb = std::max(j0, lo), je = std::min(j0 + p.kbs, hi);
-    if (jb >= je && p.ns > 1) return;                             // (the merge passes this split over, by the same rule)
-
-    // ---- the split's blocks and scales: entry e0 + lane, e0 + 64 + lane
-    const int64_t e0 = j0 >> p.c.shift;
-    int blk[2];
-    float sk[2], sv[2];
+    // ---- this work-group's run of chunks: `left` of them from chunk `at` of (sequence s, key head hk) on
+    int s = 0, left;
+    int64_t rest, run;                                            // chunks of a run; of sequence s (its heads one behind the other) in front of this one
+    {
+        int first;
+        int64_t total;
+        if (p.S == 1) {
+            total = chunks_of(p, seq_of(p, 0), first);
+        } else {
+            const int per = (p.S + WAVES * 64 - 1) / (WAVES * 64), s0 = std::min(tid * per, p.S), s1 = std::min(s0 + per, p.S);
+            int64_t mine = 0;
+            for (int i = s0; i < s1; ++i) mine += chunks_of(p, seq_of(p, i), first);
+            int64_t x = mine;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t e = e0 + i * 64 + lane;
-        blk[i] = (e << p.c.shift) < je ? kv8_block(p.c, p.c.table, s, e) : -1;
-    }
-    // ---- this lane's rows: position, first and last token seen, operands
-    s8v qh[RT][2 * KJ], ql[QS ? RT : 1][2 * KJ];
-    float qm[RT];                                                 // what a score takes besides the block's scale
-    int64_t rlo[RT], rhi[RT];                                     // tokens seen: rlo .. rhi
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int pair = pair0 + rt * 16 + n;
-        const bool live = pair < pairs;
-        const int i = live ? pair / p.G : 0, g = live ? pair - i * p.G : 0;
-        const int64_t pos = (int64_t) q.len + i;
-        rlo[rt] = live ? (p.win > 0 ? std::max<int64_t>(0, pos + 1 - p.win) : 0) : 1;
-        rhi[rt] = live ? std::min(pos, hi - 1) : 0;
-        const int64_t at = (int64_t) (q.first + i) * p.qs + (int64_t) (hk * p.G + g) * D;
-        float x[2 * KJ][8], most = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 2 * KJ; ++j) {
-            const int64_t d = at + 64 * (j / 2) + 16 * g4 + 8 * (j % 2);
-            if constexpr (QT == 0) {
-                float a[4], b[4];
-                load_row<0, 4>(p.q, d, a), load_row<0, 4>(p.q, d + 4, b);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[j][k] = a[k], x[j][4 + k] = b[k];
-            } else load_row<QT, 8>(p.q, d, x[j]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[j][k]));
-        }
-        most = rows_max(most);
-        const int e = std::min(std::max((int) (__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 13, -110), 110);
-        const float up = kv8_pow2(-e);
-        qm[rt] = p.sl2 * kv8_pow2(e);
-#pragma unroll
-        for (int j = 0; j < 2 * KJ; ++j)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float v = x[j][k] * up;
-                qh[rt][j][k] = to16<false>(v);
-                if constexpr (QS) ql[rt][j][k] = to16<false>(v - f16_to_f32((uint16_t) qh[rt][j][k]));
+            for (int d = 1; d < 64; d <<= 1) {
+                const int64_t y = __shfl_up(x, d);
+                if (lane >= d) x += y;
             }
-    }
+            if (lane == 63) sums[w] = x;
+            __syncthreads();
+            int64_t before = x - mine;
+            total = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t at = (int64_t) std::max(blk[i], 0) * Hkv + hk;
-        sk[i] = p.c.ksc[at], sv[i] = p.c.vsc[at];
-        if (blk[i] < 0) sk[i] = 0.0f, sv[i] = 0.0f;
+            for (int i = 0; i < WAVES; ++i) {
+                const int64_t y = sums[i];
+                if (i < w) before += y;
+                total += y;
+            }
+            run = (total * Hkv + p.nw - 1) / p.nw;
+            const int64_t from = wg * run;
+            if (before * Hkv <= from && from < (before + mine) * Hkv) {
+                int64_t b = before;
+                for (int i = s0; i < s1; ++i) {
+                    const int64_t y = chunks_of(p, seq_of(p, i), first);
+                    if (from < (b + y) * Hkv) {
+                        found[0] = i, found[1] = from - b * Hkv;
+                        break;
+                    }
+                    b += y;
+                }
+            }
+            __syncthreads();
+        }
+        run = (total * Hkv + p.nw - 1) / p.nw;
+        const int64_t from = wg * run;
+        if (from >= total * Hkv) return;
+        left = (int) std::min(run, total * Hkv - from);
+        rest = from;
+        if (p.S > 1) s = __builtin_amdgcn_readfirstlane((int) found[0]), rest = found[1];
     }
-    auto pick = [&](auto (&v)[2], int e) __attribute__((always_inline)) {
-        const int x = __builtin_amdgcn_readlane(__builtin_bit_cast(int, v[0]), e & 63), y = __builtin_amdgcn_readlane(__builtin_bit_cast(int, v[1]), e & 63);
-        return e < 64 ? x : y;
-    };
-    auto picked = [&](float (&v)[2], int e) __attribute__((always_inline)) { return __builtin_bit_cast(float, pick(v, e)); };
-
-    // ---- transfers: chunk position cp of token kk holds the row's chunk cp ^ kk % CH (keys: 16 tokens' same chunk meet no bank
-    // conflict), cp ^ (4 (kk / 16) + kk % 4) (values: the 8 rows of a group's transposing read). A transfer is 1024 / D rows; 16 tokens lie in one block
     uint8_t* stage = lds + w * WREG;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (__attribute__((address_space(3))) uint8_t*) stage);
+    // ---- transfers: chunk position cp of token kk holds the row's chunk cp ^ kk % CH (keys: 16 tokens' same chunk meet no bank
+    // conflict), cp ^ (4 (kk / 16) + kk % 4) (values: the 8 rows of a group's transposing read). A transfer is 1024 / D rows; 16 tokens lie in one block
     uint32_t koff[NI], voff[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -153,217 +148,337 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 ? 2 : 1) void kv8_attend_kerne
         koff[i] = (uint32_t) (r * D + (cp ^ (kk % CH)) * 16);
         voff[i] = (uint32_t) (r * D + (cp ^ (4 * (kk / 16) + kk % 4)) * 16);
     }
-    const int nt = (int) ((je - j0 + TILE - 1) / TILE), t0 = (int) ((jb - j0) / TILE);
-    auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = t * TILE + h * 16, b = std::max(pick(blk, at >> p.c.shift), 0);
-            const int64_t off = (kv8_rows(p.c, b, hk) + (at & (p.c.block - 1))) * D;
-            lds_fetch_run<true, NI / 2>(p.c.kc + off, koff + h * (NI / 2), lds0 + buf * 2 * TB + h * (TB / 2));
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = t * TILE + h * 16, b = std::max(pick(blk, at >> p.c.shift), 0);
-            const int64_t off = (kv8_rows(p.c, b, hk) + (at & (p.c.block - 1))) * D;
-            lds_fetch_run<true, NI / 2>(p.c.vc + off, voff + h * (NI / 2), lds0 + buf * 2 * TB + TB + h * (TB / 2));
-        }
-    };
 
-    float m[RT], l[RT];
-    f4v o[RT][DT];
+    for (;;) {
+        // ---- a piece of the run: chunks c0 .. c1 - 1 of one unit
+        const Kv8Seq q = seq_of(p, s);
+        int64_t lo, hi;
+        span_of(p, q, lo, hi);
+        int first;
+        const int nch = chunks_of(p, q, first);
+        const int hk = (int) (rest / nch), c0 = (int) (rest - (int64_t) hk * nch), c1 = std::min(nch, c0 + left);
+        const int pairs = q.n * p.G, pair0 = z * RT * 16;
+        if (pair0 < pairs) {
+            // from here on tokens are counted from the piece's first
+            const int64_t j0 = (int64_t) (first + c0) * CHUNK;
+            const int jb = (int) (std::max(j0, lo) - j0), je = (int) (std::min(j0 + (int64_t) (c1 - c0) * CHUNK, hi) - j0), pos0 = (int) std::max<int64_t>(q.len - j0, -(1 << 30));
+            int blk[2];                                           // entries from the span's first on: lane, 64 + lane; none: -1
+            float sk[2], sv[2];
+            auto entries = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -INFINITY, l[rt] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    // tiles that need no mask: every token seen by every row there is
-    const int64_t full_hi = std::min<int64_t>((int64_t) q.len + pair0 / p.G + 1, hi);
-    const int64_t full_lo = p.win > 0 ? std::max<int64_t>(0, (int64_t) q.len + q.n - p.win) : 0;
-
-    int t = t0 + ((w - t0) & (WAVES - 1)), buf = 0;
-    if (t < nt) fetch(t, 0);
-    if (t + WAVES < nt) fetch(t + WAVES, 1);
-    // (the scales are there before the loop: in it the compiler would wait for them, and the tiles behind them, every turn)
-    asm volatile("" : "+v"(sk[0]), "+v"(sk[1]), "+v"(sv[0]), "+v"(sv[1]));
-    for (; t < nt; t += WAVES, buf ^= 1) {
-        if (t + WAVES < nt) {
-            if constexpr (NI == 4) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-            else asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-        } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const uint8_t* kl = stage + buf * 2 * TB;
-        uint8_t* vl = stage + buf * 2 * TB + TB;
-        const int64_t key0 = j0 + t * TILE;
-        const int ent0 = (t * TILE) >> p.c.shift, ent1 = (t * TILE + 16) >> p.c.shift;
-        const bool bad0 = pick(blk, ent0) < 0, bad1 = pick(blk, ent1) < 0;
-        const bool edge = key0 + TILE > full_hi || key0 < full_lo || bad0 || bad1;
-
-        f4v sc[RT][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                const int kk = h * 16 + n, c = 4 * j + g4;
-                const uint4 r = *reinterpret_cast<const uint4*>(kl + kk * D + ((c ^ (kk % CH)) << 4));
-                const s8v a = kv8_halfs8<FORM>(r.x, r.y), b = kv8_halfs8<FORM>(r.z, r.w);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    f4v x = j == 0 ? f4v{0.0f, 0.0f, 0.0f, 0.0f} : sc[rt][h];
-                    x = mfma16<false>(a, qh[rt][2 * j], x);
-                    x = mfma16<false>(b, qh[rt][2 * j + 1], x);
-                    if constexpr (QS) {
-                        x = mfma16<false>(a, ql[rt][2 * j], x);
-                        x = mfma16<false>(b, ql[rt][2 * j + 1], x);
-                    }
-                    sc[rt][h] = x;
+                for (int i = 0; i < 2; ++i) {
+                    const int e = i * 64 + lane;
+                    blk[i] = at + (e << p.c.shift) < je ? kv8_block(p.c, p.c.table, s, ((j0 + at) >> p.c.shift) + e) : -1;
                 }
-            }
-        }
-        const float k0 = picked(sk, ent0), k1 = picked(sk, ent1);
-        s8v ph[RT], pl[RT];
+            };
+            auto scales = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float x[8];
-            const float f0 = qm[rt] * k0, f1 = qm[rt] * k1;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = sc[rt][0][i] * f0, x[4 + i] = sc[rt][1][i] * f1;
-            if (edge) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int64_t key = key0 + (i / 4) * 16 + 4 * g4 + i % 4;
-                    if (i < 4 ? bad0 : bad1) x[i] = 0.0f;         // (no block: a key of zeros)
-                    x[i] = key >= rlo[rt] && key <= rhi[rt] ? x[i] : -INFINITY;
+                for (int i = 0; i < 2; ++i) {
+                    const int64_t at = (int64_t) std::max(blk[i], 0) * Hkv + hk;
+                    sk[i] = p.c.ksc[at], sv[i] = p.c.vsc[at];
+                    if (blk[i] < 0) sk[i] = 0.0f, sv[i] = 0.0f;
                 }
-            }
-            if (p.scores) {
+            };
+            auto pick = [&](auto (&v)[2], int e) __attribute__((always_inline)) {
+                const int x = __builtin_amdgcn_readlane(__builtin_bit_cast(int, v[0]), e & 63), y = __builtin_amdgcn_readlane(__builtin_bit_cast(int, v[1]), e & 63);
+                return e < 64 ? x : y;
+            };
+            auto picked = [&](float (&v)[2], int e) __attribute__((always_inline)) { return __builtin_bit_cast(float, pick(v, e)); };
+            auto place_of = [&](int at) __attribute__((always_inline)) {
+                const int b = std::max(pick(blk, at >> p.c.shift), 0);
+                return (kv8_rows(p.c, b, hk) + (at & (p.c.block - 1))) * D;
+            };
+            // (at: from the span's first token on)
+            auto fetch_keys = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (p.nz == 1) lds_fetch_run<true, NI / 2>(p.c.kc + place_of(at + h * 16), koff + h * (NI / 2), lds0 + h * (TB / 2));
+                    else lds_fetch_run<false, NI / 2>(p.c.kc + place_of(at + h * 16), koff + h * (NI / 2), lds0 + h * (TB / 2));
+                }
+            };
+            auto fetch_values = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (p.nz == 1) lds_fetch_run<true, NI / 2>(p.c.vc + place_of(at + h * 16), voff + h * (NI / 2), lds0 + TB + h * (TB / 2));
+                    else lds_fetch_run<false, NI / 2>(p.c.vc + place_of(at + h * 16), voff + h * (NI / 2), lds0 + TB + h * (TB / 2));
+                }
+            };
+            const int span = 128 << p.c.shift;                    // tokens of the entries held
+            const int t0 = jb / TILE;
+            entries(0);
+
+            // ---- this lane's rows: first and last token seen, operands
+            s8v qh[RT][2 * KJ], ql[QS ? RT : 1][2 * KJ];
+            float qm[RT];                                         // what a score takes besides the block's scale
+            int rlo[RT], rhi[RT];                                 // tokens seen: rlo .. rhi
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
                 const int pair = pair0 + rt * 16 + n;
-                if (pair < pairs) {
-                    float* at = p.scores + (((int64_t) s * Hkv + hk) * p.most * p.G + pair) * p.pad + key0 + 4 * g4;
-                    *reinterpret_cast<f4v*>(at) = f4v{x[0], x[1], x[2], x[3]};
-                    *reinterpret_cast<f4v*>(at + 16) = f4v{x[4], x[5], x[6], x[7]};
+                const bool live = pair < pairs;
+                const int i = live ? pair / p.G : 0, g = live ? pair - i * p.G : 0;
+                rhi[rt] = live ? std::min(pos0 + i, je - 1) : -1;
+                rlo[rt] = p.win > 0 ? (int) std::max<int64_t>(jb, pos0 + i + 1 - p.win) : jb;
+                const int64_t at = (int64_t) (q.first + i) * p.qs + (int64_t) (hk * p.G + g) * D;
+                float x[2 * KJ][8], most = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 2 * KJ; ++j) {
+                    const int64_t d = at + 64 * (j / 2) + 16 * g4 + 8 * (j % 2);
+                    if constexpr (QT == 0) {
+                        float a[4], b[4];
+                        load_row<0, 4>(p.q, d, a), load_row<0, 4>(p.q, d + 4, b);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[j][k] = a[k], x[j][4 + k] = b[k];
+                    } else load_row<QT, 8>(p.q, d, x[j]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[j][k]));
                 }
-            }
-            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            top = rows_max(top);
-            if (__builtin_amdgcn_ballot_w64(top > m[rt])) {       // some row's largest score moves
-                const float m1 = fmaxf(m[rt], top), c = m1 == -INFINITY ? 1.0f : fast_exp2(m[rt] - m1);
-                m[rt] = m1;
-                l[rt] *= c;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= c;
-            }
-            const float ref = m[rt] == -INFINITY ? 0.0f : m[rt];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float e = fast_exp2(x[i] - ref);
-                l[rt] += e;
-                ph[rt][i] = to16<false>(e);
-                pl[rt][i] = to16<false>(e - f16_to_f32((uint16_t) ph[rt][i]));
-            }
-        }
-        const float v0 = picked(sv, ent0), v1 = picked(sv, ent1);
-        // which of the 8 tokens of a lane's operand there are (bytes of others may hold anything)
-        uint32_t live0 = ~0u, live1 = ~0u;
-        if (edge) {
-            live0 = live1 = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t a = key0 + 4 * g4 + i, b = a + 16;
-                live0 |= !bad0 && a >= lo && a < hi ? 0xFFu << (8 * i) : 0u;
-                live1 |= !bad1 && b >= lo && b < hi ? 0xFFu << (8 * i) : 0u;
-            }
-        }
-        {
-            // lane n of group g4 addresses token row n / 2 of the group's 8, half n % 2 of the chunk
-            const int r = n >> 1, kk = (r >> 2) * 16 + 4 * g4 + (r & 3), x = 4 * (kk / 16) + kk % 4;
-            uint8_t* at = vl + kk * D + (n & 1) * 8;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                typedef int v2i __attribute__((ext_vector_type(2)));
-                const v2i raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*) (at + ((dt ^ x) << 4)));
-                const s8v a = kv8_halfs8<FORM>((uint32_t) raw[0] & live0, (uint32_t) raw[1] & live1, v0, v1);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    o[rt][dt] = mfma16<false>(a, ph[rt], o[rt][dt]);
-                    o[rt][dt] = mfma16<false>(a, pl[rt], o[rt][dt]);
+                if (rt == 0) {
+                    // (the rows are asked for; behind them the scales and the first tile)
+                    scales();
+                    if (const int t = t0 + ((w - t0) & (WAVES - 1)); t * TILE < std::min(je, span)) fetch_keys(t * TILE), fetch_values(t * TILE);
                 }
+                most = rows_max(most);
+                const int e = most > 0.0f ? std::min(std::max((int) (__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 13, -110), 110) : 0;
+                const float up = kv8_pow2(-e);
+                qm[rt] = p.sl2 * kv8_pow2(e);
+#pragma unroll
+                for (int j = 0; j < 2 * KJ; ++j)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float v = x[j][k] * up;
+                        qh[rt][j][k] = to16<false>(v);
+                        if constexpr (QS) ql[rt][j][k] = to16<false>(v - f16_to_f32((uint16_t) qh[rt][j][k]));
+                    }
             }
-        }
-        // this buffer's reads have returned: the tile after the next may have it
-        if (t + 2 * WAVES < nt) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            fetch(t + 2 * WAVES, buf);
-        }
-    }
 
-    // ---- the waves' sums, each parked in the wave's own region
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    float* own = reinterpret_cast<float*>(stage);
+            // m: what a row's weights are taken against - moved where a score is past it by more than 2^8 -, l: this lane's part of their sum
+            float m[RT], l[RT];
+            f4v o[RT][DT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const float sum = rows_sum(l[rt]);
+            for (int rt = 0; rt < RT; ++rt) {
+                m[rt] = -INFINITY, l[rt] = 0.0f;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4v*>(own + (rt * 16 + n) * OROW + dt * 16 + 4 * g4) = o[rt][dt];
-        if (g4 == 0) ml[rt * 16 + n][0][w] = m[rt], ml[rt * 16 + n][1][w] = sum;
-    }
-    __syncthreads();
-    for (int i = tid; i < RT * 16 * (D / 4); i += WAVES * 64) {
-        const int row = i / (D / 4), d = i % (D / 4) * 4, pair = pair0 + row;
-        if (pair >= pairs) break;
-        float top = -INFINITY;
+                for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            // tiles that need no mask: every token seen by every row there is
+            const int full_hi = std::min(pos0 + pair0 / p.G + 1, je);
+            const int full_lo = p.win > 0 ? (int) std::max<int64_t>(jb, pos0 + q.n - p.win) : jb;
+
+            for (int sp = 0; sp < je; sp += span) {
+                const int t1 = (std::min(je, sp + span) + TILE - 1) / TILE;
+                int t = std::max(t0, sp / TILE);
+                t += (w - t) & (WAVES - 1);
+                if (sp > 0) {
+                    entries(sp), scales();
+                    if (t < t1) fetch_keys(t * TILE - sp), fetch_values(t * TILE - sp);
+                }
+                // (the scales are there before the loop: in it the compiler would wait for them, and what is under way behind them, every turn)
+                asm volatile("" : "+v"(sk[0]), "+v"(sk[1]), "+v"(sv[0]), "+v"(sv[1]));
+                for (; t < t1; t += WAVES) {
+                    const bool more = t + WAVES < t1;
+                    const int key0 = t * TILE, at0 = key0 - sp, next = at0 + CHUNK;
+                    // (the keys are there, the values behind them still under way)
+                    if constexpr (NI == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+                    else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+                    uint4 raw[2][KJ];
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) top = fmaxf(top, ml[row][0][k]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        f4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        float all = 0.0f;
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) {
-            const float c = fast_exp2(ml[row][0][k] - ref);
-            all += ml[row][1][k] * c;
-            sum += *reinterpret_cast<const f4v*>(reinterpret_cast<const float*>(lds + k * WREG) + row * OROW + d) * c;
+                        for (int j = 0; j < KJ; ++j) {
+                            const int kk = h * 16 + n, c = 4 * j + g4;
+                            raw[h][j] = *reinterpret_cast<const uint4*>(stage + kk * D + ((c ^ (kk % CH)) << 4));
+                        }
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if (more) fetch_keys(next);
+                    const int ent0 = at0 >> p.c.shift, ent1 = (at0 + 16) >> p.c.shift;
+                    const bool bad0 = pick(blk, ent0) < 0, bad1 = pick(blk, ent1) < 0;
+                    const bool edge = key0 + TILE > full_hi || key0 < full_lo || bad0 || bad1;
+
+                    f4v sc[RT][2];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) sc[rt][0] = sc[rt][1] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 0; j < KJ; ++j)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const s8v a = kv8_halfs8<FORM>(raw[h][j].x, raw[h][j].y), b = kv8_halfs8<FORM>(raw[h][j].z, raw[h][j].w);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) {
+                                sc[rt][h] = mfma16<false>(a, qh[rt][2 * j], sc[rt][h]);
+                                sc[rt][h] = mfma16<false>(b, qh[rt][2 * j + 1], sc[rt][h]);
+                                if constexpr (QS) {
+                                    sc[rt][h] = mfma16<false>(a, ql[rt][2 * j], sc[rt][h]);
+                                    sc[rt][h] = mfma16<false>(b, ql[rt][2 * j + 1], sc[rt][h]);
+                                }
+                            }
+                        }
+                    const float k0 = picked(sk, ent0), k1 = picked(sk, ent1);
+                    s8v ph[RT], pl[QS ? RT : 1];
+                    float kept[ACC ? RT : 1][8];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        float x[8];
+                        const float f0 = qm[rt] * k0, f1 = qm[rt] * k1;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[i] = sc[rt][0][i] * f0, x[4 + i] = sc[rt][1][i] * f1;
+                        if (edge) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int key = key0 + (i / 4) * 16 + 4 * g4 + i % 4;
+                                if (i < 4 ? bad0 : bad1) x[i] = 0.0f;      // (no block: a key of zeros)
+                                x[i] = key >= rlo[rt] && key <= rhi[rt] ? x[i] : -INFINITY;
+                            }
+                        }
+                        if constexpr (ACC)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) kept[rt][i] = x[i];
+                        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                        if (__builtin_amdgcn_ballot_w64(top > m[rt] + 8.0f)) {
+                            const float m1 = fmaxf(m[rt], rows_max(top)), c = m1 == -INFINITY ? 1.0f : fast_exp2(m[rt] - m1);
+                            m[rt] = m1;
+                            l[rt] *= c;
+#pragma unroll
+                            for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= c;
+                        }
+                        const float ref = m[rt] == -INFINITY ? 0.0f : m[rt];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float e = fast_exp2(x[i] - ref);
+                            l[rt] += e;
+                            ph[rt][i] = to16<false>(e);
+                            if constexpr (QS) pl[rt][i] = to16<false>(e - f16_to_f32((uint16_t) ph[rt][i]));
+                        }
+                    }
+                    const float v0 = picked(sv, ent0), v1 = picked(sv, ent1);
+                    if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    else if constexpr (NI == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+                    else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+                    typedef int v2i __attribute__((ext_vector_type(2)));
+                    v2i val[DT];
+                    {
+                        // lane n of group g4 addresses token row n / 2 of the group's 8, half n % 2 of the chunk
+                        const int r = n >> 1, kk = (r >> 2) * 16 + 4 * g4 + (r & 3), x = 4 * (kk / 16) + kk % 4;
+                        uint8_t* at = stage + TB + kk * D + (n & 1) * 8;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) val[dt] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*) (at + ((dt ^ x) << 4)));
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if constexpr (ACC) {
+                        // (in front of the values' transfers: the wait for the keys ahead of them then counts these too, and no more)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            if (const int pair = pair0 + rt * 16 + n; pair < pairs) {
+                                float* at = p.scores + (((int64_t) s * Hkv + hk) * p.most * p.G + pair) * p.pad + j0 + key0 + 4 * g4;
+                                *reinterpret_cast<f4v*>(at) = f4v{kept[rt][0], kept[rt][1], kept[rt][2], kept[rt][3]};
+                                *reinterpret_cast<f4v*>(at + 16) = f4v{kept[rt][4], kept[rt][5], kept[rt][6], kept[rt][7]};
+                            }
+                    }
+                    if (more) fetch_values(next);
+                    if (edge) {
+                        // (bytes of tokens that there are not may hold anything)
+                        uint32_t live0 = 0, live1 = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int a = key0 + 4 * g4 + i, b = a + 16;
+                            live0 |= !bad0 && a >= jb && a < je ? 0xFFu << (8 * i) : 0u;
+                            live1 |= !bad1 && b >= jb && b < je ? 0xFFu << (8 * i) : 0u;
+                        }
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) val[dt][0] &= (int) live0, val[dt][1] &= (int) live1;
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const s8v a = kv8_halfs8<FORM>((uint32_t) val[dt][0], (uint32_t) val[dt][1], v0, v1);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+                            o[rt][dt] = mfma16<false>(a, ph[rt], o[rt][dt]);
+                            if constexpr (QS) o[rt][dt] = mfma16<false>(a, pl[rt], o[rt][dt]);
+                        }
+                    }
+                }
+            }
+
+            // ---- the waves' sums, each parked in the wave's own region
+            float* own = reinterpret_cast<float*>(stage);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float sum = rows_sum(l[rt]);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4v*>(own + (rt * 16 + n) * OROW + dt * 16 + 4 * g4) = o[rt][dt];
+                if (g4 == 0) ml[rt * 16 + n][0][w] = m[rt], ml[rt * 16 + n][1][w] = sum;
+            }
+            __syncthreads();
+            const bool whole = c0 == 0 && c1 == nch;
+            const int64_t unit = (int64_t) s * Hkv + hk;
+            float* part = p.part + ((int64_t) wg * 2 + (c0 == 0)) * p.most * p.G * (D + 4);
+            for (int i = tid; i < RT * 16 * (D / 4); i += WAVES * 64) {
+                const int row = i / (D / 4), d = i % (D / 4) * 4, pair = pair0 + row;
+                if (pair >= pairs) break;
+                float top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < WAVES; ++k) top = fmaxf(top, ml[row][0][k]);
+                const float ref = top == -INFINITY ? 0.0f : top;
+                f4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
+                float all = 0.0f;
+#pragma unroll
+                for (int k = 0; k < WAVES; ++k) {
+                    const float c = fast_exp2(ml[row][0][k] - ref);
+                    all += ml[row][1][k] * c;
+                    sum += *reinterpret_cast<const f4v*>(reinterpret_cast<const float*>(lds + k * WREG) + row * OROW + d) * c;
+                }
+                if (whole) {
+                    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+                    const int i2 = pair / p.G, g = pair - i2 * p.G;
+                    const float v[4] = {sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
+                    const int64_t at = ((int64_t) (q.first + i2) * p.Hq + hk * p.G + g) * D + d;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) store_o<QT>(p.out, at + k, v[k]);
+                    if (p.stats && d == 0) p.stats[2 * (unit * p.most * p.G + pair)] = ref, p.stats[2 * (unit * p.most * p.G + pair) + 1] = inv;
+                } else {
+                    float* to = part + (int64_t) pair * (D + 4);
+                    *reinterpret_cast<f4v*>(to + d) = sum;
+                    if (d == 0) to[D] = top, to[D + 1] = all;
+                }
+            }
+            if (z == 0 && c0 == 0 && tid == 0 && p.units) p.units[unit] = int2{wg, whole ? wg : wg + (int) ((nch - left + run - 1) / run)};
         }
-        const int64_t place = ((int64_t) s * Hkv + hk) * p.most * p.G + pair;
-        if (p.ns == 1) {
-            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-            const int i2 = pair / p.G, g = pair - i2 * p.G;
-            const float v[4] = {sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
-            const int64_t at = ((int64_t) (q.first + i2) * p.Hq + hk * p.G + g) * D + d;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) store_o<QT>(p.out, at + k, v[k]);
-            if (p.stats && d == 0) p.stats[2 * place] = ref, p.stats[2 * place + 1] = inv;
-        } else {
-            float* to = p.part + (place * p.ns + split) * (D + 4);
-            *reinterpret_cast<f4v*>(to + d) = sum;
-            if (d == 0) to[D] = top, to[D + 1] = all;
+        left -= c1 - c0;
+        if (left <= 0) break;
+        rest += c1 - c0;
+        if (rest >= (int64_t) nch * Hkv) {
+            rest = 0;
+            do ++s;
+            while (s < p.S - 1 && seq_of(p, s).n <= 0);
         }
+        __syncthreads();                                          // (the regions are read: the next piece's transfers may begin)
     }
 }
 
-// out = sum over the splits of O 2^(m - M) / sum of l 2^(m - M): a work-group a (sequence, key head, pair), its lanes a split each for the
-// weights, then D / 4 threads x 256 / (D / 4) splits at a time in a fixed shape
+// out = sum over a unit's pieces of O 2^(m - M) / sum of l 2^(m - M): a work-group a (sequence, key head, pair), D / 4 threads x 256 / (D / 4)
+// pieces at a time in a fixed shape. The first piece lies in its work-group's second place, the others in their first
 template <int D, int QT>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(const AttendParams p) {
     constexpr int L = D / 4, SG = 256 / L;
     __shared__ __attribute__((aligned(16))) float sums[SG][D];
     __shared__ float wsum[SG];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int64_t place = blockIdx.x;
-    const int pair = (int) (place % (p.most * p.G)), hk = (int) (place / (p.most * p.G) % p.c.Hkv), s = (int) (place / ((int64_t) p.most * p.G * p.c.Hkv));
+    const int64_t place = blockIdx.x, unit = place / (p.most * p.G);
+    const int pair = (int) (place - unit * p.most * p.G), s = (int) (unit / p.c.Hkv), hk = (int) (unit - (int64_t) s * p.c.Hkv);
+    const int2 ws = p.units[unit];
     const Kv8Seq q = seq_of(p, s);
-    if (pair >= q.n * p.G) return;
-    int64_t lo, hi;
-    span_of(p, q, lo, hi);
-    const int first = (int) (lo / p.kbs), end = (int) ((hi + p.kbs - 1) / p.kbs);
-    const float* part = p.part + place * p.ns * (D + 4);
+    if (pair >= q.n * p.G || ws.x == ws.y) return;
+    auto piece = [&](int k) { return p.part + (((int64_t) (ws.x + k) * 2 + (k == 0)) * p.most * p.G + pair) * (D + 4); };
+    const int count = ws.y - ws.x + 1;
     float top = -INFINITY;
-    for (int k = first + lane; k < end; k += 64) top = fmaxf(top, part[(int64_t) k * (D + 4) + D]);
+    for (int k = lane; k < count; k += 64) top = fmaxf(top, piece(k)[D]);
     top = wave_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
     const int sg = tid / L, d = tid % L * 4;
     f4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
     float all = 0.0f;
-    for (int k = first + sg; k < end; k += SG) {
-        const float* at = part + (int64_t) k * (D + 4);
+#pragma unroll 4
+    for (int k = sg; k < count; k += SG) {
+        const float* at = piece(k);
         const float c = fast_exp2(at[D] - ref);
         all += at[D + 1] * c;
         sum += *reinterpret_cast<const f4v*>(at + d) * c;
@@ -407,35 +522,40 @@ __global__ __launch_bounds__(256) void kv8_given_kernel(const AttendParams p) {
     p.acc1[at] = (p.acc0 && t < q.len ? p.acc0[at] : 0.0f) + sum;
 }
 
-template <int D, int QT>
-void launch_attend(ns_gpu* g, int form, const AttendParams& p, int RT, unsigned grid) {
-    if (form == 0) RT == 1 ? kv8_attend_kernel<D, 1, 0, QT><<<grid, WAVES * 64, 0, g->q>>>(p) : kv8_attend_kernel<D, 2, 0, QT><<<grid, WAVES * 64, 0, g->q>>>(p);
-    else RT == 1 ? kv8_attend_kernel<D, 1, 1, QT><<<grid, WAVES * 64, 0, g->q>>>(p) : kv8_attend_kernel<D, 2, 1, QT><<<grid, WAVES * 64, 0, g->q>>>(p);
+template <int D, int RT, int QT>
+void launch_attend(ns_gpu* g, int form, const AttendParams& p, dim3 grid) {
+    if (p.acc1) form == 0 ? kv8_attend_kernel<D, RT, 0, QT, true><<<grid, WAVES * 64, 0, g->q>>>(p) : kv8_attend_kernel<D, RT, 1, QT, true><<<grid, WAVES * 64, 0, g->q>>>(p);
+    else form == 0 ? kv8_attend_kernel<D, RT, 0, QT, false><<<grid, WAVES * 64, 0, g->q>>>(p) : kv8_attend_kernel<D, RT, 1, QT, false><<<grid, WAVES * 64, 0, g->q>>>(p);
+}
+template <int QT>
+void launch_attend(ns_gpu* g, int form, const AttendParams& p, int64_t D, int RT, dim3 grid) {
+    if (D == 128) RT == 1 ? launch_attend<128, 1, QT>(g, form, p, grid) : launch_attend<128, 2, QT>(g, form, p, grid);
+    else launch_attend<256, 1, QT>(g, form, p, grid);
 }
 template <int D, int QT>
 void launch_merge(ns_gpu* g, const AttendParams& p, int64_t rows) { kv8_merge_kernel<D, QT><<<(unsigned) rows, 256, 0, g->q>>>(p); }
 
-// tokens a split and how many splits of `longest` there are. Work-groups enough for two a CU, splits of 128 to 2048 tokens
-struct Splits {
-    int64_t kbs, ns;
-};
-Splits splits_of(int64_t S, int64_t nz, int64_t Hkv, int64_t longest) {
-    const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(1, S * Hkv * nz));
-    const int64_t kbs = std::min<int64_t>(MOST_SPLIT, std::max<int64_t>(128, ((longest + want - 1) / want + 127) / 128 * 128));
-    return {kbs, (longest + kbs - 1) / kbs};
+// 16-pair tiles a wave: two where more than 16 pairs share a key head of 128 (heads of 256 have no registers for a second: 16 pairs a work-group,
+// the next ones read the tokens from L2)
+int tiles_of(int64_t pairs, int64_t D) { return pairs > 16 && D == 128 ? 2 : 1; }
+int64_t pair_chunks(int64_t pairs, int64_t D) { const int64_t rows = 16 * tiles_of(pairs, D); return (pairs + rows - 1) / rows; }
+// the work-groups that the tokens are dealt to: as many as the chip holds at once - 3 a CU of one tile over heads of 128, 2 of the others -, no more than
+// there can be chunks. (64 sequences of 125 to 8000 tokens x 8 heads of 128: 256 work-groups 84 us, 512 70, 768 60, 1024 64; 4 rows of each of 3 x 24 / 4 heads of
+// 256, two chunks of pairs: 128 pairs of work-groups 42, 256 37, 384 46)
+int64_t workgroups(int64_t S, int64_t pairs, int64_t Hkv, int64_t D, int64_t longest) {
+    const int64_t places = D == 128 && tiles_of(pairs, D) == 1 ? 768 : 512;
+    return std::min(std::max<int64_t>(1, places / pair_chunks(pairs, D)), S * Hkv * ((longest + CHUNK - 1) / CHUNK + 1));
 }
-int64_t chunks_of(int64_t pairs) { return pairs <= 16 ? 1 : (pairs + 31) / 32; }
 
 struct Scratch {
-    int64_t part, scores, stats, pad;
-    int64_t all() const { return part + scores + stats; }
+    int64_t part, units, scores, stats, pad;
+    int64_t all() const { return part + units + scores + stats; }
 };
-Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest, bool acc) {
-    const Splits sp = splits_of(S, chunks_of(most * (Hq / Hkv)), Hkv, longest);
-    const int64_t rows = S * most * Hq;
+Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest, bool acc, int64_t nw) {
+    const int64_t rows = S * most * Hq, pairs = most * (Hq / Hkv);
     Scratch x{};
     x.pad = (longest + 31) / 32 * 32;
-    x.part = sp.ns > 1 ? rows * sp.ns * (D + 4) : 0;
+    if (longest > CHUNK) x.part = nw * 2 * pairs * (D + 4), x.units = (S * Hkv * 2 + 3) / 4 * 4;
     x.scores = acc ? rows * x.pad : 0;
     x.stats = acc ? rows * 2 : 0;
     return x;
@@ -445,24 +565,29 @@ bool sizes_fit(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int6
            longest <= 2 * (int64_t) KV8_TOKENS;
 }
 
-// a checked call, its scratch at hand
+Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest, bool acc) {
+    return scratch_of(S, most, Hq, Hkv, D, longest, acc, workgroups(S, most * (Hq / Hkv), Hkv, D, longest));
+}
+
+// a checked call, its scratch at hand: scratch_of's floats for p.nw work-groups
 int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, int64_t Hkv, int64_t D, float* scratch) {
-    const int64_t nz = chunks_of((int64_t) p.most * p.G);
-    const Splits sp = splits_of(p.S, nz, Hkv, p.longest);
-    const Scratch x = scratch_of(p.S, p.most, p.Hq, Hkv, D, p.longest, p.acc1 != nullptr);
-    const int64_t units = sp.ns * Hkv * p.S, rows = (int64_t) p.S * p.most * p.Hq;
-    if ((units + 7) / 8 * 8 * nz > (int64_t) 1 << 30 || !ns_grid_fits((units + 7) / 8 * 8 * nz, 256) || !ns_grid_fits(rows, 256))
-        return ns_fail(w + ": more work-groups than a launch takes");
-    p.kbs = sp.kbs, p.ns = (int) sp.ns, p.nz = (int) nz, p.pad = x.pad;
+    const int64_t pairs = (int64_t) p.most * p.G, nz = pair_chunks(pairs, D), rows = (int64_t) p.S * p.most * p.Hq;
+    const Scratch x = scratch_of(p.S, p.most, p.Hq, Hkv, D, p.longest, p.acc1 != nullptr, p.nw);
+    p.nz = (int) nz, p.pad = x.pad;
+    const int64_t grid = nz > 1 ? (int64_t) (p.nw + 7) / 8 * 8 * nz : p.nw;
+    if (!ns_grid_fits(grid, 256) || !ns_grid_fits(rows, 256)) return ns_fail(w + ": more work-groups than a launch takes");
+    // (of sequences that are all within a chunk there are no pieces)
+    const bool pieces = x.units > 0;
     p.part = scratch;
-    p.scores = p.acc1 ? scratch + x.part : nullptr;
-    p.stats = p.acc1 ? scratch + x.part + x.scores : nullptr;
-    const unsigned grid = (unsigned) ((units + 7) / 8 * 8 * nz);
-    const int RT = p.most * p.G <= 16 ? 1 : 2;
-    if (D == 128) qt == 0 ? launch_attend<128, 0>(g, form, p, RT, grid) : qt == 1 ? launch_attend<128, 1>(g, form, p, RT, grid) : launch_attend<128, 2>(g, form, p, RT, grid);
-    else qt == 0 ? launch_attend<256, 0>(g, form, p, RT, grid) : qt == 1 ? launch_attend<256, 1>(g, form, p, RT, grid) : launch_attend<256, 2>(g, form, p, RT, grid);
+    p.units = pieces ? (int2*) (scratch + x.part) : nullptr;
+    p.scores = p.acc1 ? scratch + x.part + x.units : nullptr;
+    p.stats = p.acc1 ? scratch + x.part + x.units + x.scores : nullptr;
+    const int RT = tiles_of(pairs, D);
+    if (qt == 0) launch_attend<0>(g, form, p, D, RT, dim3((unsigned) grid));
+    else if (qt == 1) launch_attend<1>(g, form, p, D, RT, dim3((unsigned) grid));
+    else launch_attend<2>(g, form, p, D, RT, dim3((unsigned) grid));
     NS_LAUNCHED("kv8_attend");
-    if (p.ns > 1) {
+    if (pieces) {
         if (D == 128) qt == 0 ? launch_merge<128, 0>(g, p, rows) : qt == 1 ? launch_merge<128, 1>(g, p, rows) : launch_merge<128, 2>(g, p, rows);
         else qt == 0 ? launch_merge<256, 0>(g, p, rows) : qt == 1 ? launch_merge<256, 1>(g, p, rows) : launch_merge<256, 2>(g, p, rows);
         NS_LAUNCHED("kv8_merge");
@@ -498,6 +623,7 @@ int ns_kv8_attend(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     if (longest <= 0 || longest > 2 * (int64_t) KV8_TOKENS) return ns_fail(w + ": contexts of 1 to 2^31 tokens");
     if (qs < Hq * D) return ns_fail(w + ": rows at least as far apart as they are long");
     p.S = (int) S, p.most = (int) most, p.Hq = (int) Hq, p.G = (int) (Hq / Hkv), p.longest = longest, p.T = (int) T;
+    p.nw = (int) workgroups(S, most * p.G, Hkv, D, longest);
     const int64_t need = scratch_of(S, p.most, Hq, Hkv, D, longest, acc1 != nullptr).all();
     if (!g || !q || !lens || !vc || !vsc || !out || (need && !scratch)) return ns_fail(w + ": a null buffer");
     if (need && (uintptr_t) scratch % 16) return ns_fail(w + ": scratch 16-byte aligned");
@@ -541,7 +667,10 @@ int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     for (int64_t t = 0; t < T; t += DECODE_ROWS) {
         const int64_t rows = std::min(DECODE_ROWS, T - t);
         p.q = (const uint8_t*) q + t * qs * e, p.out = (uint8_t*) out + t * Hq * D * e, p.T = p.most = (int) rows, p.p0 = p0 + t, p.longest = p0 + t + rows;
-        if ((size_t) scratch_of(1, rows, Hq, Hkv, D, p.longest, false).all() > own) return ns_fail(w + ": more rows, heads and tokens than the library's scratch holds");
+        // (as many work-groups as have places for their pieces)
+        const int64_t a_wg = scratch_of(1, rows, Hq, Hkv, D, p.longest, false, 1).part, units = scratch_of(1, rows, Hq, Hkv, D, p.longest, false, 1).units;
+        p.nw = (int) std::min(workgroups(1, rows * p.G, Hkv, D, p.longest), a_wg > 0 ? ((int64_t) own - units) / a_wg : 1 << 30);
+        if (p.nw < 1) return ns_fail(w + ": more rows and heads than the library's scratch holds");
         if (attend(g, w, form, qt, p, Hkv, D, g->own_scratch)) return -1;
     }
     return 0;

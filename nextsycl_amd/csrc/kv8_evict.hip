@@ -1,8 +1,9 @@
 // kv8_evict.hip: a cache of 8-bit values in blocks of tokens shortened to the tokens of the largest accumulated softmax weights (gfx950).
 //
 // Three steps a (sequence, key head). Which tokens: the weights' bits, as whole numbers, are searched from the top 11 bits down for the
-// value at the last kept place (three histograms in LDS); the kept tokens' places follow from one scan over runs of tokens, so they keep their
-// order and of equal weights the earliest stay. Move: a work-group a block to be written, key head and stream - its rows gathered, re-rounded to the largest
+// value at the last kept place (three histograms in LDS; zeros, of which there can be many, are not counted but left over); a work-group holds up to
+// 32768 weights in registers, token 1024 i + thread, so a kept token's place is the waves' counts in front of it - one scan of them - and its lane's
+// place in a ballot: tokens keep their order, and of equal weights the earliest stay. Move: a work-group a block to be written, key head and stream - its rows gathered, re-rounded to the largest
 // of their scales. In place the blocks go through the library's scratch, since a block is read by those in front of it; blocks whose tokens stay
 // where they are are left out. Bound: the kept rows' bytes, read and written; the search by one work-group's latencies.
 #include <algorithm>
@@ -12,7 +13,7 @@
 
 namespace {
 
-constexpr int SEL = 1024, CACHE = 32768;          // threads of the search; tokens whose weights it keeps in LDS
+constexpr int SEL = 1024;                         // threads of the search
 
 struct EvictParams {
     Kv8Cache c;
@@ -29,16 +30,19 @@ struct EvictParams {
     int nb;                     // blocks of cap tokens
 };
 
-// a work-group's exclusive prefix sum of v, and the total
+// the sum over this lane and those in front of it: each row of 16, then the rows' last lanes over the rows behind them
+__device__ __forceinline__ int lanes_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);        // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);       // row_bcast 15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);       // row_bcast 31 into rows 2 and 3
+    return v;
+}
+// a work-group's exclusive prefix sum of v, and the total (a call's last read of `sums` comes before the next one's barrier)
 __device__ __forceinline__ int scan1024(int v, int* sums, int& total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    __syncthreads();
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, x = lanes_scan(v);
     if (lane == 63) sums[w] = x;
     __syncthreads();
     int before = 0;
@@ -52,96 +56,147 @@ __device__ __forceinline__ int scan1024(int v, int* sums, int& total) {
     return before + x - v;
 }
 
-template <bool CACHED>
+// this lane's place among the lanes of m
+__device__ __forceinline__ int lane_place(uint64_t m) { return __builtin_amdgcn_mbcnt_hi((uint32_t) (m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) m, 0)); }
+
+// R weights a thread; longer contexts in pieces of 1024 R, read again for each step. (One CU has the whole of a key head's search: what counts is
+// the instructions a weight. 32768 of them x 8 heads: 15 a step and 64-bit places 35 us)
+template <int R>
 __global__ __launch_bounds__(SEL) void kv8_select_kernel(const EvictParams p) {
-    __shared__ uint32_t keys[CACHED ? CACHE : 1];
+    constexpr int PIECE = SEL * R;
+    constexpr uint32_t NONE = ~0u;                                // (no weight's bits)
     __shared__ int hist[2048];
-    __shared__ int sums[SEL / 64];
-    __shared__ int found[2];
-    const int tid = threadIdx.x, hk = blockIdx.x, gs = blockIdx.y;
+    __shared__ int entries[PIECE / 16];                           // where a piece's blocks begin in acc, in 16 tokens (none: -1)
+    __shared__ int counts[R * (SEL / 64)];
+    __shared__ int sums[2][SEL / 64];                             // (of two calls in turn)
+    __shared__ int found[3];
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), hk = blockIdx.x, gs = blockIdx.y;
     const int64_t s = p.s0 + gs;
     const int n = p.lens[s];
     const bool over = n < 0 || n > p.longest, whole = n <= p.keep;
     const int rows = over || (whole && !p.to) ? 0 : whole ? n : (int) p.keep;
     if (hk == 0 && tid == 0) p.info[gs] = int2{rows, over || whole ? n : (int) p.keep};
-    if (rows == 0 || (CACHED && n > CACHE) || (!CACHED && n <= CACHE)) return;
+    if (rows == 0) return;
     int32_t* idx = p.idx + ((int64_t) gs * p.nh + hk) * p.cap;
     if (whole) {
         for (int t = tid; t < n; t += SEL) idx[t] = t;
         return;
     }
     // the weights of the tokens between those that stay anyhow, as whole numbers in the same order
-    const int lo = (int) p.first, hi = n - (int) p.last;
-    auto weight = [&](int t) -> uint32_t {
-        const int b = kv8_block(p.c, p.c.table, s, t >> p.c.shift);
-        if (b < 0) return 0;
-        const float a = p.acc[kv8_rows(p.c, b, hk) + (t & (p.c.block - 1))];
-        return a > 0.0f ? __builtin_bit_cast(uint32_t, a) : 0;
-    };
-    if constexpr (CACHED) {
-        for (int t = lo + tid; t < hi; t += SEL) keys[t] = weight(t);
+    const int lo = (int) p.first, hi = n - (int) p.last, pieces = (n + PIECE - 1) / PIECE;
+    uint32_t key[R];
+    auto load = [&](int piece) __attribute__((always_inline)) {
+        const int t0 = piece * PIECE, m = std::min(n - t0, PIECE), count = (m + p.c.block - 1) >> p.c.shift;
+        for (int i = tid; i < count; i += SEL) {
+            const int b = kv8_block(p.c, p.c.table, s, (t0 >> p.c.shift) + i);
+            entries[i] = b < 0 ? -1 : (int) (kv8_rows(p.c, b, hk) >> 4);
+        }
         __syncthreads();
-    }
-    auto key = [&](int t) -> uint32_t {
-        if constexpr (CACHED) return keys[t];
-        else return weight(t);
+        float a[R];
+        bool none = false;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int j = std::min(i * SEL + tid, m - 1), e = entries[j >> p.c.shift];
+            none |= e < 0;
+            a[i] = p.acc[((int64_t) std::max(e, 0) << 4) + (j & (p.c.block - 1))];
+        }
+        // (not a number, and below 0: 0)
+#pragma unroll
+        for (int i = 0; i < R; ++i) key[i] = __builtin_bit_cast(uint32_t, fmaxf(a[i], 0.0f)) & 0x7FFFFFFFu;
+        if (__builtin_amdgcn_ballot_w64(none))
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (entries[std::min(i * SEL + tid, m - 1) >> p.c.shift] < 0) key[i] = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if ((uint32_t) (t0 + i * SEL + tid - lo) >= (uint32_t) (hi - lo)) key[i] = NONE;
     };
+    for (int i = tid; i < 2048; i += SEL) hist[i] = 0;
+    load(0);
     // the value at place `need` from the top: 11, 10, 10 bits. `at`: what is known of it
     int need = (int) (p.keep - p.first - p.last);
-    uint32_t at = 0;
-    for (int pass = 0; pass < 3; ++pass) {
+    uint32_t at = need > 0 ? 0 : NONE;                            // (NONE: none of them)
+    for (int pass = 0; pass < 3 && at != NONE; ++pass) {
         const int shift = pass == 0 ? 20 : pass == 1 ? 10 : 0, bins = pass == 0 ? 2048 : 1024;
-        const uint32_t known = pass == 0 ? 0 : ~0u << (shift + 10);
-        for (int i = tid; i < bins; i += SEL) hist[i] = 0;
-        __syncthreads();
-        for (int t = lo + tid; t < hi; t += SEL) {
-            const uint32_t k = key(t);
-            if ((k & known) == at) atomicAdd(&hist[k >> shift & (bins - 1)], 1);
-        }
-        __syncthreads();
-        // bins from the largest down, bins / 1024 a thread
-        const int per = bins / SEL, top = bins - 1 - tid * per;
-        int mine = 0;
-        for (int i = 0; i < per; ++i) mine += hist[top - i];
-        int all;
-        const int before = scan1024(mine, sums, all);
-        if (before < need && before + mine >= need) {
-            int b = before;
-            for (int i = 0; i < per; ++i) {
-                if (b + hist[top - i] >= need) {
-                    found[0] = top - i, found[1] = need - b;
-                    break;
-                }
-                b += hist[top - i];
+        for (int piece = 0; piece < pieces; ++piece) {
+            if (pieces > 1) {
+                __syncthreads();                                  // (the entries are read)
+                load(piece);
             }
+            // (weights from `from` on, `width` of them: in the first pass all but 0)
+            const uint32_t from = pass == 0 ? 1 : at, width = pass == 0 ? 0x7FFFFFFFu : 1u << (shift + 10);
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (key[i] - from < width) atomicAdd(&hist[key[i] >> shift & (bins - 1)], 1);
         }
         __syncthreads();
-        if (need > 0) at |= (uint32_t) found[0] << shift, need = found[1];
-        else at = ~0u;                                            // (none of them)
-        __syncthreads();
-        if (at == ~0u) break;
-    }
-    // `need` of the tokens equal to `at`, the earliest, and all above it. A thread a run of tokens, of odd length: LDS banks
-    const int run = ((n + SEL - 1) / SEL) | 1, t0 = (int) std::min<int64_t>((int64_t) tid * run, n), t1 = std::min<int64_t>((int64_t) t0 + run, n);
-    int same = 0, more = 0;
-    for (int t = t0; t < t1; ++t) {
-        const bool sure = t < lo || t >= hi;
-        const uint32_t k = sure ? 0 : key(t);
-        more += sure || k > at;
-        same += !sure && k == at;
-    }
-    int all;
-    const int same0 = scan1024(same, sums, all), kept = std::min(std::max(need - same0, 0), same);
-    int place = scan1024(more + kept, sums, all), left = kept;
-    for (int t = t0; t < t1; ++t) {
-        const bool sure = t < lo || t >= hi;
-        const uint32_t k = sure ? 0 : key(t);
-        bool keep = sure || k > at;
-        if (!sure && k == at && left > 0) keep = true, --left;
-        if (keep) {
-            if (place < p.cap) idx[place] = t;
-            ++place;
+        // bins from the largest down, bins / 1024 a thread; they are cleared for the next pass
+        const int per = bins / SEL, top = bins - 1 - tid * per;
+        const int h0 = hist[top], h1 = per > 1 ? hist[top - 1] : 0;
+        hist[top] = 0;
+        if (per > 1) hist[top - 1] = 0;
+        int all;
+        const int before = scan1024(h0 + h1, sums[pass & 1], all);
+        if (pass == 0 && all < need) {                            // (all that are above 0, and the first zeros)
+            need -= all;
+            break;
         }
+        if (before < need && before + h0 + h1 >= need) {
+            const bool second = before + h0 < need;
+            found[0] = top - second, found[1] = need - before - (second ? h0 : 0), found[2] = second ? h1 : h0;
+        }
+        __syncthreads();
+        at |= (uint32_t) found[0] << shift, need = found[1];
+        if (need == found[2] && at > 0) {                         // (the whole bin: all that are no less than its least value)
+            --at, need = 0;
+            break;
+        }
+    }
+    // `need` of the tokens equal to `at`, the earliest, and all above it
+    int same0 = 0, kept0 = 0;                                     // in the pieces in front
+    for (int piece = 0; piece < pieces; ++piece) {
+        if (pieces > 1) {
+            __syncthreads();
+            load(piece);
+        }
+        const int t0 = piece * PIECE;
+        // the waves' counts of a mask in front of this one's, in the tokens' order
+        auto before = [&](auto mask, int* sums) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int c = __builtin_popcountll(mask(i));
+                if (tid % 64 == 0) counts[i * (SEL / 64) + w] = c;
+            }
+            __syncthreads();
+            const int mine = tid < R * (SEL / 64) ? counts[tid] : 0;
+            int all;
+            const int x = scan1024(mine, sums, all);
+            if (tid < R * (SEL / 64)) counts[tid] = x;
+            __syncthreads();
+            return all;
+        };
+        if (need > 0) {
+            // the equal ones that stay become larger than `at`, the others smaller
+            auto mask = [&](int i) { return __builtin_amdgcn_ballot_w64(key[i] == at); };
+            const int same = before(mask, sums[0]);
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (const uint64_t m = mask(i); m && key[i] == at) key[i] = same0 + counts[i * (SEL / 64) + w] + lane_place(m) < need ? at + 1 : 0;
+            same0 += same;
+            __syncthreads();
+        }
+        // (the first and the last tokens are NONE, above all; so are those behind the last one, out of range)
+        const uint32_t least = at == NONE ? NONE : at + 1;
+        auto mask = [&](int i) { return __builtin_amdgcn_ballot_w64(key[i] >= least && t0 + i * SEL + tid < n); };
+        const int kept = before(mask, sums[1]);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (key[i] >= least && t0 + i * SEL + tid < n) {
+                const int place = kept0 + counts[i * (SEL / 64) + w] + lane_place(mask(i));
+                if (place < p.cap) idx[place] = t0 + i * SEL + tid;
+            }
+        kept0 += kept;
+        if (pieces > 1) __syncthreads();
     }
 }
 
@@ -235,7 +290,7 @@ extern "C" int ns_kv8_evict(ns_gpu* g, int form, const int32_t* lens, int32_t* l
     p.c = kv8_cache(kc, vc, ksc, vsc, table, tmax, Hkv, D, block, blocks);
     if (ns_kv8_check(w, form, Hkv, D, block, blocks, S, tmax, p.c)) return -1;
     if (keep <= 0 || first < 0 || last < 0 || first > keep || last > keep - first) return ns_fail(w + ": 1 token or more kept, the first and last ones among them");
-    if (longest <= 0 || longest > 2 * (int64_t) KV8_TOKENS - 1) return ns_fail(w + ": contexts of 1 to 2^31 - 1 tokens");
+    if (longest <= 0 || longest > KV8_TOKENS) return ns_fail(w + ": contexts of 1 to 2^30 tokens");
     if (!g || !lens || !lens1 || !vc || !vsc || !acc) return ns_fail(w + ": a null buffer");
     if (to == table) return ns_fail(w + ": fresh blocks, or null for the sequences' own");
     p.lens = lens, p.lens1 = lens1, p.to = to, p.longest = longest, p.first = first, p.last = last, p.acc = acc, p.nh = (int) Hkv;
@@ -262,12 +317,9 @@ extern "C" int ns_kv8_evict(ns_gpu* g, int form, const int32_t* lens, int32_t* l
             p.stage_scale = take(n * places * 2);
             p.stage_acc = take(n * places * block);
         }
-        kv8_select_kernel<true><<<dim3((unsigned) Hkv, (unsigned) n), SEL, 0, g->q>>>(p);
+        if (longest <= 8 * SEL) kv8_select_kernel<8><<<dim3((unsigned) Hkv, (unsigned) n), SEL, 0, g->q>>>(p);
+        else kv8_select_kernel<32><<<dim3((unsigned) Hkv, (unsigned) n), SEL, 0, g->q>>>(p);
         NS_LAUNCHED("kv8_select");
-        if (longest > CACHE) {
-            kv8_select_kernel<false><<<dim3((unsigned) Hkv, (unsigned) n), SEL, 0, g->q>>>(p);
-            NS_LAUNCHED("kv8_select");
-        }
         const dim3 grid((unsigned) p.nb, (unsigned) (2 * Hkv), (unsigned) n);
         if (form == 0) kv8_move_kernel<0><<<grid, 256, 0, g->q>>>(p);
         else kv8_move_kernel<1><<<grid, 256, 0, g->q>>>(p);

@@ -1,11 +1,11 @@
 // kv8_weights.hip: what many rows of one sequence give each cached token of their softmax weights, summed over rows and the query heads that
 // share its key head (gfx950): column sums of softmax(q K^T), of which no row is kept.
 //
-// The weights need their row's largest score and sum first, so the product q K^T is made twice. Bound: the matrix unit and, as
-// much, the exponentials of both passes. Four kernels: rows into halfs (two of them for float32 rows) with a factor a pair (row, head), keys
-// into halfs; a pair's largest score and sum over a split of the tokens (pairs stay in registers, tokens stream past); the splits
-// of a pair together; a token's sum over a split of the pairs (tokens stay in registers, pairs stream past); the sums into acc. The streaming
-// operand comes from L2 into registers a tile ahead, waves of a work-group take tiles in turn and meet once at the end: no barrier in a loop.
+// The weights need their row's largest score and sum first, so the product q K^T is made twice. Bound: the matrix unit for float32 rows (two halfs, two
+// products), else the exponentials beside it. Both passes are one kernel: a wave keeps 64 tokens in registers, codes widened once, and pairs (row,
+// head) stream past it through LDS, 16 KiB of operands at a time, for the work-group's four waves at once: 256 neighbouring tokens. First a pair's largest
+// score and sum over each 64 tokens, then a token's sum over a split of the pairs. Between them small kernels: rows into halfs, in the order in which the lanes
+// of an operand lie, with a factor a pair; a pair's parts together; the splits' sums into acc.
 #include <algorithm>
 #include <cmath>
 
@@ -19,30 +19,33 @@ struct WeightsParams {
     const void* q;
     int64_t qs, p0, n, win;     // the rows' first token; tokens in all
     int T, G, h0, nh;           // key heads h0 .. h0 + nh - 1
-    int64_t pairs;              // T G, i G + g
+    int pairs;                  // T G, i G + g
+    uint32_t ginv;              // 2^32 / G, rounded up
     float sl2;
-    const uint16_t* k;          // [nh][n][D] half
-    uint16_t *qh, *ql;          // [nh][pairs][D] half; the rest of float32 rows
+    uint8_t* q16;               // [nh][tiles of 16 pairs][D / 32 KiB of halfs, as many of float32 rows' rest]: operands
+    int tiles;
     float4* info;               // [nh][pairs]: factor, largest score, 1 / sum
-    float2* part;               // [nh][pairs][ns]: largest score, sum
-    int64_t kbs, prs;           // tokens a split; pairs a split
-    int ns, rs;
+    float2* part;               // [nh][nb][pairs]: largest score, sum over 64 tokens
+    int64_t nb;                 // runs of 64 tokens
+    int prs, rs;                // pairs a split, splits
     float* sums;                // [rs][nh][n], or null: into acc at once
     const float* acc0;
     float* acc1;
 };
 
+// a pair's row (of up to 2^31 / G pairs)
+__device__ __forceinline__ int row_of(const WeightsParams& p, int pair) { return p.G == 1 ? pair : (int) __umulhi((uint32_t) pair, p.ginv); }
 __device__ __forceinline__ int64_t low_of(const WeightsParams& p, int64_t pos) { return p.win > 0 && pos + 1 > p.win ? pos + 1 - p.win : 0; }
 
-// a pair's row brought to exponent 13, as halfs: 16 lanes a pair
+// a pair's row brought to exponent 13, as halfs: 16 lanes a pair. Operand (tile, step 2 j + i), lane 16 g + n: pair n's features 64 j + 16 g + 8 i .. + 7, the
+// order in which a lane has a key's 16-byte chunks. (Pairs past the last: the last again)
 template <int D, int QT>
 __global__ __launch_bounds__(256) void kv8_rows_kernel(const WeightsParams p) {
-    constexpr int E = D / 16;
-    const int64_t pair = (int64_t) blockIdx.x * 16 + threadIdx.x / 16;
+    constexpr int E = D / 16, KB = D / 32, TILE_BYTES = KB * 1024 * (QT == 0 ? 2 : 1);
+    const int pair = (int) blockIdx.x * 16 + threadIdx.x / 16;
     const int h = blockIdx.y, li = threadIdx.x % 16;
-    const int64_t pc = std::min(pair, p.pairs - 1);
-    const int64_t i = pc / p.G, g = pc - i * p.G;
-    const int64_t at = i * p.qs + ((int64_t) (p.h0 + h) * p.G + g) * D + li * E;
+    const int pc = std::min(pair, p.pairs - 1), i = row_of(p, pc), g = pc - i * p.G;
+    const int64_t at = (int64_t) i * p.qs + ((int64_t) (p.h0 + h) * p.G + g) * D + li * E;
     float x[E], most = 0.0f;
 #pragma unroll
     for (int j = 0; j < E; j += 8) {
@@ -57,10 +60,9 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const WeightsParams p) {
         for (int k = 0; k < 8; ++k) x[j + k] = v[k], most = fmaxf(most, fabsf(v[k]));
     }
     most = row16_max(most);
-    const int e = std::min(std::max((int) (__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 13, -110), 110);
+    const int e = most > 0.0f ? std::min(std::max((int) (__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 13, -110), 110) : 0;
     const float up = kv8_pow2(-e);
-    if (pair >= p.pairs) return;
-    const int64_t to = ((int64_t) h * p.pairs + pair) * D + li * E;
+    uint8_t* to = p.q16 + ((int64_t) h * p.tiles + blockIdx.x) * TILE_BYTES;
 #pragma unroll
     for (int j = 0; j < E; j += 8) {
         s8v a, b;
@@ -69,120 +71,14 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const WeightsParams p) {
             a[k] = to16<false>(x[j + k] * up);
             if constexpr (QT == 0) b[k] = to16<false>(x[j + k] * up - f16_to_f32((uint16_t) a[k]));
         }
-        *reinterpret_cast<s8v*>(p.qh + to + j) = a;
-        if constexpr (QT == 0) *reinterpret_cast<s8v*>(p.ql + to + j) = b;
+        const int d = li * E + j, place = ((d / 64 * 2 + d / 8 % 2) * 64 + d / 16 % 4 * 16 + (int) (threadIdx.x / 16)) * 16;
+        *reinterpret_cast<s8v*>(to + place) = a;
+        if constexpr (QT == 0) *reinterpret_cast<s8v*>(to + KB * 1024 + place) = b;
     }
-    if (li == 0) p.info[(int64_t) h * p.pairs + pair].x = p.sl2 * kv8_pow2(e);
+    if (li == 0 && pair < p.pairs) p.info[(int64_t) h * p.pairs + pair].x = p.sl2 * kv8_pow2(e);
 }
 
-// 16 rows of halfs from row r0 on (past the last: the last again) as an operand: lane (n, g4) row n, features 32 j + 8 g4 ..
-template <int D>
-__device__ __forceinline__ void operand(s8v (&a)[D / 32], const uint16_t* rows, int64_t r0, int64_t last, int n, int g4) {
-    const uint16_t* at = rows + std::min(r0 + n, last) * D + 8 * g4;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) a[j] = *reinterpret_cast<const s8v*>(at + 32 * j);
-}
-
-// a pair's largest score and sum of 2^(score - it) over tokens [split kbs, (split + 1) kbs): RT tiles of 16 pairs in registers
-template <int D, bool QS, int RT>
-__global__ __launch_bounds__(256, 2) void kv8_stats_kernel(const WeightsParams p) {
-    constexpr int KB = D / 32;
-    __shared__ float red[4][RT * 16][2];
-    const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.x % p.nh, split = blockIdx.x / p.nh % p.ns;
-    const int64_t pair0 = (int64_t) (blockIdx.x / p.nh / p.ns) * RT * 16;
-    s8v q[RT][KB], ql[QS ? RT : 1][KB];
-    float f[RT], m[RT], l[RT];
-    int rlo[RT], rhi[RT];                                         // tokens seen, from the split's first on
-    const int64_t row0 = pair0 / p.G, row1 = std::min<int64_t>((pair0 + RT * 16 - 1) / p.G, p.T - 1);
-    const int64_t j0 = split * p.kbs;
-    const int64_t kb = std::max(j0, low_of(p, p.p0 + row0)), ke = std::min(j0 + p.kbs, p.p0 + row1 + 1);
-    const uint16_t *qh = p.qh + (int64_t) h * p.pairs * D, *qlo = p.ql + (int64_t) h * p.pairs * D, *k = p.k + (int64_t) h * p.n * D;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int64_t pair = std::min(pair0 + rt * 16 + n, p.pairs - 1), pos = p.p0 + pair / p.G;
-        operand<D>(q[rt], qh, pair0 + rt * 16, p.pairs - 1, n, g4);
-        if constexpr (QS) operand<D>(ql[rt], qlo, pair0 + rt * 16, p.pairs - 1, n, g4);
-        f[rt] = p.info[(int64_t) h * p.pairs + pair].x;
-        m[rt] = -INFINITY, l[rt] = 0.0f;
-        rlo[rt] = (int) (std::max(low_of(p, pos), j0) - j0), rhi[rt] = (int) (std::min(pos, j0 + p.kbs - 1) - j0);
-    }
-    // tokens that all of the pairs see
-    const int64_t full_lo = low_of(p, p.p0 + row1), full_hi = p.p0 + row0 + 1;
-    const int t0 = kb < ke ? (int) ((kb - j0) / 32) : 0, t1 = kb < ke ? (int) ((ke - j0 + 31) / 32) : 0;
-    s8v a[2][KB];
-    int t = t0 + ((w - t0) & 3);
-    if (t < t1)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) operand<D>(a[i], k, j0 + t * 32 + 16 * i, p.n - 1, n, g4);
-    for (; t < t1; t += 4) {
-        f4v s[RT][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                f4v x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < KB; ++j) {
-                    x = mfma16<false>(a[i][j], q[rt][j], x);
-                    if constexpr (QS) x = mfma16<false>(a[i][j], ql[rt][j], x);
-                }
-                s[rt][i] = x;
-            }
-        if (t + 4 < t1)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) operand<D>(a[i], k, j0 + (t + 4) * 32 + 16 * i, p.n - 1, n, g4);
-        const bool edge = j0 + t * 32 < full_lo || j0 + t * 32 + 32 > full_hi;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[rt][e / 4][e % 4] * f[rt];
-            if (edge)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int key = t * 32 + (e / 4) * 16 + 4 * g4 + e % 4;
-                    x[e] = key >= rlo[rt] && key <= rhi[rt] ? x[e] : -INFINITY;
-                }
-            // (each lane its own tokens' largest: the four lanes of a pair meet at the end)
-            float top = m[rt];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum += fast_exp2(x[e] - ref);
-            l[rt] = l[rt] * fast_exp2(m[rt] - ref) + sum;
-            m[rt] = top;
-        }
-    }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const float top = rows_max(m[rt]), ref = top == -INFINITY ? 0.0f : top;
-        const float sum = rows_sum(l[rt] * fast_exp2(m[rt] - ref));
-        if (g4 == 0) red[w][rt * 16 + n][0] = top, red[w][rt * 16 + n][1] = sum;
-    }
-    __syncthreads();
-    const int64_t pair = pair0 + threadIdx.x;
-    if (threadIdx.x < RT * 16 && pair < p.pairs) {
-        float top = -INFINITY, sum = 0.0f;
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, red[i][threadIdx.x][0]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        for (int i = 0; i < 4; ++i) sum += red[i][threadIdx.x][1] * fast_exp2(red[i][threadIdx.x][0] - ref);
-        p.part[((int64_t) h * p.pairs + pair) * p.ns + split] = float2{top, sum};
-    }
-}
-// a pair's splits together, in order
-__global__ __launch_bounds__(256) void kv8_stats_join_kernel(const WeightsParams p) {
-    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    if (i >= p.pairs * p.nh) return;
-    const float2* at = p.part + i * p.ns;
-    float top = -INFINITY, sum = 0.0f;
-    for (int s = 0; s < p.ns; ++s) top = fmaxf(top, at[s].x);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    for (int s = 0; s < p.ns; ++s) sum += at[s].y * fast_exp2(at[s].x - ref);
-    p.info[i].y = ref, p.info[i].z = sum == 0.0f ? 0.0f : 1.0f / sum;
-}
+constexpr int KT = 4, RUN = 16 * KT;              // tiles of 16 tokens a wave; tokens
 
 __device__ __forceinline__ void give(const WeightsParams& p, int h, int64_t t, float sum) {
     const int b = kv8_block(p.c, p.c.table, 0, t >> p.c.shift);
@@ -191,87 +87,168 @@ __device__ __forceinline__ void give(const WeightsParams& p, int h, int64_t t, f
     p.acc1[at] = (p.acc0 && t < p.p0 ? p.acc0[at] : 0.0f) + sum;
 }
 
-// what pairs [rs prs, (rs + 1) prs) give KT tiles of 16 tokens, which stay in registers
-template <int D, bool QS, int KT>
-__global__ __launch_bounds__(256, 2) void kv8_columns_kernel(const WeightsParams p) {
-    constexpr int KB = D / 32;
-    __shared__ float red[4][KT * 16];
+// pass 1 (STATS): each pair's largest score and sum over a wave's 64 tokens; pass 2: what a split of the pairs gives each of them
+template <int D, int FORM, bool QS, bool STATS>
+__global__ __launch_bounds__(256, 2) void kv8_pass_kernel(const WeightsParams p) {
+    constexpr int KB = D / 32, TILE_BYTES = KB * 1024 * (QS ? 2 : 1), TG = 16384 / TILE_BYTES;    // tiles of pairs in LDS at a time
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][16384];
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x % p.nh, r = blockIdx.x / p.nh % p.rs;
-    const int64_t key0 = (int64_t) (blockIdx.x / p.nh / p.rs) * KT * 16;
+    const int64_t run = (int64_t) (blockIdx.x / p.nh / p.rs) * 4 + w, key0 = run * RUN, first = (run - w) * RUN;
+    // the pairs that see any of the work-group's tokens: rows from the first token's own on, to the last that still has the last one in its window
+    const int row0 = (int) std::max<int64_t>(0, first - p.p0), row1 = p.win > 0 ? (int) std::min<int64_t>(p.T, std::max<int64_t>(0, first + 4 * RUN - 1 + p.win - p.p0)) : p.T;
+    const int a0 = std::max(r * p.prs, row0 >= p.T ? p.pairs : row0 * p.G / 16 * 16), a1 = std::min(std::min((r + 1) * p.prs, p.pairs), row1 * p.G);
+    const float4* info = p.info + (int64_t) h * p.pairs;
+    const uint8_t* q16 = p.q16 + (int64_t) h * p.tiles * TILE_BYTES;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (__attribute__((address_space(3))) uint8_t*) &lds[0][0]);
+    const uint32_t off[4] = {(uint32_t) lane * 16, (uint32_t) lane * 16, (uint32_t) lane * 16, (uint32_t) lane * 16};
+    float4 f[TG];
+    // (tiles past the last: the last operands again, masked)
+    auto ask = [&](int pair0, int buf) __attribute__((always_inline)) {
+        const int tile = std::min(pair0 / 16 + w * TG / 4, p.tiles - 1);
+        lds_fetch_run<false, 4>(q16 + (int64_t) tile * TILE_BYTES + (TG >= 4 ? 0 : w % (4 / TG) * 4096), off, lds0 + buf * 16384 + w * 4096);
+#pragma unroll
+        for (int i = 0; i < TG; ++i) f[i] = info[std::min(pair0 + 16 * i + n, p.pairs - 1)];
+    };
+    if (a0 < a1) ask(a0, 0);
+    // ---- the tokens
     s8v k[KT][KB];
-    float sum[KT][4];
-    const uint16_t *qh = p.qh + (int64_t) h * p.pairs * D, *qlo = p.ql + (int64_t) h * p.pairs * D, *kr = p.k + (int64_t) h * p.n * D;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-        operand<D>(k[kt], kr, key0 + kt * 16, p.n - 1, n, g4);
+        const int64_t t = key0 + kt * 16 + n;
+        const int b = t < p.n ? kv8_block(p.c, p.c.table, 0, t >> p.c.shift) : -1;
+        const uint8_t* row = p.c.kc + (kv8_rows(p.c, std::max(b, 0), p.h0 + h) + (t & (p.c.block - 1))) * D + 16 * g4;
+        const float sc = p.c.ksc[(int64_t) std::max(b, 0) * p.c.Hkv + p.h0 + h];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[kt][i] = 0.0f;
+        for (int j = 0; j < D / 64; ++j) {
+            uint4 x = *reinterpret_cast<const uint4*>(row + 64 * j);
+            if (b < 0) x = uint4{0, 0, 0, 0};
+            k[kt][2 * j] = kv8_halfs8<FORM>(x.x, x.y, sc, sc), k[kt][2 * j + 1] = kv8_halfs8<FORM>(x.z, x.w, sc, sc);
+        }
     }
-    // the pairs that see any of these tokens: rows from the first token's own on, to the last that still has the last one in its window
-    const int64_t row0 = std::max<int64_t>(0, key0 - p.p0), row1 = p.win > 0 ? std::min<int64_t>(p.T, key0 + KT * 16 - 1 + p.win - p.p0) : p.T;
-    const int64_t a0 = std::max(r * p.prs, row0 * p.G / 16 * 16), a1 = std::min(std::min((r + 1) * p.prs, p.pairs), row1 * p.G);
-    const float4* info = p.info + (int64_t) h * p.pairs;
-    s8v q[KB], ql[QS ? KB : 1];
-    float4 f{};
-    int64_t pair0 = a0 + 16 * w;
-    if (pair0 < a1) {
-        operand<D>(q, qh, pair0, p.pairs - 1, n, g4);
-        if constexpr (QS) operand<D>(ql, qlo, pair0, p.pairs - 1, n, g4);
-        f = info[std::min(pair0 + n, p.pairs - 1)];
-    }
-    for (; pair0 < a1; pair0 += 64) {
-        f4v s[KT];
+    float sum[STATS ? 1 : KT][4];
+    if constexpr (!STATS)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            f4v x = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int j = 0; j < KB; ++j) {
-                x = mfma16<false>(k[kt][j], q[j], x);
-                if constexpr (QS) x = mfma16<false>(k[kt][j], ql[j], x);
+            for (int i = 0; i < 4; ++i) sum[kt][i] = 0.0f;
+
+    int buf = 0;
+    for (int group = a0; group < a1; group += 16 * TG, buf ^= 1) {
+        // (the numbers asked for with them are waited for here: further on the compiler would wait for the next group's transfers too)
+        float4 now[TG];
+#pragma unroll
+        for (int i = 0; i < TG; ++i) {
+            now[i] = f[i];
+            asm volatile("" : "+v"(now[i].x), "+v"(now[i].y), "+v"(now[i].z));
+        }
+        // this group's operands are there, everyone's; the other buffer has been read
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (group + 16 * TG < a1) ask(group + 16 * TG, buf ^ 1);
+#pragma unroll
+        for (int tg = 0; tg < TG; ++tg) {
+            const int pair0 = group + 16 * tg, pair = pair0 + n;
+            const int64_t top = p.p0 + row_of(p, std::min(pair0, p.pairs - 1)), last = p.p0 + row_of(p, std::min(pair0 + 15, p.pairs - 1));
+            if (pair0 >= a1 || last < key0 || low_of(p, top) >= key0 + RUN) continue;     // (none of them sees this wave's tokens)
+            const uint8_t* ql = &lds[buf][tg * TILE_BYTES + lane * 16];
+            f4v s[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[kt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < KB * (QS ? 2 : 1); ++j) {
+                const s8v q = *reinterpret_cast<const s8v*>(ql + j * 1024);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) s[kt] = mfma16<false>(k[kt][j % KB], q, s[kt]);
             }
-            s[kt] = x;
-        }
-        const float4 now = f;
-        const int64_t pair = pair0 + n;
-        if (pair0 + 64 < a1) {
-            operand<D>(q, qh, pair0 + 64, p.pairs - 1, n, g4);
-            if constexpr (QS) operand<D>(ql, qlo, pair0 + 64, p.pairs - 1, n, g4);
-            f = info[std::min(pair + 64, p.pairs - 1)];
-        }
-        const int64_t first = p.p0 + pair0 / p.G, last = p.p0 + (std::min(pair0 + 15, p.pairs - 1)) / p.G;
-        const bool edge = key0 + KT * 16 > first + 1 || key0 < low_of(p, last) || pair0 + 16 > a1;
-        if (edge) {
-            const int64_t pos = p.p0 + std::min(pair, p.pairs - 1) / p.G, lo = low_of(p, pos);
-            const bool live = pair < a1;
+            const bool edge = key0 + RUN > top + 1 || key0 < low_of(p, last) || pair0 + 16 > a1;
+            int lo = 0, hi = RUN;                                 // tokens seen, from key0 on: lo .. hi - 1
+            if (edge) {
+                const int64_t pos = p.p0 + row_of(p, std::min(pair, p.pairs - 1));
+                lo = (int) std::min<int64_t>(std::max<int64_t>(low_of(p, pos) - key0, 0), RUN);
+                hi = pair < a1 ? (int) std::min<int64_t>(std::max<int64_t>(pos + 1 - key0, 0), RUN) : 0;
+            }
+            if constexpr (STATS) {
+                if (edge)
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+                    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t key = key0 + kt * 16 + 4 * g4 + i;
-                    const float e = fast_exp2(fmaf(s[kt][i], now.x, -now.y)) * now.z;
-                    sum[kt][i] += live && key >= lo && key <= pos ? e : 0.0f;
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = kt * 16 + 4 * g4 + i;
+                            if (key < lo || key >= hi) s[kt][i] = -INFINITY;
+                        }
+                float big = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) big = fmaxf(big, s[kt][i]);
+                big = rows_max(big) * now[tg].x;                  // (the factor is positive)
+                const float ref = big == -INFINITY ? 0.0f : big;
+                float all = 0.0f;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) all += fast_exp2(fmaf(s[kt][i], now[tg].x, -ref));
+                all = rows_sum(all);
+                if (g4 == 0 && pair < a1) p.part[((int64_t) h * p.nb + run) * p.pairs + pair] = float2{big, all};
+            } else if (edge) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = kt * 16 + 4 * g4 + i;
+                        const float e = fast_exp2(fmaf(s[kt][i], now[tg].x, -now[tg].y)) * now[tg].z;
+                        sum[kt][i] += key >= lo && key < hi ? e : 0.0f;
+                    }
+            } else
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[kt][i] = fmaf(fast_exp2(fmaf(s[kt][i], now[tg].x, -now[tg].y)), now[tg].z, sum[kt][i]);
+        }
+    }
+    if constexpr (!STATS)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float v = row16_sum(sum[kt][i]);
+                const int64_t t = key0 + kt * 16 + 4 * g4 + i;
+                if (n == 0 && t < p.n) {
+                    if (p.sums) p.sums[((int64_t) r * p.nh + h) * p.n + t] = v;
+                    else give(p, h, t, v);
                 }
-        } else
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum[kt][i] = fmaf(fast_exp2(fmaf(s[kt][i], now.x, -now.y)), now.z, sum[kt][i]);
+            }
+}
+
+// a pair's runs of tokens together: 16 pairs a work-group, 16 threads each a part of the runs
+__global__ __launch_bounds__(256) void kv8_stats_join_kernel(const WeightsParams p) {
+    __shared__ float2 red[16][17];
+    const int h = blockIdx.y, n = threadIdx.x & 15, part = threadIdx.x >> 4;
+    const int pair = (int) blockIdx.x * 16 + n, pc = std::min(pair, p.pairs - 1);
+    const int64_t pos = p.p0 + row_of(p, pc);
+    const float2* at = p.part + (int64_t) h * p.nb * p.pairs + pc;
+    float top = -INFINITY, sum = 0.0f;
+    const int64_t end = pos / RUN + 1;
+#pragma unroll 4
+    for (int64_t b = low_of(p, pos) / RUN + part; b < end; b += 16) {
+        const float2 v = at[b * p.pairs];
+        const float m = fmaxf(top, v.x), ref = m == -INFINITY ? 0.0f : m;
+        sum = sum * fast_exp2(top - ref) + v.y * fast_exp2(v.x - ref);
+        top = m;
     }
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float v = row16_sum(sum[kt][i]);
-            if (n == 0) red[w][kt * 16 + 4 * g4 + i] = v;
-        }
+    red[part][n] = float2{top, sum};
     __syncthreads();
-    const int64_t t = key0 + threadIdx.x;
-    if (threadIdx.x < KT * 16 && t < p.n) {
-        const float v = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-        if (p.sums) p.sums[((int64_t) r * p.nh + h) * p.n + t] = v;
-        else give(p, h, t, v);
-    }
+    if (part || pair >= p.pairs) return;
+    top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, red[i][n].x);
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += red[i][n].y * fast_exp2(red[i][n].x - ref);
+    float4* to = p.info + (int64_t) h * p.pairs + pair;
+    to->y = ref, to->z = sum == 0.0f ? 0.0f : 1.0f / sum;
 }
 __global__ __launch_bounds__(256) void kv8_columns_join_kernel(const WeightsParams p) {
     const int64_t t = (int64_t) blockIdx.x * 256 + threadIdx.x;
@@ -282,24 +259,26 @@ __global__ __launch_bounds__(256) void kv8_columns_join_kernel(const WeightsPara
     give(p, h, t, sum);
 }
 
-template <int D, int QT>
+template <int D, int FORM, int QT>
 int run(ns_gpu* g, const WeightsParams& p) {
     constexpr bool QS = QT == 0;
-    constexpr int RT = D == 128 ? 4 : 2, KT = D == 128 ? 4 : 2;
+    const unsigned grid = (unsigned) ((p.nb + 3) / 4 * p.rs * p.nh);
     kv8_rows_kernel<D, QT><<<dim3((unsigned) ((p.pairs + 15) / 16), (unsigned) p.nh), 256, 0, g->q>>>(p);
     NS_LAUNCHED("kv8_rows");
-    kv8_stats_kernel<D, QS, RT><<<(unsigned) ((p.pairs + RT * 16 - 1) / (RT * 16) * p.ns * p.nh), 256, 0, g->q>>>(p);
-    NS_LAUNCHED("kv8_stats");
-    kv8_stats_join_kernel<<<(unsigned) ((p.pairs * p.nh + 255) / 256), 256, 0, g->q>>>(p);
+    kv8_pass_kernel<D, FORM, QS, true><<<grid, 256, 0, g->q>>>(p);
+    NS_LAUNCHED("kv8_pass");
+    kv8_stats_join_kernel<<<dim3((unsigned) ((p.pairs + 15) / 16), (unsigned) p.nh), 256, 0, g->q>>>(p);
     NS_LAUNCHED("kv8_stats_join");
-    kv8_columns_kernel<D, QS, KT><<<(unsigned) ((p.n + KT * 16 - 1) / (KT * 16) * p.rs * p.nh), 256, 0, g->q>>>(p);
-    NS_LAUNCHED("kv8_columns");
+    kv8_pass_kernel<D, FORM, QS, false><<<grid, 256, 0, g->q>>>(p);
+    NS_LAUNCHED("kv8_pass");
     if (p.sums) {
         kv8_columns_join_kernel<<<dim3((unsigned) ((p.n + 255) / 256), (unsigned) p.nh), 256, 0, g->q>>>(p);
         NS_LAUNCHED("kv8_columns_join");
     }
     return 0;
 }
+template <int D, int FORM>
+int run(ns_gpu* g, int qt, const WeightsParams& p) { return qt == 0 ? run<D, FORM, 0>(g, p) : qt == 1 ? run<D, FORM, 1>(g, p) : run<D, FORM, 2>(g, p); }
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 }  // namespace
@@ -321,41 +300,33 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
     NS_HIP(hipSetDevice(g->dev));
     NS_OWN_SCRATCH(g);
     const int64_t own = (int64_t) ns_own_floats(g), G = Hq / Hkv, e = qt == 0 ? 4 : 2;
-    // as many key heads at a time as leave their keys half of the scratch, as many rows as the rest holds
-    const int64_t one = up((p0 + T) * D / 2 + 16, 64), nh0 = std::min(Hkv, own / 2 / one);
-    if (nh0 < 1) return ns_fail(w + ": more tokens than the library's scratch holds");
-    constexpr int64_t NS = 64, RS = 16;                           // splits, at most
-    // (a pair: its halfs, its four numbers, its splits' two each)
-    const int64_t per = nh0 * G * (D / 2 * (qt == 0 ? 2 : 1) + 4 + 2 * NS), sums = RS * nh0 * (p0 + T);
-    const int64_t rows = (own - nh0 * one - sums - 1024) / std::max<int64_t>(per, 1);
-    if (rows < 1) return ns_fail(w + ": more tokens and heads than the library's scratch holds");
-    p.G = (int) G, p.qs = qs, p.win = win > 0 ? win : 0;
+    // as many rows as the scratch holds - a pair its halfs, its four numbers, its two for each 64 tokens -, else fewer key heads at a time
+    constexpr int64_t RS = 16;                                    // splits of the pairs, at most
+    const int64_t runs = (p0 + T + RUN - 1) / RUN, per = G * (D / 2 * (qt == 0 ? 2 : 1) + 4 + 2 * runs), sums = RS * (p0 + T) + 16 * D + 1024;
+    const int64_t nh0 = std::min(Hkv, own / (per + sums));
+    if (nh0 < 1) return ns_fail(w + ": more tokens and heads than the library's scratch holds");
+    const int64_t rows = std::min({T, (own / nh0 - sums) / per, std::max<int64_t>(1, ((int64_t) 1 << 31) / (G * G) - 64)});
+    p.G = (int) G, p.ginv = (uint32_t) ((((int64_t) 1 << 32) + G - 1) / G), p.qs = qs, p.win = win > 0 ? win : 0;
     p.sl2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float) D)) * 1.4426950408889634f;
     for (int64_t h = 0; h < Hkv; h += nh0) {
         p.h0 = (int) h, p.nh = (int) std::min(nh0, Hkv - h);
         for (int64_t r = 0; r < T; r += rows) {
-            p.T = (int) std::min(rows, T - r), p.p0 = p0 + r, p.n = p.p0 + p.T, p.pairs = p.T * G;
+            p.T = (int) std::min(rows, T - r), p.p0 = p0 + r, p.n = p.p0 + p.T, p.pairs = (int) (p.T * G);
             p.q = (const uint8_t*) q + r * qs * e, p.acc0 = r ? acc1 : acc0, p.acc1 = acc1;
-            const int64_t tiles = D == 128 ? 64 : 32, blk = (p.pairs + tiles - 1) / tiles * p.nh, cols = (p.n + tiles - 1) / tiles * p.nh;
-            // work-groups enough for two a CU, twice
-            const int64_t ns = std::max<int64_t>(1, std::min<int64_t>({(1024 + blk - 1) / blk, NS, (p.n + 255) / 256}));
-            p.kbs = up((p.n + ns - 1) / ns, 128), p.ns = (int) ((p.n + p.kbs - 1) / p.kbs);
-            const int64_t rs = std::max<int64_t>(1, std::min<int64_t>({(1024 + cols - 1) / cols, RS, (p.pairs + 255) / 256}));
-            p.prs = up((p.pairs + rs - 1) / rs, 64), p.rs = (int) ((p.pairs + p.prs - 1) / p.prs);
-            if (!ns_grid_fits(blk * p.ns, 256) || !ns_grid_fits(cols * p.rs, 256)) return ns_fail(w + ": more work-groups than a launch takes");
+            // work-groups for the chip's places, two a CU, twice; splits of 64 pairs and more
+            p.nb = (p.n + RUN - 1) / RUN;
+            const int64_t blocks = (p.nb + 3) / 4 * p.nh, rs = std::max<int64_t>(1, std::min<int64_t>({(1024 + blocks - 1) / blocks, RS, (int64_t) (p.pairs + 63) / 64}));
+            p.prs = (int) up((p.pairs + rs - 1) / rs, 64), p.rs = (p.pairs + p.prs - 1) / p.prs;
+            if (!ns_grid_fits(blocks * p.rs, 256) || !ns_grid_fits((p.pairs + 15) / 16, 256)) return ns_fail(w + ": more work-groups than a launch takes");
             float* at = g->own_scratch;
             auto take = [&](int64_t floats) { float* was = at; at += up(floats, 64); return was; };
-            uint16_t* k = (uint16_t*) take(p.nh * p.n * D / 2);
-            p.qh = (uint16_t*) take(p.nh * p.pairs * D / 2);
-            p.ql = qt == 0 ? (uint16_t*) take(p.nh * p.pairs * D / 2) : p.qh;
-            p.info = (float4*) take(p.nh * p.pairs * 4);
-            p.part = (float2*) take(p.nh * p.pairs * p.ns * 2);
-            p.sums = p.rs > 1 ? take(p.rs * p.nh * p.n) : nullptr;
-            p.k = k;
+            p.tiles = (p.pairs + 15) / 16;
+            p.q16 = (uint8_t*) take((int64_t) p.nh * p.tiles * 16 * D / 2 * (qt == 0 ? 2 : 1));
+            p.info = (float4*) take((int64_t) p.nh * p.pairs * 4);
+            p.part = (float2*) take(p.nh * p.pairs * p.nb * 2);
+            p.sums = p.rs > 1 ? take((int64_t) p.rs * p.nh * p.n) : nullptr;
             if (at - g->own_scratch > own) return ns_fail(w + ": more tokens and heads than the library's scratch holds");
-            if (ns_kv8_widen(g, form, p.c, p.h0, p.nh, 0, p.n, k, nullptr)) return -1;
-            const int rc = D == 128 ? (qt == 0 ? run<128, 0>(g, p) : qt == 1 ? run<128, 1>(g, p) : run<128, 2>(g, p))
-                                    : (qt == 0 ? run<256, 0>(g, p) : qt == 1 ? run<256, 1>(g, p) : run<256, 2>(g, p));
+            const int rc = D == 128 ? (form == 0 ? run<128, 0>(g, qt, p) : run<128, 1>(g, qt, p)) : (form == 0 ? run<256, 0>(g, qt, p) : run<256, 1>(g, qt, p));
             if (rc) return rc;
         }
     }
