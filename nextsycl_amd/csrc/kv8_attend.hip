@@ -34,6 +34,7 @@ struct AttendParams {
     const int32_t *start, *lens;
     int64_t p0;                 // lens null: the one sequence's tokens in front of the call, its T rows
     int T, most, S, Hq, G;
+    uint32_t ginv;              // 2^32 / G, rounded up
     int64_t longest, win;
     int nw, nz;                 // work-groups the chunks are dealt to; chunks of pairs
     float sl2;                  // scale x log2(e)
@@ -56,6 +57,11 @@ __device__ __forceinline__ void span_of(const AttendParams& p, const Kv8Seq& q, 
     hi = std::min<int64_t>((int64_t) q.len + q.n, p.longest);
     lo = p.win > 0 ? std::max<int64_t>(0, (int64_t) q.len + 1 - p.win) : 0;
 }
+
+// (a 64-bit division takes some hundred instructions, a 32-bit one a few tens)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return (a | b) >> 31 ? a / b : (int64_t) ((uint32_t) a / (uint32_t) b); }
+// the row of a pair (fewer than 2^31 / G of them)
+__device__ __forceinline__ int row_of(const AttendParams& p, int pair) { return p.G == 1 ? pair : (int) __umulhi((uint32_t) pair, p.ginv); }
 
 // a sequence's chunks a key head: chunk `first` and on (a sequence with rows has one at least)
 __device__ __forceinline__ int chunks_of(const AttendParams& p, const Kv8Seq& q, int& first) {
@@ -87,18 +93,23 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
         if (wg >= p.nw) return;
     }
     const int Hkv = p.c.Hkv;
-    // ---- this work-group's run of chunks: `left` of them from chunk `at` of (sequence s, key head hk) on
-    int s = 0, left;
-    int64_t rest, run;                                            // chunks of a run; of sequence s (its heads one behind the other) in front of this one
+    // (all of the arguments at once: the compiler would ask for each group of them where it is used, one wait behind the other)
+    asm volatile("" ::"s"(p.c.kc), "s"(p.c.vc), "s"(p.c.ksc), "s"(p.c.vsc), "s"(p.c.table), "s"(p.c.tmax), "s"(p.c.blocks), "s"(p.c.shift), "s"(p.q), "s"(p.qs), "s"(p.start), "s"(p.lens),
+                 "s"(p.T), "s"(p.longest), "s"(p.win), "s"(p.sl2), "s"(p.ginv), "s"(p.nw));
+    // ---- this work-group's run of chunks: `left` of them, from the `rest`th of sequence s on (its heads one behind the other)
+    int s = 0, left, first, nch;
+    int64_t rest, run;
+    Kv8Seq q;
     {
-        int first;
         int64_t total;
         if (p.S == 1) {
-            total = chunks_of(p, seq_of(p, 0), first);
+            q = seq_of(p, 0);
+            total = nch = chunks_of(p, q, first);
         } else {
             const int per = (p.S + WAVES * 64 - 1) / (WAVES * 64), s0 = std::min(tid * per, p.S), s1 = std::min(s0 + per, p.S);
             int64_t mine = 0;
-            for (int i = s0; i < s1; ++i) mine += chunks_of(p, seq_of(p, i), first);
+            int its;                                              // (a sequence's first chunk)
+            for (int i = s0; i < s1; ++i) mine += chunks_of(p, seq_of(p, i), its);
             int64_t x = mine;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
@@ -115,12 +126,11 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                 if (i < w) before += y;
                 total += y;
             }
-            run = (total * Hkv + p.nw - 1) / p.nw;
-            const int64_t from = wg * run;
+            const int64_t from = wg * quotient(total * Hkv + p.nw - 1, p.nw);
             if (before * Hkv <= from && from < (before + mine) * Hkv) {
                 int64_t b = before;
                 for (int i = s0; i < s1; ++i) {
-                    const int64_t y = chunks_of(p, seq_of(p, i), first);
+                    const int64_t y = chunks_of(p, seq_of(p, i), its);
                     if (from < (b + y) * Hkv) {
                         found[0] = i, found[1] = from - b * Hkv;
                         break;
@@ -130,12 +140,15 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
             }
             __syncthreads();
         }
-        run = (total * Hkv + p.nw - 1) / p.nw;
-        const int64_t from = wg * run;
-        if (from >= total * Hkv) return;
-        left = (int) std::min(run, total * Hkv - from);
-        rest = from;
-        if (p.S > 1) s = __builtin_amdgcn_readfirstlane((int) found[0]), rest = found[1];
+        run = quotient(total * Hkv + p.nw - 1, p.nw);
+        rest = wg * run;
+        if (rest >= total * Hkv) return;
+        left = (int) std::min(run, total * Hkv - rest);
+        if (p.S > 1) {
+            s = __builtin_amdgcn_readfirstlane((int) found[0]), rest = found[1];
+            q = seq_of(p, s);
+            nch = chunks_of(p, q, first);
+        }
     }
     uint8_t* stage = lds + w * WREG;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (__attribute__((address_space(3))) uint8_t*) stage);
@@ -151,12 +164,9 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
 
     for (;;) {
         // ---- a piece of the run: chunks c0 .. c1 - 1 of one unit
-        const Kv8Seq q = seq_of(p, s);
         int64_t lo, hi;
         span_of(p, q, lo, hi);
-        int first;
-        const int nch = chunks_of(p, q, first);
-        const int hk = (int) (rest / nch), c0 = (int) (rest - (int64_t) hk * nch), c1 = std::min(nch, c0 + left);
+        const int hk = (int) quotient(rest, nch), c0 = (int) (rest - (int64_t) hk * nch), c1 = std::min(nch, c0 + left);
         const int pairs = q.n * p.G, pair0 = z * RT * 16;
         if (pair0 < pairs) {
             // from here on tokens are counted from the piece's first
@@ -215,7 +225,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
             for (int rt = 0; rt < RT; ++rt) {
                 const int pair = pair0 + rt * 16 + n;
                 const bool live = pair < pairs;
-                const int i = live ? pair / p.G : 0, g = live ? pair - i * p.G : 0;
+                const int i = live ? row_of(p, pair) : 0, g = live ? pair - i * p.G : 0;
                 rhi[rt] = live ? std::min(pos0 + i, je - 1) : -1;
                 rlo[rt] = p.win > 0 ? (int) std::max<int64_t>(jb, pos0 + i + 1 - p.win) : jb;
                 const int64_t at = (int64_t) (q.first + i) * p.qs + (int64_t) (hk * p.G + g) * D;
@@ -261,7 +271,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                 for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
             }
             // tiles that need no mask: every token seen by every row there is
-            const int full_hi = std::min(pos0 + pair0 / p.G + 1, je);
+            const int full_hi = std::min(pos0 + row_of(p, pair0) + 1, je);
             const int full_lo = p.win > 0 ? (int) std::max<int64_t>(jb, pos0 + q.n - p.win) : jb;
 
             for (int sp = 0; sp < je; sp += span) {
@@ -428,7 +438,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                 }
                 if (whole) {
                     const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-                    const int i2 = pair / p.G, g = pair - i2 * p.G;
+                    const int i2 = row_of(p, pair), g = pair - i2 * p.G;
                     const float v[4] = {sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv};
                     const int64_t at = ((int64_t) (q.first + i2) * p.Hq + hk * p.G + g) * D + d;
 #pragma unroll
@@ -440,15 +450,16 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                     if (d == 0) to[D] = top, to[D + 1] = all;
                 }
             }
-            if (z == 0 && c0 == 0 && tid == 0 && p.units) p.units[unit] = int2{wg, whole ? wg : wg + (int) ((nch - left + run - 1) / run)};
+            if (z == 0 && c0 == 0 && tid == 0 && p.units) p.units[unit] = int2{wg, whole ? wg : wg + (int) quotient(nch - left + run - 1, run)};
         }
         left -= c1 - c0;
         if (left <= 0) break;
         rest += c1 - c0;
         if (rest >= (int64_t) nch * Hkv) {
             rest = 0;
-            do ++s;
-            while (s < p.S - 1 && seq_of(p, s).n <= 0);
+            do q = seq_of(p, ++s), nch = chunks_of(p, q, first);
+            while (nch == 0 && s < p.S - 1);
+            if (nch == 0) return;
         }
         __syncthreads();                                          // (the regions are read: the next piece's transfers may begin)
     }
@@ -491,35 +502,54 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const AttendParams p) {
 #pragma unroll
     for (int k = 0; k < SG; ++k) sum += *reinterpret_cast<const f4v*>(&sums[k][d]), all += wsum[k];
     const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-    const int i = pair / p.G, g = pair - i * p.G;
+    const int i = row_of(p, pair), g = pair - i * p.G;
     const int64_t at = ((int64_t) (q.first + i) * p.Hq + hk * p.G + g) * D + d;
 #pragma unroll
     for (int k = 0; k < 4; ++k) store_o<QT>(p.out, at + k, sum[k] * inv);
     if (p.stats && tid == 0) p.stats[2 * place] = ref, p.stats[2 * place + 1] = inv;
 }
 
-// acc1 = acc0 + the weights of the pairs: a thread a token
+// acc1 = acc0 + the weights of the pairs: a thread 4 tokens in a row (a block holds them), pairs 4 at a time
 __global__ __launch_bounds__(256) void kv8_given_kernel(const AttendParams p) {
     const int hk = blockIdx.y, s = blockIdx.z;
     const Kv8Seq q = seq_of(p, s);
-    const int64_t t = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    const int64_t t0 = ((int64_t) blockIdx.x * 256 + threadIdx.x) * 4, end = (int64_t) q.len + q.n;
+    if (q.n <= 0 || t0 >= end) return;
+    const int b = kv8_block(p.c, p.c.table, s, t0 >> p.c.shift);
+    if (b < 0) return;
+    const int64_t at = kv8_rows(p.c, b, hk) + (t0 & (p.c.block - 1));
     int64_t lo, hi;
     span_of(p, q, lo, hi);
-    if (q.n <= 0 || t >= (int64_t) q.len + q.n) return;
-    const int b = kv8_block(p.c, p.c.table, s, t >> p.c.shift);
-    if (b < 0) return;
-    const int64_t at = kv8_rows(p.c, b, hk) + (t & (p.c.block - 1));
-    float sum = 0.0f;
-    if (t < hi) {
-        const int64_t place = ((int64_t) s * p.c.Hkv + hk) * p.most * p.G;
-        for (int pair = 0; pair < q.n * p.G; ++pair) {
-            // (only what the pair has seen was written)
-            const int64_t pos = (int64_t) q.len + pair / p.G;
-            if (t > pos || (p.win > 0 && t + p.win <= pos)) continue;
-            sum += fast_exp2(p.scores[(place + pair) * p.pad + t] - p.stats[2 * (place + pair)]) * p.stats[2 * (place + pair) + 1];
-        }
+    f4v sum = {0.0f, 0.0f, 0.0f, 0.0f}, was = sum;
+    if (p.acc0) {
+        if (t0 + 4 <= q.len) was = __builtin_bit_cast(f4v, *reinterpret_cast<const floats4_t*>(p.acc0 + at));
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) was[i] = t0 + i < q.len ? p.acc0[at + i] : 0.0f;
     }
-    p.acc1[at] = (p.acc0 && t < q.len ? p.acc0[at] : 0.0f) + sum;
+    const int64_t place = ((int64_t) s * p.c.Hkv + hk) * p.most * p.G;
+    const float* scores = p.scores + place * p.pad + t0;
+    const float* stats = p.stats + 2 * place;
+    // (only what a pair has seen was written, in whole tiles: tokens of these that one of its rows sees lie in one, the others are 0 there. A tile that
+    // none of them lies in may hold anything)
+    if (lo < hi && t0 < hi)
+        for (int i = 0; i < q.n; ++i) {
+            const int64_t pos = (int64_t) q.len + i;
+            if (t0 > pos || (p.win > 0 && t0 + 3 + p.win <= pos)) continue;
+#pragma unroll 4
+            for (int g = 0; g < p.G; ++g) {
+                const int pair = i * p.G + g;
+                const f4v x = *reinterpret_cast<const f4v*>(scores + (int64_t) pair * p.pad);
+                const float m = stats[2 * pair], inv = stats[2 * pair + 1];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum[k] = fmaf(fast_exp2(x[k] - m), inv, sum[k]);
+            }
+        }
+    if (t0 + 4 <= end) *reinterpret_cast<floats4_t*>(p.acc1 + at) = __builtin_bit_cast(floats4_t, was + sum);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (t0 + i < end) p.acc1[at + i] = was[i] + sum[i];
 }
 
 template <int D, int RT, int QT>
@@ -574,6 +604,7 @@ int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, in
     const int64_t pairs = (int64_t) p.most * p.G, nz = pair_chunks(pairs, D), rows = (int64_t) p.S * p.most * p.Hq;
     const Scratch x = scratch_of(p.S, p.most, p.Hq, Hkv, D, p.longest, p.acc1 != nullptr, p.nw);
     p.nz = (int) nz, p.pad = x.pad;
+    p.ginv = (uint32_t) ((((int64_t) 1 << 32) + p.G - 1) / p.G);
     const int64_t grid = nz > 1 ? (int64_t) (p.nw + 7) / 8 * 8 * nz : p.nw;
     if (!ns_grid_fits(grid, 256) || !ns_grid_fits(rows, 256)) return ns_fail(w + ": more work-groups than a launch takes");
     // (of sequences that are all within a chunk there are no pieces)
@@ -593,7 +624,7 @@ int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, in
         NS_LAUNCHED("kv8_merge");
     }
     if (p.acc1) {
-        kv8_given_kernel<<<dim3((unsigned) ((p.longest + 255) / 256), (unsigned) Hkv, (unsigned) p.S), 256, 0, g->q>>>(p);
+        kv8_given_kernel<<<dim3((unsigned) ((p.longest + 1023) / 1024), (unsigned) Hkv, (unsigned) p.S), 256, 0, g->q>>>(p);
         NS_LAUNCHED("kv8_given");
     }
     return 0;
@@ -657,7 +688,7 @@ int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     const size_t wide = (size_t) (Hkv * n * D);                   // floats, both streams of halfs
     if (T > DECODE_ROWS && wide <= own / 4 * 3 && n * D * 2 < (int64_t) 1 << 32) {
         uint16_t* k = reinterpret_cast<uint16_t*>(g->own_scratch + (own - wide) / 64 * 64);
-        if (ns_kv8_widen(g, form, c, 0, (int) Hkv, from, n, k, k + Hkv * n * D)) return -1;
+        if (ns_kv8_widen(g, form, c, from, n, k, k + Hkv * n * D)) return -1;
         return ns_attn_prompt_any(g, "ns_kv8_prompt", qt, 0, 0, q, qs, k, k + Hkv * n * D, T, Hq, Hkv, D, n, p0 - from, win > 0 ? win : 0, 1, -1, scale, out,
                                   (own - wide) / 64 * 64);
     }

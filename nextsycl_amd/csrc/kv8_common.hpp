@@ -127,5 +127,5 @@ inline Kv8Cache kv8_cache(const void* kc, const void* vc, const float* ksc, cons
     const int shift = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
     return {(uint8_t*) kc, (uint8_t*) vc, (float*) ksc, (float*) vsc, table, tmax, blocks, (int) Hkv, (int) D, (int) block, shift};
 }
-// kv8_store.hip: tokens from .. from + n - 1 of the table's first sequence, heads h0 .. h0 + nh - 1, as half rows [nh][n][D], values too where v is not null; 0 or -1
-int ns_kv8_widen(ns_gpu* g, int form, const Kv8Cache& c, int h0, int nh, int64_t from, int64_t n, uint16_t* k, uint16_t* v);
+// kv8_store.hip: tokens from .. from + n - 1 of the table's first sequence as half rows [Hkv][n][D]; 0 or -1
+int ns_kv8_widen(ns_gpu* g, int form, const Kv8Cache& c, int64_t from, int64_t n, uint16_t* k, uint16_t* v);

@@ -95,31 +95,41 @@ void launch_store(ns_gpu* g, int form, const StoreParams& p, dim3 grid) {
     else form == 0 ? launch_store<QT, 0, 256>(g, p, grid) : launch_store<QT, 1, 256>(g, p, grid);
 }
 
-// tokens from .. from + n of one sequence as half rows, k and v [heads][n][D]: a thread 16 values
-template <int FORM>
-__global__ __launch_bounds__(256) void kv8_widen_kernel(const Kv8Cache c, int h0, int64_t from, int64_t n, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
-    const int tpr = c.D / 16, h = h0 + blockIdx.y;
-    const int64_t j = ((int64_t) blockIdx.x * 256 + threadIdx.x) / tpr;
-    if (j >= n) return;
-    const int col = threadIdx.x % tpr * 16;
-    const int64_t t = from + j;
-    const int b = kv8_block(c, c.table, 0, t >> c.shift);
-    s8v lo = {0, 0, 0, 0, 0, 0, 0, 0}, hi = lo;
-    if (b >= 0) {
-        const uint4 w = *reinterpret_cast<const uint4*>((blockIdx.z ? c.vc : c.kc) + (kv8_rows(c, b, h) + (t & (c.block - 1))) * c.D + col);
-        const float s = (blockIdx.z ? c.vsc : c.ksc)[(int64_t) b * c.Hkv + h];
-        lo = kv8_halfs8<FORM>(w.x, w.y, s, s), hi = kv8_halfs8<FORM>(w.z, w.w, s, s);
+// tokens from .. from + n of one sequence as half rows, k and v [Hkv][n][D]: a thread 8 values of each of 8 rows, asked for together
+template <int FORM, int D>
+__global__ __launch_bounds__(256) void kv8_widen_kernel(const Kv8Cache c, int64_t from, int64_t n, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
+    constexpr int TPR = D / 8, RPP = 256 / TPR, U = 8;
+    const int h = blockIdx.y, col = threadIdx.x % TPR * 8;
+    const int64_t j0 = (int64_t) blockIdx.x * RPP * U + threadIdx.x / TPR;
+    const uint8_t* pool = blockIdx.z ? c.vc : c.kc;
+    const float* scale = blockIdx.z ? c.vsc : c.ksc;
+    uint16_t* out = (blockIdx.z ? v : k) + (int64_t) h * n * D + col;
+    int b[U];
+    uint2 w[U];
+    float s[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) b[i] = kv8_block(c, c.table, 0, (from + std::min(j0 + i * RPP, n - 1)) >> c.shift);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int64_t t = from + std::min(j0 + i * RPP, n - 1);
+        const int bc = std::max(b[i], 0);
+        w[i] = *reinterpret_cast<const uint2*>(pool + (kv8_rows(c, bc, h) + (t & (c.block - 1))) * D + col);
+        s[i] = scale[(int64_t) bc * c.Hkv + h];
     }
-    s8v* d = reinterpret_cast<s8v*>((blockIdx.z ? v : k) + ((int64_t) blockIdx.y * n + j) * c.D + col);
-    d[0] = lo, d[1] = hi;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        if (b[i] < 0) w[i] = uint2{0, 0};
+        if (j0 + i * RPP < n) *reinterpret_cast<s8v*>(out + (j0 + i * RPP) * D) = kv8_halfs8<FORM>(w[i].x, w[i].y, s[i], s[i]);
+    }
 }
 
 }  // namespace
 
-int ns_kv8_widen(ns_gpu* g, int form, const Kv8Cache& c, int h0, int nh, int64_t from, int64_t n, uint16_t* k, uint16_t* v) {
-    const dim3 grid((unsigned) ((n * (c.D / 16) + 255) / 256), (unsigned) nh, v ? 2 : 1);
-    if (form == 0) kv8_widen_kernel<0><<<grid, 256, 0, g->q>>>(c, h0, from, n, k, v);
-    else kv8_widen_kernel<1><<<grid, 256, 0, g->q>>>(c, h0, from, n, k, v);
+int ns_kv8_widen(ns_gpu* g, int form, const Kv8Cache& c, int64_t from, int64_t n, uint16_t* k, uint16_t* v) {
+    const int64_t rows = 8 * 256 / (c.D / 8);
+    const dim3 grid((unsigned) ((n + rows - 1) / rows), (unsigned) c.Hkv, 2);
+    if (c.D == 128) form == 0 ? kv8_widen_kernel<0, 128><<<grid, 256, 0, g->q>>>(c, from, n, k, v) : kv8_widen_kernel<1, 128><<<grid, 256, 0, g->q>>>(c, from, n, k, v);
+    else form == 0 ? kv8_widen_kernel<0, 256><<<grid, 256, 0, g->q>>>(c, from, n, k, v) : kv8_widen_kernel<1, 256><<<grid, 256, 0, g->q>>>(c, from, n, k, v);
     NS_LAUNCHED("kv8_widen");
     return 0;
 }
