@@ -90,11 +90,13 @@ __device__ __forceinline__ void give(const WeightsParams& p, int h, int64_t t, f
 // pass 1 (STATS): each pair's largest score and sum over a wave's 64 tokens; pass 2: what a split of the pairs gives each of them
 template <int D, int FORM, bool QS, bool STATS>
 __global__ __launch_bounds__(256, 2) void kv8_pass_kernel(const WeightsParams p) {
-    constexpr int KB = D / 32, TILE_BYTES = KB * 1024 * (QS ? 2 : 1), TG = 16384 / TILE_BYTES;    // tiles of pairs in LDS at a time
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][16384];
+    // a stage of LDS: TG tiles of operands, and the numbers of 64 pairs; asked for two ahead
+    constexpr int KB = D / 32, TILE_BYTES = KB * 1024 * (QS ? 2 : 1), TG = 16384 / TILE_BYTES, STAGE = 16384 + 1024;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[3][STAGE];
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x % p.nh, r = blockIdx.x / p.nh % p.rs;
-    const int64_t run = (int64_t) (blockIdx.x / p.nh / p.rs) * 4 + w, key0 = run * RUN, first = (run - w) * RUN;
+    // (the last tokens first: their rows' edges cost more)
+    const int64_t run = ((p.nb + 3) / 4 - 1 - (int64_t) (blockIdx.x / p.nh / p.rs)) * 4 + w, key0 = run * RUN, first = (run - w) * RUN;
     // the pairs that see any of the work-group's tokens: rows from the first token's own on, to the last that still has the last one in its window
     const int row0 = (int) std::max<int64_t>(0, first - p.p0), row1 = p.win > 0 ? (int) std::min<int64_t>(p.T, std::max<int64_t>(0, first + 4 * RUN - 1 + p.win - p.p0)) : p.T;
     const int a0 = std::max(r * p.prs, row0 >= p.T ? p.pairs : row0 * p.G / 16 * 16), a1 = std::min(std::min((r + 1) * p.prs, p.pairs), row1 * p.G);
@@ -102,15 +104,15 @@ __global__ __launch_bounds__(256, 2) void kv8_pass_kernel(const WeightsParams p)
     const uint8_t* q16 = p.q16 + (int64_t) h * p.tiles * TILE_BYTES;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (__attribute__((address_space(3))) uint8_t*) &lds[0][0]);
     const uint32_t off[4] = {(uint32_t) lane * 16, (uint32_t) lane * 16, (uint32_t) lane * 16, (uint32_t) lane * 16};
-    float4 f[TG];
-    // (tiles past the last: the last operands again, masked)
+    // (tiles past the last: the last operands again, masked; numbers past the last: whatever lies behind them, masked too)
     auto ask = [&](int pair0, int buf) __attribute__((always_inline)) {
         const int tile = std::min(pair0 / 16 + w * TG / 4, p.tiles - 1);
-        lds_fetch_run<false, 4>(q16 + (int64_t) tile * TILE_BYTES + (TG >= 4 ? 0 : w % (4 / TG) * 4096), off, lds0 + buf * 16384 + w * 4096);
-#pragma unroll
-        for (int i = 0; i < TG; ++i) f[i] = info[std::min(pair0 + 16 * i + n, p.pairs - 1)];
+        const uint32_t to = lds0 + buf * STAGE;
+        lds_fetch_run<false, 4>(q16 + (int64_t) tile * TILE_BYTES + (TG >= 4 ? 0 : w % (4 / TG) * 4096), off, to + w * 4096);
+        lds_fetch<false>(reinterpret_cast<const uint8_t*>(info + pair0), off[0], to + 16384);
     };
     if (a0 < a1) ask(a0, 0);
+    if (a0 + 16 * TG < a1) ask(a0 + 16 * TG, 1);
     // ---- the tokens
     s8v k[KT][KB];
 #pragma unroll
@@ -133,27 +135,22 @@ __global__ __launch_bounds__(256, 2) void kv8_pass_kernel(const WeightsParams p)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[kt][i] = 0.0f;
 
-    int buf = 0;
-    for (int group = a0; group < a1; group += 16 * TG, buf ^= 1) {
-        // (the numbers asked for with them are waited for here: further on the compiler would wait for the next group's transfers too)
-        float4 now[TG];
-#pragma unroll
-        for (int i = 0; i < TG; ++i) {
-            now[i] = f[i];
-            asm volatile("" : "+v"(now[i].x), "+v"(now[i].y), "+v"(now[i].z));
-        }
-        // this group's operands are there, everyone's; the other buffer has been read
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    int buf = 0, stores = 0;
+    for (int group = a0; group < a1; group += 16 * TG, buf = buf == 2 ? 0 : buf + 1) {
+        // this stage is there, everyone's; the one two ahead is of a buffer that everyone has read. What may still be under way: the next stage's 5 transfers,
+        // and the TG stores behind them where all of the last stage's parts were written
+        if (group + 16 * TG >= a1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else if (!STATS || stores == 0) asm volatile("s_waitcnt vmcnt(5) lgkmcnt(0)" ::: "memory");
+        else if constexpr (TG == 4) asm volatile("s_waitcnt vmcnt(9) lgkmcnt(0)" ::: "memory");
+        else if constexpr (TG == 2) asm volatile("s_waitcnt vmcnt(7) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (group + 16 * TG < a1) ask(group + 16 * TG, buf ^ 1);
-#pragma unroll
-        for (int tg = 0; tg < TG; ++tg) {
-            const int pair0 = group + 16 * tg, pair = pair0 + n;
-            const int64_t top = p.p0 + row_of(p, std::min(pair0, p.pairs - 1)), last = p.p0 + row_of(p, std::min(pair0 + 15, p.pairs - 1));
-            if (pair0 >= a1 || last < key0 || low_of(p, top) >= key0 + RUN) continue;     // (none of them sees this wave's tokens)
+        if (group + 32 * TG < a1) ask(group + 32 * TG, buf == 0 ? 2 : buf - 1);
+        const float4* now = reinterpret_cast<const float4*>(&lds[buf][16384]);
+        // a tile's scores; what they come to, edge: not every pair sees every token (tokens seen: lo .. hi - 1 from key0 on)
+        auto product = [&](int tg, f4v (&s)[KT]) __attribute__((always_inline)) {
             const uint8_t* ql = &lds[buf][tg * TILE_BYTES + lane * 16];
-            f4v s[KT];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) s[kt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -162,15 +159,18 @@ __global__ __launch_bounds__(256, 2) void kv8_pass_kernel(const WeightsParams p)
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) s[kt] = mfma16<false>(k[kt][j % KB], q, s[kt]);
             }
-            const bool edge = key0 + RUN > top + 1 || key0 < low_of(p, last) || pair0 + 16 > a1;
-            int lo = 0, hi = RUN;                                 // tokens seen, from key0 on: lo .. hi - 1
-            if (edge) {
-                const int64_t pos = p.p0 + row_of(p, std::min(pair, p.pairs - 1));
-                lo = (int) std::min<int64_t>(std::max<int64_t>(low_of(p, pos) - key0, 0), RUN);
-                hi = pair < a1 ? (int) std::min<int64_t>(std::max<int64_t>(pos + 1 - key0, 0), RUN) : 0;
-            }
+            // (operands are read 4 steps ahead; left alone the compiler reads each pair of them right in front of its products)
+            constexpr int N = KB * (QS ? 2 : 1), AHEAD = 4;
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+            for (int j = 0; j < N - AHEAD; ++j) __builtin_amdgcn_sched_group_barrier(0x008, KT, 0), __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, KT * AHEAD, 0);
+        };
+        auto take = [&](int tg, f4v (&s)[KT], auto edge, int lo, int hi) __attribute__((always_inline)) {
+            constexpr bool EDGE = decltype(edge)::value;
+            const float4 f = now[16 * tg + n];
             if constexpr (STATS) {
-                if (edge)
+                if constexpr (EDGE)
 #pragma unroll
                     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -183,29 +183,59 @@ __global__ __launch_bounds__(256, 2) void kv8_pass_kernel(const WeightsParams p)
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) big = fmaxf(big, s[kt][i]);
-                big = rows_max(big) * now[tg].x;                  // (the factor is positive)
+                big = rows_max(big) * f.x;                        // (the factor is positive)
                 const float ref = big == -INFINITY ? 0.0f : big;
                 float all = 0.0f;
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) all += fast_exp2(fmaf(s[kt][i], now[tg].x, -ref));
+                    for (int i = 0; i < 4; ++i) all += fast_exp2(fmaf(s[kt][i], f.x, -ref));
                 all = rows_sum(all);
+                const int pair = group + 16 * tg + n;
                 if (g4 == 0 && pair < a1) p.part[((int64_t) h * p.nb + run) * p.pairs + pair] = float2{big, all};
-            } else if (edge) {
+            } else if constexpr (EDGE) {
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int key = kt * 16 + 4 * g4 + i;
-                        const float e = fast_exp2(fmaf(s[kt][i], now[tg].x, -now[tg].y)) * now[tg].z;
+                        const float e = fast_exp2(fmaf(s[kt][i], f.x, -f.y)) * f.z;
                         sum[kt][i] += key >= lo && key < hi ? e : 0.0f;
                     }
             } else
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[kt][i] = fmaf(fast_exp2(fmaf(s[kt][i], now[tg].x, -now[tg].y)), now[tg].z, sum[kt][i]);
+                    for (int i = 0; i < 4; ++i) sum[kt][i] = fmaf(fast_exp2(fmaf(s[kt][i], f.x, -f.y)), f.z, sum[kt][i]);
+        };
+        const int64_t row_first = p.p0 + row_of(p, std::min(group, p.pairs - 1)), row_last = p.p0 + row_of(p, std::min(group + 16 * TG - 1, p.pairs - 1));
+        if (group + 16 * TG <= a1 && key0 + RUN <= row_first + 1 && key0 >= low_of(p, row_last)) {
+            // every pair sees every token: a tile's products beside the last one's exponentials
+            stores = TG;
+            f4v s[2][KT];
+            product(0, s[0]);
+#pragma unroll
+            for (int tg = 0; tg < TG; ++tg) {
+                if (tg + 1 < TG) product(tg + 1, s[(tg + 1) & 1]);
+                take(tg, s[tg & 1], std::false_type(), 0, RUN);
+            }
+        } else {
+            stores = 0;
+#pragma unroll
+            for (int tg = 0; tg < TG; ++tg) {
+                const int pair0 = group + 16 * tg, pair = pair0 + n;
+                const int64_t top = p.p0 + row_of(p, std::min(pair0, p.pairs - 1)), last = p.p0 + row_of(p, std::min(pair0 + 15, p.pairs - 1));
+                if (pair0 >= a1 || last < key0 || low_of(p, top) >= key0 + RUN) continue;     // (none of them sees this wave's tokens)
+                f4v s[KT];
+                product(tg, s);
+                if (key0 + RUN <= top + 1 && key0 >= low_of(p, last) && pair0 + 16 <= a1) take(tg, s, std::false_type(), 0, RUN);
+                else {
+                    const int64_t pos = p.p0 + row_of(p, std::min(pair, p.pairs - 1));
+                    const int lo = (int) std::min<int64_t>(std::max<int64_t>(low_of(p, pos) - key0, 0), RUN);
+                    const int hi = pair < a1 ? (int) std::min<int64_t>(std::max<int64_t>(pos + 1 - key0, 0), RUN) : 0;
+                    take(tg, s, std::true_type(), lo, hi);
+                }
+            }
         }
     }
     if constexpr (!STATS)
@@ -322,7 +352,7 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
             auto take = [&](int64_t floats) { float* was = at; at += up(floats, 64); return was; };
             p.tiles = (p.pairs + 15) / 16;
             p.q16 = (uint8_t*) take((int64_t) p.nh * p.tiles * 16 * D / 2 * (qt == 0 ? 2 : 1));
-            p.info = (float4*) take((int64_t) p.nh * p.pairs * 4);
+            p.info = (float4*) take((int64_t) p.nh * p.pairs * 4 + 256);     // (64 pairs are read at a time)
             p.part = (float2*) take(p.nh * p.pairs * p.nb * 2);
             p.sums = p.rs > 1 ? take((int64_t) p.rs * p.nh * p.n) : nullptr;
             if (at - g->own_scratch > own) return ns_fail(w + ": more tokens and heads than the library's scratch holds");
