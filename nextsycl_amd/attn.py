@@ -251,6 +251,8 @@ class Ops:
         self._at = _addresses(self._of) if _ops_fast else None
         self._layer_of = [getattr(self.k, name, None) for name in ("norm_gated", "norm_residual", "q4_bytes", "q4_product", "ssm_step")]
         self._layer_at = _addresses(self._layer_of) if hasattr(_ops_fast, "ssm_step") else None
+        self._kv8_of = [getattr(self.k, name, None) for name in ("kv8_store", "kv8_attend_scratch", "kv8_attend")]
+        self._kv8_at = _addresses(self._kv8_of) if hasattr(_ops_fast, "kv8_store") else None
 
     def raw(self):
         return self.gpu.raw
@@ -783,7 +785,13 @@ class Ops:
 
     def kv8_store(self, cache, qt, k, ks, v, vs, T, table, tmax, S, most, lens, start=None):
         """ns_kv8_store: rows k, v [T][Hkv D] of S sequences, `most` each at most, behind their lens[s] tokens."""
-        c, e = cache, _elt(qt, "kv8_store")
+        c = cache
+        if self._kv8_at and self.k.kv8_store is self._kv8_of[0]:
+            r = _ops_fast.kv8_store(self._kv8_at[0], getattr(self.gpu, "handle", None), c.form, c.blocks, c.Hkv, c.block, c.D, c.k, c.v, c.ks, c.vs, table, tmax, S, lens,
+                                    start, qt, k, ks, v, vs, T, most)
+            if r is not False:
+                return None if r is True else self.ok(r, "kv8_store")
+        e = _elt(qt, "kv8_store")
         if T > 0:
             _need(k, ((T - 1) * ks + c.Hkv * c.D) * e, "kv8_store k")
             _need(v, ((T - 1) * vs + c.Hkv * c.D) * e, "kv8_store v")
@@ -797,7 +805,13 @@ class Ops:
 
     def kv8_attend(self, cache, qt, q, qs, T, table, tmax, S, most, longest, lens, Hq, out, scratch, start=None, win=0, scale=0.0, acc0=None, acc1=None):
         """ns_kv8_attend: T rows of S sequences, 1 to 16 each, over their cached tokens and their own; acc1 = acc0 (None: zeros) + the weights they give."""
-        c, e = cache, _elt(qt, "kv8_attend")
+        c = cache
+        if self._kv8_at and self.k.kv8_attend is self._kv8_of[2] and self.k.kv8_attend_scratch is self._kv8_of[1]:
+            r = _ops_fast.kv8_attend(self._kv8_at[1], self._kv8_at[2], getattr(self.gpu, "handle", None), c.form, c.blocks, c.Hkv, c.block, c.D, c.k, c.v, c.ks, c.vs,
+                                     table, tmax, S, lens, start, qt, q, qs, T, most, longest, Hq, out, scratch, win, scale, acc0, acc1)
+            if r is not False:
+                return None if r is True else self.ok(r, "kv8_attend")
+        e = _elt(qt, "kv8_attend")
         if T > 0:
             _need(q, ((T - 1) * qs + Hq * c.D) * e, "kv8_attend q")
             _need(out, T * Hq * c.D * e, "kv8_attend out")

@@ -1,5 +1,5 @@
 /* ops_fast.c: the size checks and the call of attn.Ops.decode / prompt / pre_store, and of a token's calls of a layer beside
- * attention (ssm_step, norm_gated, norm_residual, q4_product), in one step of native code.
+ * attention (ssm_step, norm_gated, norm_residual, q4_product) and over an 8-bit cache in blocks (kv8_store, kv8_attend), in one step of native code.
  *
  * A short context's step is a few microseconds of GPU work, and the wrappers' checks and ctypes' conversion of 18 - 28 arguments
  * took longer than a launch: a token's two calls 15.2 us, of them 10 for three launches. Each function here takes the addresses
@@ -13,6 +13,7 @@
 #include <stdint.h>
 
 #include "ns_attn.h"
+#include "ns_kv8.h"
 #include "ns_layer.h"
 #include "ns_pre.h"
 
@@ -268,6 +269,83 @@ static PyObject *fast_ssm_step(PyObject *self, PyObject *const *a, Py_ssize_t n)
     Py_RETURN_FALSE;
 }
 
+/* a Kv8's (form, blocks, Hkv, block, D, k, v, ks, vs) */
+typedef struct {
+    int64_t form, blocks, Hkv, block, D;
+    buf_t k, v, ks, vs;
+} kv8_t;
+static int get_kv8(PyObject *const *a, kv8_t *c) {
+    if (!get_size(a[0], &c->form) || !get_size(a[1], &c->blocks) || !get_size(a[2], &c->Hkv) || !get_size(a[3], &c->block) || !get_size(a[4], &c->D) ||
+        !get_buf(a[5], &c->k) || !get_buf(a[6], &c->v) || !get_buf(a[7], &c->ks) || !get_buf(a[8], &c->vs))
+        return 0;
+    if (c->Hkv > 32767 || c->block > 128 || c->D > 256) return 0;
+    const __int128 rows = (__int128) c->blocks * c->Hkv;
+    return fits(&c->k, rows * c->block * c->D) && fits(&c->v, rows * c->block * c->D) && fits(&c->ks, rows * 4) && fits(&c->vs, rows * 4);
+}
+/* the sequences: (table, tmax, S, lens, start) */
+typedef struct {
+    int64_t tmax, S;
+    buf_t table, lens, start;
+} seqs_t;
+static int get_seqs(PyObject *const *a, seqs_t *q) {
+    return get_buf(a[0], &q->table) && get_size(a[1], &q->tmax) && get_size(a[2], &q->S) && get_buf(a[3], &q->lens) && get_opt(a[4], &q->start) &&
+           fits(&q->table, (__int128) q->S * q->tmax * 4) && fits(&q->lens, (__int128) q->S * 4) && fits(&q->start, ((__int128) q->S + 1) * 4);
+}
+
+/* kv8_store(entry, handle, 9 of the cache, 5 of the sequences, qt, k, ks, v, vs, T, most) */
+static PyObject *fast_kv8_store(PyObject *self, PyObject *const *a, Py_ssize_t n) {
+    void *f, *g;
+    kv8_t c;
+    seqs_t q;
+    buf_t k, v;
+    int64_t qt, ks, vs, T, most;
+    if (n == 23 && get_address(a[0], &f) && get_address(a[1], &g) && get_kv8(a + 2, &c) && get_seqs(a + 11, &q) && get_size(a[16], &qt) && get_buf(a[17], &k) &&
+        get_size(a[18], &ks) && get_buf(a[19], &v) && get_size(a[20], &vs) && get_size(a[21], &T) && get_size(a[22], &most)) {
+        const int64_t e = elt(qt), w = c.Hkv * c.D;
+        if (e > 0 && T > 0 && holds(&k, T, ks, w, e) && holds(&v, T, vs, w, e)) {
+            __typeof__(&ns_kv8_store) call = (__typeof__(&ns_kv8_store)) f;
+            int rc;
+            Py_BEGIN_ALLOW_THREADS
+            rc = call((ns_gpu *) g, (int) c.form, (int) qt, k.ptr, ks, v.ptr, vs, T, (const int32_t *) q.start.ptr, (const int32_t *) q.lens.ptr, q.S, most,
+                      (const int32_t *) q.table.ptr, q.tmax, c.Hkv, c.D, c.block, c.blocks, c.k.ptr, c.v.ptr, (float *) c.ks.ptr, (float *) c.vs.ptr);
+            Py_END_ALLOW_THREADS
+            return made(rc);
+        }
+    }
+    Py_RETURN_FALSE;
+}
+
+/* kv8_attend(scratch entry, entry, handle, 9 of the cache, 5 of the sequences, qt, q, qs, T, most, longest, Hq, out, scratch, win, scale, acc0, acc1) */
+static PyObject *fast_kv8_attend(PyObject *self, PyObject *const *a, Py_ssize_t n) {
+    void *fs, *f, *g;
+    kv8_t c;
+    seqs_t s;
+    buf_t q, out, sc, acc0, acc1;
+    int64_t qt, qs, T, most, longest, Hq, win;
+    float scale;
+    if (n == 30 && get_address(a[0], &fs) && get_address(a[1], &f) && get_address(a[2], &g) && get_kv8(a + 3, &c) && get_seqs(a + 12, &s) && get_size(a[17], &qt) &&
+        get_buf(a[18], &q) && get_size(a[19], &qs) && get_size(a[20], &T) && get_size(a[21], &most) && get_size(a[22], &longest) && get_size(a[23], &Hq) &&
+        get_buf(a[24], &out) && get_opt(a[25], &sc) && get_size(a[26], &win) && get_float(a[27], &scale) && get_opt(a[28], &acc0) && get_opt(a[29], &acc1)) {
+        const int64_t e = elt(qt);
+        const __int128 acc = (__int128) c.blocks * c.Hkv * c.block * 4;
+        if (e > 0 && T > 0 && Hq <= 1 << 20 && holds(&q, T, qs, Hq * c.D, e) && holds3(&out, T * e, Hq, c.D) && fits(&acc0, acc) && fits(&acc1, acc)) {
+            __typeof__(&ns_kv8_attend_scratch) scratch = (__typeof__(&ns_kv8_attend_scratch)) fs;
+            __typeof__(&ns_kv8_attend) call = (__typeof__(&ns_kv8_attend)) f;
+            int rc = 0, room;
+            Py_BEGIN_ALLOW_THREADS
+            const int64_t need = scratch(s.S, most, Hq, c.Hkv, c.D, longest, acc1.ptr != NULL);
+            room = need == 0 || (sc.ptr && fits(&sc, (__int128) need * 4));
+            if (room)
+                rc = call((ns_gpu *) g, (int) c.form, (int) qt, q.ptr, qs, T, (const int32_t *) s.start.ptr, (const int32_t *) s.lens.ptr, s.S, most, longest,
+                          (const int32_t *) s.table.ptr, s.tmax, Hq, c.Hkv, c.D, c.block, c.blocks, c.k.ptr, c.v.ptr, (const float *) c.ks.ptr, (const float *) c.vs.ptr,
+                          win, scale, out.ptr, (const float *) acc0.ptr, (float *) acc1.ptr, (float *) sc.ptr);
+            Py_END_ALLOW_THREADS
+            if (room) return made(rc);
+        }
+    }
+    Py_RETURN_FALSE;
+}
+
 static PyMethodDef methods[] = {{"decode", (PyCFunction) (void (*)(void)) fast_decode, METH_FASTCALL, "attn.Ops.decode's checks and call"},
                                 {"prompt", (PyCFunction) (void (*)(void)) fast_prompt, METH_FASTCALL, "attn.Ops.prompt's checks and call"},
                                 {"pre_store", (PyCFunction) (void (*)(void)) fast_pre_store, METH_FASTCALL, "attn.Ops.pre_store's checks and call"},
@@ -275,6 +353,8 @@ static PyMethodDef methods[] = {{"decode", (PyCFunction) (void (*)(void)) fast_d
                                 {"norm_residual", (PyCFunction) (void (*)(void)) fast_norm_residual, METH_FASTCALL, "attn.Ops.norm_residual's checks and call"},
                                 {"q4_product", (PyCFunction) (void (*)(void)) fast_q4_product, METH_FASTCALL, "attn.Ops.q4_product's checks and call"},
                                 {"ssm_step", (PyCFunction) (void (*)(void)) fast_ssm_step, METH_FASTCALL, "attn.Ops.ssm_step's checks and call"},
+                                {"kv8_store", (PyCFunction) (void (*)(void)) fast_kv8_store, METH_FASTCALL, "attn.Ops.kv8_store's checks and call"},
+                                {"kv8_attend", (PyCFunction) (void (*)(void)) fast_kv8_attend, METH_FASTCALL, "attn.Ops.kv8_attend's checks and call"},
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops_fast", NULL, -1, methods, NULL, NULL, NULL, NULL};
 

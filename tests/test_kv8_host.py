@@ -133,18 +133,18 @@ class Buf:
         self.ptr, self.len = 4096, n
 
 
-def wrapped():
+def wrapped(rc=0):
     calls = []
 
     class Library:
         def symbol(self, name, restype, argtypes):
             def f(*a):
                 calls.append((name, a))
-                return 1000 if name == "ns_kv8_attend_scratch" else 0
+                return 1000 if name == "ns_kv8_attend_scratch" else rc
             return C.CFUNCTYPE(restype, *argtypes)(f)
 
         def error(self):
-            return ""
+            return "refused"
 
     return Ops(types.SimpleNamespace(raw=C.c_void_p(4096), handle=4096), Kernels(Library())), calls
 
@@ -165,8 +165,14 @@ def calls_of(ops):
 
 
 @pytest.mark.parametrize("i", range(5))
-def test_the_wrappers_check_their_buffers_to_the_byte(i):
+@pytest.mark.parametrize("native", [True, False])
+def test_the_wrappers_check_their_buffers_to_the_byte(i, native):
     ops, calls = wrapped()
+    if native:
+        pytest.importorskip("nextsycl_amd._ops_fast")
+        assert ops._kv8_at
+    else:
+        ops._kv8_at = None
     name, call, need = calls_of(ops)[i]
     call({k: Buf(n) for k, n in need.items()})
     assert [c[0] for c in calls if not c[0].endswith("scratch")] == [name]
@@ -175,6 +181,35 @@ def test_the_wrappers_check_their_buffers_to_the_byte(i):
         with pytest.raises(Error, match="bytes, needs"):
             call({k: Buf(n - (k == short)) for k, n in need.items()})
         assert not [c for c in calls if not c[0].endswith("scratch")]
+
+
+@pytest.mark.parametrize("i", [0, 1])
+@pytest.mark.parametrize("without", [(), ("start",), ("acc0", "acc1"), ("acc0",)])
+def test_the_native_step_makes_the_general_ways_call(i, without):
+    fast = pytest.importorskip("nextsycl_amd._ops_fast")
+    assert fast.kv8_store and fast.kv8_attend
+    took = []
+    for general in (False, True):
+        ops, calls = wrapped()
+        if general:
+            ops._kv8_at = None
+        name, call, need = calls_of(ops)[i]
+        at = {k: None if k in without else Buf(n) for k, n in need.items()}
+        for j, b in enumerate(at.values()):
+            if b:
+                b.ptr = 1 << 20 | j << 12
+        call(at)
+        took.append(calls)
+    assert took[0] == took[1] and len([c for c in took[0] if c[0] == name]) == 1
+
+
+def test_a_refused_call_raises_once():
+    ops, calls = wrapped(rc=-1)
+    for i, (name, call, need) in enumerate(calls_of(ops)):
+        del calls[:]
+        with pytest.raises(Error, match=name[3:] + ": refused"):
+            call({k: Buf(n) for k, n in need.items()})
+        assert [c[0] for c in calls if not c[0].endswith("scratch")] == [name]
 
 
 def test_a_pool_too_small_is_no_cache():
