@@ -14,6 +14,7 @@
  * Rows of a call: sequence s has rows start[s] .. start[s + 1] - 1 of T (start [S + 1], ascending; null: row s alone, if s < T), the
  * first `most` of them; they are its tokens lens[s], lens[s] + 1, ... (lens [S] int32: the tokens in front of the call, up to 2^30). Rows
  * of no sequence, behind a sequence's first `most`, or of one whose lens is negative or larger: passed over, outputs left as they were.
+ * Query heads: a multiple of the key heads, up to 4096 times as many.
  * Row types qt: 0 float32, 1 half, 2 bfloat16; strides in elements, at least a row long; rows may start at any element.
  * acc: float32 [blocks][Hkv][block], what each cached token has been given of the softmax weights, summed over rows and over the
  * query heads that share its key head. */
@@ -37,10 +38,10 @@ int ns_kv8_store(ns_gpu* g, int form, int qt, const void* k, int64_t ks, const v
 /* Attention of a token, or a few (most 1 .. 16), of each of S sequences, whose keys are stored already: out [T][Hq D] =
  * softmax(scale q . k) v over the tokens up to the row's own, of the last `win` (win <= 0: of all); scale <= 0: 1 / sqrt(D). `longest`: no
  * token from that position on is read (a bound that the caller knows on every lens[s] + its rows; splits and scratch follow from it).
- * Query rows and softmax weights keep 22 bits in the products. A row that sees nothing: zeros. scratch:
+ * Half and bfloat16 rows enter the products exactly and their softmax weights with 11 bits, float32 rows and theirs with 22. A row that sees nothing: zeros. scratch:
  * ns_kv8_attend_scratch(..) floats, 16-byte aligned (0: may be null).
  * acc1 not null: acc1 = acc0 + the weights of this call's rows, for every token in front of lens[s] + its rows (acc0 null, and
- * tokens of this call: 0 + them); acc1 may be acc0, and tokens shared by two sequences of a call are given the last one's. */
+ * tokens of this call: 0 + them); acc1 may be acc0. A block that is given weights belongs to one sequence of the call. */
 int64_t ns_kv8_attend_scratch(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest, int acc);
 int ns_kv8_attend(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_t T, const int32_t* start, const int32_t* lens, int64_t S, int64_t most,
                   int64_t longest, const int32_t* table, int64_t tmax, int64_t Hq, int64_t Hkv, int64_t D, int64_t block, int64_t blocks, const void* kc,

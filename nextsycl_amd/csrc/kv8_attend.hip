@@ -13,9 +13,9 @@
 //
 // A tile in the transposed orientation, as in attn_decode.hip: S^T[token][pair] = K Q^T with K's codes as halfs and the block's scale on
 // the score; online softmax in base 2, float32; O^T[d][pair] += V^T P^T with V as halfs code x scale - exactly - read by the
-// transposing 8-bit LDS read (16 lanes, 8 rows x 16 bytes: lane i gets byte i of every row). Float32 rows enter the first product
-// as two halfs, softmax weights the second one as two: 22 bits of each. Rows are brought to exponent 13 first, so that the second half of no value
-// that matters is below a half's range, and their exponent rejoins the scores' factor.
+// transposing 8-bit LDS read (16 lanes, 8 rows x 16 bytes: lane i gets byte i of every row). Rows are brought to exponent 13, which rejoins the scores'
+// factor: half and bfloat16 rows are halfs then, exactly down to 2^-27 of their largest, and float32 rows two of them. The softmax weights are rounded
+// to one half where the rows have 16 bits - a relative 2^-11 each, no more than the output's own rounding -, to two, 22 bits, where they are float32.
 #include <algorithm>
 #include <cmath>
 
@@ -26,6 +26,9 @@
 namespace {
 
 constexpr int WAVES = 4, TILE = 32, CHUNK = WAVES * TILE;
+// log2 of what a row's largest weight is in the second product, if nothing larger came since: weights lie up to 2^15, a half's range ends above that, and
+// its steps begin to widen for those under 2^-14: 2^-21 to 2^-29 of the largest
+constexpr float LIFT = 7.0f;
 
 struct AttendParams {
     Kv8Cache c;
@@ -60,9 +63,13 @@ __device__ __forceinline__ void span_of(const AttendParams& p, const Kv8Seq& q, 
 
 // (a 64-bit division takes some hundred instructions, a 32-bit one a few tens)
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return (a | b) >> 31 ? a / b : (int64_t) ((uint32_t) a / (uint32_t) b); }
-// the row of a pair (fewer than 2^31 / G of them)
+// the row of a pair (16 G of them, G up to 4096: pair x G under 2^32)
 __device__ __forceinline__ int row_of(const AttendParams& p, int pair) { return p.G == 1 ? pair : (int) __umulhi((uint32_t) pair, p.ginv); }
 
+// What a unit - a sequence's key head - costs besides its chunks, in chunks: its rows' way in, its sums' way out (2.2 us, where a chunk's bytes take
+// 4 of a full chip's). Runs are dealt by chunks and that where there are more chunks than work-groups. (64 sequences of 125 to 8000 tokens x 8 heads: 63.7 us
+// without it, 57.7 with 1, 57.8 with 2, 58.8 with 3; 4 rows of 3 sequences behind 43003 44.8 / 44.8 / 42.6 / 42.7)
+constexpr int EXTRA = 2;
 // a sequence's chunks a key head: chunk `first` and on (a sequence with rows has one at least)
 __device__ __forceinline__ int chunks_of(const AttendParams& p, const Kv8Seq& q, int& first) {
     int64_t lo, hi;
@@ -97,19 +104,31 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
     asm volatile("" ::"s"(p.c.kc), "s"(p.c.vc), "s"(p.c.ksc), "s"(p.c.vsc), "s"(p.c.table), "s"(p.c.tmax), "s"(p.c.blocks), "s"(p.c.shift), "s"(p.q), "s"(p.qs), "s"(p.start), "s"(p.lens),
                  "s"(p.T), "s"(p.longest), "s"(p.win), "s"(p.sl2), "s"(p.ginv), "s"(p.nw));
     // ---- this work-group's run of chunks: `left` of them, from the `rest`th of sequence s on (its heads one behind the other)
-    int s = 0, left, first, nch;
-    int64_t rest, run;
+    int s = 0, first, nch, extra;
+    int64_t rest, run, left;
     Kv8Seq q;
     {
-        int64_t total;
+        // (chunks of a key head, and sequences that have some in bits 40 and up: both sums at once)
+        constexpr int64_t ONE = (int64_t) 1 << 40;
+        auto chunks = [](int64_t x) { return x & (ONE - 1); };
+        auto deal = [&](int64_t all) {
+            extra = chunks(all) * Hkv <= p.nw ? 0 : EXTRA;
+            const int64_t total = (chunks(all) + (all >> 40) * extra) * Hkv;
+            run = quotient(total + p.nw - 1, p.nw);
+            rest = wg * run;
+            left = std::max<int64_t>(0, std::min(run, total - rest));
+        };
         if (p.S == 1) {
             q = seq_of(p, 0);
-            total = nch = chunks_of(p, q, first);
+            nch = chunks_of(p, q, first);
+            deal(nch ? nch + ONE : 0);
+            if (left <= 0) return;
         } else {
             const int per = (p.S + WAVES * 64 - 1) / (WAVES * 64), s0 = std::min(tid * per, p.S), s1 = std::min(s0 + per, p.S);
             int64_t mine = 0;
             int its;                                              // (a sequence's first chunk)
-            for (int i = s0; i < s1; ++i) mine += chunks_of(p, seq_of(p, i), its);
+            auto some = [&](int i) { const int c = chunks_of(p, seq_of(p, i), its); return c ? c + ONE : 0; };
+            for (int i = s0; i < s1; ++i) mine += some(i);
             int64_t x = mine;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
@@ -118,33 +137,27 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
             }
             if (lane == 63) sums[w] = x;
             __syncthreads();
-            int64_t before = x - mine;
-            total = 0;
+            int64_t before = x - mine, all = 0;
 #pragma unroll
             for (int i = 0; i < WAVES; ++i) {
                 const int64_t y = sums[i];
                 if (i < w) before += y;
-                total += y;
+                all += y;
             }
-            const int64_t from = wg * quotient(total * Hkv + p.nw - 1, p.nw);
-            if (before * Hkv <= from && from < (before + mine) * Hkv) {
-                int64_t b = before;
+            deal(all);
+            if (left <= 0) return;
+            auto cost = [&](int64_t x) { return (chunks(x) + (x >> 40) * extra) * Hkv; };
+            if (cost(before) <= rest && rest < cost(before + mine)) {
                 for (int i = s0; i < s1; ++i) {
-                    const int64_t y = chunks_of(p, seq_of(p, i), its);
-                    if (from < (b + y) * Hkv) {
-                        found[0] = i, found[1] = from - b * Hkv;
+                    const int64_t y = some(i);
+                    if (rest < cost(before + y)) {
+                        found[0] = i, found[1] = rest - cost(before);
                         break;
                     }
-                    b += y;
+                    before += y;
                 }
             }
             __syncthreads();
-        }
-        run = quotient(total * Hkv + p.nw - 1, p.nw);
-        rest = wg * run;
-        if (rest >= total * Hkv) return;
-        left = (int) std::min(run, total * Hkv - rest);
-        if (p.S > 1) {
             s = __builtin_amdgcn_readfirstlane((int) found[0]), rest = found[1];
             q = seq_of(p, s);
             nch = chunks_of(p, q, first);
@@ -166,9 +179,10 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
         // ---- a piece of the run: chunks c0 .. c1 - 1 of one unit
         int64_t lo, hi;
         span_of(p, q, lo, hi);
-        const int hk = (int) quotient(rest, nch), c0 = (int) (rest - (int64_t) hk * nch), c1 = std::min(nch, c0 + left);
+        const int cost = nch + extra, hk = (int) quotient(rest, cost), from = (int) (rest - (int64_t) hk * cost), to = (int) std::min<int64_t>(cost, from + left);
+        const int c0 = std::max(from - extra, 0), c1 = to - extra;
         const int pairs = q.n * p.G, pair0 = z * RT * 16;
-        if (pair0 < pairs) {
+        if (pair0 < pairs && c1 > c0) {
             // from here on tokens are counted from the piece's first
             const int64_t j0 = (int64_t) (first + c0) * CHUNK;
             const int jb = (int) (std::max(j0, lo) - j0), je = (int) (std::min(j0 + (int64_t) (c1 - c0) * CHUNK, hi) - j0), pos0 = (int) std::max<int64_t>(q.len - j0, -(1 << 30));
@@ -261,7 +275,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                     }
             }
 
-            // m: what a row's weights are taken against - moved where a score is past it by more than 2^8 -, l: this lane's part of their sum
+            // m: what a row's weights are taken against, LIFT under the largest score it was moved to - moved where a weight would be past a half's range;
+            // l: this lane's part of their sum
             float m[RT], l[RT];
             f4v o[RT][DT];
 #pragma unroll
@@ -343,8 +358,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
 #pragma unroll
                             for (int i = 0; i < 8; ++i) kept[rt][i] = x[i];
                         const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                        if (__builtin_amdgcn_ballot_w64(top > m[rt] + 8.0f)) {
-                            const float m1 = fmaxf(m[rt], rows_max(top)), c = m1 == -INFINITY ? 1.0f : fast_exp2(m[rt] - m1);
+                        if (__builtin_amdgcn_ballot_w64(top > m[rt] + 15.0f)) {
+                            const float m1 = fmaxf(m[rt], rows_max(top) - LIFT), c = m1 == -INFINITY ? 1.0f : fast_exp2(m[rt] - m1);
                             m[rt] = m1;
                             l[rt] *= c;
 #pragma unroll
@@ -450,12 +465,12 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                     if (d == 0) to[D] = top, to[D + 1] = all;
                 }
             }
-            if (z == 0 && c0 == 0 && tid == 0 && p.units) p.units[unit] = int2{wg, whole ? wg : wg + (int) quotient(nch - left + run - 1, run)};
+            if (z == 0 && c0 == 0 && tid == 0 && p.units) p.units[unit] = int2{wg, whole ? wg : wg + (int) quotient(cost - to + run - 1, run)};
         }
-        left -= c1 - c0;
+        left -= to - from;
         if (left <= 0) break;
-        rest += c1 - c0;
-        if (rest >= (int64_t) nch * Hkv) {
+        rest += to - from;
+        if (rest >= (int64_t) cost * Hkv) {
             rest = 0;
             do q = seq_of(p, ++s), nch = chunks_of(p, q, first);
             while (nch == 0 && s < p.S - 1);
@@ -574,7 +589,7 @@ int64_t pair_chunks(int64_t pairs, int64_t D) { const int64_t rows = 16 * tiles_
 // 256, two chunks of pairs: 128 pairs of work-groups 42, 256 37, 384 46)
 int64_t workgroups(int64_t S, int64_t pairs, int64_t Hkv, int64_t D, int64_t longest) {
     const int64_t places = D == 128 && tiles_of(pairs, D) == 1 ? 768 : 512;
-    return std::min(std::max<int64_t>(1, places / pair_chunks(pairs, D)), S * Hkv * ((longest + CHUNK - 1) / CHUNK + 1));
+    return std::min(std::max<int64_t>(1, places / pair_chunks(pairs, D)), S * Hkv * ((longest + CHUNK - 1) / CHUNK + 1 + EXTRA));
 }
 
 struct Scratch {
@@ -591,7 +606,7 @@ Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, 
     return x;
 }
 bool sizes_fit(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest) {
-    return S > 0 && S <= 65535 && most > 0 && most <= DECODE_ROWS && Hkv > 0 && Hkv <= 32767 && Hq > 0 && Hq <= 1 << 20 && Hq % Hkv == 0 && (D == 128 || D == 256) && longest > 0 &&
+    return S > 0 && S <= 65535 && most > 0 && most <= DECODE_ROWS && Hkv > 0 && Hkv <= 32767 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= KV8_HEADS && (D == 128 || D == 256) && longest > 0 &&
            longest <= 2 * (int64_t) KV8_TOKENS;
 }
 
@@ -648,7 +663,7 @@ int ns_kv8_attend(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     p.c = kv8_cache(kc, vc, ksc, vsc, table, tmax, Hkv, D, block, blocks);
     if (qt < 0 || qt > 2) return ns_fail(w + ": rows of type 0 (float32), 1 (half) or 2 (bfloat16)");
     if (ns_kv8_check(w, form, Hkv, D, block, blocks, S, tmax, p.c)) return -1;
-    if (Hq <= 0 || Hq % Hkv || Hq > 1 << 20) return ns_fail(w + ": query heads a multiple of the key heads");
+    if (Hq <= 0 || Hq % Hkv || Hq / Hkv > KV8_HEADS) return ns_fail(w + ": query heads a multiple of the key heads, up to 4096 times");
     if (most > DECODE_ROWS) return ns_fail(w + ": 1 to 16 rows a sequence");
     if (T > KV8_TOKENS) return ns_fail(w + ": up to 2^30 rows");
     if (longest <= 0 || longest > 2 * (int64_t) KV8_TOKENS) return ns_fail(w + ": contexts of 1 to 2^31 tokens");
@@ -658,7 +673,7 @@ int ns_kv8_attend(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     const int64_t need = scratch_of(S, p.most, Hq, Hkv, D, longest, acc1 != nullptr).all();
     if (!g || !q || !lens || !vc || !vsc || !out || (need && !scratch)) return ns_fail(w + ": a null buffer");
     if (need && (uintptr_t) scratch % 16) return ns_fail(w + ": scratch 16-byte aligned");
-    p.q = q, p.qs = qs, p.start = start, p.lens = lens, p.win = win, p.out = out, p.acc0 = acc0, p.acc1 = acc1;
+    p.q = q, p.qs = qs, p.start = start, p.lens = lens, p.win = kv8_window(win), p.out = out, p.acc0 = acc0, p.acc1 = acc1;
     p.sl2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float) D)) * 1.4426950408889634f;
     NS_HIP(hipSetDevice(g->dev));
     return attend(g, w, form, qt, p, Hkv, D, scratch);
@@ -674,7 +689,7 @@ int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     Kv8Cache c = kv8_cache(kc, vc, ksc, vsc, table, tmax, Hkv, D, block, blocks);
     if (qt < 0 || qt > 2) return ns_fail(w + ": rows of type 0 (float32), 1 (half) or 2 (bfloat16)");
     if (ns_kv8_check(w, form, Hkv, D, block, blocks, 1, tmax, c)) return -1;
-    if (Hq <= 0 || Hq % Hkv || Hq > 1 << 20) return ns_fail(w + ": query heads a multiple of the key heads");
+    if (Hq <= 0 || Hq % Hkv || Hq / Hkv > KV8_HEADS) return ns_fail(w + ": query heads a multiple of the key heads, up to 4096 times");
     if (p0 < 0 || p0 > KV8_TOKENS || T > KV8_TOKENS) return ns_fail(w + ": positions of 0 to 2^30, up to 2^30 rows");
     if (qs < Hq * D) return ns_fail(w + ": rows at least as far apart as they are long");
     if (!g || !q || !vc || !vsc || !out) return ns_fail(w + ": a null buffer");
@@ -693,7 +708,7 @@ int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
                                   (own - wide) / 64 * 64);
     }
     AttendParams p{};
-    p.c = c, p.qs = qs, p.S = 1, p.Hq = (int) Hq, p.G = (int) (Hq / Hkv), p.win = win;
+    p.c = c, p.qs = qs, p.S = 1, p.Hq = (int) Hq, p.G = (int) (Hq / Hkv), p.win = kv8_window(win);
     p.sl2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float) D)) * 1.4426950408889634f;
     for (int64_t t = 0; t < T; t += DECODE_ROWS) {
         const int64_t rows = std::min(DECODE_ROWS, T - t);

@@ -12,6 +12,7 @@
 #include "ns_kv8.h"
 
 constexpr int KV8_TOKENS = 1 << 30;     // of a sequence, at most
+constexpr int KV8_HEADS = 4096;         // query heads a key head, at most
 
 // the pools of one cache, and the sequences' tables
 struct Kv8Cache {
@@ -120,6 +121,8 @@ __device__ __forceinline__ s8v kv8_halfs8(uint32_t w0, uint32_t w1) {
 }
 
 // ---- host side
+// a window as the kernels count it: 0 where it is none, no longer than any sequence
+inline int64_t kv8_window(int64_t win) { return win <= 0 ? 0 : win < 2 * (int64_t) KV8_TOKENS ? win : 2 * (int64_t) KV8_TOKENS; }
 // what every call over a cache refuses; 0 or -1
 int ns_kv8_check(const std::string& who, int form, int64_t Hkv, int64_t D, int64_t block, int64_t blocks, int64_t S, int64_t tmax, const Kv8Cache& c);
 inline Kv8Cache kv8_cache(const void* kc, const void* vc, const float* ksc, const float* vsc, const int32_t* table, int64_t tmax, int64_t Hkv, int64_t D, int64_t block,

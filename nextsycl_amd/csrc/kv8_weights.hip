@@ -323,7 +323,7 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
     p.c = kv8_cache(kc, nullptr, ksc, nullptr, table, tmax, Hkv, D, block, blocks);
     if (qt < 0 || qt > 2) return ns_fail(w + ": rows of type 0 (float32), 1 (half) or 2 (bfloat16)");
     if (ns_kv8_check(w, form, Hkv, D, block, blocks, 1, tmax, p.c)) return -1;
-    if (Hq <= 0 || Hq % Hkv || Hq > 1 << 20) return ns_fail(w + ": query heads a multiple of the key heads");
+    if (Hq <= 0 || Hq % Hkv || Hq / Hkv > KV8_HEADS) return ns_fail(w + ": query heads a multiple of the key heads, up to 4096 times");
     if (p0 < 0 || p0 > KV8_TOKENS || T > KV8_TOKENS) return ns_fail(w + ": positions of 0 to 2^30, up to 2^30 rows");
     if (qs < Hq * D) return ns_fail(w + ": rows at least as far apart as they are long");
     if (!g || !q || !acc1) return ns_fail(w + ": a null buffer");
@@ -336,7 +336,7 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
     const int64_t nh0 = std::min(Hkv, own / (per + sums));
     if (nh0 < 1) return ns_fail(w + ": more tokens and heads than the library's scratch holds");
     const int64_t rows = std::min({T, (own / nh0 - sums) / per, std::max<int64_t>(1, ((int64_t) 1 << 31) / (G * G) - 64)});
-    p.G = (int) G, p.ginv = (uint32_t) ((((int64_t) 1 << 32) + G - 1) / G), p.qs = qs, p.win = win > 0 ? win : 0;
+    p.G = (int) G, p.ginv = (uint32_t) ((((int64_t) 1 << 32) + G - 1) / G), p.qs = qs, p.win = kv8_window(win);
     p.sl2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float) D)) * 1.4426950408889634f;
     for (int64_t h = 0; h < Hkv; h += nh0) {
         p.h0 = (int) h, p.nh = (int) std::min(nh0, Hkv - h);

@@ -190,6 +190,11 @@ def tolerance(qt, ref, reach, vmax, D, n):
     """(absolute, relative L2) for rows against the closed form. reach: the largest sum of |q k| scale log2 e of a row and a token. A score carries 22
     bits of each product and a sum of D of them in float32, an exponential's and a weight's roundings 2^-22 and 2^-23; a weighted mean of values up to
     vmax moves by twice the largest relative error of a weight, and its own sum over n tokens in steps of 32 by a rounding each.
-    In the mean these add as squares: sqrt(D) of them for a score of the scale sqrt(mean) ~ 3, far below 2^-17."""
+    In the mean these add as squares: sqrt(D) of them for a score of the scale sqrt(mean) ~ 3, far below 2^-17.
+    Beside rows of 16 bits a weight's numerator is a half, not its sum: out = sum w (1 + d) v / sum w, |d| <= 2^-11, moves by vmax 2^-11 at most; weights
+    under 2^-21 of the row's largest, d up to a half's least step against them, 2^-25 of 2^7 x the largest: by n 2^-32 vmax at most. In the mean d's
+    signs are as random as v's: sqrt(sum (w d v)^2) <= 2^-11 sqrt(sum (w v)^2), which is 2^-11 of what the output comes to."""
     weight = np.log(2.0) * reach * (2.0 ** -22 + D * 2.0 ** -24) + 2.0 ** -21
-    return vmax * (2 * weight + (n / 32 + 8) * 2.0 ** -24) + ROUND[qt] * np.abs(ref).max() + (2.0 ** -25 if qt == F16 else 0.0), 2.0 ** -17 + ROUND[qt]
+    half = 0.0 if qt == F32 else 2.0 ** -11
+    return (vmax * (2 * weight + (n / 32 + 8) * 2.0 ** -24 + half + (n * 2.0 ** -32 if half else 0.0)) + ROUND[qt] * np.abs(ref).max() +
+            (2.0 ** -25 if qt == F16 else 0.0), 2.0 ** -17 + half + ROUND[qt])
