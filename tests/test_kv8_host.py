@@ -73,6 +73,15 @@ def test_refusals(lib, name, good, bad):
         assert said.startswith(name + ": ") and (said != name + ": a null buffer" or None in change.values() or wants_scratch), (change, said)
 
 
+@pytest.mark.parametrize("name,good", [("ns_kv8_attend", ATTEND), ("ns_kv8_prompt", PROMPT), ("ns_kv8_weights", WEIGHTS)])
+def test_query_heads_a_key_head(lib, name, good):
+    """Up to 4096 of them; more are refused (a pair's row is found by a 32-bit product)."""
+    for G, said in ((4096, ": a null buffer"), (4097, ": query heads a multiple of the key heads, up to 4096 times")):
+        assert getattr(lib, name)(*{**good, "Hq": 2 * G, "qs": 2 * G * 128}.values()) == -1
+        assert lib.ns_last_error().decode() == name + said
+    assert lib.ns_kv8_attend_scratch(1, 1, 4096, 1, 128, 1000, 0) > 0 and lib.ns_kv8_attend_scratch(1, 1, 4097, 1, 128, 1000, 0) == 0
+
+
 @pytest.mark.parametrize("name,good,none", [("ns_kv8_store", STORE, dict(T=0)), ("ns_kv8_store", STORE, dict(S=0)), ("ns_kv8_attend", ATTEND, dict(T=0)), ("ns_kv8_attend", ATTEND, dict(most=0)),
                                             ("ns_kv8_prompt", PROMPT, dict(T=0)), ("ns_kv8_weights", WEIGHTS, dict(T=0)), ("ns_kv8_evict", EVICT, dict(S=0))])
 def test_nothing_to_do_is_no_call(lib, name, good, none):
