@@ -64,7 +64,8 @@ int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64
  * order and move to tokens 0 .. keep - 1, acc with them. to null: within the sequence's own blocks, by way of the library's
  * scratch; else into the blocks of `to` [S][tmax], none of which may be a block that the call reads - sequences that stay as long as they are move too. A
  * block's scale becomes the largest of those its tokens come with, codes re-rounded as a store does. lens1 [S] = min(lens, keep)
- * (may be lens; sequences of negative lens: lens). No length is over `longest`, up to 2^30 (a longer sequence is passed over, its lens1 = lens). */
+ * (may be lens; sequences of negative lens: lens). No length is over `longest`, up to 2^30 (a longer sequence is passed over, its lens1 = lens); pools of
+ * fewer than 2^32 rows, blocks x Hkv x block. */
 int ns_kv8_evict(ns_gpu* g, int form, const int32_t* lens, int32_t* lens1, int64_t S, int64_t longest, int64_t keep, int64_t first, int64_t last,
                  const int32_t* table, const int32_t* to, int64_t tmax, int64_t Hkv, int64_t D, int64_t block, int64_t blocks, void* kc, void* vc,
                  float* ksc, float* vsc, float* acc);

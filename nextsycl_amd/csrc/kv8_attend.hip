@@ -480,42 +480,59 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
     }
 }
 
-// out = sum over a unit's pieces of O 2^(m - M) / sum of l 2^(m - M): a work-group a (sequence, key head, pair), D / 4 threads x 256 / (D / 4)
-// pieces at a time in a fixed shape. The first piece lies in its work-group's second place, the others in their first
-template <int D, int QT>
-__global__ __launch_bounds__(256) void kv8_merge_kernel(const AttendParams p) {
-    constexpr int L = D / 4, SG = 256 / L;
+// out = sum over a unit's pieces of O 2^(m - M) / sum of l 2^(m - M): a work-group a (sequence, key head, pair), D / 4 threads x SG
+// pieces at a time in a fixed shape, each of them against the largest m of its own. The first piece lies in its work-group's second place, the others in their first
+template <int D, int QT, int TH>
+__global__ __launch_bounds__(TH) void kv8_merge_kernel(const AttendParams p) {
+    constexpr int L = D / 4, SG = TH / L, U = 8;
     __shared__ __attribute__((aligned(16))) float sums[SG][D];
-    __shared__ float wsum[SG];
-    const int tid = threadIdx.x, lane = tid & 63;
+    __shared__ float2 ml[SG];
+    const int tid = threadIdx.x;
     const int64_t place = blockIdx.x, unit = place / (p.most * p.G);
     const int pair = (int) (place - unit * p.most * p.G), s = (int) (unit / p.c.Hkv), hk = (int) (unit - (int64_t) s * p.c.Hkv);
     const int2 ws = p.units[unit];
     const Kv8Seq q = seq_of(p, s);
     if (pair >= q.n * p.G || ws.x == ws.y) return;
-    auto piece = [&](int k) { return p.part + (((int64_t) (ws.x + k) * 2 + (k == 0)) * p.most * p.G + pair) * (D + 4); };
-    const int count = ws.y - ws.x + 1;
-    float top = -INFINITY;
-    for (int k = lane; k < count; k += 64) top = fmaxf(top, piece(k)[D]);
-    top = wave_max(top);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    const int sg = tid / L, d = tid % L * 4;
+    const int64_t row = (int64_t) p.most * p.G * (D + 4);
+    const float* first = p.part + (int64_t) ws.x * 2 * row + pair * (D + 4);
+    const int count = ws.y - ws.x + 1, sg = tid / L, d = tid % L * 4;
+    float m = -INFINITY, l = 0.0f;
     f4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    float all = 0.0f;
-#pragma unroll 4
-    for (int k = sg; k < count; k += SG) {
-        const float* at = piece(k);
-        const float c = fast_exp2(at[D] - ref);
-        all += at[D + 1] * c;
-        sum += *reinterpret_cast<const f4v*>(at + d) * c;
+    for (int k0 = sg; k0 < count; k0 += SG * U) {
+        f4v o[U];
+        float2 x[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int k = std::min(k0 + i * SG, count - 1);
+            const float* at = first + (2 * (int64_t) k + (k == 0)) * row;
+            o[i] = *reinterpret_cast<const f4v*>(at + d), x[i] = *reinterpret_cast<const float2*>(at + D);
+            if (k0 + i * SG >= count) x[i].x = -INFINITY;
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < U; ++i) top = fmaxf(top, x[i].x);
+        const float ref = top == -INFINITY ? 0.0f : top, c0 = fast_exp2(m - ref);
+        sum *= c0, l *= c0, m = top;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const float c = fast_exp2(x[i].x - ref);
+            if (k0 + i * SG < count) sum += o[i] * c, l += x[i].y * c;
+        }
     }
     *reinterpret_cast<f4v*>(&sums[sg][d]) = sum;
-    if (d == 0) wsum[sg] = all;
+    if (d == 0) ml[sg] = float2{m, l};
     __syncthreads();
     if (tid >= L) return;
-    sum = f4v{0.0f, 0.0f, 0.0f, 0.0f}, all = 0.0f;
-#pragma unroll
-    for (int k = 0; k < SG; ++k) sum += *reinterpret_cast<const f4v*>(&sums[k][d]), all += wsum[k];
+    float top = -INFINITY, all = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < SG; ++k) top = fmaxf(top, ml[k].x);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    sum = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int k = 0; k < SG; ++k) {
+        const float c = fast_exp2(ml[k].x - ref);
+        sum += *reinterpret_cast<const f4v*>(&sums[k][d]) * c, all += ml[k].y * c;
+    }
     const float inv = all == 0.0f ? 0.0f : 1.0f / all;
     const int i = row_of(p, pair), g = pair - i * p.G;
     const int64_t at = ((int64_t) (q.first + i) * p.Hq + hk * p.G + g) * D + d;
@@ -551,7 +568,7 @@ __global__ __launch_bounds__(256) void kv8_given_kernel(const AttendParams p) {
         for (int i = 0; i < q.n; ++i) {
             const int64_t pos = (int64_t) q.len + i;
             if (t0 > pos || (p.win > 0 && t0 + 3 + p.win <= pos)) continue;
-#pragma unroll 4
+#pragma unroll 8
             for (int g = 0; g < p.G; ++g) {
                 const int pair = i * p.G + g;
                 const f4v x = *reinterpret_cast<const f4v*>(scores + (int64_t) pair * p.pad);
@@ -577,8 +594,12 @@ void launch_attend(ns_gpu* g, int form, const AttendParams& p, int64_t D, int RT
     if (D == 128) RT == 1 ? launch_attend<128, 1, QT>(g, form, p, grid) : launch_attend<128, 2, QT>(g, form, p, grid);
     else launch_attend<256, 1, QT>(g, form, p, grid);
 }
+// (1024 threads a pair where a unit may be in more pieces than 256 take in one round)
 template <int D, int QT>
-void launch_merge(ns_gpu* g, const AttendParams& p, int64_t rows) { kv8_merge_kernel<D, QT><<<(unsigned) rows, 256, 0, g->q>>>(p); }
+void launch_merge(ns_gpu* g, const AttendParams& p, int64_t rows) {
+    if (p.nw > (int64_t) p.S * p.c.Hkv * 8 * (1024 / D)) kv8_merge_kernel<D, QT, 1024><<<(unsigned) rows, 1024, 0, g->q>>>(p);
+    else kv8_merge_kernel<D, QT, 256><<<(unsigned) rows, 256, 0, g->q>>>(p);
+}
 
 // 16-pair tiles a wave: two where more than 16 pairs share a key head of 128 (heads of 256 have no registers for a second: 16 pairs a work-group,
 // the next ones read the tokens from L2)

@@ -61,7 +61,7 @@ QUERY = [dict(Hq=3), dict(Hq=0), dict(Hq=1 << 21), dict(qs=511), dict(q=None)]
     ("ns_kv8_prompt", PROMPT, CACHE + ROWS + QUERY + [dict(p0=-1), dict(p0=1 << 31), dict(T=1 << 31), dict(out=None), dict(vc=None), dict(vsc=None)]),
     ("ns_kv8_weights", WEIGHTS, CACHE + ROWS + QUERY + [dict(p0=-1), dict(p0=1 << 31), dict(T=1 << 31), dict(acc1=None)]),
     ("ns_kv8_evict", EVICT, CACHE + SEQS + [dict(keep=0), dict(first=-1), dict(last=-1), dict(first=9), dict(last=10), dict(first=11), dict(longest=0), dict(longest=1 << 31), dict(lens=None),
-                                            dict(lens1=None), dict(acc=None), dict(vc=None), dict(vsc=None)]),
+                                            dict(blocks=1 << 27), dict(lens1=None), dict(acc=None), dict(vc=None), dict(vsc=None)]),
 ])
 def test_refusals(lib, name, good, bad):
     f = getattr(lib, name)
