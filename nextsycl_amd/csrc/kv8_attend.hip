@@ -192,7 +192,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int e = i * 64 + lane;
-                    blk[i] = at + (e << p.c.shift) < je ? kv8_block(p.c, p.c.table, s, ((j0 + at) >> p.c.shift) + e) : -1;
+                    blk[i] = kv8_block(p.c, p.c.table, s, ((j0 + at) >> p.c.shift) + e);
+                    if (at + (e << p.c.shift) >= je) blk[i] = -1;
                 }
             };
             auto scales = [&]() __attribute__((always_inline)) {

@@ -22,11 +22,11 @@ struct Kv8Cache {
     int64_t tmax, blocks;
     int Hkv, D, block, shift;    // block = 1 << shift tokens
 };
-// the block of entry e of a sequence's table, or -1
+// the block of entry e of a sequence's table, or -1. (Some entry is read whatever e is: several of these in a row are under way together, where a
+// branch around each would wait for the one in front)
 __device__ __forceinline__ int kv8_block(const Kv8Cache& c, const int32_t* table, int64_t seq, int64_t e) {
-    if (e < 0 || e >= c.tmax) return -1;
-    const int b = table[seq * c.tmax + e];
-    return b >= 0 && b < c.blocks ? b : -1;
+    const uint32_t b = (uint32_t) table[seq * c.tmax + (e < 0 ? 0 : e < c.tmax ? e : c.tmax - 1)];
+    return b < (uint32_t) c.blocks && e >= 0 && e < c.tmax ? (int) b : -1;
 }
 // where block b's rows of head h begin, in rows
 __device__ __forceinline__ int64_t kv8_rows(const Kv8Cache& c, int b, int h) { return ((int64_t) b * c.Hkv + h) * c.block; }

@@ -78,6 +78,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const WeightsParams p) {
     if (li == 0 && pair < p.pairs) p.info[(int64_t) h * p.pairs + pair].x = p.sl2 * kv8_pow2(e);
 }
 
+constexpr int RS = 16;                            // splits of the pairs, at most
 constexpr int KT = 4, RUN = 16 * KT;              // tiles of 16 tokens a wave; tokens
 
 __device__ __forceinline__ void give(const WeightsParams& p, int h, int64_t t, float sum) {
@@ -115,10 +116,17 @@ __global__ __launch_bounds__(256, 2) void kv8_pass_kernel(const WeightsParams p)
     if (a0 + 16 * TG < a1) ask(a0 + 16 * TG, 1);
     // ---- the tokens
     s8v k[KT][KB];
+    int blk[KT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
         const int64_t t = key0 + kt * 16 + n;
-        const int b = t < p.n ? kv8_block(p.c, p.c.table, 0, t >> p.c.shift) : -1;
+        blk[kt] = kv8_block(p.c, p.c.table, 0, t >> p.c.shift);
+        if (t >= p.n) blk[kt] = -1;
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        const int64_t t = key0 + kt * 16 + n;
+        const int b = blk[kt];
         const uint8_t* row = p.c.kc + (kv8_rows(p.c, std::max(b, 0), p.h0 + h) + (t & (p.c.block - 1))) * D + 16 * g4;
         const float sc = p.c.ksc[(int64_t) std::max(b, 0) * p.c.Hkv + p.h0 + h];
 #pragma unroll
@@ -284,8 +292,11 @@ __global__ __launch_bounds__(256) void kv8_columns_join_kernel(const WeightsPara
     const int64_t t = (int64_t) blockIdx.x * 256 + threadIdx.x;
     const int h = blockIdx.y;
     if (t >= p.n) return;
-    float sum = 0.0f;
-    for (int r = 0; r < p.rs; ++r) sum += p.sums[((int64_t) r * p.nh + h) * p.n + t];
+    float v[RS], sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < RS; ++r) v[r] = r < p.rs ? p.sums[((int64_t) r * p.nh + h) * p.n + t] : 0.0f;
+#pragma unroll
+    for (int r = 0; r < RS; ++r) sum += v[r];
     give(p, h, t, sum);
 }
 
@@ -331,7 +342,6 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
     NS_OWN_SCRATCH(g);
     const int64_t own = (int64_t) ns_own_floats(g), G = Hq / Hkv, e = qt == 0 ? 4 : 2;
     // as many rows as the scratch holds - a pair its halfs, its four numbers, its two for each 64 tokens -, else fewer key heads at a time
-    constexpr int64_t RS = 16;                                    // splits of the pairs, at most
     const int64_t runs = (p0 + T + RUN - 1) / RUN, per = G * (D / 2 * (qt == 0 ? 2 : 1) + 4 + 2 * runs), sums = RS * (p0 + T) + 16 * D + 1024;
     const int64_t nh0 = std::min(Hkv, own / (per + sums));
     if (nh0 < 1) return ns_fail(w + ": more tokens and heads than the library's scratch holds");
@@ -345,7 +355,7 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
             p.q = (const uint8_t*) q + r * qs * e, p.acc0 = r ? acc1 : acc0, p.acc1 = acc1;
             // work-groups for the chip's places, two a CU, twice; splits of 64 pairs and more
             p.nb = (p.n + RUN - 1) / RUN;
-            const int64_t blocks = (p.nb + 3) / 4 * p.nh, rs = std::max<int64_t>(1, std::min<int64_t>({(1024 + blocks - 1) / blocks, RS, (int64_t) (p.pairs + 63) / 64}));
+            const int64_t blocks = (p.nb + 3) / 4 * p.nh, rs = std::max<int64_t>(1, std::min<int64_t>({(1024 + blocks - 1) / blocks, (int64_t) RS, (int64_t) (p.pairs + 63) / 64}));
             p.prs = (int) up((p.pairs + rs - 1) / rs, 64), p.rs = (p.pairs + p.prs - 1) / p.prs;
             if (!ns_grid_fits(blocks * p.rs, 256) || !ns_grid_fits((p.pairs + 15) / 16, 256)) return ns_fail(w + ": more work-groups than a launch takes");
             float* at = g->own_scratch;
