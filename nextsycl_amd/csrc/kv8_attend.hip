@@ -42,10 +42,11 @@ struct AttendParams {
     int nw, nz;                 // work-groups the chunks are dealt to; chunks of pairs
     float sl2;                  // scale x log2(e)
     void* out;
-    float* part;                // [nw][2][most G] x (D + 4): O, m, l, -, - of a run that begins inside a unit; of one that ends in it
+    float* part;                // [nw][2][most G][D]: O of a run that begins inside a unit; of one that ends in it
+    float2* ml;                 // [nw][2][most G]: its m, l
     int2* units;                // [S][Hkv]: the first and the last work-group with tokens of a unit
     float* scores;              // [S][Hkv][most G][pad]: scores in log2 units, or null
-    float* stats;               // [S][Hkv][most G][2]: a pair's largest score and its sum, or null
+    float2* stats;              // [S][Hkv][most G]: the largest score and 1 / sum of a pair whose unit is in one piece, or null
     int64_t pad;
     const float* acc0;
     float* acc1;
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
             __syncthreads();
             const bool whole = c0 == 0 && c1 == nch;
             const int64_t unit = (int64_t) s * Hkv + hk;
-            float* part = p.part + ((int64_t) wg * 2 + (c0 == 0)) * p.most * p.G * (D + 4);
+            const int64_t piece = ((int64_t) wg * 2 + (c0 == 0)) * p.most * p.G;
             for (int i = tid; i < RT * 16 * (D / 4); i += WAVES * 64) {
                 const int row = i / (D / 4), d = i % (D / 4) * 4, pair = pair0 + row;
                 if (pair >= pairs) break;
@@ -459,11 +460,10 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                     const int64_t at = ((int64_t) (q.first + i2) * p.Hq + hk * p.G + g) * D + d;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) store_o<QT>(p.out, at + k, v[k]);
-                    if (p.stats && d == 0) p.stats[2 * (unit * p.most * p.G + pair)] = ref, p.stats[2 * (unit * p.most * p.G + pair) + 1] = inv;
+                    if (p.stats && d == 0) p.stats[unit * p.most * p.G + pair] = float2{ref, inv};
                 } else {
-                    float* to = part + (int64_t) pair * (D + 4);
-                    *reinterpret_cast<f4v*>(to + d) = sum;
-                    if (d == 0) to[D] = top, to[D + 1] = all;
+                    *reinterpret_cast<f4v*>(p.part + (piece + pair) * D + d) = sum;
+                    if (d == 0) p.ml[piece + pair] = float2{top, all};
                 }
             }
             if (z == 0 && c0 == 0 && tid == 0 && p.units) p.units[unit] = int2{wg, whole ? wg : wg + (int) quotient(cost - to + run - 1, run)};
@@ -481,21 +481,25 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
     }
 }
 
-// out = sum over a unit's pieces of O 2^(m - M) / sum of l 2^(m - M): a work-group a (sequence, key head, pair), D / 4 threads x SG
-// pieces at a time in a fixed shape, each of them against the largest m of its own. The first piece lies in its work-group's second place, the others in their first
-template <int D, int QT, int TH>
-__global__ __launch_bounds__(TH) void kv8_merge_kernel(const AttendParams p) {
+// What comes behind the tokens, in one launch: `rows` work-groups put the pieces of a (sequence, key head, pair) together, others (with acc) sum up what 1024 tokens
+// of a key head have been given, from the scores and the pieces' m and l. (131072 tokens x 4 key heads of 16 rows, 192 pieces each: a launch each took 6.4 and
+// 8.0 us one behind the other, 50.2 us the call instead of 53.4)
+constexpr int TH = 256;
+
+// out = sum over a unit's pieces of O 2^(m - M) / sum of l 2^(m - M): D / 4 threads x SG pieces at a time in a fixed shape, each of them against the largest m
+// of its own. The first piece lies in its work-group's second place, the others in their first
+template <int D, int QT>
+__device__ __forceinline__ void merge(const AttendParams& p, int64_t place, uint8_t* lds) {
     constexpr int L = D / 4, SG = TH / L, U = 8;
-    __shared__ __attribute__((aligned(16))) float sums[SG][D];
-    __shared__ float2 ml[SG];
+    float* sums = reinterpret_cast<float*>(lds);                  // [SG][D]
+    float2* ml = reinterpret_cast<float2*>(lds + SG * D * 4);     // [SG]
     const int tid = threadIdx.x;
-    const int64_t place = blockIdx.x, unit = place / (p.most * p.G);
+    const int64_t unit = place / (p.most * p.G);
     const int pair = (int) (place - unit * p.most * p.G), s = (int) (unit / p.c.Hkv), hk = (int) (unit - (int64_t) s * p.c.Hkv);
     const int2 ws = p.units[unit];
     const Kv8Seq q = seq_of(p, s);
     if (pair >= q.n * p.G || ws.x == ws.y) return;
-    const int64_t row = (int64_t) p.most * p.G * (D + 4);
-    const float* first = p.part + (int64_t) ws.x * 2 * row + pair * (D + 4);
+    const int64_t row = (int64_t) p.most * p.G, first = ws.x * 2 * row + pair;
     const int count = ws.y - ws.x + 1, sg = tid / L, d = tid % L * 4;
     float m = -INFINITY, l = 0.0f;
     f4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -505,8 +509,8 @@ __global__ __launch_bounds__(TH) void kv8_merge_kernel(const AttendParams p) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int k = std::min(k0 + i * SG, count - 1);
-            const float* at = first + (2 * (int64_t) k + (k == 0)) * row;
-            o[i] = *reinterpret_cast<const f4v*>(at + d), x[i] = *reinterpret_cast<const float2*>(at + D);
+            const int64_t at = first + (2 * (int64_t) k + (k == 0)) * row;
+            o[i] = *reinterpret_cast<const f4v*>(p.part + at * D + d), x[i] = p.ml[at];
             if (k0 + i * SG >= count) x[i].x = -INFINITY;
         }
         float top = m;
@@ -520,7 +524,7 @@ __global__ __launch_bounds__(TH) void kv8_merge_kernel(const AttendParams p) {
             if (k0 + i * SG < count) sum += o[i] * c, l += x[i].y * c;
         }
     }
-    *reinterpret_cast<f4v*>(&sums[sg][d]) = sum;
+    *reinterpret_cast<f4v*>(sums + sg * D + d) = sum;
     if (d == 0) ml[sg] = float2{m, l};
     __syncthreads();
     if (tid >= L) return;
@@ -532,57 +536,120 @@ __global__ __launch_bounds__(TH) void kv8_merge_kernel(const AttendParams p) {
 #pragma unroll 4
     for (int k = 0; k < SG; ++k) {
         const float c = fast_exp2(ml[k].x - ref);
-        sum += *reinterpret_cast<const f4v*>(&sums[k][d]) * c, all += ml[k].y * c;
+        sum += *reinterpret_cast<const f4v*>(sums + k * D + d) * c, all += ml[k].y * c;
     }
     const float inv = all == 0.0f ? 0.0f : 1.0f / all;
     const int i = row_of(p, pair), g = pair - i * p.G;
     const int64_t at = ((int64_t) (q.first + i) * p.Hq + hk * p.G + g) * D + d;
 #pragma unroll
     for (int k = 0; k < 4; ++k) store_o<QT>(p.out, at + k, sum[k] * inv);
-    if (p.stats && tid == 0) p.stats[2 * place] = ref, p.stats[2 * place + 1] = inv;
 }
 
-// acc1 = acc0 + the weights of the pairs: a thread 4 tokens in a row (a block holds them), pairs 4 at a time
-__global__ __launch_bounds__(256) void kv8_given_kernel(const AttendParams p) {
-    const int hk = blockIdx.y, s = blockIdx.z;
+// acc1 = acc0 + the weights of the pairs: a thread 4 tokens in a row (a block holds them), pairs 8 at a time, 64 pairs' largest scores and sums at a time in LDS
+__device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8_t* lds) {
+    constexpr int PAIRS = 64, U = 8;
+    float2* stat = reinterpret_cast<float2*>(lds);                // [PAIRS]: m, 1 / l
+    float2* part = stat + PAIRS;                                  // [TH]
+    const int tid = threadIdx.x;
+    const int64_t runs = (p.longest + 4 * TH - 1) / (4 * TH), unit = place / runs;
+    const int s = (int) (unit / p.c.Hkv), hk = (int) (unit - (int64_t) s * p.c.Hkv);
+    const int64_t t0 = ((place - unit * runs) * TH + tid) * 4;
     const Kv8Seq q = seq_of(p, s);
-    const int64_t t0 = ((int64_t) blockIdx.x * 256 + threadIdx.x) * 4, end = (int64_t) q.len + q.n;
-    if (q.n <= 0 || t0 >= end) return;
+    const int64_t end = (int64_t) q.len + q.n;
+    if (q.n <= 0 || t0 - 4 * tid >= end) return;
+    const int2 ws = p.units ? p.units[unit] : int2{0, 0};
     const int b = kv8_block(p.c, p.c.table, s, t0 >> p.c.shift);
-    if (b < 0) return;
-    const int64_t at = kv8_rows(p.c, b, hk) + (t0 & (p.c.block - 1));
+    const bool live = t0 < end && b >= 0;
+    const int64_t at = kv8_rows(p.c, std::max(b, 0), hk) + (t0 & (p.c.block - 1));
     int64_t lo, hi;
     span_of(p, q, lo, hi);
     f4v sum = {0.0f, 0.0f, 0.0f, 0.0f}, was = sum;
-    if (p.acc0) {
+    if (p.acc0 && live) {
         if (t0 + 4 <= q.len) was = __builtin_bit_cast(f4v, *reinterpret_cast<const floats4_t*>(p.acc0 + at));
         else
 #pragma unroll
             for (int i = 0; i < 4; ++i) was[i] = t0 + i < q.len ? p.acc0[at + i] : 0.0f;
     }
-    const int64_t place = ((int64_t) s * p.c.Hkv + hk) * p.most * p.G;
-    const float* scores = p.scores + place * p.pad + t0;
-    const float* stats = p.stats + 2 * place;
-    // (only what a pair has seen was written, in whole tiles: tokens of these that one of its rows sees lie in one, the others are 0 there. A tile that
-    // none of them lies in may hold anything)
-    if (lo < hi && t0 < hi)
-        for (int i = 0; i < q.n; ++i) {
-            const int64_t pos = (int64_t) q.len + i;
-            if (t0 > pos || (p.win > 0 && t0 + 3 + p.win <= pos)) continue;
-#pragma unroll 8
-            for (int g = 0; g < p.G; ++g) {
-                const int pair = i * p.G + g;
-                const f4v x = *reinterpret_cast<const f4v*>(scores + (int64_t) pair * p.pad);
-                const float m = stats[2 * pair], inv = stats[2 * pair + 1];
+    const int64_t row = (int64_t) p.most * p.G;
+    const int pairs = q.n * p.G;
+    const bool seen = live && lo < hi && t0 < hi;
+    for (int p0 = 0; p0 < pairs; p0 += PAIRS) {
+        // (only what a pair has seen was written, in whole tiles: tokens of these that one of its rows sees lie in one, the others are 0 there. A tile that
+        // none of them lies in may hold anything)
+        auto ask = [&](int at, f4v (&x)[U]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sum[k] = fmaf(fast_exp2(x[k] - m), inv, sum[k]);
+            for (int i = 0; i < U; ++i) {
+                const int pair = at + i;
+                x[i] = f4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (pair >= std::min(p0 + PAIRS, pairs)) continue;
+                const int64_t pos = (int64_t) q.len + row_of(p, pair);
+                if (seen && t0 <= pos && (p.win <= 0 || t0 + 3 + p.win > pos)) x[i] = *reinterpret_cast<const f4v*>(p.scores + (unit * row + pair) * p.pad + t0);
+            }
+        };
+        f4v x[U];
+        ask(p0, x);
+        // the pairs' m and l over their pieces: as many threads a pair as there are
+        const int n = std::min(PAIRS, pairs - p0), bits = n > 1 ? 32 - __builtin_clz(n - 1) : 0, mine = tid & ((1 << bits) - 1), sub = tid >> bits, subs = TH >> bits;
+        if (ws.x == ws.y) {
+            if (tid < n) stat[tid] = p.stats[unit * row + p0 + tid];
+        } else {
+            const int count = ws.y - ws.x + 1;
+            float m = -INFINITY, l = 0.0f;
+            if (mine < n)
+                for (int k0 = sub; k0 < count; k0 += subs * U) {
+                    float2 v[U];
+                    float top = m;
+#pragma unroll
+                    for (int i = 0; i < U; ++i) {
+                        const int k = std::min(k0 + i * subs, count - 1);
+                        v[i] = p.ml[((int64_t) (ws.x + k) * 2 + (k == 0)) * row + p0 + mine];
+                        if (k0 + i * subs >= count) v[i] = float2{-INFINITY, 0.0f};
+                    }
+#pragma unroll
+                    for (int i = 0; i < U; ++i) top = fmaxf(top, v[i].x);
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    l *= fast_exp2(m - ref), m = top;
+#pragma unroll
+                    for (int i = 0; i < U; ++i) l += v[i].y * fast_exp2(v[i].x - ref);
+                }
+            part[tid] = float2{m, l};
+            __syncthreads();
+            if (tid < n) {
+                for (int k = 1; k < subs; ++k) m = fmaxf(m, part[(k << bits) + tid].x);
+                const float ref = m == -INFINITY ? 0.0f : m;
+                l = 0.0f;
+                for (int k = 0; k < subs; ++k) l += part[(k << bits) + tid].y * fast_exp2(part[(k << bits) + tid].x - ref);
+                stat[tid] = float2{ref, l == 0.0f ? 0.0f : 1.0f / l};
             }
         }
+        __syncthreads();
+        for (int at = p0; at < p0 + n; at += U) {
+            f4v next[U];
+            if (at + U < p0 + n) ask(at + U, next);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const float2 f = stat[std::min(at - p0 + i, n - 1)];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum[k] = fmaf(fast_exp2(x[i][k] - f.x), f.y, sum[k]);
+                x[i] = next[i];
+            }
+        }
+        __syncthreads();                                          // (the numbers are read)
+    }
+    if (!live) return;
     if (t0 + 4 <= end) *reinterpret_cast<floats4_t*>(p.acc1 + at) = __builtin_bit_cast(floats4_t, was + sum);
     else
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (t0 + i < end) p.acc1[at + i] = was[i] + sum[i];
+}
+
+template <int D, int QT, bool ACC>
+__global__ __launch_bounds__(TH) void kv8_join_kernel(const AttendParams p, int64_t rows) {
+    constexpr int SG = TH / (D / 4), MERGE = SG * D * 4 + SG * 8, GIVE = ACC ? (64 + TH) * 8 : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[MERGE > GIVE ? MERGE : GIVE];
+    if (!ACC || (int64_t) blockIdx.x < rows) merge<D, QT>(p, blockIdx.x, lds);
+    else give(p, (int64_t) blockIdx.x - rows, lds);
 }
 
 template <int D, int RT, int QT>
@@ -595,11 +662,10 @@ void launch_attend(ns_gpu* g, int form, const AttendParams& p, int64_t D, int RT
     if (D == 128) RT == 1 ? launch_attend<128, 1, QT>(g, form, p, grid) : launch_attend<128, 2, QT>(g, form, p, grid);
     else launch_attend<256, 1, QT>(g, form, p, grid);
 }
-// (1024 threads a pair where a unit may be in more pieces than 256 take in one round)
 template <int D, int QT>
-void launch_merge(ns_gpu* g, const AttendParams& p, int64_t rows) {
-    if (p.nw > (int64_t) p.S * p.c.Hkv * 8 * (1024 / D)) kv8_merge_kernel<D, QT, 1024><<<(unsigned) rows, 1024, 0, g->q>>>(p);
-    else kv8_merge_kernel<D, QT, 256><<<(unsigned) rows, 256, 0, g->q>>>(p);
+void launch_join(ns_gpu* g, const AttendParams& p, int64_t rows, int64_t grid) {
+    if (p.acc1) kv8_join_kernel<D, QT, true><<<(unsigned) grid, TH, 0, g->q>>>(p, rows);
+    else kv8_join_kernel<D, QT, false><<<(unsigned) grid, TH, 0, g->q>>>(p, rows);
 }
 
 // 16-pair tiles a wave: two where more than 16 pairs share a key head of 128 (heads of 256 have no registers for a second: 16 pairs a work-group,
@@ -615,14 +681,14 @@ int64_t workgroups(int64_t S, int64_t pairs, int64_t Hkv, int64_t D, int64_t lon
 }
 
 struct Scratch {
-    int64_t part, units, scores, stats, pad;
-    int64_t all() const { return part + units + scores + stats; }
+    int64_t part, ml, units, scores, stats, pad;
+    int64_t all() const { return part + ml + units + scores + stats; }
 };
 Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest, bool acc, int64_t nw) {
     const int64_t rows = S * most * Hq, pairs = most * (Hq / Hkv);
     Scratch x{};
     x.pad = (longest + 31) / 32 * 32;
-    if (longest > CHUNK) x.part = nw * 2 * pairs * (D + 4), x.units = (S * Hkv * 2 + 3) / 4 * 4;
+    if (longest > CHUNK) x.part = nw * 2 * pairs * D, x.ml = nw * 2 * pairs * 2, x.units = (S * Hkv * 2 + 3) / 4 * 4;
     x.scores = acc ? rows * x.pad : 0;
     x.stats = acc ? rows * 2 : 0;
     return x;
@@ -643,26 +709,24 @@ int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, in
     p.nz = (int) nz, p.pad = x.pad;
     p.ginv = (uint32_t) ((((int64_t) 1 << 32) + p.G - 1) / p.G);
     const int64_t grid = nz > 1 ? (int64_t) (p.nw + 7) / 8 * 8 * nz : p.nw;
-    if (!ns_grid_fits(grid, 256) || !ns_grid_fits(rows, 256)) return ns_fail(w + ": more work-groups than a launch takes");
     // (of sequences that are all within a chunk there are no pieces)
     const bool pieces = x.units > 0;
     p.part = scratch;
-    p.units = pieces ? (int2*) (scratch + x.part) : nullptr;
-    p.scores = p.acc1 ? scratch + x.part + x.units : nullptr;
-    p.stats = p.acc1 ? scratch + x.part + x.units + x.scores : nullptr;
+    p.ml = (float2*) (scratch + x.part);
+    p.units = pieces ? (int2*) (scratch + x.part + x.ml) : nullptr;
+    p.scores = p.acc1 ? scratch + x.part + x.ml + x.units : nullptr;
+    p.stats = p.acc1 ? (float2*) (scratch + x.part + x.ml + x.units + x.scores) : nullptr;
+    const int64_t merges = pieces ? rows : 0, gives = p.acc1 ? (p.longest + 4 * TH - 1) / (4 * TH) * Hkv * p.S : 0;
+    if (!ns_grid_fits(grid, 256) || !ns_grid_fits(merges + gives, TH)) return ns_fail(w + ": more work-groups than a launch takes");
     const int RT = tiles_of(pairs, D);
     if (qt == 0) launch_attend<0>(g, form, p, D, RT, dim3((unsigned) grid));
     else if (qt == 1) launch_attend<1>(g, form, p, D, RT, dim3((unsigned) grid));
     else launch_attend<2>(g, form, p, D, RT, dim3((unsigned) grid));
     NS_LAUNCHED("kv8_attend");
-    if (pieces) {
-        if (D == 128) qt == 0 ? launch_merge<128, 0>(g, p, rows) : qt == 1 ? launch_merge<128, 1>(g, p, rows) : launch_merge<128, 2>(g, p, rows);
-        else qt == 0 ? launch_merge<256, 0>(g, p, rows) : qt == 1 ? launch_merge<256, 1>(g, p, rows) : launch_merge<256, 2>(g, p, rows);
-        NS_LAUNCHED("kv8_merge");
-    }
-    if (p.acc1) {
-        kv8_given_kernel<<<dim3((unsigned) ((p.longest + 1023) / 1024), (unsigned) Hkv, (unsigned) p.S), 256, 0, g->q>>>(p);
-        NS_LAUNCHED("kv8_given");
+    if (merges + gives > 0) {
+        if (D == 128) qt == 0 ? launch_join<128, 0>(g, p, merges, merges + gives) : qt == 1 ? launch_join<128, 1>(g, p, merges, merges + gives) : launch_join<128, 2>(g, p, merges, merges + gives);
+        else qt == 0 ? launch_join<256, 0>(g, p, merges, merges + gives) : qt == 1 ? launch_join<256, 1>(g, p, merges, merges + gives) : launch_join<256, 2>(g, p, merges, merges + gives);
+        NS_LAUNCHED("kv8_join");
     }
     return 0;
 }
@@ -736,7 +800,8 @@ int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
         const int64_t rows = std::min(DECODE_ROWS, T - t);
         p.q = (const uint8_t*) q + t * qs * e, p.out = (uint8_t*) out + t * Hq * D * e, p.T = p.most = (int) rows, p.p0 = p0 + t, p.longest = p0 + t + rows;
         // (as many work-groups as have places for their pieces)
-        const int64_t a_wg = scratch_of(1, rows, Hq, Hkv, D, p.longest, false, 1).part, units = scratch_of(1, rows, Hq, Hkv, D, p.longest, false, 1).units;
+        const Scratch one = scratch_of(1, rows, Hq, Hkv, D, p.longest, false, 1);
+        const int64_t a_wg = one.part + one.ml, units = one.units;
         p.nw = (int) std::min(workgroups(1, rows * p.G, Hkv, D, p.longest), a_wg > 0 ? ((int64_t) own - units) / a_wg : 1 << 30);
         if (p.nw < 1) return ns_fail(w + ": more rows and heads than the library's scratch holds");
         if (attend(g, w, form, qt, p, Hkv, D, g->own_scratch)) return -1;
