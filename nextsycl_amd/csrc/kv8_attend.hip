@@ -237,6 +237,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
             s8v qh[RT][2 * KJ], ql[QS ? RT : 1][2 * KJ];
             float qm[RT];                                         // what a score takes besides the block's scale
             int rlo[RT], rhi[RT];                                 // tokens seen: rlo .. rhi
+            float x[RT][2 * KJ][8], most[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const int pair = pair0 + rt * 16 + n;
@@ -245,7 +246,7 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                 rhi[rt] = live ? std::min(pos0 + i, je - 1) : -1;
                 rlo[rt] = p.win > 0 ? (int) std::max<int64_t>(jb, pos0 + i + 1 - p.win) : jb;
                 const int64_t at = (int64_t) (q.first + i) * p.qs + (int64_t) (hk * p.G + g) * D;
-                float x[2 * KJ][8], most = 0.0f;
+                most[rt] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 2 * KJ; ++j) {
                     const int64_t d = at + 64 * (j / 2) + 16 * g4 + 8 * (j % 2);
@@ -253,25 +254,28 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                         float a[4], b[4];
                         load_row<0, 4>(p.q, d, a), load_row<0, 4>(p.q, d + 4, b);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) x[j][k] = a[k], x[j][4 + k] = b[k];
-                    } else load_row<QT, 8>(p.q, d, x[j]);
+                        for (int k = 0; k < 4; ++k) x[rt][j][k] = a[k], x[rt][j][4 + k] = b[k];
+                    } else load_row<QT, 8>(p.q, d, x[rt][j]);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[j][k]));
+                    for (int k = 0; k < 8; ++k) most[rt] = fmaxf(most[rt], fabsf(x[rt][j][k]));
                 }
-                if (rt == 0) {
-                    // (the rows are asked for; behind them the scales and the first tile)
-                    scales();
-                    if (const int t = t0 + ((w - t0) & (WAVES - 1)); t * TILE < std::min(je, span)) fetch_keys(t * TILE), fetch_values(t * TILE);
-                }
-                most = rows_max(most);
-                const int e = most > 0.0f ? std::min(std::max((int) (__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 13, -110), 110) : 0;
+            }
+            // (the rows are there, as the entries are; the scales and the first tile are under way while they become operands)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) asm volatile("" : "+v"(most[rt]));
+            scales();
+            if (const int t = t0 + ((w - t0) & (WAVES - 1)); t * TILE < std::min(je, span)) fetch_keys(t * TILE), fetch_values(t * TILE);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float top = rows_max(most[rt]);
+                const int e = top > 0.0f ? std::min(std::max((int) (__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 13, -110), 110) : 0;
                 const float up = kv8_pow2(-e);
                 qm[rt] = p.sl2 * kv8_pow2(e);
 #pragma unroll
                 for (int j = 0; j < 2 * KJ; ++j)
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const float v = x[j][k] * up;
+                        const float v = x[rt][j][k] * up;
                         qh[rt][j][k] = to16<false>(v);
                         if constexpr (QS) ql[rt][j][k] = to16<false>(v - f16_to_f32((uint16_t) qh[rt][j][k]));
                     }
@@ -391,7 +395,8 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                     }
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     if constexpr (ACC) {
-                        // (in front of the values' transfers: the wait for the keys ahead of them then counts these too, and no more)
+                        // (in front of the values' transfers: the wait for the keys ahead of them then counts these too, and no more; leaving them under way as well is no
+                        // faster)
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
                             if (const int pair = pair0 + rt * 16 + n; pair < pairs) {
