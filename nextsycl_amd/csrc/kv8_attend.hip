@@ -44,7 +44,7 @@ struct AttendParams {
     void* out;
     float* part;                // [nw][2][most G][D]: O of a run that begins inside a unit; of one that ends in it
     float2* ml;                 // [nw][2][most G]: its m, l
-    int2* units;                // [S][Hkv]: the first and the last work-group with tokens of a unit
+    int2* units;                // [S][Hkv]: the first and the last work-group with tokens of a unit; null: work-groups take a unit each
     float* scores;              // [S][Hkv][most G][pad]: scores in log2 units, or null
     float2* stats;              // [S][Hkv][most G]: the largest score and 1 / sum of a pair whose unit is in one piece, or null
     int64_t pad;
@@ -64,12 +64,15 @@ __device__ __forceinline__ void span_of(const AttendParams& p, const Kv8Seq& q, 
 
 // (a 64-bit division takes some hundred instructions, a 32-bit one a few tens)
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return (a | b) >> 31 ? a / b : (int64_t) ((uint32_t) a / (uint32_t) b); }
+__device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
+    return (int64_t) (uint32_t) __builtin_amdgcn_readlane((int) (uint32_t) v, lane) | (int64_t) __builtin_amdgcn_readlane((int) (v >> 32), lane) << 32;
+}
 // the row of a pair (16 G of them, G up to 4096: pair x G under 2^32)
 __device__ __forceinline__ int row_of(const AttendParams& p, int pair) { return p.G == 1 ? pair : (int) __umulhi((uint32_t) pair, p.ginv); }
 
 // What a unit - a sequence's key head - costs besides its chunks, in chunks: its rows' way in, its sums' way out (2.2 us, where a chunk's bytes take
-// 4 of a full chip's). Runs are dealt by chunks and that where there are more chunks than work-groups. (64 sequences of 125 to 8000 tokens x 8 heads: 63.7 us
-// without it, 57.7 with 1, 57.8 with 2, 58.8 with 3; 4 rows of 3 sequences behind 43003 44.8 / 44.8 / 42.6 / 42.7)
+// 3 of a full chip's). Runs are dealt by chunks and that where there are more chunks than work-groups. (64 sequences of 125 to 8000 tokens x 8 heads, 768 work-groups:
+// 63.7 us without it, 57.7 with 1, 57.8 with 2, 58.8 with 3, 512 work-groups: 54.8 with 2, 55.6 with 3; 4 rows of 3 sequences behind 43003 44.8 / 44.8 / 42.6 / 42.7)
 constexpr int EXTRA = 2;
 // a sequence's chunks a key head: chunk `first` and on (a sequence with rows has one at least)
 __device__ __forceinline__ int chunks_of(const AttendParams& p, const Kv8Seq& q, int& first) {
@@ -81,7 +84,7 @@ __device__ __forceinline__ int chunks_of(const AttendParams& p, const Kv8Seq& q,
 
 // QT: the rows' type; RT row tiles of 16 pairs a wave; ACC: the scores are kept
 template <int D, int RT, int FORM, int QT, bool ACC>
-__global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_attend_kernel(const AttendParams p) {
+__global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendParams p) {
     constexpr bool QS = QT == 0;                                  // rows and weights in two parts
     constexpr int CH = D / 16, KJ = D / 64, DT = D / 16;          // 16-byte chunks a row; chunks a lane reads of a key; tiles of 16 features
     constexpr int TB = TILE * D, NI = TB / 1024;                  // bytes a tile and stream; transfers
@@ -89,7 +92,6 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
     constexpr int WREG = ((2 * TB > MERGE ? 2 * TB : MERGE) + 1023) / 1024 * 1024;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * WREG];
     __shared__ __attribute__((aligned(16))) float ml[RT * 16][2][WAVES];
-    __shared__ int64_t sums[WAVES + 1], found[2];
 
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g4 = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -119,13 +121,21 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
             rest = wg * run;
             left = std::max<int64_t>(0, std::min(run, total - rest));
         };
-        if (p.S == 1) {
+        if (!p.units) {
+            // (a unit each)
+            s = wg / Hkv;
+            q = seq_of(p, s);
+            nch = chunks_of(p, q, first);
+            if (nch == 0) return;
+            extra = 0, left = run = nch, rest = (int64_t) (wg - s * Hkv) * nch;
+        } else if (p.S == 1) {
             q = seq_of(p, 0);
             nch = chunks_of(p, q, first);
             deal(nch ? nch + ONE : 0);
             if (left <= 0) return;
         } else {
-            const int per = (p.S + WAVES * 64 - 1) / (WAVES * 64), s0 = std::min(tid * per, p.S), s1 = std::min(s0 + per, p.S);
+            // (each wave for itself: a lane some of the sequences in a row)
+            const int per = (p.S + 63) / 64, s0 = std::min(lane * per, p.S), s1 = std::min(s0 + per, p.S);
             int64_t mine = 0;
             int its;                                              // (a sequence's first chunk)
             auto some = [&](int i) { const int c = chunks_of(p, seq_of(p, i), its); return c ? c + ONE : 0; };
@@ -136,30 +146,24 @@ __global__ __launch_bounds__(WAVES * 64, D == 128 && RT == 1 ? 3 : 2) void kv8_a
                 const int64_t y = __shfl_up(x, d);
                 if (lane >= d) x += y;
             }
-            if (lane == 63) sums[w] = x;
-            __syncthreads();
-            int64_t before = x - mine, all = 0;
-#pragma unroll
-            for (int i = 0; i < WAVES; ++i) {
-                const int64_t y = sums[i];
-                if (i < w) before += y;
-                all += y;
-            }
-            deal(all);
+            deal(lane_of(x, 63));
             if (left <= 0) return;
             auto cost = [&](int64_t x) { return (chunks(x) + (x >> 40) * extra) * Hkv; };
-            if (cost(before) <= rest && rest < cost(before + mine)) {
+            int64_t before = x - mine, at = 0;
+            int found = 0;
+            const bool here = cost(before) <= rest && rest < cost(x);
+            if (here)
                 for (int i = s0; i < s1; ++i) {
                     const int64_t y = some(i);
                     if (rest < cost(before + y)) {
-                        found[0] = i, found[1] = rest - cost(before);
+                        found = i, at = rest - cost(before);
                         break;
                     }
                     before += y;
                 }
-            }
-            __syncthreads();
-            s = __builtin_amdgcn_readfirstlane((int) found[0]), rest = found[1];
+            const int lane0 = __builtin_ctzll(__builtin_amdgcn_ballot_w64(here));
+            s = __builtin_amdgcn_readlane(found, lane0);
+            rest = lane_of(at, lane0);
             q = seq_of(p, s);
             nch = chunks_of(p, q, first);
         }
@@ -677,12 +681,20 @@ void launch_join(ns_gpu* g, const AttendParams& p, int64_t rows, int64_t grid) {
 // the next ones read the tokens from L2)
 int tiles_of(int64_t pairs, int64_t D) { return pairs > 16 && D == 128 ? 2 : 1; }
 int64_t pair_chunks(int64_t pairs, int64_t D) { const int64_t rows = 16 * tiles_of(pairs, D); return (pairs + rows - 1) / rows; }
-// the work-groups that the tokens are dealt to: as many as the chip holds at once - 3 a CU of one tile over heads of 128, 2 of the others -, no more than
-// there can be chunks. (64 sequences of 125 to 8000 tokens x 8 heads of 128: 256 work-groups 84 us, 512 70, 768 60, 1024 64; 4 rows of each of 3 x 24 / 4 heads of
-// 256, two chunks of pairs: 128 pairs of work-groups 42, 256 37, 384 46)
+// chunks up to which work-groups take a unit each, by the number of units: nothing is put together behind them then, and no run is looked for. 2 of 4 units, 4 of
+// 8, 10 of 64, 12 of 128, 16 of 512 and more. (us, a unit each against runs: 8 units of 400 tokens 9.9 / 11.1, of 800 13.7 / 11.5; 4 units of 24 rows of 256
+// features, 200 tokens 12.1 / 14.0, 400 15.9 / 14.4; 128 units of 800 tokens 14.1 / 17.6, of 1600 21.2 / 21.3; 512 units of 1600 38.2 / 48.8)
+int64_t whole_chunks(int64_t units) {
+    int64_t log2 = 0;
+    while (units >> (log2 + 1)) ++log2;
+    return std::max<int64_t>(1, std::min<int64_t>(2 * log2 - 2, 16));
+}
+// the work-groups that the tokens are dealt to: two a CU, no more than there can be chunks. (64 sequences of 125 to 8000 tokens x 8 heads of 128: 448
+// work-groups 56.3 us, 512 54.8, 640 61.9, 768 57.6; all of 8000: 175 / 169 / 189 / 179; 4 rows of each of 64 x 24 / 4 heads of 256, two chunks of pairs, 4000 tokens:
+// 192 pairs of work-groups 173, 256 133)
 int64_t workgroups(int64_t S, int64_t pairs, int64_t Hkv, int64_t D, int64_t longest) {
-    const int64_t places = D == 128 && tiles_of(pairs, D) == 1 ? 768 : 512;
-    return std::min(std::max<int64_t>(1, places / pair_chunks(pairs, D)), S * Hkv * ((longest + CHUNK - 1) / CHUNK + 1 + EXTRA));
+    if (longest <= whole_chunks(S * Hkv) * CHUNK) return S * Hkv;
+    return std::min(std::max<int64_t>(1, 512 / pair_chunks(pairs, D)), S * Hkv * ((longest + CHUNK - 1) / CHUNK + 1 + EXTRA));
 }
 
 struct Scratch {
@@ -693,7 +705,7 @@ Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, 
     const int64_t rows = S * most * Hq, pairs = most * (Hq / Hkv);
     Scratch x{};
     x.pad = (longest + 31) / 32 * 32;
-    if (longest > CHUNK) x.part = nw * 2 * pairs * D, x.ml = nw * 2 * pairs * 2, x.units = (S * Hkv * 2 + 3) / 4 * 4;
+    if (longest > whole_chunks(S * Hkv) * CHUNK) x.part = nw * 2 * pairs * D, x.ml = nw * 2 * pairs * 2, x.units = (S * Hkv * 2 + 3) / 4 * 4;
     x.scores = acc ? rows * x.pad : 0;
     x.stats = acc ? rows * 2 : 0;
     return x;
@@ -714,7 +726,6 @@ int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, in
     p.nz = (int) nz, p.pad = x.pad;
     p.ginv = (uint32_t) ((((int64_t) 1 << 32) + p.G - 1) / p.G);
     const int64_t grid = nz > 1 ? (int64_t) (p.nw + 7) / 8 * 8 * nz : p.nw;
-    // (of sequences that are all within a chunk there are no pieces)
     const bool pieces = x.units > 0;
     p.part = scratch;
     p.ml = (float2*) (scratch + x.part);
