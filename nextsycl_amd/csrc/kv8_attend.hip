@@ -4,12 +4,12 @@
 // Bound: HBM - every visible key and value byte read once for all rows and query heads of its key head; 4 D flops a (row, head,
 // token), far under the matrix unit's ridge.
 //
-// Work split: the tokens of all sequences and key heads lie end to end in chunks of 128, and each work-group takes an equal run of them - the
-// lengths are known on the device only, and differ: with a grid over the longest sequence's splits 64 sequences of 125 to 8000 tokens
-// kept a quarter of the waves' places busy. A run that ends inside a (sequence, key head) leaves a partial there, one that begins inside it another: two places a
-// work-group hold them, and a second kernel puts a unit's pieces together. Wave w takes a chunk's tile w of 32 tokens through one buffer of keys
-// and one of values of its own in LDS, asked for again as soon as their values lie in registers: no barrier in the loop. The waves' (O, m, l) meet in LDS
-// in wave order. A wave holds its next 128 table entries and scales in two registers a lane and picks them by lane reads.
+// Work split: the lengths are known on the device only, and differ. Short contexts are a work-group's each; a few longer ones take a work-group a chunk of 128
+// tokens; else the tokens of all sequences and key heads lie end to end in chunks, and each work-group takes an equal run of them (with a grid over the longest
+// sequence's splits 64 sequences of 125 to 8000 tokens kept a quarter of the waves' places busy). A run that ends inside a (sequence, key head) leaves a partial there,
+// one that begins inside it another: two places a work-group hold them, and a second kernel puts a unit's pieces together. Wave w takes a chunk's tile w of 32 tokens
+// through one buffer of keys and one of values of its own in LDS, asked for again as soon as their values lie in registers: no barrier in the loop. The waves'
+// (O, m, l) meet in LDS in wave order. A wave holds its next 128 table entries and scales in two registers a lane and picks them by lane reads.
 //
 // A tile in the transposed orientation, as in attn_decode.hip: S^T[token][pair] = K Q^T with K's codes as halfs and the block's scale on
 // the score; online softmax in base 2, float32; O^T[d][pair] += V^T P^T with V as halfs code x scale - exactly - read by the
@@ -40,11 +40,12 @@ struct AttendParams {
     uint32_t ginv;              // 2^32 / G, rounded up
     int64_t longest, win;
     int nw, nz;                 // work-groups the chunks are dealt to; chunks of pairs
+    int per, ns;                // a work-group's chunks, `per` of one unit, and how many of these a unit may be in; 0: runs
     float sl2;                  // scale x log2(e)
     void* out;
-    float* part;                // [nw][2][most G][D]: O of a run that begins inside a unit; of one that ends in it
-    float2* ml;                 // [nw][2][most G]: its m, l
-    int2* units;                // [S][Hkv]: the first and the last work-group with tokens of a unit; null: work-groups take a unit each
+    float* part;                // [nw][most G][D]: O of a piece; runs: [nw][2]..: of one that begins inside a unit; of one that ends in it
+    float2* ml;                 // [nw]..[most G]: its m, l
+    int2* units;                // runs: [S][Hkv]: the first and the last work-group with tokens of a unit
     float* scores;              // [S][Hkv][most G][pad]: scores in log2 units, or null
     float2* stats;              // [S][Hkv][most G]: the largest score and 1 / sum of a pair whose unit is in one piece, or null
     int64_t pad;
@@ -107,10 +108,18 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
     asm volatile("" ::"s"(p.c.kc), "s"(p.c.vc), "s"(p.c.ksc), "s"(p.c.vsc), "s"(p.c.table), "s"(p.c.tmax), "s"(p.c.blocks), "s"(p.c.shift), "s"(p.q), "s"(p.qs), "s"(p.start), "s"(p.lens),
                  "s"(p.T), "s"(p.longest), "s"(p.win), "s"(p.sl2), "s"(p.ginv), "s"(p.nw));
     // ---- this work-group's run of chunks: `left` of them, from the `rest`th of sequence s on (its heads one behind the other)
-    int s = 0, first, nch, extra;
-    int64_t rest, run, left;
+    int s = 0, first, nch, extra = 0;
+    int64_t rest = 0, run = 0, left = 0;
+    int raw0 = 0, raw1 = 0;                                       // a piece's first entries where they are known in front of its length
     Kv8Seq q;
-    {
+    if (p.per) {
+        const int unit = wg / p.ns, e0 = (wg - unit * p.ns) * (p.per * CHUNK >> p.c.shift) + lane;
+        s = unit / Hkv;
+        raw0 = p.c.table[s * p.c.tmax + std::min<int64_t>(e0, p.c.tmax - 1)], raw1 = p.c.table[s * p.c.tmax + std::min<int64_t>(e0 + 64, p.c.tmax - 1)];
+        q = seq_of(p, s);
+        nch = chunks_of(p, q, first);
+        if ((wg - unit * p.ns) * p.per >= nch) return;
+    } else {
         // (chunks of a key head, and sequences that have some in bits 40 and up: both sums at once)
         constexpr int64_t ONE = (int64_t) 1 << 40;
         auto chunks = [](int64_t x) { return x & (ONE - 1); };
@@ -121,14 +130,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
             rest = wg * run;
             left = std::max<int64_t>(0, std::min(run, total - rest));
         };
-        if (!p.units) {
-            // (a unit each)
-            s = wg / Hkv;
-            q = seq_of(p, s);
-            nch = chunks_of(p, q, first);
-            if (nch == 0) return;
-            extra = 0, left = run = nch, rest = (int64_t) (wg - s * Hkv) * nch;
-        } else if (p.S == 1) {
+        if (p.S == 1) {
             q = seq_of(p, 0);
             nch = chunks_of(p, q, first);
             deal(nch ? nch + ONE : 0);
@@ -184,7 +186,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
         // ---- a piece of the run: chunks c0 .. c1 - 1 of one unit
         int64_t lo, hi;
         span_of(p, q, lo, hi);
-        const int cost = nch + extra, hk = (int) quotient(rest, cost), from = (int) (rest - (int64_t) hk * cost), to = (int) std::min<int64_t>(cost, from + left);
+        const int cost = nch + extra;
+        int hk, from, to;
+        if (p.per) hk = wg / p.ns - s * Hkv, from = (wg - wg / p.ns * p.ns) * p.per, to = std::min(cost, from + p.per);
+        else hk = (int) quotient(rest, cost), from = (int) (rest - (int64_t) hk * cost), to = (int) std::min<int64_t>(cost, from + left);
         const int c0 = std::max(from - extra, 0), c1 = to - extra;
         const int pairs = q.n * p.G, pair0 = z * RT * 16;
         if (pair0 < pairs && c1 > c0) {
@@ -235,7 +240,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
             };
             const int span = 128 << p.c.shift;                    // tokens of the entries held
             const int t0 = jb / TILE;
-            entries(0);
+            if (p.per && p.win <= 0) {
+                const int e0 = (int) (j0 >> p.c.shift) + lane;
+                blk[0] = e0 < p.c.tmax && (uint32_t) raw0 < (uint32_t) p.c.blocks && (lane << p.c.shift) < je ? raw0 : -1;
+                blk[1] = e0 + 64 < p.c.tmax && (uint32_t) raw1 < (uint32_t) p.c.blocks && ((64 + lane) << p.c.shift) < je ? raw1 : -1;
+            } else entries(0);
 
             // ---- this lane's rows: first and last token seen, operands
             s8v qh[RT][2 * KJ], ql[QS ? RT : 1][2 * KJ];
@@ -446,7 +455,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
             __syncthreads();
             const bool whole = c0 == 0 && c1 == nch;
             const int64_t unit = (int64_t) s * Hkv + hk;
-            const int64_t piece = ((int64_t) wg * 2 + (c0 == 0)) * p.most * p.G;
+            const int64_t piece = (p.per ? wg : (int64_t) wg * 2 + (c0 == 0)) * p.most * p.G;
             for (int i = tid; i < RT * 16 * (D / 4); i += WAVES * 64) {
                 const int row = i / (D / 4), d = i % (D / 4) * 4, pair = pair0 + row;
                 if (pair >= pairs) break;
@@ -478,7 +487,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
             if (z == 0 && c0 == 0 && tid == 0 && p.units) p.units[unit] = int2{wg, whole ? wg : wg + (int) quotient(cost - to + run - 1, run)};
         }
         left -= to - from;
-        if (left <= 0) break;
+        if (left <= 0) break;                                     // (a piece alone: at once)
         rest += to - from;
         if (rest >= (int64_t) cost * Hkv) {
             rest = 0;
@@ -495,8 +504,25 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
 // 8.0 us one behind the other, 50.2 us the call instead of 53.4)
 constexpr int TH = 256;
 
+// where a unit's pieces lie, and how many there are: of runs the first one lies in its work-group's second place, the others in their first
+struct Pieces {
+    int64_t first;
+    int last;
+    bool runs;
+    __device__ __forceinline__ int64_t at(int k) const { return runs ? 2 * (first + k) + (k == 0) : first + k; }
+    __device__ __forceinline__ int count(const AttendParams& p, const Kv8Seq& q) const {
+        int its;
+        return runs ? last - (int) first + 1 : (chunks_of(p, q, its) + p.per - 1) / p.per;
+    }
+};
+__device__ __forceinline__ Pieces pieces_of(const AttendParams& p, int64_t unit) {
+    if (p.per) return {unit * p.ns, 0, false};
+    const int2 ws = p.units[unit];
+    return {ws.x, ws.y, true};
+}
+
 // out = sum over a unit's pieces of O 2^(m - M) / sum of l 2^(m - M): D / 4 threads x SG pieces at a time in a fixed shape, each of them against the largest m
-// of its own. The first piece lies in its work-group's second place, the others in their first
+// of its own
 template <int D, int QT>
 __device__ __forceinline__ void merge(const AttendParams& p, int64_t place, uint8_t* lds) {
     constexpr int L = D / 4, SG = TH / L, U = 8;
@@ -505,11 +531,11 @@ __device__ __forceinline__ void merge(const AttendParams& p, int64_t place, uint
     const int tid = threadIdx.x;
     const int64_t unit = place / (p.most * p.G);
     const int pair = (int) (place - unit * p.most * p.G), s = (int) (unit / p.c.Hkv), hk = (int) (unit - (int64_t) s * p.c.Hkv);
-    const int2 ws = p.units[unit];
+    const Pieces ps = pieces_of(p, unit);
     const Kv8Seq q = seq_of(p, s);
-    if (pair >= q.n * p.G || ws.x == ws.y) return;
-    const int64_t row = (int64_t) p.most * p.G, first = ws.x * 2 * row + pair;
-    const int count = ws.y - ws.x + 1, sg = tid / L, d = tid % L * 4;
+    const int64_t row = (int64_t) p.most * p.G;
+    const int count = ps.count(p, q), sg = tid / L, d = tid % L * 4;
+    if (pair >= q.n * p.G || count == 1) return;
     float m = -INFINITY, l = 0.0f;
     f4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int k0 = sg; k0 < count; k0 += SG * U) {
@@ -518,7 +544,7 @@ __device__ __forceinline__ void merge(const AttendParams& p, int64_t place, uint
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int k = std::min(k0 + i * SG, count - 1);
-            const int64_t at = first + (2 * (int64_t) k + (k == 0)) * row;
+            const int64_t at = ps.at(k) * row + pair;
             o[i] = *reinterpret_cast<const f4v*>(p.part + at * D + d), x[i] = p.ml[at];
             if (k0 + i * SG >= count) x[i].x = -INFINITY;
         }
@@ -566,7 +592,8 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
     const Kv8Seq q = seq_of(p, s);
     const int64_t end = (int64_t) q.len + q.n;
     if (q.n <= 0 || t0 - 4 * tid >= end) return;
-    const int2 ws = p.units ? p.units[unit] : int2{0, 0};
+    const Pieces ps = pieces_of(p, unit);
+    const int count = ps.count(p, q);
     const int b = kv8_block(p.c, p.c.table, s, t0 >> p.c.shift);
     const bool live = t0 < end && b >= 0;
     const int64_t at = kv8_rows(p.c, std::max(b, 0), hk) + (t0 & (p.c.block - 1));
@@ -599,10 +626,9 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
         ask(p0, x);
         // the pairs' m and l over their pieces: as many threads a pair as there are
         const int n = std::min(PAIRS, pairs - p0), bits = n > 1 ? 32 - __builtin_clz(n - 1) : 0, mine = tid & ((1 << bits) - 1), sub = tid >> bits, subs = TH >> bits;
-        if (ws.x == ws.y) {
+        if (count == 1) {
             if (tid < n) stat[tid] = p.stats[unit * row + p0 + tid];
         } else {
-            const int count = ws.y - ws.x + 1;
             float m = -INFINITY, l = 0.0f;
             if (mine < n)
                 for (int k0 = sub; k0 < count; k0 += subs * U) {
@@ -611,7 +637,7 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
 #pragma unroll
                     for (int i = 0; i < U; ++i) {
                         const int k = std::min(k0 + i * subs, count - 1);
-                        v[i] = p.ml[((int64_t) (ws.x + k) * 2 + (k == 0)) * row + p0 + mine];
+                        v[i] = p.ml[ps.at(k) * row + p0 + mine];
                         if (k0 + i * subs >= count) v[i] = float2{-INFINITY, 0.0f};
                     }
 #pragma unroll
@@ -689,23 +715,31 @@ int64_t whole_chunks(int64_t units) {
     while (units >> (log2 + 1)) ++log2;
     return std::max<int64_t>(1, std::min<int64_t>(2 * log2 - 2, 16));
 }
-// the work-groups that the tokens are dealt to: two a CU, no more than there can be chunks. (64 sequences of 125 to 8000 tokens x 8 heads of 128: 448
-// work-groups 56.3 us, 512 54.8, 640 61.9, 768 57.6; all of 8000: 175 / 169 / 189 / 179; 4 rows of each of 64 x 24 / 4 heads of 256, two chunks of pairs, 4000 tokens:
-// 192 pairs of work-groups 173, 256 133)
-int64_t workgroups(int64_t S, int64_t pairs, int64_t Hkv, int64_t D, int64_t longest) {
-    if (longest <= whole_chunks(S * Hkv) * CHUNK) return S * Hkv;
-    return std::min(std::max<int64_t>(1, 512 / pair_chunks(pairs, D)), S * Hkv * ((longest + CHUNK - 1) / CHUNK + 1 + EXTRA));
+// How the tokens are dealt out. A work-group a piece of at most `per` chunks of a unit: all of its chunks where contexts are short (above), one where 512
+// work-groups, two a CU, are enough for that - its table entries are asked for beside its length then, not behind it (us, beside runs: 3 sequences of 800
+// tokens x 8 heads 11.4 / 13.0, 4 rows of each x 4 heads of 256 15.7 / 17.7, a token behind 4095 11.5 / 11.7). Else
+// runs, on as many work-groups. (64 sequences of 125 to 8000 tokens x 8 heads of 128: 448 work-groups 56.3 us, 512 54.8, 640 61.9, 768 57.6; all of 8000: 175 / 169 /
+// 189 / 179; 4 rows of each of 64 x 24 / 4 heads of 256, two chunks of pairs, 4000 tokens: 192 pairs of work-groups 173, 256 133)
+struct Deal {
+    int64_t nw, per, ns;
+};
+Deal deal_of(int64_t S, int64_t pairs, int64_t Hkv, int64_t D, int64_t longest) {
+    const int64_t chunks = (longest + CHUNK - 1) / CHUNK, units = S * Hkv, places = std::max<int64_t>(1, 512 / pair_chunks(pairs, D));
+    if (chunks <= whole_chunks(units)) return {units, chunks, 1};
+    if (units * chunks <= places) return {units * chunks, 1, chunks};
+    return {std::min(places, units * (chunks + EXTRA)), 0, 0};
 }
 
 struct Scratch {
     int64_t part, ml, units, scores, stats, pad;
     int64_t all() const { return part + ml + units + scores + stats; }
 };
-Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest, bool acc, int64_t nw) {
-    const int64_t rows = S * most * Hq, pairs = most * (Hq / Hkv);
+Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest, bool acc, const Deal& deal) {
+    const int64_t rows = S * most * Hq, pairs = most * (Hq / Hkv), pieces = deal.per ? (deal.ns > 1 ? deal.nw : 0) : 2 * deal.nw;
     Scratch x{};
     x.pad = (longest + 31) / 32 * 32;
-    if (longest > whole_chunks(S * Hkv) * CHUNK) x.part = nw * 2 * pairs * D, x.ml = nw * 2 * pairs * 2, x.units = (S * Hkv * 2 + 3) / 4 * 4;
+    x.part = pieces * pairs * D, x.ml = (pieces * pairs * 2 + 3) / 4 * 4;
+    x.units = deal.per ? 0 : (S * Hkv * 2 + 3) / 4 * 4;
     x.scores = acc ? rows * x.pad : 0;
     x.stats = acc ? rows * 2 : 0;
     return x;
@@ -716,20 +750,20 @@ bool sizes_fit(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int6
 }
 
 Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest, bool acc) {
-    return scratch_of(S, most, Hq, Hkv, D, longest, acc, workgroups(S, most * (Hq / Hkv), Hkv, D, longest));
+    return scratch_of(S, most, Hq, Hkv, D, longest, acc, deal_of(S, most * (Hq / Hkv), Hkv, D, longest));
 }
 
-// a checked call, its scratch at hand: scratch_of's floats for p.nw work-groups
-int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, int64_t Hkv, int64_t D, float* scratch) {
+// a checked call, its scratch at hand: scratch_of's floats
+int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, int64_t Hkv, int64_t D, const Deal& deal, float* scratch) {
     const int64_t pairs = (int64_t) p.most * p.G, nz = pair_chunks(pairs, D), rows = (int64_t) p.S * p.most * p.Hq;
-    const Scratch x = scratch_of(p.S, p.most, p.Hq, Hkv, D, p.longest, p.acc1 != nullptr, p.nw);
-    p.nz = (int) nz, p.pad = x.pad;
+    const Scratch x = scratch_of(p.S, p.most, p.Hq, Hkv, D, p.longest, p.acc1 != nullptr, deal);
+    p.nw = (int) deal.nw, p.per = (int) deal.per, p.ns = (int) deal.ns, p.nz = (int) nz, p.pad = x.pad;
     p.ginv = (uint32_t) ((((int64_t) 1 << 32) + p.G - 1) / p.G);
-    const int64_t grid = nz > 1 ? (int64_t) (p.nw + 7) / 8 * 8 * nz : p.nw;
-    const bool pieces = x.units > 0;
+    const int64_t grid = nz > 1 ? (deal.nw + 7) / 8 * 8 * nz : deal.nw;
+    const bool pieces = x.part > 0;
     p.part = scratch;
     p.ml = (float2*) (scratch + x.part);
-    p.units = pieces ? (int2*) (scratch + x.part + x.ml) : nullptr;
+    p.units = deal.per ? nullptr : (int2*) (scratch + x.part + x.ml);
     p.scores = p.acc1 ? scratch + x.part + x.ml + x.units : nullptr;
     p.stats = p.acc1 ? (float2*) (scratch + x.part + x.ml + x.units + x.scores) : nullptr;
     const int64_t merges = pieces ? rows : 0, gives = p.acc1 ? (p.longest + 4 * TH - 1) / (4 * TH) * Hkv * p.S : 0;
@@ -771,14 +805,13 @@ int ns_kv8_attend(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     if (longest <= 0 || longest > 2 * (int64_t) KV8_TOKENS) return ns_fail(w + ": contexts of 1 to 2^31 tokens");
     if (qs < Hq * D) return ns_fail(w + ": rows at least as far apart as they are long");
     p.S = (int) S, p.most = (int) most, p.Hq = (int) Hq, p.G = (int) (Hq / Hkv), p.longest = longest, p.T = (int) T;
-    p.nw = (int) workgroups(S, most * p.G, Hkv, D, longest);
     const int64_t need = scratch_of(S, p.most, Hq, Hkv, D, longest, acc1 != nullptr).all();
     if (!g || !q || !lens || !vc || !vsc || !out || (need && !scratch)) return ns_fail(w + ": a null buffer");
     if (need && (uintptr_t) scratch % 16) return ns_fail(w + ": scratch 16-byte aligned");
     p.q = q, p.qs = qs, p.start = start, p.lens = lens, p.win = kv8_window(win), p.out = out, p.acc0 = acc0, p.acc1 = acc1;
     p.sl2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float) D)) * 1.4426950408889634f;
     NS_HIP(hipSetDevice(g->dev));
-    return attend(g, w, form, qt, p, Hkv, D, scratch);
+    return attend(g, w, form, qt, p, Hkv, D, deal_of(S, most * p.G, Hkv, D, longest), scratch);
     NS_CATCH
 }
 
@@ -815,12 +848,14 @@ int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     for (int64_t t = 0; t < T; t += DECODE_ROWS) {
         const int64_t rows = std::min(DECODE_ROWS, T - t);
         p.q = (const uint8_t*) q + t * qs * e, p.out = (uint8_t*) out + t * Hq * D * e, p.T = p.most = (int) rows, p.p0 = p0 + t, p.longest = p0 + t + rows;
-        // (as many work-groups as have places for their pieces)
-        const Scratch one = scratch_of(1, rows, Hq, Hkv, D, p.longest, false, 1);
-        const int64_t a_wg = one.part + one.ml, units = one.units;
-        p.nw = (int) std::min(workgroups(1, rows * p.G, Hkv, D, p.longest), a_wg > 0 ? ((int64_t) own - units) / a_wg : 1 << 30);
-        if (p.nw < 1) return ns_fail(w + ": more rows and heads than the library's scratch holds");
-        if (attend(g, w, form, qt, p, Hkv, D, g->own_scratch)) return -1;
+        // (runs on as many work-groups as have places for their pieces, where the scratch does not hold them all)
+        Deal deal = deal_of(1, rows * p.G, Hkv, D, p.longest);
+        if (scratch_of(1, rows, Hq, Hkv, D, p.longest, false, deal).all() > (int64_t) own) {
+            const Scratch one = scratch_of(1, rows, Hq, Hkv, D, p.longest, false, {1, 0, 0});
+            deal = {std::min(deal.nw, ((int64_t) own - one.units) / (one.part + one.ml + 4)), 0, 0};
+            if (deal.nw < 1) return ns_fail(w + ": more rows and heads than the library's scratch holds");
+        }
+        if (attend(g, w, form, qt, p, Hkv, D, deal, g->own_scratch)) return -1;
     }
     return 0;
     NS_CATCH

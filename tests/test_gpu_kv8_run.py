@@ -232,6 +232,30 @@ def test_many_sequences_over_the_same_blocks(ops, Hkv, G, D, B, S):
         check_rows(F32, raw[s:s + 1], ref, qv[s:s + 1], k[:m], v[:m], D, what=str(s))
 
 
+@pytest.mark.parametrize("qt", [F32, BF16])
+@pytest.mark.parametrize("n", [300, 1500, 9000])
+@pytest.mark.parametrize("win", [0, 1000])
+def test_entries_that_are_no_blocks_however_the_tokens_are_dealt(ops, qt, n, win):
+    """A unit a work-group, a chunk a work-group, runs: keys and values of zeros for entries out of range and for those behind the table's end."""
+    r = np.random.default_rng(n)
+    H, D, B = 8, 128, 16
+    tmax = (n + B - 1) // B
+    table = r.permutation(tmax).astype(np.int32)[None]
+    c = Cache(E4M3, tmax, H, B, D, seed=1)
+    c.k[:], c.v[:] = (r.integers(0, 126, c.k.shape).astype(np.uint8) | (r.integers(0, 2, c.k.shape).astype(np.uint8) << 7) for _ in range(2))
+    c.ks[:], c.vs[:] = (2.0 ** r.integers(-8, -5, c.ks.shape) for _ in range(2))
+    bad = r.random(tmax) < 0.1
+    c.k[table[0, bad]] = 0x7F                              # (nothing is read from them)
+    c.v[table[0, bad]] = 0x7F
+    table[0, bad] = r.choice([-1, tmax, 1 << 30, -(1 << 31)], bad.sum())
+    c.k[table[0, -3:].clip(0, tmax - 1)] = 0x7F
+    short = np.ascontiguousarray(table[:, :-3])
+    q, qs, qv = rows_of(qt, r, 1, H, D)
+    raw = attend(ops, c, on_gpu(ops, c), qt, q, qs, short, np.array([n - 1]), None, 1, 1, H, longest=n, win=win)
+    ref, _ = c.attend(qv, short, 0, n - 1, win)
+    check_rows(qt, raw, ref, qv, *c.tokens(short, 0, n), D)
+
+
 def test_pools_past_4_gib(ops):
     """Blocks behind the first 4 GiB of each pool: every call as on a small pool, bit for bit."""
     r = np.random.default_rng(5)
