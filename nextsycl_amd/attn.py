@@ -1,8 +1,8 @@
-"""The library's ABI (include/ns_attn.h, ns_mla.h, ns_pre.h, ns_layer.h) bound by name, and the size-checked wrappers an engine calls.
+"""The library's ABI (include/ns_attn.h, ns_mla.h, ns_pre.h, ns_layer.h, ns_kv8.h) bound by name, and the size-checked wrappers an engine calls.
 
 `Kernels` is the table of function pointers - the counterpart of an engine's `ffi.rs` (llm/qwen35/src/ffi.rs:42-52,
 70-136; llm/museglimmer/src/ffi.rs; llm/deepseek2/src/ffi.rs:36-39): every entry point looked up by name when the table
-is built, a missing symbol being a load error (ns_layer.h's apart: those raise where they are called). `Ops` is the counterpart of `ops.rs` (llm/deepseek2/src/ops.rs:391-445):
+is built, a missing symbol being a load error (ns_layer.h's and ns_kv8.h's apart: those raise where they are called). `Ops` is the counterpart of `ops.rs` (llm/deepseek2/src/ops.rs:391-445):
 each wrapper checks that its buffers hold what the kernel will touch, then makes the C call and turns -1 into
 Error("<what>: <ns_last_error>"). The call order of a pass is the engines': kv_store -> *_scratch -> attention
 (llm/museglimmer/src/engine.rs:856-873). Nothing here computes: the HIP library does, or the call fails."""

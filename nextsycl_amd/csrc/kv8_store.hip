@@ -5,7 +5,8 @@
 // (or e4m3) of the old unit, are re-rounded to the new one, 2^k of it: half a step of the new unit at most, and over any number of
 // growths 1/2 + 1/4 + .. of the final one.
 //
-// Bound: HBM, rows read once and codes written. A work-group takes one block of one key head and stream, all of its new rows
+// Bound: HBM, rows read once and codes written (8192 float32 rows of 8 heads of 128: 15.6 us, 5.4 TB/s; a row of each of 64 sequences: 4.4, the lengths',
+// entries', scale's and rows' reads behind one another). A work-group takes one block of one key head and stream, all of its new rows
 // in registers (16 threads a row of 128, 8 values each): their largest magnitude, then their codes.
 #include "attn_host.hpp"
 #include "kv8_common.hpp"
@@ -95,7 +96,8 @@ void launch_store(ns_gpu* g, int form, const StoreParams& p, dim3 grid) {
     else form == 0 ? launch_store<QT, 0, 256>(g, p, grid) : launch_store<QT, 1, 256>(g, p, grid);
 }
 
-// tokens from .. from + n of one sequence as half rows, k and v [Hkv][n][D]: a thread 8 values of each of 8 rows, asked for together
+// tokens from .. from + n of one sequence as half rows, k and v [Hkv][n][D]: a thread 8 values of each of 8 rows, asked for together. (20126 tokens of 2
+// heads of 256: 11.2 us, 5.5 TB/s)
 template <int FORM, int D>
 __global__ __launch_bounds__(256) void kv8_widen_kernel(const Kv8Cache c, int64_t from, int64_t n, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
     constexpr int TPR = D / 8, RPP = 256 / TPR, U = 8;

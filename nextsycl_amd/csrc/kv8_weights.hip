@@ -2,7 +2,8 @@
 // share its key head (gfx950): column sums of softmax(q K^T), of which no row is kept.
 //
 // The weights need their row's largest score and sum first, so the product q K^T is made twice. Bound: the matrix unit for float32 rows (two halfs, two
-// products), else the exponentials beside it. Both passes are one kernel: a wave keeps 64 tokens in registers, codes widened once, and pairs (row,
+// products: 1024 rows behind 3001 tokens, 24 / 4 heads of 256, 168 us, 84 % of a large product's rate in the passes), else the exponentials beside it and the
+// passes' starts (64 bfloat16 rows behind 16320, 32 / 8 heads of 128: 44 us, two passes of 20). Both passes are one kernel: a wave keeps 64 tokens in registers, codes widened once, and pairs (row,
 // head) stream past it through LDS, 16 KiB of operands at a time, for the work-group's four waves at once: 256 neighbouring tokens. First a pair's largest
 // score and sum over each 64 tokens, then a token's sum over a split of the pairs. Between them small kernels: rows into halfs, in the order in which the lanes
 // of an operand lie, with a factor a pair; a pair's parts together; the splits' sums into acc.
@@ -353,7 +354,8 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
         for (int64_t r = 0; r < T; r += rows) {
             p.T = (int) std::min(rows, T - r), p.p0 = p0 + r, p.n = p.p0 + p.T, p.pairs = (int) (p.T * G);
             p.q = (const uint8_t*) q + r * qs * e, p.acc0 = r ? acc1 : acc0, p.acc1 = acc1;
-            // work-groups for the chip's places, two a CU, twice; splits of 64 pairs and more
+            // work-groups for the chip's places, two a CU, twice; splits of 64 pairs and more. (Once: the 1024 rows above 186 us, the 64 rows 49.0 where it is
+            // 47.1; three times: the same)
             p.nb = (p.n + RUN - 1) / RUN;
             const int64_t blocks = (p.nb + 3) / 4 * p.nh, rs = std::max<int64_t>(1, std::min<int64_t>({(1024 + blocks - 1) / blocks, (int64_t) RS, (int64_t) (p.pairs + 63) / 64}));
             p.prs = (int) up((p.pairs + rs - 1) / rs, 64), p.rs = (p.pairs + p.prs - 1) / p.prs;
