@@ -747,7 +747,7 @@ Scratch scratch_of(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, 
     return x;
 }
 bool sizes_fit(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest) {
-    return S > 0 && S <= 65535 && most > 0 && most <= DECODE_ROWS && Hkv > 0 && Hkv <= 32767 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= KV8_HEADS && (D == 128 || D == 256) && longest > 0 &&
+    return S > 0 && S <= 65535 && most > 0 && most <= DECODE_ROWS && Hkv > 0 && Hkv <= 32767 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= KV8_HEADS && S * most * Hq <= INT32_MAX && (D == 128 || D == 256) && longest > 0 &&
            longest <= 2 * (int64_t) KV8_TOKENS;
 }
 
@@ -803,6 +803,7 @@ int ns_kv8_attend(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     if (ns_kv8_check(w, form, Hkv, D, block, blocks, S, tmax, p.c)) return -1;
     if (Hq <= 0 || Hq % Hkv || Hq / Hkv > KV8_HEADS) return ns_fail(w + ": query heads a multiple of the key heads, up to 4096 times");
     if (most > DECODE_ROWS) return ns_fail(w + ": 1 to 16 rows a sequence");
+    if (S * most * Hq > INT32_MAX) return ns_fail(w + ": up to 2^31 - 1 rows x heads");
     if (T > KV8_TOKENS) return ns_fail(w + ": up to 2^30 rows");
     if (longest <= 0 || longest > 2 * (int64_t) KV8_TOKENS) return ns_fail(w + ": contexts of 1 to 2^31 tokens");
     if (qs < Hq * D) return ns_fail(w + ": rows at least as far apart as they are long");

@@ -57,7 +57,7 @@ QUERY = [dict(Hq=3), dict(Hq=0), dict(Hq=1 << 21), dict(qs=511), dict(q=None)]
 @pytest.mark.parametrize("name,good,bad", [
     ("ns_kv8_store", STORE, CACHE + SEQS + ROWS + [dict(ks=255), dict(vs=255), dict(k=None), dict(v=None), dict(lens=None), dict(vc=None), dict(vsc=None), dict(vc=AT + 4), dict(T=1 << 31)]),
     ("ns_kv8_attend", ATTEND, CACHE + SEQS + ROWS + QUERY + [dict(most=17), dict(longest=0), dict(longest=1 << 32), dict(T=1 << 31), dict(lens=None), dict(out=None), dict(vc=None), dict(vsc=None),
-                                                            dict(longest=4096), dict(acc1=AT), dict(longest=4096, scratch=AT + 4)]),
+                                                            dict(S=65535, most=16, Hq=8192, qs=1 << 20), dict(longest=4096), dict(acc1=AT), dict(longest=4096, scratch=AT + 4)]),
     ("ns_kv8_prompt", PROMPT, CACHE + ROWS + QUERY + [dict(p0=-1), dict(p0=1 << 31), dict(T=1 << 31), dict(out=None), dict(vc=None), dict(vsc=None)]),
     ("ns_kv8_weights", WEIGHTS, CACHE + ROWS + QUERY + [dict(p0=-1), dict(p0=1 << 31), dict(T=1 << 31), dict(acc1=None)]),
     ("ns_kv8_evict", EVICT, CACHE + SEQS + [dict(keep=0), dict(first=-1), dict(last=-1), dict(first=9), dict(last=10), dict(first=11), dict(longest=0), dict(longest=1 << 31), dict(lens=None),
@@ -92,7 +92,7 @@ def test_scratch(lib):
     f = lib.ns_kv8_attend_scratch
     assert f(1, 1, 32, 8, 128, 100, 0) == 0                               # one split: no partials
     assert f(1, 1, 32, 8, 128, 100000, 0) > 0 and f(1, 1, 32, 8, 128, 100, 1) >= 32 * 102
-    for bad in ((0, 1, 32, 8, 128, 100), (1, 17, 32, 8, 128, 100), (1, 1, 33, 8, 128, 100), (1, 1, 32, 8, 64, 100), (1, 1, 32, 8, 128, 0), (70000, 1, 32, 8, 128, 100), (1, 1, 32, 0, 128, 100)):
+    for bad in ((0, 1, 32, 8, 128, 100), (1, 17, 32, 8, 128, 100), (1, 1, 33, 8, 128, 100), (1, 1, 32, 8, 64, 100), (1, 1, 32, 8, 128, 0), (70000, 1, 32, 8, 128, 100), (1, 1, 32, 0, 128, 100), (65535, 16, 8192, 2, 128, 1 << 31)):
         assert f(*bad, 0) == 0 and f(*bad, 1) == 0, bad
 
 
