@@ -354,11 +354,14 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
         for (int64_t r = 0; r < T; r += rows) {
             p.T = (int) std::min(rows, T - r), p.p0 = p0 + r, p.n = p.p0 + p.T, p.pairs = (int) (p.T * G);
             p.q = (const uint8_t*) q + r * qs * e, p.acc0 = r ? acc1 : acc0, p.acc1 = acc1;
-            // work-groups for the chip's places, two a CU, twice; splits of 64 pairs and more. (Once: the 1024 rows above 186 us, the 64 rows 49.0 where it is
-            // 47.1; three times: the same)
+            // splits: as fine as a stage of LDS until the chip's places, two a CU, are taken once; of 64 pairs and more until they are taken twice. (Once, the 1024
+            // rows above 186 us, the 64 rows 49.0 where it is 47.1; three times the same. Always 64: 64 float32 rows behind 40, 24 / 4 heads of 256, 32.5 us where it
+            // is 28.1; always a stage: behind 4000 46 where it is 36.6)
             p.nb = (p.n + RUN - 1) / RUN;
-            const int64_t blocks = (p.nb + 3) / 4 * p.nh, rs = std::max<int64_t>(1, std::min<int64_t>({(1024 + blocks - 1) / blocks, (int64_t) RS, (int64_t) (p.pairs + 63) / 64}));
-            p.prs = (int) up((p.pairs + rs - 1) / rs, 64), p.rs = (p.pairs + p.prs - 1) / p.prs;
+            const int64_t stage = 16384 / (D * (qt == 0 ? 4 : 2)), blocks = (p.nb + 3) / 4 * p.nh;
+            auto splits = [&](int64_t places, int64_t least) { return std::min((places + blocks - 1) / blocks, (p.pairs + least - 1) / least); };
+            const int64_t fine = splits(512, stage), coarse = splits(1024, 64), rs = std::min<int64_t>(RS, std::max(fine, coarse));
+            p.prs = (int) up((p.pairs + rs - 1) / rs, fine > coarse ? stage : 64), p.rs = (p.pairs + p.prs - 1) / p.prs;
             if (!ns_grid_fits(blocks * p.rs, 256) || !ns_grid_fits((p.pairs + 15) / 16, 256)) return ns_fail(w + ": more work-groups than a launch takes");
             float* at = g->own_scratch;
             auto take = [&](int64_t floats) { float* was = at; at += up(floats, 64); return was; };
