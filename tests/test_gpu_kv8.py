@@ -560,6 +560,27 @@ def test_evict_a_long_context_and_equal_weights(ops):
             assert same_codes(INT8, d.k.read(np.uint8).reshape(c.k.shape)[to[0, j], h, :len(rows)], want)
 
 
+@pytest.mark.parametrize("n,keep,first,last", [(2048, 600, 3, 0), (2049, 2000, 0, 70), (5000, 77, 4, 60), (8192, 3000, 0, 1), (8193, 8192, 1, 1), (20000, 1500, 2, 100)])
+def test_evict_at_the_searchs_sizes(ops, n, keep, first, last):
+    """As many weights a thread as there are registers for, at both ends; many equal ones around the last kept place; entries that are no blocks; a
+    second sequence that stays whole."""
+    r = np.random.default_rng(n)
+    Hkv, D, B, lens = 2, 128, 128, [n, 60]
+    need = (keep + B - 1) // B
+    c, table, acc, tmax = evict_case(r, E4M3, Hkv, D, B, lens, spare=2 * need)
+    acc[:, 1] = np.round(acc[:, 1] * 2) / 2
+    to = np.full(table.shape, -1, np.int32)
+    to[:, :need] = table.size + r.permutation(2 * need).reshape(2, need)
+    table[0, [1, tmax // 2]] = -1, 1 << 20
+    before = Cache.__new__(Cache)
+    before.__dict__ = {k: v.copy() if isinstance(v, np.ndarray) else v for k, v in c.__dict__.items()}
+    d, got, l1 = run_evict(ops, before, table, acc, lens, keep, first, last, n, to=to)
+    want = acc.copy()
+    new = c.evict(want, table, np.array(lens), keep, first, last, to=to)
+    assert np.array_equal(l1, new) and np.array_equal(got, want, equal_nan=True)
+    check_pools(c, d)
+
+
 @pytest.mark.parametrize("inside", [True, False])
 def test_evict_sequences_a_few_at_a_time(ops, tune, inside):
     """Where the scratch holds a few sequences' lists and blocks only."""
