@@ -626,13 +626,13 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
         };
         f4v x[U];
         ask(p0, x);
-        // the pairs' m and l over their pieces: as many threads a pair as there are
-        const int n = std::min(PAIRS, pairs - p0), bits = n > 1 ? 32 - __builtin_clz(n - 1) : 0, mine = tid & ((1 << bits) - 1), sub = tid >> bits, subs = TH >> bits;
+        // the pairs' m and l over their pieces: up to 16 threads a pair
+        const int n = std::min(PAIRS, pairs - p0), bits = n > 1 ? 32 - __builtin_clz(n - 1) : 0, mine = tid & ((1 << bits) - 1), sub = tid >> bits, subs = std::min(TH >> bits, 16);
         if (count == 1) {
             if (tid < n) stat[tid] = p.stats[unit * row + p0 + tid];
         } else {
             float m = -INFINITY, l = 0.0f;
-            if (mine < n)
+            if (mine < n && sub < subs)
                 for (int k0 = sub; k0 < count; k0 += subs * U) {
                     float2 v[U];
                     float top = m;
@@ -784,6 +784,19 @@ int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, in
 }
 
 }  // namespace
+
+int ns_kv8_rows_weights(ns_gpu* g, const std::string& w, int form, int qt, const Kv8Cache& c, const void* q, int64_t qs, int64_t T, int64_t p0, int64_t Hq, int64_t win,
+                        float sl2, const float* acc0, float* acc1, float* scratch, int64_t floats) {
+    AttendParams p{};
+    p.c = c, p.c.vc = c.kc, p.c.vsc = c.ksc;
+    p.q = q, p.qs = qs, p.p0 = p0, p.T = p.most = (int) T, p.S = 1, p.Hq = (int) Hq, p.G = (int) (Hq / c.Hkv), p.longest = p0 + T, p.win = win, p.sl2 = sl2;
+    p.acc0 = acc0, p.acc1 = acc1;
+    const Deal deal = deal_of(1, T * p.G, c.Hkv, c.D, p.longest);
+    const int64_t rows = (T * Hq * c.D + 3) / 4 * 4, need = scratch_of(1, T, Hq, c.Hkv, c.D, p.longest, true, deal).all();
+    if (T > DECODE_ROWS || need + rows > floats) return 1;
+    p.out = scratch + need;
+    return attend(g, w, form, qt, p, c.Hkv, c.D, deal, scratch);
+}
 
 extern "C" {
 

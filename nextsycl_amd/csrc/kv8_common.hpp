@@ -130,5 +130,8 @@ inline Kv8Cache kv8_cache(const void* kc, const void* vc, const float* ksc, cons
     const int shift = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
     return {(uint8_t*) kc, (uint8_t*) vc, (float*) ksc, (float*) vsc, table, tmax, blocks, (int) Hkv, (int) D, (int) block, shift};
 }
+// kv8_attend.hip: up to 16 rows' weights (acc1 = acc0 + them) as a token's attention makes them, with the keys as values; 0, -1, or 1: not with so much scratch
+int ns_kv8_rows_weights(ns_gpu* g, const std::string& w, int form, int qt, const Kv8Cache& c, const void* q, int64_t qs, int64_t T, int64_t p0, int64_t Hq, int64_t win,
+                        float sl2, const float* acc0, float* acc1, float* scratch, int64_t floats);
 // kv8_store.hip: tokens from .. from + n - 1 of the table's first sequence as half rows [Hkv][n][D]; 0 or -1
 int ns_kv8_widen(ns_gpu* g, int form, const Kv8Cache& c, int64_t from, int64_t n, uint16_t* k, uint16_t* v);

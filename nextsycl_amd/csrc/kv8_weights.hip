@@ -6,7 +6,7 @@
 // passes' starts (64 bfloat16 rows behind 16320, 32 / 8 heads of 128: 44 us, two passes of 20). Both passes are one kernel: a wave keeps 64 tokens in registers, codes widened once, and pairs (row,
 // head) stream past it through LDS, 16 KiB of operands at a time, for the work-group's four waves at once: 256 neighbouring tokens. First a pair's largest
 // score and sum over each 64 tokens, then a token's sum over a split of the pairs. Between them small kernels: rows into halfs, in the order in which the lanes
-// of an operand lie, with a factor a pair; a pair's parts together; the splits' sums into acc.
+// of an operand lie, with a factor a pair; a pair's parts together; the splits' sums into acc. Few pairs go the way of a token's attention with weights instead.
 #include <algorithm>
 #include <cmath>
 
@@ -79,6 +79,9 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const WeightsParams p) {
     if (li == 0 && pair < p.pairs) p.info[(int64_t) h * p.pairs + pair].x = p.sl2 * kv8_pow2(e);
 }
 
+// pairs a key head up to which the rows go as a token's do, the keys once more in the place of the values: two launches, not four or five. (16 pairs of 8
+// heads of 128 behind 4000 tokens: 15.8 us instead of 21.6, behind 100000 62 / 89; 32 pairs 22.6 / 23.4, 84 / 93; 48 of 4 heads of 256 28.0 / 27.6; 64 33.5 / 25.7)
+constexpr int64_t FEW = 32;
 constexpr int RS = 16;                            // splits of the pairs, at most
 constexpr int KT = 4, RUN = 16 * KT;              // tiles of 16 tokens a wave; tokens
 
@@ -342,13 +345,17 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
     NS_HIP(hipSetDevice(g->dev));
     NS_OWN_SCRATCH(g);
     const int64_t own = (int64_t) ns_own_floats(g), G = Hq / Hkv, e = qt == 0 ? 4 : 2;
+    p.sl2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float) D)) * 1.4426950408889634f;
+    if (T * G <= FEW) {
+        const int rc = ns_kv8_rows_weights(g, w, form, qt, p.c, q, qs, T, p0, Hq, kv8_window(win), p.sl2, acc0, acc1, g->own_scratch, own);
+        if (rc <= 0) return rc;
+    }
     // as many rows as the scratch holds - a pair its halfs, its four numbers, its two for each 64 tokens -, else fewer key heads at a time
     const int64_t runs = (p0 + T + RUN - 1) / RUN, per = G * (D / 2 * (qt == 0 ? 2 : 1) + 4 + 2 * runs), sums = RS * (p0 + T) + 16 * D + 1024;
     const int64_t nh0 = std::min(Hkv, own / (per + sums));
     if (nh0 < 1) return ns_fail(w + ": more tokens and heads than the library's scratch holds");
     const int64_t rows = std::min({T, (own / nh0 - sums) / per, std::max<int64_t>(1, ((int64_t) 1 << 31) / (G * G) - 64)});
     p.G = (int) G, p.ginv = (uint32_t) ((((int64_t) 1 << 32) + G - 1) / G), p.qs = qs, p.win = kv8_window(win);
-    p.sl2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float) D)) * 1.4426950408889634f;
     for (int64_t h = 0; h < Hkv; h += nh0) {
         p.h0 = (int) h, p.nh = (int) std::min(nh0, Hkv - h);
         for (int64_t r = 0; r < T; r += rows) {

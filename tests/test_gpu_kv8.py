@@ -398,6 +398,12 @@ WEIGHTS = [  # Hq, Hkv, D, B, T, p0, window
     (8, 2, 128, 32, 300, 0, 0),
     (9, 3, 128, 64, 100, 1500, 200),
     (64, 4, 128, 16, 3, 2500, 0),
+    (8, 8, 128, 64, 16, 500, 0),                           # up to 32 pairs a key head: as a token's
+    (32, 8, 128, 16, 8, 2100, 300),
+    (24, 4, 256, 32, 5, 90, 0),
+    (40, 1, 128, 128, 1, 3700, 0),
+    (16, 1, 256, 16, 2, 1203, 1),
+    (8, 4, 128, 32, 16, 3, 0),
 ]
 
 
@@ -423,6 +429,26 @@ def test_weights(ops, form, qt, Hq, Hkv, D, B, T, p0, win):
     # a weight as the rows' (2^-17 in the mean; here of sums of T G of them), the sum's own roundings
     assert np.abs(got - want).max() <= 2.0 ** -17 * max(1.0, want.max())
     assert np.linalg.norm(got - want) <= 2.0 ** -18 * np.linalg.norm(want)
+
+
+def test_few_rows_weights_where_the_scratch_holds_no_scores(ops, tune):
+    """4 rows of 8 x 2 heads behind 5000 tokens: with 1 MiB the way of many rows; the same sums but for roundings, both into themselves."""
+    r = np.random.default_rng(10)
+    Hq, Hkv, D, B, T, p0 = 16, 8, 128, 64, 4, 5000
+    tmax = (p0 + T + B - 1) // B
+    table = tables(r, 1, tmax, tmax)
+    c = filled(r, E4M3, tmax, Hkv, B, D, table, [p0 + T])
+    d = on_gpu(ops, c)
+    q, qs, qv = rows_of(BF16, r, T, Hq, D)
+    acc0 = r.uniform(0, 3, (c.blocks, Hkv, B)).astype(np.float32)
+    want = acc0.astype(np.float64)
+    c.give(want.copy(), want, table, 0, p0, c.attend(qv, table, 0, p0)[1])
+    for mib in (0, 1):
+        tune(TUNE_SCRATCH_MIB, mib)
+        acc = DevBuf.of(ops.gpu, acc0)
+        ops.kv8_weights(d, BF16, DevBuf.of(ops.gpu, q), qs, T, ints(ops, table), tmax, p0, Hq, acc, acc)
+        ops.gpu.sync()
+        assert np.abs(acc.read(np.float32).reshape(want.shape) - want).max() <= 2.0 ** -17 * want.max(), mib
 
 
 def test_weights_in_pieces(ops, tune):
