@@ -48,6 +48,7 @@ struct AttendParams {
     float* part;                // [nw][most G][D]: O of a piece; runs: [nw][2]..: of one that begins inside a unit; of one that ends in it
     float2* ml;                 // [nw]..[most G]: its m, l
     int2* units;                // runs: [S][Hkv]: the first and the last work-group with tokens of a unit
+    int pg;                     // groups of pairs that a sum of weights is shared by
     float* scores;              // [S][Hkv][most G][pad]: scores in log2 units, or null
     float2* stats;              // [S][Hkv][most G]: the largest score and 1 / sum of a pair whose unit is in one piece, or null
     int64_t pad;
@@ -502,7 +503,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
 }
 
 // What comes behind the tokens, in one launch: `rows` work-groups put the pieces of a (sequence, key head, pair) together, others (with acc) sum up what 1024 tokens
-// of a key head have been given, from the scores and the pieces' m and l. (131072 tokens x 4 key heads of 16 rows, 192 pieces each: a launch each took 6.4 and
+// of a key head, or fewer of many pairs, have been given, from the scores and the pieces' m and l. (131072 tokens x 4 key heads of 16 rows, 192 pieces each: a launch each took 6.4 and
 // 8.0 us one behind the other, 50.2 us the call instead of 53.4)
 constexpr int TH = 256;
 
@@ -582,18 +583,21 @@ __device__ __forceinline__ void merge(const AttendParams& p, int64_t place, uint
     for (int k = 0; k < 4; ++k) store_o<QT>(p.out, at + k, sum[k] * inv);
 }
 
-// acc1 = acc0 + the weights of the pairs: a thread 4 tokens in a row (a block holds them), pairs 8 at a time, 64 pairs' largest scores and sums at a time in LDS
+// acc1 = acc0 + the weights of the pairs: a thread 4 tokens in a row (a block holds them) and one of `pg` groups of the pairs, 8 at a time; 256 pairs' largest
+// scores and sums at a time in LDS; the groups' sums meet there in their order
+constexpr int PAIRS = 256;
 __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8_t* lds) {
-    constexpr int PAIRS = 64, U = 8;
+    constexpr int U = 8;
     float2* stat = reinterpret_cast<float2*>(lds);                // [PAIRS]: m, 1 / l
     float2* part = stat + PAIRS;                                  // [TH]
-    const int tid = threadIdx.x;
-    const int64_t runs = (p.longest + 4 * TH - 1) / (4 * TH), unit = place / runs;
+    f4v* sums = reinterpret_cast<f4v*>(part);                     // [TH], behind the last of `part`
+    const int tid = threadIdx.x, tokens = TH / p.pg, pg = tid / tokens, slot = tid - pg * tokens;
+    const int64_t runs = (p.longest + 4 * tokens - 1) / (4 * tokens), unit = place / runs;
     const int s = (int) (unit / p.c.Hkv), hk = (int) (unit - (int64_t) s * p.c.Hkv);
-    const int64_t t0 = ((place - unit * runs) * TH + tid) * 4;
+    const int64_t t0 = ((place - unit * runs) * tokens + slot) * 4;
     const Kv8Seq q = seq_of(p, s);
     const int64_t end = (int64_t) q.len + q.n;
-    if (q.n <= 0 || t0 - 4 * tid >= end) return;
+    if (q.n <= 0 || t0 - 4 * slot >= end) return;
     const Pieces ps = pieces_of(p, unit);
     const int count = ps.count(p, q);
     const int b = kv8_block(p.c, p.c.table, s, t0 >> p.c.shift);
@@ -602,32 +606,33 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
     int64_t lo, hi;
     span_of(p, q, lo, hi);
     f4v sum = {0.0f, 0.0f, 0.0f, 0.0f}, was = sum;
-    if (p.acc0 && live) {
+    if (p.acc0 && live && pg == 0) {
         if (t0 + 4 <= q.len) was = __builtin_bit_cast(f4v, *reinterpret_cast<const floats4_t*>(p.acc0 + at));
         else
 #pragma unroll
             for (int i = 0; i < 4; ++i) was[i] = t0 + i < q.len ? p.acc0[at + i] : 0.0f;
     }
     const int64_t row = (int64_t) p.most * p.G;
-    const int pairs = q.n * p.G;
+    const int pairs = q.n * p.G, step = p.pg * U;
     const bool seen = live && lo < hi && t0 < hi;
     for (int p0 = 0; p0 < pairs; p0 += PAIRS) {
+        const int n = std::min(PAIRS, pairs - p0);
         // (only what a pair has seen was written, in whole tiles: tokens of these that one of its rows sees lie in one, the others are 0 there. A tile that
         // none of them lies in may hold anything)
         auto ask = [&](int at, f4v (&x)[U]) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < U; ++i) {
-                const int pair = at + i;
+                const int pair = p0 + at + i;
                 x[i] = f4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (pair >= std::min(p0 + PAIRS, pairs)) continue;
+                if (at + i >= n) continue;
                 const int64_t pos = (int64_t) q.len + row_of(p, pair);
                 if (seen && t0 <= pos && (p.win <= 0 || t0 + 3 + p.win > pos)) x[i] = *reinterpret_cast<const f4v*>(p.scores + (unit * row + pair) * p.pad + t0);
             }
         };
         f4v x[U];
-        ask(p0, x);
+        ask(pg * U, x);
         // the pairs' m and l over their pieces: up to 16 threads a pair
-        const int n = std::min(PAIRS, pairs - p0), bits = n > 1 ? 32 - __builtin_clz(n - 1) : 0, mine = tid & ((1 << bits) - 1), sub = tid >> bits, subs = std::min(TH >> bits, 16);
+        const int bits = n > 1 ? 32 - __builtin_clz(n - 1) : 0, mine = tid & ((1 << bits) - 1), sub = tid >> bits, subs = std::min(TH >> bits, 16);
         if (count == 1) {
             if (tid < n) stat[tid] = p.stats[unit * row + p0 + tid];
         } else {
@@ -660,18 +665,24 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
             }
         }
         __syncthreads();
-        for (int at = p0; at < p0 + n; at += U) {
+        for (int at = pg * U; at < n; at += step) {
             f4v next[U];
-            if (at + U < p0 + n) ask(at + U, next);
+            if (at + step < n) ask(at + step, next);
 #pragma unroll
             for (int i = 0; i < U; ++i) {
-                const float2 f = stat[std::min(at - p0 + i, n - 1)];
+                const float2 f = stat[std::min(at + i, n - 1)];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) sum[k] = fmaf(fast_exp2(x[i][k] - f.x), f.y, sum[k]);
                 x[i] = next[i];
             }
         }
         __syncthreads();                                          // (the numbers are read)
+    }
+    if (p.pg > 1) {
+        sums[tid] = sum;
+        __syncthreads();
+        if (pg) return;
+        for (int i = 1; i < p.pg; ++i) sum += sums[i * tokens + slot];
     }
     if (!live) return;
     if (t0 + 4 <= end) *reinterpret_cast<floats4_t*>(p.acc1 + at) = __builtin_bit_cast(floats4_t, was + sum);
@@ -683,7 +694,7 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
 
 template <int D, int QT, bool ACC>
 __global__ __launch_bounds__(TH) void kv8_join_kernel(const AttendParams p, int64_t rows) {
-    constexpr int SG = TH / (D / 4), MERGE = SG * D * 4 + SG * 8, GIVE = ACC ? (64 + TH) * 8 : 0;
+    constexpr int SG = TH / (D / 4), MERGE = SG * D * 4 + SG * 8, GIVE = ACC ? PAIRS * 8 + TH * 16 : 0;
     __shared__ __attribute__((aligned(16))) uint8_t lds[MERGE > GIVE ? MERGE : GIVE];
     if (!ACC || (int64_t) blockIdx.x < rows) merge<D, QT>(p, blockIdx.x, lds);
     else give(p, (int64_t) blockIdx.x - rows, lds);
@@ -768,7 +779,9 @@ int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, in
     p.units = deal.per ? nullptr : (int2*) (scratch + x.part + x.ml);
     p.scores = p.acc1 ? scratch + x.part + x.ml + x.units : nullptr;
     p.stats = p.acc1 ? (float2*) (scratch + x.part + x.ml + x.units + x.scores) : nullptr;
-    const int64_t merges = pieces ? rows : 0, gives = p.acc1 ? (p.longest + 4 * TH - 1) / (4 * TH) * Hkv * p.S : 0;
+    // (up to 16 pairs a thread's, while that leaves the chip empty: 256 pairs of 4 key heads behind 500 tokens 20.8 us, all by one thread 60.6; behind 30000 102, 127)
+    for (p.pg = 1; p.pg < 16 && p.pg * 16 < pairs && (p.longest * p.pg + 4 * TH - 1) / (4 * TH) * Hkv * p.S < 512;) p.pg *= 2;
+    const int64_t merges = pieces ? rows : 0, tokens = 4 * TH / p.pg, gives = p.acc1 ? (p.longest + tokens - 1) / tokens * Hkv * p.S : 0;
     if (!ns_grid_fits(grid, 256) || !ns_grid_fits(merges + gives, TH)) return ns_fail(w + ": more work-groups than a launch takes");
     const int RT = tiles_of(pairs, D);
     if (qt == 0) launch_attend<0>(g, form, p, D, RT, dim3((unsigned) grid));
