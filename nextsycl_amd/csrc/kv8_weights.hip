@@ -79,9 +79,10 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const WeightsParams p) {
     if (li == 0 && pair < p.pairs) p.info[(int64_t) h * p.pairs + pair].x = p.sl2 * kv8_pow2(e);
 }
 
-// pairs a key head up to which the rows go as a token's do, the keys once more in the place of the values: two launches, not four or five. (16 pairs of 8
-// heads of 128 behind 4000 tokens: 15.8 us instead of 21.6, behind 100000 62 / 89; 32 pairs 22.6 / 23.4, 84 / 93; 48 of 4 heads of 256 28.0 / 27.6; 64 33.5 / 25.7)
-constexpr int64_t FEW = 32;
+// pairs a key head, and scores in all, up to which the rows go as a token's do, the keys once more in the place of the values: two launches, not four or
+// five, and the scores written. (us, instead of: 16 pairs of 8 heads of 128 behind 4000 tokens 15.9 / 22.0, behind 100000 62 / 89; 48 of 4 heads of 256 behind 4000
+// 23.3 / 26.5, behind 100000 92.5 / 92.9; 64 of 8 heads of 128 behind 600 17.4 / 24.0, behind 4000 26.4 / 25.3; 96 of 4 of 256 behind 4000 27.6 / 27.7)
+constexpr int64_t FEW = 48, FEW_SCORES = 3 << 19;
 constexpr int RS = 16;                            // splits of the pairs, at most
 constexpr int KT = 4, RUN = 16 * KT;              // tiles of 16 tokens a wave; tokens
 
@@ -346,7 +347,7 @@ extern "C" int ns_kv8_weights(ns_gpu* g, int form, int qt, const void* q, int64_
     NS_OWN_SCRATCH(g);
     const int64_t own = (int64_t) ns_own_floats(g), G = Hq / Hkv, e = qt == 0 ? 4 : 2;
     p.sl2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float) D)) * 1.4426950408889634f;
-    if (T * G <= FEW) {
+    if (T <= 16 && (T * G <= FEW || T * Hq * (p0 + T) <= FEW_SCORES)) {
         const int rc = ns_kv8_rows_weights(g, w, form, qt, p.c, q, qs, T, p0, Hq, kv8_window(win), p.sl2, acc0, acc1, g->own_scratch, own);
         if (rc <= 0) return rc;
     }

@@ -398,7 +398,9 @@ WEIGHTS = [  # Hq, Hkv, D, B, T, p0, window
     (8, 2, 128, 32, 300, 0, 0),
     (9, 3, 128, 64, 100, 1500, 200),
     (64, 4, 128, 16, 3, 2500, 0),
-    (8, 8, 128, 64, 16, 500, 0),                           # up to 32 pairs a key head: as a token's
+    (8, 8, 128, 64, 16, 500, 0),                           # few pairs: as a token's
+    (32, 2, 128, 32, 16, 260, 0),
+    (48, 1, 256, 64, 9, 700, 90),
     (32, 8, 128, 16, 8, 2100, 300),
     (24, 4, 256, 32, 5, 90, 0),
     (40, 1, 128, 128, 1, 3700, 0),
