@@ -7,7 +7,10 @@
 //
 // Bound: HBM, rows read once and codes written (8192 float32 rows of 8 heads of 128: 15.6 us, 5.4 TB/s; a row of each of 64 sequences: 4.4, the lengths',
 // entries', scale's and rows' reads behind one another). A work-group takes one block of one key head and stream, all of its new rows
-// in registers (16 threads a row of 128, 8 values each): their largest magnitude, then their codes.
+// in registers - a thread 8 float32 or 16 half values -: their largest magnitude, then their codes. (8192 bfloat16 rows in blocks of 16 11.7 us, 4.3 TB/s; with 8
+// values a thread 13.7)
+#include <type_traits>
+
 #include "attn_host.hpp"
 #include "kv8_common.hpp"
 
@@ -21,10 +24,11 @@ struct StoreParams {
     int T, most;
 };
 
-// TH threads, NP passes over a block's rows: block x D = 8 TH NP values
+// TH threads of E values, NP passes over a block's rows: block x D = E TH NP values
 template <int QT, int FORM, int D, int TH, int NP>
 __global__ __launch_bounds__(TH) void kv8_store_kernel(const StoreParams p) {
-    constexpr int TPR = D / 8, RPP = TH / TPR, B = RPP * NP;      // threads a row, rows a pass, rows a block
+    constexpr int E = QT == 0 ? 8 : 16, TPR = D / E, RPP = TH / TPR, B = RPP * NP;      // values a thread, threads a row, rows a pass, rows a block
+    using codes_t = std::conditional_t<E == 8, uint2, uint4>;
     __shared__ float red[TH / 64];
     const int tid = threadIdx.x, s = blockIdx.z;
     const int h = blockIdx.y >> 1, val = blockIdx.y & 1;
@@ -39,10 +43,10 @@ __global__ __launch_bounds__(TH) void kv8_store_kernel(const StoreParams p) {
     float* scale = (val ? p.c.vsc : p.c.ksc) + (int64_t) b * p.c.Hkv + h;
     const void* src = val ? p.v : p.k;
     const int64_t stride = val ? p.vs : p.ks;
-    const int row = tid / TPR, col = tid % TPR * 8;
+    const int row = tid / TPR, col = tid % TPR * E;
     const float s0 = fresh ? 0.0f : *scale;
 
-    float x[NP][8], most = 0.0f;
+    float x[NP][E], most = 0.0f;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int64_t t = t0 + i * RPP + row;
@@ -53,9 +57,14 @@ __global__ __launch_bounds__(TH) void kv8_store_kernel(const StoreParams p) {
             load_row<0, 4>(src, at, lo), load_row<0, 4>(src, at + 4, hi);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[i][j] = lo[j], x[i][4 + j] = hi[j];
-        } else load_row<QT, 8>(src, at, x[i]);
+        } else {
+            float lo[8], hi[8];
+            load_row<QT, 8>(src, at, lo), load_row<QT, 8>(src, at + 8, hi);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[i][j]));      // (fmaxf: NaN counts as nothing)
+            for (int j = 0; j < 8; ++j) x[i][j] = lo[j], x[i][8 + j] = hi[j];
+        }
+#pragma unroll
+        for (int j = 0; j < E; ++j) most = fmaxf(most, fabsf(x[i][j]));      // (fmaxf: NaN counts as nothing)
     }
     most = wave_max(most);
     if (tid % 64 == 0) red[tid / 64] = most;
@@ -68,27 +77,34 @@ __global__ __launch_bounds__(TH) void kv8_store_kernel(const StoreParams p) {
         for (int i = 0; i < NP; ++i) {
             const int64_t t = t0 + i * RPP + row;
             if (t >= q.len && t < end) continue;
-            uint2* at = reinterpret_cast<uint2*>(pool + (i * RPP + row) * D + col);
-            const uint2 w = *at;
-            *at = uint2{kv8_reround<FORM>(w.x, ratio), kv8_reround<FORM>(w.y, ratio)};
+            codes_t* at = reinterpret_cast<codes_t*>(pool + (i * RPP + row) * D + col);
+            codes_t w = *at;
+            w.x = kv8_reround<FORM>(w.x, ratio), w.y = kv8_reround<FORM>(w.y, ratio);
+            if constexpr (E == 16) w.z = kv8_reround<FORM>(w.z, ratio), w.w = kv8_reround<FORM>(w.w, ratio);
+            *at = w;
         }
     }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int64_t t = t0 + i * RPP + row;
         if (t < q.len || t >= end) continue;
-        *reinterpret_cast<uint2*>(pool + (i * RPP + row) * D + col) =
-            uint2{kv8_codes<FORM>(x[i][0] * inv, x[i][1] * inv, x[i][2] * inv, x[i][3] * inv), kv8_codes<FORM>(x[i][4] * inv, x[i][5] * inv, x[i][6] * inv, x[i][7] * inv)};
+        auto four = [&](int j) { return kv8_codes<FORM>(x[i][j] * inv, x[i][j + 1] * inv, x[i][j + 2] * inv, x[i][j + 3] * inv); };
+        codes_t w;
+        w.x = four(0), w.y = four(4);
+        if constexpr (E == 16) w.z = four(8), w.w = four(12);
+        *reinterpret_cast<codes_t*>(pool + (i * RPP + row) * D + col) = w;
     }
     if (tid == 0 && (fresh || s1 > s0)) *scale = s1;
 }
 
 template <int QT, int FORM, int D>
 void launch_store(ns_gpu* g, const StoreParams& p, dim3 grid) {
-    if (p.c.block == 16) kv8_store_kernel<QT, FORM, D, 16 * D / 8, 1><<<grid, 16 * D / 8, 0, g->q>>>(p);
-    else if (p.c.block == 32) kv8_store_kernel<QT, FORM, D, 16 * D / 8, 2><<<grid, 16 * D / 8, 0, g->q>>>(p);
-    else if (p.c.block == 64) kv8_store_kernel<QT, FORM, D, 16 * D / 8, 4><<<grid, 16 * D / 8, 0, g->q>>>(p);
-    else kv8_store_kernel<QT, FORM, D, 16 * D / 8, 8><<<grid, 16 * D / 8, 0, g->q>>>(p);
+    // (16 rows' threads of 8 values; of 16 values 32 rows' where there are as many)
+    constexpr int TH = 2 * D, S = QT == 0 ? 1 : 2;
+    if (p.c.block == 16) kv8_store_kernel<QT, FORM, D, TH / S, 1><<<grid, TH / S, 0, g->q>>>(p);
+    else if (p.c.block == 32) kv8_store_kernel<QT, FORM, D, TH, 2 / S><<<grid, TH, 0, g->q>>>(p);
+    else if (p.c.block == 64) kv8_store_kernel<QT, FORM, D, TH, 4 / S><<<grid, TH, 0, g->q>>>(p);
+    else kv8_store_kernel<QT, FORM, D, TH, 8 / S><<<grid, TH, 0, g->q>>>(p);
 }
 template <int QT>
 void launch_store(ns_gpu* g, int form, const StoreParams& p, dim3 grid) {
