@@ -49,6 +49,7 @@ struct AttendParams {
     float2* ml;                 // [nw]..[most G]: its m, l
     int2* units;                // runs: [S][Hkv]: the first and the last work-group with tokens of a unit
     int pg;                     // groups of pairs that a sum of weights is shared by
+    bool alone;                 // a work-group has all of a unit's scores and sums them up itself
     float* scores;              // [S][Hkv][most G][pad]: scores in log2 units, or null
     float2* stats;              // [S][Hkv][most G]: the largest score and 1 / sum of a pair whose unit is in one piece, or null
     int64_t pad;
@@ -74,6 +75,61 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
 // the row of a pair (16 G of them, G up to 4096: pair x G under 2^32)
 __device__ __forceinline__ int row_of(const AttendParams& p, int pair) { return p.G == 1 ? pair : (int) __umulhi((uint32_t) pair, p.ginv); }
 
+// what 4 tokens in a row (a block holds them) have been given
+struct Given {
+    static constexpr int U = 8;
+    int64_t t0, at, scores;
+    bool live, seen;
+    f4v sum, was;
+    __device__ __forceinline__ Given(const AttendParams& p, const Kv8Seq& q, int s, int hk, int64_t t, bool first = true) {
+        t0 = t;
+        const int64_t end = (int64_t) q.len + q.n;
+        const int b = kv8_block(p.c, p.c.table, s, t0 >> p.c.shift);
+        live = t0 < end && b >= 0;
+        at = kv8_rows(p.c, std::max(b, 0), hk) + (t0 & (p.c.block - 1));
+        scores = ((int64_t) s * p.c.Hkv + hk) * p.most * p.G * p.pad + t0;
+        int64_t lo, hi;
+        span_of(p, q, lo, hi);
+        seen = live && lo < hi && t0 < hi;
+        sum = was = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.acc0 && live && first) {
+            if (t0 + 4 <= q.len) was = __builtin_bit_cast(f4v, *reinterpret_cast<const floats4_t*>(p.acc0 + at));
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i) was[i] = t0 + i < q.len ? p.acc0[at + i] : 0.0f;
+        }
+    }
+    // the scores of pairs `pair` and on, up to `end`. (Only what a pair has seen was written, in whole tiles: tokens of these that one of its rows sees lie in one, the
+    // others are 0 there. A tile that none of them lies in may hold anything)
+    __device__ __forceinline__ void ask(const AttendParams& p, const Kv8Seq& q, int pair, int end, f4v (&x)[U]) const {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            x[i] = f4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (pair + i >= end) continue;
+            const int64_t pos = (int64_t) q.len + row_of(p, pair + i);
+            if (seen && t0 <= pos && (p.win <= 0 || t0 + 3 + p.win > pos)) x[i] = *reinterpret_cast<const f4v*>(p.scores + scores + (pair + i) * p.pad);
+        }
+    }
+    // stat[i]: a pair's largest score and 1 / sum
+    __device__ __forceinline__ void add(const f4v (&x)[U], const float2* stat, int i, int last) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const float2 f = stat[std::min(i + j, last)];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] = fmaf(fast_exp2(x[j][k] - f.x), f.y, sum[k]);
+        }
+    }
+    __device__ __forceinline__ void give(const AttendParams& p, const Kv8Seq& q) const {
+        const int64_t end = (int64_t) q.len + q.n;
+        if (!live) return;
+        if (t0 + 4 <= end) *reinterpret_cast<floats4_t*>(p.acc1 + at) = __builtin_bit_cast(floats4_t, was + sum);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (t0 + i < end) p.acc1[at + i] = was[i] + sum[i];
+    }
+};
+
 // What a unit - a sequence's key head - costs besides its chunks, in chunks: its rows' way in, its sums' way out (2.2 us, where a chunk's bytes take
 // 3 of a full chip's). Runs are dealt by chunks and that where there are more chunks than work-groups. (64 sequences of 125 to 8000 tokens x 8 heads, 768 work-groups:
 // 63.7 us without it, 57.7 with 1, 57.8 with 2, 58.8 with 3, 512 work-groups: 54.8 with 2, 55.6 with 3; 4 rows of 3 sequences behind 43003 44.8 / 44.8 / 42.6 / 42.7)
@@ -96,6 +152,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
     constexpr int WREG = ((2 * TB > MERGE ? 2 * TB : MERGE) + 1023) / 1024 * 1024;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * WREG];
     __shared__ __attribute__((aligned(16))) float ml[RT * 16][2][WAVES];
+    __shared__ float2 stat[ACC ? RT * 16 : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g4 = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -481,12 +538,28 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
                     const int64_t at = ((int64_t) (q.first + i2) * p.Hq + hk * p.G + g) * D + d;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) store_o<QT>(p.out, at + k, v[k]);
-                    if (p.stats && d == 0) p.stats[unit * p.most * p.G + pair] = float2{ref, inv};
+                    if (ACC && d == 0) {
+                        if (p.alone) stat[row] = float2{ref, inv};
+                        else p.stats[unit * p.most * p.G + pair] = float2{ref, inv};
+                    }
                 } else {
                     *reinterpret_cast<f4v*>(p.part + (piece + pair) * D + d) = sum;
                     if (d == 0) p.ml[piece + pair] = float2{top, all};
                 }
             }
+            if constexpr (ACC)
+                if (p.alone) {
+                    __syncthreads();                              // (the scores are written, the numbers there)
+                    for (int64_t t = tid * 4; t < (int64_t) q.len + q.n; t += WAVES * 64 * 4) {
+                        Given x(p, q, s, hk, t);
+                        for (int at = 0; at < pairs; at += Given::U) {
+                            f4v v[Given::U];
+                            x.ask(p, q, at, pairs, v);
+                            x.add(v, stat, at, pairs - 1);
+                        }
+                        x.give(p, q);
+                    }
+                }
             if (z == 0 && c0 == 0 && tid == 0 && p.units) p.units[unit] = int2{wg, whole ? wg : wg + (int) quotient(cost - to + run - 1, run)};
         }
         left -= to - from;
@@ -583,11 +656,11 @@ __device__ __forceinline__ void merge(const AttendParams& p, int64_t place, uint
     for (int k = 0; k < 4; ++k) store_o<QT>(p.out, at + k, sum[k] * inv);
 }
 
-// acc1 = acc0 + the weights of the pairs: a thread 4 tokens in a row (a block holds them) and one of `pg` groups of the pairs, 8 at a time; 256 pairs' largest
-// scores and sums at a time in LDS; the groups' sums meet there in their order
+// acc1 = acc0 + the weights of the pairs: a thread 4 tokens and one of `pg` groups of the pairs, 8 at a time; 256 pairs' largest scores and sums at a time in
+// LDS; the groups' sums meet there in their order
 constexpr int PAIRS = 256;
 __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8_t* lds) {
-    constexpr int U = 8;
+    constexpr int U = Given::U;
     float2* stat = reinterpret_cast<float2*>(lds);                // [PAIRS]: m, 1 / l
     float2* part = stat + PAIRS;                                  // [TH]
     f4v* sums = reinterpret_cast<f4v*>(part);                     // [TH], behind the last of `part`
@@ -596,41 +669,16 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
     const int s = (int) (unit / p.c.Hkv), hk = (int) (unit - (int64_t) s * p.c.Hkv);
     const int64_t t0 = ((place - unit * runs) * tokens + slot) * 4;
     const Kv8Seq q = seq_of(p, s);
-    const int64_t end = (int64_t) q.len + q.n;
-    if (q.n <= 0 || t0 - 4 * slot >= end) return;
+    if (q.n <= 0 || t0 - 4 * slot >= (int64_t) q.len + q.n) return;
     const Pieces ps = pieces_of(p, unit);
     const int count = ps.count(p, q);
-    const int b = kv8_block(p.c, p.c.table, s, t0 >> p.c.shift);
-    const bool live = t0 < end && b >= 0;
-    const int64_t at = kv8_rows(p.c, std::max(b, 0), hk) + (t0 & (p.c.block - 1));
-    int64_t lo, hi;
-    span_of(p, q, lo, hi);
-    f4v sum = {0.0f, 0.0f, 0.0f, 0.0f}, was = sum;
-    if (p.acc0 && live && pg == 0) {
-        if (t0 + 4 <= q.len) was = __builtin_bit_cast(f4v, *reinterpret_cast<const floats4_t*>(p.acc0 + at));
-        else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) was[i] = t0 + i < q.len ? p.acc0[at + i] : 0.0f;
-    }
+    Given given(p, q, s, hk, t0, pg == 0);
     const int64_t row = (int64_t) p.most * p.G;
     const int pairs = q.n * p.G, step = p.pg * U;
-    const bool seen = live && lo < hi && t0 < hi;
     for (int p0 = 0; p0 < pairs; p0 += PAIRS) {
         const int n = std::min(PAIRS, pairs - p0);
-        // (only what a pair has seen was written, in whole tiles: tokens of these that one of its rows sees lie in one, the others are 0 there. A tile that
-        // none of them lies in may hold anything)
-        auto ask = [&](int at, f4v (&x)[U]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int pair = p0 + at + i;
-                x[i] = f4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (at + i >= n) continue;
-                const int64_t pos = (int64_t) q.len + row_of(p, pair);
-                if (seen && t0 <= pos && (p.win <= 0 || t0 + 3 + p.win > pos)) x[i] = *reinterpret_cast<const f4v*>(p.scores + (unit * row + pair) * p.pad + t0);
-            }
-        };
         f4v x[U];
-        ask(pg * U, x);
+        given.ask(p, q, p0 + pg * U, p0 + n, x);
         // the pairs' m and l over their pieces: up to 16 threads a pair
         const int bits = n > 1 ? 32 - __builtin_clz(n - 1) : 0, mine = tid & ((1 << bits) - 1), sub = tid >> bits, subs = std::min(TH >> bits, 16);
         if (count == 1) {
@@ -667,29 +715,20 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
         __syncthreads();
         for (int at = pg * U; at < n; at += step) {
             f4v next[U];
-            if (at + step < n) ask(at + step, next);
+            if (at + step < n) given.ask(p, q, p0 + at + step, p0 + n, next);
+            given.add(x, stat, at, n - 1);
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const float2 f = stat[std::min(at + i, n - 1)];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) sum[k] = fmaf(fast_exp2(x[i][k] - f.x), f.y, sum[k]);
-                x[i] = next[i];
-            }
+            for (int i = 0; i < U; ++i) x[i] = next[i];
         }
         __syncthreads();                                          // (the numbers are read)
     }
     if (p.pg > 1) {
-        sums[tid] = sum;
+        sums[tid] = given.sum;
         __syncthreads();
         if (pg) return;
-        for (int i = 1; i < p.pg; ++i) sum += sums[i * tokens + slot];
+        for (int i = 1; i < p.pg; ++i) given.sum += sums[i * tokens + slot];
     }
-    if (!live) return;
-    if (t0 + 4 <= end) *reinterpret_cast<floats4_t*>(p.acc1 + at) = __builtin_bit_cast(floats4_t, was + sum);
-    else
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (t0 + i < end) p.acc1[at + i] = was[i] + sum[i];
+    given.give(p, q);
 }
 
 template <int D, int QT, bool ACC>
@@ -779,9 +818,12 @@ int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, in
     p.units = deal.per ? nullptr : (int2*) (scratch + x.part + x.ml);
     p.scores = p.acc1 ? scratch + x.part + x.ml + x.units : nullptr;
     p.stats = p.acc1 ? (float2*) (scratch + x.part + x.ml + x.units + x.scores) : nullptr;
+    // (a unit's work-group, where it has all its pairs, sums up their weights too: 8 heads behind 100 tokens 9.2 us, in a launch of their own 12.0; 64 sequences behind
+    // 800 25.9 / 27.8)
+    p.alone = p.acc1 && deal.per && deal.ns == 1 && nz == 1;
     // (up to 16 pairs a thread's, while that leaves the chip empty: 256 pairs of 4 key heads behind 500 tokens 20.8 us, all by one thread 60.6; behind 30000 102, 127)
     for (p.pg = 1; p.pg < 16 && p.pg * 16 < pairs && (p.longest * p.pg + 4 * TH - 1) / (4 * TH) * Hkv * p.S < 512;) p.pg *= 2;
-    const int64_t merges = pieces ? rows : 0, tokens = 4 * TH / p.pg, gives = p.acc1 ? (p.longest + tokens - 1) / tokens * Hkv * p.S : 0;
+    const int64_t merges = pieces ? rows : 0, tokens = 4 * TH / p.pg, gives = p.acc1 && !p.alone ? (p.longest + tokens - 1) / tokens * Hkv * p.S : 0;
     if (!ns_grid_fits(grid, 256) || !ns_grid_fits(merges + gives, TH)) return ns_fail(w + ": more work-groups than a launch takes");
     const int RT = tiles_of(pairs, D);
     if (qt == 0) launch_attend<0>(g, form, p, D, RT, dim3((unsigned) grid));
