@@ -134,9 +134,10 @@ __global__ __launch_bounds__(256) void kv8_widen_kernel(const Kv8Cache c, int64_
         w[i] = *reinterpret_cast<const uint2*>(pool + (kv8_rows(c, bc, h) + (t & (c.block - 1))) * D + col);
         s[i] = scale[(int64_t) bc * c.Hkv + h];
     }
+    // (no block: codes and scale 0 - the block read in its place may never have been stored into, its scale be anything, NaN and infinity too)
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-        if (b[i] < 0) w[i] = uint2{0, 0};
+        if (b[i] < 0) w[i] = uint2{0, 0}, s[i] = 0.0f;
         if (j0 + i * RPP < n) *reinterpret_cast<s8v*>(out + (j0 + i * RPP) * D) = kv8_halfs8<FORM>(w[i].x, w[i].y, s[i], s[i]);
     }
 }

@@ -1,0 +1,47 @@
+"""Caches of 8-bit values in blocks of tokens (include/ns_kv8.h) where a call meets what nothing wrote: scales and codes of blocks that were never
+stored into hold anything at all, not finite numbers among it."""
+import numpy as np
+import pytest
+
+from kv8_ref import BF16, E4M3, F16, F32, INT8, Cache, from_type
+from nextsycl_amd import DevBuf
+from test_gpu_kv8 import filled, ints, on_gpu, prompt_close, rows_of, tables
+
+pytestmark = pytest.mark.gpu
+ANYTHING = [np.nan, np.inf, -np.inf, 1e30, 70000.0]
+
+
+def unwritten(r, form, Hkv, B, D, table, n, what):
+    """A cache of which only the table's own blocks are stored into; block 0 and the last are not, and no entry is them. The scales there: `what`."""
+    blocks = table.max() + 2
+    assert table.min() < 0 and not (table == 0).any()
+    c = filled(r, form, blocks, Hkv, B, D, table, [n], sigma=0.7)
+    for b in set(range(blocks)) - set(table.ravel()):
+        c.ks[b], c.vs[b] = what, what
+    return c
+
+
+def holes(r, tmax, at):
+    table = (1 + r.permutation(tmax)).astype(np.int32)[None]
+    for e, x in at:
+        table[0, e] = x
+    return table
+
+
+@pytest.mark.parametrize("what", ANYTHING)
+@pytest.mark.parametrize("form", [INT8, E4M3])
+@pytest.mark.parametrize("qt,Hq,Hkv,D,B,T,p0,win", [(BF16, 8, 2, 128, 16, 40, 100, 0), (F16, 4, 2, 256, 32, 150, 33, 0), (F32, 6, 3, 128, 64, 70, 300, 150),
+                                                    (BF16, 4, 4, 128, 128, 12, 300, 0)])
+def test_prompt_entries_that_are_no_blocks(ops, what, form, qt, Hq, Hkv, D, B, T, p0, win):
+    """Keys and values of zeros, whatever block 0 holds."""
+    r = np.random.default_rng(B)
+    n = p0 + T
+    tmax = (n + B - 1) // B
+    table = holes(r, tmax, [(1, -1), (tmax - 1, 1 << 30)])
+    c = unwritten(r, form, Hkv, B, D, np.where(table > tmax, -1, table), n, what)
+    q, qs, qv = rows_of(qt, r, T, Hq, D, pad=8)
+    ob = DevBuf(ops.gpu, T * Hq * D * (4 if qt == F32 else 2))
+    ops.kv8_prompt(on_gpu(ops, c), qt, DevBuf.of(ops.gpu, q), qs, T, ints(ops, table), tmax, p0, Hq, ob, win=win)
+    ops.gpu.sync()
+    ref, _ = c.attend(qv, table, 0, p0, win)
+    prompt_close(qt, from_type(qt, ob.read(np.float32 if qt == F32 else np.uint16)).reshape(ref.shape), ref, qv, *c.tokens(table, 0, n), D)
