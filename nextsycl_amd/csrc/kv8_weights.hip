@@ -133,7 +133,8 @@ __global__ __launch_bounds__(256, 2) void kv8_pass_kernel(const WeightsParams p)
         const int64_t t = key0 + kt * 16 + n;
         const int b = blk[kt];
         const uint8_t* row = p.c.kc + (kv8_rows(p.c, std::max(b, 0), p.h0 + h) + (t & (p.c.block - 1))) * D + 16 * g4;
-        const float sc = p.c.ksc[(int64_t) std::max(b, 0) * p.c.Hkv + p.h0 + h];
+        float sc = p.c.ksc[(int64_t) std::max(b, 0) * p.c.Hkv + p.h0 + h];
+        if (b < 0) sc = 0.0f;                                     // (no block: nothing may have been stored into the one that was read, its scale be no number)
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
             uint4 x = *reinterpret_cast<const uint4*>(row + 64 * j);

@@ -45,3 +45,25 @@ def test_prompt_entries_that_are_no_blocks(ops, what, form, qt, Hq, Hkv, D, B, T
     ops.gpu.sync()
     ref, _ = c.attend(qv, table, 0, p0, win)
     prompt_close(qt, from_type(qt, ob.read(np.float32 if qt == F32 else np.uint16)).reshape(ref.shape), ref, qv, *c.tokens(table, 0, n), D)
+
+
+@pytest.mark.parametrize("what", ANYTHING)
+@pytest.mark.parametrize("form", [INT8, E4M3])
+@pytest.mark.parametrize("qt,Hq,Hkv,D,B,T,p0,win", [(BF16, 32, 2, 128, 16, 40, 100, 0), (F16, 12, 2, 256, 32, 90, 33, 0), (F32, 24, 3, 128, 64, 70, 300, 150),
+                                                    (BF16, 4, 4, 128, 128, 3, 300, 0)])
+def test_weights_entries_that_are_no_blocks(ops, what, form, qt, Hq, Hkv, D, B, T, p0, win):
+    """Their share of a row's sum is a key of zeros', whatever block 0 holds; nothing is written for them. (Many rows; few rows, as a token's.)"""
+    r = np.random.default_rng(B + 1)
+    n = p0 + T
+    tmax = (n + B - 1) // B
+    table = holes(r, tmax, [(1, -1), (tmax - 1, 1 << 30)])
+    c = unwritten(r, form, Hkv, B, D, np.where(table > tmax, -1, table), n, what)
+    q, qs, qv = rows_of(qt, r, T, Hq, D, pad=3)
+    acc0 = r.uniform(0, 3, (c.blocks, Hkv, B)).astype(np.float32)
+    want = np.full(acc0.shape, -1.0)
+    c.give(acc0.astype(np.float64), want, table, 0, p0, c.attend(qv, table, 0, p0, win)[1])
+    a1 = DevBuf.of(ops.gpu, np.full_like(acc0, -1))
+    ops.kv8_weights(on_gpu(ops, c), qt, DevBuf.of(ops.gpu, q), qs, T, ints(ops, table), tmax, p0, Hq, DevBuf.of(ops.gpu, acc0), a1, win=win)
+    ops.gpu.sync()
+    got = a1.read(np.float32).reshape(acc0.shape)
+    assert np.abs(got - want).max() <= 2.0 ** -17 * max(1.0, want.max())
