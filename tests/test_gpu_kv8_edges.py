@@ -3,9 +3,9 @@ stored into hold anything at all, not finite numbers among it."""
 import numpy as np
 import pytest
 
-from kv8_ref import BF16, E4M3, F16, F32, INT8, Cache, from_type
+from kv8_ref import BF16, E4M3, F16, F32, INT8, from_type, to_type
 from nextsycl_amd import DevBuf
-from test_gpu_kv8 import filled, ints, on_gpu, prompt_close, rows_of, tables
+from test_gpu_kv8 import attend, filled, ints, on_gpu, prompt_close, rows_of, tables
 
 pytestmark = pytest.mark.gpu
 ANYTHING = [np.nan, np.inf, -np.inf, 1e30, 70000.0]
@@ -67,3 +67,25 @@ def test_weights_entries_that_are_no_blocks(ops, what, form, qt, Hq, Hkv, D, B, 
     ops.gpu.sync()
     got = a1.read(np.float32).reshape(acc0.shape)
     assert np.abs(got - want).max() <= 2.0 ** -17 * max(1.0, want.max())
+
+
+# ---- what is lost on the way
+
+@pytest.mark.parametrize("form", [INT8, E4M3])
+@pytest.mark.parametrize("qt", [F16, BF16])
+@pytest.mark.parametrize("Hq,Hkv,D,B,lens,counts,most,win", [(32, 8, 128, 32, [4000], [1], 1, 0), (8, 2, 128, 64, [300, 1999, 40], [1, 1, 1], 1, 0), (24, 4, 256, 16, [700, 90], [4, 2], 4, 0),
+                                                             (64, 2, 128, 16, [1500], [2], 2, 800)])
+def test_a_tokens_16_bit_rows_are_rounded_once(ops, form, qt, Hq, Hkv, D, B, lens, counts, most, win):
+    """A row of two bytes a value is the sum x, within d of the exact one, rounded: no further from the exact one than that rounded is, and twice d. d as
+    float32 rows': 2^-17 in the mean (weights of 22 bits, `tolerance`). With weights of 11 bits half rows lie 1.4 times as far off."""
+    r = np.random.default_rng(Hq + B)
+    ends = [a + b for a, b in zip(lens, counts)]
+    S, tmax = len(lens), max((e + B - 1) // B for e in ends)
+    table = tables(r, S, tmax, S * tmax)
+    c = filled(r, form, S * tmax, Hkv, B, D, table, ends)
+    start = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    q, qs, qv = rows_of(qt, r, int(start[-1]), Hq, D)
+    raw = attend(ops, c, on_gpu(ops, c), qt, q, qs, table, lens, start, int(start[-1]), most, Hq, win=win)
+    ref = np.concatenate([c.attend(qv[start[s]:start[s + 1]], table, s, lens[s], win)[0] for s in range(S)])
+    rounded = to_type(qt, ref)[1]
+    assert np.linalg.norm(from_type(qt, raw) - ref) <= np.linalg.norm(rounded - ref) + 2 * 2.0 ** -17 * np.linalg.norm(ref)
