@@ -50,7 +50,8 @@ int ns_kv8_attend(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
 
 /* A prompt's T rows, tokens p0 .. p0 + T - 1 of one sequence (table: its tmax entries), whose keys are stored already: the values are widened to half - exactly
  * - in the library's scratch and the pass runs as ns_attn_prompt_t's over a half cache (q and out 16-byte aligned, qs a multiple
- * of 16 bytes); up to 16 rows, and a pass whose values do not fit that scratch, as ns_kv8_attend's do. */
+ * of 16 bytes); up to 16 rows, and a pass whose values do not fit that scratch, as ns_kv8_attend's do. Rows and weights have ns_kv8_attend's bits and range whichever way
+ * they go, but for half and bfloat16 rows' softmax weights in the pass: 11 bits, the same in a row's sum, off by no more than a half's rounding. */
 int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_t T, const int32_t* table, int64_t tmax, int64_t p0, int64_t Hq, int64_t Hkv,
                   int64_t D, int64_t block, int64_t blocks, const void* kc, const void* vc, const float* ksc, const float* vsc, int64_t win, float scale,
                   void* out);

@@ -191,6 +191,13 @@ __device__ __forceinline__ int wave_min(int v) {
     return (int) wave_reduce_u32((uint32_t) v, [](uint32_t a, uint32_t b) { return (uint32_t) min((int) a, (int) b); });
 }
 
+__device__ __forceinline__ float pow2_of(int e) { return __builtin_bit_cast(float, (uint32_t) (e + 127) << 23); }       // (e: -126 .. 127)
+// The exponent e by which a row of largest magnitude `top` is divided - x 2^-e: its largest has exponent 13 then, of a half's 15 - before it enters a
+// product as halfs. (Up to the largest of all numbers; from 2^-107 down the rows keep some of their smallness, and scores that nothing of it shows in)
+__device__ __forceinline__ int row_exponent(float top) { return top > 0.0f ? min(max((int) (__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 13, -120), 114) : 0; }
+// what a score of such a row takes besides: the softmax scale x log2 e and 2^e (never 0: minus infinity stays what it is under it)
+__device__ __forceinline__ float row_factor(float sl2, int e) { return fmaxf(sl2 * pow2_of(e), 0x1p-126f); }
+
 // element i of a row of query / output type QT (0 float32, 1 half, 2 bfloat16)
 template <int QT>
 __device__ __forceinline__ float load_q(const void* p, int64_t i) {

@@ -31,10 +31,11 @@ int ns_attn_sel_rows(ns_gpu* g, const float* q, const uint16_t* kc, const uint16
 // attn_decode.hip: the merge of [rows][ns][D + 2] partials (also the prompt kernel's key splits')
 int ns_attn_merge_partials(ns_gpu* g, int64_t D, const float* part, int64_t ns, int qt, int64_t rows, void* out);
 // attn_prefill.hip: a checked prompt pass; causal 0 = every row sees to the pass's last key; kfirst as above; own > 0: floats of the
-// library's scratch, from its start, that the pass may use (the caller keeps something behind them, and holds own_use)
+// library's scratch, from its start, that the pass may use (the caller keeps something behind them, and holds own_use); exact, over half rows
+// alone: query rows enter the products with an exponent of their own, exactly if they have 16 bits, with 22 bits - and their weights too - if float32
 int ns_attn_prompt_any(ns_gpu* g, const char* who, int qt, int kt, int pm, const void* q, int64_t qs, const void* kc, const void* vc, int64_t T,
                        int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, int64_t p0, int64_t win, int causal, int64_t kfirst, float scale,
-                       void* out, size_t own = 0);
+                       void* out, size_t own = 0, bool exact = false);
 
 // Tuning knobs, 0 = the library's own choice: work-groups a decode pass aims for, key splits and waves of a prompt pass (16: its rows
 // end to end, in 8 waves; 12: in 4, unsplit; any other number: one head's rows, waves by the rule), work-groups an MLA pass aims for, heads a wave of the pre-attention kernel, and whether a prompt pass over a bfloat16,

@@ -38,6 +38,7 @@
 #include "attn_common.hpp"
 #include "attn_host.hpp"
 #include "kv_formats.hpp"
+#include "layer_common.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -113,9 +114,10 @@ __device__ __forceinline__ int wave_tiles(int w, int tn, int waves) { return w <
 // BF: bfloat16 operands (a bfloat16 cache too long to be widened to half first), else half. QS (bfloat16 operands only):
 // query rows of another type enter the first product as two bfloat16 numbers - the rounded row and the rounded rest, 16
 // significant bits between them - a second matrix instruction a key block.
+// XR (half rows only; float32 query rows: with QS): rows of an exponent of their own, and the weights' bits with them (attn_prefill_wave.hpp).
 // NTS (16-bit rows of 128 only): the tiles' transfers carry the streaming cache policy - a pass whose keys are each read
 // by one work-group, once.
-template <int D, bool BF, int KT, int PW, bool QS = false, bool NTS = false>
+template <int D, bool BF, int KT, int PW, bool QS = false, bool NTS = false, bool XR = false>
 __global__ __launch_bounds__(PW * 64, PW == 4 && D == 128 ? 2 : 1) void attn_prefill_kernel(const PrefillParams p) {
     constexpr bool FLAT = false;
     // a wave owns RT row tiles of 16: 32 rows at D = 128; 16 at D = 256, whose accumulators are twice as wide
@@ -123,7 +125,7 @@ __global__ __launch_bounds__(PW * 64, PW == 4 && D == 128 ? 2 : 1) void attn_pre
 #include "attn_prefill_wave.hpp"
 }
 
-template <int D, bool BF, int KT, int PW, bool QS, bool NTS, int RT>
+template <int D, bool BF, int KT, int PW, bool QS, bool NTS, int RT, bool XR>
 __device__ __forceinline__ void flat_wave(const PrefillParams& p) {
     constexpr bool FLAT = true;
 #include "attn_prefill_wave.hpp"
@@ -134,14 +136,14 @@ __device__ __forceinline__ void flat_wave(const PrefillParams& p) {
 // 4); waves without one stage their share of the keys and meet the barriers. For passes whose rows leave places of whole
 // 32-row waves empty (flat_plan). Bound: at few pairs HBM, else as the kernel above, LDS the more where waves hold one tile. New turn of 37 rows x
 // 32 / 8 bfloat16 heads behind 20011 keys, this kernel 34 us, the one above 41.7.
-template <int D, bool BF, int KT, bool QS = false, bool NTS = false, int PW = 8>
+template <int D, bool BF, int KT, bool QS = false, bool NTS = false, int PW = 8, bool XR = false>
 __global__ __launch_bounds__(PW * 64, PW == 4 ? 2 : 1) void attn_prefill_flat_kernel(const PrefillParams p) {
     const int w = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
     const int Hkv = p.Hq / p.G, xi = (int) blockIdx.x / 8, nfull = p.nbf * Hkv, u2 = xi / p.gb * 8 + (int) blockIdx.x % 8 - nfull;
     const int unit = u2 < 0 ? u2 + nfull : u2 % std::max(1, p.ngb * Hkv - nfull) + nfull;
     const int nblk = ((p.T * p.G + 15) / 16 + p.tb - 1) / p.tb, blk = nblk - 1 - (unit / Hkv * p.gb + xi % p.gb);
-    if (D == 128 && wave_tiles(w, flat_tiles(p, blk * p.tb), PW) == 2) flat_wave<D, BF, KT, PW, QS, NTS, D == 128 ? 2 : 1>(p);
-    else flat_wave<D, BF, KT, PW, QS, NTS, 1>(p);
+    if (D == 128 && wave_tiles(w, flat_tiles(p, blk * p.tb), PW) == 2) flat_wave<D, BF, KT, PW, QS, NTS, D == 128 ? 2 : 1, XR>(p);
+    else flat_wave<D, BF, KT, PW, QS, NTS, 1, XR>(p);
 }
 
 // A bfloat16 cache's rows on their way to half rows in position order: positions [kf, kf + n) of every key head, out of a
@@ -374,10 +376,31 @@ bool own_form_pays(int kt, int qt, int64_t D, int64_t T, int64_t G, int64_t keys
     }
 }
 
+// half rows, query rows of an exponent of their own (end to end: 16-bit ones)
+template <int D>
+void launch_flat_exact(ns_gpu* g, const PrefillParams& p, dim3 grid, bool stream, bool small) {
+    if constexpr (D == 128) {
+        if (small) attn_prefill_flat_kernel<D, false, 0, false, false, 4, true><<<grid, 256, 0, g->q>>>(p);
+        else if (stream) attn_prefill_flat_kernel<D, false, 0, false, true, 8, true><<<grid, 512, 0, g->q>>>(p);
+        else attn_prefill_flat_kernel<D, false, 0, false, false, 8, true><<<grid, 512, 0, g->q>>>(p);
+    } else attn_prefill_flat_kernel<D, false, 0, false, false, 8, true><<<grid, 512, 0, g->q>>>(p);
+}
+template <int D, int PW, bool QS>
+void launch_prefill_exact(ns_gpu* g, const PrefillParams& p, dim3 grid, bool stream) {
+    if constexpr (D == 128) {
+        if (stream) {
+            attn_prefill_kernel<D, false, 0, PW, QS, true, true><<<grid, PW * 64, 0, g->q>>>(p);
+            return;
+        }
+    }
+    attn_prefill_kernel<D, false, 0, PW, QS, false, true><<<grid, PW * 64, 0, g->q>>>(p);
+}
+
 // the passes whose rows lie end to end: work-groups of 8 waves, or of 4 (small: half rows of 128)
 template <int D>
-void launch_flat(ns_gpu* g, int kt, const PrefillParams& p, dim3 grid, bool stream, bool small) {
+void launch_flat(ns_gpu* g, int kt, const PrefillParams& p, dim3 grid, bool stream, bool small, bool exact) {
     constexpr int TH = 512;
+    if (exact) return launch_flat_exact<D>(g, p, grid, stream, small);
     if constexpr (D == 128) {
         if (small && kt == 0) {
             attn_prefill_flat_kernel<D, false, 0, false, false, 4><<<grid, 256, 0, g->q>>>(p);
@@ -398,8 +421,12 @@ void launch_flat(ns_gpu* g, int kt, const PrefillParams& p, dim3 grid, bool stre
 }
 
 template <int D, int PW>
-int launch_prefill(ns_gpu* g, int kt, const PrefillParams& p, dim3 grid, bool stream) {
+int launch_prefill(ns_gpu* g, int kt, const PrefillParams& p, dim3 grid, bool stream, bool exact) {
     constexpr int TH = PW * 64;
+    if (exact) {
+        p.qt == 0 ? launch_prefill_exact<D, PW, true>(g, p, grid, stream) : launch_prefill_exact<D, PW, false>(g, p, grid, stream);
+        return 0;
+    }
     if constexpr (D == 128) {
         // (the streaming forms: half rows with either work-group size, bfloat16 rows - short passes keep them - with 4 waves)
         if (stream && kt == 0) {
@@ -441,8 +468,8 @@ struct PromptPlan {
     bool stream = false;                                          // one work-group reads a key, once: the streaming cache policy
     int waves = 4, pack = 1;                                      // of a work-group; query heads it holds (rows end to end: fl's)
 };
-// The plan of a pass whose arguments have been checked, with `own` floats of scratch: arithmetic on the sizes alone
-PromptPlan prompt_plan(size_t own, int qt, int kt, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t p0, int64_t win, int causal, int64_t kfirst) {
+// The plan of a pass whose arguments have been checked, with `own` floats of scratch: arithmetic on the sizes alone. ends: rows may lie end to end
+PromptPlan prompt_plan(size_t own, int qt, int kt, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t p0, int64_t win, int causal, int64_t kfirst, bool ends = true) {
     // (512 work-groups of 256 rows: two for each of the chip's 256 CUs; NS_PREFILL_WAVES = 4 or 8 overrides, 16 - 12 with
     // work-groups of 4 waves, unsplit - lays rows end to end: tuning, tests)
     PromptPlan pl;
@@ -458,7 +485,7 @@ PromptPlan prompt_plan(size_t own, int qt, int kt, int64_t T, int64_t Hq, int64_
     const int64_t wkf = pl.kf = kfirst >= 0 ? kfirst : win > 0 ? std::max<int64_t>(0, p0 + 1 - win) : 0, wn = pl.keys = p0 + T - wkf;
     const int64_t waves = ns_tune_get(NS_TUNE_PREFILL_WAVES), fit_splits = (int64_t) (own / (size_t) (T * Hq * (D + 2)));
     FlatPlan& fl = pl.fl;
-    if (T * (Hq / Hkv) < ((int64_t) 1 << 31) / (Hq / Hkv)) {
+    if (ends && T * (Hq / Hkv) < ((int64_t) 1 << 31) / (Hq / Hkv)) {
         // (no more splits than leave room to widen the rows behind the partials: 8224 rows x 64 / 8 bfloat16 heads behind 60000 keys, three splits
         // that left none against two: 21.4 -> 14.5 ms, q8_0 16.3 -> 14.9, q4_0 16.0 -> 14.6)
         const size_t wide = kt != 0 ? (size_t) (Hkv * wn * D) + 64 : 0;
@@ -593,7 +620,7 @@ PromptPlan prompt_plan(size_t own, int qt, int kt, int64_t T, int64_t Hq, int64_
 
 int ns_attn_prompt_any(ns_gpu* g, const char* who, int qt, int kt, int pm, const void* q, int64_t qs, const void* kc, const void* vc, int64_t T,
                        int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, int64_t p0, int64_t win, int causal, int64_t kfirst, float scale,
-                       void* out, size_t own) {
+                       void* out, size_t own, bool exact) {
     NS_TRY
     const std::string w(who);
     if (T <= 0) return 0;
@@ -611,7 +638,7 @@ int ns_attn_prompt_any(ns_gpu* g, const char* who, int qt, int kt, int pm, const
     // rows are fetched in 16-byte chunks: every 16-bit row keeps that alignment, q8_0 / q4_0 rows do at D = 256 (272 / 144
     // bytes; the reference's quantized prompt form is D = 256 only); at D = 128 (136 / 72 bytes) the chunks are 8-byte aligned
     if (((uintptr_t) kc | (uintptr_t) vc) % (rb % 16 ? 8 : 16)) return ns_fail(w + (rb % 16 ? ": caches 8-byte aligned" : ": caches 16-byte aligned"));
-    const PromptPlan pl = prompt_plan(own ? own : ns_own_floats(g), qt, kt, T, Hq, Hkv, D, p0, win, causal, kfirst);
+    const PromptPlan pl = prompt_plan(own ? own : ns_own_floats(g), qt, kt, T, Hq, Hkv, D, p0, win, causal, kfirst, !(exact && qt == 0));
     const int PWs = pl.waves;
     const int64_t ROWS = rows_of((int) D, PWs);
     if (T > (int64_t) 1 << 30 || ((T + ROWS - 1) / ROWS + 1) * Hq > (int64_t) 1 << 30) return ns_fail(w + ": too many rows or heads");
@@ -697,8 +724,8 @@ int ns_attn_prompt_any(ns_gpu* g, const char* who, int qt, int kt, int pm, const
         p.pack = p.gw = 1;
         dim3 grid((unsigned) ((Hkv * (p.nbf + (p.ngb - p.nbf) * p.ns) + 7) / 8 * 8 * p.gb));
         if (ns_profile_mark(g, 0)) return -1;
-        if (D == 256) launch_flat<256>(g, kt_run, p, grid, false, false);
-        else launch_flat<128>(g, kt_run, p, grid, pl.stream, fl.waves == 4);
+        if (D == 256) launch_flat<256>(g, kt_run, p, grid, false, false, exact);
+        else launch_flat<128>(g, kt_run, p, grid, pl.stream, fl.waves == 4, exact);
         NS_LAUNCHED("attn_prefill");
         if (ns_profile_mark(g, 1)) return -1;
         if (p.ns > 1) {
@@ -714,8 +741,8 @@ int ns_attn_prompt_any(ns_gpu* g, const char* who, int qt, int kt, int pm, const
     if ((units + 7) / 8 * 8 * p.gw >= (int64_t) 1 << 31) return ns_fail(w + ": too many work-groups");
     dim3 grid((unsigned) ((units + 7) / 8 * 8 * p.gw));
     if (ns_profile_mark(g, 0)) return -1;
-    if ((D == 256 ? (PWs == 8 ? launch_prefill<256, 8>(g, kt_run, p, grid, false) : launch_prefill<256, 4>(g, kt_run, p, grid, false))
-                  : PWs == 8 ? launch_prefill<128, 8>(g, kt_run, p, grid, pl.stream) : launch_prefill<128, 4>(g, kt_run, p, grid, pl.stream)) != 0)
+    if ((D == 256 ? (PWs == 8 ? launch_prefill<256, 8>(g, kt_run, p, grid, false, exact) : launch_prefill<256, 4>(g, kt_run, p, grid, false, exact))
+                  : PWs == 8 ? launch_prefill<128, 8>(g, kt_run, p, grid, pl.stream, exact) : launch_prefill<128, 4>(g, kt_run, p, grid, pl.stream, exact)) != 0)
         return -1;
     NS_LAUNCHED("attn_prefill");
     if (ns_profile_mark(g, 1)) return -1;

@@ -1,10 +1,12 @@
-// attn_prefill_wave.hpp: the body of the prompt kernel (attn_prefill.hip), included where D, BF, KT, PW, QS, NTS, FLAT, RT (a wave's row
+// attn_prefill_wave.hpp: the body of the prompt kernel (attn_prefill.hip), included where D, BF, KT, PW, QS, NTS, XR, FLAT, RT (a wave's row
 // tiles of 16) and p are known: in the kernel itself, and in the function that a FLAT kernel's waves call for one tile or two. (All of it
 // as a function, the kernels that hold whole waves of one head's rows came out with another schedule: q4_0 rows of 128, 19 rows x 64
 // / 4 heads behind 3316 keys 22.9 -> 23.4 us, 25 x 32 / 8 behind 30842 36.2 -> 37.4.)
     static_assert(D == 128 || D == 256, "head size 128 or 256");
     static_assert(KT == 0 || !BF, "quantized rows are widened to half");
-    static_assert(!QS || BF, "query rows in two parts: bfloat16 operands only");
+    static_assert(!QS || BF || XR, "query rows in two parts: bfloat16 operands, or rows of an exponent of their own");
+    static_assert(!XR || (KT == 0 && !BF), "rows of an exponent of their own: over half rows");
+    static_assert(!XR || !QS || !FLAT, "two row tiles of them end to end would spill registers over a tile");
     constexpr int WROWS = RT * 16;
     constexpr int KB = D / 32, DT = D / 16;
     // Half operands: the query enters the first product scaled by the softmax scale x log2 e and rounded once to half - what
@@ -12,7 +14,12 @@
     // the softmax reference (ntile), so a score leaves the matrix unit as the argument of its exponential: no vector
     // instruction a score between the two. bfloat16 operands (8 bits: a second rounding would show) keep the scale in a
     // fused multiply-add a score.
-    constexpr bool PRESCALE = !BF;
+    // XR: no row takes the scale either. It is brought to exponent 13 - 16-bit rows are halfs then, exactly down to 2^-27 of their largest, float32 rows two
+    // (QS) -, whatever its range, and the power of two joins the scale in that multiply-add. With QS the weights are two halfs too, 22 bits; beside 16-bit
+    // rows one: a second would be half the pass's products again for what lies under the output's own rounding. The largest weight
+    // is lifted by 2^7, so that those down to 2^-21 of it keep all of a half's bits (they lie up to 2^15, a half's range ends above).
+    constexpr bool PRESCALE = !BF && !XR, TWO = BF || (XR && QS);   // TWO: weights in two parts
+    constexpr float LIFT = XR ? 7.0f : 0.0f;
     constexpr int KS = padded_row(D), VS = padded_row(D);
     constexpr int KBUF = KT_TILE * KS, VBUF = KT_TILE * VS;
     // DMA: 8 waves over 16-bit rows of 128 stage their tiles global -> LDS directly (global_load_lds_dwordx4: no register in
@@ -76,6 +83,7 @@
     // ---- this lane's two rows: positions, key ranges, Q^T operands
     int64_t lo_r[RT], hi_r[RT];
     s8v qreg[RT][KB], qlo[QS ? RT : 1][KB];
+    float fs[XR ? RT : 1];                                        // XR: what a raw score takes
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int place = wbase + rt * 16 + n;
@@ -85,7 +93,27 @@
         lo_r[rt] = live ? std::max(kbeg, p.kfirst >= 0 ? p.kfirst : p.win > 0 ? std::max<int64_t>(0, pos + 1 - p.win) : 0) : 1;
         hi_r[rt] = live ? std::min(p.causal ? pos : p.p0 + p.T - 1, kend - 1) : 0;
         const int64_t qoff = (int64_t) rr * p.qs + (int64_t) (FLAT ? hk * p.G + (live ? place - rr * p.G : 0) : hq) * D + g4 * 8;
-        if (p.qt == 0) {
+        if constexpr (XR) {
+            float f[KB][8], top = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                if constexpr (QS) load_row<0, 8>(p.q, qoff + kb * 32, f[kb]);
+                else if (p.qt == 1) load_row<1, 8>(p.q, qoff + kb * 32, f[kb]);
+                else load_row<2, 8>(p.q, qoff + kb * 32, f[kb]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(f[kb][i]));
+            }
+            const int e = row_exponent(rows_max(top));
+            const float up = pow2_of(-e);
+            fs[rt] = row_factor(p.sl2, e);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    qreg[rt][kb][i] = to16<false>(f[kb][i] * up);
+                    if constexpr (QS) qlo[rt][kb][i] = to16<false>(f[kb][i] * up - f16_to_f32((uint16_t) qreg[rt][kb][i]));
+                }
+        } else if (p.qt == 0) {
             float4 raw[KB][2];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -336,16 +364,16 @@
     }
     // (bfloat16 operands: a weight enters the second product as two bfloat16 numbers, the rounded weight pb and the rounded
     // rest pl - 16 significant bits between them, where one alone would carry 8 and cost the output ~1.6e-3 of relative L2)
-    s8v pb[RT], pl[BF ? RT : 1];
+    s8v pb[RT], pl[TWO ? RT : 1];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) pb[rt] = s8v{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-    for (int rt = 0; rt < (BF ? RT : 1); ++rt) pl[rt] = s8v{0, 0, 0, 0, 0, 0, 0, 0};
+    for (int rt = 0; rt < (TWO ? RT : 1); ++rt) pl[rt] = s8v{0, 0, 0, 0, 0, 0, 0, 0};
     // S^T of one 32-key half (LDS byte offset kl) against the wave's 32 rows: the raw dot products
     // (the operands of a block's first matrix instructions are read a block earlier - kread / vread - so that their LDS
     // latency passes under the other block's work instead of at the head of this one)
     // (rows in two parts: the registers of half the value operands read ahead go to the rows' second part - no spills)
-    constexpr int VPRE = D == 128 && !QS ? DT : 4;                // value operands read ahead
+    constexpr int VPRE = D == 128 && !QS ? DT : XR && QS && D == 256 ? 1 : 4;     // value operands read ahead
     constexpr int KPRE = D == 128 ? 2 : 1;                        // 16-key halves whose key operands are read ahead
     auto kread = [&](s8v (&ka)[KPRE][KB], const lds_u8* kl) __attribute__((always_inline)) {
 #pragma unroll
@@ -412,7 +440,7 @@
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             l4[rt] = mfma16<BF>(ones, pb[rt], l4[rt]);
-            if constexpr (BF) l4[rt] = mfma16<BF>(ones, pl[rt], l4[rt]);
+            if constexpr (TWO) l4[rt] = mfma16<BF>(ones, pl[rt], l4[rt]);
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
@@ -420,7 +448,7 @@
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 o[rt][dt] = mfma16<BF>(va, pb[rt], o[rt][dt]);
-                if constexpr (BF) o[rt][dt] = mfma16<BF>(va, pl[rt], o[rt][dt]);
+                if constexpr (TWO) o[rt][dt] = mfma16<BF>(va, pl[rt], o[rt][dt]);
             }
         }
     };
@@ -465,7 +493,10 @@
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) a[rt][e] = PRESCALE ? sc[rt][e >> 2][e & 3] : __builtin_fmaf(sc[rt][e >> 2][e & 3], p.sl2, nbr[rt]);
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (XR) a[rt][e] = __builtin_fmaf(sc[rt][e >> 2][e & 3], fs[rt], nbr[rt]);
+                else a[rt][e] = PRESCALE ? sc[rt][e >> 2][e & 3] : __builtin_fmaf(sc[rt][e >> 2][e & 3], p.sl2, nbr[rt]);
+            }
         weigh(vl_prev, vpre);
         bool grow = false;
 #pragma unroll
@@ -479,7 +510,7 @@
         if constexpr (D == 128) {
             // the matrix instructions of this block with two vector instructions between each
 #pragma unroll
-            for (int i = 0; i < (BF ? 2 : 1) * (RT * DT + RT); ++i) {
+            for (int i = 0; i < (TWO ? 2 : 1) * (RT * DT + RT); ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x002, PRESCALE ? 1 : 2, 0);
             }
@@ -491,7 +522,8 @@
                 const float mx = rows_max(amax[rt]);
                 const bool fresh = thr[rt] < 0.0f;
                 const bool nokey = mx == -INFINITY;
-                const float delta = fresh ? (nokey ? 0.0f : mx) : fmaxf(mx, 0.0f);
+                const float up = XR ? mx - LIFT : mx;
+                const float delta = fresh ? (nokey ? 0.0f : up) : fmaxf(up, 0.0f);
                 const float c = fresh ? 1.0f : fast_exp2(-delta);
                 l4[rt] *= c;
 #pragma unroll
@@ -503,7 +535,7 @@
                 // (end to end under a window a wave's few rows begin at one key half, whose maximum would stay their reference; 32 rows of one head
                 // begin at two. With the second half's too, the largest weights are 1 - a half as it is - as often as there: 2001 x 32 / 2, window
                 // 1024, 2.969e-4 of relative L2 from float64 in whole waves of a head, 2.971e-4 end to end, 2.961e-4 so, for 0.1 of 43.2 us)
-                thr[rt] = fresh && nokey ? -INFINITY : FLAT && PRESCALE && fresh && p.win > 0 ? 0.0f : 8.0f;
+                thr[rt] = fresh && nokey ? -INFINITY : FLAT && PRESCALE && fresh && p.win > 0 ? 0.0f : 8.0f + LIFT;
             }
         }
         scores(sn, kl_next, kpre);
@@ -514,6 +546,7 @@
                 const float pv = fast_exp2(a[rt][e]);                                   // -inf -> 0
                 pb[rt][e] = to16<BF>(pv);
                 if constexpr (BF) pl[rt][e] = to16<BF>(pv - __builtin_bit_cast(float, (uint32_t) (uint16_t) pb[rt][e] << 16));
+                else if constexpr (TWO) pl[rt][e] = to16<false>(pv - f16_to_f32((uint16_t) pb[rt][e]));
             }
         }
         if constexpr (D == 128) {
@@ -528,8 +561,8 @@
         // the step's results are complete here, in program order: nothing of it drifts past the next barrier or branch
         if constexpr (RT == 2) asm volatile("" : "+v"(pb[0]), "+v"(pb[1]));
         else asm volatile("" : "+v"(pb[0]));
-        if constexpr (BF && RT == 2) asm volatile("" : "+v"(pl[0]), "+v"(pl[1]));
-        else if constexpr (BF) asm volatile("" : "+v"(pl[0]));
+        if constexpr (TWO && RT == 2) asm volatile("" : "+v"(pl[0]), "+v"(pl[1]));
+        else if constexpr (TWO) asm volatile("" : "+v"(pl[0]));
         __builtin_amdgcn_s_setprio(0);
     };
 

@@ -3,8 +3,9 @@ stored into hold anything at all, not finite numbers among it."""
 import numpy as np
 import pytest
 
-from kv8_ref import BF16, E4M3, F16, F32, INT8, from_type, to_type
+from kv8_ref import BF16, E4M3, F16, F32, INT8, Cache, from_type, to_type, tolerance
 from nextsycl_amd import DevBuf
+from nextsycl_amd.attn import TUNE_PREFILL_SPLITS, TUNE_PREFILL_WAVES
 from test_gpu_kv8 import attend, filled, ints, on_gpu, prompt_close, rows_of, tables
 
 pytestmark = pytest.mark.gpu
@@ -89,3 +90,100 @@ def test_a_tokens_16_bit_rows_are_rounded_once(ops, form, qt, Hq, Hkv, D, B, len
     ref = np.concatenate([c.attend(qv[start[s]:start[s + 1]], table, s, lens[s], win)[0] for s in range(S)])
     rounded = to_type(qt, ref)[1]
     assert np.linalg.norm(from_type(qt, raw) - ref) <= np.linalg.norm(rounded - ref) + 2 * 2.0 ** -17 * np.linalg.norm(ref)
+
+
+def one_prompt(r, form, qt, Hq, Hkv, D, B, T, p0, rows=1.0, keys=0.7):
+    n = p0 + T
+    tmax = (n + B - 1) // B
+    table = tables(r, 1, tmax, tmax)
+    c = Cache(form, tmax, Hkv, B, D, seed=B)
+    k, v = (r.standard_normal((n, Hkv, D)) * sigma * np.exp(0.4 * r.standard_normal((1, Hkv, D))) for sigma in (keys, 1.0))
+    c.store(k, v, table, [0], [0, n], n)
+    q, qs, _ = rows_of(F32, r, T, Hq, D)
+    q, qv = to_type(qt, q.reshape(T, Hq, D) * np.float32(rows))
+    return c, table, q, qv
+
+
+def run_prompt(ops, c, qt, q, table, p0, Hq, win=0, scale=0.0):
+    ob = DevBuf(ops.gpu, q.shape[0] * Hq * c.D * (4 if qt == F32 else 2))
+    ops.kv8_prompt(on_gpu(ops, c), qt, DevBuf.of(ops.gpu, q), Hq * c.D, q.shape[0], ints(ops, table), table.shape[1], p0, Hq, ob, win=win, scale=scale)
+    ops.gpu.sync()
+    return ob.read(np.float32 if qt == F32 else np.uint16).reshape(q.shape)
+
+
+def check_prompt(qt, raw, ref, qv, k, v, D, scale=0.0, what=""):
+    """A prompt's rows as a token's (`tolerance`), but for what sums up beside 16-bit rows: numerator and sum of a row carry the same weights of 11 bits there, and
+    sum w (1 + d) v / sum w (1 + d) moves by sum w d (v - mean) / sum w, twice vmax 2^-11 at most."""
+    got = from_type(qt, raw)
+    Hq, Hkv = qv.shape[1], k.shape[1]
+    reach = max(float((np.abs(qv[:, h]) @ np.abs(k[:, h * Hkv // Hq]).T).max()) for h in range(Hq)) * (scale or D ** -0.5) * np.log2(np.e)
+    vmax = float(np.abs(v).max())
+    tol, rel = tolerance(qt, ref, reach, vmax, D, len(k))
+    tol += 0.0 if qt == F32 else vmax * 2.0 ** -11
+    assert np.isfinite(got).all(), what
+    assert np.abs(got - ref).max() <= tol, "%s: %.3g (<= %.3g)" % (what, np.abs(got - ref).max(), tol)
+    assert np.linalg.norm(got - ref) <= rel * np.linalg.norm(ref), "%s: relative L2 %.3g (<= %.3g)" % (what, np.linalg.norm(got - ref) / np.linalg.norm(ref), rel)
+
+
+LONG = [  # Hq, Hkv, D, B, T, p0, window, waves, splits
+    (8, 2, 128, 64, 17, 300, 0, 0, 0),
+    (6, 3, 256, 16, 33, 70, 0, 0, 0),
+    (16, 2, 128, 32, 40, 2000, 0, 0, 0),
+    (8, 2, 256, 64, 40, 2000, 0, 0, 0),
+    (8, 8, 128, 32, 300, 0, 0, 8, 0),
+    (4, 4, 256, 128, 200, 31, 0, 8, 0),
+    (10, 2, 128, 16, 150, 500, 100, 4, 3),
+    (12, 2, 256, 32, 70, 900, 0, 4, 2),
+    (12, 3, 128, 32, 90, 700, 0, 16, 2),
+    (12, 3, 128, 32, 200, 100, 64, 12, 0),
+    (8, 1, 256, 32, 60, 300, 0, 16, 0),
+]
+
+
+@pytest.mark.parametrize("form", [INT8, E4M3])
+@pytest.mark.parametrize("qt", [F32, F16, BF16])
+@pytest.mark.parametrize("Hq,Hkv,D,B,T,p0,win,waves,splits", LONG)
+def test_prompts_of_more_than_16_rows_keep_a_tokens_bits(ops, tune, form, qt, Hq, Hkv, D, B, T, p0, win, waves, splits):
+    """Float32 rows 22 bits of themselves and of their weights, whatever form the pass takes; 16-bit rows all of theirs."""
+    r = np.random.default_rng(T + D)
+    c, table, q, qv = one_prompt(r, form, qt, Hq, Hkv, D, B, T, p0)
+    if waves:
+        tune(TUNE_PREFILL_WAVES, waves)
+    if splits:
+        tune(TUNE_PREFILL_SPLITS, splits)
+    raw = run_prompt(ops, c, qt, q, table, p0, Hq, win)
+    check_prompt(qt, raw, c.attend(qv, table, 0, p0, win)[0], qv, *c.tokens(table, 0, p0 + T), D)
+
+
+@pytest.mark.parametrize("form", [INT8, E4M3])
+@pytest.mark.parametrize("qt,rows,keys", [(F32, 2.0 ** 18, 2.0 ** -18), (BF16, 2.0 ** 18, 2.0 ** -18), (F16, 2.0 ** 11, 2.0 ** -11), (F32, 2.0 ** -14, 2.0 ** 13), (BF16, 2.0 ** -14, 2.0 ** 13),
+                                          (F16, 2.0 ** -12, 2.0 ** 12)])
+@pytest.mark.parametrize("Hq,Hkv,D,B,T,p0", [(8, 2, 128, 32, 40, 300), (4, 2, 256, 64, 40, 60), (16, 2, 128, 16, 20, 3000), (8, 1, 256, 16, 30, 2000)])
+def test_prompts_rows_of_any_range(ops, form, qt, rows, keys, Hq, Hkv, D, B, T, p0):
+    """Rows far outside a half's range, or where its steps are wide, against keys that bring the scores back."""
+    r = np.random.default_rng(T)
+    c, table, q, qv = one_prompt(r, form, qt, Hq, Hkv, D, B, T, p0, rows, keys)
+    check_prompt(qt, run_prompt(ops, c, qt, q, table, p0, Hq), c.attend(qv, table, 0, p0)[0], qv, *c.tokens(table, 0, p0 + T), D)
+
+
+@pytest.mark.parametrize("form", [INT8, E4M3])
+@pytest.mark.parametrize("rows,scale", [(2.0 ** 122, 2.0 ** -125), (2.0 ** 100, 2.0 ** -103), (2.0 ** -100, 2.0 ** 97)])
+def test_prompts_at_the_ends_of_float32(ops, form, rows, scale):
+    """Rows of every magnitude, a scale that brings the scores back (below 2^-107 the rows keep fewer bits: not asked for here); rows of zeros; NaN and
+    infinities stay in their row and head."""
+    Hq, Hkv, D, B, T, p0 = 4, 2, 128, 16, 24, 60
+    r = np.random.default_rng(5)
+    c, table, q, _ = one_prompt(r, form, F32, Hq, Hkv, D, B, T, p0, 1.0, 0.7)
+    q = q * np.float32(rows)
+    q[3] = 0
+    qv = q.astype(np.float64)
+    ref, _ = c.attend(qv, table, 0, p0, scale=scale)
+    k, v = c.tokens(table, 0, p0 + T)
+    check_prompt(F32, run_prompt(ops, c, F32, q, table, p0, Hq, scale=scale), ref, qv, k, v, D, scale)
+    q[5, 1, 7], q[9, 2, 3], q[11, 0, 2] = np.nan, np.inf, -np.inf
+    raw = run_prompt(ops, c, F32, q, table, p0, Hq, scale=scale)
+    bad = np.zeros((T, Hq), bool)
+    bad[[5, 9, 11], [1, 2, 0]] = True
+    assert np.isnan(raw[bad]).all()
+    rel = np.linalg.norm(raw[~bad].astype(np.float64) - ref[~bad]) / np.linalg.norm(ref[~bad])
+    assert rel <= 2.0 ** -17 + 2.0 ** -24
