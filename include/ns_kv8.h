@@ -42,7 +42,7 @@ int ns_kv8_store(ns_gpu* g, int form, int qt, const void* k, int64_t ks, const v
  * sees nothing: zeros. scratch:
  * ns_kv8_attend_scratch(..) floats, 16-byte aligned (0: may be null).
  * acc1 not null: acc1 = acc0 + the weights of this call's rows, for every token in front of lens[s] + its rows (acc0 null, and
- * tokens of this call: 0 + them); acc1 may be acc0. A block that is given weights belongs to one sequence of the call. */
+ * tokens of this call: 0 + them; to tokens from `longest` on none are given); acc1 may be acc0. A block that is given weights belongs to one sequence of the call. */
 int64_t ns_kv8_attend_scratch(int64_t S, int64_t most, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest, int acc);
 int ns_kv8_attend(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_t T, const int32_t* start, const int32_t* lens, int64_t S, int64_t most,
                   int64_t longest, const int32_t* table, int64_t tmax, int64_t Hq, int64_t Hkv, int64_t D, int64_t block, int64_t blocks, const void* kc,

@@ -723,6 +723,9 @@ __device__ __forceinline__ void give(const AttendParams& p, int64_t place, uint8
         }
         __syncthreads();                                          // (the numbers are read)
     }
+    // (tokens from `longest` on, if a sequence has any: nothing was given to them. Its last work-group's)
+    if (place - unit * runs == runs - 1)
+        for (int64_t t = (runs * tokens + tid) * 4; t < (int64_t) q.len + q.n; t += TH * 4) Given(p, q, s, hk, t).give(p, q);
     if (p.pg > 1) {
         sums[tid] = given.sum;
         __syncthreads();

@@ -187,3 +187,33 @@ def test_prompts_at_the_ends_of_float32(ops, form, rows, scale):
     assert np.isnan(raw[bad]).all()
     rel = np.linalg.norm(raw[~bad].astype(np.float64) - ref[~bad]) / np.linalg.norm(ref[~bad])
     assert rel <= 2.0 ** -17 + 2.0 ** -24
+
+
+# ---- sequences longer than said
+
+@pytest.mark.parametrize("Hq,Hkv,S,most,longest,lens", [(8, 4, 4, 2, 60, [40, -5, 100, 700]), (64, 2, 2, 3, 100, [3000, 90]), (4, 1, 1, 1, 900, [5000]), (16, 8, 40, 1, 9000, [300, 12000, 9001] + 37 * [50]),
+                                                        (32, 1, 1, 16, 500, [2000])])
+@pytest.mark.parametrize("acc0", [True, False])
+def test_weights_of_tokens_past_longest(ops, Hq, Hkv, S, most, longest, lens, acc0):
+    """acc1 = acc0 + what is given for every token in front of a sequence's end, those from `longest` on too - nothing is given to them -, whether a work-group sums
+    up its own unit, the chunks are a work-group's each or lie end to end."""
+    r = np.random.default_rng(longest)
+    D, B = 128, 16
+    n = max(lens) + most
+    tmax = (n + B - 1) // B - 1                          # (and the last tokens lie behind the table)
+    one = tables(r, 1, tmax, tmax)[0]
+    c = Cache(INT8, S * tmax, Hkv, B, D, seed=2)
+    c.k[:], c.v[:] = (r.integers(-127, 128, c.k.shape).astype(np.int8).view(np.uint8) for _ in range(2))
+    c.ks[:], c.vs[:] = (2.0 ** r.integers(-8, -5, c.ks.shape) for _ in range(2))
+    table = (one + np.arange(S)[:, None] * tmax).astype(np.int32)
+    start = np.arange(S + 1) * most
+    q, qs, qv = rows_of(F32, r, S * most, Hq, D)
+    was = r.uniform(0, 3, (c.blocks, Hkv, B)).astype(np.float32)
+    want = np.full(was.shape, -1.0)
+    a1 = DevBuf.of(ops.gpu, np.full_like(was, -1))
+    attend(ops, c, on_gpu(ops, c), F32, q, qs, table, lens, start, S * most, most, Hq, longest=longest, acc0=DevBuf.of(ops.gpu, was) if acc0 else None, acc1=a1)
+    for s in range(S):
+        if lens[s] >= 0:
+            _, given = c.attend(qv[start[s]:start[s + 1]], table, s, lens[s], longest=longest)
+            c.give(was.astype(np.float64) if acc0 else None, want, table, s, lens[s], given)
+    assert np.abs(a1.read(np.float32).reshape(was.shape) - want).max() <= 2.0 ** -17 * max(1.0, want.max())
