@@ -38,8 +38,8 @@ int ns_kv8_store(ns_gpu* g, int form, int qt, const void* k, int64_t ks, const v
 /* Attention of a token, or a few (most 1 .. 16), of each of S sequences, whose keys are stored already: out [T][Hq D] =
  * softmax(scale q . k) v over the tokens up to the row's own, of the last `win` (win <= 0: of all); scale <= 0: 1 / sqrt(D). `longest`: no
  * token from that position on is read (a bound that the caller knows on every lens[s] + its rows; splits and scratch follow from it). S x most x Hq: under 2^31.
- * Half and bfloat16 rows enter the products exactly (values down to 2^-27 of a row and head's largest), float32 rows and the softmax weights with 22 bits. A row that
- * sees nothing: zeros. scratch:
+ * Half and bfloat16 rows enter the products exactly (values down to 2^-27 of a row and head's largest), float32 rows (of largest values from 2^-107 up) and the
+ * softmax weights with 22 bits. A row that sees nothing: zeros. scratch:
  * ns_kv8_attend_scratch(..) floats, 16-byte aligned (0: may be null).
  * acc1 not null: acc1 = acc0 + the weights of this call's rows, for every token in front of lens[s] + its rows (acc0 null, and
  * tokens of this call: 0 + them; to tokens from `longest` on none are given); acc1 may be acc0. A block that is given weights belongs to one sequence of the call. */

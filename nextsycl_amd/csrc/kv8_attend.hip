@@ -342,9 +342,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void kv8_attend_kernel(const AttendP
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const float top = rows_max(most[rt]);
-                const int e = top > 0.0f ? std::min(std::max((int) (__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 13, -110), 110) : 0;
-                const float up = kv8_pow2(-e);
-                qm[rt] = p.sl2 * kv8_pow2(e);
+                const int e = row_exponent(top);
+                const float up = pow2_of(-e);
+                qm[rt] = row_factor(p.sl2, e);
 #pragma unroll
                 for (int j = 0; j < 2 * KJ; ++j)
 #pragma unroll

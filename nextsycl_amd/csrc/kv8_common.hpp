@@ -60,7 +60,6 @@ __device__ __forceinline__ int kv8_exponent(float a) {
     const int e = (int) (u >> 23) - 127 - F::WIDTH + ((u & 0x7FFFFFu) > F::TOP);
     return min(max(e, F::LO), F::HI);
 }
-__device__ __forceinline__ float kv8_pow2(int e) { return __builtin_bit_cast(float, (uint32_t) (e + 127) << 23); }
 
 // 4 values in units of their scale -> 4 codes, nearest even, magnitudes held to the largest (NaN: 0)
 template <int FORM>

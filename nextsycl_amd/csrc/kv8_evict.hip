@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256) void kv8_move_kernel(const EvictParams p) {
     if (tid < 128) scale[tid] = mine == NONE ? 0.0f : (val ? p.c.vsc : p.c.ksc)[mine >> p.c.shift];
     const float a = !val && tid < rows && mine != NONE ? p.acc[mine] : 0.0f;
     __syncthreads();
-    const float most = wave_max(fmaxf(kv8_pow2(Kv8Form<FORM>::LO), fmaxf(scale[tid % 64], scale[64 + tid % 64])));
+    const float most = wave_max(fmaxf(pow2_of(Kv8Form<FORM>::LO), fmaxf(scale[tid % 64], scale[64 + tid % 64])));
     const int64_t place = ((int64_t) gs * p.nb + j) * p.nh + hk;
     uint8_t* out = p.to ? (val ? p.c.vc : p.c.kc) + (int64_t) to0 * p.c.D : p.stage + (place * 2 + val) * B * p.c.D;
 #pragma unroll

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(TH) void kv8_store_kernel(const StoreParams p) {
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < TH / 64; ++w) most = fmaxf(most, red[w]);
-    const float s1 = fmaxf(s0, kv8_pow2(kv8_exponent<FORM>(most))), inv = 1.0f / s1, ratio = s0 * inv;
+    const float s1 = fmaxf(s0, pow2_of(kv8_exponent<FORM>(most))), inv = 1.0f / s1, ratio = s0 * inv;
     if (!fresh && s1 > s0) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {

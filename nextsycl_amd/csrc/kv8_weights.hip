@@ -61,8 +61,8 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const WeightsParams p) {
         for (int k = 0; k < 8; ++k) x[j + k] = v[k], most = fmaxf(most, fabsf(v[k]));
     }
     most = row16_max(most);
-    const int e = most > 0.0f ? std::min(std::max((int) (__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 13, -110), 110) : 0;
-    const float up = kv8_pow2(-e);
+    const int e = row_exponent(most);
+    const float up = pow2_of(-e);
     uint8_t* to = p.q16 + ((int64_t) h * p.tiles + blockIdx.x) * TILE_BYTES;
 #pragma unroll
     for (int j = 0; j < E; j += 8) {
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const WeightsParams p) {
         *reinterpret_cast<s8v*>(to + place) = a;
         if constexpr (QT == 0) *reinterpret_cast<s8v*>(to + KB * 1024 + place) = b;
     }
-    if (li == 0 && pair < p.pairs) p.info[(int64_t) h * p.pairs + pair].x = p.sl2 * kv8_pow2(e);
+    if (li == 0 && pair < p.pairs) p.info[(int64_t) h * p.pairs + pair].x = row_factor(p.sl2, e);
 }
 
 // pairs a key head, and scores in all, up to which the rows go as a token's do, the keys once more in the place of the values: two launches, not four or

@@ -217,3 +217,55 @@ def test_weights_of_tokens_past_longest(ops, Hq, Hkv, S, most, longest, lens, ac
             _, given = c.attend(qv[start[s]:start[s + 1]], table, s, lens[s], longest=longest)
             c.give(was.astype(np.float64) if acc0 else None, want, table, s, lens[s], given)
     assert np.abs(a1.read(np.float32).reshape(was.shape) - want).max() <= 2.0 ** -17 * max(1.0, want.max())
+
+
+# ---- rows of every magnitude that float32 has
+
+ENDS = [(2.0 ** 123, 2.0 ** -126), (2.0 ** 100, 2.0 ** -103), (2.0 ** -104, 2.0 ** 101)]
+
+
+def end_rows(r, form, Hq, Hkv, D, B, T, p0, rows):
+    """The largest value 2^127 and more where rows are 2^123; a row of zeros."""
+    c, table, q, _ = one_prompt(r, form, F32, Hq, Hkv, D, B, T, p0)
+    q = np.clip(q, -15.5, 15.5) * np.float32(rows)
+    q[0, 0, 3] = np.float32(15.5) * np.float32(rows)
+    if T > 2:
+        q[2] = 0
+    return c, table, q, q.astype(np.float64)
+
+
+@pytest.mark.parametrize("form", [INT8, E4M3])
+@pytest.mark.parametrize("rows,scale", ENDS)
+@pytest.mark.parametrize("Hq,Hkv,D,B,T,p0", [(8, 2, 128, 32, 1, 500), (4, 2, 256, 16, 9, 60), (6, 2, 128, 64, 40, 300), (4, 1, 256, 32, 20, 100)])
+def test_rows_at_the_ends_of_float32(ops, form, rows, scale, Hq, Hkv, D, B, T, p0):
+    """A scale, or keys, that bring the scores back: tokens' rows (up to 16), prompts, weights."""
+    r = np.random.default_rng(T)
+    c, table, q, qv = end_rows(r, form, Hq, Hkv, D, B, T, p0, rows)
+    ref, given = c.attend(qv, table, 0, p0, scale=scale)
+    k, v = c.tokens(table, 0, p0 + T)
+    check_prompt(F32, run_prompt(ops, c, F32, q, table, p0, Hq, scale=scale), ref, qv, k, v, D, scale, "prompt")
+    want = np.zeros((c.blocks, Hkv, B))
+    c.give(None, want, table, 0, p0, given)
+    acc = DevBuf.of(ops.gpu, np.zeros(want.shape, np.float32))
+    if T <= 16:
+        raw = attend(ops, c, on_gpu(ops, c), F32, q, Hq * D, table, np.array([p0]), np.array([0, T]), T, T, Hq, scale=scale, acc1=acc)
+        check_prompt(F32, raw, ref, qv, k, v, D, scale, "tokens")
+        assert np.abs(acc.read(np.float32).reshape(want.shape) - want).max() <= 2.0 ** -17 * max(1.0, want.max())
+    ops.kv8_weights(on_gpu(ops, c), F32, DevBuf.of(ops.gpu, q), Hq * D, T, ints(ops, table), table.shape[1], p0, Hq, None, acc, scale=scale)
+    assert np.abs(acc.read(np.float32).reshape(want.shape) - want).max() <= 2.0 ** -17 * max(1.0, want.max())
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_rows_that_a_small_scale_makes_nothing_of(ops, T):
+    """Scores of 2^-140 and less: a mean of all that a row sees, also where tokens are masked."""
+    r = np.random.default_rng(T)
+    c, table, q, qv = end_rows(r, INT8, 4, 2, 128, 16, T, 90, 2.0 ** -110)
+    scale = 2.0 ** -60
+    ref, given = c.attend(qv, table, 0, 90, 50, scale=scale)
+    k, v = c.tokens(table, 0, 90 + T)
+    check_prompt(F32, run_prompt(ops, c, F32, q, table, 90, 4, 50, scale), ref, qv, k, v, 128, scale)
+    want = np.zeros((c.blocks, 2, 16))
+    c.give(None, want, table, 0, 90, given)
+    acc = DevBuf.of(ops.gpu, np.zeros(want.shape, np.float32))
+    ops.kv8_weights(on_gpu(ops, c), F32, DevBuf.of(ops.gpu, q), 512, T, ints(ops, table), table.shape[1], 90, 4, None, acc, win=50, scale=scale)
+    assert np.abs(acc.read(np.float32).reshape(want.shape) - want).max() <= 2.0 ** -17 * max(1.0, want.max())
