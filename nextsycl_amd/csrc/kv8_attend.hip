@@ -908,6 +908,7 @@ int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     NS_HIP(hipSetDevice(g->dev));
     NS_OWN_SCRATCH(g);
     const size_t own = ns_own_floats(g);
+    win = kv8_window(win);
     // the tokens that the rows see, from a block's first on, widened at the scratch's end; the pass plans with what is in front of them. (From the 17th row
     // on, whatever the heads: where few share a key head two trips of 16 and 1 rows would be shorter, 17 x 8 / 8 heads behind 20000 34.7 us, widened 42.9)
     const int64_t from = win > 0 ? std::max<int64_t>(0, p0 + 1 - win) >> c.shift << c.shift : 0, n = p0 + T - from;
@@ -915,11 +916,11 @@ int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     if (T > DECODE_ROWS && wide <= own / 4 * 3 && n * D * 2 < (int64_t) 1 << 32) {
         uint16_t* k = reinterpret_cast<uint16_t*>(g->own_scratch + (own - wide) / 64 * 64);
         if (ns_kv8_widen(g, form, c, from, n, k, k + Hkv * n * D)) return -1;
-        return ns_attn_prompt_any(g, "ns_kv8_prompt", qt, 0, 0, q, qs, k, k + Hkv * n * D, T, Hq, Hkv, D, n, p0 - from, win > 0 ? win : 0, 1, -1, scale, out,
+        return ns_attn_prompt_any(g, "ns_kv8_prompt", qt, 0, 0, q, qs, k, k + Hkv * n * D, T, Hq, Hkv, D, n, p0 - from, win, 1, -1, scale, out,
                                   (own - wide) / 64 * 64, true);
     }
     AttendParams p{};
-    p.c = c, p.qs = qs, p.S = 1, p.Hq = (int) Hq, p.G = (int) (Hq / Hkv), p.win = kv8_window(win);
+    p.c = c, p.qs = qs, p.S = 1, p.Hq = (int) Hq, p.G = (int) (Hq / Hkv), p.win = win;
     p.sl2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float) D)) * 1.4426950408889634f;
     for (int64_t t = 0; t < T; t += DECODE_ROWS) {
         const int64_t rows = std::min(DECODE_ROWS, T - t);

@@ -269,3 +269,13 @@ def test_rows_that_a_small_scale_makes_nothing_of(ops, T):
     acc = DevBuf.of(ops.gpu, np.zeros(want.shape, np.float32))
     ops.kv8_weights(on_gpu(ops, c), F32, DevBuf.of(ops.gpu, q), 512, T, ints(ops, table), table.shape[1], 90, 4, None, acc, win=50, scale=scale)
     assert np.abs(acc.read(np.float32).reshape(want.shape) - want).max() <= 2.0 ** -17 * max(1.0, want.max())
+
+
+@pytest.mark.parametrize("qt,Hq,Hkv,D,T,p0", [(BF16, 8, 2, 128, 40, 260), (F32, 8, 8, 128, 300, 3), (F16, 4, 2, 256, 150, 50)])
+def test_a_prompts_window_longer_than_any_sequence(ops, qt, Hq, Hkv, D, T, p0):
+    """The bits of none, up to the longest there is to say."""
+    r = np.random.default_rng(T)
+    c, table, q, _ = one_prompt(r, INT8, qt, Hq, Hkv, D, 32, T, p0)
+    first = run_prompt(ops, c, qt, q, table, p0, Hq)
+    for win in (-1, 1 << 31, (1 << 62) + 3, (1 << 63) - 1):
+        assert np.array_equal(run_prompt(ops, c, qt, q, table, p0, Hq, win), first), win
