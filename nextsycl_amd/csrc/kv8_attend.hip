@@ -2,9 +2,9 @@
 // blocks of tokens (gfx950).
 //
 // Bound: HBM - every visible key and value byte read once for all rows and query heads of its key head; 4 D flops a (row, head,
-// token), far under the matrix unit's ridge. (64 sequences of 126 to 8000 tokens x 32 / 8 heads of 128, 252 MB: 50.0 us, 6.2 TB/s between a start of 7 us and the
-// merge's 5; a half row behind 131071 tokens with weights, 64 / 4 heads: 48.2; 12 float32 rows of 3 sequences behind 10698 to 43003, 24 / 4 heads of 256: 40.2, the
-// widening's and the two halfs' instructions beside 134 MB; a row behind 4095, 32 / 8 heads: 11.0, two launches)
+// token), far under the matrix unit's ridge. (64 sequences of 126 to 8000 tokens x 32 / 8 heads of 128, 258 MB: 55.6 us, 6.0 TB/s between a start of 7 us and the
+// merge's 5; a half row behind 131071 tokens with weights, 64 / 4 heads: 49.3; 7 float32 rows of 3 sequences behind 2398 to 43003, 24 / 4 heads of 256: 40.1, the
+// widening's and the two halfs' instructions beside 131 MB; a row behind 4095, 32 / 8 heads: 11.2, two launches)
 //
 // Work split: the lengths are known on the device only, and differ. Short contexts are a work-group's each; a few longer ones take a work-group a chunk of 128
 // tokens; else the tokens of all sequences and key heads lie end to end in chunks, and each work-group takes an equal run of them (with a grid over the longest
@@ -132,8 +132,9 @@ struct Given {
 };
 
 // What a unit - a sequence's key head - costs besides its chunks, in chunks: its rows' way in, its sums' way out (2.2 us, where a chunk's bytes take
-// 3 of a full chip's). Runs are dealt by chunks and that where there are more chunks than work-groups. (64 sequences of 125 to 8000 tokens x 8 heads, 768 work-groups:
-// 63.7 us without it, 57.7 with 1, 57.8 with 2, 58.8 with 3, 512 work-groups: 54.8 with 2, 55.6 with 3; 4 rows of 3 sequences behind 43003 44.8 / 44.8 / 42.6 / 42.7)
+// 3 of a full chip's). Runs are dealt by chunks and that where there are more chunks than work-groups. (64 sequences of 125 to 8000 tokens x 8 heads:
+// 72 us without it, 61.4 with 1, 57.2 with 2, 57.8 with 3; up to 4 float32 rows of each x 4 heads of 256, 62 to 4000 tokens, 84 / 63.8 / 59.2 / 57.2; of 3 sequences of up
+// to 43003 48.2 / 46.5 / 44.8 / 44.0)
 constexpr int EXTRA = 2;
 // a sequence's chunks a key head: chunk `first` and on (a sequence with rows has one at least)
 __device__ __forceinline__ int chunks_of(const AttendParams& p, const Kv8Seq& q, int& first) {
@@ -764,8 +765,8 @@ void launch_join(ns_gpu* g, const AttendParams& p, int64_t rows, int64_t grid) {
 int tiles_of(int64_t pairs, int64_t D) { return pairs > 16 && D == 128 ? 2 : 1; }
 int64_t pair_chunks(int64_t pairs, int64_t D) { const int64_t rows = 16 * tiles_of(pairs, D); return (pairs + rows - 1) / rows; }
 // chunks up to which work-groups take a unit each, by the number of units: nothing is put together behind them then, and no run is looked for. 2 of 4 units, 4 of
-// 8, 10 of 64, 12 of 128, 16 of 512 and more. (us, a unit each against runs: 8 units of 400 tokens 9.9 / 11.1, of 800 13.7 / 11.5; 4 units of 24 rows of 256
-// features, 200 tokens 12.1 / 14.0, 400 15.9 / 14.4; 128 units of 800 tokens 14.1 / 17.6, of 1600 21.2 / 21.3; 512 units of 1600 38.2 / 48.8)
+// 8, 10 of 64, 12 of 128, 16 of 512 and more. (us, a unit each against runs: 8 units of 400 tokens 10.3 / 11.4, of 800 14.5 / 11.6; 4 units of 24 rows of 256
+// features, 200 tokens 11.9 / 14.4, 400 15.6 / 13.9; 128 units of 800 tokens 14.9 / 18.3, of 1600 22.6 / 21.0; 512 units of 1600 38.5 / 43.0)
 int64_t whole_chunks(int64_t units) {
     int64_t log2 = 0;
     while (units >> (log2 + 1)) ++log2;
@@ -773,9 +774,10 @@ int64_t whole_chunks(int64_t units) {
 }
 // How the tokens are dealt out. A work-group a piece of at most `per` chunks of a unit: all of its chunks where contexts are short (above), one where 512
 // work-groups, two a CU, are enough for that - its table entries are asked for beside its length then, not behind it (us, beside runs: 3 sequences of 800
-// tokens x 8 heads 11.4 / 13.0, 4 rows of each x 4 heads of 256 15.7 / 17.7, a token behind 4095 11.5 / 11.7). Else
-// runs, on as many work-groups. (64 sequences of 125 to 8000 tokens x 8 heads of 128: 448 work-groups 56.3 us, 512 54.8, 640 61.9, 768 57.6; all of 8000: 175 / 169 /
-// 189 / 179; 4 rows of each of 64 x 24 / 4 heads of 256, two chunks of pairs, 4000 tokens: 192 pairs of work-groups 173, 256 133)
+// tokens x 8 heads 11.5 / 13.0, 4 rows of each x 4 heads of 256 15.1 / 17.1, a token behind 4095 12.0 / 12.0; the wrong side, 3 sequences of 25 to 1600 - every
+// one's places are counted at the longest - 18.3 / 16.8). Else
+// runs, on as many work-groups. (64 sequences of 125 to 8000 tokens x 8 heads of 128: 448 work-groups 59.0 us, 512 57.2, 640 64.5, 768 59.4; all of 8000: 180 / 171 /
+// 195 / 181; 4 rows of each of 64 x 24 / 4 heads of 256, two chunks of pairs, 4000 tokens: 192 pairs of work-groups 172, 256 136)
 struct Deal {
     int64_t nw, per, ns;
 };
@@ -822,10 +824,10 @@ int attend(ns_gpu* g, const std::string& w, int form, int qt, AttendParams p, in
     p.units = deal.per ? nullptr : (int2*) (scratch + x.part + x.ml);
     p.scores = p.acc1 ? scratch + x.part + x.ml + x.units : nullptr;
     p.stats = p.acc1 ? (float2*) (scratch + x.part + x.ml + x.units + x.scores) : nullptr;
-    // (a unit's work-group, where it has all its pairs, sums up their weights too: 8 heads behind 100 tokens 9.2 us, in a launch of their own 12.0; 64 sequences behind
-    // 800 25.9 / 27.8)
+    // (a unit's work-group, where it has all its pairs, sums up their weights too: 8 heads behind 100 tokens 9.2 us, in a launch of their own 11.6; 64 sequences behind
+    // 800 28.1 / 30.7)
     p.alone = p.acc1 && deal.per && deal.ns == 1 && nz == 1;
-    // (up to 16 pairs a thread's, while that leaves the chip empty: 256 pairs of 4 key heads behind 500 tokens 20.8 us, all by one thread 60.6; behind 30000 102, 127)
+    // (up to 16 pairs a thread's, while that leaves the chip empty: 256 pairs of 4 key heads behind 500 tokens 21.0 us, all by one thread 60.1; behind 30000 104, 128)
     for (p.pg = 1; p.pg < 16 && p.pg * 16 < pairs && (p.longest * p.pg + 4 * TH - 1) / (4 * TH) * Hkv * p.S < 512;) p.pg *= 2;
     const int64_t merges = pieces ? rows : 0, tokens = 4 * TH / p.pg, gives = p.acc1 && !p.alone ? (p.longest + tokens - 1) / tokens * Hkv * p.S : 0;
     if (!ns_grid_fits(grid, 256) || !ns_grid_fits(merges + gives, TH)) return ns_fail(w + ": more work-groups than a launch takes");
@@ -910,7 +912,8 @@ int ns_kv8_prompt(ns_gpu* g, int form, int qt, const void* q, int64_t qs, int64_
     const size_t own = ns_own_floats(g);
     win = kv8_window(win);
     // the tokens that the rows see, from a block's first on, widened at the scratch's end; the pass plans with what is in front of them. (From the 17th row
-    // on, whatever the heads: where few share a key head two trips of 16 and 1 rows would be shorter, 17 x 8 / 8 heads behind 20000 34.7 us, widened 42.9)
+    // on: 32 x 32 / 8 heads behind 4000 28.4 us, as tokens, 16 rows a trip, 37.8; 64 x 16 / 2 of 256 behind 20000 53.5, 118. The wrong side, which the rule does not
+    // count: few heads a key head, or very many tokens, 17 x 8 / 8 behind 20000 42.5, 34.6, 32 x 32 / 8 behind 100000 188, 156)
     const int64_t from = win > 0 ? std::max<int64_t>(0, p0 + 1 - win) >> c.shift << c.shift : 0, n = p0 + T - from;
     const size_t wide = (size_t) (Hkv * n * D);                   // floats, both streams of halfs
     if (T > DECODE_ROWS && wide <= own / 4 * 3 && n * D * 2 < (int64_t) 1 << 32) {

@@ -6,8 +6,8 @@
 // order, and of equal weights the earliest stay. Move: a work-group a block to be written, key head and
 // stream - its rows gathered, re-rounded to the largest of their scales. In place the blocks go through the library's scratch, since a block is read by
 // those in front of it; blocks whose tokens stay where they are are left out. Bound: the kept rows' bytes, read and written; the search by one CU's instructions.
-// (32768 tokens of 8 heads of 128 to 8192: 26.3 us, the search 17 - 42 vector instructions a weight -, the move 9.6, 3.5 TB/s. 12 sequences of 59 to 3001 tokens x
-// 4 heads of 256 to 517: 15.4, 8.4 + 6.8. With thread-strided tokens and counts in LDS the search took 20; with a list of the first bin's weights for the
+// (32768 tokens of 8 heads of 128 to 8192: 26.6 us, the search 17 - 42 vector instructions a weight -, the move 9.6, 3.5 TB/s. 12 sequences of 59 to 3001 tokens x
+// 4 heads of 256 to 517: 14.7, 8.2 + 6.6. With thread-strided tokens and counts in LDS the search took 20; with a list of the first bin's weights for the
 // second and third sweep 26)
 #include <algorithm>
 

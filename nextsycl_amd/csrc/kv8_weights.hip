@@ -2,8 +2,8 @@
 // share its key head (gfx950): column sums of softmax(q K^T), of which no row is kept.
 //
 // The weights need their row's largest score and sum first, so the product q K^T is made twice. Bound: the matrix unit for float32 rows (two halfs, two
-// products: 1024 rows behind 3001 tokens, 24 / 4 heads of 256, 168 us, 84 % of a large product's rate in the passes), else the exponentials beside it and the
-// passes' starts (64 bfloat16 rows behind 16320, 32 / 8 heads of 128: 44 us, two passes of 20). Both passes are one kernel: a wave keeps 64 tokens in registers, codes widened once, and pairs (row,
+// products: 1024 rows behind 3001 tokens, 24 / 4 heads of 256, 167 us, 84 % of a large product's rate in the passes), else the exponentials beside it and the
+// passes' starts (64 bfloat16 rows behind 16320, 32 / 8 heads of 128: 44.5 us, two passes of 20). Both passes are one kernel: a wave keeps 64 tokens in registers, codes widened once, and pairs (row,
 // head) stream past it through LDS, 16 KiB of operands at a time, for the work-group's four waves at once: 256 neighbouring tokens. First a pair's largest
 // score and sum over each 64 tokens, then a token's sum over a split of the pairs. Between them small kernels: rows into halfs, in the order in which the lanes
 // of an operand lie, with a factor a pair; a pair's parts together; the splits' sums into acc. Few pairs go the way of a token's attention with weights instead.
@@ -80,8 +80,8 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const WeightsParams p) {
 }
 
 // pairs a key head, and scores in all, up to which the rows go as a token's do, the keys once more in the place of the values: two launches, not four or
-// five, and the scores written. (us, instead of: 16 pairs of 8 heads of 128 behind 4000 tokens 15.9 / 22.0, behind 100000 62 / 89; 48 of 4 heads of 256 behind 4000
-// 23.3 / 26.5, behind 100000 92.5 / 92.9; 64 of 8 heads of 128 behind 600 17.4 / 24.0, behind 4000 26.4 / 25.3; 96 of 4 of 256 behind 4000 27.6 / 27.7)
+// five, and the scores written. (us, instead of: 16 pairs of 8 heads of 128 behind 4000 tokens 15.9 / 20.1, behind 100000 62 / 89; 48 of 4 heads of 256 behind 4000
+// 23.7 / 25.6, behind 100000 92.6 / 92.9; 64 of 8 heads of 128 behind 600 17.9 / 22.5, behind 4000 26.4 / 24.7; 96 of 4 of 256 behind 4000 28.1 / 28.1)
 constexpr int64_t FEW = 48, FEW_SCORES = 3 << 19;
 constexpr int RS = 16;                            // splits of the pairs, at most
 constexpr int KT = 4, RUN = 16 * KT;              // tiles of 16 tokens a wave; tokens
