@@ -5,8 +5,8 @@ import pytest
 
 from kv8_ref import BF16, E4M3, F16, F32, INT8, Cache, from_type, to_type, tolerance
 from nextsycl_amd import DevBuf
-from nextsycl_amd.attn import TUNE_PREFILL_SPLITS, TUNE_PREFILL_WAVES
-from test_gpu_kv8 import attend, filled, ints, on_gpu, prompt_close, rows_of, tables
+from nextsycl_amd.attn import TUNE_PREFILL_SPLITS, TUNE_PREFILL_WAVES, Kv8
+from test_gpu_kv8 import attend, check_pools, check_rows, filled, ints, on_gpu, prompt_close, rows_of, store, tables
 
 pytestmark = pytest.mark.gpu
 ANYTHING = [np.nan, np.inf, -np.inf, 1e30, 70000.0]
@@ -279,3 +279,99 @@ def test_a_prompts_window_longer_than_any_sequence(ops, qt, Hq, Hkv, D, T, p0):
     first = run_prompt(ops, c, qt, q, table, p0, Hq)
     for win in (-1, 1 << 31, (1 << 62) + 3, (1 << 63) - 1):
         assert np.array_equal(run_prompt(ops, c, qt, q, table, p0, Hq, win), first), win
+
+
+# ---- the largest sizes
+
+@pytest.mark.parametrize("G,D,n,T", [(4096, 128, 40, 1), (4096, 128, 150, 2), (3001, 128, 70, 17), (4096, 256, 33, 20), (1025, 256, 300, 5)])
+def test_thousands_of_query_heads_a_key_head(ops, G, D, n, T):
+    r = np.random.default_rng(G + T)
+    c, table, q, qv = one_prompt(r, INT8, F16, G, 1, D, 16, T, n - T)
+    ref, given = c.attend(qv, table, 0, n - T)
+    k, v = c.tokens(table, 0, n)
+    check_prompt(F16, run_prompt(ops, c, F16, q, table, n - T, G), ref, qv, k, v, D, what="prompt")
+    want = np.zeros((c.blocks, 1, 16))
+    c.give(None, want, table, 0, n - T, given)
+    accs = [DevBuf.of(ops.gpu, np.zeros(want.shape, np.float32)) for _ in range(2)]
+    if T <= 16:
+        raw = attend(ops, c, on_gpu(ops, c), F16, q, G * D, table, np.array([n - T]), np.array([0, T]), T, T, G, acc1=accs[0])
+        check_prompt(F16, raw, ref, qv, k, v, D, what="tokens")
+        assert np.abs(accs[0].read(np.float32).reshape(want.shape) - want).max() <= 2.0 ** -17 * want.max()
+    ops.kv8_weights(on_gpu(ops, c), F16, DevBuf.of(ops.gpu, q), G * D, T, ints(ops, table), table.shape[1], n - T, G, None, accs[1])
+    assert np.abs(accs[1].read(np.float32).reshape(want.shape) - want).max() <= 2.0 ** -17 * want.max()
+
+
+@pytest.mark.parametrize("longest", [30, 2100])
+def test_65535_sequences(ops, longest):
+    """Most of them without a row or a length; a unit a work-group, and runs."""
+    r = np.random.default_rng(longest)
+    S, Hq, Hkv, D, B = 65535, 2, 1, 128, 16
+    tmax = (longest + B - 1) // B
+    some = [0, 1, 63, 64, 1023, 1024, 40000, 65533, 65534]
+    lens = np.full(S, -1)
+    lens[some] = [longest - 1, 0, 7, longest - 1, 16, longest // 2, 3, 15, longest - 2]
+    table = np.full((S, tmax), -1, np.int32)
+    table[some] = np.arange(len(some) * tmax).reshape(len(some), tmax)
+    start = np.zeros(S + 1, np.int64)
+    start[1:] = np.cumsum(lens >= 0)
+    c = Cache(INT8, len(some) * tmax, Hkv, B, D, seed=1)
+    c.k[:], c.v[:] = (r.integers(-127, 128, c.k.shape).astype(np.int8).view(np.uint8) for _ in range(2))
+    c.ks[:], c.vs[:] = (2.0 ** r.integers(-8, -5, c.ks.shape) for _ in range(2))
+    d = on_gpu(ops, c)
+    q, qs, qv = rows_of(F32, r, len(some), Hq, D)
+    k, ks, kv = rows_of(F32, r, len(some), Hkv, D)
+    store(ops, c, d, F32, k, ks, k, ks, len(some), table, lens, start, 1)
+    one = [0 if i == 0 else i for i in range(len(some) + 1)]
+    c.store(kv, kv, table[some], lens[some], one, 1)
+    check_pools(c, d)
+    acc = DevBuf.of(ops.gpu, np.zeros((c.blocks, Hkv, B), np.float32))
+    raw = attend(ops, c, d, F32, q, qs, table, lens, start, len(some), 1, Hq, longest=longest, acc1=acc)
+    want = np.zeros((c.blocks, Hkv, B))
+    for i, s in enumerate(some):
+        ref, given = c.attend(qv[i:i + 1], table, s, int(lens[s]))
+        check_rows(F32, raw[i:i + 1], ref, qv[i:i + 1], *c.tokens(table, s, int(lens[s]) + 1), D, what=str(s))
+        c.give(None, want, table, s, int(lens[s]), given)
+    assert np.abs(acc.read(np.float32).reshape(want.shape) - want).max() <= 2.0 ** -17
+    # and all of them shortened, in groups as the scratch holds them
+    l1 = ints(ops, np.full(S, 77))
+    ops.kv8_evict(d, acc, ints(ops, table), tmax, S, longest, ints(ops, lens), l1, 12, 1, 3)
+    sums = acc.read(np.float32).reshape(want.shape)
+    assert np.array_equal(l1.read(np.int32), np.minimum(lens, 12)) and np.isfinite(sums).all()
+
+
+def test_32767_key_heads(ops):
+    r = np.random.default_rng(8)
+    H, D, B, n = 32767, 128, 16, 21
+    table = np.array([[1, 0]], np.int32)
+    k = DevBuf.of(ops.gpu, to_type(BF16, r.standard_normal((n, H * D), np.float32))[0])
+    cache = Kv8.new(ops.gpu, INT8, 2, H, B, D)
+    ops.kv8_store(cache, BF16, k, H * D, k, H * D, n, ints(ops, table), 2, 1, n, ints(ops, [0]), start=ints(ops, [0, n]))
+    out, acc = DevBuf(ops.gpu, H * D * 2), DevBuf(ops.gpu, 2 * H * B * 4)
+    acc.fill(0)
+    lens = ints(ops, [n - 1])
+    sc = DevBuf(ops.gpu, max(4, 4 * ops.kv8_attend_scratch(1, 1, H, H, D, n, True)))
+    q = k.view(H * D * 2 * (n - 1), H * D * 2)
+    ops.kv8_attend(cache, BF16, q, H * D, 1, ints(ops, table), 2, 1, 1, n, lens, H, out, sc, acc1=acc)
+    prompt, many = DevBuf(ops.gpu, n * H * D * 2), DevBuf(ops.gpu, 2 * H * B * 4)
+    many.fill(0)
+    ops.kv8_prompt(cache, BF16, k, H * D, n, ints(ops, table), 2, 0, H, prompt)
+    ops.kv8_weights(cache, BF16, k, H * D, n, ints(ops, table), 2, 0, H, None, many)
+    ops.gpu.sync()
+    sums = acc.read(np.float32).reshape(2, H, B)
+    whole = sums[1].astype(np.float64).sum(1) + sums[0, :, :n - B].astype(np.float64).sum(1)
+    assert np.abs(whole - 1.0).max() <= 2.0 ** -17                      # (a row's weights)
+    total = many.read(np.float32).reshape(2, H, B)
+    total = total[1].astype(np.float64).sum(1) + total[0, :, :n - B].astype(np.float64).sum(1)
+    assert np.abs(total - n).max() <= n * 2.0 ** -17
+    # some heads against the definition; the prompt's last row is the token's, but for its weights' bits
+    codes, scale = (cache.k.read(np.uint8).view(np.int8).reshape(2, H, B, D), cache.ks.read(np.float32).reshape(2, H))
+    vals = from_type(BF16, k.read(np.uint16)).reshape(n, H, D)
+    got, last = from_type(BF16, out.read(np.uint16)).reshape(H, D), from_type(BF16, prompt.read(np.uint16, H * D, (n - 1) * H * D * 2)).reshape(H, D)
+    for h in (0, 1, 255, 16383, 16384, 32766):
+        x = np.concatenate([codes[1, h] * float(scale[1, h]), codes[0, h, :n - B] * float(scale[0, h])])
+        w = np.exp(x @ vals[n - 1, h] * D ** -0.5 - (x @ vals[n - 1, h] * D ** -0.5).max())
+        ref = w @ x / w.sum()
+        assert np.abs(got[h] - ref).max() <= (2.0 ** -8 + 2.0 ** -17) * np.abs(x).max() and np.abs(last[h] - ref).max() <= (2.0 ** -8 + 2.0 ** -10) * np.abs(x).max()
+    # kept: 9 tokens a head
+    ops.kv8_evict(cache, many, ints(ops, table), 2, 1, n, ints(ops, [n]), lens, 9, 1, 2)
+    assert lens.read(np.int32)[0] == 9
