@@ -1,5 +1,5 @@
-"""Caches of 8-bit values in blocks of tokens (include/ns_kv8.h) where a call meets what nothing wrote: scales and codes of blocks that were never
-stored into hold anything at all, not finite numbers among it."""
+"""Caches of 8-bit values in blocks of tokens (include/ns_kv8.h) at their edges: blocks that were never stored into, whose scales and codes hold anything at
+all, not finite numbers among it; the bits that rows and weights keep, and rows of every magnitude; sequences longer than said; the largest sizes."""
 import numpy as np
 import pytest
 
